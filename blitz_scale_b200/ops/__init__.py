@@ -67,7 +67,26 @@ class LatentKV(NamedTuple):
     rank: int
 
 
-KVLayer = Union[torch.Tensor, KVPair, LatentKV]
+class QuantKV(NamedTuple):
+    """Paged cache of a layer held in 4 bits: bytes [pages, kv_heads, page / 16, block] (`quant_kv_pool` makes one).  Every ``group``
+    dimensions of a head's key or value have an offset z and a scale s in bf16, and a dimension is z + s c with a code c of 4 bits:
+    z = the smallest number of the group rounded down, s = (the largest - z) / 15 rounded up, c = rint((x - z) / s), ties to even.  Heads
+    of 64 or 128 dimensions, groups of 32, 64 or 128, pages of 16 tokens times a power of two.  A group with an infinity or NaN reads back
+    as NaN.  A page's bytes move as they are (their order within a block: csrc/kernels/quant_kv.cuh)."""
+    pool: torch.Tensor
+    dim: int
+    group: int
+
+    @property
+    def kv_heads(self) -> int:
+        return self.pool.shape[1]
+
+    @property
+    def page_size(self) -> int:
+        return 16 * self.pool.shape[2]
+
+
+KVLayer = Union[torch.Tensor, KVPair, LatentKV, QuantKV]
 
 
 def _kv(kv: KVLayer):
@@ -431,6 +450,139 @@ def attn_decode_workspace_bytes(batch: int, q_heads: int, value_dim: int, num_sp
     return int(lib().blitz_attn_decode_workspace_bytes(batch, q_heads, value_dim, num_splits))
 
 
+def quant_kv_block_bytes(dim: int, group: int) -> int:
+    """Bytes of 16 tokens of one head in a 4-bit cache, keys and values."""
+    if dim not in (64, 128) or group not in (32, 64, 128) or group > dim:
+        raise ValueError(f"a 4-bit cache takes heads of 64 or 128 dimensions in groups of 32, 64 or 128 of them, got {dim} in groups of {group}")
+    return 16 * (dim + 8 * (dim // group))
+
+
+def quant_kv_pool(pages: int, page_size: int, kv_heads: int, dim: int, group: int = 32, device="cuda") -> QuantKV:
+    """An empty 4-bit cache of a layer (all zeros)."""
+    if page_size < 16 or page_size & (page_size - 1):
+        raise ValueError(f"pages of a 4-bit cache hold 16 tokens times a power of two, got {page_size}")
+    return QuantKV(torch.zeros(pages, kv_heads, page_size // 16, quant_kv_block_bytes(dim, group), dtype=torch.uint8, device=device), dim, group)
+
+
+def _quant(cache: QuantKV, *others: torch.Tensor) -> torch.Tensor:
+    """The pool of a 4-bit cache, after checks of it and of what a call brings beside it."""
+    pool = cache.pool
+    if pool.dtype != torch.uint8 or pool.dim() != 4 or not pool.is_contiguous() or pool.shape[3] != quant_kv_block_bytes(cache.dim, cache.group) \
+            or pool.data_ptr() % 16:
+        raise ValueError(f"not a 4-bit cache of heads of {cache.dim} in groups of {cache.group}: {tuple(pool.shape)} {pool.dtype}")
+    if pool.shape[2] & (pool.shape[2] - 1) or pool.shape[2] < 1:
+        raise ValueError(f"pages of a 4-bit cache hold 16 tokens times a power of two, got {16 * pool.shape[2]}")
+    for t in (pool, *others):
+        if not t.is_cuda or t.get_device() != torch.cuda.current_device():
+            raise ValueError(f"a tensor on {t.device}: the kernels run on the current CUDA device")
+    return pool
+
+
+def _quant_rows(x: torch.Tensor, cache: QuantKV, what: str) -> torch.Tensor:
+    """Rows [T, kv_heads * dim] (or [T, kv_heads, dim]) of keys or values in 16 bits, with any pitch of whole 16 bytes."""
+    _dt(x)
+    H, D = cache.pool.shape[1], cache.dim
+    if x.dim() not in (2, 3) or x.shape[1:] not in ((H * D,), (H, D)) or x.stride(-1) != 1 or (x.dim() == 3 and x.stride(1) != D):
+        raise ValueError(f"{what}: rows of {H} heads of {D} dimensions, got {tuple(x.shape)} with strides {x.stride()}")
+    if x.stride(0) % 8 or x.data_ptr() % 16:
+        raise ValueError(f"{what}: rows have to start on 16-byte boundaries")
+    return x
+
+
+def _int32(t: torch.Tensor, n: Optional[int], what: str) -> torch.Tensor:
+    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.numel() < n):
+        raise ValueError(f"{what}: {'' if n is None else f'at least {n} '}int32 numbers, got {tuple(t.shape)} {t.dtype}")
+    return t
+
+
+def quant_kv_store(k: torch.Tensor, v: torch.Tensor, slot: torch.Tensor, cache: QuantKV) -> None:
+    """Quantise rows of (rotated) keys and values into a 4-bit cache.  ``k``, ``v``: [T, kv_heads * dim] in 16 bits, e.g. column ranges of
+    the fused projection; ``slot`` [T]: page * page_size + offset (negative: the row is not written).  Each slot once in a call."""
+    pool = _quant(cache, k, v, slot)
+    T = k.shape[0]
+    _quant_rows(k, cache, "k")
+    _quant_rows(v, cache, "v")
+    if v.shape[0] != T or v.dtype != k.dtype:
+        raise ValueError(f"as many values as keys, of their type: {tuple(v.shape)} {v.dtype} beside {tuple(k.shape)} {k.dtype}")
+    _int32(slot, T, "slot")
+    _check(lib().blitz_quant_kv_store(_p(k), k.stride(0), _p(v), v.stride(0), _p(slot), _p(pool), T, pool.shape[1], cache.dim, cache.group,
+                                      cache.page_size, pool.shape[0], _status_ptr(k), _dt(k), _stream()), "blitz_quant_kv_store")
+
+
+def quant_kv_load(cache: QuantKV, slot: torch.Tensor, *, dtype: torch.dtype = torch.bfloat16, k: Optional[torch.Tensor] = None,
+                  v: Optional[torch.Tensor] = None):
+    """Keys and values [T, kv_heads, dim] of slots of a 4-bit cache, rounded to 16 bits (rows with a negative slot are left as they are)."""
+    _int32(slot, None, "slot")
+    shape = (slot.numel(), cache.pool.shape[1], cache.dim)
+    k = torch.empty(shape, dtype=dtype, device=cache.pool.device) if k is None else k
+    v = torch.empty(shape, dtype=dtype, device=cache.pool.device) if v is None else v
+    if any(t.shape != shape or not t.is_contiguous() or t.dtype != k.dtype or t.data_ptr() % 16 for t in (k, v)):
+        raise ValueError(f"k and v: contiguous {shape} of one type")
+    pool = _quant(cache, slot, k, v)
+    _check(lib().blitz_quant_kv_load(_p(pool), _p(slot), slot.numel(), 0, _p(k), _p(v), pool.shape[1], cache.dim, cache.group, cache.page_size,
+                                     0, pool.shape[0], _status_ptr(pool), _dt(k), _stream()), "blitz_quant_kv_load")
+    return k, v
+
+
+def quant_kv_pages(cache: QuantKV, pages: torch.Tensor, *, dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Whole pages of a 4-bit cache in the layout of a 16-bit one, [len(pages), 2, page, kv_heads, dim], rounded to 16 bits."""
+    _int32(pages, None, "pages")
+    ps = cache.page_size
+    shape = (pages.numel(), 2, ps, cache.pool.shape[1], cache.dim)
+    out = torch.empty(shape, dtype=dtype, device=cache.pool.device) if out is None else out
+    if out.shape != shape or not out.is_contiguous() or out.data_ptr() % 16:
+        raise ValueError(f"out: contiguous {shape}, got {tuple(out.shape)}")
+    pool = _quant(cache, pages, out)
+    _check(lib().blitz_quant_kv_load(_p(pool), _p(pages), pages.numel(), 1, _p(out), _p(out) + out.stride(1) * out.element_size(), pool.shape[1],
+                                     cache.dim, cache.group, ps, 2 * ps, pool.shape[0], _status_ptr(pool), _dt(out), _stream()), "blitz_quant_kv_load")
+    return out
+
+
+def quant_attn_workspace_bytes(batch: int, q_heads: int, head_dim: int, device="cuda") -> int:
+    """Scratch of `attn_decode` over a 4-bit cache."""
+    return 256
+
+
+def _quant_attn(q: torch.Tensor, cache: QuantKV, q_heads: int, kv_heads: int, head_dim: int, page_size: int, window: int, keep_first: int,
+                softcap: float, sink: Optional[torch.Tensor], out: Optional[torch.Tensor], refused: dict, *others: torch.Tensor):
+    """Checks of an attention call over a 4-bit cache; returns (pool, out)."""
+    named = [n for n, x in refused.items() if x is not None and x is not False]
+    if named:
+        raise ValueError(f"attention over a 4-bit cache has no {', '.join(named)}")
+    _dt(q)
+    D = cache.dim
+    if (kv_heads, head_dim, page_size) != (cache.pool.shape[1], D, cache.page_size) or q_heads < 1 or q_heads % kv_heads:
+        raise ValueError(f"{q_heads} query and {kv_heads} KV heads of {head_dim}, pages of {page_size}: the 4-bit cache has {cache.pool.shape[1]} "
+                         f"heads of {D}, pages of {cache.page_size}")
+    if q.dim() != 2 or q.shape[1] < q_heads * D or q.stride(1) != 1 or q.stride(0) % 8 or q.data_ptr() % 16:
+        raise ValueError(f"q: rows of {q_heads} heads of {D} dimensions that start on 16-byte boundaries, got {tuple(q.shape)}, strides {q.stride()}")
+    if window < 0 or keep_first < 0 or not softcap >= 0.0:
+        raise ValueError(f"window {window}, keep_first {keep_first}, softcap {softcap}")
+    if sink is not None and (sink.dtype != q.dtype or sink.numel() != q_heads or not sink.is_contiguous()):
+        raise ValueError(f"sink: {q_heads} numbers of {q.dtype}")
+    if out is None:
+        out = torch.empty((q.shape[0], q_heads * D), dtype=q.dtype, device=q.device)
+    elif out.dim() != 2 or out.shape[1] < q_heads * D or out.dtype != q.dtype or out.stride(1) != 1 or out.stride(0) % 8 or out.data_ptr() % 16:
+        raise ValueError(f"out: rows of {q_heads * D} {q.dtype} that start on 16-byte boundaries, got {tuple(out.shape)} {out.dtype}")
+    return _quant(cache, q, out, *others, *([] if sink is None else [sink])), out
+
+
+def _attn_decode_quant(q, cache, indices, indptr, last_page_len, q_heads, kv_heads, head_dim, page_size, num_splits, workspace, out, sm_scale,
+                       window, keep_first, softcap, sink, refused, static_table):
+    B = indptr.numel() - 1
+    if num_splits < 0 or B < 0 or q.shape[0] < B or (out is not None and out.shape[0] < B):
+        raise ValueError(f"{B} sequences: q {tuple(q.shape)}, out {None if out is None else tuple(out.shape)}, num_splits {num_splits}")
+    _int32(indptr, None, "indptr")
+    _int32(last_page_len, B, "last_page_len")
+    _int32(indices, None, "indices")
+    pool, out = _quant_attn(q[:B], cache, q_heads, kv_heads, head_dim, page_size, window, keep_first, softcap, sink, out, refused, indices, indptr,
+                            last_page_len)
+    _check(lib().blitz_attn_decode_quant(_p(q), q.stride(0), _p(pool), _p(indices), _p(indptr), _p(last_page_len), _p(out), out.stride(0), B, q_heads,
+                                         kv_heads, head_dim, cache.group, page_size, pool.shape[0], head_dim ** -0.5 if sm_scale is None else sm_scale,
+                                         window, keep_first, softcap, _p(sink), _status_ptr(q), _dt(q), _stream()), "blitz_attn_decode_quant")
+    return out
+
+
 def attn_decode(q: torch.Tensor, kv_layer: KVLayer, indices: torch.Tensor, indptr: torch.Tensor,
                 last_page_len: torch.Tensor, *, q_heads: int, kv_heads: int, head_dim: int, page_size: int,
                 num_splits: int = 1, workspace: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
@@ -446,7 +598,13 @@ def attn_decode(q: torch.Tensor, kv_layer: KVLayer, indices: torch.Tensor, indpt
     [batch, q_heads]: a head's output is multiplied by its sigmoid; ``bias`` [q_heads, n]: added to the scaled scores by the
     key's distance, the last column for all longer ones.  ``chunked``: the window is a chunk counted from position 0, of which
     the keys up to the position are visible; ``sigmoid``: the weights are sigmoids of the scores, not normalised.  Values may have a size of their own (KVPair).  ``static_table`` promises that ``indices``, ``indptr`` and
-    ``last_page_len`` are not written by kernels still running in this stream (the copy that brings a step's tables is no kernel)."""
+    ``last_page_len`` are not written by kernels still running in this stream (the copy that brings a step's tables is no kernel).
+
+    Over a 4-bit cache (QuantKV) keys and values enter as they are, without a rounding to 16 bits; no gate, bias, ``chunked`` or
+    ``sigmoid``; ``num_splits`` is 1 or 0 (any other number counts as 0), ``workspace`` of `quant_attn_workspace_bytes`."""
+    if isinstance(kv_layer, QuantKV):
+        return _attn_decode_quant(q, kv_layer, indices, indptr, last_page_len, q_heads, kv_heads, head_dim, page_size, num_splits, workspace, out, sm_scale,
+                                  window, keep_first, softcap, sink, dict(gate=gate, bias=bias, chunked=chunked, sigmoid=sigmoid), static_table)
     B = indptr.numel() - 1
     kp, vp, page_rows, pages, vdim = _kv(kv_layer)
     if out is None:
@@ -500,12 +658,29 @@ def attn_prefill_paged(q: torch.Tensor, kv_layer: KVLayer, page_indices: torch.T
                        sm_scale: Optional[float] = None, poly_exp: bool = False, window: int = 0, keep_first: int = 0,
                        softcap: float = 0.0, sink: Optional[torch.Tensor] = None,
                        gate: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, chunked: bool = False,
-                       sigmoid: bool = False) -> torch.Tensor:
+                       sigmoid: bool = False, skip_pages: int = 0) -> torch.Tensor:
     """Causal attention of the pass's rows over the paged cache (which already holds the rows' own keys and values,
     after whatever earlier passes stored).  ``q``: rotated query columns, e.g. the fused qkv buffer (rope_kv_store);
     ``page_indices``: the sequences' page ids back to back, covering prefix + rows; ``work`` from `prefill_work_list`
     for the same sequences.  ``window`` / ``keep_first`` / ``softcap`` / ``sink`` / ``gate`` / ``bias`` / ``chunked`` / ``sigmoid``
-    as for `attn_decode` (no bias beside a window, cap or sink; with sigmoid weights a bias of one column)."""
+    as for `attn_decode` (no bias beside a window, cap or sink; with sigmoid weights a bias of one column).
+
+    Over a 4-bit cache (QuantKV): the pages named by ``page_indices`` are read back first, rounded to the queries' type, into scratch of
+    this call; no record of ``work`` refers to the first ``skip_pages`` of them, which are passed over."""
+    if isinstance(kv_layer, QuantKV):
+        _int32(page_indices, None, "page_indices")
+        if not 0 <= skip_pages <= page_indices.numel():
+            raise ValueError(f"skip_pages {skip_pages} of {page_indices.numel()} pages")
+        if work.dtype != torch.int32 or work.dim() != 2 or work.shape[1] != 8 or not work.is_contiguous():
+            raise ValueError(f"work: records of prefill_work_list, got {tuple(work.shape)} {work.dtype}")
+        if out is not None and out.shape[0] < q.shape[0]:
+            raise ValueError(f"out: {q.shape[0]} rows, got {tuple(out.shape)}")
+        _, out = _quant_attn(q, kv_layer, q_heads, kv_heads, head_dim, page_size, window, keep_first, softcap, sink, out,
+                             dict(gate=gate, bias=bias, chunked=chunked, sigmoid=sigmoid), page_indices, work)
+        if work.shape[0] == 0 or q.shape[0] == 0:
+            return out
+        kv_layer = quant_kv_pages(kv_layer, page_indices[skip_pages:], dtype=q.dtype)
+        page_indices = torch.arange(-skip_pages, kv_layer.shape[0], dtype=torch.int32, device=q.device)
     T = q.shape[0]
     kp, vp, page_rows, pages, vdim = _kv(kv_layer)
     if out is None:
