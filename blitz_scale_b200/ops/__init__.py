@@ -539,8 +539,9 @@ def quant_kv_pages(cache: QuantKV, pages: torch.Tensor, *, dtype: torch.dtype = 
 
 
 def quant_attn_workspace_bytes(batch: int, q_heads: int, head_dim: int, device="cuda") -> int:
-    """Scratch of `attn_decode` over a 4-bit cache."""
-    return 256
+    """Scratch of `attn_decode` over a 4-bit cache, for up to `batch` sequences: zero-filled before its first use, for one call at a time."""
+    with torch.cuda.device(device):
+        return int(lib().blitz_attn_decode_quant_workspace_bytes(batch, q_heads, head_dim))
 
 
 def _quant_attn(q: torch.Tensor, cache: QuantKV, q_heads: int, kv_heads: int, head_dim: int, page_size: int, window: int, keep_first: int,
@@ -575,11 +576,22 @@ def _attn_decode_quant(q, cache, indices, indptr, last_page_len, q_heads, kv_hea
     _int32(indptr, None, "indptr")
     _int32(last_page_len, B, "last_page_len")
     _int32(indices, None, "indices")
+    if workspace is not None and (workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.data_ptr() % 256):
+        raise ValueError(f"workspace: bytes that start on a 256-byte boundary, got {workspace.dtype}")
     pool, out = _quant_attn(q[:B], cache, q_heads, kv_heads, head_dim, page_size, window, keep_first, softcap, sink, out, refused, indices, indptr,
-                            last_page_len)
-    _check(lib().blitz_attn_decode_quant(_p(q), q.stride(0), _p(pool), _p(indices), _p(indptr), _p(last_page_len), _p(out), out.stride(0), B, q_heads,
-                                         kv_heads, head_dim, cache.group, page_size, pool.shape[0], head_dim ** -0.5 if sm_scale is None else sm_scale,
-                                         window, keep_first, softcap, _p(sink), _status_ptr(q), _dt(q), _stream()), "blitz_attn_decode_quant")
+                            last_page_len, *([] if workspace is None else [workspace]))
+    if B == 0:
+        return out
+    if num_splits != 1:
+        n = int(lib().blitz_attn_decode_quant_workspace_bytes(B, q_heads, head_dim))
+        if workspace is None:
+            workspace = torch.zeros(n, dtype=torch.uint8, device=q.device)
+        elif workspace.numel() < n:
+            raise ValueError(f"workspace of {workspace.numel()} bytes, {n} are needed")
+    _check(lib().blitz_attn_decode_quant(_p(q), q.stride(0), _p(pool), _p(indices), _p(indptr), _p(last_page_len), _p(out), out.stride(0), _p(workspace),
+                                         0 if workspace is None else workspace.numel(), B, q_heads, kv_heads, head_dim, cache.group, page_size,
+                                         pool.shape[0], num_splits, head_dim ** -0.5 if sm_scale is None else sm_scale, window, keep_first, softcap,
+                                         _p(sink), int(static_table), _status_ptr(q), _dt(q), _stream()), "blitz_attn_decode_quant")
     return out
 
 
