@@ -582,15 +582,14 @@ def _attn_decode_quant(q, cache, indices, indptr, last_page_len, q_heads, kv_hea
                             last_page_len, *([] if workspace is None else [workspace]))
     if B == 0:
         return out
-    if num_splits != 1:
-        n = int(lib().blitz_attn_decode_quant_workspace_bytes(B, q_heads, head_dim))
-        if workspace is None:
-            workspace = torch.zeros(n, dtype=torch.uint8, device=q.device)
-        elif workspace.numel() < n:
-            raise ValueError(f"workspace of {workspace.numel()} bytes, {n} are needed")
+    n = int(lib().blitz_attn_decode_quant_workspace_bytes(B, q_heads, head_dim))
+    if workspace is None:
+        workspace = torch.zeros(n, dtype=torch.uint8, device=q.device)
+    elif workspace.numel() < n:
+        raise ValueError(f"workspace of {workspace.numel()} bytes, {n} are needed")
     _check(lib().blitz_attn_decode_quant(_p(q), q.stride(0), _p(pool), _p(indices), _p(indptr), _p(last_page_len), _p(out), out.stride(0), _p(workspace),
-                                         0 if workspace is None else workspace.numel(), B, q_heads, kv_heads, head_dim, cache.group, page_size,
-                                         pool.shape[0], num_splits, head_dim ** -0.5 if sm_scale is None else sm_scale, window, keep_first, softcap,
+                                         workspace.numel(), B, q_heads, kv_heads, head_dim, cache.group, page_size,
+                                         pool.shape[0], head_dim ** -0.5 if sm_scale is None else sm_scale, window, keep_first, softcap,
                                          _p(sink), int(static_table), _status_ptr(q), _dt(q), _stream()), "blitz_attn_decode_quant")
     return out
 
@@ -613,7 +612,8 @@ def attn_decode(q: torch.Tensor, kv_layer: KVLayer, indices: torch.Tensor, indpt
     ``last_page_len`` are not written by kernels still running in this stream (the copy that brings a step's tables is no kernel).
 
     Over a 4-bit cache (QuantKV) keys and values enter as they are, without a rounding to 16 bits; no gate, bias, ``chunked`` or
-    ``sigmoid``; ``num_splits`` is 1 or 0 (any other number counts as 0), ``workspace`` of `quant_attn_workspace_bytes`."""
+    ``sigmoid``; the keys of all sequences are always taken in equal shares, whatever ``num_splits``, and ``workspace`` has the size of
+    `quant_attn_workspace_bytes`."""
     if isinstance(kv_layer, QuantKV):
         return _attn_decode_quant(q, kv_layer, indices, indptr, last_page_len, q_heads, kv_heads, head_dim, page_size, num_splits, workspace, out, sm_scale,
                                   window, keep_first, softcap, sink, dict(gate=gate, bias=bias, chunked=chunked, sigmoid=sigmoid), static_table)
