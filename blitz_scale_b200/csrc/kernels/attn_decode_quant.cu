@@ -7,13 +7,16 @@
 //   q.k = sum_g s_g (sum_{d in g} q_d c_d) + z_g (sum_{d in g} q_d)
 //   o_d = sum_j (p_j s_j) (c_jd - 8) + sum_j p_j (z_j + 8 s_j)
 //
-// A code becomes a 16-bit float by one mask and one "or" into the mantissa of a power of two, which adds a constant:
-// keys: 1024 + c and 64 + c in fp16 (two nibbles a shift), the constants' part of the product is the accumulator's initial value;
-// values: 128 + c in bf16, and a product of a constant matrix with the weights takes 136 off again (the codes around zero, so that
-// the rounding of p_j s_j is not amplified by an offset that cancels).  Queries enter in fp16, a head divided by a power of two near its
-// largest entry: bf16 and fp16 numbers are exact there (next to the largest, that is), and so are their products with codes.  p s is
-// rounded to bf16 (its range is the scales'), as in attention over 16-bit caches; in fp16 models to two bf16 numbers, hi + lo.  The part
-// of z_j stays in 32 bits; the sums of q_d z_g in the scores are one more product, of z as stored with sums of q in two bf16 numbers.
+// A code becomes an fp16 number by one mask and one "or" into the mantissa of a power of two, which adds a constant, 1024 or 64: a word
+// of 8 codes takes five instructions.  For keys the constants' part of the product is the accumulator's initial value, for values a product
+// of a constant matrix with the same weights takes it off again, and 8 with it (the codes around zero, so that the rounding of p_j s_j is not
+// amplified by what cancels).  Queries enter in fp16, a head divided by a power of two near its largest entry: bf16 and fp16 numbers are
+// exact there (next to the largest, that is), and so are their products with codes.  Weights times scales are rounded to fp16, times a power of
+// two that brings the largest scale so far to 2^6 .. 2^7: 2^-11 of each down to scales 2^-20 of the largest, less below.  The part of z_j stays in 32
+// bits; the sums of q_d z_g in the scores are one more product, in bf16, of z as stored with sums of q in two numbers.
+//
+// The maximum that weights refer to follows the scores only when they pass it by 2^8 (fp16 has room for that): nearly every chunk finds
+// that out with a vote, without a maximum over its lanes or a rescaling.
 //
 // S^T = K Q^T has 16 tokens as rows and at most 8 query heads as columns, O^T = V^T P^T dimensions as rows and the same columns: a lane
 // has the same heads in both.  Between them the weights' 8 x 8 blocks are transposed by movmatrix.  Scales of K multiply the accumulators
@@ -24,8 +27,10 @@
 // head's tokens in a page are one contiguous piece), a lane for each of the others.
 //
 // The chunks of all sequences of all heads, end to end, are cut into equal ranges, one per warp of the GPU, so that neither lengths nor the
-// number of sequences leave warps idle.  A sequence of a head that is whole within a range is stored at once; pieces are added up, in the order
-// of the ranges, at the end of the launch: through shared memory within a block, through scratch and a ticket between blocks.
+// number of sequences leave warps idle.  A sequence that is cut leaves its pieces' sums in shared memory, where the warps that end with it
+// wait for them and add them up, a head each (the warp it begins in comes to it last, the next one began with it: nobody waits long);
+// pieces in several blocks go through scratch and a ticket per head, and the last block adds up.  The order is that of the ranges,
+// whoever is last.
 #include "launch.cuh"
 #include "ptx.cuh"
 #include "mma.cuh"
@@ -35,7 +40,10 @@
 
 namespace blitz {
 
-constexpr int kQdWarps = 15, kQdThreads = (kQdWarps + 1) * 32;
+#ifndef QDW
+#define QDW 15
+#endif
+constexpr int kQdWarps = QDW, kQdThreads = (kQdWarps + 1) * 32;
 constexpr int kQdChunk = 32;
 constexpr int kQdMaxBatch = 1024;   // sequences of a launch
 constexpr int kQdMaxStages = 4;
@@ -48,7 +56,7 @@ struct DecodeQuantParams {
   const int32_t *indices, *indptr, *last_page_len;
   void* out;
   int64_t out_stride;
-  unsigned* tickets;   // [batch][heads] pieces finished, zero between launches
+  unsigned* tickets;   // [batch][query heads] pieces finished, zero between launches
   float* part;         // [2 blocks][rep][D] sums, then [2 blocks][rep] of (maximum, sum of weights)
   int batch, kv_heads, heads, div, rep;  // heads: groups of at most 8 query heads, div of which share a KV head; rep: query heads of one
   int page_size, page_shift, max_pages, stages, static_table;
@@ -58,9 +66,9 @@ struct DecodeQuantParams {
   int* status;
 };
 
-// Shared memory: rings, a slot per warp for the first piece's sums, tables of the sequences, barriers.
+// Shared memory: rings, a slot per warp for the sums of its first piece (the last one's go into the ring), tables of the sequences, barriers.
 __host__ __device__ constexpr int qd_slot_floats(int D, int rep) { return rep * (D + 4) + 16; }  // rows in different banks, then maxima and sums
-__host__ __device__ constexpr int qd_table_bytes() { return (3 * kQdMaxBatch + 4 + 16) * 4; }
+__host__ __device__ constexpr int qd_table_bytes() { return (3 * kQdMaxBatch + 4 + 8 + kQdWarps * 16) * 4; }
 inline int qd_smem(int D, int stage, int rep, int stages) { return kQdWarps * (stages * stage + qd_slot_floats(D, rep) * 4) + qd_table_bytes() + kQdWarps * kQdMaxStages * 16; }
 
 struct QdTables {
@@ -81,10 +89,15 @@ __device__ __forceinline__ QdSeen qd_seen(const DecodeQuantParams& p, int len) {
   v.c_window = max(v.lo / kQdChunk, v.n_first);
   return v;
 }
-// How `all` chunks are cut into `n` ranges.
+// How `all` chunks are cut into ranges: `each` warps of a block take one (all of them where there are chunks enough; few chunks go to
+// more blocks, whose warps then have an SM's pipes to themselves).
 struct QdCut {
-  unsigned base, rem;
-  __device__ __forceinline__ QdCut(unsigned all, unsigned n) : base(all / n), rem(all % n) {}
+  unsigned each, base, rem;
+  __device__ __forceinline__ QdCut(unsigned all, unsigned blocks) {
+    each = min(static_cast<unsigned>(kQdWarps), max(4u, (all + blocks - 1) / blocks));
+    base = all / (blocks * each);
+    rem = all % (blocks * each);
+  }
   __device__ __forceinline__ unsigned begin(unsigned v) const { return v * base + min(v, rem); }
   __device__ __forceinline__ unsigned range(unsigned x) const { return x < rem * (base + 1) ? x / (base + 1) : rem + (x - rem * (base + 1)) / base; }
 };
@@ -131,6 +144,28 @@ __device__ __forceinline__ bool qd_next(const QdTables& t, int batch, QdWalk& w,
   return true;
 }
 
+__device__ __forceinline__ void qd_keep(volatile int* to, const QdPiece& it) {
+  to[0] = it.head; to[1] = it.b; to[2] = it.start; to[3] = it.stop;
+}
+__device__ __forceinline__ QdPiece qd_kept(const volatile int* from) {
+  return {from[0], from[1], 0, 0, static_cast<unsigned>(from[2]), static_cast<unsigned>(from[3])};
+}
+
+// Waits (in a converged warp) until words of shared memory that other warps of the block write are not zero: a lane for each that counts.
+__device__ __forceinline__ bool qd_wait(const volatile int* word, bool counts, volatile int* abort_flag) {
+  bool on = !counts || *word != 0;
+  const uint64_t since = ptx::globaltimer_ns();
+  for (uint32_t it = 1; !__all_sync(0xffffffffu, on); on = !counts || *word != 0, ++it) {
+    __nanosleep(32);
+    if ((it & 63u) == 0 && __any_sync(0xffffffffu, *abort_flag != 0 || ptx::globaltimer_ns() - since > ptx::kDefaultWaitNs)) {
+      *abort_flag = 1;
+      return false;
+    }
+  }
+  __threadfence_block();
+  return true;
+}
+
 // d = a b + (c0, c1, c0, c1)
 __device__ __forceinline__ void qd_mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float c0, float c1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
@@ -147,14 +182,16 @@ __device__ __forceinline__ void qd_mma_bf16(float (&d)[4], uint32_t a0, uint32_t
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
-__device__ __forceinline__ void qd_mma_bf16_add(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 __device__ __forceinline__ uint32_t qd_transposed(uint32_t x) {
   uint32_t y;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+// (x & mask) | bits
+template <uint32_t MASK, uint32_t BITS>
+__device__ __forceinline__ uint32_t qd_pick(uint32_t x) {
+  uint32_t y;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "r"(MASK), "r"(BITS));
   return y;
 }
 __device__ __forceinline__ float qd_low(uint32_t w) { return __uint_as_float(w << 16); }
@@ -181,25 +218,23 @@ struct QdScales {
     }
   }
   float mid[N];  // z + 8 s
-  __device__ __forceinline__ void values(const uint8_t* token, int x, bool on) {
-    uint32_t a = 0, b = 0, c = 0, d = 0;
-    if (on) {  // (what is not visible may hold no numbers)
-      if (G == 4 && HALVES) {
-        a = *reinterpret_cast<const uint32_t*>(token + 4 * x);
-        c = *reinterpret_cast<const uint32_t*>(token + 8 + 4 * x);
-      } else if (G == 4) {
-        const uint4 w = *reinterpret_cast<const uint4*>(token);
-        a = w.x; b = w.y; c = w.z; d = w.w;
-      } else if (G == 2 && HALVES) {
-        a = *reinterpret_cast<const uint16_t*>(token + 2 * x);
-        c = *reinterpret_cast<const uint16_t*>(token + 4 + 2 * x);
-      } else if (G == 2) {
-        const uint2 w = *reinterpret_cast<const uint2*>(token);
-        a = w.x; c = w.y;
-      } else {
-        a = *reinterpret_cast<const uint32_t*>(token);
-        c = a >> 16;
-      }
+  __device__ __forceinline__ void values(const uint8_t* token, int x) {
+    uint32_t a, b = 0, c, d = 0;
+    if (G == 4 && HALVES) {
+      a = *reinterpret_cast<const uint32_t*>(token + 4 * x);
+      c = *reinterpret_cast<const uint32_t*>(token + 8 + 4 * x);
+    } else if (G == 4) {
+      const uint4 w = *reinterpret_cast<const uint4*>(token);
+      a = w.x; b = w.y; c = w.z; d = w.w;
+    } else if (G == 2 && HALVES) {
+      a = *reinterpret_cast<const uint16_t*>(token + 2 * x);
+      c = *reinterpret_cast<const uint16_t*>(token + 4 + 2 * x);
+    } else if (G == 2) {
+      const uint2 w = *reinterpret_cast<const uint2*>(token);
+      a = w.x; c = w.y;
+    } else {
+      a = *reinterpret_cast<const uint32_t*>(token);
+      c = a >> 16;
     }
     s[0] = qd_low(a);
     mid[0] = fmaf(8.f, s[0], qd_low(c));
@@ -212,13 +247,22 @@ struct QdScales {
       mid[2 % N] = fmaf(8.f, s[2 % N], qd_low(d)); mid[3 % N] = fmaf(8.f, s[3 % N], qd_high(d));
     }
   }
+  __device__ __forceinline__ void none() {
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] = mid[i] = 0.f;
+  }
+  __device__ __forceinline__ float largest() const {
+    float v = s[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) v = fmaxf(v, s[i]);
+    return v;
+  }
 };
 
 template <typename T, int D, int GROUP, bool HALVES>
 __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const __grid_constant__ DecodeQuantParams p) {
   constexpr QuantKv F = quant_kv(D, GROUP);
   constexpr int G = D / GROUP, W = D / 32, WG = GROUP / 32, MT = D / 16, N = QdScales<G, HALVES>::N;
-  constexpr bool kTwo = std::is_same<T, __half>::value;  // weights as two bf16 numbers
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int ring_bytes = p.stages * 2 * F.block, slot = qd_slot_floats(D, p.rep);
@@ -227,9 +271,10 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
   tab.before = reinterpret_cast<int*>(slots + kQdWarps * slot);
   tab.len = tab.before + kQdMaxBatch + 4;
   tab.page = tab.len + kQdMaxBatch;
-  int* const across = tab.page + kQdMaxBatch;  // [2]: sequence and head that goes on before, after this block (-1: none); [2] flag of the last piece
-  volatile int* const abort_flag = across + 8;
-  uint64_t* const full = reinterpret_cast<uint64_t*>(across + 16);  // [warp][stage]
+  volatile int* const abort_flag = tab.page + kQdMaxBatch;
+  // [warp][16]: where its walk is, the piece it is at (kept here: the products need the registers), whether its sums are in its slot, its ring
+  volatile int* const records = abort_flag + 8;
+  uint64_t* const full = reinterpret_cast<uint64_t*>(tab.page + kQdMaxBatch + 8 + kQdWarps * 16);  // [warp][stage]
   uint64_t* const empty = full + kQdWarps * kQdMaxStages;
 
   if (threadIdx.x < kQdWarps * kQdMaxStages) {
@@ -238,8 +283,8 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
   }
   if (threadIdx.x == 0) {
     *abort_flag = 0;
-    across[0] = across[1] = -1;
   }
+  if (threadIdx.x < kQdWarps) records[threadIdx.x * 16 + 8] = records[threadIdx.x * 16 + 9] = 0;
   ptx::fence_mbar_init();
   ptx::fence_proxy_async_smem();
   ptx::griddep_launch_dependents();
@@ -273,18 +318,18 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
   ptx::griddep_wait();
 
   T* const out = reinterpret_cast<T*>(p.out);
-  const QdCut cut(static_cast<unsigned>(tab.before[p.batch]) * p.heads, kQdWarps * gridDim.x);
-  const unsigned first_warp = blockIdx.x * kQdWarps;
+  const QdCut cut(static_cast<unsigned>(tab.before[p.batch]) * p.heads, gridDim.x);
+  const unsigned first_warp = blockIdx.x * cut.each;
+  const int warps = cut.each;
   // (sequences without a visible key are in nobody's range: their output is zero)
   for (int b = blockIdx.x; b < p.batch; b += gridDim.x)
     if (tab.before[b] == tab.before[b + 1])
       for (int e = threadIdx.x; e < p.heads * p.rep * D; e += kQdThreads) stf(out + b * p.out_stride + e, 0.f);
 
-  QdPiece first_piece{}, last_piece{};  // of this warp's range
   if (warp == kQdWarps) {
     // ---------------------------------------------------------------- copies: a lane for each warp
-    const unsigned v = first_warp + min(lane, kQdWarps - 1);
-    QdWalk walk = qd_walk(tab, p.batch, cut.begin(v), lane < kQdWarps ? cut.begin(v + 1) : 0u);
+    const unsigned v = first_warp + min(lane, warps - 1);
+    QdWalk walk = qd_walk(tab, p.batch, cut.begin(v), lane < warps ? cut.begin(v + 1) : 0u);
     QdPiece it{};
     QdSeen see{};
     bool more = qd_next(tab, p.batch, walk, it);
@@ -341,7 +386,7 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
       if (__any_sync(0xffffffffu, go)) {
         idle = 0;
       } else {
-        __nanosleep(100);
+        __nanosleep(200);
         if ((++idle & 63u) == 0) {
           const uint64_t now = ptx::globaltimer_ns();
           if (idle == 64) since = now;
@@ -356,7 +401,7 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
       }
     }
     // (after a time-out: no copy may land in shared memory that another block has by then)
-    if (lane < kQdWarps && *abort_flag) {
+    if (lane < warps && *abort_flag) {
       since = ptx::globaltimer_ns();
       for (int s = 0; s < p.stages; ++s) {
         if (stage == 0) phase ^= 1u;
@@ -365,7 +410,7 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
         }
       }
     }
-  } else {
+  } else if (warp < warps) {
     // ---------------------------------------------------------------- products
     const int g = lane >> 2, t4 = lane & 3;
     const int x = HALVES ? t4 >> 1 : 0;                     // half of the groups that this lane's columns 2 t4, 2 t4 + 1 stand for
@@ -377,12 +422,21 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
-    const unsigned x0 = cut.begin(first_warp + warp), x1 = cut.begin(first_warp + warp + 1);
-    QdWalk walk = qd_walk(tab, p.batch, x0, x1);
-    QdPiece it{};
-    for (bool first = true; qd_next(tab, p.batch, walk, it); first = false) {
-      if (first) first_piece = it;
-      last_piece = it;
+    volatile int* const rec = records + warp * 16;
+    {
+      const QdWalk walk = qd_walk(tab, p.batch, cut.begin(first_warp + warp), cut.begin(first_warp + warp + 1));
+      rec[0] = walk.x; rec[1] = walk.end; rec[2] = walk.head; rec[3] = walk.b;
+    }
+    for (;;) {
+      QdPiece it;
+      {
+        QdWalk walk{static_cast<unsigned>(rec[0]), static_cast<unsigned>(rec[1]), rec[2], rec[3]};
+        __syncwarp();
+        if (!qd_next(tab, p.batch, walk, it)) break;
+        rec[0] = walk.x; rec[2] = walk.head; rec[3] = walk.b;
+        qd_keep(rec + 4, it);
+        __syncwarp();
+      }
       const QdSeen see = qd_seen(p, tab.len[it.b]);
       // queries: word w of a lane's key codes holds dimensions 32 w + 8 t4 .. + 7, pairs (i, i + 4) of which are a register's halves
       uint32_t qb[W][4], zb0, zb1 = 0;
@@ -449,17 +503,18 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
         // what the lane's own columns need
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          scale[k] = __shfl_sync(0xffffffffu, up, (2 * t4 + k) * 4);
+          scale[k] = __shfl_sync(0xffffffffu, up, (2 * t4 + k) * 4) * (p.cap_log2 > 0.f ? p.cap_scale : p.scale_log2);
 #pragma unroll
           for (int i = 0; i < N; ++i) qc[i][k] = __shfl_sync(0xffffffffu, zero[i], (2 * t4 + k) * 4);
         }
       }
 
-      float o[MT][4], oc[N][4], zs[N][2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+      // `down` takes scales to 16 bits, `most` is the largest one that it is good for
+      float o[MT][4], zs[N][2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, down = 1.f, most = 0.f;
 #pragma unroll
       for (int i = 0; i < MT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 #pragma unroll
-      for (int i = 0; i < N; ++i) oc[i][0] = oc[i][1] = oc[i][2] = oc[i][3] = zs[i][0] = zs[i][1] = 0.f;
+      for (int i = 0; i < N; ++i) zs[i][0] = zs[i][1] = 0.f;
 
       for (int c = it.beg; c < it.end; ++c) {
         if (ok && !__all_sync(0xffffffffu, ptx::bounded_mbar_wait(&my_full[stage], phase, abort_flag))) {
@@ -468,143 +523,141 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
         }
         if (!ok) continue;
         const uint8_t* st = ring + stage * 2 * F.block;
-        const int tok0 = see.token(c), blocks = min(kQdChunk, see.len - tok0 + 15) >> 4;
+        const int tok0 = see.token(c);
         const bool edge = tok0 + kQdChunk > see.len || (tok0 < see.lo && tok0 + kQdChunk > see.first);  // some key is not visible
+        // (16 tokens that a short last chunk does not have: whatever the stage holds, and not visible)
         float s[2][4];  // (tau, first head), (tau, second), (tau + 2, first), (tau + 2, second)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          s[u][0] = s[u][1] = s[u][2] = s[u][3] = 0.f;
-          if (u < blocks) {
-            const uint8_t* ka = st + u * F.block + tau * (D / 2) + t4 * (D / 8);
-            const uint8_t* sa = st + u * F.block + F.codes + tau * 4 * G;
-            uint32_t ku[W], kv[W];
-            if (W == 4) {
-              const uint4 a = *reinterpret_cast<const uint4*>(ka), b = *reinterpret_cast<const uint4*>(ka + D);
-              ku[0] = a.x; ku[1] = a.y; ku[2 % W] = a.z; ku[3 % W] = a.w;
-              kv[0] = b.x; kv[1] = b.y; kv[2 % W] = b.z; kv[3 % W] = b.w;
-            } else {
-              const uint2 a = *reinterpret_cast<const uint2*>(ka), b = *reinterpret_cast<const uint2*>(ka + D);
-              ku[0] = a.x; ku[1] = a.y;
-              kv[0] = b.x; kv[1] = b.y;
-            }
-            const int z_at = G == 4 ? 8 + 4 * (t4 & 1) : G == 2 ? 4 : 0;
-            const uint32_t za = *reinterpret_cast<const uint32_t*>(sa + z_at), zb = *reinterpret_cast<const uint32_t*>(sa + 8 * G + z_at);
-            QdScales<G, HALVES> fa, fb;
-            fa.keys(sa, x);
-            fb.keys(sa + 8 * G, x);
-            qd_mma_bf16(s[u], za, zb, za, zb, zb0, zb1);
-            float acc[N][4];
+          const uint8_t* ka = st + u * F.block + tau * (D / 2) + t4 * (D / 8);
+          const uint8_t* sa = st + u * F.block + F.codes + tau * 4 * G;
+          uint32_t ku[W], kv[W];
+          if (W == 4) {
+            const uint4 a = *reinterpret_cast<const uint4*>(ka), b = *reinterpret_cast<const uint4*>(ka + D);
+            ku[0] = a.x; ku[1] = a.y; ku[2 % W] = a.z; ku[3 % W] = a.w;
+            kv[0] = b.x; kv[1] = b.y; kv[2 % W] = b.z; kv[3 % W] = b.w;
+          } else {
+            const uint2 a = *reinterpret_cast<const uint2*>(ka), b = *reinterpret_cast<const uint2*>(ka + D);
+            ku[0] = a.x; ku[1] = a.y;
+            kv[0] = b.x; kv[1] = b.y;
+          }
+          const int z_at = G == 4 ? 8 + 4 * (t4 & 1) : G == 2 ? 4 : 0;
+          const uint32_t za = *reinterpret_cast<const uint32_t*>(sa + z_at), zb = *reinterpret_cast<const uint32_t*>(sa + 8 * G + z_at);
+          QdScales<G, HALVES> fa, fb;
+          fa.keys(sa, x);
+          fb.keys(sa + 8 * G, x);
+          qd_mma_bf16(s[u], za, zb, za, zb, zb0, zb1);
+          float acc[N][4];
 #pragma unroll
-            for (int w = 0; w < W; ++w) {
-              const int i = (w / WG) % N;
-              const uint32_t a = ku[w], b = kv[w], ah = a >> 8, bh = b >> 8;
-              const uint32_t a0 = (a & 0x000f000fu) | 0x64006400u, a1 = (b & 0x000f000fu) | 0x64006400u;
-              const uint32_t a2 = (a & 0x00f000f0u) | 0x54005400u, a3 = (b & 0x00f000f0u) | 0x54005400u;
-              const uint32_t c0 = (ah & 0x000f000fu) | 0x64006400u, c1 = (bh & 0x000f000fu) | 0x64006400u;
-              const uint32_t c2 = (ah & 0x00f000f0u) | 0x54005400u, c3 = (bh & 0x00f000f0u) | 0x54005400u;
-              if (w % WG == 0 && w / WG < N) qd_mma_f16(acc[i], a0, a1, a2, a3, qb[w][0], qb[w][1], qc[i][0], qc[i][1]);
-              else qd_mma_f16_add(acc[i], a0, a1, a2, a3, qb[w][0], qb[w][1]);
-              qd_mma_f16_add(acc[i], c0, c1, c2, c3, qb[w][2], qb[w][3]);
-            }
+          for (int w = 0; w < W; ++w) {
+            const int i = (w / WG) % N;
+            const uint32_t a = ku[w], b = kv[w], ah = a >> 8, bh = b >> 8;
+            const uint32_t a0 = qd_pick<0x000f000fu, 0x64006400u>(a), a1 = qd_pick<0x000f000fu, 0x64006400u>(b);
+            const uint32_t a2 = qd_pick<0x00f000f0u, 0x54005400u>(a), a3 = qd_pick<0x00f000f0u, 0x54005400u>(b);
+            const uint32_t c0 = qd_pick<0x000f000fu, 0x64006400u>(ah), c1 = qd_pick<0x000f000fu, 0x64006400u>(bh);
+            const uint32_t c2 = qd_pick<0x00f000f0u, 0x54005400u>(ah), c3 = qd_pick<0x00f000f0u, 0x54005400u>(bh);
+            if (w % WG == 0 && w / WG < N) qd_mma_f16(acc[i], a0, a1, a2, a3, qb[w][0], qb[w][1], qc[i][0], qc[i][1]);
+            else qd_mma_f16_add(acc[i], a0, a1, a2, a3, qb[w][0], qb[w][1]);
+            qd_mma_f16_add(acc[i], c0, c1, c2, c3, qb[w][2], qb[w][3]);
+          }
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-              s[u][0] = fmaf(fa.s[i], acc[i][0], s[u][0]);
-              s[u][1] = fmaf(fa.s[i], acc[i][1], s[u][1]);
-              s[u][2] = fmaf(fb.s[i], acc[i][2], s[u][2]);
-              s[u][3] = fmaf(fb.s[i], acc[i][3], s[u][3]);
-            }
-            if (HALVES) {
+          for (int i = 0; i < N; ++i) {
+            s[u][0] = fmaf(fa.s[i], acc[i][0], s[u][0]);
+            s[u][1] = fmaf(fa.s[i], acc[i][1], s[u][1]);
+            s[u][2] = fmaf(fb.s[i], acc[i][2], s[u][2]);
+            s[u][3] = fmaf(fb.s[i], acc[i][3], s[u][3]);
+          }
+          if (HALVES) {
 #pragma unroll
-              for (int i = 0; i < 4; ++i) s[u][i] += __shfl_xor_sync(0xffffffffu, s[u][i], 2);
-            }
+            for (int i = 0; i < 4; ++i) s[u][i] += __shfl_xor_sync(0xffffffffu, s[u][i], 2);
           }
         }
-        // scores in log2 units, and which of them count: bit 2 u + (0: token tau, 1: tau + 2)
-        uint32_t seen = 15u;
-        if (edge) {
-          seen = 0;
+        // scores in log2 units; what is not visible has none (bit 2 u + (0: token tau, 1: tau + 2) of `seen`)
+        if (p.cap_log2 > 0.f) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) s[i >> 2][i & 3] = p.cap_log2 * ptx::tanh_ex2(s[i >> 2][i & 3] * scale[i & 1]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) s[i >> 2][i & 3] *= scale[i & 1];
+        }
+        QdScales<G, HALVES> f[4];  // of the values of tokens tau, tau + 2, 16 + tau, 18 + tau
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i].values(st + (i >> 1) * F.block + F.part + F.codes + (tau + 2 * (i & 1)) * 4 * G, x);
+        if (edge) {  // (what is not visible has no weight, and may hold no numbers)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int j = tok0 + (i >> 1) * 16 + tau + 2 * (i & 1);
-            if (j < see.len && (j >= see.lo || j < see.first)) seen |= 1u << i;
+            if (j >= see.len || (j < see.lo && j >= see.first)) {
+              s[i >> 1][2 * (i & 1)] = s[i >> 1][2 * (i & 1) + 1] = -INFINITY;
+              f[i].none();
+            }
           }
         }
-        float top[2] = {-INFINITY, -INFINITY};
+        float top[2] = {s[0][0], s[0][1]}, wide = fmaxf(fmaxf(f[0].largest(), f[1].largest()), fmaxf(f[2].largest(), f[3].largest()));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          float& v = s[i >> 2][i & 3];
-          v = p.cap_log2 > 0.f ? p.cap_log2 * ptx::tanh_ex2(v * scale[i & 1] * p.cap_scale) : v * scale[i & 1] * p.scale_log2;
-          if (edge && !((seen >> (i >> 1)) & 1u)) v = -INFINITY;
-          top[i & 1] = fmaxf(top[i & 1], v);
-        }
+        for (int i = 2; i < 8; ++i) top[i & 1] = fmaxf(top[i & 1], s[i >> 2][i & 3]);
+        if (__any_sync(0xffffffffu, top[0] > m[0] + 8.f || top[1] > m[1] + 8.f || wide > most)) {
 #pragma unroll
-        for (int d = 4; d < 32; d <<= 1) {
-          top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], d));
-          top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], d));
-        }
-        if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
-          float a[2];
+          for (int d = 4; d < 32; d <<= 1) {
+            top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], d));
+            top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], d));
+            wide = fmaxf(wide, __shfl_xor_sync(0xffffffffu, wide, d));
+          }
+          float a[2], more = 1.f;
+          if (wide > most) {  // 2^k <= wide < 2^(k + 1): up to 2^(k + 1), at 2^7 then
+            const int k = max(-100, static_cast<int>(__float_as_uint(wide) >> 23) - 127);
+            const float to = __uint_as_float(static_cast<uint32_t>(127 + 6 - k) << 23);
+            more = most > 0.f ? to / down : 1.f;  // (nothing has been added up yet: zeros)
+            down = to;
+            most = __uint_as_float(static_cast<uint32_t>(128 + k) << 23);
+          }
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             a[k] = top[k] > m[k] ? ptx::ex2_approx(m[k] - top[k]) : 1.f;
             m[k] = fmaxf(m[k], top[k]);
             l[k] *= a[k];
+#pragma unroll
+            for (int i = 0; i < N; ++i) zs[i][k] *= a[k];
+            a[k] *= more;
           }
 #pragma unroll
           for (int i = 0; i < MT; ++i) {
             o[i][0] *= a[0]; o[i][1] *= a[1]; o[i][2] *= a[0]; o[i][3] *= a[1];
           }
-#pragma unroll
-          for (int i = 0; i < N; ++i) {
-            oc[i][0] *= a[0]; oc[i][1] *= a[1];
-            zs[i][0] *= a[0]; zs[i][1] *= a[1];
-          }
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           float& v = s[i >> 2][i & 3];
-          v = edge && !((seen >> (i >> 1)) & 1u) ? 0.f : ptx::ex2_approx(v - m[i & 1]);
+          v = ptx::ex2_approx(v - m[i & 1]);  // (a chunk has a visible key, whose score m has seen: zero for what is not visible)
           l[i & 1] += v;
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          if (u < blocks) {
-            const uint8_t* vb = st + u * F.block + F.part;
-            QdScales<G, HALVES> fa, fb;
-            fa.values(vb + F.codes + tau * 4 * G, x, !edge || ((seen >> (2 * u)) & 1u));
-            fb.values(vb + F.codes + (tau + 2) * 4 * G, x, !edge || ((seen >> (2 * u + 1)) & 1u));
-            uint32_t vw[MT];
+          const uint8_t* vb = st + u * F.block + F.part;
+          const QdScales<G, HALVES>&fa = f[2 * u], &fb = f[2 * u + 1];
+          uint32_t vw[MT];
 #pragma unroll
-            for (int h = 0; h < D / 64; ++h) {
-              const uint4 v = *reinterpret_cast<const uint4*>(vb + h * 512 + g * 64 + t4 * 16);
-              vw[4 * h] = v.x; vw[4 * h + 1] = v.y; vw[4 * h + 2] = v.z; vw[4 * h + 3] = v.w;
-            }
-            uint32_t b0[N], b1[N], c0[N], c1[N];
+          for (int h = 0; h < D / 64; ++h) {
+            const uint4 v = *reinterpret_cast<const uint4*>(vb + h * 512 + g * 64 + t4 * 16);
+            vw[4 * h] = v.x; vw[4 * h + 1] = v.y; vw[4 * h + 2] = v.z; vw[4 * h + 3] = v.w;
+          }
+          uint32_t b0[N], b1[N];
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-              const float p0 = s[u][0] * fa.s[i], p1 = s[u][1] * fa.s[i], p2 = s[u][2] * fb.s[i], p3 = s[u][3] * fb.s[i];
-              zs[i][0] = fmaf(s[u][0], fa.mid[i], fmaf(s[u][2], fb.mid[i], zs[i][0]));
-              zs[i][1] = fmaf(s[u][1], fa.mid[i], fmaf(s[u][3], fb.mid[i], zs[i][1]));
-              const uint32_t r0 = pk2<__nv_bfloat16>(p0, p1), r1 = pk2<__nv_bfloat16>(p2, p3);
-              b0[i] = qd_transposed(r0);
-              b1[i] = qd_transposed(r1);
-              if (kTwo) {
-                c0[i] = qd_transposed(pk2<__nv_bfloat16>(p0 - qd_low(r0), p1 - qd_high(r0)));
-                c1[i] = qd_transposed(pk2<__nv_bfloat16>(p2 - qd_low(r1), p3 - qd_high(r1)));
-              }
-              constexpr uint32_t kOff = 0xc308c308u;  // -136
-              qd_mma_bf16_add(oc[i], kOff, kOff, kOff, kOff, b0[i], b1[i]);
-              if (kTwo) qd_mma_bf16_add(oc[i], kOff, kOff, kOff, kOff, c0[i], c1[i]);
-            }
+          for (int i = 0; i < N; ++i) {
+            const float sa = fa.s[i] * down, sb = fb.s[i] * down;
+            zs[i][0] = fmaf(s[u][0], fa.mid[i], fmaf(s[u][2], fb.mid[i], zs[i][0]));
+            zs[i][1] = fmaf(s[u][1], fa.mid[i], fmaf(s[u][3], fb.mid[i], zs[i][1]));
+            b0[i] = qd_transposed(pk2<__half>(s[u][0] * sa, s[u][1] * sa));
+            b1[i] = qd_transposed(pk2<__half>(s[u][2] * sb, s[u][3] * sb));
+          }
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-              const int j = (i * 16 / GROUP) % N;
-              const uint32_t v = vw[i];
-              const uint32_t a0 = (v & 0x000f000fu) | 0x43004300u, a1 = ((v >> 4) & 0x000f000fu) | 0x43004300u;
-              const uint32_t a2 = ((v >> 8) & 0x000f000fu) | 0x43004300u, a3 = ((v >> 12) & 0x000f000fu) | 0x43004300u;
-              qd_mma_bf16_add(o[i], a0, a1, a2, a3, b0[j], b1[j]);
-              if (kTwo) qd_mma_bf16_add(o[i], a0, a1, a2, a3, c0[j], c1[j]);
-            }
+          for (int i = 0; i < MT; ++i) {
+            const int j = (i * 16 / GROUP) % N;
+            const uint32_t v = vw[i], vh = v >> 8;
+            const uint32_t a0 = qd_pick<0x000f000fu, 0x64006400u>(v), a1 = qd_pick<0x00f000f0u, 0x54005400u>(v);
+            const uint32_t a2 = qd_pick<0x000f000fu, 0x64006400u>(vh), a3 = qd_pick<0x00f000f0u, 0x54005400u>(vh);
+            qd_mma_f16_add(o[i], 0xe408e408u, 0xd480d480u, 0xe408e408u, 0xd480d480u, b0[j], b1[j]);  // -1032, -72
+            qd_mma_f16_add(o[i], a0, a1, a2, a3, b0[j], b1[j]);
           }
         }
         __syncwarp();  // every lane has read the stage
@@ -616,6 +669,7 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
       }
 
       // ------------------------------------------------------------ the end of a piece
+      it = qd_kept(rec + 4);
 #pragma unroll
       for (int d = 4; d < 32; d <<= 1) {
 #pragma unroll
@@ -625,12 +679,14 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
           for (int i = 0; i < N; ++i) zs[i][k] += __shfl_xor_sync(0xffffffffu, zs[i][k], d);
         }
       }
+      const float up = 1.f / down;
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         const int j = (i * 16 / GROUP) % N;
-        o[i][0] += oc[j][0] + zs[j][0]; o[i][1] += oc[j][1] + zs[j][1];
-        o[i][2] += oc[j][0] + zs[j][0]; o[i][3] += oc[j][1] + zs[j][1];
+        o[i][0] = fmaf(o[i][0], up, zs[j][0]); o[i][1] = fmaf(o[i][1], up, zs[j][1]);
+        o[i][2] = fmaf(o[i][2], up, zs[j][0]); o[i][3] = fmaf(o[i][3], up, zs[j][1]);
       }
+      const unsigned X0 = cut.begin(first_warp), X1 = cut.begin(first_warp + warps), x0 = cut.begin(first_warp + warp), x1 = cut.begin(first_warp + warp + 1);
       if (it.start >= x0 && it.stop <= x1) {
         float r[2];
 #pragma unroll
@@ -641,7 +697,7 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
             f = ptx::ex2_approx(m[k] - top);
             sum = fmaf(f, l[k], ptx::ex2_approx(snk - top));
           }
-          r[k] = sum != 0.f ? f / sum : 0.f;
+          r[k] = sum != 0.f ? f * ptx::rcp_approx(sum) : 0.f;
         }
         // rounded, and 8 x 8 blocks transposed, so that a lane has two neighbouring dimensions of head g
         const int hq = HALVES ? g & 3 : g, xq = HALVES ? g >> 2 : 0;
@@ -654,10 +710,13 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
             *reinterpret_cast<uint32_t*>(to + 16 * i + 8) = b;
           }
         }
-      } else {
-        // a piece: the range's first one has a slot, the last one the ring, which has nothing to take any more
-        float* to = first ? slots + warp * slot : reinterpret_cast<float*>(smem + warp * ring_bytes);
-        if (!first) __syncwarp();
+        continue;
+      }
+
+      // ------------------------------------------------------------ a piece: its sums into the slot, or the ring, which takes no more
+      const bool in_slot = x0 >= it.start;
+      {
+        float* to = in_slot ? slots + warp * slot : reinterpret_cast<float*>(smem + warp * ring_bytes);
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
           if (!HALVES || (i * 16 / GROUP) / N == x) {
@@ -680,105 +739,152 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
               ml[2 * (col + k) + 1] = l[k];
             }
         }
+        __threadfence_block();
+        __syncwarp();
+        if (lane == 0) rec[in_slot ? 8 : 9] = 1;
       }
-    }
-  }
-  __syncthreads();
-
-  // -------------------------------------------------------------------- pieces within the block
-  const unsigned X0 = cut.begin(first_warp), X1 = cut.begin(first_warp + kQdWarps);
-  float* const part_ml = p.part + static_cast<int64_t>(2) * gridDim.x * p.rep * D;
-  // the sum of a sequence's pieces is written as its output or, where other blocks have some, to scratch
-  auto store = [&](int b, int hd, int d, const float (&acc)[4], float M, float L) {
-    float f = 1.f, sum = L;
-    if (p.sink != nullptr) {
-      const float snk = ldf<T>(reinterpret_cast<const T*>(p.sink) + hd) * 1.4426950408889634f, top = fmaxf(snk, M);
-      f = exp2f(M - top);
-      sum = fmaf(f, L, exp2f(snk - top));
-    }
-    const float r = sum != 0.f ? f / sum : 0.f;
-    stf4<T>(out + b * p.out_stride + static_cast<int64_t>(hd) * D + d, make_float4(acc[0] * r, acc[1] * r, acc[2] * r, acc[3] * r));
-  };
-  if (warp < kQdWarps) {
-    const unsigned x0 = cut.begin(first_warp + warp), x1 = cut.begin(first_warp + warp + 1);
-#pragma unroll 1
-    for (int k = 0; k < 2; ++k) {
-      const QdPiece& it = k ? last_piece : first_piece;
-      if (x0 == x1 || (k && first_piece.start == last_piece.start)) continue;  // (one piece only)
-      const bool whole = it.start >= x0 && it.stop <= x1;
-      if (whole || (it.start < x0 && warp != 0)) continue;   // stored already, or an earlier warp's to add up
+      // The warps of this block that end with the sequence share its heads (one that goes on with the next sequence has them to itself, where
+      // nobody else has a piece); the i-th lane looks after the i-th of all warps that have one.
+      const unsigned at = cut.begin(first_warp + min(lane, warps)), behind = cut.begin(first_warp + min(lane + 1, warps));
+      const bool has = lane < warps && at < it.stop && behind > it.start;
+      const uint32_t having = __ballot_sync(0xffffffffu, has), ending = __ballot_sync(0xffffffffu, has && behind <= it.stop);
+      const int w0 = __ffs(having) - 1, n = __popc(having), each = max(1, __popc(ending)), h0 = warp - w0;
+      if (h0 >= p.rep || (n > 1 && x1 > it.stop)) continue;
+      const unsigned begin = cut.begin(first_warp + min(w0 + lane, warps));
+      const int from = (lane < n && begin < it.start ? (w0 + lane) * (ring_bytes / 4) : kQdWarps * ring_bytes / 4 + min(w0 + lane, kQdWarps - 1) * slot);
+      if (!qd_wait(records + min(w0 + lane, kQdWarps - 1) * 16 + (begin < it.start ? 9 : 8), lane < n, abort_flag)) {
+        if (p.status && lane == 0) atomicCAS(p.status, 0, kStatusTimeoutEpilogue);
+        continue;
+      }
+      constexpr int C = D / 32;  // dimensions of a lane
       const bool inside = it.start >= X0 && it.stop <= X1;
-      const int place = blockIdx.x * 2 + (it.start < X0 ? 0 : 1);
-      auto source = [&](int v) -> const float* {  // where warp v has its piece
-        return max(it.start, cut.begin(first_warp + v)) == cut.begin(first_warp + v) ? slots + v * slot : reinterpret_cast<const float*>(smem + v * ring_bytes);
+      float* const part_ml = p.part + static_cast<int64_t>(2) * gridDim.x * p.rep * D;
+      const int64_t place = (blockIdx.x * 2 + (it.start < X0 ? 0 : 1)) * p.rep;
+      auto store = [&](int hh, const float (&acc)[C], float M, float L) {  // the sum of all pieces, divided
+        float f = 1.f, sum = L;
+        if (p.sink != nullptr) {
+          const float snk = ldf<T>(reinterpret_cast<const T*>(p.sink) + it.head * p.rep + hh) * 1.4426950408889634f, most = fmaxf(snk, M);
+          f = ptx::ex2_approx(M - most);
+          sum = fmaf(f, L, ptx::ex2_approx(snk - most));
+        }
+        const float r = sum != 0.f ? f * ptx::rcp_approx(sum) : 0.f;
+        T* to = out + it.b * p.out_stride + static_cast<int64_t>(it.head * p.rep + hh) * D + lane * C;
+#pragma unroll
+        for (int i = 0; i < C; i += 2) stf2<T>(to + i, acc[i] * r, acc[i + 1] * r);
       };
-      for (int e = lane; e < p.rep * (D / 4); e += 32) {
-        const int hh = e / (D / 4), d = (e % (D / 4)) * 4;
-        float M = -INFINITY, L = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int v = warp; v < kQdWarps && cut.begin(first_warp + v) < it.stop; ++v) M = fmaxf(M, source(v)[p.rep * (D + 4) + 2 * hh]);
-        for (int v = warp; v < kQdWarps && cut.begin(first_warp + v) < it.stop; ++v) {
-          const float* from = source(v);
-          const float mv = from[p.rep * (D + 4) + 2 * hh], f = mv == M ? 1.f : exp2f(mv - M);
-          L = fmaf(f, from[p.rep * (D + 4) + 2 * hh + 1], L);
-          const float4 o = *reinterpret_cast<const float4*>(from + hh * (D + 4) + d);
-          acc[0] = fmaf(f, o.x, acc[0]);
-          acc[1] = fmaf(f, o.y, acc[1]);
-          acc[2] = fmaf(f, o.z, acc[2]);
-          acc[3] = fmaf(f, o.w, acc[3]);
-        }
-        if (inside) {
-          store(it.b, it.head * p.rep + hh, d, acc, M, L);
+      auto four = [&](const float* v, float f, float (&acc)[C], bool global) {
+        if (C == 4) {
+          const float4 t = global ? __ldcg(reinterpret_cast<const float4*>(v)) : *reinterpret_cast<const float4*>(v);
+          acc[0] = fmaf(f, t.x, acc[0]); acc[1] = fmaf(f, t.y, acc[1]); acc[2 % C] = fmaf(f, t.z, acc[2 % C]); acc[3 % C] = fmaf(f, t.w, acc[3 % C]);
         } else {
-          __stcg(reinterpret_cast<float4*>(p.part + (static_cast<int64_t>(place) * p.rep + hh) * D + d), make_float4(acc[0], acc[1], acc[2], acc[3]));
-          if (d == 0) __stcg(reinterpret_cast<float2*>(part_ml) + static_cast<int64_t>(place) * p.rep + hh, make_float2(M, L));
+          const float2 t = global ? __ldcg(reinterpret_cast<const float2*>(v)) : *reinterpret_cast<const float2*>(v);
+          acc[0] = fmaf(f, t.x, acc[0]); acc[1] = fmaf(f, t.y, acc[1]);
         }
-      }
-      if (!inside) {
-        __threadfence();
-        if (lane == 0) {
-          across[it.start < X0 ? 0 : 1] = it.b * p.heads + it.head;
-        }
-      }
-    }
-  }
-  __syncthreads();
-
-  // -------------------------------------------------------------------- pieces of several blocks: whoever is last adds them up
+      };
+      auto add_up = [&](auto heads) {  // H heads at a time: their loads follow one another without a wait
+        constexpr int H = decltype(heads)::value;
+        const float* const all = reinterpret_cast<const float*>(smem);
 #pragma unroll 1
-  for (int k = 0; k < 2; ++k) {
-    const int item = across[k];
-    if (item < 0) continue;
-    const int b = item / p.heads, head = item % p.heads;
-    const unsigned start = static_cast<unsigned>(head) * tab.before[p.batch] + tab.before[b], stop = start + tab.before[b + 1] - tab.before[b];
-    const unsigned c0 = cut.range(start) / kQdWarps, c1 = cut.range(stop - 1) / kQdWarps;
-    if (threadIdx.x == 0) {
-      __threadfence();
-      const bool is_last = atomicAdd(p.tickets + item, 1u) == c1 - c0;
-      if (is_last) p.tickets[item] = 0u;
-      __threadfence();
-      across[2 + k] = is_last;
-    }
-    __syncthreads();
-    if (!across[2 + k]) continue;
-    for (int e = threadIdx.x; e < p.rep * (D / 4); e += kQdThreads) {
-      const int hh = e / (D / 4), d = (e % (D / 4)) * 4;
-      auto place = [&](unsigned c) { return static_cast<int64_t>(c * 2 + (start < cut.begin(c * kQdWarps) ? 0 : 1)) * p.rep + hh; };
-      float M = -INFINITY, L = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-      for (unsigned c = c0; c <= c1; ++c) M = fmaxf(M, __ldcg(reinterpret_cast<const float2*>(part_ml) + place(c)).x);
-#pragma unroll 4
-      for (unsigned c = c0; c <= c1; ++c) {
-        const int64_t at = place(c);
-        const float2 ml = __ldcg(reinterpret_cast<const float2*>(part_ml) + at);
-        const float f = ml.x == M ? 1.f : exp2f(ml.x - M);
-        const float4 o = __ldcg(reinterpret_cast<const float4*>(p.part + at * D + d));
-        L = fmaf(f, ml.y, L);
-        acc[0] = fmaf(f, o.x, acc[0]);
-        acc[1] = fmaf(f, o.y, acc[1]);
-        acc[2] = fmaf(f, o.z, acc[2]);
-        acc[3] = fmaf(f, o.w, acc[3]);
+        for (int hb = h0; hb < p.rep; hb += H * each) {
+          float2 ml[H];
+          float M[H], L[H], f[H], acc[H][C];
+          int hh[H];
+#pragma unroll
+          for (int h = 0; h < H; ++h) {  // (fewer heads than H: the first one again)
+            hh[h] = hb + h * each < p.rep ? hb + h * each : hb;
+            ml[h] = lane < n ? *reinterpret_cast<const float2*>(all + from + p.rep * (D + 4) + 2 * hh[h]) : make_float2(-INFINITY, 0.f);
+          }
+#pragma unroll
+          for (int h = 0; h < H; ++h) {
+            M[h] = warp_max(ml[h].x);
+            f[h] = ml[h].x == M[h] ? 1.f : ptx::ex2_approx(ml[h].x - M[h]);
+            L[h] = warp_sum(lane < n ? f[h] * ml[h].y : 0.f);
+#pragma unroll
+            for (int i = 0; i < C; ++i) acc[h][i] = 0.f;
+          }
+          for (int v = 0; v < n; ++v) {
+            const float* o = all + __shfl_sync(0xffffffffu, from, v) + lane * C;
+#pragma unroll
+            for (int h = 0; h < H; ++h) four(o + hh[h] * (D + 4), __shfl_sync(0xffffffffu, f[h], v), acc[h], false);
+          }
+#pragma unroll
+          for (int h = 0; h < H; ++h) {
+            if (inside) {
+              store(hh[h], acc[h], M[h], L[h]);
+            } else {
+              float* to = p.part + (place + hh[h]) * D + lane * C;
+              if (C == 4) __stcg(reinterpret_cast<float4*>(to), make_float4(acc[h][0], acc[h][1], acc[h][2 % C], acc[h][3 % C]));
+              else __stcg(reinterpret_cast<float2*>(to), make_float2(acc[h][0], acc[h][1]));
+              if (lane == 0) __stcg(reinterpret_cast<float2*>(part_ml) + place + hh[h], make_float2(M[h], L[h]));
+            }
+          }
+        }
+      };
+      if (h0 + each < p.rep) add_up(std::integral_constant<int, 4>{});
+      else add_up(std::integral_constant<int, 1>{});
+      if (inside) continue;
+
+      // ------------------------------------------------------------ pieces of several blocks: for each head, whoever is last adds them up
+      const int c0 = cut.range(it.start) / warps, blocks = static_cast<int>(cut.range(it.stop - 1) / warps) - c0 + 1;
+      __syncwarp();
+      bool is_last = false;
+      if (h0 + lane * each < p.rep) {
+        unsigned* ticket = p.tickets + (it.b * p.heads + it.head) * p.rep + h0 + lane * each;
+        __threadfence();
+        is_last = atomicAdd(ticket, 1u) == static_cast<unsigned>(blocks - 1);
+        if (is_last) *ticket = 0u;
+        __threadfence();
       }
-      store(b, head * p.rep + hh, d, acc, M, L);
+      __syncwarp();
+      uint32_t todo = __ballot_sync(0xffffffffu, is_last);
+      // H heads at a time, UNROLL of their pieces: eight loads are on their way
+      auto merge = [&](auto heads, auto unroll) {
+        constexpr int H = decltype(heads)::value, UNROLL = decltype(unroll)::value;
+        const float* from[H];
+        const float2* ml_from[H];
+        int hh[H];
+        float M[H], L[H], acc[H][C];
+#pragma unroll
+        for (int h = 0; h < H; ++h) {  // (fewer heads than H: the last one again)
+          hh[h] = h0 + (__ffs(todo) - 1) * each;
+          if (todo & (todo - 1) || h == H - 1) todo &= todo - 1;
+          // the first block has its piece in its second place, the others in their first: piece c is 2 c - 1 places behind that
+          from[h] = p.part + (static_cast<int64_t>(2 * c0 + 1) * p.rep + hh[h]) * D + lane * C;
+          ml_from[h] = reinterpret_cast<const float2*>(part_ml) + static_cast<int64_t>(2 * c0 + 1) * p.rep + hh[h];
+          M[h] = -INFINITY;
+          L[h] = 0.f;
+#pragma unroll
+          for (int i = 0; i < C; ++i) acc[h][i] = 0.f;
+        }
+        for (int c = 0; c < blocks; c += 32) {
+          const int n = min(32, blocks - c);
+          float f[H];
+          float2 ml[H];
+#pragma unroll
+          for (int h = 0; h < H; ++h) ml[h] = lane < n ? __ldcg(ml_from[h] + max(0, 2 * (c + lane) - 1) * p.rep) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+          for (int h = 0; h < H; ++h) {
+            const float top = fmaxf(M[h], warp_max(ml[h].x)), a = M[h] == top ? 1.f : ptx::ex2_approx(M[h] - top);
+            M[h] = top;
+            f[h] = ml[h].x == top ? 1.f : ptx::ex2_approx(ml[h].x - top);
+            L[h] = fmaf(a, L[h], warp_sum(lane < n ? f[h] * ml[h].y : 0.f));
+#pragma unroll
+            for (int i = 0; i < C; ++i) acc[h][i] *= a;
+          }
+#pragma unroll UNROLL
+          for (int v = 0; v < n; ++v) {
+            const int64_t at = static_cast<int64_t>(max(0, 2 * (c + v) - 1)) * p.rep * D;
+#pragma unroll
+            for (int h = 0; h < H; ++h) four(from[h] + at, __shfl_sync(0xffffffffu, f[h], v), acc[h], true);
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < H; ++h) store(hh[h], acc[h], M[h], L[h]);
+      };
+      while (todo) {
+        if (todo & (todo - 1)) merge(std::integral_constant<int, 4>{}, std::integral_constant<int, 2>{});
+        else merge(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});
+      }
     }
   }
 }
@@ -847,7 +953,7 @@ int blitz_attn_decode_quant(const void* q, int64_t q_stride, const void* pool, c
     p.q = (const char*)q + (int64_t)b * q_stride * 2;
     p.out = (char*)out + (int64_t)b * out_stride * 2;
     p.indptr = indptr + b; p.last_page_len = last_page_len + b;
-    p.tickets = (unsigned*)workspace + (int64_t)b * p.heads;
+    p.tickets = (unsigned*)workspace + (int64_t)b * q_heads;
     const int rc = quant_kv_dispatch(dtype, dim, group, DecodeQuantLaunch{p, device_sm_count(), stream});
     if (rc) return rc;
   }

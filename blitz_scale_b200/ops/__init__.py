@@ -464,33 +464,37 @@ def quant_kv_pool(pages: int, page_size: int, kv_heads: int, dim: int, group: in
     return QuantKV(torch.zeros(pages, kv_heads, page_size // 16, quant_kv_block_bytes(dim, group), dtype=torch.uint8, device=device), dim, group)
 
 
-def _quant(cache: QuantKV, *others: torch.Tensor) -> torch.Tensor:
-    """The pool of a 4-bit cache, after checks of it and of what a call brings beside it."""
-    pool = cache.pool
-    if pool.dtype != torch.uint8 or pool.dim() != 4 or not pool.is_contiguous() or pool.shape[3] != quant_kv_block_bytes(cache.dim, cache.group) \
-            or pool.data_ptr() % 16:
-        raise ValueError(f"not a 4-bit cache of heads of {cache.dim} in groups of {cache.group}: {tuple(pool.shape)} {pool.dtype}")
-    if pool.shape[2] & (pool.shape[2] - 1) or pool.shape[2] < 1:
-        raise ValueError(f"pages of a 4-bit cache hold 16 tokens times a power of two, got {16 * pool.shape[2]}")
-    for t in (pool, *others):
-        if not t.is_cuda or t.get_device() != torch.cuda.current_device():
-            raise ValueError(f"a tensor on {t.device}: the kernels run on the current CUDA device")
+def _quant(cache: QuantKV, *others: Optional[torch.Tensor]) -> torch.Tensor:
+    """The pool of a 4-bit cache, after checks of it and of what a call brings beside it (None: nothing)."""
+    pool, dim, group = cache
+    shape = pool.shape
+    if pool.dtype != torch.uint8 or len(shape) != 4 or not pool.is_contiguous() or shape[3] != quant_kv_block_bytes(dim, group) or pool.data_ptr() & 15:
+        raise ValueError(f"not a 4-bit cache of heads of {dim} in groups of {group}: {tuple(shape)} {pool.dtype}")
+    if shape[2] < 1 or shape[2] & (shape[2] - 1):
+        raise ValueError(f"pages of a 4-bit cache hold 16 tokens times a power of two, got {16 * shape[2]}")
+    at = pool.get_device()
+    if at < 0 or at != _raw_device():
+        raise ValueError(f"a cache on {pool.device}: the kernels run on the current CUDA device")
+    for t in others:
+        if t is not None and t.get_device() != at:
+            raise ValueError(f"a tensor on {t.device}, the cache on {pool.device}: the kernels run on the current CUDA device")
     return pool
 
 
-def _quant_rows(x: torch.Tensor, cache: QuantKV, what: str) -> torch.Tensor:
+def _quant_rows(x: torch.Tensor, cache: QuantKV, what: str) -> None:
     """Rows [T, kv_heads * dim] (or [T, kv_heads, dim]) of keys or values in 16 bits, with any pitch of whole 16 bytes."""
-    _dt(x)
+    if x.dtype not in _DT:
+        raise TypeError(f"{what}: kernels take fp16/bf16 tensors, got {x.dtype}")
     H, D = cache.pool.shape[1], cache.dim
-    if x.dim() not in (2, 3) or x.shape[1:] not in ((H * D,), (H, D)) or x.stride(-1) != 1 or (x.dim() == 3 and x.stride(1) != D):
-        raise ValueError(f"{what}: rows of {H} heads of {D} dimensions, got {tuple(x.shape)} with strides {x.stride()}")
-    if x.stride(0) % 8 or x.data_ptr() % 16:
+    shape, step = x.shape, x.stride()
+    if len(shape) == 2 and (shape[1] != H * D or step[1] != 1) or len(shape) == 3 and (shape[1:] != (H, D) or step[1:] != (D, 1)) or len(shape) not in (2, 3):
+        raise ValueError(f"{what}: rows of {H} heads of {D} dimensions, got {tuple(shape)} with strides {step}")
+    if step[0] & 7 or x.data_ptr() & 15:
         raise ValueError(f"{what}: rows have to start on 16-byte boundaries")
-    return x
 
 
 def _int32(t: torch.Tensor, n: Optional[int], what: str) -> torch.Tensor:
-    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.numel() < n):
+    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or (n and t.shape[0] < n):
         raise ValueError(f"{what}: {'' if n is None else f'at least {n} '}int32 numbers, got {tuple(t.shape)} {t.dtype}")
     return t
 
@@ -499,28 +503,36 @@ def quant_kv_store(k: torch.Tensor, v: torch.Tensor, slot: torch.Tensor, cache: 
     """Quantise rows of (rotated) keys and values into a 4-bit cache.  ``k``, ``v``: [T, kv_heads * dim] in 16 bits, e.g. column ranges of
     the fused projection; ``slot`` [T]: page * page_size + offset (negative: the row is not written).  Each slot once in a call."""
     pool = _quant(cache, k, v, slot)
-    T = k.shape[0]
+    T, shape = k.shape[0], pool.shape
     _quant_rows(k, cache, "k")
     _quant_rows(v, cache, "v")
     if v.shape[0] != T or v.dtype != k.dtype:
         raise ValueError(f"as many values as keys, of their type: {tuple(v.shape)} {v.dtype} beside {tuple(k.shape)} {k.dtype}")
     _int32(slot, T, "slot")
-    _check(lib().blitz_quant_kv_store(_p(k), k.stride(0), _p(v), v.stride(0), _p(slot), _p(pool), T, pool.shape[1], cache.dim, cache.group,
-                                      cache.page_size, pool.shape[0], _status_ptr(k), _dt(k), _stream()), "blitz_quant_kv_store")
+    rc = lib().blitz_quant_kv_store(k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), slot.data_ptr(), pool.data_ptr(), T, shape[1], cache.dim,
+                                    cache.group, 16 * shape[2], shape[0], _status_ptr(k), _DT[k.dtype], _stream())
+    if rc:
+        _check(rc, "blitz_quant_kv_store")
 
 
 def quant_kv_load(cache: QuantKV, slot: torch.Tensor, *, dtype: torch.dtype = torch.bfloat16, k: Optional[torch.Tensor] = None,
                   v: Optional[torch.Tensor] = None):
     """Keys and values [T, kv_heads, dim] of slots of a 4-bit cache, rounded to 16 bits (rows with a negative slot are left as they are)."""
+    pool, D, group = cache
     _int32(slot, None, "slot")
-    shape = (slot.numel(), cache.pool.shape[1], cache.dim)
-    k = torch.empty(shape, dtype=dtype, device=cache.pool.device) if k is None else k
-    v = torch.empty(shape, dtype=dtype, device=cache.pool.device) if v is None else v
-    if any(t.shape != shape or not t.is_contiguous() or t.dtype != k.dtype or t.data_ptr() % 16 for t in (k, v)):
-        raise ValueError(f"k and v: contiguous {shape} of one type")
-    pool = _quant(cache, slot, k, v)
-    _check(lib().blitz_quant_kv_load(_p(pool), _p(slot), slot.numel(), 0, _p(k), _p(v), pool.shape[1], cache.dim, cache.group, cache.page_size,
-                                     0, pool.shape[0], _status_ptr(pool), _dt(k), _stream()), "blitz_quant_kv_load")
+    n, (pages, H, blocks, _) = slot.shape[0], pool.shape
+    if k is None:
+        k = torch.empty((n, H, D), dtype=dtype, device=pool.device)
+    if v is None:
+        v = torch.empty((n, H, D), dtype=k.dtype, device=pool.device)
+    for t in (k, v):
+        if t.shape != (n, H, D) or not t.is_contiguous() or t.dtype != k.dtype or t.data_ptr() & 15:
+            raise ValueError(f"k and v: contiguous {(n, H, D)} of one type, got {tuple(t.shape)} {t.dtype}")
+    _quant(cache, slot, k, v)
+    rc = lib().blitz_quant_kv_load(pool.data_ptr(), slot.data_ptr(), n, 0, k.data_ptr(), v.data_ptr(), H, D, group, 16 * blocks, 0, pages, _status_ptr(pool),
+                                   _dt(k), _stream())
+    if rc:
+        _check(rc, "blitz_quant_kv_load")
     return k, v
 
 
@@ -538,59 +550,64 @@ def quant_kv_pages(cache: QuantKV, pages: torch.Tensor, *, dtype: torch.dtype = 
     return out
 
 
-def quant_attn_workspace_bytes(batch: int, q_heads: int, head_dim: int, device="cuda") -> int:
+def quant_attn_workspace_bytes(batch: int, q_heads: int, head_dim: int, device=None) -> int:
     """Scratch of `attn_decode` over a 4-bit cache, for up to `batch` sequences: zero-filled before its first use, for one call at a time."""
-    with torch.cuda.device(device):
+    with torch.cuda.device(device):         # (None: the current one)
         return int(lib().blitz_attn_decode_quant_workspace_bytes(batch, q_heads, head_dim))
 
 
-def _quant_attn(q: torch.Tensor, cache: QuantKV, q_heads: int, kv_heads: int, head_dim: int, page_size: int, window: int, keep_first: int,
-                softcap: float, sink: Optional[torch.Tensor], out: Optional[torch.Tensor], refused: dict, *others: torch.Tensor):
-    """Checks of an attention call over a 4-bit cache; returns (pool, out)."""
-    named = [n for n, x in refused.items() if x is not None and x is not False]
-    if named:
-        raise ValueError(f"attention over a 4-bit cache has no {', '.join(named)}")
-    _dt(q)
-    D = cache.dim
-    if (kv_heads, head_dim, page_size) != (cache.pool.shape[1], D, cache.page_size) or q_heads < 1 or q_heads % kv_heads:
-        raise ValueError(f"{q_heads} query and {kv_heads} KV heads of {head_dim}, pages of {page_size}: the 4-bit cache has {cache.pool.shape[1]} "
-                         f"heads of {D}, pages of {cache.page_size}")
-    if q.dim() != 2 or q.shape[1] < q_heads * D or q.stride(1) != 1 or q.stride(0) % 8 or q.data_ptr() % 16:
-        raise ValueError(f"q: rows of {q_heads} heads of {D} dimensions that start on 16-byte boundaries, got {tuple(q.shape)}, strides {q.stride()}")
+def _quant_attn(q: torch.Tensor, rows: int, cache: QuantKV, q_heads: int, kv_heads: int, head_dim: int, page_size: int, window: int, keep_first: int,
+                softcap: float, sink: Optional[torch.Tensor], out: Optional[torch.Tensor], refused: dict, *others: Optional[torch.Tensor]) -> torch.Tensor:
+    """Checks of an attention call over a 4-bit cache; returns where its output goes."""
+    for name, x in refused.items():
+        if x is not None and x is not False:
+            raise ValueError(f"attention over a 4-bit cache has no {name}")
+    dt, D, shape = q.dtype, cache.dim, cache.pool.shape
+    if dt not in _DT:
+        raise TypeError(f"kernels take fp16/bf16 tensors, got {dt}")
+    if kv_heads != shape[1] or head_dim != D or page_size != 16 * shape[2] or q_heads < 1 or q_heads % kv_heads:
+        raise ValueError(f"{q_heads} query and {kv_heads} KV heads of {head_dim}, pages of {page_size}: the 4-bit cache has {shape[1]} "
+                         f"heads of {D}, pages of {16 * shape[2]}")
+    if q.dim() != 2 or q.shape[0] < rows or q.shape[1] < q_heads * D or q.stride(1) != 1 or q.stride(0) & 7 or q.data_ptr() & 15:
+        raise ValueError(f"q: {rows} rows of {q_heads} heads of {D} dimensions that start on 16-byte boundaries, got {tuple(q.shape)}, strides {q.stride()}")
     if window < 0 or keep_first < 0 or not softcap >= 0.0:
         raise ValueError(f"window {window}, keep_first {keep_first}, softcap {softcap}")
-    if sink is not None and (sink.dtype != q.dtype or sink.numel() != q_heads or not sink.is_contiguous()):
-        raise ValueError(f"sink: {q_heads} numbers of {q.dtype}")
+    if sink is not None and (sink.dtype != dt or sink.numel() != q_heads or not sink.is_contiguous()):
+        raise ValueError(f"sink: {q_heads} numbers of {dt}")
     if out is None:
-        out = torch.empty((q.shape[0], q_heads * D), dtype=q.dtype, device=q.device)
-    elif out.dim() != 2 or out.shape[1] < q_heads * D or out.dtype != q.dtype or out.stride(1) != 1 or out.stride(0) % 8 or out.data_ptr() % 16:
-        raise ValueError(f"out: rows of {q_heads * D} {q.dtype} that start on 16-byte boundaries, got {tuple(out.shape)} {out.dtype}")
-    return _quant(cache, q, out, *others, *([] if sink is None else [sink])), out
+        out = torch.empty((rows, q_heads * D), dtype=dt, device=q.device)
+    elif out.dim() != 2 or out.shape[0] < rows or out.shape[1] < q_heads * D or out.dtype != dt or out.stride(1) != 1 or out.stride(0) & 7 or out.data_ptr() & 15:
+        raise ValueError(f"out: {rows} rows of {q_heads * D} {dt} that start on 16-byte boundaries, got {tuple(out.shape)} {out.dtype}")
+    _quant(cache, q, out, sink, *others)
+    return out
 
 
 def _attn_decode_quant(q, cache, indices, indptr, last_page_len, q_heads, kv_heads, head_dim, page_size, num_splits, workspace, out, sm_scale,
                        window, keep_first, softcap, sink, refused, static_table):
-    B = indptr.numel() - 1
-    if num_splits < 0 or B < 0 or q.shape[0] < B or (out is not None and out.shape[0] < B):
-        raise ValueError(f"{B} sequences: q {tuple(q.shape)}, out {None if out is None else tuple(out.shape)}, num_splits {num_splits}")
-    _int32(indptr, None, "indptr")
+    _int32(indptr, 1, "indptr")
+    B = indptr.shape[0] - 1
     _int32(last_page_len, B, "last_page_len")
     _int32(indices, None, "indices")
-    if workspace is not None and (workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.data_ptr() % 256):
-        raise ValueError(f"workspace: bytes that start on a 256-byte boundary, got {workspace.dtype}")
-    pool, out = _quant_attn(q[:B], cache, q_heads, kv_heads, head_dim, page_size, window, keep_first, softcap, sink, out, refused, indices, indptr,
-                            last_page_len, *([] if workspace is None else [workspace]))
+    if num_splits < 0:
+        raise ValueError(f"num_splits {num_splits}")
+    out = _quant_attn(q, B, cache, q_heads, kv_heads, head_dim, page_size, window, keep_first, softcap, sink, out, refused, indices, indptr, last_page_len,
+                      workspace)
     if B == 0:
         return out
-    n = int(lib().blitz_attn_decode_quant_workspace_bytes(B, q_heads, head_dim))
     if workspace is None:
-        workspace = torch.zeros(n, dtype=torch.uint8, device=q.device)
-    elif workspace.numel() < n:
-        raise ValueError(f"workspace of {workspace.numel()} bytes, {n} are needed")
-    _check(lib().blitz_attn_decode_quant(_p(q), q.stride(0), _p(pool), _p(indices), _p(indptr), _p(last_page_len), _p(out), out.stride(0), _p(workspace),
-                                         workspace.numel(), B, q_heads, kv_heads, head_dim, cache.group, page_size,
-                                         pool.shape[0], head_dim ** -0.5 if sm_scale is None else sm_scale, window, keep_first, softcap,
-                                         _p(sink), int(static_table), _status_ptr(q), _dt(q), _stream()), "blitz_attn_decode_quant")
+        workspace = torch.zeros(quant_attn_workspace_bytes(B, q_heads, head_dim), dtype=torch.uint8, device=q.device)
+    elif workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.data_ptr() & 255:
+        raise ValueError(f"workspace: bytes that start on a 256-byte boundary, got {workspace.dtype}")
+    pool, size = cache.pool, workspace.numel()
+    rc = lib().blitz_attn_decode_quant(q.data_ptr(), q.stride(0), pool.data_ptr(), indices.data_ptr(), indptr.data_ptr(), last_page_len.data_ptr(),
+                                       out.data_ptr(), out.stride(0), workspace.data_ptr(), size, B, q_heads, kv_heads, head_dim, cache.group, page_size,
+                                       pool.shape[0], head_dim ** -0.5 if sm_scale is None else sm_scale, window, keep_first, softcap,
+                                       None if sink is None else sink.data_ptr(), 1 if static_table else 0, _status_ptr(q), _DT[q.dtype], _stream())
+    if rc:
+        need = quant_attn_workspace_bytes(B, q_heads, head_dim)
+        if size < need:
+            raise ValueError(f"workspace of {size} bytes, {need} are needed")
+        _check(rc, "blitz_attn_decode_quant")
     return out
 
 
@@ -685,9 +702,7 @@ def attn_prefill_paged(q: torch.Tensor, kv_layer: KVLayer, page_indices: torch.T
             raise ValueError(f"skip_pages {skip_pages} of {page_indices.numel()} pages")
         if work.dtype != torch.int32 or work.dim() != 2 or work.shape[1] != 8 or not work.is_contiguous():
             raise ValueError(f"work: records of prefill_work_list, got {tuple(work.shape)} {work.dtype}")
-        if out is not None and out.shape[0] < q.shape[0]:
-            raise ValueError(f"out: {q.shape[0]} rows, got {tuple(out.shape)}")
-        _, out = _quant_attn(q, kv_layer, q_heads, kv_heads, head_dim, page_size, window, keep_first, softcap, sink, out,
+        out = _quant_attn(q, q.shape[0], kv_layer, q_heads, kv_heads, head_dim, page_size, window, keep_first, softcap, sink, out,
                              dict(gate=gate, bias=bias, chunked=chunked, sigmoid=sigmoid), page_indices, work)
         if work.shape[0] == 0 or q.shape[0] == 0:
             return out
