@@ -187,13 +187,6 @@ __device__ __forceinline__ uint32_t qd_transposed(uint32_t x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-// (x & mask) | bits
-template <uint32_t MASK, uint32_t BITS>
-__device__ __forceinline__ uint32_t qd_pick(uint32_t x) {
-  uint32_t y;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "r"(MASK), "r"(BITS));
-  return y;
-}
 __device__ __forceinline__ float qd_low(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float qd_high(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
@@ -552,10 +545,10 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
           for (int w = 0; w < W; ++w) {
             const int i = (w / WG) % N;
             const uint32_t a = ku[w], b = kv[w], ah = a >> 8, bh = b >> 8;
-            const uint32_t a0 = qd_pick<0x000f000fu, 0x64006400u>(a), a1 = qd_pick<0x000f000fu, 0x64006400u>(b);
-            const uint32_t a2 = qd_pick<0x00f000f0u, 0x54005400u>(a), a3 = qd_pick<0x00f000f0u, 0x54005400u>(b);
-            const uint32_t c0 = qd_pick<0x000f000fu, 0x64006400u>(ah), c1 = qd_pick<0x000f000fu, 0x64006400u>(bh);
-            const uint32_t c2 = qd_pick<0x00f000f0u, 0x54005400u>(ah), c3 = qd_pick<0x00f000f0u, 0x54005400u>(bh);
+            const uint32_t a0 = quant_kv_pick<0x000f000fu, 0x64006400u>(a), a1 = quant_kv_pick<0x000f000fu, 0x64006400u>(b);
+            const uint32_t a2 = quant_kv_pick<0x00f000f0u, 0x54005400u>(a), a3 = quant_kv_pick<0x00f000f0u, 0x54005400u>(b);
+            const uint32_t c0 = quant_kv_pick<0x000f000fu, 0x64006400u>(ah), c1 = quant_kv_pick<0x000f000fu, 0x64006400u>(bh);
+            const uint32_t c2 = quant_kv_pick<0x00f000f0u, 0x54005400u>(ah), c3 = quant_kv_pick<0x00f000f0u, 0x54005400u>(bh);
             if (w % WG == 0 && w / WG < N) qd_mma_f16(acc[i], a0, a1, a2, a3, qb[w][0], qb[w][1], qc[i][0], qc[i][1]);
             else qd_mma_f16_add(acc[i], a0, a1, a2, a3, qb[w][0], qb[w][1]);
             qd_mma_f16_add(acc[i], c0, c1, c2, c3, qb[w][2], qb[w][3]);
@@ -654,8 +647,8 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
           for (int i = 0; i < MT; ++i) {
             const int j = (i * 16 / GROUP) % N;
             const uint32_t v = vw[i], vh = v >> 8;
-            const uint32_t a0 = qd_pick<0x000f000fu, 0x64006400u>(v), a1 = qd_pick<0x00f000f0u, 0x54005400u>(v);
-            const uint32_t a2 = qd_pick<0x000f000fu, 0x64006400u>(vh), a3 = qd_pick<0x00f000f0u, 0x54005400u>(vh);
+            const uint32_t a0 = quant_kv_pick<0x000f000fu, 0x64006400u>(v), a1 = quant_kv_pick<0x00f000f0u, 0x54005400u>(v);
+            const uint32_t a2 = quant_kv_pick<0x000f000fu, 0x64006400u>(vh), a3 = quant_kv_pick<0x00f000f0u, 0x54005400u>(vh);
             qd_mma_f16_add(o[i], 0xe408e408u, 0xd480d480u, 0xe408e408u, 0xd480d480u, b0[j], b1[j]);  // -1032, -72
             qd_mma_f16_add(o[i], a0, a1, a2, a3, b0[j], b1[j]);
           }

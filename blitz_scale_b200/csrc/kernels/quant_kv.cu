@@ -3,157 +3,389 @@
 #include "ptx.cuh"
 #include "quant_kv.cuh"
 #include "scalar.cuh"
+#include "tmap.cuh"
 
 namespace blitz {
 
+// ------------------------------------------------------------------ rows in
 struct QuantStoreParams {
   const void *k, *v;  // [tokens][kv_heads * dim], pitches in elements
   int64_t k_row, v_row;
   const int32_t* slot;
   uint8_t* pool;
-  int64_t items;  // tokens * 2 * kv_heads * dim / 8
-  int kv_heads, page_size, max_pages;
+  int64_t units;  // (four rows, head) each
+  int tokens, kv_heads, page_shift, max_pages;
   int* status;
 };
 
-// Eight dimensions of a token a thread: the lanes of a group find its smallest and largest number together.
+// A warp takes four rows of one head, keys and values: D / 8 lanes a row, eight dimensions each; the lanes of a group find its smallest and
+// largest number together.  (Bound by the chain of a warp, loads, shuffles, stores: slots, keys and values are asked for at once.)  Keys go out as they are, a word a lane.  A word of the values holds four tokens of two dimensions: where the four
+// rows are the four tokens of a word (rows of a prompt) the lanes exchange their codes through shared memory and write words; else (the
+// tokens of a batch) every row writes its bytes.
 template <typename T, int D, int GROUP>
 __global__ void __launch_bounds__(256) quant_kv_store_kernel(const QuantStoreParams p) {
   constexpr QuantKv F = quant_kv(D, GROUP);
-  constexpr int LANES = D / 8;
+  constexpr int LANES = D / 8, ROWS = 32 / LANES;  // rows a warp takes at a time
+  __shared__ uint32_t s_codes[8][4 * LANES];
   ptx::griddep_launch_dependents();
   ptx::griddep_wait();
-  const int64_t it = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  const bool real = it < p.items;
-  const int l = static_cast<int>(it % LANES);
-  const int64_t rest = it / LANES;
-  const int head = static_cast<int>(rest % p.kv_heads);
-  const bool value = (rest / p.kv_heads) & 1;
-  const int64_t t = rest / (2 * p.kv_heads);
-  int s = real ? p.slot[t] : -1;
-  if (s >= 0 && s / p.page_size >= p.max_pages) {
+  const int lane = threadIdx.x & 31, l = lane % LANES;
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (unit >= p.units) return;
+  const int head = static_cast<int>(unit % p.kv_heads);
+  const int64_t t0 = unit / p.kv_heads * 4;
+  uint32_t* const codes = s_codes[threadIdx.x >> 5];
+  // the four slots: lane i has the i-th
+  int slots = lane < 4 && t0 + lane < p.tokens ? p.slot[t0 + lane] : -1;
+  uint4 raw[2][4 / ROWS];
+#pragma unroll
+  for (int r = 0; r < 4 / ROWS; ++r) {
+    const int64_t t = t0 + r * ROWS + lane / LANES, at = static_cast<int64_t>(head) * D + l * 8;
+    const bool real = t < p.tokens;
+    raw[0][r] = real ? *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.k) + t * p.k_row + at) : make_uint4(0, 0, 0, 0);
+    raw[1][r] = real ? *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.v) + t * p.v_row + at) : make_uint4(0, 0, 0, 0);
+  }
+  if (slots >= 0 && slots >> p.page_shift >= p.max_pages) {
     if (p.status) atomicCAS(p.status, 0, kStatusBadIndex);
-    s = -1;
+    slots = -1;
   }
-  float x[8];
+  const int s0 = __shfl_sync(0xffffffffu, slots, 0);
+  const bool quad = s0 >= 0 && (s0 & 3) == 0 && __all_sync(0xffffffffu, lane >= 4 || slots == s0 + lane);
+  auto block_of = [&](int s) {
+    const int page = s >> p.page_shift;
+    return p.pool + (((static_cast<int64_t>(page) * p.kv_heads + head) << (p.page_shift - 4)) + ((s - (page << p.page_shift)) >> 4)) * F.block;
+  };
+  auto rows = [&](auto plane) {
+    constexpr bool value = decltype(plane)::value;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = 0.f;
-  if (s >= 0)
-    ldf8<T>(reinterpret_cast<const T*>(value ? p.v : p.k) + t * (value ? p.v_row : p.k_row) + static_cast<int64_t>(head) * D + l * 8, x);
-  float lo = x[0], hi = x[0], bad = 0.f;
+    for (int r = 0; r < 4 / ROWS; ++r) {
+      const int s = __shfl_sync(0xffffffffu, slots, r * ROWS + lane / LANES);
+      // the smallest number and the negative of the largest, as a pair (NaN where there is one)
+      using T2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
+      auto pair = [](uint32_t u) { return *reinterpret_cast<T2*>(&u); };
+      auto bits = [](T2 v) { return *reinterpret_cast<uint32_t*>(&v); };
+      const uint4 u = raw[value][r];
+      uint32_t lo2 = bits(__hmin2_nan(__hmin2_nan(pair(u.x), pair(u.y)), __hmin2_nan(pair(u.z), pair(u.w))));
+      uint32_t hi2 = bits(__hmax2_nan(__hmax2_nan(pair(u.x), pair(u.y)), __hmax2_nan(pair(u.z), pair(u.w)))) ^ 0x80008000u;
+      uint32_t ends = bits(__hmin2_nan(pair(__byte_perm(lo2, hi2, 0x5410)), pair(__byte_perm(lo2, hi2, 0x7632))));
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    lo = fminf(lo, x[i]);
-    hi = fmaxf(hi, x[i]);
-    bad += x[i] * 0.f;  // NaN where a number is not finite
-  }
+      for (int d = 1; d < GROUP / 8; d <<= 1) ends = bits(__hmin2_nan(pair(ends), pair(__shfl_xor_sync(0xffffffffu, ends, d))));
+      const float2 end = cvt2<T>(ends);
+      __nv_bfloat16 z16 = __float2bfloat16_rd(end.x);
+      const float z = __bfloat162float(z16), range = -end.y - z;
+      // the smallest scale whose 15 steps cover the range: near range / 15, and then by what its product says
+      uint32_t sb = __bfloat16_as_ushort(__float2bfloat16_ru(range * (1.f / 15.f)));
+      if (fmaf(__uint_as_float(sb << 16), 15.f, -range) < 0.f) ++sb;
+      else if (sb > 0 && fmaf(__uint_as_float((sb - 1) << 16), 15.f, -range) >= 0.f) --sb;
+      if (!(range <= 3.4e38f)) {
+        z16 = __ushort_as_bfloat16(0x7fff);
+        sb = 0;
+      }
+      const __nv_bfloat16 s16 = __ushort_as_bfloat16(static_cast<unsigned short>(sb));
+      const float sc = __uint_as_float(sb << 16);
+      // rint((x - z) / s), between 0 and 15: by the reciprocal, whose error (2^-22 of the quotient) counts next to a tie only; those few are
+      // divided.  (A scale below 2^-120 has no reciprocal that serves: all are divided.)  Rounded by what is left of a mantissa.
+      uint32_t word = 0;
+      if (sc > 0.f) {
+        float x[8], c[8], near = 0.f;
+        unpack8<T>(u, x);
+        const float inv = ptx::rcp_approx(sc);
 #pragma unroll
-  for (int d = 1; d < GROUP / 8; d <<= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, d));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, d));
-    bad += __shfl_xor_sync(0xffffffffu, bad, d);
-  }
-  __nv_bfloat16 z16 = __float2bfloat16_rd(lo);
-  const float z = __bfloat162float(z16), range = hi - z + bad;
-  __nv_bfloat16 s16 = __float2bfloat16_ru(__fdiv_rn(range, 15.f));
-  if (!(range <= 3.4e38f)) {
-    z16 = __ushort_as_bfloat16(0x7fff);
-    s16 = __ushort_as_bfloat16(0);
-  }
-  const float sc = __bfloat162float(s16);
-  uint32_t word = 0;
-  if (sc > 0.f) {
+        for (int i = 0; i < 8; ++i) {
+          const float q = (x[i] - z) * inv;
+          c[i] = (q + 12582912.f) - 12582912.f;
+          near = fmaxf(near, fabsf(q - c[i]));
+        }
+        if (near > 0.4999f || sc < 7.6e-37f) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float c = fminf(fmaxf(rintf(__fdiv_rn(x[i] - z, sc)), 0.f), 15.f);
-      word |= static_cast<uint32_t>(c) << (4 * i);
+          for (int i = 0; i < 8; ++i) c[i] = rintf(__fdiv_rn(x[i] - z, sc));
+        }
+        // four codes are a number of 16 bits
+        const float low = fmaf(fmaf(fmaf(c[3], 16.f, c[2]), 16.f, c[1]), 16.f, c[0]) + 8388608.f;
+        const float high = fmaf(fmaf(fmaf(c[7], 16.f, c[6]), 16.f, c[5]), 16.f, c[4]) + 8388608.f;
+        word = __byte_perm(__float_as_uint(low), __float_as_uint(high), 0x5410);
+      }
+      const int tok = s & 15;  // (pages hold a multiple of 16 tokens)
+      uint8_t* const block = block_of(max(s, 0)) + (value ? F.part : 0);
+      if (!value) {
+        if (s >= 0) reinterpret_cast<uint32_t*>(block + tok * (D / 2))[(l & 3) * (D / 32) + (l >> 2)] = word;
+      } else if (quad) {
+        codes[(r * ROWS + lane / LANES) * LANES + l] = word;
+      } else {
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, word, 1);  // the eight dimensions beside these of a tile of 16
+        // nibble i of this half of the tile beside nibble i of the other: even lanes write the first four such bytes, odd ones the rest
+        const uint32_t low = l & 1 ? other : word, high = l & 1 ? word : other;
+        if (s >= 0) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int g = (l & 1) * 4 + i;
+            block[quant_kv_value_byte(tok, (l >> 1) * 16 + g)] = static_cast<uint8_t>(((low >> (4 * g)) & 15u) | (((high >> (4 * g)) & 15u) << 4));
+          }
+        }
+      }
+      if (l % (GROUP / 8) == 0 && s >= 0) {
+        __nv_bfloat16* w = reinterpret_cast<__nv_bfloat16*>(block + F.codes) + tok * 2 * F.groups + l / (GROUP / 8);
+        w[0] = s16;
+        w[F.groups] = z16;
+      }
     }
-  }
-  const uint32_t other = __shfl_xor_sync(0xffffffffu, word, 1);  // the eight dimensions beside these of a tile of 16
-  if (s < 0) return;
-  const int off = s % p.page_size, tok = off & 15;
-  uint8_t* block = p.pool + ((static_cast<int64_t>(s / p.page_size) * p.kv_heads + head) * (p.page_size >> 4) + (off >> 4)) * F.block;
-  if (value) block += F.part;
-  if (!value) {
-    reinterpret_cast<uint32_t*>(block + tok * (D / 2))[(l & 3) * (D / 32) + (l >> 2)] = word;
-  } else {
-    // nibble i of this half of the tile beside nibble i of the other: even lanes write the first four such bytes, odd ones the rest
-    const uint32_t low = l & 1 ? other : word, high = l & 1 ? word : other;
+    if (value && quad) {
+      __syncwarp();
+      // word (m / 4, g, quad, m % 4): bytes are tokens 0, 2, 1, 3, nibbles dimensions 16 m + g and 16 m + 8 + g
+      uint8_t* const block = block_of(s0) + F.part;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int g = (l & 1) * 4 + i;
-      block[quant_kv_value_byte(tok, (l >> 1) * 16 + g)] = static_cast<uint8_t>(((low >> (4 * g)) & 15u) | (((high >> (4 * g)) & 15u) << 4));
+      for (int i = lane; i < D / 2; i += 32) {
+        const int m = (i >> 5) * 4 + (i & 3), g = (i >> 2) & 7;
+        uint32_t word = 0;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const uint32_t* from = codes + ((b & 1) * 2 + (b >> 1)) * LANES + 2 * m;
+          word |= (((from[0] >> (4 * g)) & 15u) | (((from[1] >> (4 * g)) & 15u) << 4)) << (8 * b);
+        }
+        *reinterpret_cast<uint32_t*>(block + (i >> 5) * 512 + g * 64 + ((s0 & 15) >> 2) * 16 + (i & 3) * 4) = word;
+      }
     }
-  }
-  if (l % (GROUP / 8) == 0) {
-    __nv_bfloat16* w = reinterpret_cast<__nv_bfloat16*>(block + F.codes) + tok * 2 * F.groups + l / (GROUP / 8);
-    w[0] = s16;
-    w[F.groups] = z16;
-  }
+  };
+  rows(std::false_type{});
+  rows(std::true_type{});
 }
 
+// ------------------------------------------------------------------ rows back
 struct QuantLoadParams {
   const uint8_t* pool;
-  const int32_t* at;  // a slot per row, or a page per page_size rows
-  void *k, *v;        // row r of page n of the output at n * page_rows + r (slots: rows back to back)
-  int64_t items;      // rows * 2 * kv_heads * dim / 8
-  int kv_heads, page_size, page_rows, max_pages, whole_pages;
+  const int32_t* slot;
+  void *k, *v;    // row r of both
+  int64_t rows, units;  // (four rows, head) each
+  int kv_heads, page_shift, max_pages;
   int* status;
 };
 
-template <typename T>
-__device__ __forceinline__ float quant_kv_value(float z, float s, uint32_t c) {
-  // (a scale that was rounded up can carry the largest number of a group past the type's)
-  constexpr float most = std::is_same<T, __half>::value ? 65504.f : 3.3895313892515355e38f;
-  const float x = fmaf(s, static_cast<float>(c), z);
-  return fabsf(x) > most ? copysignf(most, x) : x;
-}
-
+// Rows of slots: a warp takes four of one head, as the store does.  Values of four tokens of a word come by words, through shared memory;
+// others byte by byte.
 template <typename T, int D, int GROUP>
 __global__ void __launch_bounds__(256) quant_kv_load_kernel(const QuantLoadParams p) {
   constexpr QuantKv F = quant_kv(D, GROUP);
-  constexpr int LANES = D / 8;
+  constexpr int LANES = D / 8, ROWS = 32 / LANES;
+  __shared__ __align__(16) T s_rows[8][4 * D];
   ptx::griddep_launch_dependents();
   ptx::griddep_wait();
-  const int64_t it = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (it >= p.items) return;
-  const int l = static_cast<int>(it % LANES);
-  const int64_t rest = it / LANES;
-  const int head = static_cast<int>(rest % p.kv_heads);
-  const bool value = (rest / p.kv_heads) & 1;
-  const int64_t r = rest / (2 * p.kv_heads);
-  int64_t page, to = r;
-  int off;
-  if (p.whole_pages) {
-    off = static_cast<int>(r % p.page_size);
-    page = p.at[r / p.page_size];
-    to = r / p.page_size * p.page_rows + off;
-  } else {
-    const int s = p.at[r];
-    if (s < 0) return;
-    page = s / p.page_size;
-    off = s % p.page_size;
-  }
-  if (page < 0 || page >= p.max_pages) {
+  const int lane = threadIdx.x & 31, l = lane % LANES;
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (unit >= p.units) return;
+  const int head = static_cast<int>(unit % p.kv_heads);
+  const int64_t t0 = unit / p.kv_heads * 4;
+  T* const rows = s_rows[threadIdx.x >> 5];
+  int slots = lane < 4 && t0 + lane < p.rows ? p.slot[t0 + lane] : -1;
+  if (slots >= 0 && slots >> p.page_shift >= p.max_pages) {
     if (p.status) atomicCAS(p.status, 0, kStatusBadIndex);
-    return;
+    slots = -1;
   }
-  const int tok = off & 15;
-  const uint8_t* block = p.pool + ((page * p.kv_heads + head) * (p.page_size >> 4) + (off >> 4)) * F.block;
-  if (value) block += F.part;
-  const __nv_bfloat16* w = reinterpret_cast<const __nv_bfloat16*>(block + F.codes) + tok * 2 * F.groups + l / (GROUP / 8);
-  const float s = __bfloat162float(w[0]), z = __bfloat162float(w[F.groups]);
-  float x[8];
-  if (!value) {
-    const uint32_t word = reinterpret_cast<const uint32_t*>(block + tok * (D / 2))[(l & 3) * (D / 32) + (l >> 2)];
+  const int s0 = __shfl_sync(0xffffffffu, slots, 0);
+  const bool quad = s0 >= 0 && (s0 & 3) == 0 && __all_sync(0xffffffffu, lane >= 4 || slots == s0 + lane);
+  auto block_of = [&](int s) {
+    const int page = s >> p.page_shift;
+    return p.pool + (((static_cast<int64_t>(page) * p.kv_heads + head) << (p.page_shift - 4)) + ((s - (page << p.page_shift)) >> 4)) * F.block;
+  };
+  auto scales = [&](const uint8_t* part, int tok) { return reinterpret_cast<const __nv_bfloat16*>(part + F.codes) + tok * 2 * F.groups; };
+  uint32_t word[4 / ROWS];
+  __nv_bfloat16 ks[4 / ROWS], kz[4 / ROWS], vs[4 / ROWS], vz[4 / ROWS];
+  uint32_t vw[4 / ROWS];  // of a row: eight codes; of a quad: words lane and lane + 32
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = quant_kv_value<T>(z, s, (word >> (4 * i)) & 15u);
-  } else {
+  for (int r = 0; r < 4 / ROWS; ++r) {
+    const int s = max(0, __shfl_sync(0xffffffffu, slots, r * ROWS + lane / LANES)), tok = s & 15, g = l / (GROUP / 8);
+    const uint8_t* block = block_of(s);
+    word[r] = reinterpret_cast<const uint32_t*>(block + tok * (D / 2))[(l & 3) * (D / 32) + (l >> 2)];
+    ks[r] = scales(block, tok)[g];
+    kz[r] = scales(block, tok)[F.groups + g];
+    vs[r] = scales(block + F.part, tok)[g];
+    vz[r] = scales(block + F.part, tok)[F.groups + g];
+    vw[r] = 0;
+    if (quad) {
+      const int i = lane + 32 * r;
+      if (i < D / 2) vw[r] = *reinterpret_cast<const uint32_t*>(block_of(s0) + F.part + (i >> 5) * 512 + ((i >> 2) & 7) * 64 + ((s0 & 15) >> 2) * 16 + (i & 3) * 4);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      x[i] = quant_kv_value<T>(z, s, (static_cast<uint32_t>(block[quant_kv_value_byte(tok, (l >> 1) * 16 + i)]) >> (4 * (l & 1))) & 15u);
+      for (int i = 0; i < 8; ++i)
+        vw[r] |= ((static_cast<uint32_t>(block[F.part + quant_kv_value_byte(tok, (l >> 1) * 16 + i)]) >> (4 * (l & 1))) & 15u) << (4 * i);
+    }
   }
-  stf8<T>(reinterpret_cast<T*>(value ? p.v : p.k) + (to * p.kv_heads + head) * D + l * 8, x);
+  if (quad) {  // codes as they are, in 16 bits a place, into rows
+#pragma unroll
+    for (int r = 0; r < 4 / ROWS; ++r) {
+      const int i = lane + 32 * r, d = (i >> 5) * 64 + (i & 3) * 16 + ((i >> 2) & 7);
+      if (i < D / 2) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const int tok = (b & 1) * 2 + (b >> 1);
+          reinterpret_cast<uint16_t*>(rows)[tok * D + d] = static_cast<uint16_t>((vw[r] >> (8 * b)) & 15u);
+          reinterpret_cast<uint16_t*>(rows)[tok * D + d + 8] = static_cast<uint16_t>((vw[r] >> (8 * b + 4)) & 15u);
+        }
+      }
+    }
+    __syncwarp();
+  }
+#pragma unroll
+  for (int r = 0; r < 4 / ROWS; ++r) {
+    const int row = r * ROWS + lane / LANES;
+    if (__shfl_sync(0xffffffffu, slots, row) < 0) continue;
+    const int64_t at = ((t0 + row) * p.kv_heads + head) * D + l * 8;
+    const float k_s = __bfloat162float(ks[r]), k_z = __bfloat162float(kz[r]), v_s = __bfloat162float(vs[r]), v_z = __bfloat162float(vz[r]);
+    float x[8], y[8];
+    quant_kv_codes(word[r], x);
+    const uint4 c4 = quad ? *reinterpret_cast<const uint4*>(rows + row * D + l * 8) : make_uint4(0, 0, 0, 0);
+    if (quad) {  // (one in 16 bits each)
+      const uint32_t c2[4] = {c4.x, c4.y, c4.z, c4.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = __uint_as_float(0x4b000000u | (i & 1 ? c2[i >> 1] >> 16 : c2[i >> 1] & 15u)) - 8388608.f;
+    } else {
+      quant_kv_codes(vw[r], y);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x[i] = fmaf(k_s, x[i], k_z);
+      y[i] = fmaf(v_s, y[i], v_z);
+    }
+    constexpr float most = quant_kv_most<T>();
+    if (quant_kv_past(k_s, k_z, most) || quant_kv_past(v_s, v_z, most)) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[i] = quant_kv_cut(x[i], most);
+        y[i] = quant_kv_cut(y[i], most);
+      }
+    }
+    stf8<T>(reinterpret_cast<T*>(p.k) + at, x);
+    stf8<T>(reinterpret_cast<T*>(p.v) + at, y);
+  }
+}
+
+// ------------------------------------------------------------------ pages back
+struct QuantPagesParams {
+  const uint8_t* pool;
+  const int32_t* pages;
+  void *k, *v;       // page n's token `off` at row n * page_rows + off
+  int64_t units;     // (page, 16 tokens of it, head) each
+  int kv_heads, page_size, page_rows, max_pages;
+  int* status;
+};
+
+// The codes of a warp's 16 tokens of a head, 8 x 8 blocks of (token, dimension) at a time as tensor-core fragments have them.
+__device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+// A warp takes 16 tokens of a head.  Keys: four lanes a token, 32 codes each.  Values: a lane has four tokens of eight dimensions 8 apart, which
+// stmatrix turns into rows of a token.  Both go out from shared memory, whole rows at a time.
+// Bound by the 16-bit rows that it writes (four times the codes).
+template <typename T, int D, int GROUP>
+__global__ void __launch_bounds__(256, 3) quant_kv_pages_kernel(const QuantPagesParams p) {
+  constexpr QuantKv F = quant_kv(D, GROUP);
+  constexpr int W = D / 32, G = F.groups;
+  // bytes from row to row in shared memory: pairs of rows in different halves of the banks (keys: 64 bytes of each a time), rows 4 banks on
+  // (values: 16 bytes of eight a time)
+  constexpr int KROW = D * 2 + 64, ROW = D * 2 + 16;
+  __shared__ __align__(16) uint8_t s_rows[8][16 * KROW];
+  ptx::griddep_launch_dependents();
+  ptx::griddep_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+  uint8_t* const rows = s_rows[warp];
+  const int blocks = p.page_size >> 4;
+  for (int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + warp; unit < p.units; unit += static_cast<int64_t>(gridDim.x) * 8) {
+    const int head = static_cast<int>(unit % p.kv_heads), b = static_cast<int>(unit / p.kv_heads % blocks);
+    const int64_t n = unit / p.kv_heads / blocks;
+    const int page = p.pages[n];
+    if (page < 0 || page >= p.max_pages) {
+      if (p.status && lane == 0) atomicCAS(p.status, 0, kStatusBadIndex);
+      continue;
+    }
+    const uint8_t* block = p.pool + ((static_cast<int64_t>(page) * p.kv_heads + head) * blocks + b) * F.block;
+    const int64_t row0 = n * p.page_rows + b * 16, pitch = static_cast<int64_t>(p.kv_heads) * D;
+    // everything is asked for before anything is used
+    uint32_t kw[2][W], vw[D / 16];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const uint8_t* at = block + (g + 8 * r) * (D / 2) + t4 * (D / 8);
+      if (W == 4) {
+        const uint4 x = *reinterpret_cast<const uint4*>(at);
+        kw[r][0] = x.x; kw[r][1] = x.y; kw[r][2 % W] = x.z; kw[r][3 % W] = x.w;
+      } else {
+        const uint2 x = *reinterpret_cast<const uint2*>(at);
+        kw[r][0] = x.x; kw[r][1] = x.y;
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < D / 64; ++h) {
+      const uint4 x = *reinterpret_cast<const uint4*>(block + F.part + h * 512 + lane * 16);
+      vw[4 * h] = x.x; vw[4 * h + 1] = x.y; vw[4 * h + 2] = x.z; vw[4 * h + 3] = x.w;
+    }
+    // a token's scales and offsets, 2 G numbers of 16 bits
+    uint32_t ks[2][G], vs[4][G];
+    auto numbers = [&](const uint8_t* at, uint32_t (&to)[G]) {
+      if (G == 4) {
+        const uint4 x = *reinterpret_cast<const uint4*>(at);
+        to[0] = x.x; to[1 % G] = x.y; to[2 % G] = x.z; to[3 % G] = x.w;
+      } else if (G == 2) {
+        const uint2 x = *reinterpret_cast<const uint2*>(at);
+        to[0] = x.x; to[1 % G] = x.y;
+      } else {
+        to[0] = *reinterpret_cast<const uint32_t*>(at);
+      }
+    };
+    auto number = [](const uint32_t (&from)[G], int i) { return __uint_as_float(i & 1 ? from[i >> 1] & 0xffff0000u : from[i >> 1] << 16); };
+#pragma unroll
+    for (int r = 0; r < 2; ++r) numbers(block + F.codes + (g + 8 * r) * 4 * G, ks[r]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) numbers(block + F.part + F.codes + (4 * t4 + j) * 4 * G, vs[j]);
+    constexpr float most = quant_kv_most<T>();
+    bool past = false;
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) past |= quant_kv_past(number(ks[r], i), number(ks[r], G + i), most);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) past |= quant_kv_past(number(vs[j], i), number(vs[j], G + i), most);
+    }
+    auto out = [&](void* to, int row_bytes) {
+      T* const d = reinterpret_cast<T*>(to) + row0 * pitch + static_cast<int64_t>(head) * D;
+      __syncwarp();
+#pragma unroll
+      for (int i = lane; i < 16 * D / 8; i += 32)
+        *reinterpret_cast<uint4*>(d + (i / (D / 8)) * pitch + (i % (D / 8)) * 8) = *reinterpret_cast<const uint4*>(rows + (i / (D / 8)) * row_bytes + (i % (D / 8)) * 16);
+      __syncwarp();
+    };
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        float x[8];
+        quant_kv_codes(kw[r][w], x);
+        const float sc = number(ks[r], w * 32 / GROUP), z = number(ks[r], G + w * 32 / GROUP);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = fmaf(sc, x[i], z);
+        if (past) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = quant_kv_cut(x[i], most);
+        }
+        stf8<T>(reinterpret_cast<T*>(rows + (g + 8 * r) * KROW) + 32 * w + 8 * t4, x);
+      }
+    out(p.k, KROW);
+#pragma unroll
+    for (int m = 0; m < D / 16; ++m) {
+      const int i = m * 16 / GROUP;
+      // nibbles of a word: (token 0, dimension g), (0, g + 8), (2, g), (2, g + 8), and tokens 1 and 3 in the upper half
+      float x[8];
+      quant_kv_codes(vw[m], x);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = fmaf(number(vs[(j & 2) + (j >> 2)], i), x[j], number(vs[(j & 2) + (j >> 2)], G + i));
+      if (past) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = quant_kv_cut(x[j], most);
+      }
+      // 8 x 8 blocks: dimensions 16 m + g by (tokens 4 t4, + 1), 16 m + 8 + g by the same, and both by (4 t4 + 2, + 3).  Lane i gives the address of
+      // row i % 8 of block i / 8: its token (columns 2 t4, 2 t4 + 1 of a block are tokens 4 t4 (+ 2), + 1), eight dimensions.
+      const int mat = lane >> 3, c = lane & 7, token = 4 * (c >> 1) + (c & 1) + (mat >> 1) * 2;
+      stmatrix_x4_trans(ptx::smem_u32(rows + token * ROW + m * 32 + (mat & 1) * 16), pk2<T>(x[0], x[4]), pk2<T>(x[1], x[5]), pk2<T>(x[2], x[6]), pk2<T>(x[3], x[7]));
+    }
+    out(p.v, ROW);
+  }
 }
 
 struct StoreLaunch {
@@ -161,7 +393,7 @@ struct StoreLaunch {
   cudaStream_t stream;
   template <typename T, int D, int GROUP>
   int operator()() const {
-    return (int)launch_pdl(quant_kv_store_kernel<T, D, GROUP>, dim3((unsigned)((p.items + 255) / 256)), dim3(256), 0, stream, p);
+    return (int)launch_pdl(quant_kv_store_kernel<T, D, GROUP>, dim3((unsigned)((p.units + 7) / 8)), dim3(256), 0, stream, p);
   }
 };
 struct LoadLaunch {
@@ -169,7 +401,16 @@ struct LoadLaunch {
   cudaStream_t stream;
   template <typename T, int D, int GROUP>
   int operator()() const {
-    return (int)launch_pdl(quant_kv_load_kernel<T, D, GROUP>, dim3((unsigned)((p.items + 255) / 256)), dim3(256), 0, stream, p);
+    return (int)launch_pdl(quant_kv_load_kernel<T, D, GROUP>, dim3((unsigned)((p.units + 7) / 8)), dim3(256), 0, stream, p);
+  }
+};
+struct PagesLaunch {
+  const QuantPagesParams& p;
+  cudaStream_t stream;
+  template <typename T, int D, int GROUP>
+  int operator()() const {
+    const int64_t blocks = (p.units + 7) / 8, most = (int64_t)device_sm_count() * 16;
+    return (int)launch_pdl(quant_kv_pages_kernel<T, D, GROUP>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, stream, p);
   }
 };
 
@@ -179,27 +420,36 @@ extern "C" {
 using namespace blitz;
 
 // k, v: [num_tokens] rows of kv_heads * dim elements, pitches k_row and v_row (multiples of 8, 16-byte aligned).  slot[t] = page *
-// page_size + offset, negative: the row is not written.  The same slot twice: either row's bytes.
+// page_size + offset, negative: the row is not written.  The same slot twice: some of both rows' bytes.
 int blitz_quant_kv_store(const void* k, int64_t k_row, const void* v, int64_t v_row, const int32_t* slot, void* pool, int num_tokens,
                          int kv_heads, int dim, int group, int page_size, int max_pages, int* status, int dtype, cudaStream_t stream) {
   if (num_tokens <= 0) return 0;
   if (!quant_kv_supported(dim, group, page_size) || kv_heads < 1 || ((k_row | v_row) & 7)) return -1;
   if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(pool)) & 15) return -1;
-  QuantStoreParams p{k, v, k_row, v_row, slot, (uint8_t*)pool, (int64_t)num_tokens * 2 * kv_heads * (dim / 8), kv_heads, page_size, max_pages, status};
-  if (p.items > (int64_t)256 * 0x7fffffff) return -1;
+  QuantStoreParams p{k, v, k_row, v_row, slot, (uint8_t*)pool, ((int64_t)num_tokens + 3) / 4 * kv_heads, num_tokens, kv_heads, quant_kv_shift(page_size), max_pages, status};
+  if (p.units > (int64_t)8 * 0x7fffffff) return -1;
   return quant_kv_dispatch(dtype, dim, group, StoreLaunch{p, stream});
 }
 
-// Rows back in 16 bits.  whole_pages = 0: at[r] is a slot (negative: row r is left as it is), row r goes to row r of k and v; else at[n] is a
-// page, whose tokens go to rows n * page_rows .. of k and v.  `count`: entries of at.
-int blitz_quant_kv_load(const void* pool, const int32_t* at, int64_t count, int whole_pages, void* k, void* v, int kv_heads, int dim, int group,
-                        int page_size, int page_rows, int max_pages, int* status, int dtype, cudaStream_t stream) {
-  if (count <= 0) return 0;
+// Row slot[r] to row r of k and v, in 16 bits (a negative slot: row r is left as it is).
+int blitz_quant_kv_load(const void* pool, const int32_t* slot, int64_t rows, void* k, void* v, int kv_heads, int dim, int group, int page_size,
+                        int max_pages, int* status, int dtype, cudaStream_t stream) {
+  if (rows <= 0) return 0;
   if (!quant_kv_supported(dim, group, page_size) || kv_heads < 1) return -1;
   if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(pool)) & 15) return -1;
-  QuantLoadParams p{(const uint8_t*)pool, at, k, v, count * (whole_pages ? page_size : 1) * 2 * kv_heads * (dim / 8), kv_heads, page_size, page_rows, max_pages, whole_pages, status};
-  if (p.items > (int64_t)256 * 0x7fffffff) return -1;
+  QuantLoadParams p{(const uint8_t*)pool, slot, k, v, rows, (rows + 3) / 4 * kv_heads, kv_heads, quant_kv_shift(page_size), max_pages, status};
+  if (p.units > (int64_t)8 * 0x7fffffff) return -1;
   return quant_kv_dispatch(dtype, dim, group, LoadLaunch{p, stream});
+}
+
+// Page pages[n], in 16 bits, to rows n * page_rows .. of k and v (each row kv_heads * dim).
+int blitz_quant_kv_pages(const void* pool, const int32_t* pages, int64_t count, void* k, void* v, int kv_heads, int dim, int group, int page_size,
+                         int page_rows, int max_pages, int* status, int dtype, cudaStream_t stream) {
+  if (count <= 0) return 0;
+  if (!quant_kv_supported(dim, group, page_size) || kv_heads < 1 || page_rows < page_size) return -1;
+  if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(pool)) & 15) return -1;
+  QuantPagesParams p{(const uint8_t*)pool, pages, k, v, count * kv_heads * (page_size / 16), kv_heads, page_size, page_rows, max_pages, status};
+  return quant_kv_dispatch(dtype, dim, group, PagesLaunch{p, stream});
 }
 
 }  // extern "C"

@@ -31,10 +31,40 @@ inline bool quant_kv_supported(int dim, int group, int page_size) {
   return (dim == 64 || dim == 128) && (group == 32 || group == 64 || group == 128) && group <= dim && page_size >= 16 &&
          page_size <= (1 << 20) && (page_size & (page_size - 1)) == 0;
 }
+inline int quant_kv_shift(int page_size) {
+  int n = 0;
+  while ((1 << n) < page_size) ++n;
+  return n;
+}
 // Byte of the values' codes that holds token t (of 16) of dimension d; the nibble is d / 8 % 2.
 __host__ __device__ constexpr int quant_kv_value_byte(int t, int d) {
   return (d >> 6) * 512 + (d & 7) * 64 + (t >> 2) * 16 + ((d >> 4) & 3) * 4 + (t & 1) * 2 + ((t >> 1) & 1);
 }
+
+// (x & MASK) | BITS
+template <uint32_t MASK, uint32_t BITS>
+__device__ __forceinline__ uint32_t quant_kv_pick(uint32_t x) {
+  uint32_t y;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "r"(MASK), "r"(BITS));
+  return y;
+}
+// The eight codes of a word, low nibbles first, as numbers: a nibble within the mantissa of a power of two that makes its lowest bit one.
+__device__ __forceinline__ void quant_kv_codes(uint32_t w, float (&c)[8]) {
+  const uint32_t v = w >> 12;  // nibbles 5 .. 7 where 2 .. 4 are
+  c[0] = __uint_as_float(quant_kv_pick<0x0000fu, 0x4b000000u>(w)) - 8388608.f;
+  c[1] = __uint_as_float(quant_kv_pick<0x000f0u, 0x49000000u>(w)) - 524288.f;
+  c[2] = __uint_as_float(quant_kv_pick<0x00f00u, 0x47000000u>(w)) - 32768.f;
+  c[3] = __uint_as_float(quant_kv_pick<0x0f000u, 0x45000000u>(w)) - 2048.f;
+  c[4] = __uint_as_float(quant_kv_pick<0xf0000u, 0x43000000u>(w)) - 128.f;
+  c[5] = __uint_as_float(quant_kv_pick<0x00f00u, 0x47000000u>(v)) - 32768.f;
+  c[6] = __uint_as_float(quant_kv_pick<0x0f000u, 0x45000000u>(v)) - 2048.f;
+  c[7] = __uint_as_float(quant_kv_pick<0xf0000u, 0x43000000u>(v)) - 128.f;
+}
+// The largest finite number of a type.  A scale that was rounded up can carry the largest number of a group past it: such groups are cut.
+template <typename T>
+__device__ __forceinline__ constexpr float quant_kv_most() { return std::is_same<T, __half>::value ? 65504.f : 3.3895313892515355e38f; }
+__device__ __forceinline__ bool quant_kv_past(float s, float z, float most) { return fmaxf(fabsf(z), fabsf(fmaf(15.f, s, z))) > most; }
+__device__ __forceinline__ float quant_kv_cut(float x, float most) { return fabsf(x) > most ? copysignf(most, x) : x; }
 
 // Calls f with the element type and the sizes as types and constants.
 template <typename F>

@@ -529,8 +529,8 @@ def quant_kv_load(cache: QuantKV, slot: torch.Tensor, *, dtype: torch.dtype = to
         if t.shape != (n, H, D) or not t.is_contiguous() or t.dtype != k.dtype or t.data_ptr() & 15:
             raise ValueError(f"k and v: contiguous {(n, H, D)} of one type, got {tuple(t.shape)} {t.dtype}")
     _quant(cache, slot, k, v)
-    rc = lib().blitz_quant_kv_load(pool.data_ptr(), slot.data_ptr(), n, 0, k.data_ptr(), v.data_ptr(), H, D, group, 16 * blocks, 0, pages, _status_ptr(pool),
-                                   _dt(k), _stream())
+    rc = lib().blitz_quant_kv_load(pool.data_ptr(), slot.data_ptr(), n, k.data_ptr(), v.data_ptr(), H, D, group, 16 * blocks, pages, _status_ptr(pool), _dt(k),
+                                   _stream())
     if rc:
         _check(rc, "blitz_quant_kv_load")
     return k, v
@@ -538,15 +538,20 @@ def quant_kv_load(cache: QuantKV, slot: torch.Tensor, *, dtype: torch.dtype = to
 
 def quant_kv_pages(cache: QuantKV, pages: torch.Tensor, *, dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Whole pages of a 4-bit cache in the layout of a 16-bit one, [len(pages), 2, page, kv_heads, dim], rounded to 16 bits."""
+    pool, D, group = cache
     _int32(pages, None, "pages")
-    ps = cache.page_size
-    shape = (pages.numel(), 2, ps, cache.pool.shape[1], cache.dim)
-    out = torch.empty(shape, dtype=dtype, device=cache.pool.device) if out is None else out
-    if out.shape != shape or not out.is_contiguous() or out.data_ptr() % 16:
+    n, (count, H, blocks, _) = pages.shape[0], pool.shape
+    shape = (n, 2, 16 * blocks, H, D)
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=pool.device)
+    elif out.shape != shape or not out.is_contiguous() or out.data_ptr() & 15:
         raise ValueError(f"out: contiguous {shape}, got {tuple(out.shape)}")
-    pool = _quant(cache, pages, out)
-    _check(lib().blitz_quant_kv_load(_p(pool), _p(pages), pages.numel(), 1, _p(out), _p(out) + out.stride(1) * out.element_size(), pool.shape[1],
-                                     cache.dim, cache.group, ps, 2 * ps, pool.shape[0], _status_ptr(pool), _dt(out), _stream()), "blitz_quant_kv_load")
+    _quant(cache, pages, out)
+    at = out.data_ptr()
+    rc = lib().blitz_quant_kv_pages(pool.data_ptr(), pages.data_ptr(), n, at, at + 32 * blocks * H * D, H, D, group, 16 * blocks, 32 * blocks, count,
+                                    _status_ptr(pool), _dt(out), _stream())
+    if rc:
+        _check(rc, "blitz_quant_kv_pages")
     return out
 
 
