@@ -50,6 +50,10 @@
 // neighbours share a reciprocal, 1 / a = b (c d) / (a b c d), unless a product of some four leaves the range of fp32 (one vote per
 // half a block).
 //
+// Operands in fp16 for a bf16 model (IO: the type of sink and output): queries, keys and values were divided by powers of two (a row's of a
+// head, a KV head's) so that fp16 holds them, which a row's scale and its output's factor make up for; a 4-bit cache read back for a
+// pass comes so (quant_kv.cu).
+//
 // Replaces FlashInfer's BatchPrefillWithRaggedKVCacheWrapper / paged wrapper calls and their host Plan()
 // (src/kernel/attention_prefill.cu:11-45, src/kernel/flashinfer_types.cu:24-49).
 #include "launch.cuh"
@@ -81,6 +85,7 @@ struct PagedPrefillParams {
   const void* sink;           // EXT: [q_heads] in the activation type, or null
   const void* bias;           // BIAS: [q_heads][bias_len] in the activation type (SIG: [q_heads], or null)
   int bias_len;
+  const float *q_up, *kv_up;  // IO: powers of two taken out of queries [tokens][q_heads], and of keys and values [2][kv_heads]
   int* status;
   long long* trace;  // profiling aid (null in production): clock stamps of CTA 0's first item, see the set_trace call
 };
@@ -145,11 +150,12 @@ __device__ __forceinline__ int pp_index(int r, int total) {
   return idx < total ? idx : -1;
 }
 
-template <typename T, int HD, int VD, bool POLY, bool EXT, bool BIAS, bool SIG>
+template <typename T, int HD, int VD, bool POLY, bool EXT, bool BIAS, bool SIG, typename IO = T>
 __global__ void __launch_bounds__(kPpThreads, 1)
 attn_prefill_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                           const __grid_constant__ CUtensorMap tmap_v, const PagedPrefillParams p) {
   using C = PpCfg<HD, VD>;
+  constexpr bool SCALED = !std::is_same<T, IO>::value;
   constexpr int TB = C::kTileBytes, VB = C::kValueBytes, SB = C::kSlabBytes;
   constexpr uint32_t kFmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
   constexpr uint32_t kIdescS = ptx::make_idesc_f16(kFmt, 0u, 0u, 128, 128);
@@ -374,6 +380,10 @@ attn_prefill_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
       const int limit = it.prefix + q_idx;         // last key position this row may see
       const int chunk_from = EXT && p.chunked ? limit - limit % p.window : -1;  // first key of the row's chunk
       float m_ref = 0.f, l = 0.f;
+      float row_up = 1.f;
+      if constexpr (SCALED) row_up = q_idx < it.q_len ? p.q_up[static_cast<int64_t>(it.seq_start + q_idx) * p.q_heads + it.head] * p.kv_up[it.kv_head] : 0.f;
+      auto scale_log2 = [&]() { return SCALED ? p.scale_log2 * row_up : p.scale_log2; };
+      auto cap_scale = [&]() { return SCALED ? p.cap_scale * row_up : p.cap_scale; };
       const float sig_bias = SIG && p.bias ? -1.4426950408889634f * to_f<T>(reinterpret_cast<const T*>(p.bias)[it.head]) : 0.f;
       const T* bias_row = BIAS ? reinterpret_cast<const T*>(p.bias) + static_cast<int64_t>(it.head) * p.bias_len : nullptr;
       const float far_bias = BIAS ? to_f<T>(bias_row[p.bias_len - 1]) * 1.4426950408889634f : 0.f;
@@ -481,11 +491,11 @@ attn_prefill_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
           // distance of key i to this row: nearest + r_ + 127 - i
 #pragma unroll
           for (int i = 0; i < kPpTile; ++i)
-            score(i) = __float_as_uint(fmaf(__uint_as_float(score(i)), p.scale_log2, sb[r_ + kPpTile - 1 - i]));
+            score(i) = __float_as_uint(fmaf(__uint_as_float(score(i)), scale_log2(), sb[r_ + kPpTile - 1 - i]));
         } else if (BIAS) {
           bias = far_bias;
         }
-        const float score_scale = near ? 1.f : p.scale_log2;
+        const float score_scale = near ? 1.f : scale_log2();
         // largest of the row's 128 scores, or of their magnitudes: eight independent chains of three-input maxima (with two
         // softmax warps per scheduler nothing else hides a serial one)
         auto largest = [&](auto&& max3) {
@@ -509,7 +519,7 @@ attn_prefill_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
           small = __all_sync(0xffffffffu, mx <= p.small_max);
         }
         if (small) {
-          mx *= p.scale_log2;  // |cap tanh(x / cap)| <= |x|
+          mx *= scale_log2();  // |cap tanh(x / cap)| <= |x|
         } else {
           if (masked) {
 #pragma unroll
@@ -517,8 +527,8 @@ attn_prefill_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
               if (!visible(i)) score(i) = 0xff800000u;  // -inf
           }
           mx = largest([](float a, float b, float c) { return ptx::fmax3(a, b, c); });
-          if (capped) mx = mx == -INFINITY ? mx : p.cap_log2 * ptx::tanh_ex2(mx * p.cap_scale);
-          else mx = BIAS ? fmaf(mx, score_scale, bias) : mx * p.scale_log2;
+          if (capped) mx = mx == -INFINITY ? mx : p.cap_log2 * ptx::tanh_ex2(mx * cap_scale());
+          else mx = BIAS ? fmaf(mx, score_scale, bias) : mx * scale_log2();
         }
         // (S of this block was issued after P V of the previous one, so that product is complete: O_t is stable and
         // the columns P is about to overwrite have been read)
@@ -583,12 +593,12 @@ attn_prefill_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
             probabilities(poly);
           }
         } else if (capped) {
-          auto cap = [&](float x) { return x == -INFINITY ? x : fmaf(ptx::tanh_ex2(x * p.cap_scale), p.cap_log2, neg_m); };
+          auto cap = [&](float x) { return x == -INFINITY ? x : fmaf(ptx::tanh_ex2(x * cap_scale()), p.cap_log2, neg_m); };
           probabilities([&](int c) { return make_float2(cap(__uint_as_float(score(c))), cap(__uint_as_float(score(c + 1)))); });
         } else {
           probabilities([&](int c) {
-            return make_float2(fmaf(__uint_as_float(score(c)), BIAS ? score_scale : p.scale_log2, neg_m),
-                               fmaf(__uint_as_float(score(c + 1)), BIAS ? score_scale : p.scale_log2, neg_m));
+            return make_float2(fmaf(__uint_as_float(score(c)), BIAS ? score_scale : scale_log2(), neg_m),
+                               fmaf(__uint_as_float(score(c + 1)), BIAS ? score_scale : scale_log2(), neg_m));
           });
         }
         pp_trace(p, tracer, t, j, 4);
@@ -603,13 +613,14 @@ attn_prefill_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
       cnt += my_blocks;
       ptx::tc_fence_after_sync();
       if (EXT && p.sink != nullptr && l > 0.f)
-        l += ptx::ex2_approx(to_f<T>(reinterpret_cast<const T*>(p.sink)[it.head]) * 1.4426950408889634f - m_ref);
+        l += ptx::ex2_approx(to_f<IO>(reinterpret_cast<const IO*>(p.sink)[it.head]) * 1.4426950408889634f - m_ref);
       float inv = l > 0.f ? 1.f / l : 0.f;
+      if constexpr (SCALED) inv *= p.kv_up[p.kv_heads + it.kv_head];
       if (p.gate != nullptr && q_idx < it.q_len) {
         const T z = reinterpret_cast<const T*>(p.gate)[static_cast<int64_t>(it.seq_start + q_idx) * p.gate_stride + it.head];
         inv /= 1.f + expf(-to_f<T>(z));
       }
-      T* dst = reinterpret_cast<T*>(p.out) + static_cast<int64_t>(it.seq_start + q_idx) * p.out_stride + it.head * p.vdim;
+      IO* dst = reinterpret_cast<IO*>(p.out) + static_cast<int64_t>(it.seq_start + q_idx) * p.out_stride + it.head * p.vdim;
 #pragma unroll 1
       for (int c = 0; c < VD; c += 32) {
         uint32_t o[32];
@@ -623,10 +634,10 @@ attn_prefill_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
             if (c + i < p.vdim) *reinterpret_cast<uint4*>(dst + c + i) = make_uint4(
-                pk2<T>(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv),
-                pk2<T>(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv),
-                pk2<T>(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv),
-                pk2<T>(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv));
+                pk2<IO>(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv),
+                pk2<IO>(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv),
+                pk2<IO>(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv),
+                pk2<IO>(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv));
           }
         }
       }
@@ -642,15 +653,15 @@ attn_prefill_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
   }
 }
 
-template <typename T, int HD, int VD, bool POLY, bool EXT, bool BIAS, bool SIG>
+template <typename T, int HD, int VD, bool POLY, bool EXT, bool BIAS, bool SIG, typename IO = T>
 static int launch_paged_prefill(const CUtensorMap (&tm)[3], const PagedPrefillParams& p, int grid, cudaStream_t stream) {
   constexpr int kSmem = PpCfg<HD, VD>::kSmemBytes + (BIAS ? PpCfg<HD, VD>::kBiasFloats * 4 : 0);
   static PerDeviceOnce once;
   cudaError_t e = once.run([] {
-    return cudaFuncSetAttribute(attn_prefill_paged_kernel<T, HD, VD, POLY, EXT, BIAS, SIG>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    return cudaFuncSetAttribute(attn_prefill_paged_kernel<T, HD, VD, POLY, EXT, BIAS, SIG, IO>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   });
   if (e != cudaSuccess) return (int)e;
-  return (int)launch_pdl(attn_prefill_paged_kernel<T, HD, VD, POLY, EXT, BIAS, SIG>, dim3(grid), dim3(kPpThreads), (size_t)kSmem, stream, tm[0], tm[1], tm[2], p);
+  return (int)launch_pdl(attn_prefill_paged_kernel<T, HD, VD, POLY, EXT, BIAS, SIG, IO>, dim3(grid), dim3(kPpThreads), (size_t)kSmem, stream, tm[0], tm[1], tm[2], p);
 }
 
 static long long* g_pp_trace = nullptr;
@@ -675,11 +686,12 @@ void blitz_attn_prefill_paged_set_trace(long long* buf) { blitz::g_pp_trace = bu
 // exponentials on the FMA pipe (not with a window, cap or sink).  window (0 = none) / keep_first, softcap (0 = none), sink
 // and gate (null = none), chunked and sigmoid: see the top of the file.  bias: [q_heads][bias_len] in the activation type, or null
 // (not with a window, cap or sink; with sigmoid weights only bias_len 1).
-int blitz_attn_prefill_paged(const void* q, int64_t q_stride, const void* k_pool, const void* v_pool, void* out, int64_t out_stride,
+static int prefill_paged(const void* q, int64_t q_stride, const void* k_pool, const void* v_pool, void* out, int64_t out_stride,
                              const int32_t* page_indices, const int32_t* work, int entries, int num_tokens,
                              int q_heads, int kv_heads, int dim, int vdim, int page_size, int page_rows, int max_pages,
                              float sm_scale, int flags, int window, int keep_first, int chunked, int sigmoid, float softcap, const void* sink,
-                             const void* bias, int bias_len, const void* gate, int64_t gate_stride, int* status, int dtype, cudaStream_t stream) {
+                             const void* bias, int bias_len, const void* gate, int64_t gate_stride, const float* q_up, const float* kv_up, int* status,
+                             int dtype, cudaStream_t stream) {
   if (num_tokens <= 0 || entries <= 0) return 0;
   if (dim < 8 || dim > 128 || (dim & 7) || vdim < 8 || vdim > 128 || (vdim & 7)) return -1;
   if (kv_heads < 1 || (q_heads % kv_heads) != 0 || (out_stride & 7) || (q_stride & 7)) return -1;
@@ -703,7 +715,7 @@ int blitz_attn_prefill_paged(const void* q, int64_t q_stride, const void* k_pool
   p.q_heads = q_heads; p.kv_heads = kv_heads; p.page_size = page_size; p.box_tokens = bt;
   p.oob_row = (int)rows;
   p.scale_log2 = sm_scale * 1.4426950408889634f; p.status = status; p.trace = g_pp_trace;
-  p.chunked = chunked;
+  p.chunked = chunked; p.q_up = q_up; p.kv_up = kv_up;
   p.window = window; p.keep_first = keep_first; p.sink = sink; p.bias = bias; p.bias_len = bias_len;
   p.cap_scale = softcap > 0.f ? sm_scale / softcap : 0.f; p.cap_log2 = softcap * 1.4426950408889634f;
   // tanh(z) = z (k0 + k1 z^2 + k2 z^4 + k3 z^6) for |z| <= 0.5 (Chebyshev interpolation of tanh(z) / z in z^2, absolute
@@ -736,7 +748,38 @@ int blitz_attn_prefill_paged(const void* q, int64_t q_stride, const void* k_pool
     if (poly) return sized(type, yes, no, no, no);
     return sized(type, no, no, no, no);
   };
+  if (q_up != nullptr) {
+    if (dim != vdim || (dim != 64 && dim != 128)) return -1;
+    auto scaled = [&](auto ext_) {
+      constexpr bool X = decltype(ext_)::value;
+      return dim > 64 ? launch_paged_prefill<__half, 128, 128, false, X, false, false, __nv_bfloat16>(tm, p, grid, stream)
+                      : launch_paged_prefill<__half, 64, 64, false, X, false, false, __nv_bfloat16>(tm, p, grid, stream);
+    };
+    return ext ? scaled(std::true_type{}) : scaled(std::false_type{});
+  }
   return dtype == 1 ? launch(__nv_bfloat16{}) : launch(__half{});
+}
+
+int blitz_attn_prefill_paged(const void* q, int64_t q_stride, const void* k_pool, const void* v_pool, void* out, int64_t out_stride,
+                             const int32_t* page_indices, const int32_t* work, int entries, int num_tokens,
+                             int q_heads, int kv_heads, int dim, int vdim, int page_size, int page_rows, int max_pages,
+                             float sm_scale, int flags, int window, int keep_first, int chunked, int sigmoid, float softcap, const void* sink,
+                             const void* bias, int bias_len, const void* gate, int64_t gate_stride, int* status, int dtype, cudaStream_t stream) {
+  return prefill_paged(q, q_stride, k_pool, v_pool, out, out_stride, page_indices, work, entries, num_tokens, q_heads, kv_heads, dim, vdim, page_size,
+                       page_rows, max_pages, sm_scale, flags, window, keep_first, chunked, sigmoid, softcap, sink, bias, bias_len, gate, gate_stride,
+                       nullptr, nullptr, status, dtype, stream);
+}
+
+// The same for a bf16 model (sink and out) with operands in fp16: q [num_tokens][q_heads * dim] was multiplied by 1 / q_up [num_tokens][q_heads],
+// keys and values by 1 / kv_up [2][kv_heads], powers of two.  dim 64 or 128.
+int blitz_attn_prefill_scaled(const void* q, const void* k_pool, const void* v_pool, void* out, int64_t out_stride, const int32_t* page_indices,
+                              const int32_t* work, int entries, int num_tokens, int q_heads, int kv_heads, int dim, int page_size, int page_rows,
+                              int max_pages, float sm_scale, int window, int keep_first, float softcap, const void* sink, const float* q_up,
+                              const float* kv_up, int* status, cudaStream_t stream) {
+  if (q_up == nullptr || kv_up == nullptr) return -1;
+  return prefill_paged(q, (int64_t)q_heads * dim, k_pool, v_pool, out, out_stride, page_indices, work, entries, num_tokens, q_heads, kv_heads, dim, dim,
+                       page_size, page_rows, max_pages, sm_scale, 0, window, keep_first, 0, 0, softcap, sink, nullptr, 0, nullptr, 0, q_up, kv_up, status, 0,
+                       stream);
 }
 
 }  // extern "C"

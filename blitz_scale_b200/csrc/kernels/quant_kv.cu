@@ -266,7 +266,69 @@ struct QuantPagesParams {
   int64_t units;     // (page, 16 tokens of it, head) each
   int kv_heads, page_size, page_rows, max_pages;
   int* status;
+  // for attention of portions: records of the pass (see attn_prefill_paged.cu), whose page numbers count from `first` pages before the first one
+  const int32_t* work;
+  int entries, first;
+  int32_t* table;     // numbers of the pages read back, for all of those that the records count
+  const float* spans; // SCALED: [span_blocks][2][kv_heads] largest magnitudes
+  int span_blocks;
+  float* up;          // SCALED: [2][kv_heads] powers of two that were taken out of keys and values
+  // ... and its queries: [tokens][q_heads * dim] to fp16, and a power of two for each row of a head
+  const void* q;
+  void* q_to;
+  float* q_up;
+  int64_t q_row;
+  int tokens, q_heads, page_blocks;
 };
+
+// Tokens of page `n` (counted as the records do) that its sequence has, -1: no record has it.  The whole warp asks.
+__device__ __forceinline__ int quant_kv_held(const QuantPagesParams& p, int n) {
+  int held = -1;
+  for (int e = threadIdx.x & 31; e < p.entries; e += 32) {
+    const int4 r = __ldg(reinterpret_cast<const int4*>(p.work + e * 8));
+    if (n >= r.z && n < r.z + r.w) held = min(p.page_size, max(0, __ldg(p.work + e * 8 + 4) - (n - r.z) * p.page_size));
+  }
+  return __reduce_max_sync(0xffffffffu, held);
+}
+// 2^-e, 2^e <= x < 2^(e + 1): what brings numbers up to x to below 2
+__device__ __forceinline__ float quant_kv_down(float x) {
+  const int e = x > 0.f && x <= 3.4e38f ? max(-100, min(126, static_cast<int>(__float_as_uint(x) >> 23) - 127)) : 0;
+  return __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+}
+
+// The largest magnitudes of a pass's keys and values, by head: of every block, a part of them.  Half a warp looks at the scales of the
+// keys of 16 tokens, the other half at those of the values.
+template <int D, int GROUP>
+__global__ void __launch_bounds__(256) quant_kv_span_kernel(const QuantPagesParams p, float* __restrict__ spans) {
+  constexpr QuantKv F = quant_kv(D, GROUP);
+  constexpr int G = F.groups;
+  extern __shared__ int s_most[];  // [2][kv_heads] bits of numbers that are not negative
+  for (int i = threadIdx.x; i < 2 * p.kv_heads; i += blockDim.x) s_most[i] = 0;
+  ptx::griddep_launch_dependents();
+  ptx::griddep_wait();
+  __syncthreads();
+  const int lane = threadIdx.x & 31, blocks = p.page_size >> 4;
+  for (int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); unit < p.units; unit += static_cast<int64_t>(gridDim.x) * 8) {
+    const int head = static_cast<int>(unit % p.kv_heads), b = static_cast<int>(unit / p.kv_heads % blocks);
+    const int n = static_cast<int>(unit / p.kv_heads / blocks), held = quant_kv_held(p, n + p.first), page = p.pages[n];
+    if (held <= b * 16 || page < 0 || page >= p.max_pages) continue;
+    const uint8_t* block = p.pool + ((static_cast<int64_t>(page) * p.kv_heads + head) * blocks + b) * F.block;
+    const __nv_bfloat16* w = reinterpret_cast<const __nv_bfloat16*>(block + (lane < 16 ? 0 : F.part) + F.codes) + (lane & 15) * 2 * G;
+    float most = 0.f;
+    if (b * 16 + (lane & 15) < held) {
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        const float s = __bfloat162float(w[i]), z = __bfloat162float(w[G + i]);
+        most = fmaxf(most, fmaxf(fabsf(z), fabsf(fmaf(15.f, s, z))));  // (NaN: not counted)
+      }
+    }
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+    if ((lane & 15) == 0) atomicMax(&s_most[(lane >> 4) * p.kv_heads + head], __float_as_int(most));
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * p.kv_heads; i += blockDim.x) spans[static_cast<int64_t>(blockIdx.x) * 2 * p.kv_heads + i] = __int_as_float(s_most[i]);
+}
 
 // The codes of a warp's 16 tokens of a head, 8 x 8 blocks of (token, dimension) at a time as tensor-core fragments have them.
 __device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -275,7 +337,11 @@ __device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t a, uin
 // A warp takes 16 tokens of a head.  Keys: four lanes a token, 32 codes each.  Values: a lane has four tokens of eight dimensions 8 apart, which
 // stmatrix turns into rows of a token.  Both go out from shared memory, whole rows at a time.
 // Bound by the 16-bit rows that it writes (four times the codes).
-template <typename T, int D, int GROUP>
+//
+// For attention of portions (WORK) the tokens behind a sequence's end are zeros, whatever the cache has there.  SCALED: queries, keys and
+// values of a bf16 model go to fp16, which keeps three bits more of what z + s c is: keys and values divided by a power of two near the
+// largest of their head, a row of queries by one near its own largest entry, so that the type's range does not matter.
+template <typename T, int D, int GROUP, bool WORK, bool SCALED>
 __global__ void __launch_bounds__(256, 3) quant_kv_pages_kernel(const QuantPagesParams p) {
   constexpr QuantKv F = quant_kv(D, GROUP);
   constexpr int W = D / 32, G = F.groups;
@@ -288,10 +354,56 @@ __global__ void __launch_bounds__(256, 3) quant_kv_pages_kernel(const QuantPages
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
   uint8_t* const rows = s_rows[warp];
   const int blocks = p.page_size >> 4;
-  for (int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + warp; unit < p.units; unit += static_cast<int64_t>(gridDim.x) * 8) {
+  if (SCALED && static_cast<int>(blockIdx.x) >= p.page_blocks) {
+    // queries: D / 8 lanes a row of a head
+    constexpr int LANES = D / 8;
+    const int64_t all = static_cast<int64_t>(p.tokens) * p.q_heads, step = static_cast<int64_t>(gridDim.x - p.page_blocks) * (256 / LANES);
+    for (int64_t r = static_cast<int64_t>(blockIdx.x - p.page_blocks) * (256 / LANES) + threadIdx.x / LANES; r - threadIdx.x / LANES < all; r += step) {
+      const int64_t t = r / p.q_heads;
+      const int h = static_cast<int>(r - t * p.q_heads), l = threadIdx.x % LANES;
+      float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, most = 0.f;
+      if (r < all) ldf8<__nv_bfloat16>(reinterpret_cast<const __nv_bfloat16*>(p.q) + t * p.q_row + static_cast<int64_t>(h) * D + l * 8, x);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(x[i]));
+#pragma unroll
+      for (int d = 1; d < LANES; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+      const float down = quant_kv_down(most);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] *= down;
+      if (r < all) {
+        stf8<__half>(reinterpret_cast<__half*>(p.q_to) + r * D + l * 8, x);
+        if (l == 0) p.q_up[r] = 1.f / down;
+      }
+    }
+    return;
+  }
+  if (WORK && blockIdx.x == 0)
+    for (int64_t i = threadIdx.x; i < p.units / p.kv_heads / blocks + p.first; i += 256) p.table[i] = max(0, static_cast<int>(i) - p.first);
+  __shared__ float s_down[SCALED ? 256 : 1];  // of keys, then of values, by head
+  if (SCALED) {
+    for (int i = warp; i < 2 * p.kv_heads; i += 8) {
+      float most = 0.f;
+      for (int c = lane; c < p.span_blocks; c += 32) most = fmaxf(most, p.spans[static_cast<int64_t>(c) * 2 * p.kv_heads + i]);
+      const float down = quant_kv_down(warp_max(most));
+      if (lane == 0) {
+        s_down[i] = down;
+        if (blockIdx.x == 0) p.up[i] = 1.f / down;
+      }
+    }
+    __syncthreads();
+  }
+  const int64_t step = static_cast<int64_t>(SCALED ? p.page_blocks : gridDim.x) * 8;
+  for (int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + warp; unit < p.units; unit += step) {
     const int head = static_cast<int>(unit % p.kv_heads), b = static_cast<int>(unit / p.kv_heads % blocks);
     const int64_t n = unit / p.kv_heads / blocks;
     const int page = p.pages[n];
+    int held = p.page_size;
+    if (WORK) {
+      held = quant_kv_held(p, static_cast<int>(n) + p.first);
+      if (held < 0) continue;  // (no record has the page)
+    }
+    held -= b * 16;            // of these 16 tokens
+    const float k_down = SCALED ? s_down[head] : 1.f, v_down = SCALED ? s_down[p.kv_heads + head] : 1.f;
     if (page < 0 || page >= p.max_pages) {
       if (p.status && lane == 0) atomicCAS(p.status, 0, kStatusBadIndex);
       continue;
@@ -336,6 +448,7 @@ __global__ void __launch_bounds__(256, 3) quant_kv_pages_kernel(const QuantPages
     for (int j = 0; j < 4; ++j) numbers(block + F.part + F.codes + (4 * t4 + j) * 4 * G, vs[j]);
     constexpr float most = quant_kv_most<T>();
     bool past = false;
+    if (!SCALED)
 #pragma unroll
     for (int i = 0; i < G; ++i) {
 #pragma unroll
@@ -357,7 +470,9 @@ __global__ void __launch_bounds__(256, 3) quant_kv_pages_kernel(const QuantPages
       for (int w = 0; w < W; ++w) {
         float x[8];
         quant_kv_codes(kw[r][w], x);
-        const float sc = number(ks[r], w * 32 / GROUP), z = number(ks[r], G + w * 32 / GROUP);
+        float sc = number(ks[r], w * 32 / GROUP), z = number(ks[r], G + w * 32 / GROUP);
+        if (SCALED) sc *= k_down, z *= k_down;
+        if (WORK && g + 8 * r >= held) sc = z = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = fmaf(sc, x[i], z);
         if (past) {
@@ -374,7 +489,13 @@ __global__ void __launch_bounds__(256, 3) quant_kv_pages_kernel(const QuantPages
       float x[8];
       quant_kv_codes(vw[m], x);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = fmaf(number(vs[(j & 2) + (j >> 2)], i), x[j], number(vs[(j & 2) + (j >> 2)], G + i));
+      for (int j = 0; j < 8; ++j) {
+        const int tok = (j & 2) + (j >> 2);
+        float sc = number(vs[tok], i), z = number(vs[tok], G + i);
+        if (SCALED) sc *= v_down, z *= v_down;
+        if (WORK && 4 * t4 + tok >= held) sc = z = 0.f;
+        x[j] = fmaf(sc, x[j], z);
+      }
       if (past) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] = quant_kv_cut(x[j], most);
@@ -410,7 +531,26 @@ struct PagesLaunch {
   template <typename T, int D, int GROUP>
   int operator()() const {
     const int64_t blocks = (p.units + 7) / 8, most = (int64_t)device_sm_count() * 16;
-    return (int)launch_pdl(quant_kv_pages_kernel<T, D, GROUP>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, stream, p);
+    return (int)launch_pdl(quant_kv_pages_kernel<T, D, GROUP, false, false>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, stream, p);
+  }
+};
+constexpr int kQuantSpanBlocks = 128;
+struct PortionLaunch {
+  QuantPagesParams& p;
+  float* spans;
+  cudaStream_t stream;
+  template <typename T, int D, int GROUP>
+  int operator()() const {
+    const int64_t blocks = (p.units + 7) / 8, most = (int64_t)device_sm_count() * 16;
+    p.page_blocks = (int)(blocks < most ? blocks : most);
+    if (std::is_same<T, __half>::value)
+      return (int)launch_pdl(quant_kv_pages_kernel<__half, D, GROUP, true, false>, dim3((unsigned)p.page_blocks), dim3(256), 0, stream, p);
+    p.spans = spans;
+    p.span_blocks = (int)(blocks < kQuantSpanBlocks ? blocks : kQuantSpanBlocks);
+    const int rc = (int)launch_pdl(quant_kv_span_kernel<D, GROUP>, dim3((unsigned)p.span_blocks), dim3(256), (size_t)2 * p.kv_heads * 4, stream, p, spans);
+    if (rc) return rc;
+    const int64_t rows = ((int64_t)p.tokens * p.q_heads + 256 / (D / 8) - 1) / (256 / (D / 8));
+    return (int)launch_pdl(quant_kv_pages_kernel<__half, D, GROUP, true, true>, dim3((unsigned)(p.page_blocks + (rows < most ? rows : most))), dim3(256), 0, stream, p);
   }
 };
 
@@ -450,6 +590,39 @@ int blitz_quant_kv_pages(const void* pool, const int32_t* pages, int64_t count, 
   if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(pool)) & 15) return -1;
   QuantPagesParams p{(const uint8_t*)pool, pages, k, v, count * kv_heads * (page_size / 16), kv_heads, page_size, page_rows, max_pages, status};
   return quant_kv_dispatch(dtype, dim, group, PagesLaunch{p, stream});
+}
+
+// Scratch of blitz_quant_kv_portion for `pages` pages and `first` more that the records count, in the order of its layout: keys and values read
+// back [pages][2][page_size][kv_heads][dim] in 16 bits, page numbers; of a bf16 model also queries [tokens][q_heads * dim] in fp16, their
+// powers of two, those of keys and values, the parts of their largest magnitudes.  offsets (may be null): where the 7 parts begin, and the end.
+int64_t blitz_quant_kv_portion_bytes(int64_t pages, int64_t first, int tokens, int q_heads, int kv_heads, int dim, int page_size, int dtype, int64_t* offsets) {
+  const int64_t q = dtype == 1 ? (int64_t)tokens * q_heads : 0, h = dtype == 1 ? 2 * (int64_t)kv_heads : 0;
+  const int64_t sizes[6] = {pages * 4 * page_size * kv_heads * dim, (pages + first) * 4, q * dim * 2, q * 4, h * 4, h * 4 * kQuantSpanBlocks};
+  int64_t at = 0;
+  for (int i = 0; i < 6; ++i) {
+    if (offsets) offsets[i] = at;
+    at += (sizes[i] + 255) / 256 * 256;
+  }
+  if (offsets) offsets[6] = at;
+  return at;
+}
+
+// What attention of portions (blitz_attn_prefill_paged, or blitz_attn_prefill_scaled for a bf16 model) reads instead of a 4-bit cache: pages[n], the
+// (first + n)-th page that the records of `work` count, in 16 bits, zeros behind the end of its sequence; of a bf16 model in fp16, and its queries.
+int blitz_quant_kv_portion(const void* q, int64_t q_row, const void* pool, const int32_t* pages, int64_t count, int64_t first, const int32_t* work,
+                           int entries, int tokens, int q_heads, int kv_heads, int dim, int group, int page_size, int max_pages, void* scratch,
+                           int* status, int dtype, cudaStream_t stream) {
+  if (count <= 0 || entries <= 0 || tokens <= 0) return 0;
+  if (!quant_kv_supported(dim, group, page_size) || kv_heads < 1 || kv_heads > 128 || (q_row & 7) || first < 0 || count + first > 0x7fffffff) return -1;
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(work) | reinterpret_cast<uintptr_t>(pool) | reinterpret_cast<uintptr_t>(scratch)) & 15) return -1;
+  int64_t at[7];
+  blitz_quant_kv_portion_bytes(count, first, tokens, q_heads, kv_heads, dim, page_size, dtype, at);
+  char* s = (char*)scratch;
+  QuantPagesParams p{(const uint8_t*)pool, pages, s, s + (int64_t)page_size * kv_heads * dim * 2, count * kv_heads * (page_size / 16), kv_heads, page_size, 2 * page_size, max_pages, status};
+  p.work = work; p.entries = entries; p.first = (int)first; p.table = (int32_t*)(s + at[1]);
+  p.q = q; p.q_row = q_row; p.tokens = tokens; p.q_heads = q_heads;
+  p.q_to = s + at[2]; p.q_up = (float*)(s + at[3]); p.up = (float*)(s + at[4]);
+  return quant_kv_dispatch(dtype, dim, group, PortionLaunch{p, (float*)(s + at[5]), stream});
 }
 
 }  // extern "C"

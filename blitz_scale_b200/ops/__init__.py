@@ -616,6 +616,37 @@ def _attn_decode_quant(q, cache, indices, indptr, last_page_len, q_heads, kv_hea
     return out
 
 
+def _attn_portion_quant(q, cache, page_indices, work, q_heads, kv_heads, head_dim, page_size, out, sm_scale, window, keep_first, softcap, sink, refused,
+                        skip_pages):
+    _int32(page_indices, None, "page_indices")
+    P = page_indices.shape[0]
+    if not 0 <= skip_pages <= P:
+        raise ValueError(f"skip_pages {skip_pages} of {P} pages")
+    if work.dtype != torch.int32 or work.dim() != 2 or work.shape[1] != 8 or not work.is_contiguous() or work.data_ptr() & 15:
+        raise ValueError(f"work: records of prefill_work_list, got {tuple(work.shape)} {work.dtype}")
+    T, entries, n = q.shape[0], work.shape[0], P - skip_pages
+    out = _quant_attn(q, T, cache, q_heads, kv_heads, head_dim, page_size, window, keep_first, softcap, sink, out, refused, page_indices, work)
+    if entries == 0 or T == 0 or n == 0:
+        return out
+    L, pool, dt, status, stream = lib(), cache.pool, _DT[q.dtype], _status_ptr(q), _stream()
+    at = (ctypes.c_int64 * 7)()
+    scratch = torch.empty(L.blitz_quant_kv_portion_bytes(n, skip_pages, T, q_heads, kv_heads, head_dim, page_size, dt, at), dtype=torch.uint8, device=q.device)
+    base = scratch.data_ptr()
+    _check(L.blitz_quant_kv_portion(q.data_ptr(), q.stride(0), pool.data_ptr(), page_indices.data_ptr() + 4 * skip_pages, n, skip_pages, work.data_ptr(),
+                                    entries, T, q_heads, kv_heads, head_dim, cache.group, page_size, pool.shape[0], base, status, dt, stream),
+           "blitz_quant_kv_portion")
+    scale, values, snk = head_dim ** -0.5 if sm_scale is None else sm_scale, base + 2 * page_size * kv_heads * head_dim, None if sink is None else sink.data_ptr()
+    if dt == 1:
+        _check(L.blitz_attn_prefill_scaled(base + at[2], base, values, out.data_ptr(), out.stride(0), base + at[1], work.data_ptr(), entries, T, q_heads,
+                                           kv_heads, head_dim, page_size, 2 * page_size, n, scale, window, keep_first, softcap, snk, base + at[3],
+                                           base + at[4], status, stream), "blitz_attn_prefill_scaled")
+    else:
+        _check(L.blitz_attn_prefill_paged(q.data_ptr(), q.stride(0), base, values, out.data_ptr(), out.stride(0), base + at[1], work.data_ptr(), entries, T,
+                                          q_heads, kv_heads, head_dim, head_dim, page_size, 2 * page_size, n, scale, 0, window, keep_first, 0, 0, softcap,
+                                          snk, None, 0, None, 0, status, dt, stream), "blitz_attn_prefill_paged")
+    return out
+
+
 def attn_decode(q: torch.Tensor, kv_layer: KVLayer, indices: torch.Tensor, indptr: torch.Tensor,
                 last_page_len: torch.Tensor, *, q_heads: int, kv_heads: int, head_dim: int, page_size: int,
                 num_splits: int = 1, workspace: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
@@ -699,20 +730,12 @@ def attn_prefill_paged(q: torch.Tensor, kv_layer: KVLayer, page_indices: torch.T
     for the same sequences.  ``window`` / ``keep_first`` / ``softcap`` / ``sink`` / ``gate`` / ``bias`` / ``chunked`` / ``sigmoid``
     as for `attn_decode` (no bias beside a window, cap or sink; with sigmoid weights a bias of one column).
 
-    Over a 4-bit cache (QuantKV): the pages named by ``page_indices`` are read back first, rounded to the queries' type, into scratch of
-    this call; no record of ``work`` refers to the first ``skip_pages`` of them, which are passed over."""
+    Over a 4-bit cache (QuantKV): the pages that ``work`` refers to are read back first, into scratch of this call (of a bf16 model in
+    fp16, with its queries, scaled so that the type's range does not matter); tokens behind a sequence's end may hold anything; no gate,
+    bias, ``chunked`` or ``sigmoid``; no record of ``work`` refers to the first ``skip_pages`` entries of ``page_indices``."""
     if isinstance(kv_layer, QuantKV):
-        _int32(page_indices, None, "page_indices")
-        if not 0 <= skip_pages <= page_indices.numel():
-            raise ValueError(f"skip_pages {skip_pages} of {page_indices.numel()} pages")
-        if work.dtype != torch.int32 or work.dim() != 2 or work.shape[1] != 8 or not work.is_contiguous():
-            raise ValueError(f"work: records of prefill_work_list, got {tuple(work.shape)} {work.dtype}")
-        out = _quant_attn(q, q.shape[0], kv_layer, q_heads, kv_heads, head_dim, page_size, window, keep_first, softcap, sink, out,
-                             dict(gate=gate, bias=bias, chunked=chunked, sigmoid=sigmoid), page_indices, work)
-        if work.shape[0] == 0 or q.shape[0] == 0:
-            return out
-        kv_layer = quant_kv_pages(kv_layer, page_indices[skip_pages:], dtype=q.dtype)
-        page_indices = torch.arange(-skip_pages, kv_layer.shape[0], dtype=torch.int32, device=q.device)
+        return _attn_portion_quant(q, kv_layer, page_indices, work, q_heads, kv_heads, head_dim, page_size, out, sm_scale, window, keep_first, softcap, sink,
+                                   dict(gate=gate, bias=bias, chunked=chunked, sigmoid=sigmoid), skip_pages)
     T = q.shape[0]
     kp, vp, page_rows, pages, vdim = _kv(kv_layer)
     if out is None:
