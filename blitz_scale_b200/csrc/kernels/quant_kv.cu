@@ -7,6 +7,101 @@
 
 namespace blitz {
 
+// Eight numbers of a lane, whose group the lanes around it share: their codes, and the group's scale and offset.
+template <typename T, int GROUP>
+__device__ __forceinline__ void quant_kv_group(const uint4& u, uint32_t& word, __nv_bfloat16& s16, __nv_bfloat16& z16) {
+  // the smallest number and the negative of the largest, as a pair (NaN where there is one)
+  using T2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
+  auto pair = [](uint32_t u) { return *reinterpret_cast<T2*>(&u); };
+  auto bits = [](T2 v) { return *reinterpret_cast<uint32_t*>(&v); };
+  uint32_t lo2 = bits(__hmin2_nan(__hmin2_nan(pair(u.x), pair(u.y)), __hmin2_nan(pair(u.z), pair(u.w))));
+  uint32_t hi2 = bits(__hmax2_nan(__hmax2_nan(pair(u.x), pair(u.y)), __hmax2_nan(pair(u.z), pair(u.w)))) ^ 0x80008000u;
+  uint32_t ends = bits(__hmin2_nan(pair(__byte_perm(lo2, hi2, 0x5410)), pair(__byte_perm(lo2, hi2, 0x7632))));
+#pragma unroll
+  for (int d = 1; d < GROUP / 8; d <<= 1) ends = bits(__hmin2_nan(pair(ends), pair(__shfl_xor_sync(0xffffffffu, ends, d))));
+  const float2 end = cvt2<T>(ends);
+  z16 = __float2bfloat16_rd(end.x);
+  const float z = __bfloat162float(z16), range = -end.y - z;
+  // the smallest scale whose 15 steps cover the range: near range / 15, and then by what its product says
+  uint32_t sb = __bfloat16_as_ushort(__float2bfloat16_ru(range * (1.f / 15.f)));
+  if (fmaf(__uint_as_float(sb << 16), 15.f, -range) < 0.f) ++sb;
+  else if (sb > 0 && fmaf(__uint_as_float((sb - 1) << 16), 15.f, -range) >= 0.f) --sb;
+  if (!(range <= 3.4e38f)) {
+    z16 = __ushort_as_bfloat16(0x7fff);
+    sb = 0;
+  }
+  s16 = __ushort_as_bfloat16(static_cast<unsigned short>(sb));
+  const float sc = __uint_as_float(sb << 16);
+  // rint((x - z) / s), between 0 and 15: by the reciprocal, whose error (2^-22 of the quotient) counts next to a tie only; those few are
+  // divided.  (A scale below 2^-120 has no reciprocal that serves: all are divided.)  Rounded by what is left of a mantissa.
+  word = 0;
+  if (sc > 0.f) {
+    float x[8], c[8], near = 0.f;
+    unpack8<T>(u, x);
+    const float inv = ptx::rcp_approx(sc);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float q = (x[i] - z) * inv;
+      c[i] = (q + 12582912.f) - 12582912.f;
+      near = fmaxf(near, fabsf(q - c[i]));
+    }
+    if (near > 0.4999f || sc < 7.6e-37f) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) c[i] = rintf(__fdiv_rn(x[i] - z, sc));
+    }
+    // four codes are a number of 16 bits
+    const float low = fmaf(fmaf(fmaf(c[3], 16.f, c[2]), 16.f, c[1]), 16.f, c[0]) + 8388608.f;
+    const float high = fmaf(fmaf(fmaf(c[7], 16.f, c[6]), 16.f, c[5]), 16.f, c[4]) + 8388608.f;
+    word = __byte_perm(__float_as_uint(low), __float_as_uint(high), 0x5410);
+  }
+}
+
+// A lane's eight codes of token `tok` of a block (null: nowhere) and, by a group's first lane, its scale and offset.  Values of four tokens of a
+// word go to `exchange` instead (quant_kv_write_quad follows); others write their bytes.  The whole warp calls.
+template <int D, int GROUP>
+__device__ __forceinline__ void quant_kv_write(uint8_t* block, int tok, int l, bool value, uint32_t* exchange, uint32_t word, __nv_bfloat16 s16, __nv_bfloat16 z16) {
+  constexpr QuantKv F = quant_kv(D, GROUP);
+  if (value) block = block ? block + F.part : nullptr;
+  const uint32_t other = __shfl_xor_sync(0xffffffffu, word, 1);  // the eight dimensions beside these of a tile of 16
+  if (exchange != nullptr) {
+    exchange[l] = word;
+  } else if (block != nullptr && !value) {
+    reinterpret_cast<uint32_t*>(block + tok * (D / 2))[(l & 3) * (D / 32) + (l >> 2)] = word;
+  } else if (block != nullptr) {
+    // nibble i of this half of the tile beside nibble i of the other: even lanes write the first four such bytes, odd ones the rest
+    const uint32_t low = l & 1 ? other : word, high = l & 1 ? word : other;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int g = (l & 1) * 4 + i;
+      block[quant_kv_value_byte(tok, (l >> 1) * 16 + g)] = static_cast<uint8_t>(((low >> (4 * g)) & 15u) | (((high >> (4 * g)) & 15u) << 4));
+    }
+  }
+  if (l % (GROUP / 8) == 0 && block != nullptr) {
+    __nv_bfloat16* w = reinterpret_cast<__nv_bfloat16*>(block + F.codes) + tok * 2 * F.groups + l / (GROUP / 8);
+    w[0] = s16;
+    w[F.groups] = z16;
+  }
+}
+// The words of four tokens, from token `tok` of a block on, whose codes the warp has put into `codes` [4][D / 8].
+template <int D, int GROUP>
+__device__ __forceinline__ void quant_kv_write_quad(uint8_t* block, int tok, const uint32_t* codes) {
+  constexpr int LANES = D / 8;
+  block += quant_kv(D, GROUP).part;
+  __syncwarp();
+  // word (m / 4, g, quad, m % 4): bytes are tokens 0, 2, 1, 3, nibbles dimensions 16 m + g and 16 m + 8 + g
+#pragma unroll
+  for (int i = threadIdx.x & 31; i < D / 2; i += 32) {
+    const int m = (i >> 5) * 4 + (i & 3), g = (i >> 2) & 7;
+    uint32_t word = 0;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const uint32_t* from = codes + ((b & 1) * 2 + (b >> 1)) * LANES + 2 * m;
+      word |= (((from[0] >> (4 * g)) & 15u) | (((from[1] >> (4 * g)) & 15u) << 4)) << (8 * b);
+    }
+    *reinterpret_cast<uint32_t*>(block + (i >> 5) * 512 + g * 64 + (tok >> 2) * 16 + (i & 3) * 4) = word;
+  }
+}
+
 // ------------------------------------------------------------------ rows in
 struct QuantStoreParams {
   const void *k, *v;  // [tokens][kv_heads * dim], pitches in elements
@@ -60,94 +155,105 @@ __global__ void __launch_bounds__(256) quant_kv_store_kernel(const QuantStorePar
 #pragma unroll
     for (int r = 0; r < 4 / ROWS; ++r) {
       const int s = __shfl_sync(0xffffffffu, slots, r * ROWS + lane / LANES);
-      // the smallest number and the negative of the largest, as a pair (NaN where there is one)
-      using T2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
-      auto pair = [](uint32_t u) { return *reinterpret_cast<T2*>(&u); };
-      auto bits = [](T2 v) { return *reinterpret_cast<uint32_t*>(&v); };
-      const uint4 u = raw[value][r];
-      uint32_t lo2 = bits(__hmin2_nan(__hmin2_nan(pair(u.x), pair(u.y)), __hmin2_nan(pair(u.z), pair(u.w))));
-      uint32_t hi2 = bits(__hmax2_nan(__hmax2_nan(pair(u.x), pair(u.y)), __hmax2_nan(pair(u.z), pair(u.w)))) ^ 0x80008000u;
-      uint32_t ends = bits(__hmin2_nan(pair(__byte_perm(lo2, hi2, 0x5410)), pair(__byte_perm(lo2, hi2, 0x7632))));
-#pragma unroll
-      for (int d = 1; d < GROUP / 8; d <<= 1) ends = bits(__hmin2_nan(pair(ends), pair(__shfl_xor_sync(0xffffffffu, ends, d))));
-      const float2 end = cvt2<T>(ends);
-      __nv_bfloat16 z16 = __float2bfloat16_rd(end.x);
-      const float z = __bfloat162float(z16), range = -end.y - z;
-      // the smallest scale whose 15 steps cover the range: near range / 15, and then by what its product says
-      uint32_t sb = __bfloat16_as_ushort(__float2bfloat16_ru(range * (1.f / 15.f)));
-      if (fmaf(__uint_as_float(sb << 16), 15.f, -range) < 0.f) ++sb;
-      else if (sb > 0 && fmaf(__uint_as_float((sb - 1) << 16), 15.f, -range) >= 0.f) --sb;
-      if (!(range <= 3.4e38f)) {
-        z16 = __ushort_as_bfloat16(0x7fff);
-        sb = 0;
-      }
-      const __nv_bfloat16 s16 = __ushort_as_bfloat16(static_cast<unsigned short>(sb));
-      const float sc = __uint_as_float(sb << 16);
-      // rint((x - z) / s), between 0 and 15: by the reciprocal, whose error (2^-22 of the quotient) counts next to a tie only; those few are
-      // divided.  (A scale below 2^-120 has no reciprocal that serves: all are divided.)  Rounded by what is left of a mantissa.
-      uint32_t word = 0;
-      if (sc > 0.f) {
-        float x[8], c[8], near = 0.f;
-        unpack8<T>(u, x);
-        const float inv = ptx::rcp_approx(sc);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float q = (x[i] - z) * inv;
-          c[i] = (q + 12582912.f) - 12582912.f;
-          near = fmaxf(near, fabsf(q - c[i]));
-        }
-        if (near > 0.4999f || sc < 7.6e-37f) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) c[i] = rintf(__fdiv_rn(x[i] - z, sc));
-        }
-        // four codes are a number of 16 bits
-        const float low = fmaf(fmaf(fmaf(c[3], 16.f, c[2]), 16.f, c[1]), 16.f, c[0]) + 8388608.f;
-        const float high = fmaf(fmaf(fmaf(c[7], 16.f, c[6]), 16.f, c[5]), 16.f, c[4]) + 8388608.f;
-        word = __byte_perm(__float_as_uint(low), __float_as_uint(high), 0x5410);
-      }
-      const int tok = s & 15;  // (pages hold a multiple of 16 tokens)
-      uint8_t* const block = block_of(max(s, 0)) + (value ? F.part : 0);
-      if (!value) {
-        if (s >= 0) reinterpret_cast<uint32_t*>(block + tok * (D / 2))[(l & 3) * (D / 32) + (l >> 2)] = word;
-      } else if (quad) {
-        codes[(r * ROWS + lane / LANES) * LANES + l] = word;
-      } else {
-        const uint32_t other = __shfl_xor_sync(0xffffffffu, word, 1);  // the eight dimensions beside these of a tile of 16
-        // nibble i of this half of the tile beside nibble i of the other: even lanes write the first four such bytes, odd ones the rest
-        const uint32_t low = l & 1 ? other : word, high = l & 1 ? word : other;
-        if (s >= 0) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int g = (l & 1) * 4 + i;
-            block[quant_kv_value_byte(tok, (l >> 1) * 16 + g)] = static_cast<uint8_t>(((low >> (4 * g)) & 15u) | (((high >> (4 * g)) & 15u) << 4));
-          }
-        }
-      }
-      if (l % (GROUP / 8) == 0 && s >= 0) {
-        __nv_bfloat16* w = reinterpret_cast<__nv_bfloat16*>(block + F.codes) + tok * 2 * F.groups + l / (GROUP / 8);
-        w[0] = s16;
-        w[F.groups] = z16;
-      }
+      uint32_t word;
+      __nv_bfloat16 s16, z16;
+      quant_kv_group<T, GROUP>(raw[value][r], word, s16, z16);
+      quant_kv_write<D, GROUP>(s >= 0 ? block_of(s) : nullptr, s & 15, l, value, value && quad ? codes + (r * ROWS + lane / LANES) * LANES : nullptr, word, s16, z16);
     }
-    if (value && quad) {
-      __syncwarp();
-      // word (m / 4, g, quad, m % 4): bytes are tokens 0, 2, 1, 3, nibbles dimensions 16 m + g and 16 m + 8 + g
-      uint8_t* const block = block_of(s0) + F.part;
-#pragma unroll
-      for (int i = lane; i < D / 2; i += 32) {
-        const int m = (i >> 5) * 4 + (i & 3), g = (i >> 2) & 7;
-        uint32_t word = 0;
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const uint32_t* from = codes + ((b & 1) * 2 + (b >> 1)) * LANES + 2 * m;
-          word |= (((from[0] >> (4 * g)) & 15u) | (((from[1] >> (4 * g)) & 15u) << 4)) << (8 * b);
-        }
-        *reinterpret_cast<uint32_t*>(block + (i >> 5) * 512 + g * 64 + ((s0 & 15) >> 2) * 16 + (i & 3) * 4) = word;
-      }
-    }
+    if (value && quad) quant_kv_write_quad<D, GROUP>(block_of(s0), s0 & 15, codes);
   };
   rows(std::false_type{});
   rows(std::true_type{});
+}
+
+// ------------------------------------------------------------------ rotation and rows in
+struct QuantRopeParams {
+  void* qkv;  // [tokens][(q_heads + 2 kv_heads) * dim], queries and keys are rotated in place
+  const int32_t *pos, *slot;
+  uint8_t* pool;
+  int tokens, q_heads, kv_heads, page_shift, max_pages;
+  float log2_theta;
+  int* status;
+};
+
+// Queries and keys of a fused projection rotated in place (half-split pairs, as rope_kv_store does), keys and values into the cache: what goes
+// there is what the 16-bit rows hold.  A block takes R tokens, whose angles it computes once; a warp four (row, head) pairs at a time:
+// four rows of a head (R = 4: values go out by words), or four heads of a row (R = 1: more blocks where there are few tokens).
+// STATIC: positions and slots that no kernel in flight writes: angles are ready when the projection is.
+template <typename T, int D, int GROUP, int R, bool STATIC>
+__global__ void __launch_bounds__(256) quant_kv_rope_kernel(const QuantRopeParams p) {
+  constexpr QuantKv F = quant_kv(D, GROUP);
+  constexpr int LANES = D / 8, ROWS = 32 / LANES, HALF = D / 2;
+  __shared__ float s_cos[R][HALF], s_sin[R][HALF];
+  __shared__ uint32_t s_codes[8][R == 4 ? 4 * LANES : 1];
+  ptx::griddep_launch_dependents();
+  if (!STATIC) ptx::griddep_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % LANES;
+  const int t0 = blockIdx.x * R;
+  int slots = lane < R && t0 + lane < p.tokens ? p.slot[t0 + lane] : -1;
+  const bool bad = slots >= 0 && slots >> p.page_shift >= p.max_pages;
+  if (bad) slots = -1;
+  for (int i = threadIdx.x; i < R * HALF; i += 256) {
+    const int r = i / HALF, k = i % HALF;
+    const float x = static_cast<float>(t0 + r < p.tokens ? p.pos[t0 + r] : 0) * exp2f(-(2.0f * static_cast<float>(k) / static_cast<float>(D)) * p.log2_theta);
+    sincosf(x, &s_sin[r][k], &s_cos[r][k]);
+  }
+  if (STATIC) ptx::griddep_wait();
+  if (bad && warp == 0 && p.status) atomicCAS(p.status, 0, kStatusBadIndex);
+  __syncthreads();
+  const int s0 = __shfl_sync(0xffffffffu, slots, 0), turned = p.q_heads + p.kv_heads, heads = turned + p.kv_heads;
+  const bool quad = R == 4 && s0 >= 0 && (s0 & 3) == 0 && __all_sync(0xffffffffu, lane >= 4 || slots == s0 + lane);
+  const int64_t pitch = static_cast<int64_t>(heads) * D;
+  auto block_of = [&](int s, int kv) {
+    const int page = s >> p.page_shift;
+    return p.pool + (((static_cast<int64_t>(page) * p.kv_heads + kv) << (p.page_shift - 4)) + ((s - (page << p.page_shift)) >> 4)) * F.block;
+  };
+  for (int unit = warp; unit < (R == 4 ? heads : (heads + 3) / 4); unit += 8) {
+    uint4 raw[4 / ROWS];
+    T* at[4 / ROWS];
+#pragma unroll
+    for (int k = 0; k < 4 / ROWS; ++k) {
+      const int i = k * ROWS + lane / LANES, row = R == 4 ? i : 0, h = R == 4 ? unit : unit * 4 + i;
+      const bool real = t0 + row < p.tokens && h < heads;
+      at[k] = real ? reinterpret_cast<T*>(p.qkv) + static_cast<int64_t>(t0 + row) * pitch + static_cast<int64_t>(h) * D + l * 8 : nullptr;
+      raw[k] = real ? *reinterpret_cast<const uint4*>(at[k]) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int k = 0; k < 4 / ROWS; ++k) {
+      const int i = k * ROWS + lane / LANES, row = R == 4 ? i : 0, h = R == 4 ? unit : unit * 4 + i;
+      if (R == 1 || h < turned) {
+        // the other half of the pairs is LANES / 2 lanes away
+        uint4 o;
+        o.x = __shfl_xor_sync(0xffffffffu, raw[k].x, LANES / 2);
+        o.y = __shfl_xor_sync(0xffffffffu, raw[k].y, LANES / 2);
+        o.z = __shfl_xor_sync(0xffffffffu, raw[k].z, LANES / 2);
+        o.w = __shfl_xor_sync(0xffffffffu, raw[k].w, LANES / 2);
+        if (h < turned) {
+          float x[8], y[8];
+          unpack8<T>(raw[k], x);
+          unpack8<T>(o, y);
+          const float sign = l < LANES / 2 ? -1.f : 1.f;
+          const int first = (l * 8) % HALF;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] = x[j] * s_cos[row][first + j] + sign * y[j] * s_sin[row][first + j];
+          raw[k] = pack8<T>(x);
+          if (at[k] != nullptr) *reinterpret_cast<uint4*>(at[k]) = raw[k];
+        }
+      }
+      if (R == 4 ? h < p.q_heads : unit * 4 + 3 < p.q_heads) continue;  // (the whole warp: nothing but queries)
+      uint32_t word;
+      __nv_bfloat16 s16, z16;
+      quant_kv_group<T, GROUP>(raw[k], word, s16, z16);
+      const bool value = h >= turned;
+      const int s = __shfl_sync(0xffffffffu, slots, row);
+      uint8_t* const block = s >= 0 && h >= p.q_heads && h < heads ? block_of(s, value ? h - turned : h - p.q_heads) : nullptr;
+      quant_kv_write<D, GROUP>(block, s & 15, l, value, R == 4 && value && quad ? s_codes[warp] + i * LANES : nullptr, word, s16, z16);
+    }
+    if (R == 4 && quad && unit >= turned) {
+      quant_kv_write_quad<D, GROUP>(block_of(s0, unit - turned), s0 & 15, s_codes[warp]);
+      __syncwarp();  // (the next head's codes)
+    }
+  }
 }
 
 // ------------------------------------------------------------------ rows back
@@ -278,7 +384,7 @@ struct QuantPagesParams {
   void* q_to;
   float* q_up;
   int64_t q_row;
-  int tokens, q_heads, page_blocks;
+  int tokens, q_heads;
 };
 
 // Tokens of page `n` (counted as the records do) that its sequence has, -1: no record has it.  The whole warp asks.
@@ -296,8 +402,43 @@ __device__ __forceinline__ float quant_kv_down(float x) {
   return __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
 }
 
+// Queries to fp16: D / 8 lanes a row of a head, four rows at a time (bound by memory: 64 bytes a thread on their way).
+template <int D>
+__device__ __forceinline__ void quant_kv_queries(const QuantPagesParams& p, int block, int blocks) {
+  constexpr int LANES = D / 8, ROWS = 256 / LANES, U = 4;
+  const int64_t all = static_cast<int64_t>(p.tokens) * p.q_heads;
+  const int l = threadIdx.x % LANES;
+  for (int64_t r0 = static_cast<int64_t>(block) * ROWS * U; r0 < all; r0 += static_cast<int64_t>(blocks) * ROWS * U) {
+    uint4 raw[U];
+    int64_t r[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      r[u] = r0 + u * ROWS + threadIdx.x / LANES;
+      const int64_t t = r[u] / p.q_heads;
+      const int h = static_cast<int>(r[u] - t * p.q_heads);
+      raw[u] = r[u] < all ? ld_nc16(reinterpret_cast<const __nv_bfloat16*>(p.q) + t * p.q_row + static_cast<int64_t>(h) * D + l * 8) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float x[8], most = 0.f;
+      unpack8<__nv_bfloat16>(raw[u], x);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(x[i]));
+#pragma unroll
+      for (int d = 1; d < LANES; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+      const float down = quant_kv_down(most);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] *= down;
+      if (r[u] < all) {
+        stf8<__half>(reinterpret_cast<__half*>(p.q_to) + r[u] * D + l * 8, x);
+        if (l == 0) p.q_up[r[u]] = 1.f / down;
+      }
+    }
+  }
+}
+
 // The largest magnitudes of a pass's keys and values, by head: of every block, a part of them.  Half a warp looks at the scales of the
-// keys of 16 tokens, the other half at those of the values.
+// keys of 16 tokens, the other half at those of the values.  The blocks behind those bring the queries to fp16 meanwhile.
 template <int D, int GROUP>
 __global__ void __launch_bounds__(256) quant_kv_span_kernel(const QuantPagesParams p, float* __restrict__ spans) {
   constexpr QuantKv F = quant_kv(D, GROUP);
@@ -306,9 +447,13 @@ __global__ void __launch_bounds__(256) quant_kv_span_kernel(const QuantPagesPara
   for (int i = threadIdx.x; i < 2 * p.kv_heads; i += blockDim.x) s_most[i] = 0;
   ptx::griddep_launch_dependents();
   ptx::griddep_wait();
+  if (static_cast<int>(blockIdx.x) >= p.span_blocks) {
+    quant_kv_queries<D>(p, blockIdx.x - p.span_blocks, gridDim.x - p.span_blocks);
+    return;
+  }
   __syncthreads();
   const int lane = threadIdx.x & 31, blocks = p.page_size >> 4;
-  for (int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); unit < p.units; unit += static_cast<int64_t>(gridDim.x) * 8) {
+  for (int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); unit < p.units; unit += static_cast<int64_t>(p.span_blocks) * 8) {
     const int head = static_cast<int>(unit % p.kv_heads), b = static_cast<int>(unit / p.kv_heads % blocks);
     const int n = static_cast<int>(unit / p.kv_heads / blocks), held = quant_kv_held(p, n + p.first), page = p.pages[n];
     if (held <= b * 16 || page < 0 || page >= p.max_pages) continue;
@@ -354,29 +499,6 @@ __global__ void __launch_bounds__(256, 3) quant_kv_pages_kernel(const QuantPages
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
   uint8_t* const rows = s_rows[warp];
   const int blocks = p.page_size >> 4;
-  if (SCALED && static_cast<int>(blockIdx.x) >= p.page_blocks) {
-    // queries: D / 8 lanes a row of a head
-    constexpr int LANES = D / 8;
-    const int64_t all = static_cast<int64_t>(p.tokens) * p.q_heads, step = static_cast<int64_t>(gridDim.x - p.page_blocks) * (256 / LANES);
-    for (int64_t r = static_cast<int64_t>(blockIdx.x - p.page_blocks) * (256 / LANES) + threadIdx.x / LANES; r - threadIdx.x / LANES < all; r += step) {
-      const int64_t t = r / p.q_heads;
-      const int h = static_cast<int>(r - t * p.q_heads), l = threadIdx.x % LANES;
-      float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, most = 0.f;
-      if (r < all) ldf8<__nv_bfloat16>(reinterpret_cast<const __nv_bfloat16*>(p.q) + t * p.q_row + static_cast<int64_t>(h) * D + l * 8, x);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(x[i]));
-#pragma unroll
-      for (int d = 1; d < LANES; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-      const float down = quant_kv_down(most);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] *= down;
-      if (r < all) {
-        stf8<__half>(reinterpret_cast<__half*>(p.q_to) + r * D + l * 8, x);
-        if (l == 0) p.q_up[r] = 1.f / down;
-      }
-    }
-    return;
-  }
   if (WORK && blockIdx.x == 0)
     for (int64_t i = threadIdx.x; i < p.units / p.kv_heads / blocks + p.first; i += 256) p.table[i] = max(0, static_cast<int>(i) - p.first);
   __shared__ float s_down[SCALED ? 256 : 1];  // of keys, then of values, by head
@@ -392,8 +514,7 @@ __global__ void __launch_bounds__(256, 3) quant_kv_pages_kernel(const QuantPages
     }
     __syncthreads();
   }
-  const int64_t step = static_cast<int64_t>(SCALED ? p.page_blocks : gridDim.x) * 8;
-  for (int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + warp; unit < p.units; unit += step) {
+  for (int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + warp; unit < p.units; unit += static_cast<int64_t>(gridDim.x) * 8) {
     const int head = static_cast<int>(unit % p.kv_heads), b = static_cast<int>(unit / p.kv_heads % blocks);
     const int64_t n = unit / p.kv_heads / blocks;
     const int page = p.pages[n];
@@ -525,6 +646,20 @@ struct LoadLaunch {
     return (int)launch_pdl(quant_kv_load_kernel<T, D, GROUP>, dim3((unsigned)((p.units + 7) / 8)), dim3(256), 0, stream, p);
   }
 };
+struct RopeLaunch {
+  const QuantRopeParams& p;
+  int static_meta;
+  cudaStream_t stream;
+  template <typename T, int D, int GROUP>
+  int operator()() const {
+    // (four tokens a block from four blocks on every SM on)
+    if (p.tokens >= 16 * device_sm_count())
+      return (int)launch_pdl(static_meta ? quant_kv_rope_kernel<T, D, GROUP, 4, true> : quant_kv_rope_kernel<T, D, GROUP, 4, false>,
+                             dim3((unsigned)((p.tokens + 3) / 4)), dim3(256), 0, stream, p);
+    return (int)launch_pdl(static_meta ? quant_kv_rope_kernel<T, D, GROUP, 1, true> : quant_kv_rope_kernel<T, D, GROUP, 1, false>,
+                           dim3((unsigned)p.tokens), dim3(256), 0, stream, p);
+  }
+};
 struct PagesLaunch {
   const QuantPagesParams& p;
   cudaStream_t stream;
@@ -542,15 +677,16 @@ struct PortionLaunch {
   template <typename T, int D, int GROUP>
   int operator()() const {
     const int64_t blocks = (p.units + 7) / 8, most = (int64_t)device_sm_count() * 16;
-    p.page_blocks = (int)(blocks < most ? blocks : most);
+    const unsigned page_blocks = (unsigned)(blocks < most ? blocks : most);
     if (std::is_same<T, __half>::value)
-      return (int)launch_pdl(quant_kv_pages_kernel<__half, D, GROUP, true, false>, dim3((unsigned)p.page_blocks), dim3(256), 0, stream, p);
+      return (int)launch_pdl(quant_kv_pages_kernel<__half, D, GROUP, true, false>, dim3(page_blocks), dim3(256), 0, stream, p);
     p.spans = spans;
     p.span_blocks = (int)(blocks < kQuantSpanBlocks ? blocks : kQuantSpanBlocks);
-    const int rc = (int)launch_pdl(quant_kv_span_kernel<D, GROUP>, dim3((unsigned)p.span_blocks), dim3(256), (size_t)2 * p.kv_heads * 4, stream, p, spans);
+    const int64_t rows = ((int64_t)p.tokens * p.q_heads + 1024 / (D / 8) - 1) / (1024 / (D / 8));
+    const int rc = (int)launch_pdl(quant_kv_span_kernel<D, GROUP>, dim3((unsigned)(p.span_blocks + (rows < most ? rows : most))), dim3(256),
+                                   (size_t)2 * p.kv_heads * 4, stream, p, spans);
     if (rc) return rc;
-    const int64_t rows = ((int64_t)p.tokens * p.q_heads + 256 / (D / 8) - 1) / (256 / (D / 8));
-    return (int)launch_pdl(quant_kv_pages_kernel<__half, D, GROUP, true, true>, dim3((unsigned)(p.page_blocks + (rows < most ? rows : most))), dim3(256), 0, stream, p);
+    return (int)launch_pdl(quant_kv_pages_kernel<__half, D, GROUP, true, true>, dim3(page_blocks), dim3(256), 0, stream, p);
   }
 };
 
@@ -569,6 +705,18 @@ int blitz_quant_kv_store(const void* k, int64_t k_row, const void* v, int64_t v_
   QuantStoreParams p{k, v, k_row, v_row, slot, (uint8_t*)pool, ((int64_t)num_tokens + 3) / 4 * kv_heads, num_tokens, kv_heads, quant_kv_shift(page_size), max_pages, status};
   if (p.units > (int64_t)8 * 0x7fffffff) return -1;
   return quant_kv_dispatch(dtype, dim, group, StoreLaunch{p, stream});
+}
+
+// qkv: [num_tokens][(q_heads + 2 kv_heads) * dim]: queries and keys are rotated in place to position pos[t] (half-split pairs, base rope_theta),
+// keys and values written as blitz_quant_kv_store does.  static_meta != 0 promises that pos and slot are not written by kernels still running
+// in this stream.
+int blitz_quant_kv_rope(void* qkv, const int32_t* pos, const int32_t* slot, void* pool, int num_tokens, int q_heads, int kv_heads, int dim, int group,
+                        int page_size, int max_pages, float rope_theta, int static_meta, int* status, int dtype, cudaStream_t stream) {
+  if (num_tokens <= 0) return 0;
+  if (!quant_kv_supported(dim, group, page_size) || kv_heads < 1 || q_heads < 0) return -1;
+  if ((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(pool)) & 15) return -1;
+  QuantRopeParams p{qkv, pos, slot, (uint8_t*)pool, num_tokens, q_heads, kv_heads, quant_kv_shift(page_size), max_pages, log2f(rope_theta), status};
+  return quant_kv_dispatch(dtype, dim, group, RopeLaunch{p, static_meta, stream});
 }
 
 // Row slot[r] to row r of k and v, in 16 bits (a negative slot: row r is left as it is).

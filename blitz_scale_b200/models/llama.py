@@ -20,7 +20,7 @@ src/layer/attn.h:217-233, src/layer/glu.h:138-154); the LM head exchanges one
 from __future__ import annotations
 
 from dataclasses import dataclass, field
-from typing import Callable, Dict, List, Optional
+from typing import Callable, Dict, List, Optional, Sequence, Union
 
 import torch
 
@@ -92,7 +92,7 @@ class TPComm:
 
 
 class LlamaRunner:
-    def __init__(self, seg: WeightSegment, kv_cache: torch.Tensor, max_tokens: int, max_batch: int,
+    def __init__(self, seg: WeightSegment, kv_cache: Union[torch.Tensor, Sequence[ops.QuantKV]], max_tokens: int, max_batch: int,
                  comm: Optional[TPComm] = None):
         cfg = seg.cfg
         self.cfg: ModelConfig = cfg
@@ -100,8 +100,13 @@ class LlamaRunner:
         self.tp = seg.tp
         self.qh, self.kvh, self.hd = cfg.q_heads // self.tp, cfg.kv_heads // self.tp, cfg.head_dim
         self.inter = cfg.inter // self.tp
-        self.page_size = kv_cache.shape[3]
-        assert kv_cache.shape[0] == cfg.layers and kv_cache.shape[4] == self.kvh and kv_cache.shape[5] == self.hd
+        self.quant = not isinstance(kv_cache, torch.Tensor)         # a 4-bit cache of every layer
+        if self.quant:
+            assert len(kv_cache) == cfg.layers and all(c.kv_heads == self.kvh and c.dim == self.hd for c in kv_cache)
+            self.page_size = kv_cache[0].page_size
+        else:
+            self.page_size = kv_cache.shape[3]
+            assert kv_cache.shape[0] == cfg.layers and kv_cache.shape[4] == self.kvh and kv_cache.shape[5] == self.hd
         dev, dt = seg.buffer.device, seg.dtype
         H = cfg.hidden
         self.max_tokens, self.max_batch = max_tokens, max_batch
@@ -132,6 +137,11 @@ class LlamaRunner:
             self.comm.all_reduce_(self.res[:T])
 
     def _workspace(self, B: int, splits: int) -> Optional[torch.Tensor]:
+        if self.quant:
+            if "quant" not in self._ws:       # (a batch of any size; the kernel's tickets in it stay zero)
+                self._ws["quant"] = torch.zeros(ops.quant_attn_workspace_bytes(self.max_batch, self.qh, self.hd, self.res.device), dtype=torch.uint8,
+                                                device=self.res.device)
+            return self._ws["quant"]
         if splits == 1:
             return None
         n = ops.attn_decode_workspace_bytes(B, self.qh, self.hd, splits)
@@ -144,7 +154,7 @@ class LlamaRunner:
             ws = self._ws[key] = torch.zeros(n, dtype=torch.uint8, device=self.res.device)
         return ws
 
-    def _layer_cache(self, l: int, m: StepMeta) -> torch.Tensor:
+    def _layer_cache(self, l: int, m: StepMeta) -> Union[torch.Tensor, ops.QuantKV]:
         """Pages of layer l in the cache that the runner has now."""
         return m.view("kv layers", self.kv, list)[l]
 
@@ -185,8 +195,10 @@ class LlamaRunner:
         if m.prefill_work is None:      # a caller that built the step by hand
             m.prefill_work = ops.prefill_work_list(m.seq_lens_host, m.kv_lens_host or m.seq_lens_host, self.page_size,
                                                    self.qkv.device, skip=ns)
+        # (a 4-bit cache: the pages of the single tokens' sequences, which come first, are not read back)
+        skip = sum(-(-n // self.page_size) for n in m.kv_lens_host[:ns]) if self.quant else 0
         ops.attn_prefill_paged(m.rows("qkv", self.qkv, T), kv, m.page_indices, m.prefill_work, q_heads=self.qh,
-                               kv_heads=self.kvh, head_dim=self.hd, page_size=self.page_size, out=m.rows("attn", self.attn, T))
+                               kv_heads=self.kvh, head_dim=self.hd, page_size=self.page_size, out=m.rows("attn", self.attn, T), skip_pages=skip)
 
     def last_rows(self, m: StepMeta) -> torch.Tensor:
         """[batch, hidden]: the state `head` starts from, for the last row of every sequence of a prefill pass."""

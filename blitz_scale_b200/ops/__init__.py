@@ -428,11 +428,14 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor,
     return out
 
 
-def rope_kv_store(qkv: torch.Tensor, pos: torch.Tensor, slot: torch.Tensor, kv_layer: torch.Tensor, *, q_heads: int,
+def rope_kv_store(qkv: torch.Tensor, pos: torch.Tensor, slot: torch.Tensor, kv_layer: Union[torch.Tensor, QuantKV], *, q_heads: int,
                   kv_heads: int, head_dim: int, page_size: int, rope_theta: float, static_meta: bool = False) -> None:
     """Rotate q and k of ``qkv`` in place and write rotated k and v to ``kv_layer`` ([pages, 2, page, kvh, hd]).  ``static_meta``
     promises that ``pos`` and ``slot`` are not written by kernels still running in this stream (the copy that brings them is no
-    kernel): the angles are then computed while the projection is still running."""
+    kernel): the angles are then computed while the projection is still running.  ``kv_layer`` may be a 4-bit cache (QuantKV): what is
+    quantised is what the rows hold then."""
+    if isinstance(kv_layer, QuantKV):
+        return _rope_quant(qkv, pos, slot, kv_layer, q_heads, kv_heads, head_dim, page_size, rope_theta, static_meta)
     T = qkv.shape[0]
     assert qkv.is_contiguous() and qkv.shape[1] == (q_heads + 2 * kv_heads) * head_dim
     assert pos.dtype == torch.int32 and slot.dtype == torch.int32
@@ -513,6 +516,26 @@ def quant_kv_store(k: torch.Tensor, v: torch.Tensor, slot: torch.Tensor, cache: 
                                     cache.group, 16 * shape[2], shape[0], _status_ptr(k), _DT[k.dtype], _stream())
     if rc:
         _check(rc, "blitz_quant_kv_store")
+
+
+def _rope_quant(qkv, pos, slot, cache, q_heads, kv_heads, head_dim, page_size, rope_theta, static_meta) -> None:
+    T, pool = qkv.shape[0], cache.pool
+    if qkv.dtype not in _DT:
+        raise TypeError(f"kernels take fp16/bf16 tensors, got {qkv.dtype}")
+    if kv_heads != pool.shape[1] or head_dim != cache.dim or page_size != 16 * pool.shape[2] or q_heads < 0:
+        raise ValueError(f"{q_heads} query and {kv_heads} KV heads of {head_dim}, pages of {page_size}: the 4-bit cache has {pool.shape[1]} heads of "
+                         f"{cache.dim}, pages of {16 * pool.shape[2]}")
+    if qkv.dim() != 2 or not qkv.is_contiguous() or qkv.shape[1] != (q_heads + 2 * kv_heads) * head_dim or qkv.data_ptr() & 15:
+        raise ValueError(f"qkv: contiguous rows of {q_heads} + 2 x {kv_heads} heads of {head_dim}, got {tuple(qkv.shape)}")
+    if not rope_theta > 0.0:
+        raise ValueError(f"rope_theta {rope_theta}")
+    _int32(pos, T, "pos")
+    _int32(slot, T, "slot")
+    _quant(cache, qkv, pos, slot)
+    rc = lib().blitz_quant_kv_rope(qkv.data_ptr(), pos.data_ptr(), slot.data_ptr(), pool.data_ptr(), T, q_heads, kv_heads, head_dim, cache.group, page_size,
+                                   pool.shape[0], rope_theta, 1 if static_meta else 0, _status_ptr(qkv), _DT[qkv.dtype], _stream())
+    if rc:
+        _check(rc, "blitz_quant_kv_rope")
 
 
 def quant_kv_load(cache: QuantKV, slot: torch.Tensor, *, dtype: torch.dtype = torch.bfloat16, k: Optional[torch.Tensor] = None,

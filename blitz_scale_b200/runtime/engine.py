@@ -81,13 +81,29 @@ def singles_apart(q_heads: int, single_lens: Sequence[int], portion_lens: Sequen
     return q_heads * sum(3 + n / 64 for n in single_lens) > 148 * (10 + max(portion_lens, default=0) / 500)
 
 
+def kv_page_bytes(cfg: ModelConfig, page_size: int, tp: int = 1, kv_bits: int = 16, kv_group: int = 32) -> int:
+    """Bytes of a cache page of one layer of a uniform model: keys and values of `page_size` tokens, contiguous."""
+    if kv_bits not in (16, 4):
+        raise ValueError(f"a cache holds 16 or 4 bits, not {kv_bits}")
+    kvh = cfg.kv_heads // tp
+    if kv_bits == 16:
+        return 2 * page_size * kvh * cfg.head_dim * 2
+    if page_size < 16 or page_size & (page_size - 1):
+        raise ValueError(f"pages of a 4-bit cache hold 16 tokens times a power of two, got {page_size}")
+    return kvh * page_size // 16 * ops.quant_kv_block_bytes(cfg.head_dim, kv_group)
+
+
 class Engine:
+    kv_bits, kv_group = 16, 32      # of the cache
+
     def __init__(self, model: str | ModelConfig, *, num_pages: int, page_size: int = 64, max_batch: int = 256,
                  max_batch_tokens: int = 8192, tp: int = 1, tp_rank: int = 0, dtype=torch.bfloat16,
                  device: Optional[torch.device] = None, comm: Optional[TPComm] = None, use_graphs: bool = True,
                  seg_buffer: Optional[torch.Tensor] = None, kv_buffer: Optional[torch.Tensor] = None,
                  ready: bool = True, seed: int = 0, fused_tp: bool = True, oneshot_max_rows: int = 1024,
-                 tp_contexts: int = 1, use_switch: bool = True, state_slots: Optional[int] = None):
+                 tp_contexts: int = 1, use_switch: bool = True, state_slots: Optional[int] = None, kv_bits: int = 16, kv_group: int = 32):
+        """`kv_bits` 4: keys and values are held in 4 bits, with a scale and an offset of 16 bits for every `kv_group` dimensions of a head
+        (uniform models on one GPU; see ops.QuantKV)."""
         self.cfg = get_config(model) if isinstance(model, str) else model
         self.device = device or torch.device("cuda", torch.cuda.current_device())
         self.dtype, self.tp, self.tp_rank = dtype, tp, tp_rank
@@ -97,6 +113,11 @@ class Engine:
         self.seg = WeightSegment(c, tp, tp_rank, dtype, device=self.device, buffer=seg_buffer)
         self.fused = None
         self.slots = None           # state slots of models with recurrent layers
+        self.kv_bits, self.kv_group = kv_bits, kv_group
+        if kv_bits not in (16, 4):
+            raise ValueError(f"a cache holds 16 or 4 bits, not {kv_bits}")
+        if kv_bits == 4 and (c.family == "hybrid" or tp > 1):
+            raise ValueError(f"{c.name}: a 4-bit cache is for uniform models on one GPU")
         if c.family == "hybrid":
             if tp > 1 or kv_buffer is not None:
                 raise ValueError(f"{c.name}: a hybrid model runs on one GPU, with its own cache memory")
@@ -108,13 +129,16 @@ class Engine:
         else:
             if dtype == torch.float32:
                 raise ValueError(f"{c.name}: the kernels of this model take 16-bit types")
-            kvh = c.kv_heads // tp
+            kvh, kv_type = c.kv_heads // tp, dtype
             kv_shape = (c.layers, num_pages, 2, page_size, kvh, c.head_dim)
+            if kv_bits == 4:
+                kv_type = torch.uint8
+                kv_shape = (c.layers, num_pages, kvh, page_size // 16, kv_page_bytes(c, page_size, tp, 4, kv_group) // (kvh * (page_size // 16)))
             if kv_buffer is None:
                 # zero-filled: the attention kernels require finite values in every slot of an allocated page
-                self.kv = torch.zeros(kv_shape, dtype=dtype, device=self.device)
+                self.kv = torch.zeros(kv_shape, dtype=kv_type, device=self.device)
             else:
-                self.kv = kv_buffer.view(dtype)[:int(np.prod(kv_shape))].view(kv_shape)
+                self.kv = kv_buffer.view(kv_type)[:int(np.prod(kv_shape))].view(kv_shape)
         if c.family == "hybrid":
             self.runner = HybridRunner(self.seg, self.cache, max(max_batch_tokens, max_batch), max_batch)
         elif tp > 1 and comm is not None and fused_tp:
@@ -127,7 +151,8 @@ class Engine:
                                         oneshot_max_rows=oneshot_max_rows)
             self.runner.use_switch = use_switch
         else:
-            self.runner = LlamaRunner(self.seg, self.kv, max_tokens=max(max_batch_tokens, max_batch), max_batch=max_batch,
+            cache = self.kv if kv_bits == 16 else [ops.QuantKV(layer, c.head_dim, kv_group) for layer in self.kv]
+            self.runner = LlamaRunner(self.seg, cache, max_tokens=max(max_batch_tokens, max_batch), max_batch=max_batch,
                                       comm=comm)
         self.pool = core.PagePool(num_pages, page_size)
         self.layout = core.MetaLayout.make(max(max_batch_tokens, max_batch), max_batch, num_pages)
@@ -184,7 +209,9 @@ class Engine:
 
     def choose_splits(self, rows: int, max_len: int, tokens: int = 0) -> int:
         """How decode attention divides the keys of `rows` sequences (rows of padding not counted), the longest of max_len and `tokens`
-        in all (0: not known, taken for unequal lengths): see decode_parts."""
+        in all (0: not known, taken for unequal lengths): see decode_parts.  (A 4-bit cache's keys are always taken in equal shares.)"""
+        if self.kv_bits == 4:
+            return 0
         if self.cfg.family == "hybrid":
             # (latent attention divides its keys by itself)
             kv_heads, max_len = self.cfg.attention_work(max_len, ("attention",))

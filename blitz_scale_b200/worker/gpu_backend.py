@@ -34,7 +34,7 @@ from ..parallel import symm
 from ..parallel.agreement import LoadAgreement, StepLog
 from ..pb.schema import pb
 from ..runtime import core
-from ..runtime.engine import Engine
+from ..runtime.engine import Engine, kv_page_bytes
 from .service import Backend, seq_spec_from_request
 from .stopping import StopSequences
 
@@ -47,9 +47,11 @@ class GpuBackend(Backend):
                  max_batch: int = 256, max_batch_tokens: int = 8192, ready: bool = True, use_fabric: bool = True,
                  tp_group=None, model_path: str = "", seed: int = 0, use_multimem: bool = False, copy_ctas: int = 128,
                  fused_tp: bool = True, precapture: bool = False, eos_token: Optional[int] = None,
-                 tokenizer_path: str = ""):
+                 tokenizer_path: str = "", kv_bits: int = 16, kv_group: int = 32):
         self.rank, self.world, self.tp = rank, world, tp
         self.cfg = get_config(model)
+        if kv_bits == 4 and (self.cfg.family == "hybrid" or tp > 1):
+            raise ValueError(f"{self.cfg.name}: a 4-bit cache is for uniform models on one GPU")
         self.eos_token = self.cfg.eos_token if eos_token is None else int(eos_token)
         self.stopper = StopSequences.from_tokenizer_file(tokenizer_path)
         self.model, self.model_path = model, model_path
@@ -64,8 +66,7 @@ class GpuBackend(Backend):
             self.page_bytes = self.cfg.kv_bytes_per_token(tp, 2) * page_size
             self.kv_layer_stride, kv_bytes = 0, 256
         else:
-            kvh = self.cfg.kv_heads // tp
-            self.page_bytes = 2 * page_size * kvh * self.cfg.head_dim * 2
+            self.page_bytes = kv_page_bytes(self.cfg, page_size, tp, kv_bits, kv_group)
             self.kv_layer_stride = num_pages * self.page_bytes
             kv_bytes = self.cfg.layers * self.kv_layer_stride
         self.slot_bytes = max_batch_tokens * self.cfg.hidden * 2
@@ -95,7 +96,8 @@ class GpuBackend(Backend):
                              max_batch_tokens=max_batch_tokens, tp=tp, tp_rank=rank % tp, dtype=dt, comm=comm,
                              seg_buffer=seg_buf, kv_buffer=kv_buf, ready=ready and not from_checkpoint, seed=seed,
                              fused_tp=fused_tp, tp_contexts=5 if tp > 1 else 1,     # context 0 + one per live-execution slot
-                             state_slots=2 * max_batch)                             # a full decode batch and a prefill batch
+                             state_slots=2 * max_batch,                             # a full decode batch and a prefill batch
+                             kv_bits=kv_bits, kv_group=kv_group)
         if from_checkpoint:
             self.engine.load_checkpoint(model)
         self.units = [(n, o, b) for n, o, b in self.engine.seg.layout.units]

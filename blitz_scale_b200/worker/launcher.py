@@ -41,6 +41,10 @@ def parse_args(argv=None):
     ap.add_argument("-A", "--activation-slots", type=int, default=4)
     ap.add_argument("--num-total-blocks", type=int, default=4096)
     ap.add_argument("--page-size", type=int, default=64)
+    ap.add_argument("--kv-bits", type=int, default=16, choices=[16, 4], help="bits of cached keys and values (4: uniform models on one GPU "
+                    "per replica; every replica of a cluster the same)")
+    ap.add_argument("--kv-group", type=int, default=32, choices=[32, 64, 128], help="dimensions of a head that share a scale and an offset "
+                    "in a 4-bit cache")
     ap.add_argument("--max-batch-size", type=int, default=256)
     ap.add_argument("--max-batch-tokens", type=int, default=8192)
     ap.add_argument("--log-dir", default="")
@@ -106,7 +110,7 @@ def main(argv=None) -> int:
                          max_batch=a.max_batch_size, max_batch_tokens=a.max_batch_tokens,
                          ready=states[rank] != "Inactive", tp_group=tp_group, model_path=a.model_path,
                          seed=0, use_multimem=a.multimem, fused_tp=not a.no_fused_tp, precapture=a.precapture_graphs,
-                         eos_token=a.eos_token_id, tokenizer_path=a.tokenizer)
+                         eos_token=a.eos_token_id, tokenizer_path=a.tokenizer, kv_bits=a.kv_bits, kv_group=a.kv_group)
     urls = [f"{a.host}:{a.port + r}" for r in range(world)]
 
     async def run():

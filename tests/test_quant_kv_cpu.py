@@ -88,3 +88,46 @@ def test_attention_refused():
             ops.attn_prefill_paged(q, good, t, **{**base, "work": work, **more})
     with pytest.raises(ValueError, match="current CUDA device"):
         ops.attn_prefill_paged(q, good, t, work, **base)
+
+
+def test_rotation_refused():
+    good, qkv, t = _pool(), torch.zeros(3, 8 * 64, dtype=torch.bfloat16), torch.zeros(3, dtype=torch.int32)
+    base = dict(q_heads=4, kv_heads=2, head_dim=64, page_size=16, rope_theta=1e4)
+    for more in (dict(kv_heads=1), dict(head_dim=128), dict(page_size=64), dict(q_heads=3), dict(rope_theta=0.0), dict(rope_theta=float("nan"))):
+        with pytest.raises(ValueError):
+            ops.rope_kv_store(qkv, t, t, good, **{**base, **more})
+    for bad in (qkv.t(), qkv[:, ::2], torch.zeros(6, 512, dtype=torch.bfloat16)[::2]):
+        with pytest.raises(ValueError):
+            ops.rope_kv_store(bad, t, t, good, **base)
+    with pytest.raises(TypeError):
+        ops.rope_kv_store(qkv.float(), t, t, good, **base)
+    for pos, slot in ((t[:2], t), (t, t[:2]), (t.long(), t)):
+        with pytest.raises(ValueError):
+            ops.rope_kv_store(qkv, pos, slot, good, **base)
+    with pytest.raises(ValueError, match="current CUDA device"):
+        ops.rope_kv_store(qkv, t, t, good, **base)
+
+
+def test_bytes_of_a_page():
+    from blitz_scale_b200.models.config import get_config
+    from blitz_scale_b200.runtime.engine import kv_page_bytes
+    c = get_config("llama3_8b")
+    assert kv_page_bytes(c, 64) == 2 * 64 * 8 * 128 * 2 and kv_page_bytes(c, 64, tp=2) == 64 * 8 * 128 * 2
+    # a token of a head: 64 bytes of codes and four pairs of 16-bit numbers, of its key and of its value
+    assert kv_page_bytes(c, 64, kv_bits=4, kv_group=32) == 64 * 8 * 2 * (64 + 16)
+    assert kv_page_bytes(c, 16, kv_bits=4, kv_group=128) == 16 * 8 * 2 * (64 + 4)
+    pool = ops.quant_kv_pool(3, 64, 8, 128, 64, device="cpu")
+    assert pool.pool[0].numel() == kv_page_bytes(c, 64, kv_bits=4, kv_group=64) and pool.kv_heads == 8 and pool.page_size == 64
+    for more in (dict(kv_bits=8), dict(kv_bits=4, kv_group=16), dict(kv_bits=4, page_size=8)):
+        with pytest.raises(ValueError):
+            kv_page_bytes(c, more.pop("page_size", 64), **more)
+
+
+def test_engines_that_take_no_4_bit_cache():
+    from blitz_scale_b200.runtime.engine import Engine
+    cpu = torch.device("cpu")
+    with pytest.raises(ValueError, match="16 or 4 bits"):
+        Engine("tiny", num_pages=4, device=cpu, kv_bits=8)
+    for model, more in (("fafudra_tiny", {}), ("tiny", dict(tp=2))):
+        with pytest.raises(ValueError, match="uniform models on one GPU"):
+            Engine(model, num_pages=4, device=cpu, kv_bits=4, **more)
