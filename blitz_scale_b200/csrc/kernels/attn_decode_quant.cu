@@ -818,14 +818,20 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
       if (inside) continue;
 
       // ------------------------------------------------------------ pieces of several blocks: for each head, whoever is last adds them up
-      const int c0 = cut.range(it.start) / warps, blocks = static_cast<int>(cut.range(it.stop - 1) / warps) - c0 + 1;
+      // (a ticket counts chunks; which blocks have them is worked out while it is on its way)
       __syncwarp();
-      bool is_last = false;
-      if (h0 + lane * each < p.rep) {
-        unsigned* ticket = p.tickets + (it.b * p.heads + it.head) * p.rep + h0 + lane * each;
+      const unsigned have = min(it.stop, X1) - max(it.start, X0);
+      const bool asks = h0 + lane * each < p.rep;
+      unsigned* const ticket = p.tickets + (it.b * p.heads + it.head) * p.rep + h0 + lane * each;
+      unsigned before = 0;
+      if (asks) {
         __threadfence();
-        is_last = atomicAdd(ticket, 1u) == static_cast<unsigned>(blocks - 1);
-        if (is_last) *ticket = 0u;
+        before = atomicAdd(ticket, have);
+      }
+      const int c0 = cut.range(it.start) / warps, blocks = static_cast<int>(cut.range(it.stop - 1) / warps) - c0 + 1;
+      const bool is_last = asks && before + have == it.stop - it.start;
+      if (is_last) {
+        *ticket = 0u;
         __threadfence();
       }
       __syncwarp();
@@ -851,8 +857,24 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
         }
         for (int c = 0; c < blocks; c += 32) {
           const int n = min(32, blocks - c);
-          float f[H];
+          float f[H], ahead[UNROLL][H][C];  // (the first pieces are asked for beside what they are worth)
           float2 ml[H];
+#pragma unroll
+          for (int v = 0; v < UNROLL; ++v)
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+              const float* o = from[h] + static_cast<int64_t>(max(0, 2 * (c + v) - 1)) * p.rep * D;
+              if (v >= n) {
+#pragma unroll
+                for (int i = 0; i < C; ++i) ahead[v][h][i] = 0.f;
+              } else if (C == 4) {
+                const float4 t = __ldcg(reinterpret_cast<const float4*>(o));
+                ahead[v][h][0] = t.x; ahead[v][h][1] = t.y; ahead[v][h][2 % C] = t.z; ahead[v][h][3 % C] = t.w;
+              } else {
+                const float2 t = __ldcg(reinterpret_cast<const float2*>(o));
+                ahead[v][h][0] = t.x; ahead[v][h][1] = t.y;
+              }
+            }
 #pragma unroll
           for (int h = 0; h < H; ++h) ml[h] = lane < n ? __ldcg(ml_from[h] + max(0, 2 * (c + lane) - 1) * p.rep) : make_float2(-INFINITY, 0.f);
 #pragma unroll
@@ -864,8 +886,17 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
 #pragma unroll
             for (int i = 0; i < C; ++i) acc[h][i] *= a;
           }
+#pragma unroll
+          for (int v = 0; v < UNROLL; ++v)
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+              const float fv = __shfl_sync(0xffffffffu, f[h], v);
+#pragma unroll
+              for (int i = 0; i < C; ++i)
+                if (v < n) acc[h][i] = fmaf(fv, ahead[v][h][i], acc[h][i]);
+            }
 #pragma unroll UNROLL
-          for (int v = 0; v < n; ++v) {
+          for (int v = UNROLL; v < n; ++v) {
             const int64_t at = static_cast<int64_t>(max(0, 2 * (c + v) - 1)) * p.rep * D;
 #pragma unroll
             for (int h = 0; h < H; ++h) four(from[h] + at, __shfl_sync(0xffffffffu, f[h], v), acc[h], true);

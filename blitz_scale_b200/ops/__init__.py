@@ -453,11 +453,14 @@ def attn_decode_workspace_bytes(batch: int, q_heads: int, value_dim: int, num_sp
     return int(lib().blitz_attn_decode_workspace_bytes(batch, q_heads, value_dim, num_splits))
 
 
+_QUANT_BLOCK = {(dim, group): 16 * (dim + 8 * (dim // group)) for dim in (64, 128) for group in (32, 64, 128) if group <= dim}
+
+
 def quant_kv_block_bytes(dim: int, group: int) -> int:
     """Bytes of 16 tokens of one head in a 4-bit cache, keys and values."""
-    if dim not in (64, 128) or group not in (32, 64, 128) or group > dim:
+    if (dim, group) not in _QUANT_BLOCK:
         raise ValueError(f"a 4-bit cache takes heads of 64 or 128 dimensions in groups of 32, 64 or 128 of them, got {dim} in groups of {group}")
-    return 16 * (dim + 8 * (dim // group))
+    return _QUANT_BLOCK[dim, group]
 
 
 def quant_kv_pool(pages: int, page_size: int, kv_heads: int, dim: int, group: int = 32, device="cuda") -> QuantKV:
@@ -470,12 +473,13 @@ def quant_kv_pool(pages: int, page_size: int, kv_heads: int, dim: int, group: in
 def _quant(cache: QuantKV, *others: Optional[torch.Tensor]) -> torch.Tensor:
     """The pool of a 4-bit cache, after checks of it and of what a call brings beside it (None: nothing)."""
     pool, dim, group = cache
-    shape = pool.shape
-    if pool.dtype != torch.uint8 or len(shape) != 4 or not pool.is_contiguous() or shape[3] != quant_kv_block_bytes(dim, group) or pool.data_ptr() & 15:
+    shape, at = pool.shape, pool.get_device()
+    if len(shape) != 4 or shape[3] != _QUANT_BLOCK.get((dim, group)) or pool.dtype is not torch.uint8 or not pool.is_contiguous() or pool.data_ptr() & 15:
+        quant_kv_block_bytes(dim, group)
         raise ValueError(f"not a 4-bit cache of heads of {dim} in groups of {group}: {tuple(shape)} {pool.dtype}")
-    if shape[2] < 1 or shape[2] & (shape[2] - 1):
-        raise ValueError(f"pages of a 4-bit cache hold 16 tokens times a power of two, got {16 * shape[2]}")
-    at = pool.get_device()
+    blocks = shape[2]
+    if blocks < 1 or blocks & (blocks - 1):
+        raise ValueError(f"pages of a 4-bit cache hold 16 tokens times a power of two, got {16 * blocks}")
     if at < 0 or at != _raw_device():
         raise ValueError(f"a cache on {pool.device}: the kernels run on the current CUDA device")
     for t in others:
@@ -484,20 +488,21 @@ def _quant(cache: QuantKV, *others: Optional[torch.Tensor]) -> torch.Tensor:
     return pool
 
 
-def _quant_rows(x: torch.Tensor, cache: QuantKV, what: str) -> None:
+def _quant_rows(x: torch.Tensor, H: int, D: int, what: str) -> None:
     """Rows [T, kv_heads * dim] (or [T, kv_heads, dim]) of keys or values in 16 bits, with any pitch of whole 16 bytes."""
+    shape, step = x.shape, x.stride()
+    n = len(shape)
     if x.dtype not in _DT:
         raise TypeError(f"{what}: kernels take fp16/bf16 tensors, got {x.dtype}")
-    H, D = cache.pool.shape[1], cache.dim
-    shape, step = x.shape, x.stride()
-    if len(shape) == 2 and (shape[1] != H * D or step[1] != 1) or len(shape) == 3 and (shape[1:] != (H, D) or step[1:] != (D, 1)) or len(shape) not in (2, 3):
+    if not (n == 2 and shape[1] == H * D and step[1] == 1 or n == 3 and shape[1] == H and shape[2] == D and step[1] == D and step[2] == 1):
         raise ValueError(f"{what}: rows of {H} heads of {D} dimensions, got {tuple(shape)} with strides {step}")
-    if step[0] & 7 or x.data_ptr() & 15:
+    if (step[0] | x.data_ptr() >> 1) & 7:
         raise ValueError(f"{what}: rows have to start on 16-byte boundaries")
 
 
 def _int32(t: torch.Tensor, n: Optional[int], what: str) -> torch.Tensor:
-    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or (n and t.shape[0] < n):
+    shape = t.shape
+    if len(shape) != 1 or t.dtype is not torch.int32 or not t.is_contiguous() or (n and shape[0] < n):
         raise ValueError(f"{what}: {'' if n is None else f'at least {n} '}int32 numbers, got {tuple(t.shape)} {t.dtype}")
     return t
 
@@ -505,15 +510,17 @@ def _int32(t: torch.Tensor, n: Optional[int], what: str) -> torch.Tensor:
 def quant_kv_store(k: torch.Tensor, v: torch.Tensor, slot: torch.Tensor, cache: QuantKV) -> None:
     """Quantise rows of (rotated) keys and values into a 4-bit cache.  ``k``, ``v``: [T, kv_heads * dim] in 16 bits, e.g. column ranges of
     the fused projection; ``slot`` [T]: page * page_size + offset (negative: the row is not written).  Each slot once in a call."""
-    pool = _quant(cache, k, v, slot)
-    T, shape = k.shape[0], pool.shape
-    _quant_rows(k, cache, "k")
-    _quant_rows(v, cache, "v")
-    if v.shape[0] != T or v.dtype != k.dtype:
-        raise ValueError(f"as many values as keys, of their type: {tuple(v.shape)} {v.dtype} beside {tuple(k.shape)} {k.dtype}")
+    pool, D, group = cache
+    _quant(cache, k, v, slot)
+    pages, H, blocks, _ = pool.shape
+    _quant_rows(k, H, D, "k")
+    _quant_rows(v, H, D, "v")
+    T, dt = k.shape[0], k.dtype
+    if v.shape[0] != T or v.dtype is not dt:
+        raise ValueError(f"as many values as keys, of their type: {tuple(v.shape)} {v.dtype} beside {tuple(k.shape)} {dt}")
     _int32(slot, T, "slot")
-    rc = lib().blitz_quant_kv_store(k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), slot.data_ptr(), pool.data_ptr(), T, shape[1], cache.dim,
-                                    cache.group, 16 * shape[2], shape[0], _status_ptr(k), _DT[k.dtype], _stream())
+    rc = lib().blitz_quant_kv_store(k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), slot.data_ptr(), pool.data_ptr(), T, H, D, group, 16 * blocks, pages,
+                                    _status_ptr(pool), _DT[dt], _stream())
     if rc:
         _check(rc, "blitz_quant_kv_store")
 
@@ -544,9 +551,11 @@ def quant_kv_load(cache: QuantKV, slot: torch.Tensor, *, dtype: torch.dtype = to
     pool, D, group = cache
     _int32(slot, None, "slot")
     n, (pages, H, blocks, _) = slot.shape[0], pool.shape
-    if k is None:
-        k = torch.empty((n, H, D), dtype=dtype, device=pool.device)
-    if v is None:
+    if k is None and v is None:
+        k, v = torch.empty((2, n, H, D), dtype=dtype, device=pool.device).unbind()
+    elif k is None:
+        k = torch.empty((n, H, D), dtype=v.dtype, device=pool.device)
+    elif v is None:
         v = torch.empty((n, H, D), dtype=k.dtype, device=pool.device)
     for t in (k, v):
         if t.shape != (n, H, D) or not t.is_contiguous() or t.dtype != k.dtype or t.data_ptr() & 15:
@@ -585,52 +594,55 @@ def quant_attn_workspace_bytes(batch: int, q_heads: int, head_dim: int, device=N
 
 
 def _quant_attn(q: torch.Tensor, rows: int, cache: QuantKV, q_heads: int, kv_heads: int, head_dim: int, page_size: int, window: int, keep_first: int,
-                softcap: float, sink: Optional[torch.Tensor], out: Optional[torch.Tensor], refused: dict, *others: Optional[torch.Tensor]) -> torch.Tensor:
+                softcap: float, sink: Optional[torch.Tensor], out: Optional[torch.Tensor], *others: Optional[torch.Tensor]) -> torch.Tensor:
     """Checks of an attention call over a 4-bit cache; returns where its output goes."""
-    for name, x in refused.items():
-        if x is not None and x is not False:
-            raise ValueError(f"attention over a 4-bit cache has no {name}")
-    dt, D, shape = q.dtype, cache.dim, cache.pool.shape
+    dt, D, shape, width = q.dtype, cache.dim, cache.pool.shape, q_heads * head_dim
     if dt not in _DT:
         raise TypeError(f"kernels take fp16/bf16 tensors, got {dt}")
-    if kv_heads != shape[1] or head_dim != D or page_size != 16 * shape[2] or q_heads < 1 or q_heads % kv_heads:
-        raise ValueError(f"{q_heads} query and {kv_heads} KV heads of {head_dim}, pages of {page_size}: the 4-bit cache has {shape[1]} "
-                         f"heads of {D}, pages of {16 * shape[2]}")
-    if q.dim() != 2 or q.shape[0] < rows or q.shape[1] < q_heads * D or q.stride(1) != 1 or q.stride(0) & 7 or q.data_ptr() & 15:
-        raise ValueError(f"q: {rows} rows of {q_heads} heads of {D} dimensions that start on 16-byte boundaries, got {tuple(q.shape)}, strides {q.stride()}")
+    if head_dim != D or len(shape) != 4 or kv_heads != shape[1] or page_size != 16 * shape[2] or q_heads < 1 or q_heads % kv_heads:
+        raise ValueError(f"{q_heads} query and {kv_heads} KV heads of {head_dim}, pages of {page_size}: the 4-bit cache has heads of {D}, {tuple(shape)}")
+    size, step = q.shape, q.stride()
+    if len(size) != 2 or size[0] < rows or size[1] < width or step[1] != 1 or (step[0] | q.data_ptr() >> 1) & 7:
+        raise ValueError(f"q: {rows} rows of {q_heads} heads of {D} dimensions that start on 16-byte boundaries, got {tuple(size)}, strides {step}")
     if window < 0 or keep_first < 0 or not softcap >= 0.0:
         raise ValueError(f"window {window}, keep_first {keep_first}, softcap {softcap}")
-    if sink is not None and (sink.dtype != dt or sink.numel() != q_heads or not sink.is_contiguous()):
+    if sink is not None and (sink.dtype is not dt or sink.numel() != q_heads or not sink.is_contiguous()):
         raise ValueError(f"sink: {q_heads} numbers of {dt}")
     if out is None:
-        out = torch.empty((rows, q_heads * D), dtype=dt, device=q.device)
-    elif out.dim() != 2 or out.shape[0] < rows or out.shape[1] < q_heads * D or out.dtype != dt or out.stride(1) != 1 or out.stride(0) & 7 or out.data_ptr() & 15:
-        raise ValueError(f"out: {rows} rows of {q_heads * D} {dt} that start on 16-byte boundaries, got {tuple(out.shape)} {out.dtype}")
+        out = torch.empty((rows, width), dtype=dt, device=q.device)
+    else:
+        size, step = out.shape, out.stride()
+        if len(size) != 2 or size[0] < rows or size[1] < width or out.dtype is not dt or step[1] != 1 or (step[0] | out.data_ptr() >> 1) & 7:
+            raise ValueError(f"out: {rows} rows of {width} {dt} that start on 16-byte boundaries, got {tuple(size)} {out.dtype}")
     _quant(cache, q, out, sink, *others)
     return out
 
 
+def _quant_refuses(gate, bias, chunked, sigmoid) -> None:
+    if gate is not None or bias is not None or chunked or sigmoid:
+        raise ValueError("attention over a 4-bit cache has no gate, bias, chunked windows or sigmoid weights")
+
+
 def _attn_decode_quant(q, cache, indices, indptr, last_page_len, q_heads, kv_heads, head_dim, page_size, num_splits, workspace, out, sm_scale,
-                       window, keep_first, softcap, sink, refused, static_table):
+                       window, keep_first, softcap, sink, static_table):
     _int32(indptr, 1, "indptr")
     B = indptr.shape[0] - 1
     _int32(last_page_len, B, "last_page_len")
     _int32(indices, None, "indices")
     if num_splits < 0:
         raise ValueError(f"num_splits {num_splits}")
-    out = _quant_attn(q, B, cache, q_heads, kv_heads, head_dim, page_size, window, keep_first, softcap, sink, out, refused, indices, indptr, last_page_len,
-                      workspace)
+    out = _quant_attn(q, B, cache, q_heads, kv_heads, head_dim, page_size, window, keep_first, softcap, sink, out, indices, indptr, last_page_len, workspace)
     if B == 0:
         return out
     if workspace is None:
         workspace = torch.zeros(quant_attn_workspace_bytes(B, q_heads, head_dim), dtype=torch.uint8, device=q.device)
-    elif workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.data_ptr() & 255:
+    elif workspace.dtype is not torch.uint8 or not workspace.is_contiguous() or workspace.data_ptr() & 255:
         raise ValueError(f"workspace: bytes that start on a 256-byte boundary, got {workspace.dtype}")
     pool, size = cache.pool, workspace.numel()
     rc = lib().blitz_attn_decode_quant(q.data_ptr(), q.stride(0), pool.data_ptr(), indices.data_ptr(), indptr.data_ptr(), last_page_len.data_ptr(),
                                        out.data_ptr(), out.stride(0), workspace.data_ptr(), size, B, q_heads, kv_heads, head_dim, cache.group, page_size,
                                        pool.shape[0], head_dim ** -0.5 if sm_scale is None else sm_scale, window, keep_first, softcap,
-                                       None if sink is None else sink.data_ptr(), 1 if static_table else 0, _status_ptr(q), _DT[q.dtype], _stream())
+                                       None if sink is None else sink.data_ptr(), 1 if static_table else 0, _status_ptr(pool), _DT[q.dtype], _stream())
     if rc:
         need = quant_attn_workspace_bytes(B, q_heads, head_dim)
         if size < need:
@@ -639,8 +651,7 @@ def _attn_decode_quant(q, cache, indices, indptr, last_page_len, q_heads, kv_hea
     return out
 
 
-def _attn_portion_quant(q, cache, page_indices, work, q_heads, kv_heads, head_dim, page_size, out, sm_scale, window, keep_first, softcap, sink, refused,
-                        skip_pages):
+def _attn_portion_quant(q, cache, page_indices, work, q_heads, kv_heads, head_dim, page_size, out, sm_scale, window, keep_first, softcap, sink, skip_pages):
     _int32(page_indices, None, "page_indices")
     P = page_indices.shape[0]
     if not 0 <= skip_pages <= P:
@@ -648,7 +659,7 @@ def _attn_portion_quant(q, cache, page_indices, work, q_heads, kv_heads, head_di
     if work.dtype != torch.int32 or work.dim() != 2 or work.shape[1] != 8 or not work.is_contiguous() or work.data_ptr() & 15:
         raise ValueError(f"work: records of prefill_work_list, got {tuple(work.shape)} {work.dtype}")
     T, entries, n = q.shape[0], work.shape[0], P - skip_pages
-    out = _quant_attn(q, T, cache, q_heads, kv_heads, head_dim, page_size, window, keep_first, softcap, sink, out, refused, page_indices, work)
+    out = _quant_attn(q, T, cache, q_heads, kv_heads, head_dim, page_size, window, keep_first, softcap, sink, out, page_indices, work)
     if entries == 0 or T == 0 or n == 0:
         return out
     L, pool, dt, status, stream = lib(), cache.pool, _DT[q.dtype], _status_ptr(q), _stream()
@@ -691,8 +702,9 @@ def attn_decode(q: torch.Tensor, kv_layer: KVLayer, indices: torch.Tensor, indpt
     ``sigmoid``; the keys of all sequences are always taken in equal shares, whatever ``num_splits``, and ``workspace`` has the size of
     `quant_attn_workspace_bytes`."""
     if isinstance(kv_layer, QuantKV):
+        _quant_refuses(gate, bias, chunked, sigmoid)
         return _attn_decode_quant(q, kv_layer, indices, indptr, last_page_len, q_heads, kv_heads, head_dim, page_size, num_splits, workspace, out, sm_scale,
-                                  window, keep_first, softcap, sink, dict(gate=gate, bias=bias, chunked=chunked, sigmoid=sigmoid), static_table)
+                                  window, keep_first, softcap, sink, static_table)
     B = indptr.numel() - 1
     kp, vp, page_rows, pages, vdim = _kv(kv_layer)
     if out is None:
@@ -757,8 +769,9 @@ def attn_prefill_paged(q: torch.Tensor, kv_layer: KVLayer, page_indices: torch.T
     fp16, with its queries, scaled so that the type's range does not matter); tokens behind a sequence's end may hold anything; no gate,
     bias, ``chunked`` or ``sigmoid``; no record of ``work`` refers to the first ``skip_pages`` entries of ``page_indices``."""
     if isinstance(kv_layer, QuantKV):
+        _quant_refuses(gate, bias, chunked, sigmoid)
         return _attn_portion_quant(q, kv_layer, page_indices, work, q_heads, kv_heads, head_dim, page_size, out, sm_scale, window, keep_first, softcap, sink,
-                                   dict(gate=gate, bias=bias, chunked=chunked, sigmoid=sigmoid), skip_pages)
+                                   skip_pages)
     T = q.shape[0]
     kp, vp, page_rows, pages, vdim = _kv(kv_layer)
     if out is None:

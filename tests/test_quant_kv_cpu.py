@@ -45,10 +45,10 @@ def test_caches_and_rows_refused():
         ops.quant_kv_store(k, k, slot, good)
     for bad in (k.float(), k.double()):
         with pytest.raises(TypeError):
-            ops._quant_rows(bad, good, "k")
+            ops._quant_rows(bad, 2, 64, "k")
     for bad in (k[:, :64], k.t(), k[:, 1:], torch.zeros(3, 132, dtype=torch.bfloat16)[:, :128], k.view(3, 4, 32), k.flatten()):
         with pytest.raises(ValueError):
-            ops._quant_rows(bad, good, "k")
+            ops._quant_rows(bad, 2, 64, "k")
     for bad, n in ((slot.long(), 3), (slot, 4), (slot[::2], 1), (slot.view(1, 3), 3)):
         with pytest.raises(ValueError):
             ops._int32(bad, n, "slot")
