@@ -7,12 +7,12 @@
 //   q.k = sum_g s_g (sum_{d in g} q_d c_d) + z_g (sum_{d in g} q_d)
 //   o_d = sum_j (p_j s_j) (c_jd - 8) + sum_j p_j (z_j + 8 s_j)
 //
-// A code becomes an fp16 number by one mask and one "or" into the mantissa of a power of two, which adds a constant, 1024 or 64: a word
-// of 8 codes takes five instructions.  For keys the constants' part of the product is the accumulator's initial value, for values a product
-// of a constant matrix with the same weights takes it off again, and 8 with it (the codes around zero, so that the rounding of p_j s_j is not
-// amplified by what cancels).  Queries enter in fp16, a head divided by a power of two near its largest entry: bf16 and fp16 numbers are
-// exact there (next to the largest, that is), and so are their products with codes.  Weights times scales are rounded to fp16, times a power of
-// two that brings the largest scale so far to 2^6 .. 2^7: 2^-11 of each down to scales 2^-20 of the largest, less below.  The part of z_j stays in 32
+// A code, or 16 times one, is an fp16 number as its bits stand in a half's low byte: a denormal, c 2^-24, which the tensor cores multiply like any
+// other.  A word of 8 codes takes five instructions and no constant has to come off again.  Queries enter in fp16, a head divided by a power of
+// two that brings its largest entry to 2^14 .. 2^15 (2^10 .. 2^11 for what meets 16 times a code): bf16 and fp16 numbers are exact there down to
+// 2^-24 of the largest, and so are their products with codes.  Weights times scales are rounded to fp16, times a power of two that brings the
+// largest scale so far to 2^6 .. 2^7: 2^-11 of each down to scales 2^-20 of the largest, less below.  Their product with -8, one more matrix
+// product a group, makes the codes lie around zero, so that this rounding is not amplified by what cancels.  The part of z_j + 8 s_j stays in 32
 // bits; the sums of q_d z_g in the scores are one more product, in bf16, of z as stored with sums of q in two numbers.
 //
 // The maximum that weights refer to follows the scores only when they pass it by 2^8 (fp16 has room for that): nearly every chunk finds
@@ -24,7 +24,8 @@
 // halves of the groups (HALVES): lanes of columns 0..3 handle the scales of the first half of the groups, the others those of the second.
 //
 // A warp takes chunks of 32 tokens by itself, through a ring of stages of its own; one more warp issues the copies (bulk copies: a
-// head's tokens in a page are one contiguous piece), a lane for each of the others.
+// head's tokens in a page are one contiguous piece), a lane for each of the others.  Eleven warps have 168 registers each and none
+// spills; fifteen with 128 measured 43.4 us where these take 40.4 (256 sequences of 513 tokens, 32 query heads over 8, groups of 32).
 //
 // The chunks of all sequences of all heads, end to end, are cut into equal ranges, one per warp of the GPU, so that neither lengths nor the
 // number of sequences leave warps idle.  A sequence that is cut leaves its pieces' sums in shared memory, where the warps that end with it
@@ -40,10 +41,7 @@
 
 namespace blitz {
 
-#ifndef QDW
-#define QDW 15
-#endif
-constexpr int kQdWarps = QDW, kQdThreads = (kQdWarps + 1) * 32;
+constexpr int kQdWarps = 11, kQdThreads = (kQdWarps + 1) * 32;
 constexpr int kQdChunk = 32;
 constexpr int kQdMaxBatch = 1024;   // sequences of a launch
 constexpr int kQdMaxStages = 4;
@@ -60,7 +58,7 @@ struct DecodeQuantParams {
   float* part;         // [2 blocks][rep][D] sums, then [2 blocks][rep] of (maximum, sum of weights)
   int batch, kv_heads, heads, div, rep;  // heads: groups of at most 8 query heads, div of which share a KV head; rep: query heads of one
   int page_size, page_shift, max_pages, stages, static_table;
-  float scale_log2, cap_scale, cap_log2;
+  float sign, scale_log2, cap_scale, cap_log2;  // the scale's sign (0, NaN: itself) goes into the queries, its magnitude into the factors
   int window, keep_first;
   const void* sink;
   int* status;
@@ -166,11 +164,10 @@ __device__ __forceinline__ bool qd_wait(const volatile int* word, bool counts, v
   return true;
 }
 
-// d = a b + (c0, c1, c0, c1)
-__device__ __forceinline__ void qd_mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float c0, float c1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+__device__ __forceinline__ void qd_mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ void qd_mma_f16_add(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -433,7 +430,7 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
       const QdSeen see = qd_seen(p, tab.len[it.b]);
       // queries: word w of a lane's key codes holds dimensions 32 w + 8 t4 .. + 7, pairs (i, i + 4) of which are a register's halves
       uint32_t qb[W][4], zb0, zb1 = 0;
-      float qc[N][2], scale[2];
+      float scale[2];
       {
         const int hq = HALVES ? g & 3 : g, xq = HALVES ? g >> 2 : 0;  // head and half of column g
         float v[W][8], most = 0.f;
@@ -454,32 +451,25 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
         // 2^-e with most in [2^e, 2^(e + 1)); an all-zero head, and one that is not finite, as it is
         const int e = most > 0.f && most <= 3.4e38f ? max(-126, min(126, static_cast<int>(__float_as_uint(most) >> 23) - 127)) : 0;
         const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23), up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-        float sum[G], zero[N];
+        const float turn = down * p.sign;
+        float sum[G];
 #pragma unroll
         for (int i = 0; i < G; ++i) sum[i] = 0.f;
 #pragma unroll
-        for (int i = 0; i < N; ++i) zero[i] = 0.f;
-#pragma unroll
         for (int w = 0; w < W; ++w) {
           const bool mine = !HALVES || (w / WG) / N == xq;
-          float r[8];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            qb[w][i] = mine ? pk2<__half>(v[w][i] * down, v[w][i + 4] * down) : 0u;
+          for (int i = 0; i < 4; ++i) {  // (odd pairs meet codes times 16)
+            const float by = i & 1 ? 1024.f : 16384.f, back = i & 1 ? 0x1p-20f : 0x1p-24f;
+            qb[w][i] = mine ? pk2<__half>(v[w][i] * turn * by, v[w][i + 4] * turn * by) : 0u;
             const float2 f = cvt2<__half>(qb[w][i]);  // (as they enter the products)
-            r[i] = f.x;
-            r[i + 4] = f.y;
+            sum[w / WG] += (f.x + f.y) * back;
           }
-          // the zero of a register's codes: 1024 in the first and third pair, 64 in the others
-          sum[w / WG] += ((r[0] + r[4]) + (r[1] + r[5])) + ((r[2] + r[6]) + (r[3] + r[7]));
-          zero[(w / WG) % N] -= 1024.f * ((r[0] + r[4]) + (r[2] + r[6])) + 64.f * ((r[1] + r[5]) + (r[3] + r[7]));
         }
 #pragma unroll
         for (int d = 1; d < 4; d <<= 1) {
 #pragma unroll
           for (int i = 0; i < G; ++i) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], d);
-#pragma unroll
-          for (int i = 0; i < N; ++i) zero[i] += __shfl_xor_sync(0xffffffffu, zero[i], d);
         }
         float hi[G], lo[G];
 #pragma unroll
@@ -496,18 +486,16 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
         // what the lane's own columns need
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          scale[k] = __shfl_sync(0xffffffffu, up, (2 * t4 + k) * 4) * (p.cap_log2 > 0.f ? p.cap_scale : p.scale_log2);
-#pragma unroll
-          for (int i = 0; i < N; ++i) qc[i][k] = __shfl_sync(0xffffffffu, zero[i], (2 * t4 + k) * 4);
+          scale[k] = fmaxf(0x1p-126f, __shfl_sync(0xffffffffu, up, (2 * t4 + k) * 4) * (1024.f * (p.cap_log2 > 0.f ? p.cap_scale : p.scale_log2)));
         }
       }
 
       // `down` takes scales to 16 bits, `most` is the largest one that it is good for
-      float o[MT][4], zs[N][2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, down = 1.f, most = 0.f;
+      float o[MT][4], eight[N][4], zs[N][2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, down = 1.f, most = 0.f;
 #pragma unroll
       for (int i = 0; i < MT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 #pragma unroll
-      for (int i = 0; i < N; ++i) zs[i][0] = zs[i][1] = 0.f;
+      for (int i = 0; i < N; ++i) zs[i][0] = zs[i][1] = eight[i][0] = eight[i][1] = eight[i][2] = eight[i][3] = 0.f;
 
       for (int c = it.beg; c < it.end; ++c) {
         if (ok && !__all_sync(0xffffffffu, ptx::bounded_mbar_wait(&my_full[stage], phase, abort_flag))) {
@@ -545,13 +533,10 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
           for (int w = 0; w < W; ++w) {
             const int i = (w / WG) % N;
             const uint32_t a = ku[w], b = kv[w], ah = a >> 8, bh = b >> 8;
-            const uint32_t a0 = quant_kv_pick<0x000f000fu, 0x64006400u>(a), a1 = quant_kv_pick<0x000f000fu, 0x64006400u>(b);
-            const uint32_t a2 = quant_kv_pick<0x00f000f0u, 0x54005400u>(a), a3 = quant_kv_pick<0x00f000f0u, 0x54005400u>(b);
-            const uint32_t c0 = quant_kv_pick<0x000f000fu, 0x64006400u>(ah), c1 = quant_kv_pick<0x000f000fu, 0x64006400u>(bh);
-            const uint32_t c2 = quant_kv_pick<0x00f000f0u, 0x54005400u>(ah), c3 = quant_kv_pick<0x00f000f0u, 0x54005400u>(bh);
-            if (w % WG == 0 && w / WG < N) qd_mma_f16(acc[i], a0, a1, a2, a3, qb[w][0], qb[w][1], qc[i][0], qc[i][1]);
-            else qd_mma_f16_add(acc[i], a0, a1, a2, a3, qb[w][0], qb[w][1]);
-            qd_mma_f16_add(acc[i], c0, c1, c2, c3, qb[w][2], qb[w][3]);
+            const uint32_t even = 0x000f000fu, odd = 0x00f000f0u;
+            if (w % WG == 0 && w / WG < N) qd_mma_f16(acc[i], a & even, b & even, a & odd, b & odd, qb[w][0], qb[w][1]);
+            else qd_mma_f16_add(acc[i], a & even, b & even, a & odd, b & odd, qb[w][0], qb[w][1]);
+            qd_mma_f16_add(acc[i], ah & even, bh & even, ah & odd, bh & odd, qb[w][2], qb[w][3]);
           }
 #pragma unroll
           for (int i = 0; i < N; ++i) {
@@ -565,13 +550,12 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
             for (int i = 0; i < 4; ++i) s[u][i] += __shfl_xor_sync(0xffffffffu, s[u][i], 2);
           }
         }
-        // scores in log2 units; what is not visible has none (bit 2 u + (0: token tau, 1: tau + 2) of `seen`)
+        // scores in log2 units are these times a factor, which the maximum and the exponent's argument take in
+        float by[2] = {scale[0], scale[1]};
         if (p.cap_log2 > 0.f) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) s[i >> 2][i & 3] = p.cap_log2 * ptx::tanh_ex2(s[i >> 2][i & 3] * scale[i & 1]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) s[i >> 2][i & 3] *= scale[i & 1];
+          by[0] = by[1] = 1.f;
         }
         QdScales<G, HALVES> f[4];  // of the values of tokens tau, tau + 2, 16 + tau, 18 + tau
 #pragma unroll
@@ -589,7 +573,7 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
         float top[2] = {s[0][0], s[0][1]}, wide = fmaxf(fmaxf(f[0].largest(), f[1].largest()), fmaxf(f[2].largest(), f[3].largest()));
 #pragma unroll
         for (int i = 2; i < 8; ++i) top[i & 1] = fmaxf(top[i & 1], s[i >> 2][i & 3]);
-        if (__any_sync(0xffffffffu, top[0] > m[0] + 8.f || top[1] > m[1] + 8.f || wide > most)) {
+        if (__any_sync(0xffffffffu, top[0] * by[0] > m[0] + 8.f || top[1] * by[1] > m[1] + 8.f || wide > most)) {
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) {
             top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], d));
@@ -606,6 +590,7 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
           }
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
+            top[k] *= by[k];
             a[k] = top[k] > m[k] ? ptx::ex2_approx(m[k] - top[k]) : 1.f;
             m[k] = fmaxf(m[k], top[k]);
             l[k] *= a[k];
@@ -617,11 +602,15 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
           for (int i = 0; i < MT; ++i) {
             o[i][0] *= a[0]; o[i][1] *= a[1]; o[i][2] *= a[0]; o[i][3] *= a[1];
           }
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            eight[i][0] *= a[0]; eight[i][1] *= a[1]; eight[i][2] *= a[0]; eight[i][3] *= a[1];
+          }
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           float& v = s[i >> 2][i & 3];
-          v = ptx::ex2_approx(v - m[i & 1]);  // (a chunk has a visible key, whose score m has seen: zero for what is not visible)
+          v = ptx::ex2_approx(fmaf(v, by[i & 1], -m[i & 1]));  // (a chunk has a visible key, whose score m has seen: zero for what is not visible)
           l[i & 1] += v;
         }
 #pragma unroll
@@ -635,22 +624,40 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
             vw[4 * h] = v.x; vw[4 * h + 1] = v.y; vw[4 * h + 2] = v.z; vw[4 * h + 3] = v.w;
           }
           uint32_t b0[N], b1[N];
+          if constexpr (N == 1) {
+            const float sa = fa.s[0] * down, sb = fb.s[0] * down;
+            zs[0][0] = fmaf(s[u][0], fa.mid[0], fmaf(s[u][2], fb.mid[0], zs[0][0]));
+            zs[0][1] = fmaf(s[u][1], fa.mid[0], fmaf(s[u][3], fb.mid[0], zs[0][1]));
+            b0[0] = qd_transposed(pk2<__half>(s[u][0] * sa, s[u][1] * sa));
+            b1[0] = qd_transposed(pk2<__half>(s[u][2] * sb, s[u][3] * sb));
+          } else {  // two groups an instruction
+            const uint64_t down2 = ptx::f32x2(down, down);
+            const uint64_t w0 = ptx::f32x2(s[u][0], s[u][0]), w1 = ptx::f32x2(s[u][1], s[u][1]), w2 = ptx::f32x2(s[u][2], s[u][2]), w3 = ptx::f32x2(s[u][3], s[u][3]);
 #pragma unroll
-          for (int i = 0; i < N; ++i) {
-            const float sa = fa.s[i] * down, sb = fb.s[i] * down;
-            zs[i][0] = fmaf(s[u][0], fa.mid[i], fmaf(s[u][2], fb.mid[i], zs[i][0]));
-            zs[i][1] = fmaf(s[u][1], fa.mid[i], fmaf(s[u][3], fb.mid[i], zs[i][1]));
-            b0[i] = qd_transposed(pk2<__half>(s[u][0] * sa, s[u][1] * sa));
-            b1[i] = qd_transposed(pk2<__half>(s[u][2] * sb, s[u][3] * sb));
+            for (int i = 0; i < N; i += 2) {
+              const uint64_t sa = ptx::mul_f32x2(ptx::f32x2(fa.s[i], fa.s[(i + 1) % N]), down2), sb = ptx::mul_f32x2(ptx::f32x2(fb.s[i], fb.s[(i + 1) % N]), down2);
+              const uint64_t ma = ptx::f32x2(fa.mid[i], fa.mid[(i + 1) % N]), mb = ptx::f32x2(fb.mid[i], fb.mid[(i + 1) % N]);
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const float2 z = ptx::f32x2_get(ptx::fma_f32x2(k ? w1 : w0, ma, ptx::fma_f32x2(k ? w3 : w2, mb, ptx::f32x2(zs[i][k], zs[(i + 1) % N][k]))));
+                zs[i][k] = z.x;
+                zs[(i + 1) % N][k] = z.y;
+              }
+              const float2 p0 = ptx::f32x2_get(ptx::mul_f32x2(w0, sa)), p1 = ptx::f32x2_get(ptx::mul_f32x2(w1, sa));
+              const float2 p2 = ptx::f32x2_get(ptx::mul_f32x2(w2, sb)), p3 = ptx::f32x2_get(ptx::mul_f32x2(w3, sb));
+              b0[i] = qd_transposed(pk2<__half>(p0.x, p1.x));
+              b1[i] = qd_transposed(pk2<__half>(p2.x, p3.x));
+              b0[(i + 1) % N] = qd_transposed(pk2<__half>(p0.y, p1.y));
+              b1[(i + 1) % N] = qd_transposed(pk2<__half>(p2.y, p3.y));
+            }
           }
+#pragma unroll
+          for (int i = 0; i < N; ++i) qd_mma_f16_add(eight[i], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, b0[i], b1[i]);  // -8, -8 times 16
 #pragma unroll
           for (int i = 0; i < MT; ++i) {
             const int j = (i * 16 / GROUP) % N;
-            const uint32_t v = vw[i], vh = v >> 8;
-            const uint32_t a0 = quant_kv_pick<0x000f000fu, 0x64006400u>(v), a1 = quant_kv_pick<0x00f000f0u, 0x54005400u>(v);
-            const uint32_t a2 = quant_kv_pick<0x000f000fu, 0x64006400u>(vh), a3 = quant_kv_pick<0x00f000f0u, 0x54005400u>(vh);
-            qd_mma_f16_add(o[i], 0xe408e408u, 0xd480d480u, 0xe408e408u, 0xd480d480u, b0[j], b1[j]);  // -1032, -72
-            qd_mma_f16_add(o[i], a0, a1, a2, a3, b0[j], b1[j]);
+            const uint32_t v = vw[i], vh = v >> 8, even = 0x000f000fu, odd = 0x00f000f0u;
+            qd_mma_f16_add(o[i], v & even, v & odd, vh & even, vh & odd, b0[j], b1[j]);
           }
         }
         __syncwarp();  // every lane has read the stage
@@ -676,8 +683,8 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         const int j = (i * 16 / GROUP) % N;
-        o[i][0] = fmaf(o[i][0], up, zs[j][0]); o[i][1] = fmaf(o[i][1], up, zs[j][1]);
-        o[i][2] = fmaf(o[i][2], up, zs[j][0]); o[i][3] = fmaf(o[i][3], up, zs[j][1]);
+        o[i][0] = fmaf((o[i][0] + eight[j][0]) * 0x1p24f, up, zs[j][0]); o[i][1] = fmaf((o[i][1] + eight[j][1]) * 0x1p24f, up, zs[j][1]);
+        o[i][2] = fmaf((o[i][2] + eight[j][2]) * 0x1p20f, up, zs[j][0]); o[i][3] = fmaf((o[i][3] + eight[j][3]) * 0x1p20f, up, zs[j][1]);
       }
       const unsigned X0 = cut.begin(first_warp), X1 = cut.begin(first_warp + warps), x0 = cut.begin(first_warp + warp), x1 = cut.begin(first_warp + warp + 1);
       if (it.start >= x0 && it.stop <= x1) {
@@ -970,7 +977,9 @@ int blitz_attn_decode_quant(const void* q, int64_t q_stride, const void* pool, c
   p.part = (float*)((char*)workspace + ((int64_t)batch * q_heads * 4 + 255) / 256 * 256);
   p.page_size = page_size; p.max_pages = max_pages; p.page_shift = 0; p.stages = 2;
   while ((1 << p.page_shift) < page_size) ++p.page_shift;
-  p.scale_log2 = sm_scale * 1.4426950408889634f; p.cap_scale = softcap > 0.f ? sm_scale / softcap : 0.f; p.cap_log2 = softcap * 1.4426950408889634f;
+  const float size = sm_scale < 0.f ? -sm_scale : sm_scale > 0.f ? sm_scale : 1.f;
+  p.sign = sm_scale < 0.f ? -1.f : sm_scale > 0.f ? 1.f : sm_scale;
+  p.scale_log2 = size * 1.4426950408889634f; p.cap_scale = softcap > 0.f ? size / softcap : 0.f; p.cap_log2 = softcap * 1.4426950408889634f;
   p.window = window; p.keep_first = keep_first; p.sink = sink; p.static_table = static_table; p.status = status;
   for (int b = 0; b < batch; b += kQdMaxBatch) {
     p.batch = batch - b < kQdMaxBatch ? batch - b : kQdMaxBatch;

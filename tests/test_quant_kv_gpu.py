@@ -217,6 +217,28 @@ def test_decode(ops, case, dt, splits):
         assert worst <= 1, (s, n, worst)
 
 
+@pytest.mark.parametrize("rep", [4, 8])
+@pytest.mark.parametrize("scale", [-0.11, 0.0, 0.07])
+@pytest.mark.parametrize("softcap", [0.0, 3.0])
+def test_decode_scales(ops, rep, scale, softcap):
+    """A factor of either sign, or zero; queries and factor times powers of two that cancel change no bit."""
+    lens, H, D, group, dt = [300, 1, 2000], 2, 128, 32, torch.bfloat16
+    cache, table, indptr, last, kept = filled(ops, lens, H, D, group, 64, dt, 7)
+    q = torch.randn(len(lens), rep * H, D, generator=torch.Generator().manual_seed(3)).to(dt)
+    run = lambda q, scale: ops.attn_decode(q.flatten(1).to(DEV), cache, table, indptr, last, q_heads=rep * H, kv_heads=H, head_dim=D, page_size=64,
+                                           num_splits=0, sm_scale=scale, softcap=softcap).cpu()
+    got = run(q, scale)
+    for s, n in enumerate(lens):
+        k, v, ks, kz, vs = kept[s]
+        want = attention(q[s:s + 1], k, v, torch.tensor([n - 1]), scale=scale, softcap=softcap)
+        spread = attention(q[s:s + 1], k, 8 * vs.repeat_interleave(group, -1), torch.tensor([n - 1]), scale=scale, softcap=softcap)[0]
+        step = 2.0 ** -11 + 2.0 ** -15 + n / 16 * 2.0 ** -22
+        tol = tolerance(q[s:s + 1], kept[s], abs(scale), want, spread, step, dt, group) + n * 2.0 ** -28 * vs.max()
+        assert ((got[s].double().view(-1, D) - want[0][0]).abs() <= tol[0]).all(), (s, n)
+    for e in (-100, -30, 30, 100):
+        assert torch.equal(run((q.float() * 2.0 ** e).to(dt), scale * 2.0 ** -e), got), e
+
+
 # (tokens cached before, rows) of every sequence
 PORTIONS = [
     ([(0, 1)], 4, 2, 128, 32, 64, {}),
