@@ -50,9 +50,9 @@
 // neighbours share a reciprocal, 1 / a = b (c d) / (a b c d), unless a product of some four leaves the range of fp32 (one vote per
 // half a block).
 //
-// Operands in fp16 for a bf16 model (IO: the type of sink and output): queries, keys and values were divided by powers of two (a row's of a
-// head, a KV head's) so that fp16 holds them, which a row's scale and its output's factor make up for; a 4-bit cache read back for a
-// pass comes so (quant_kv.cu).
+// Operands in fp16 for a bf16 model (IO: the type of queries, sink and output): keys and values were divided by powers of two (a KV head's) so
+// that fp16 holds them, and each thread turns its row of queries into fp16 in shared memory, divided by a power of two near the row's
+// largest entry, as an item begins.  The row's scale and the output's factor make up for both.  A 4-bit cache read back for a pass comes so (quant_kv.cu).
 //
 // Replaces FlashInfer's BatchPrefillWithRaggedKVCacheWrapper / paged wrapper calls and their host Plan()
 // (src/kernel/attention_prefill.cu:11-45, src/kernel/flashinfer_types.cu:24-49).
@@ -60,6 +60,7 @@
 #include "ptx.cuh"
 #include "tmap.cuh"
 #include "common.cuh"
+#include "quant_kv.cuh"
 #include <cmath>
 
 namespace blitz {
@@ -85,7 +86,7 @@ struct PagedPrefillParams {
   const void* sink;           // EXT: [q_heads] in the activation type, or null
   const void* bias;           // BIAS: [q_heads][bias_len] in the activation type (SIG: [q_heads], or null)
   int bias_len;
-  const float *q_up, *kv_up;  // IO: powers of two taken out of queries [tokens][q_heads], and of keys and values [2][kv_heads]
+  const float* kv_up;         // IO: powers of two taken out of keys and values [2][kv_heads]
   int* status;
   long long* trace;  // profiling aid (null in production): clock stamps of CTA 0's first item, see the set_trace call
 };
@@ -168,17 +169,18 @@ attn_prefill_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
   uint8_t* sK = sQ + 2 * TB;     // [2 stages]
   uint8_t* sV = sK + 2 * TB;     // [2 stages]
   uint64_t* bars = reinterpret_cast<uint64_t*>(sV + 2 * VB);
-  uint64_t* q_full = bars;        // once per item
-  uint64_t* q_empty = bars + 1;   // once per item: its last S products are done
-  uint64_t* k_full = bars + 2;    // [2] per block
-  uint64_t* k_empty = bars + 4;   // [2]
-  uint64_t* v_full = bars + 6;    // [2]
-  uint64_t* v_empty = bars + 8;   // [2]
-  uint64_t* s_full = bars + 10;   // [2] per tile and block
-  uint64_t* p_ready = bars + 12;  // [2]
-  uint64_t* o_full = bars + 14;   // [2]
-  uint64_t* o_free = bars + 16;   // [2] per tile and item: the warpgroup has read its output rows
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
+  uint64_t* q_full = bars;        // [2] per tile and item
+  uint64_t* q_empty = bars + 2;   // once per item: its last S products are done
+  uint64_t* k_full = bars + 3;    // [2] per block
+  uint64_t* k_empty = bars + 5;   // [2]
+  uint64_t* v_full = bars + 7;    // [2]
+  uint64_t* v_empty = bars + 9;   // [2]
+  uint64_t* s_full = bars + 11;   // [2] per tile and block
+  uint64_t* p_ready = bars + 13;  // [2]
+  uint64_t* o_full = bars + 15;   // [2]
+  uint64_t* o_free = bars + 17;   // [2] per tile and item: the warpgroup has read its output rows
+  uint64_t* q_fp16 = bars + 19;   // [2] per tile and item, IO: the warpgroup has turned its queries into fp16
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 21);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float* s_bias = reinterpret_cast<float*>(sV + 2 * VB + C::kBarBytes);  // BIAS only
 
@@ -186,9 +188,10 @@ attn_prefill_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
   const int total = p.entries * p.q_heads;
 
   if (threadIdx.x == 0) {
-    ptx::mbar_init(q_full, 1);
     ptx::mbar_init(q_empty, 1);
     for (int i = 0; i < 2; ++i) {
+      ptx::mbar_init(&q_full[i], 1);
+      ptx::mbar_init(&q_fp16[i], 128);
       ptx::mbar_init(&k_full[i], 1);
       ptx::mbar_init(&k_empty[i], 1);
       ptx::mbar_init(&v_full[i], 1);
@@ -250,11 +253,21 @@ attn_prefill_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
       if (n_items > 0) ok = wait(q_empty, (n_items - 1) & 1);  // the previous item's S products have read Q
       if (!ok) break;
       if (lane == 0) {
-        ptx::mbar_expect_tx(q_full, it.nt * TB);
-        for (int t = 0; t < it.nt; ++t)
+        for (int t = 0; t < 2; ++t) {
+          if (it.nblk_t[t] == 0) continue;
+          ptx::mbar_expect_tx(&q_full[t], TB);
 #pragma unroll
           for (int s = 0; s < C::kSlabs; ++s)
-            ptx::tma_load_3d(sQ + t * TB + s * SB, &tmap_q, q_full, s * 64, it.head, it.seq_start + it.q0 + t * kPpTile);
+            ptx::tma_load_3d(sQ + t * TB + s * SB, &tmap_q, &q_full[t], s * 64, it.head, it.seq_start + it.q0 + t * kPpTile);
+        }
+      }
+      if constexpr (SCALED) {  // the next item's queries into L2: what brings them to fp16 waits for them
+        const int next = (r + 1) * static_cast<int>(gridDim.x) < total ? pp_index(r + 1, total) : -1;
+        if (next >= 0 && lane < 2 * C::kSlabs) {
+          const PpItem n = pp_item<EXT>(p, next);
+          const int t = lane / C::kSlabs;
+          if (n.nblk_t[t] > 0) ptx::tma_prefetch_3d(&tmap_q, lane % C::kSlabs * 64, n.head, n.seq_start + n.q0 + t * kPpTile);
+        }
       }
       int row = box_row(it, 0);
       for (int j = 0; j < it.nblk && ok; ++j, ++g) {
@@ -309,12 +322,18 @@ attn_prefill_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
         const PpItem it = pp_item<EXT>(p, idx);
         const int nb0 = it.nblk_t[0], nb1 = it.nblk_t[1], nblk = it.nblk;
         const bool tr = n_items == 0 && blockIdx.x == 0;
-        ok = wait(q_full, n_items & 1) && wait(&k_full[g & 1], (g >> 1) & 1);
+        uint64_t* const q_there = SCALED ? q_fp16 : q_full;
+        ok = (nb0 == 0 || wait(&q_there[0], outs0 & 1)) && wait(&k_full[g & 1], (g >> 1) & 1);
         if (!ok) break;
         ptx::tc_fence_after_sync();
         // S of the first block: the tiles' score columns are free (their last P of the previous item was waited for)
-        issue_S(0, g & 1);
-        if (nb1 > 0) issue_S(1, g & 1);
+        if (nb0 > 0) issue_S(0, g & 1);
+        if (nb1 > 0) {
+          ok = wait(&q_there[1], outs1 & 1);
+          if (!ok) break;
+          ptx::tc_fence_after_sync();
+          issue_S(1, g & 1);
+        }
         ptx::umma_commit(&k_empty[g & 1]);
         if (nblk == 1) ptx::umma_commit(q_empty);
         for (int j = 0; j < nblk && ok; ++j) {
@@ -351,7 +370,7 @@ attn_prefill_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
         }
         cnt0 += nb0;
         cnt1 += nb1;
-        outs0 += 1;
+        outs0 += nb0 > 0 ? 1 : 0;
         outs1 += nb1 > 0 ? 1 : 0;
         g += nblk;
         ++n_items;
@@ -368,6 +387,7 @@ attn_prefill_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
     bool ok = true;
     uint32_t cnt = 0;  // blocks this tile has been through
     bool first = true;
+    uint32_t items = 0;  // that have the tile
     for (int r = 0; r * static_cast<int>(gridDim.x) < total && ok; ++r) {
       const int idx = pp_index(r, total);
       if (idx < 0) continue;
@@ -381,7 +401,15 @@ attn_prefill_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
       const int chunk_from = EXT && p.chunked ? limit - limit % p.window : -1;  // first key of the row's chunk
       float m_ref = 0.f, l = 0.f;
       float row_up = 1.f;
-      if constexpr (SCALED) row_up = q_idx < it.q_len ? p.q_up[static_cast<int64_t>(it.seq_start + q_idx) * p.q_heads + it.head] * p.kv_up[it.kv_head] : 0.f;
+      if constexpr (SCALED) {
+        if (!ptx::bounded_mbar_wait(&q_full[t], items++ & 1, abort_flag)) {
+          ok = false;
+          break;
+        }
+        row_up = quant_kv_row_fp16<C::kSlabs>(sQ + t * TB + r_ * 128, SB, r_ & 7) * p.kv_up[it.kv_head];
+        ptx::fence_proxy_async_smem();
+        ptx::mbar_arrive(&q_fp16[t]);
+      }
       auto scale_log2 = [&]() { return SCALED ? p.scale_log2 * row_up : p.scale_log2; };
       auto cap_scale = [&]() { return SCALED ? p.cap_scale * row_up : p.cap_scale; };
       const float sig_bias = SIG && p.bias ? -1.4426950408889634f * to_f<T>(reinterpret_cast<const T*>(p.bias)[it.head]) : 0.f;
@@ -690,7 +718,7 @@ static int prefill_paged(const void* q, int64_t q_stride, const void* k_pool, co
                              const int32_t* page_indices, const int32_t* work, int entries, int num_tokens,
                              int q_heads, int kv_heads, int dim, int vdim, int page_size, int page_rows, int max_pages,
                              float sm_scale, int flags, int window, int keep_first, int chunked, int sigmoid, float softcap, const void* sink,
-                             const void* bias, int bias_len, const void* gate, int64_t gate_stride, const float* q_up, const float* kv_up, int* status,
+                             const void* bias, int bias_len, const void* gate, int64_t gate_stride, const float* kv_up, int* status,
                              int dtype, cudaStream_t stream) {
   if (num_tokens <= 0 || entries <= 0) return 0;
   if (dim < 8 || dim > 128 || (dim & 7) || vdim < 8 || vdim > 128 || (vdim & 7)) return -1;
@@ -715,7 +743,7 @@ static int prefill_paged(const void* q, int64_t q_stride, const void* k_pool, co
   p.q_heads = q_heads; p.kv_heads = kv_heads; p.page_size = page_size; p.box_tokens = bt;
   p.oob_row = (int)rows;
   p.scale_log2 = sm_scale * 1.4426950408889634f; p.status = status; p.trace = g_pp_trace;
-  p.chunked = chunked; p.q_up = q_up; p.kv_up = kv_up;
+  p.chunked = chunked; p.kv_up = kv_up;
   p.window = window; p.keep_first = keep_first; p.sink = sink; p.bias = bias; p.bias_len = bias_len;
   p.cap_scale = softcap > 0.f ? sm_scale / softcap : 0.f; p.cap_log2 = softcap * 1.4426950408889634f;
   // tanh(z) = z (k0 + k1 z^2 + k2 z^4 + k3 z^6) for |z| <= 0.5 (Chebyshev interpolation of tanh(z) / z in z^2, absolute
@@ -748,7 +776,7 @@ static int prefill_paged(const void* q, int64_t q_stride, const void* k_pool, co
     if (poly) return sized(type, yes, no, no, no);
     return sized(type, no, no, no, no);
   };
-  if (q_up != nullptr) {
+  if (kv_up != nullptr) {
     if (dim != vdim || (dim != 64 && dim != 128)) return -1;
     auto scaled = [&](auto ext_) {
       constexpr bool X = decltype(ext_)::value;
@@ -767,19 +795,18 @@ int blitz_attn_prefill_paged(const void* q, int64_t q_stride, const void* k_pool
                              const void* bias, int bias_len, const void* gate, int64_t gate_stride, int* status, int dtype, cudaStream_t stream) {
   return prefill_paged(q, q_stride, k_pool, v_pool, out, out_stride, page_indices, work, entries, num_tokens, q_heads, kv_heads, dim, vdim, page_size,
                        page_rows, max_pages, sm_scale, flags, window, keep_first, chunked, sigmoid, softcap, sink, bias, bias_len, gate, gate_stride,
-                       nullptr, nullptr, status, dtype, stream);
+                       nullptr, status, dtype, stream);
 }
 
-// The same for a bf16 model (sink and out) with operands in fp16: q [num_tokens][q_heads * dim] was multiplied by 1 / q_up [num_tokens][q_heads],
-// keys and values by 1 / kv_up [2][kv_heads], powers of two.  dim 64 or 128.
-int blitz_attn_prefill_scaled(const void* q, const void* k_pool, const void* v_pool, void* out, int64_t out_stride, const int32_t* page_indices,
-                              const int32_t* work, int entries, int num_tokens, int q_heads, int kv_heads, int dim, int page_size, int page_rows,
-                              int max_pages, float sm_scale, int window, int keep_first, float softcap, const void* sink, const float* q_up,
+// The same for a bf16 model (q, sink and out) with keys and values in fp16, which were multiplied by 1 / kv_up [2][kv_heads], powers of two.
+// dim 64 or 128.
+int blitz_attn_prefill_scaled(const void* q, int64_t q_stride, const void* k_pool, const void* v_pool, void* out, int64_t out_stride,
+                              const int32_t* page_indices, const int32_t* work, int entries, int num_tokens, int q_heads, int kv_heads, int dim,
+                              int page_size, int page_rows, int max_pages, float sm_scale, int window, int keep_first, float softcap, const void* sink,
                               const float* kv_up, int* status, cudaStream_t stream) {
-  if (q_up == nullptr || kv_up == nullptr) return -1;
-  return prefill_paged(q, (int64_t)q_heads * dim, k_pool, v_pool, out, out_stride, page_indices, work, entries, num_tokens, q_heads, kv_heads, dim, dim,
-                       page_size, page_rows, max_pages, sm_scale, 0, window, keep_first, 0, 0, softcap, sink, nullptr, 0, nullptr, 0, q_up, kv_up, status, 0,
-                       stream);
+  if (kv_up == nullptr) return -1;
+  return prefill_paged(q, q_stride, k_pool, v_pool, out, out_stride, page_indices, work, entries, num_tokens, q_heads, kv_heads, dim, dim, page_size,
+                       page_rows, max_pages, sm_scale, 0, window, keep_first, 0, 0, softcap, sink, nullptr, 0, nullptr, 0, kv_up, status, 0, stream);
 }
 
 }  // extern "C"

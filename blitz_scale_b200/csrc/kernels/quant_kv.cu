@@ -365,6 +365,7 @@ __global__ void __launch_bounds__(256) quant_kv_load_kernel(const QuantLoadParam
 }
 
 // ------------------------------------------------------------------ pages back
+constexpr int kQuantSpanBlocks = 256;
 struct QuantPagesParams {
   const uint8_t* pool;
   const int32_t* pages;
@@ -376,15 +377,9 @@ struct QuantPagesParams {
   const int32_t* work;
   int entries, first;
   int32_t* table;     // numbers of the pages read back, for all of those that the records count
-  const float* spans; // SCALED: [span_blocks][2][kv_heads] largest magnitudes
+  const float* spans; // SCALED: [2][kv_heads][kQuantSpanBlocks] largest magnitudes, by block
   int span_blocks;
   float* up;          // SCALED: [2][kv_heads] powers of two that were taken out of keys and values
-  // ... and its queries: [tokens][q_heads * dim] to fp16, and a power of two for each row of a head
-  const void* q;
-  void* q_to;
-  float* q_up;
-  int64_t q_row;
-  int tokens, q_heads;
 };
 
 // Tokens of page `n` (counted as the records do) that its sequence has, -1: no record has it.  The whole warp asks.
@@ -396,49 +391,8 @@ __device__ __forceinline__ int quant_kv_held(const QuantPagesParams& p, int n) {
   }
   return __reduce_max_sync(0xffffffffu, held);
 }
-// 2^-e, 2^e <= x < 2^(e + 1): what brings numbers up to x to below 2
-__device__ __forceinline__ float quant_kv_down(float x) {
-  const int e = x > 0.f && x <= 3.4e38f ? max(-100, min(126, static_cast<int>(__float_as_uint(x) >> 23) - 127)) : 0;
-  return __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-}
-
-// Queries to fp16: D / 8 lanes a row of a head, four rows at a time (bound by memory: 64 bytes a thread on their way).
-template <int D>
-__device__ __forceinline__ void quant_kv_queries(const QuantPagesParams& p, int block, int blocks) {
-  constexpr int LANES = D / 8, ROWS = 256 / LANES, U = 4;
-  const int64_t all = static_cast<int64_t>(p.tokens) * p.q_heads;
-  const int l = threadIdx.x % LANES;
-  for (int64_t r0 = static_cast<int64_t>(block) * ROWS * U; r0 < all; r0 += static_cast<int64_t>(blocks) * ROWS * U) {
-    uint4 raw[U];
-    int64_t r[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      r[u] = r0 + u * ROWS + threadIdx.x / LANES;
-      const int64_t t = r[u] / p.q_heads;
-      const int h = static_cast<int>(r[u] - t * p.q_heads);
-      raw[u] = r[u] < all ? ld_nc16(reinterpret_cast<const __nv_bfloat16*>(p.q) + t * p.q_row + static_cast<int64_t>(h) * D + l * 8) : make_uint4(0, 0, 0, 0);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float x[8], most = 0.f;
-      unpack8<__nv_bfloat16>(raw[u], x);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(x[i]));
-#pragma unroll
-      for (int d = 1; d < LANES; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-      const float down = quant_kv_down(most);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] *= down;
-      if (r[u] < all) {
-        stf8<__half>(reinterpret_cast<__half*>(p.q_to) + r[u] * D + l * 8, x);
-        if (l == 0) p.q_up[r[u]] = 1.f / down;
-      }
-    }
-  }
-}
-
 // The largest magnitudes of a pass's keys and values, by head: of every block, a part of them.  Half a warp looks at the scales of the
-// keys of 16 tokens, the other half at those of the values.  The blocks behind those bring the queries to fp16 meanwhile.
+// keys of 16 tokens, the other half at those of the values.
 template <int D, int GROUP>
 __global__ void __launch_bounds__(256) quant_kv_span_kernel(const QuantPagesParams p, float* __restrict__ spans) {
   constexpr QuantKv F = quant_kv(D, GROUP);
@@ -447,10 +401,6 @@ __global__ void __launch_bounds__(256) quant_kv_span_kernel(const QuantPagesPara
   for (int i = threadIdx.x; i < 2 * p.kv_heads; i += blockDim.x) s_most[i] = 0;
   ptx::griddep_launch_dependents();
   ptx::griddep_wait();
-  if (static_cast<int>(blockIdx.x) >= p.span_blocks) {
-    quant_kv_queries<D>(p, blockIdx.x - p.span_blocks, gridDim.x - p.span_blocks);
-    return;
-  }
   __syncthreads();
   const int lane = threadIdx.x & 31, blocks = p.page_size >> 4;
   for (int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); unit < p.units; unit += static_cast<int64_t>(p.span_blocks) * 8) {
@@ -472,7 +422,7 @@ __global__ void __launch_bounds__(256) quant_kv_span_kernel(const QuantPagesPara
     if ((lane & 15) == 0) atomicMax(&s_most[(lane >> 4) * p.kv_heads + head], __float_as_int(most));
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < 2 * p.kv_heads; i += blockDim.x) spans[static_cast<int64_t>(blockIdx.x) * 2 * p.kv_heads + i] = __int_as_float(s_most[i]);
+  for (int i = threadIdx.x; i < 2 * p.kv_heads; i += blockDim.x) spans[i * kQuantSpanBlocks + blockIdx.x] = __int_as_float(s_most[i]);
 }
 
 // The codes of a warp's 16 tokens of a head, 8 x 8 blocks of (token, dimension) at a time as tensor-core fragments have them.
@@ -483,9 +433,9 @@ __device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t a, uin
 // stmatrix turns into rows of a token.  Both go out from shared memory, whole rows at a time.
 // Bound by the 16-bit rows that it writes (four times the codes).
 //
-// For attention of portions (WORK) the tokens behind a sequence's end are zeros, whatever the cache has there.  SCALED: queries, keys and
-// values of a bf16 model go to fp16, which keeps three bits more of what z + s c is: keys and values divided by a power of two near the
-// largest of their head, a row of queries by one near its own largest entry, so that the type's range does not matter.
+// For attention of portions (WORK) the tokens behind a sequence's end are zeros, whatever the cache has there.  SCALED: keys and
+// values of a bf16 model go to fp16, which keeps three bits more of what z + s c is, divided by a power of two near the largest of their head, so that
+// the type's range does not matter.
 template <typename T, int D, int GROUP, bool WORK, bool SCALED>
 __global__ void __launch_bounds__(256, 3) quant_kv_pages_kernel(const QuantPagesParams p) {
   constexpr QuantKv F = quant_kv(D, GROUP);
@@ -505,7 +455,9 @@ __global__ void __launch_bounds__(256, 3) quant_kv_pages_kernel(const QuantPages
   if (SCALED) {
     for (int i = warp; i < 2 * p.kv_heads; i += 8) {
       float most = 0.f;
-      for (int c = lane; c < p.span_blocks; c += 32) most = fmaxf(most, p.spans[static_cast<int64_t>(c) * 2 * p.kv_heads + i]);
+#pragma unroll
+      for (int c = 0; c < kQuantSpanBlocks; c += 32)
+        if (c + lane < p.span_blocks) most = fmaxf(most, p.spans[i * kQuantSpanBlocks + c + lane]);
       const float down = quant_kv_down(warp_max(most));
       if (lane == 0) {
         s_down[i] = down;
@@ -518,18 +470,9 @@ __global__ void __launch_bounds__(256, 3) quant_kv_pages_kernel(const QuantPages
     const int head = static_cast<int>(unit % p.kv_heads), b = static_cast<int>(unit / p.kv_heads % blocks);
     const int64_t n = unit / p.kv_heads / blocks;
     const int page = p.pages[n];
-    int held = p.page_size;
-    if (WORK) {
-      held = quant_kv_held(p, static_cast<int>(n) + p.first);
-      if (held < 0) continue;  // (no record has the page)
-    }
-    held -= b * 16;            // of these 16 tokens
+    const bool bad = page < 0 || page >= p.max_pages;  // (the first page is read instead, and nothing written)
     const float k_down = SCALED ? s_down[head] : 1.f, v_down = SCALED ? s_down[p.kv_heads + head] : 1.f;
-    if (page < 0 || page >= p.max_pages) {
-      if (p.status && lane == 0) atomicCAS(p.status, 0, kStatusBadIndex);
-      continue;
-    }
-    const uint8_t* block = p.pool + ((static_cast<int64_t>(page) * p.kv_heads + head) * blocks + b) * F.block;
+    const uint8_t* block = p.pool + ((static_cast<int64_t>(bad ? 0 : page) * p.kv_heads + head) * blocks + b) * F.block;
     const int64_t row0 = n * p.page_rows + b * 16, pitch = static_cast<int64_t>(p.kv_heads) * D;
     // everything is asked for before anything is used
     uint32_t kw[2][W], vw[D / 16];
@@ -567,6 +510,16 @@ __global__ void __launch_bounds__(256, 3) quant_kv_pages_kernel(const QuantPages
     for (int r = 0; r < 2; ++r) numbers(block + F.codes + (g + 8 * r) * 4 * G, ks[r]);
 #pragma unroll
     for (int j = 0; j < 4; ++j) numbers(block + F.part + F.codes + (4 * t4 + j) * 4 * G, vs[j]);
+    int held = p.page_size;
+    if (WORK) {
+      held = quant_kv_held(p, static_cast<int>(n) + p.first);
+      if (held < 0) continue;  // (no record has the page)
+    }
+    held -= b * 16;            // of these 16 tokens
+    if (bad) {
+      if (p.status && lane == 0) atomicCAS(p.status, 0, kStatusBadIndex);
+      continue;
+    }
     constexpr float most = quant_kv_most<T>();
     bool past = false;
     if (!SCALED)
@@ -669,7 +622,6 @@ struct PagesLaunch {
     return (int)launch_pdl(quant_kv_pages_kernel<T, D, GROUP, false, false>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, stream, p);
   }
 };
-constexpr int kQuantSpanBlocks = 128;
 struct PortionLaunch {
   QuantPagesParams& p;
   float* spans;
@@ -682,9 +634,7 @@ struct PortionLaunch {
       return (int)launch_pdl(quant_kv_pages_kernel<__half, D, GROUP, true, false>, dim3(page_blocks), dim3(256), 0, stream, p);
     p.spans = spans;
     p.span_blocks = (int)(blocks < kQuantSpanBlocks ? blocks : kQuantSpanBlocks);
-    const int64_t rows = ((int64_t)p.tokens * p.q_heads + 1024 / (D / 8) - 1) / (1024 / (D / 8));
-    const int rc = (int)launch_pdl(quant_kv_span_kernel<D, GROUP>, dim3((unsigned)(p.span_blocks + (rows < most ? rows : most))), dim3(256),
-                                   (size_t)2 * p.kv_heads * 4, stream, p, spans);
+    const int rc = (int)launch_pdl(quant_kv_span_kernel<D, GROUP>, dim3((unsigned)p.span_blocks), dim3(256), (size_t)2 * p.kv_heads * 4, stream, p, spans);
     if (rc) return rc;
     return (int)launch_pdl(quant_kv_pages_kernel<__half, D, GROUP, true, true>, dim3(page_blocks), dim3(256), 0, stream, p);
   }
@@ -741,36 +691,33 @@ int blitz_quant_kv_pages(const void* pool, const int32_t* pages, int64_t count, 
 }
 
 // Scratch of blitz_quant_kv_portion for `pages` pages and `first` more that the records count, in the order of its layout: keys and values read
-// back [pages][2][page_size][kv_heads][dim] in 16 bits, page numbers; of a bf16 model also queries [tokens][q_heads * dim] in fp16, their
-// powers of two, those of keys and values, the parts of their largest magnitudes.  offsets (may be null): where the 7 parts begin, and the end.
-int64_t blitz_quant_kv_portion_bytes(int64_t pages, int64_t first, int tokens, int q_heads, int kv_heads, int dim, int page_size, int dtype, int64_t* offsets) {
-  const int64_t q = dtype == 1 ? (int64_t)tokens * q_heads : 0, h = dtype == 1 ? 2 * (int64_t)kv_heads : 0;
-  const int64_t sizes[6] = {pages * 4 * page_size * kv_heads * dim, (pages + first) * 4, q * dim * 2, q * 4, h * 4, h * 4 * kQuantSpanBlocks};
+// back [pages][2][page_size][kv_heads][dim] in 16 bits, page numbers; of a bf16 model also the powers of two of keys and values, and the parts of
+// their largest magnitudes.  offsets (may be null): where the 4 parts begin, and the end.
+int64_t blitz_quant_kv_portion_bytes(int64_t pages, int64_t first, int kv_heads, int dim, int page_size, int dtype, int64_t* offsets) {
+  const int64_t h = dtype == 1 ? 2 * (int64_t)kv_heads : 0;
+  const int64_t sizes[4] = {pages * 4 * page_size * kv_heads * dim, (pages + first) * 4, h * 4, h * 4 * kQuantSpanBlocks};
   int64_t at = 0;
-  for (int i = 0; i < 6; ++i) {
+  for (int i = 0; i < 4; ++i) {
     if (offsets) offsets[i] = at;
     at += (sizes[i] + 255) / 256 * 256;
   }
-  if (offsets) offsets[6] = at;
+  if (offsets) offsets[4] = at;
   return at;
 }
 
 // What attention of portions (blitz_attn_prefill_paged, or blitz_attn_prefill_scaled for a bf16 model) reads instead of a 4-bit cache: pages[n], the
-// (first + n)-th page that the records of `work` count, in 16 bits, zeros behind the end of its sequence; of a bf16 model in fp16, and its queries.
-int blitz_quant_kv_portion(const void* q, int64_t q_row, const void* pool, const int32_t* pages, int64_t count, int64_t first, const int32_t* work,
-                           int entries, int tokens, int q_heads, int kv_heads, int dim, int group, int page_size, int max_pages, void* scratch,
-                           int* status, int dtype, cudaStream_t stream) {
-  if (count <= 0 || entries <= 0 || tokens <= 0) return 0;
-  if (!quant_kv_supported(dim, group, page_size) || kv_heads < 1 || kv_heads > 128 || (q_row & 7) || first < 0 || count + first > 0x7fffffff) return -1;
-  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(work) | reinterpret_cast<uintptr_t>(pool) | reinterpret_cast<uintptr_t>(scratch)) & 15) return -1;
-  int64_t at[7];
-  blitz_quant_kv_portion_bytes(count, first, tokens, q_heads, kv_heads, dim, page_size, dtype, at);
+// (first + n)-th page that the records of `work` count, in 16 bits (of a bf16 model: fp16), zeros behind the end of its sequence.
+int blitz_quant_kv_portion(const void* pool, const int32_t* pages, int64_t count, int64_t first, const int32_t* work, int entries, int kv_heads, int dim,
+                           int group, int page_size, int max_pages, void* scratch, int* status, int dtype, cudaStream_t stream) {
+  if (count <= 0 || entries <= 0) return 0;
+  if (!quant_kv_supported(dim, group, page_size) || kv_heads < 1 || kv_heads > 128 || first < 0 || count + first > 0x7fffffff) return -1;
+  if ((reinterpret_cast<uintptr_t>(work) | reinterpret_cast<uintptr_t>(pool) | reinterpret_cast<uintptr_t>(scratch)) & 15) return -1;
+  int64_t at[5];
+  blitz_quant_kv_portion_bytes(count, first, kv_heads, dim, page_size, dtype, at);
   char* s = (char*)scratch;
   QuantPagesParams p{(const uint8_t*)pool, pages, s, s + (int64_t)page_size * kv_heads * dim * 2, count * kv_heads * (page_size / 16), kv_heads, page_size, 2 * page_size, max_pages, status};
-  p.work = work; p.entries = entries; p.first = (int)first; p.table = (int32_t*)(s + at[1]);
-  p.q = q; p.q_row = q_row; p.tokens = tokens; p.q_heads = q_heads;
-  p.q_to = s + at[2]; p.q_up = (float*)(s + at[3]); p.up = (float*)(s + at[4]);
-  return quant_kv_dispatch(dtype, dim, group, PortionLaunch{p, (float*)(s + at[5]), stream});
+  p.work = work; p.entries = entries; p.first = (int)first; p.table = (int32_t*)(s + at[1]); p.up = (float*)(s + at[2]);
+  return quant_kv_dispatch(dtype, dim, group, PortionLaunch{p, (float*)(s + at[3]), stream});
 }
 
 }  // extern "C"

@@ -77,4 +77,33 @@ static inline int quant_kv_dispatch(int dtype, int dim, int group, F&& f) {
   return dtype == 1 ? sizes(__nv_bfloat16{}) : sizes(__half{});
 }
 
+// 2^-e, 2^e <= x < 2^(e + 1): what brings numbers up to x to below 2
+__device__ __forceinline__ float quant_kv_down(float x) {
+  const int e = x > 0.f && x <= 3.4e38f ? max(-100, min(126, static_cast<int>(__float_as_uint(x) >> 23) - 127)) : 0;
+  return __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+}
+
+// A row of bf16 numbers in a tile that TMA wrote with a 128-byte swizzle, to fp16 where it stands, divided by a power of two near the largest,
+// which it returns.  row: of the first slab of 64 columns, `slab` bytes from one to the next; x: which exclusive-or its 16-byte pieces are at (lanes
+// that have rows next to each other then read different banks).
+template <int SLABS>
+__device__ __forceinline__ float quant_kv_row_fp16(uint8_t* row, int slab, int x) {
+  __nv_bfloat162 most = __float2bfloat162_rn(0.f);
+#pragma unroll
+  for (int i = 0; i < SLABS * 8; ++i) {
+    const uint4 v = *reinterpret_cast<const uint4*>(row + (i >> 3) * slab + (((i & 7) ^ x) << 4));
+    const __nv_bfloat162* e = reinterpret_cast<const __nv_bfloat162*>(&v);
+    most = __hmax2(most, __hmax2(__hmax2(__habs2(e[0]), __habs2(e[1])), __hmax2(__habs2(e[2]), __habs2(e[3]))));
+  }
+  const float down = quant_kv_down(fmaxf(__low2float(most), __high2float(most)));
+#pragma unroll
+  for (int i = 0; i < SLABS * 8; ++i) {
+    uint4* const at = reinterpret_cast<uint4*>(row + (i >> 3) * slab + (((i & 7) ^ x) << 4));
+    const uint4 v = *at;
+    auto both = [&](uint32_t w) { return pk2<__half>(__uint_as_float(w << 16) * down, __uint_as_float(w & 0xffff0000u) * down); };
+    *at = make_uint4(both(v.x), both(v.y), both(v.z), both(v.w));
+  }
+  return 1.f / down;
+}
+
 }  // namespace blitz

@@ -663,17 +663,16 @@ def _attn_portion_quant(q, cache, page_indices, work, q_heads, kv_heads, head_di
     if entries == 0 or T == 0 or n == 0:
         return out
     L, pool, dt, status, stream = lib(), cache.pool, _DT[q.dtype], _status_ptr(q), _stream()
-    at = (ctypes.c_int64 * 7)()
-    scratch = torch.empty(L.blitz_quant_kv_portion_bytes(n, skip_pages, T, q_heads, kv_heads, head_dim, page_size, dt, at), dtype=torch.uint8, device=q.device)
+    at = (ctypes.c_int64 * 5)()
+    scratch = torch.empty(L.blitz_quant_kv_portion_bytes(n, skip_pages, kv_heads, head_dim, page_size, dt, at), dtype=torch.uint8, device=q.device)
     base = scratch.data_ptr()
-    _check(L.blitz_quant_kv_portion(q.data_ptr(), q.stride(0), pool.data_ptr(), page_indices.data_ptr() + 4 * skip_pages, n, skip_pages, work.data_ptr(),
-                                    entries, T, q_heads, kv_heads, head_dim, cache.group, page_size, pool.shape[0], base, status, dt, stream),
-           "blitz_quant_kv_portion")
+    _check(L.blitz_quant_kv_portion(pool.data_ptr(), page_indices.data_ptr() + 4 * skip_pages, n, skip_pages, work.data_ptr(), entries, kv_heads,
+                                    head_dim, cache.group, page_size, pool.shape[0], base, status, dt, stream), "blitz_quant_kv_portion")
     scale, values, snk = head_dim ** -0.5 if sm_scale is None else sm_scale, base + 2 * page_size * kv_heads * head_dim, None if sink is None else sink.data_ptr()
     if dt == 1:
-        _check(L.blitz_attn_prefill_scaled(base + at[2], base, values, out.data_ptr(), out.stride(0), base + at[1], work.data_ptr(), entries, T, q_heads,
-                                           kv_heads, head_dim, page_size, 2 * page_size, n, scale, window, keep_first, softcap, snk, base + at[3],
-                                           base + at[4], status, stream), "blitz_attn_prefill_scaled")
+        _check(L.blitz_attn_prefill_scaled(q.data_ptr(), q.stride(0), base, values, out.data_ptr(), out.stride(0), base + at[1], work.data_ptr(), entries,
+                                           T, q_heads, kv_heads, head_dim, page_size, 2 * page_size, n, scale, window, keep_first, softcap, snk,
+                                           base + at[2], status, stream), "blitz_attn_prefill_scaled")
     else:
         _check(L.blitz_attn_prefill_paged(q.data_ptr(), q.stride(0), base, values, out.data_ptr(), out.stride(0), base + at[1], work.data_ptr(), entries, T,
                                           q_heads, kv_heads, head_dim, head_dim, page_size, 2 * page_size, n, scale, 0, window, keep_first, 0, 0, softcap,
