@@ -32,27 +32,33 @@ __device__ __forceinline__ void quant_kv_group(const uint4& u, uint32_t& word, _
   }
   s16 = __ushort_as_bfloat16(static_cast<unsigned short>(sb));
   const float sc = __uint_as_float(sb << 16);
-  // rint((x - z) / s), between 0 and 15: by the reciprocal, whose error (2^-22 of the quotient) counts next to a tie only; those few are
-  // divided.  (A scale below 2^-120 has no reciprocal that serves: all are divided.)  Rounded by what is left of a mantissa.
+  // rint((x - z) / s), between 0 and 15, the quotient rounded to fp32 as a division's: y = 1 / s correctly rounded by a Newton step (s has 8
+  // bits, which keeps 1 / s away from halfway between two numbers), a quotient q within two units of the last place, and q + (d - q s) y,
+  // Markstein's correction, where d - q s is exact and d / s is never halfway either.  (Below 2^-100 it might not be exact: those are
+  // divided.)  Rounded by what is left of a mantissa; two at a time, numbers i and i + 4.
   word = 0;
   if (sc > 0.f) {
-    float x[8], c[8], near = 0.f;
+    float x[8];
     unpack8<T>(u, x);
-    const float inv = ptx::rcp_approx(sc);
+    uint64_t c[4];
+    if (sc >= 7.9e-31f) {
+      float y = ptx::rcp_approx(sc);
+      y = fmaf(fmaf(-sc, y, 1.f), y, y);
+      const uint64_t y2 = ptx::f32x2(y, y), s2 = ptx::f32x2(-sc, -sc), z2 = ptx::f32x2(-z, -z);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float q = (x[i] - z) * inv;
-      c[i] = (q + 12582912.f) - 12582912.f;
-      near = fmaxf(near, fabsf(q - c[i]));
-    }
-    if (near > 0.4999f || sc < 7.6e-37f) {
+      for (int i = 0; i < 4; ++i) {
+        const uint64_t d = ptx::add_f32x2(ptx::f32x2(x[i], x[i + 4]), z2), q = ptx::mul_f32x2(d, y2);
+        c[i] = ptx::fma_f32x2(ptx::fma_f32x2(q, s2, d), y2, q);
+        c[i] = ptx::add_f32x2(ptx::add_f32x2(c[i], ptx::f32x2(12582912.f, 12582912.f)), ptx::f32x2(-12582912.f, -12582912.f));
+      }
+    } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) c[i] = rintf(__fdiv_rn(x[i] - z, sc));
+      for (int i = 0; i < 4; ++i) c[i] = ptx::f32x2(rintf(__fdiv_rn(x[i] - z, sc)), rintf(__fdiv_rn(x[i + 4] - z, sc)));
     }
     // four codes are a number of 16 bits
-    const float low = fmaf(fmaf(fmaf(c[3], 16.f, c[2]), 16.f, c[1]), 16.f, c[0]) + 8388608.f;
-    const float high = fmaf(fmaf(fmaf(c[7], 16.f, c[6]), 16.f, c[5]), 16.f, c[4]) + 8388608.f;
-    word = __byte_perm(__float_as_uint(low), __float_as_uint(high), 0x5410);
+    const uint64_t sixteen = ptx::f32x2(16.f, 16.f);
+    const float2 four = ptx::f32x2_get(ptx::add_f32x2(ptx::fma_f32x2(ptx::fma_f32x2(ptx::fma_f32x2(c[3], sixteen, c[2]), sixteen, c[1]), sixteen, c[0]), ptx::f32x2(8388608.f, 8388608.f)));
+    word = __byte_perm(__float_as_uint(four.x), __float_as_uint(four.y), 0x5410);
   }
 }
 
@@ -82,23 +88,34 @@ __device__ __forceinline__ void quant_kv_write(uint8_t* block, int tok, int l, b
     w[F.groups] = z16;
   }
 }
+// Nibbles of a tile of 16 dimensions: lane i looks after tile m and, of its dimensions, 2 a, 2 a + 1 and those 8 behind.
+struct QuantTile {
+  int m, a;
+  __device__ __forceinline__ QuantTile() {
+    const int i = threadIdx.x & 31;
+    m = (i >> 4) * 4 + (i & 3);
+    a = (i >> 2) & 3;
+  }
+  // of the first of its two words, of the four tokens from `tok` on, in the values' codes
+  __device__ __forceinline__ int at(int tok) const { return (m >> 2) * 512 + a * 128 + (tok >> 2) * 16 + (m & 3) * 4; }
+};
 // The words of four tokens, from token `tok` of a block on, whose codes the warp has put into `codes` [4][D / 8].
 template <int D, int GROUP>
 __device__ __forceinline__ void quant_kv_write_quad(uint8_t* block, int tok, const uint32_t* codes) {
   constexpr int LANES = D / 8;
-  block += quant_kv(D, GROUP).part;
+  const QuantTile t;
   __syncwarp();
-  // word (m / 4, g, quad, m % 4): bytes are tokens 0, 2, 1, 3, nibbles dimensions 16 m + g and 16 m + 8 + g
+  if (t.m < D / 16) {
+    // a word's bytes are tokens 0, 2, 1, 3, nibbles dimensions 16 m + g and 16 m + 8 + g; byte a of a row's word has g = 2 a and 2 a + 1
+    uint2 w[4];
 #pragma unroll
-  for (int i = threadIdx.x & 31; i < D / 2; i += 32) {
-    const int m = (i >> 5) * 4 + (i & 3), g = (i >> 2) & 7;
-    uint32_t word = 0;
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      const uint32_t* from = codes + ((b & 1) * 2 + (b >> 1)) * LANES + 2 * m;
-      word |= (((from[0] >> (4 * g)) & 15u) | (((from[1] >> (4 * g)) & 15u) << 4)) << (8 * b);
-    }
-    *reinterpret_cast<uint32_t*>(block + (i >> 5) * 512 + g * 64 + (tok >> 2) * 16 + (i & 3) * 4) = word;
+    for (int b = 0; b < 4; ++b) w[b] = *reinterpret_cast<const uint2*>(codes + ((b & 1) * 2 + (b >> 1)) * LANES + 2 * t.m);
+    const uint32_t pick = t.a | (t.a + 4) << 4;
+    const uint32_t low = __byte_perm(__byte_perm(w[0].x, w[1].x, pick), __byte_perm(w[2].x, w[3].x, pick), 0x5410);
+    const uint32_t high = __byte_perm(__byte_perm(w[0].y, w[1].y, pick), __byte_perm(w[2].y, w[3].y, pick), 0x5410);
+    uint8_t* const to = block + quant_kv(D, GROUP).part + t.at(tok);
+    *reinterpret_cast<uint32_t*>(to) = (low & 0x0f0f0f0fu) | ((high << 4) & 0xf0f0f0f0u);
+    *reinterpret_cast<uint32_t*>(to + 64) = ((low >> 4) & 0x0f0f0f0fu) | (high & 0xf0f0f0f0u);
   }
 }
 
@@ -121,7 +138,7 @@ template <typename T, int D, int GROUP>
 __global__ void __launch_bounds__(256) quant_kv_store_kernel(const QuantStoreParams p) {
   constexpr QuantKv F = quant_kv(D, GROUP);
   constexpr int LANES = D / 8, ROWS = 32 / LANES;  // rows a warp takes at a time
-  __shared__ uint32_t s_codes[8][4 * LANES];
+  __shared__ __align__(8) uint32_t s_codes[8][4 * LANES];
   ptx::griddep_launch_dependents();
   ptx::griddep_wait();
   const int lane = threadIdx.x & 31, l = lane % LANES;
@@ -185,7 +202,7 @@ __global__ void __launch_bounds__(256) quant_kv_rope_kernel(const QuantRopeParam
   constexpr QuantKv F = quant_kv(D, GROUP);
   constexpr int LANES = D / 8, ROWS = 32 / LANES, HALF = D / 2;
   __shared__ float s_cos[R][HALF], s_sin[R][HALF];
-  __shared__ uint32_t s_codes[8][R == 4 ? 4 * LANES : 1];
+  __shared__ __align__(8) uint32_t s_codes[8][R == 4 ? 4 * LANES : 1];
   ptx::griddep_launch_dependents();
   if (!STATIC) ptx::griddep_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % LANES;
@@ -272,7 +289,7 @@ template <typename T, int D, int GROUP>
 __global__ void __launch_bounds__(256) quant_kv_load_kernel(const QuantLoadParams p) {
   constexpr QuantKv F = quant_kv(D, GROUP);
   constexpr int LANES = D / 8, ROWS = 32 / LANES;
-  __shared__ __align__(16) T s_rows[8][4 * D];
+  __shared__ uint32_t s_codes[8][4 * LANES];
   ptx::griddep_launch_dependents();
   ptx::griddep_wait();
   const int lane = threadIdx.x & 31, l = lane % LANES;
@@ -280,7 +297,7 @@ __global__ void __launch_bounds__(256) quant_kv_load_kernel(const QuantLoadParam
   if (unit >= p.units) return;
   const int head = static_cast<int>(unit % p.kv_heads);
   const int64_t t0 = unit / p.kv_heads * 4;
-  T* const rows = s_rows[threadIdx.x >> 5];
+  uint32_t* const codes = s_codes[threadIdx.x >> 5];
   int slots = lane < 4 && t0 + lane < p.rows ? p.slot[t0 + lane] : -1;
   if (slots >= 0 && slots >> p.page_shift >= p.max_pages) {
     if (p.status) atomicCAS(p.status, 0, kStatusBadIndex);
@@ -295,7 +312,8 @@ __global__ void __launch_bounds__(256) quant_kv_load_kernel(const QuantLoadParam
   auto scales = [&](const uint8_t* part, int tok) { return reinterpret_cast<const __nv_bfloat16*>(part + F.codes) + tok * 2 * F.groups; };
   uint32_t word[4 / ROWS];
   __nv_bfloat16 ks[4 / ROWS], kz[4 / ROWS], vs[4 / ROWS], vz[4 / ROWS];
-  uint32_t vw[4 / ROWS];  // of a row: eight codes; of a quad: words lane and lane + 32
+  uint32_t vw[4 / ROWS];  // of the values, unless they come by quads
+  const QuantTile own;
 #pragma unroll
   for (int r = 0; r < 4 / ROWS; ++r) {
     const int s = max(0, __shfl_sync(0xffffffffu, slots, r * ROWS + lane / LANES)), tok = s & 15, g = l / (GROUP / 8);
@@ -306,30 +324,25 @@ __global__ void __launch_bounds__(256) quant_kv_load_kernel(const QuantLoadParam
     vs[r] = scales(block + F.part, tok)[g];
     vz[r] = scales(block + F.part, tok)[F.groups + g];
     vw[r] = 0;
-    if (quad) {
-      const int i = lane + 32 * r;
-      if (i < D / 2) vw[r] = *reinterpret_cast<const uint32_t*>(block_of(s0) + F.part + (i >> 5) * 512 + ((i >> 2) & 7) * 64 + ((s0 & 15) >> 2) * 16 + (i & 3) * 4);
-    } else {
+    if (!quad) {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         vw[r] |= ((static_cast<uint32_t>(block[F.part + quant_kv_value_byte(tok, (l >> 1) * 16 + i)]) >> (4 * (l & 1))) & 15u) << (4 * i);
     }
   }
-  if (quad) {  // codes as they are, in 16 bits a place, into rows
+  if (quad && own.m < D / 16) {
+    const uint8_t* from = block_of(s0) + F.part + own.at(s0 & 15);
+    const uint32_t tile[2] = {*reinterpret_cast<const uint32_t*>(from), *reinterpret_cast<const uint32_t*>(from + 64)};
+    // byte own.a of a row's words of the tile, tokens 0, 2, 1, 3
+    const uint32_t low = (tile[0] & 0x0f0f0f0fu) | ((tile[1] << 4) & 0xf0f0f0f0u), high = ((tile[0] >> 4) & 0x0f0f0f0fu) | (tile[1] & 0xf0f0f0f0u);
 #pragma unroll
-    for (int r = 0; r < 4 / ROWS; ++r) {
-      const int i = lane + 32 * r, d = (i >> 5) * 64 + (i & 3) * 16 + ((i >> 2) & 7);
-      if (i < D / 2) {
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const int tok = (b & 1) * 2 + (b >> 1);
-          reinterpret_cast<uint16_t*>(rows)[tok * D + d] = static_cast<uint16_t>((vw[r] >> (8 * b)) & 15u);
-          reinterpret_cast<uint16_t*>(rows)[tok * D + d + 8] = static_cast<uint16_t>((vw[r] >> (8 * b + 4)) & 15u);
-        }
-      }
+    for (int b = 0; b < 4; ++b) {
+      uint8_t* to = reinterpret_cast<uint8_t*>(codes + ((b & 1) * 2 + (b >> 1)) * LANES + 2 * own.m) + own.a;
+      to[0] = static_cast<uint8_t>(low >> (8 * b));
+      to[4] = static_cast<uint8_t>(high >> (8 * b));
     }
-    __syncwarp();
   }
+  if (quad) __syncwarp();
 #pragma unroll
   for (int r = 0; r < 4 / ROWS; ++r) {
     const int row = r * ROWS + lane / LANES;
@@ -337,20 +350,11 @@ __global__ void __launch_bounds__(256) quant_kv_load_kernel(const QuantLoadParam
     const int64_t at = ((t0 + row) * p.kv_heads + head) * D + l * 8;
     const float k_s = __bfloat162float(ks[r]), k_z = __bfloat162float(kz[r]), v_s = __bfloat162float(vs[r]), v_z = __bfloat162float(vz[r]);
     float x[8], y[8];
-    quant_kv_codes(word[r], x);
-    const uint4 c4 = quad ? *reinterpret_cast<const uint4*>(rows + row * D + l * 8) : make_uint4(0, 0, 0, 0);
-    if (quad) {  // (one in 16 bits each)
-      const uint32_t c2[4] = {c4.x, c4.y, c4.z, c4.w};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = __uint_as_float(0x4b000000u | (i & 1 ? c2[i >> 1] >> 16 : c2[i >> 1] & 15u)) - 8388608.f;
-    } else {
-      quant_kv_codes(vw[r], y);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      x[i] = fmaf(k_s, x[i], k_z);
-      y[i] = fmaf(v_s, y[i], v_z);
-    }
+    uint64_t c[4];
+    quant_kv_codes(word[r], c);
+    quant_kv_numbers(c, k_s, k_z, x);
+    quant_kv_codes(quad ? codes[row * LANES + l] : vw[r], c);
+    quant_kv_numbers(c, v_s, v_z, y);
     constexpr float most = quant_kv_most<T>();
     if (quant_kv_past(k_s, k_z, most) || quant_kv_past(v_s, v_z, most)) {
 #pragma unroll

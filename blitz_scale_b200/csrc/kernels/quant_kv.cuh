@@ -18,6 +18,7 @@
 // Scales: per token the groups' s, then their z.
 #pragma once
 #include "common.cuh"
+#include "ptx.cuh"
 
 namespace blitz {
 
@@ -59,6 +60,24 @@ __device__ __forceinline__ void quant_kv_codes(uint32_t w, float (&c)[8]) {
   c[5] = __uint_as_float(quant_kv_pick<0x00f00u, 0x47000000u>(v)) - 32768.f;
   c[6] = __uint_as_float(quant_kv_pick<0x0f000u, 0x45000000u>(v)) - 2048.f;
   c[7] = __uint_as_float(quant_kv_pick<0xf0000u, 0x43000000u>(v)) - 128.f;
+}
+// The same, two an instruction (pairs of registers: where there is room for them).
+__device__ __forceinline__ void quant_kv_codes(uint32_t w, uint64_t (&c)[4]) {
+  const uint32_t v = w >> 12;
+  auto two = [](uint32_t a, uint32_t b, float za, float zb) { return ptx::add_f32x2(ptx::f32x2(__uint_as_float(a), __uint_as_float(b)), ptx::f32x2(za, zb)); };
+  c[0] = two(quant_kv_pick<0x0000fu, 0x4b000000u>(w), quant_kv_pick<0x000f0u, 0x49000000u>(w), -8388608.f, -524288.f);
+  c[1] = two(quant_kv_pick<0x00f00u, 0x47000000u>(w), quant_kv_pick<0x0f000u, 0x45000000u>(w), -32768.f, -2048.f);
+  c[2] = two(quant_kv_pick<0xf0000u, 0x43000000u>(w), quant_kv_pick<0x00f00u, 0x47000000u>(v), -128.f, -32768.f);
+  c[3] = two(quant_kv_pick<0x0f000u, 0x45000000u>(v), quant_kv_pick<0xf0000u, 0x43000000u>(v), -2048.f, -128.f);
+}
+// s c + z
+__device__ __forceinline__ void quant_kv_numbers(const uint64_t (&c)[4], float s, float z, float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = ptx::f32x2_get(ptx::fma_f32x2(c[i], ptx::f32x2(s, s), ptx::f32x2(z, z)));
+    x[2 * i] = v.x;
+    x[2 * i + 1] = v.y;
+  }
 }
 // The largest finite number of a type.  A scale that was rounded up can carry the largest number of a group past it: such groups are cut.
 template <typename T>
