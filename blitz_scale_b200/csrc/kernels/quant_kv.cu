@@ -7,18 +7,40 @@
 
 namespace blitz {
 
-// Eight numbers of a lane, whose group the lanes around it share: their codes, and the group's scale and offset.
-template <typename T, int GROUP>
-__device__ __forceinline__ void quant_kv_group(const uint4& u, uint32_t& word, __nv_bfloat16& s16, __nv_bfloat16& z16) {
+// The smaller, or larger, of two pairs of numbers (NaN where there is one).
+template <typename T>
+using QuantPair = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
+template <typename T>
+__device__ __forceinline__ uint32_t quant_kv_least(uint32_t a, uint32_t b) {
+  const QuantPair<T> m = __hmin2_nan(*reinterpret_cast<QuantPair<T>*>(&a), *reinterpret_cast<QuantPair<T>*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t quant_kv_largest(uint32_t a, uint32_t b) {
+  const QuantPair<T> m = __hmax2_nan(*reinterpret_cast<QuantPair<T>*>(&a), *reinterpret_cast<QuantPair<T>*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+// A lane's numbers, eight in each of N words of four registers, of a group that LANES lanes share: codes, and the group's scale and offset.
+template <typename T, int N, int LANES>
+__device__ __forceinline__ void quant_kv_group(const uint4 (&u)[N], uint32_t (&word)[N], __nv_bfloat16& s16, __nv_bfloat16& z16) {
   // the smallest number and the negative of the largest, as a pair (NaN where there is one)
-  using T2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
-  auto pair = [](uint32_t u) { return *reinterpret_cast<T2*>(&u); };
-  auto bits = [](T2 v) { return *reinterpret_cast<uint32_t*>(&v); };
-  uint32_t lo2 = bits(__hmin2_nan(__hmin2_nan(pair(u.x), pair(u.y)), __hmin2_nan(pair(u.z), pair(u.w))));
-  uint32_t hi2 = bits(__hmax2_nan(__hmax2_nan(pair(u.x), pair(u.y)), __hmax2_nan(pair(u.z), pair(u.w)))) ^ 0x80008000u;
-  uint32_t ends = bits(__hmin2_nan(pair(__byte_perm(lo2, hi2, 0x5410)), pair(__byte_perm(lo2, hi2, 0x7632))));
+  uint32_t lo2[N], hi2[N];
 #pragma unroll
-  for (int d = 1; d < GROUP / 8; d <<= 1) ends = bits(__hmin2_nan(pair(ends), pair(__shfl_xor_sync(0xffffffffu, ends, d))));
+  for (int i = 0; i < N; ++i) {
+    lo2[i] = quant_kv_least<T>(quant_kv_least<T>(u[i].x, u[i].y), quant_kv_least<T>(u[i].z, u[i].w));
+    hi2[i] = quant_kv_largest<T>(quant_kv_largest<T>(u[i].x, u[i].y), quant_kv_largest<T>(u[i].z, u[i].w));
+  }
+#pragma unroll
+  for (int d = N / 2; d > 0; d >>= 1)
+#pragma unroll
+    for (int i = 0; i < d; ++i) {
+      lo2[i] = quant_kv_least<T>(lo2[i], lo2[i + d]);
+      hi2[i] = quant_kv_largest<T>(hi2[i], hi2[i + d]);
+    }
+  hi2[0] ^= 0x80008000u;
+  uint32_t ends = quant_kv_least<T>(__byte_perm(lo2[0], hi2[0], 0x5410), __byte_perm(lo2[0], hi2[0], 0x7632));
+#pragma unroll
+  for (int d = 1; d < LANES; d <<= 1) ends = quant_kv_least<T>(ends, __shfl_xor_sync(0xffffffffu, ends, d));
   const float2 end = cvt2<T>(ends);
   z16 = __float2bfloat16_rd(end.x);
   const float z = __bfloat162float(z16), range = -end.y - z;
@@ -36,29 +58,33 @@ __device__ __forceinline__ void quant_kv_group(const uint4& u, uint32_t& word, _
   // bits, which keeps 1 / s away from halfway between two numbers), a quotient q within two units of the last place, and q + (d - q s) y,
   // Markstein's correction, where d - q s is exact and d / s is never halfway either.  (Below 2^-100 it might not be exact: those are
   // divided.)  Rounded by what is left of a mantissa; two at a time, numbers i and i + 4.
-  word = 0;
   if (sc > 0.f) {
-    float x[8];
-    unpack8<T>(u, x);
-    uint64_t c[4];
-    if (sc >= 7.9e-31f) {
-      float y = ptx::rcp_approx(sc);
-      y = fmaf(fmaf(-sc, y, 1.f), y, y);
-      const uint64_t y2 = ptx::f32x2(y, y), s2 = ptx::f32x2(-sc, -sc), z2 = ptx::f32x2(-z, -z);
+    float y = ptx::rcp_approx(sc);
+    y = fmaf(fmaf(-sc, y, 1.f), y, y);
+    const uint64_t y2 = ptx::f32x2(y, y), s2 = ptx::f32x2(-sc, -sc), z2 = ptx::f32x2(-z, -z);
+    const uint64_t sixteen = ptx::f32x2(16.f, 16.f), up = ptx::f32x2(12582912.f, 12582912.f), down = ptx::f32x2(-12582912.f, -12582912.f);
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      float x[8];
+      unpack8<T>(u[k], x);
+      uint64_t c[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint64_t d = ptx::add_f32x2(ptx::f32x2(x[i], x[i + 4]), z2), q = ptx::mul_f32x2(d, y2);
         c[i] = ptx::fma_f32x2(ptx::fma_f32x2(q, s2, d), y2, q);
-        c[i] = ptx::add_f32x2(ptx::add_f32x2(c[i], ptx::f32x2(12582912.f, 12582912.f)), ptx::f32x2(-12582912.f, -12582912.f));
+        c[i] = ptx::add_f32x2(ptx::add_f32x2(c[i], up), down);
       }
-    } else {
+      if (sc < 7.9e-31f) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) c[i] = ptx::f32x2(rintf(__fdiv_rn(x[i] - z, sc)), rintf(__fdiv_rn(x[i + 4] - z, sc)));
+        for (int i = 0; i < 4; ++i) c[i] = ptx::f32x2(rintf(__fdiv_rn(x[i] - z, sc)), rintf(__fdiv_rn(x[i + 4] - z, sc)));
+      }
+      // four codes are a number of 16 bits
+      const float2 four = ptx::f32x2_get(ptx::add_f32x2(ptx::fma_f32x2(ptx::fma_f32x2(ptx::fma_f32x2(c[3], sixteen, c[2]), sixteen, c[1]), sixteen, c[0]), ptx::f32x2(8388608.f, 8388608.f)));
+      word[k] = __byte_perm(__float_as_uint(four.x), __float_as_uint(four.y), 0x5410);
     }
-    // four codes are a number of 16 bits
-    const uint64_t sixteen = ptx::f32x2(16.f, 16.f);
-    const float2 four = ptx::f32x2_get(ptx::add_f32x2(ptx::fma_f32x2(ptx::fma_f32x2(ptx::fma_f32x2(c[3], sixteen, c[2]), sixteen, c[1]), sixteen, c[0]), ptx::f32x2(8388608.f, 8388608.f)));
-    word = __byte_perm(__float_as_uint(four.x), __float_as_uint(four.y), 0x5410);
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k) word[k] = 0;
   }
 }
 
@@ -99,17 +125,16 @@ struct QuantTile {
   // of the first of its two words, of the four tokens from `tok` on, in the values' codes
   __device__ __forceinline__ int at(int tok) const { return (m >> 2) * 512 + a * 128 + (tok >> 2) * 16 + (m & 3) * 4; }
 };
-// The words of four tokens, from token `tok` of a block on, whose codes the warp has put into `codes` [4][D / 8].
-template <int D, int GROUP>
+// The words of four tokens, from token `tok` of a block on, whose codes the warp has put into `codes` [4][PITCH].
+template <int D, int GROUP, int PITCH = D / 8>
 __device__ __forceinline__ void quant_kv_write_quad(uint8_t* block, int tok, const uint32_t* codes) {
-  constexpr int LANES = D / 8;
   const QuantTile t;
   __syncwarp();
   if (t.m < D / 16) {
     // a word's bytes are tokens 0, 2, 1, 3, nibbles dimensions 16 m + g and 16 m + 8 + g; byte a of a row's word has g = 2 a and 2 a + 1
     uint2 w[4];
 #pragma unroll
-    for (int b = 0; b < 4; ++b) w[b] = *reinterpret_cast<const uint2*>(codes + ((b & 1) * 2 + (b >> 1)) * LANES + 2 * t.m);
+    for (int b = 0; b < 4; ++b) w[b] = *reinterpret_cast<const uint2*>(codes + ((b & 1) * 2 + (b >> 1)) * PITCH + 2 * t.m);
     const uint32_t pick = t.a | (t.a + 4) << 4;
     const uint32_t low = __byte_perm(__byte_perm(w[0].x, w[1].x, pick), __byte_perm(w[2].x, w[3].x, pick), 0x5410);
     const uint32_t high = __byte_perm(__byte_perm(w[0].y, w[1].y, pick), __byte_perm(w[2].y, w[3].y, pick), 0x5410);
@@ -125,62 +150,90 @@ struct QuantStoreParams {
   int64_t k_row, v_row;
   const int32_t* slot;
   uint8_t* pool;
-  int64_t units;  // (four rows, head) each
+  int64_t units;  // (rows of a warp, head, keys or values) each
   int tokens, kv_heads, page_shift, max_pages;
   int* status;
 };
 
-// A warp takes four rows of one head, keys and values: D / 8 lanes a row, eight dimensions each; the lanes of a group find its smallest and
-// largest number together.  (Bound by the chain of a warp, loads, shuffles, stores: slots, keys and values are asked for at once.)  Keys go out as they are, a word a lane.  A word of the values holds four tokens of two dimensions: where the four
-// rows are the four tokens of a word (rows of a prompt) the lanes exchange their codes through shared memory and write words; else (the
-// tokens of a batch) every row writes its bytes.
+// A warp takes keys or values of a head, of 8 rows (16 of 64 dimensions): a lane has 32 dimensions, so that what a group needs once, its ends
+// and its scale, is worked out by the one lane, two or four that have it (with eight dimensions a lane that was half of 195 instructions for
+// 256 numbers, and 8192 rows took 16.5 us).  The codes go
+// through shared memory: keys leave in rows of 16 bytes a lane.  A word of the values holds four tokens of two dimensions: where four rows
+// are the four tokens of a word (rows of a prompt) words are written, else (the tokens of a batch) every row's bytes.
 template <typename T, int D, int GROUP>
-__global__ void __launch_bounds__(256) quant_kv_store_kernel(const QuantStoreParams p) {
+__global__ void __launch_bounds__(128) quant_kv_store_kernel(const QuantStoreParams p) {
   constexpr QuantKv F = quant_kv(D, GROUP);
-  constexpr int LANES = D / 8, ROWS = 32 / LANES;  // rows a warp takes at a time
-  __shared__ __align__(8) uint32_t s_codes[8][4 * LANES];
+  constexpr int LANES = D / 32, ROWS = 32 / LANES, PITCH = D / 8 + 4;  // (rows in different banks)
+  __shared__ __align__(16) uint32_t s_codes[4][ROWS * PITCH + 0];
   ptx::griddep_launch_dependents();
   ptx::griddep_wait();
-  const int lane = threadIdx.x & 31, l = lane % LANES;
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, l = lane % LANES, row = lane / LANES;
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
   if (unit >= p.units) return;
-  const int head = static_cast<int>(unit % p.kv_heads);
-  const int64_t t0 = unit / p.kv_heads * 4;
+  const bool value = unit & 1;
+  const int head = static_cast<int>((unit >> 1) % p.kv_heads);
+  const int64_t t0 = (unit >> 1) / p.kv_heads * ROWS, t = t0 + row;
   uint32_t* const codes = s_codes[threadIdx.x >> 5];
-  // the four slots: lane i has the i-th
-  int slots = lane < 4 && t0 + lane < p.tokens ? p.slot[t0 + lane] : -1;
-  uint4 raw[2][4 / ROWS];
+  // lane i has the i-th slot
+  int slots = lane < ROWS && t0 + lane < p.tokens ? p.slot[t0 + lane] : -1;
+  uint4 raw[4];
+  const T* from = reinterpret_cast<const T*>(value ? p.v : p.k) + t * (value ? p.v_row : p.k_row) + static_cast<int64_t>(head) * D + l * 32;
 #pragma unroll
-  for (int r = 0; r < 4 / ROWS; ++r) {
-    const int64_t t = t0 + r * ROWS + lane / LANES, at = static_cast<int64_t>(head) * D + l * 8;
-    const bool real = t < p.tokens;
-    raw[0][r] = real ? *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.k) + t * p.k_row + at) : make_uint4(0, 0, 0, 0);
-    raw[1][r] = real ? *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.v) + t * p.v_row + at) : make_uint4(0, 0, 0, 0);
-  }
+  for (int i = 0; i < 4; ++i) raw[i] = t < p.tokens ? *reinterpret_cast<const uint4*>(from + i * 8) : make_uint4(0, 0, 0, 0);
   if (slots >= 0 && slots >> p.page_shift >= p.max_pages) {
     if (p.status) atomicCAS(p.status, 0, kStatusBadIndex);
     slots = -1;
   }
-  const int s0 = __shfl_sync(0xffffffffu, slots, 0);
-  const bool quad = s0 >= 0 && (s0 & 3) == 0 && __all_sync(0xffffffffu, lane >= 4 || slots == s0 + lane);
+  const int s0 = __shfl_sync(0xffffffffu, slots, lane & 28);  // of four rows, the first one's
+  const uint32_t quads = __ballot_sync(0xffffffffu, s0 >= 0 && (s0 & 3) == 0 && slots == s0 + (lane & 3));
+  const int s = __shfl_sync(0xffffffffu, slots, row);
   auto block_of = [&](int s) {
     const int page = s >> p.page_shift;
-    return p.pool + (((static_cast<int64_t>(page) * p.kv_heads + head) << (p.page_shift - 4)) + ((s - (page << p.page_shift)) >> 4)) * F.block;
+    return p.pool + (((static_cast<int64_t>(page) * p.kv_heads + head) << (p.page_shift - 4)) + ((s - (page << p.page_shift)) >> 4)) * F.block + (value ? F.part : 0);
   };
-  auto rows = [&](auto plane) {
-    constexpr bool value = decltype(plane)::value;
-#pragma unroll
-    for (int r = 0; r < 4 / ROWS; ++r) {
-      const int s = __shfl_sync(0xffffffffu, slots, r * ROWS + lane / LANES);
-      uint32_t word;
-      __nv_bfloat16 s16, z16;
-      quant_kv_group<T, GROUP>(raw[value][r], word, s16, z16);
-      quant_kv_write<D, GROUP>(s >= 0 ? block_of(s) : nullptr, s & 15, l, value, value && quad ? codes + (r * ROWS + lane / LANES) * LANES : nullptr, word, s16, z16);
+  uint32_t word[4];
+  __nv_bfloat16 s16, z16;
+  quant_kv_group<T, 4, GROUP / 32>(raw, word, s16, z16);
+  const bool quad = ((quads >> (row & 28)) & 15u) == 15u;
+  const int tok = s & 15;
+  if (s >= 0) {
+    uint8_t* const block = block_of(s);
+    if (l % (GROUP / 32) == 0) {
+      __nv_bfloat16* w = reinterpret_cast<__nv_bfloat16*>(block + F.codes) + tok * 2 * F.groups + l / (GROUP / 32);
+      w[0] = s16;
+      w[F.groups] = z16;
     }
-    if (value && quad) quant_kv_write_quad<D, GROUP>(block_of(s0), s0 & 15, codes);
-  };
-  rows(std::false_type{});
-  rows(std::true_type{});
+  }
+  if (!value) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) codes[row * PITCH + i * LANES + l] = word[i];
+    __syncwarp();
+    if (s >= 0) *reinterpret_cast<uint4*>(block_of(s) + tok * (D / 2) + l * 16) = *reinterpret_cast<const uint4*>(codes + row * PITCH + l * 4);
+    return;
+  }
+  *reinterpret_cast<uint4*>(codes + row * PITCH + l * 4) = make_uint4(word[0], word[1], word[2], word[3]);
+  __syncwarp();
+#pragma unroll
+  for (int r = 0; r < ROWS; r += 4) {
+    const int at = __shfl_sync(0xffffffffu, s0, r);
+    if (((quads >> r) & 15u) == 15u) quant_kv_write_quad<D, GROUP, PITCH>(block_of(at) - F.part, at & 15, codes + r * PITCH);
+  }
+  if (__all_sync(0xffffffffu, quad || s < 0)) return;
+  // a lane has a tile of 16 dimensions of a row, g = 0 .. 3 or 4 .. 7 of it: nibbles 16 m + g and 16 m + 8 + g are a byte
+  constexpr int EACH = D / 8, TIMES = ROWS * EACH / 32;
+  const int m = lane % EACH >> 1, half = lane & 1;
+#pragma unroll 1
+  for (int i = 0; i < TIMES; ++i) {
+    const int r = i * (32 / EACH) + lane / EACH, to = __shfl_sync(0xffffffffu, slots, r);
+    if (to < 0 || ((quads >> (r & 28)) & 15u) == 15u) continue;
+    const uint2 w = *reinterpret_cast<const uint2*>(codes + r * PITCH + 2 * m);
+    const uint32_t even = ((w.x & 0x0f0f0f0fu) | ((w.y << 4) & 0xf0f0f0f0u)) >> (16 * half), odd = (((w.x >> 4) & 0x0f0f0f0fu) | (w.y & 0xf0f0f0f0u)) >> (16 * half);
+    uint8_t* const d = block_of(to) + quant_kv_value_byte(to & 15, m * 16) + half * 256;
+    d[0] = static_cast<uint8_t>(even);
+    d[64] = static_cast<uint8_t>(odd);
+    d[128] = static_cast<uint8_t>(even >> 8);
+    d[192] = static_cast<uint8_t>(odd >> 8);
+  }
 }
 
 // ------------------------------------------------------------------ rotation and rows in
@@ -258,13 +311,13 @@ __global__ void __launch_bounds__(256) quant_kv_rope_kernel(const QuantRopeParam
         }
       }
       if (R == 4 ? h < p.q_heads : unit * 4 + 3 < p.q_heads) continue;  // (the whole warp: nothing but queries)
-      uint32_t word;
+      uint32_t word[1];
       __nv_bfloat16 s16, z16;
-      quant_kv_group<T, GROUP>(raw[k], word, s16, z16);
+      quant_kv_group<T, 1, GROUP / 8>({raw[k]}, word, s16, z16);
       const bool value = h >= turned;
       const int s = __shfl_sync(0xffffffffu, slots, row);
       uint8_t* const block = s >= 0 && h >= p.q_heads && h < heads ? block_of(s, value ? h - turned : h - p.q_heads) : nullptr;
-      quant_kv_write<D, GROUP>(block, s & 15, l, value, R == 4 && value && quad ? s_codes[warp] + i * LANES : nullptr, word, s16, z16);
+      quant_kv_write<D, GROUP>(block, s & 15, l, value, R == 4 && value && quad ? s_codes[warp] + i * LANES : nullptr, word[0], s16, z16);
     }
     if (R == 4 && quad && unit >= turned) {
       quant_kv_write_quad<D, GROUP>(block_of(s0, unit - turned), s0 & 15, s_codes[warp]);
@@ -278,93 +331,119 @@ struct QuantLoadParams {
   const uint8_t* pool;
   const int32_t* slot;
   void *k, *v;    // row r of both
-  int64_t rows, units;  // (four rows, head) each
+  int64_t rows, units;  // (rows of a warp, head, keys or values) each
   int kv_heads, page_shift, max_pages;
   int* status;
 };
 
-// Rows of slots: a warp takes four of one head, as the store does.  Values of four tokens of a word come by words, through shared memory;
-// others byte by byte.
+// Rows of slots: a warp takes keys or values of a head, of 8 rows (16 of 64 dimensions), as the store does; a lane has four words of a row's codes,
+// spread so that the lanes of a row write next to each other.  Values of four tokens of a word come 16 bytes a lane and are put into rows
+// through shared memory; others byte by byte.
 template <typename T, int D, int GROUP>
-__global__ void __launch_bounds__(256) quant_kv_load_kernel(const QuantLoadParams p) {
+__global__ void __launch_bounds__(128) quant_kv_load_kernel(const QuantLoadParams p) {
   constexpr QuantKv F = quant_kv(D, GROUP);
-  constexpr int LANES = D / 8, ROWS = 32 / LANES;
-  __shared__ uint32_t s_codes[8][4 * LANES];
+  constexpr int LANES = D / 32, ROWS = 32 / LANES, PITCH = D / 8 + 4, G = F.groups, EACH = D / 8;
+  __shared__ __align__(16) uint32_t s_codes[4][ROWS * PITCH], s_words[4][ROWS / 4 * (D / 2)];
   ptx::griddep_launch_dependents();
   ptx::griddep_wait();
-  const int lane = threadIdx.x & 31, l = lane % LANES;
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % LANES, row = lane / LANES;
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * 4 + warp;
   if (unit >= p.units) return;
-  const int head = static_cast<int>(unit % p.kv_heads);
-  const int64_t t0 = unit / p.kv_heads * 4;
-  uint32_t* const codes = s_codes[threadIdx.x >> 5];
-  int slots = lane < 4 && t0 + lane < p.rows ? p.slot[t0 + lane] : -1;
+  const bool value = unit & 1;
+  const int head = static_cast<int>((unit >> 1) % p.kv_heads);
+  const int64_t t0 = (unit >> 1) / p.kv_heads * ROWS;
+  uint32_t *const codes = s_codes[warp], *const words = s_words[warp];
+  int slots = lane < ROWS && t0 + lane < p.rows ? p.slot[t0 + lane] : -1;
   if (slots >= 0 && slots >> p.page_shift >= p.max_pages) {
     if (p.status) atomicCAS(p.status, 0, kStatusBadIndex);
     slots = -1;
   }
-  const int s0 = __shfl_sync(0xffffffffu, slots, 0);
-  const bool quad = s0 >= 0 && (s0 & 3) == 0 && __all_sync(0xffffffffu, lane >= 4 || slots == s0 + lane);
+  const int s0 = __shfl_sync(0xffffffffu, slots, lane & 28);  // of four rows, the first one's
+  const uint32_t quads = __ballot_sync(0xffffffffu, s0 >= 0 && (s0 & 3) == 0 && slots == s0 + (lane & 3));
+  auto is_quad = [&](int r) { return ((quads >> (r & 28)) & 15u) == 15u; };
+  const int s = __shfl_sync(0xffffffffu, slots, row), tok = s & 15;
   auto block_of = [&](int s) {
     const int page = s >> p.page_shift;
-    return p.pool + (((static_cast<int64_t>(page) * p.kv_heads + head) << (p.page_shift - 4)) + ((s - (page << p.page_shift)) >> 4)) * F.block;
+    return p.pool + (((static_cast<int64_t>(page) * p.kv_heads + head) << (p.page_shift - 4)) + ((s - (page << p.page_shift)) >> 4)) * F.block + (value ? F.part : 0);
   };
-  auto scales = [&](const uint8_t* part, int tok) { return reinterpret_cast<const __nv_bfloat16*>(part + F.codes) + tok * 2 * F.groups; };
-  uint32_t word[4 / ROWS];
-  __nv_bfloat16 ks[4 / ROWS], kz[4 / ROWS], vs[4 / ROWS], vz[4 / ROWS];
-  uint32_t vw[4 / ROWS];  // of the values, unless they come by quads
-  const QuantTile own;
-#pragma unroll
-  for (int r = 0; r < 4 / ROWS; ++r) {
-    const int s = max(0, __shfl_sync(0xffffffffu, slots, r * ROWS + lane / LANES)), tok = s & 15, g = l / (GROUP / 8);
+  // a row's scales, then its offsets, two a word (one group: both in a word)
+  uint32_t numbers[G];
+  uint4 word = make_uint4(0, 0, 0, 0);
+  if (s >= 0) {
     const uint8_t* block = block_of(s);
-    word[r] = reinterpret_cast<const uint32_t*>(block + tok * (D / 2))[(l & 3) * (D / 32) + (l >> 2)];
-    ks[r] = scales(block, tok)[g];
-    kz[r] = scales(block, tok)[F.groups + g];
-    vs[r] = scales(block + F.part, tok)[g];
-    vz[r] = scales(block + F.part, tok)[F.groups + g];
-    vw[r] = 0;
-    if (!quad) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        vw[r] |= ((static_cast<uint32_t>(block[F.part + quant_kv_value_byte(tok, (l >> 1) * 16 + i)]) >> (4 * (l & 1))) & 15u) << (4 * i);
-    }
+    for (int i = 0; i < G; ++i) numbers[i] = reinterpret_cast<const uint32_t*>(block + F.codes + tok * 4 * G)[i];
+    if (!value) word = *reinterpret_cast<const uint4*>(block + tok * (D / 2) + l * 16);
   }
-  if (quad && own.m < D / 16) {
-    const uint8_t* from = block_of(s0) + F.part + own.at(s0 & 15);
-    const uint32_t tile[2] = {*reinterpret_cast<const uint32_t*>(from), *reinterpret_cast<const uint32_t*>(from + 64)};
-    // byte own.a of a row's words of the tile, tokens 0, 2, 1, 3
-    const uint32_t low = (tile[0] & 0x0f0f0f0fu) | ((tile[1] << 4) & 0xf0f0f0f0u), high = ((tile[0] >> 4) & 0x0f0f0f0fu) | (tile[1] & 0xf0f0f0f0u);
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      uint8_t* to = reinterpret_cast<uint8_t*>(codes + ((b & 1) * 2 + (b >> 1)) * LANES + 2 * own.m) + own.a;
-      to[0] = static_cast<uint8_t>(low >> (8 * b));
-      to[4] = static_cast<uint8_t>(high >> (8 * b));
+  uint32_t w[4] = {word.x, word.y, word.z, word.w};  // eight codes each, of dimensions dim(i) on
+  auto dim = [&](int i) { return D == 128 ? 32 * i + 8 * l : 32 * (i & 1) + 16 * l + 8 * (i >> 1); };
+  if (value) {
+    // words (m / 4, g, of these four tokens, m % 4): 16 bytes are four tiles m of a g
+    const int q = lane / EACH, mg = lane % EACH >> 3, g = lane & 7, from = __shfl_sync(0xffffffffu, s0, 4 * q);
+    if (is_quad(4 * q)) {
+      const uint4 v = *reinterpret_cast<const uint4*>(block_of(from) + mg * 512 + g * 64 + ((from & 15) >> 2) * 16);
+      uint32_t* to = words + q * (D / 2) + mg * 32 + g;
+      to[0] = v.x; to[8] = v.y; to[16] = v.z; to[24] = v.w;
     }
-  }
-  if (quad) __syncwarp();
+    __syncwarp();
+    if (is_quad(row)) {
+      // byte b of the words of a tile is this token's, nibbles dimensions 16 m + g and 16 m + 8 + g
+      const int b = (row & 1) * 2 + ((row >> 1) & 1);
+      const uint32_t pick = b | (b + 4) << 4;
+      uint32_t row_words[4];
 #pragma unroll
-  for (int r = 0; r < 4 / ROWS; ++r) {
-    const int row = r * ROWS + lane / LANES;
-    if (__shfl_sync(0xffffffffu, slots, row) < 0) continue;
-    const int64_t at = ((t0 + row) * p.kv_heads + head) * D + l * 8;
-    const float k_s = __bfloat162float(ks[r]), k_z = __bfloat162float(kz[r]), v_s = __bfloat162float(vs[r]), v_z = __bfloat162float(vz[r]);
-    float x[8], y[8];
-    uint64_t c[4];
-    quant_kv_codes(word[r], c);
-    quant_kv_numbers(c, k_s, k_z, x);
-    quant_kv_codes(quad ? codes[row * LANES + l] : vw[r], c);
-    quant_kv_numbers(c, v_s, v_z, y);
-    constexpr float most = quant_kv_most<T>();
-    if (quant_kv_past(k_s, k_z, most) || quant_kv_past(v_s, v_z, most)) {
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t* at = words + (row >> 2) * (D / 2) + (2 * l + h) * 8;
+        const uint4 x = *reinterpret_cast<const uint4*>(at), y = *reinterpret_cast<const uint4*>(at + 4);
+        const uint32_t even = __byte_perm(__byte_perm(x.x, x.z, pick), __byte_perm(y.x, y.z, pick), 0x5410);
+        const uint32_t odd = __byte_perm(__byte_perm(x.y, x.w, pick), __byte_perm(y.y, y.w, pick), 0x5410);
+        row_words[2 * h] = (even & 0x0f0f0f0fu) | ((odd << 4) & 0xf0f0f0f0u);
+        row_words[2 * h + 1] = ((even >> 4) & 0x0f0f0f0fu) | (odd & 0xf0f0f0f0u);
+      }
+      *reinterpret_cast<uint4*>(codes + row * PITCH + 4 * l) = make_uint4(row_words[0], row_words[1], row_words[2], row_words[3]);
+    }
+    if (!__all_sync(0xffffffffu, is_quad(row) || s < 0)) {
+      const int m = lane % EACH >> 1, half = lane & 1;  // a tile, g = 0 .. 3 or 4 .. 7 of it
+      constexpr int TIMES = ROWS * EACH / 32;
+      uint32_t all[TIMES];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[i] = quant_kv_cut(x[i], most);
-        y[i] = quant_kv_cut(y[i], most);
+      for (int i = 0; i < TIMES; ++i) {  // (asked for together)
+        const int r = i * (32 / EACH) + lane / EACH, at = __shfl_sync(0xffffffffu, slots, r);
+        const uint8_t* d = block_of(max(at, 0)) + quant_kv_value_byte(max(at, 0) & 15, m * 16) + half * 256;
+        all[i] = at < 0 || is_quad(r) ? 0u : d[0] | d[64] << 8 | d[128] << 16 | static_cast<uint32_t>(d[192]) << 24;
+      }
+#pragma unroll
+      for (int i = 0; i < TIMES; ++i) {
+        const int r = i * (32 / EACH) + lane / EACH;
+        auto close = [](uint32_t x) { return static_cast<uint16_t>(((x | x >> 4) & 0xffu) | ((x >> 8 | x >> 12) & 0xff00u)); };  // four nibbles together
+        uint16_t* to = reinterpret_cast<uint16_t*>(codes + r * PITCH + 2 * m) + half;
+        if (!is_quad(r)) {
+          to[0] = close(all[i] & 0x0f0f0f0fu);
+          to[2] = close((all[i] >> 4) & 0x0f0f0f0fu);
+        }
       }
     }
-    stf8<T>(reinterpret_cast<T*>(p.k) + at, x);
-    stf8<T>(reinterpret_cast<T*>(p.v) + at, y);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = codes[row * PITCH + dim(i) / 8];
+  }
+  if (s < 0) return;
+  T* const to = reinterpret_cast<T*>(value ? p.v : p.k) + ((t0 + row) * p.kv_heads + head) * D;
+  auto number = [&](int i) { return __uint_as_float(i & 1 ? numbers[i >> 1] & 0xffff0000u : numbers[i >> 1] << 16); };
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int group = (D == 128 ? 32 * i : 32 * (i & 1)) / GROUP;
+    const float sc = number(group), z = number(G + group);
+    uint64_t c[4];
+    float x[8];
+    quant_kv_codes(w[i], c);
+    quant_kv_numbers(c, sc, z, x);
+    constexpr float most = quant_kv_most<T>();
+    if (quant_kv_past(sc, z, most)) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = quant_kv_cut(x[j], most);
+    }
+    stf8<T>(to + dim(i), x);
   }
 }
 
@@ -588,19 +667,25 @@ __global__ void __launch_bounds__(256, 3) quant_kv_pages_kernel(const QuantPages
 }
 
 struct StoreLaunch {
-  const QuantStoreParams& p;
+  QuantStoreParams& p;
   cudaStream_t stream;
   template <typename T, int D, int GROUP>
   int operator()() const {
-    return (int)launch_pdl(quant_kv_store_kernel<T, D, GROUP>, dim3((unsigned)((p.units + 7) / 8)), dim3(256), 0, stream, p);
+    constexpr int ROWS = 1024 / D;
+    p.units = ((int64_t)p.tokens + ROWS - 1) / ROWS * p.kv_heads * 2;
+    if (p.units > (int64_t)4 * 0x7fffffff) return -1;
+    return (int)launch_pdl(quant_kv_store_kernel<T, D, GROUP>, dim3((unsigned)((p.units + 3) / 4)), dim3(128), 0, stream, p);
   }
 };
 struct LoadLaunch {
-  const QuantLoadParams& p;
+  QuantLoadParams& p;
   cudaStream_t stream;
   template <typename T, int D, int GROUP>
   int operator()() const {
-    return (int)launch_pdl(quant_kv_load_kernel<T, D, GROUP>, dim3((unsigned)((p.units + 7) / 8)), dim3(256), 0, stream, p);
+    constexpr int ROWS = 1024 / D;
+    p.units = (p.rows + ROWS - 1) / ROWS * p.kv_heads * 2;
+    if (p.units > (int64_t)4 * 0x7fffffff) return -1;
+    return (int)launch_pdl(quant_kv_load_kernel<T, D, GROUP>, dim3((unsigned)((p.units + 3) / 4)), dim3(128), 0, stream, p);
   }
 };
 struct RopeLaunch {
@@ -656,8 +741,7 @@ int blitz_quant_kv_store(const void* k, int64_t k_row, const void* v, int64_t v_
   if (num_tokens <= 0) return 0;
   if (!quant_kv_supported(dim, group, page_size) || kv_heads < 1 || ((k_row | v_row) & 7)) return -1;
   if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(pool)) & 15) return -1;
-  QuantStoreParams p{k, v, k_row, v_row, slot, (uint8_t*)pool, ((int64_t)num_tokens + 3) / 4 * kv_heads, num_tokens, kv_heads, quant_kv_shift(page_size), max_pages, status};
-  if (p.units > (int64_t)8 * 0x7fffffff) return -1;
+  QuantStoreParams p{k, v, k_row, v_row, slot, (uint8_t*)pool, 0, num_tokens, kv_heads, quant_kv_shift(page_size), max_pages, status};
   return quant_kv_dispatch(dtype, dim, group, StoreLaunch{p, stream});
 }
 
@@ -679,8 +763,7 @@ int blitz_quant_kv_load(const void* pool, const int32_t* slot, int64_t rows, voi
   if (rows <= 0) return 0;
   if (!quant_kv_supported(dim, group, page_size) || kv_heads < 1) return -1;
   if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(pool)) & 15) return -1;
-  QuantLoadParams p{(const uint8_t*)pool, slot, k, v, rows, (rows + 3) / 4 * kv_heads, kv_heads, quant_kv_shift(page_size), max_pages, status};
-  if (p.units > (int64_t)8 * 0x7fffffff) return -1;
+  QuantLoadParams p{(const uint8_t*)pool, slot, k, v, rows, 0, kv_heads, quant_kv_shift(page_size), max_pages, status};
   return quant_kv_dispatch(dtype, dim, group, LoadLaunch{p, stream});
 }
 
