@@ -634,6 +634,8 @@ def _attn_decode_quant(q, cache, indices, indptr, last_page_len, q_heads, kv_hea
     out = _quant_attn(q, B, cache, q_heads, kv_heads, head_dim, page_size, window, keep_first, softcap, sink, out, indices, indptr, last_page_len, workspace)
     if B == 0:
         return out
+    if indices.shape[0] * (page_size // 16) * q_heads >= 1 << 31:      # (more than there are of 32 tokens, even where a window cuts one in two)
+        raise ValueError(f"{indices.shape[0]} pages of {page_size} tokens for {q_heads} query heads: too many chunks for a count in 32 bits")
     if workspace is None:
         workspace = torch.zeros(quant_attn_workspace_bytes(B, q_heads, head_dim), dtype=torch.uint8, device=q.device)
     elif workspace.dtype is not torch.uint8 or not workspace.is_contiguous() or workspace.data_ptr() & 255:
@@ -765,7 +767,7 @@ def attn_prefill_paged(q: torch.Tensor, kv_layer: KVLayer, page_indices: torch.T
     as for `attn_decode` (no bias beside a window, cap or sink; with sigmoid weights a bias of one column).
 
     Over a 4-bit cache (QuantKV): the pages that ``work`` refers to are read back first, into scratch of this call (of a bf16 model in
-    fp16, with its queries, scaled so that the type's range does not matter); tokens behind a sequence's end may hold anything; no gate,
+    fp16, as its queries enter, scaled so that the type's range does not matter); tokens behind a sequence's end may hold anything; no gate,
     bias, ``chunked`` or ``sigmoid``; no record of ``work`` refers to the first ``skip_pages`` entries of ``page_indices``."""
     if isinstance(kv_layer, QuantKV):
         _quant_refuses(gate, bias, chunked, sigmoid)
