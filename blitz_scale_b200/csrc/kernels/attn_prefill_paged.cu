@@ -52,7 +52,9 @@
 //
 // Operands in fp16 for a bf16 model (IO: the type of queries, sink and output): keys and values were divided by powers of two (a KV head's) so
 // that fp16 holds them, and each thread turns its row of queries into fp16 in shared memory, divided by a power of two near the row's
-// largest entry, as an item begins.  The row's scale and the output's factor make up for both.  A 4-bit cache read back for a pass comes so (quant_kv.cu).
+// largest entry, as an item begins.  The row's scale and the output's factor make up for both.  A 4-bit cache read back for a pass
+// comes so (quant_kv.cu).  8192 rows of nine prompts, 32 heads of 128: 187 us where a bf16 cache takes 174 (what an item waits for at its start, and
+// registers); with queries converted by a pass before it 184 us behind 20 us of that.
 //
 // Replaces FlashInfer's BatchPrefillWithRaggedKVCacheWrapper / paged wrapper calls and their host Plan()
 // (src/kernel/attention_prefill.cu:11-45, src/kernel/flashinfer_types.cu:24-49).

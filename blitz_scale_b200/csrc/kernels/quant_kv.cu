@@ -157,9 +157,12 @@ struct QuantStoreParams {
 
 // A warp takes keys or values of a head, of 8 rows (16 of 64 dimensions): a lane has 32 dimensions, so that what a group needs once, its ends
 // and its scale, is worked out by the one lane, two or four that have it (with eight dimensions a lane that was half of 195 instructions for
-// 256 numbers, and 8192 rows took 16.5 us).  The codes go
-// through shared memory: keys leave in rows of 16 bytes a lane.  A word of the values holds four tokens of two dimensions: where four rows
-// are the four tokens of a word (rows of a prompt) words are written, else (the tokens of a batch) every row's bytes.
+// 256 numbers, and 8192 rows took 16.5 us).  The codes go through shared memory: keys leave in rows of 16 bytes a lane.  A word of the values
+// holds four tokens of two dimensions: where four rows are the four tokens of a word (rows of a prompt) words are written, else (the tokens
+// of a batch) every row's bytes.
+//
+// Measured, 8 heads of 128: 8192 rows 12.0 us (44 MB, 3.7 TB/s, bound by the issue of instructions), 256 rows in pages of their own 2.6 us, one
+// row 2.0 us (latency: slot, row, code).  Blocks of 128 threads: of 256 they took 12.9, 3.1 and 2.15 us.
 template <typename T, int D, int GROUP>
 __global__ void __launch_bounds__(128) quant_kv_store_kernel(const QuantStoreParams p) {
   constexpr QuantKv F = quant_kv(D, GROUP);
@@ -250,6 +253,7 @@ struct QuantRopeParams {
 // there is what the 16-bit rows hold.  A block takes R tokens, whose angles it computes once; a warp four (row, head) pairs at a time:
 // four rows of a head (R = 4: values go out by words), or four heads of a row (R = 1: more blocks where there are few tokens).
 // STATIC: positions and slots that no kernel in flight writes: angles are ready when the projection is.
+// Measured, 32 query heads and 8 KV heads of 128: 8192 rows 51 us (195 MB, 3.8 TB/s; into a 16-bit cache 43 us), 256 rows 4.8 us, one row 3.0 us.
 template <typename T, int D, int GROUP, int R, bool STATIC>
 __global__ void __launch_bounds__(256) quant_kv_rope_kernel(const QuantRopeParams p) {
   constexpr QuantKv F = quant_kv(D, GROUP);
@@ -338,7 +342,8 @@ struct QuantLoadParams {
 
 // Rows of slots: a warp takes keys or values of a head, of 8 rows (16 of 64 dimensions), as the store does; a lane has four words of a row's codes,
 // spread so that the lanes of a row write next to each other.  Values of four tokens of a word come 16 bytes a lane and are put into rows
-// through shared memory; others byte by byte.
+// through shared memory; others byte by byte.  Measured, 8 heads of 128: 8192 rows 9.4 us (44 MB, 4.7 TB/s, most of them written), 256 rows
+// in pages of their own 2.85 us, one row 2.0 us.
 template <typename T, int D, int GROUP>
 __global__ void __launch_bounds__(128) quant_kv_load_kernel(const QuantLoadParams p) {
   constexpr QuantKv F = quant_kv(D, GROUP);
@@ -476,6 +481,7 @@ __device__ __forceinline__ int quant_kv_held(const QuantPagesParams& p, int n) {
 }
 // The largest magnitudes of a pass's keys and values, by head: of every block, a part of them.  Half a warp looks at the scales of the
 // keys of 16 tokens, the other half at those of the values.
+// Measured: 8200 tokens of 8 heads of 128 7.6 us, 3900 4.6 us (latency: record, page, scales).
 template <int D, int GROUP>
 __global__ void __launch_bounds__(256) quant_kv_span_kernel(const QuantPagesParams p, float* __restrict__ spans) {
   constexpr QuantKv F = quant_kv(D, GROUP);
@@ -514,7 +520,8 @@ __device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t a, uin
 }
 // A warp takes 16 tokens of a head.  Keys: four lanes a token, 32 codes each.  Values: a lane has four tokens of eight dimensions 8 apart, which
 // stmatrix turns into rows of a token.  Both go out from shared memory, whole rows at a time.
-// Bound by the 16-bit rows that it writes (four times the codes).
+// Bound by the 16-bit rows that it writes (four times the codes): 1024 pages of 64 tokens of 8 heads of 128 63 us (352 MB, 5.6 TB/s), 37 pages of 4 heads
+// of 64 3.4 us; for attention of portions 8200 tokens 15 us after their largest magnitudes are known.
 //
 // For attention of portions (WORK) the tokens behind a sequence's end are zeros, whatever the cache has there.  SCALED: keys and
 // values of a bf16 model go to fp16, which keeps three bits more of what z + s c is, divided by a power of two near the largest of their head, so that

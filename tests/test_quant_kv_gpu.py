@@ -153,7 +153,8 @@ def filled(ops, lens, H, D, group, page, dt, seed, behind=255):
 
 def tolerance(q, kept, scale, want, spread, weight_step, dt, group, value_step=0.0):
     """What arithmetic allows for rows q [n, heads, D] of a sequence.  Weights: a score is a sum of products that are exact in 32 bits, of
-    codes that carry an offset of at most 1024 (a sum of `group` of them is off by less than 2^-22 of its parts, 1040 |q| each), times s, and
+    codes that enter as numbers whose leading bit may be ten places up (a sum of `group` of them is off by less than 2^-22 of 1040 |q|
+    each), times s, and
     of offsets z times sums of q that are held in 16 bits: |error| <= scale sum_g (2^-12 s_g + 2^-16 |z_g|) sum |q|, and 2^-20 of
     the score for the rest.  Every weight, and their sum, is off by that factor at most, so twice.  Then the rounding of a weight times its
     scale (`weight_step`) times codes between -8 and 7, of values where they are read back (`value_step`), and of the output."""
@@ -209,8 +210,8 @@ def test_decode(ops, case, dt, splits):
         at = torch.tensor([n - 1])
         want = attention(q[s:s + 1], k, v, at, scale=scale, **opts)
         spread = attention(q[s:s + 1], k, 8 * vs.repeat_interleave(group, -1), at, scale=scale, **opts)[0]
-        # weights times scales in fp16 (below 2^-14 in steps of 2^-24, where the largest scale is at 2^6 at least); their products with codes up to
-        # 1039, 16 tokens at a time, and with 1032, are sums in 32 bits beside the output so far: 2^-22 of their parts
+        # weights times scales in fp16 (below 2^-14 in steps of 2^-24, where the largest scale is at 2^6 at least); their products with codes (as
+        # if up to 1039), 16 tokens at a time, and with 8, are sums in 32 bits beside the output so far: 2^-22 of their parts
         step = 2.0 ** -11 + 2.0 ** -15 + n / 16 * 2.0 ** -22
         tol = tolerance(q[s:s + 1], kept[s], scale, want, spread, step, dt, group) + n * 2.0 ** -28 * vs.max()
         worst = ((got[s] - want[0][0]).abs() / tol[0]).max().item()
