@@ -35,8 +35,8 @@
 //
 // Measured, bf16, 32 query heads over 8 of 128: 256 sequences of 512 tokens in groups of 32 40.3 us (172 MB, 4.3 TB/s; the 16-bit kernel
 // 98 us); one of 100003 in groups of 128 30.0 us (3.6 TB/s); 61 of 1100 on average in groups of 64 23.7 us (fp16); one of 977 10.3 us.  Bound by the stream where
-// it is long (copies alone take 31 us of the 40, the warps issue in three cycles of four); 10 us of every call are its ends: tables, first
-// pages, and pieces added up.
+// it is long (5.7 TB/s beside the ends; the warps issue in half of the cycles); 10 us of every call are its ends: tables, first pages, and
+// pieces added up.
 #include "launch.cuh"
 #include "ptx.cuh"
 #include "mma.cuh"

@@ -552,15 +552,19 @@ def quant_kv_load(cache: QuantKV, slot: torch.Tensor, *, dtype: torch.dtype = to
     _int32(slot, None, "slot")
     n, (pages, H, blocks, _) = slot.shape[0], pool.shape
     if k is None and v is None:
-        k, v = torch.empty((2, n, H, D), dtype=dtype, device=pool.device).unbind()
-    elif k is None:
-        k = torch.empty((n, H, D), dtype=v.dtype, device=pool.device)
-    elif v is None:
-        v = torch.empty((n, H, D), dtype=k.dtype, device=pool.device)
-    for t in (k, v):
-        if t.shape != (n, H, D) or not t.is_contiguous() or t.dtype != k.dtype or t.data_ptr() & 15:
-            raise ValueError(f"k and v: contiguous {(n, H, D)} of one type, got {tuple(t.shape)} {t.dtype}")
-    _quant(cache, slot, k, v)
+        if dtype not in _DT:
+            raise TypeError(f"kernels give fp16/bf16 tensors, not {dtype}")
+        _quant(cache, slot)
+        k, v = pool.new_empty((2, n, H, D), dtype=dtype).unbind()
+    else:
+        if k is None:
+            k = v.new_empty((n, H, D))
+        elif v is None:
+            v = k.new_empty((n, H, D))
+        for t in (k, v):
+            if t.shape != (n, H, D) or not t.is_contiguous() or t.dtype != k.dtype or t.data_ptr() & 15:
+                raise ValueError(f"k and v: contiguous {(n, H, D)} of one type, got {tuple(t.shape)} {t.dtype}")
+        _quant(cache, slot, k, v)
     rc = lib().blitz_quant_kv_load(pool.data_ptr(), slot.data_ptr(), n, k.data_ptr(), v.data_ptr(), H, D, group, 16 * blocks, pages, _status_ptr(pool), _dt(k),
                                    _stream())
     if rc:
@@ -575,7 +579,7 @@ def quant_kv_pages(cache: QuantKV, pages: torch.Tensor, *, dtype: torch.dtype = 
     n, (count, H, blocks, _) = pages.shape[0], pool.shape
     shape = (n, 2, 16 * blocks, H, D)
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=pool.device)
+        out = pool.new_empty(shape, dtype=dtype)
     elif out.shape != shape or not out.is_contiguous() or out.data_ptr() & 15:
         raise ValueError(f"out: contiguous {shape}, got {tuple(out.shape)}")
     _quant(cache, pages, out)
@@ -609,7 +613,7 @@ def _quant_attn(q: torch.Tensor, rows: int, cache: QuantKV, q_heads: int, kv_hea
     if sink is not None and (sink.dtype is not dt or sink.numel() != q_heads or not sink.is_contiguous()):
         raise ValueError(f"sink: {q_heads} numbers of {dt}")
     if out is None:
-        out = torch.empty((rows, width), dtype=dt, device=q.device)
+        out = q.new_empty((rows, width))
     else:
         size, step = out.shape, out.stride()
         if len(size) != 2 or size[0] < rows or size[1] < width or out.dtype is not dt or step[1] != 1 or (step[0] | out.data_ptr() >> 1) & 7:
