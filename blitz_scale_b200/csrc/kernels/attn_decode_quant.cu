@@ -25,7 +25,7 @@
 //
 // A warp takes chunks of 32 tokens by itself, through a ring of stages of its own; one more warp issues the copies (bulk copies: a
 // head's tokens in a page are one contiguous piece), a lane for each of the others.  Eleven warps have 168 registers each and none
-// spills; fifteen with 128 took 43.4 us where these take 40.3 (256 sequences of 512 tokens, 32 query heads over 8 of 128, groups of 32).
+// spills; fifteen with 128 took 43.4 us where these took 40.3 (256 sequences of 512 tokens, 32 query heads over 8 of 128, groups of 32).
 //
 // The chunks of all sequences of all heads, end to end, are cut into equal ranges, one per warp of the GPU, so that neither lengths nor the
 // number of sequences leave warps idle.  A sequence that is cut leaves its pieces' sums in shared memory, where the warps that end with it
@@ -33,8 +33,8 @@
 // pieces in several blocks go through scratch and a ticket per head, and the last block adds up.  The order is that of the ranges,
 // whoever is last.
 //
-// Measured, bf16, 32 query heads over 8 of 128: 256 sequences of 512 tokens in groups of 32 40.3 us (172 MB, 4.3 TB/s; the 16-bit kernel
-// 98 us); one of 100003 in groups of 128 30.0 us (3.6 TB/s); 61 of 1100 on average in groups of 64 23.7 us (fp16); one of 977 10.3 us.  Bound by the stream where
+// Measured, bf16, 32 query heads over 8 of 128: 256 sequences of 512 tokens in groups of 32 39.7 us (172 MB, 4.3 TB/s; the 16-bit kernel
+// 98 us); one of 100003 in groups of 128 29.0 us (3.75 TB/s); 61 of 1100 on average in groups of 64 23.7 us (fp16); one of 977 10.3 us.  Bound by the stream where
 // it is long (5.7 TB/s beside the ends; the warps issue in half of the cycles); 10 us of every call are its ends: tables, first pages, and
 // pieces added up.
 #include "launch.cuh"
@@ -103,6 +103,23 @@ struct QdCut {
   }
   __device__ __forceinline__ unsigned begin(unsigned v) const { return v * base + min(v, rem); }
   __device__ __forceinline__ unsigned range(unsigned x) const { return x < rem * (base + 1) ? x / (base + 1) : rem + (x - rem * (base + 1)) / base; }
+};
+// The ranges of a block's warps.  Where there is work enough, those that share their quarter of the SM with one more and the warp that copies,
+// not with two others, get 8 chunks where the others get 7: with equal ranges they were done 14 % earlier (one sequence of 100003 tokens
+// 30.0 -> 29.0 us, 256 of 512 40.1 -> 39.7).
+struct QdRanges {
+  unsigned first, x0, n;
+  bool equal;
+  __device__ __forceinline__ QdRanges(const QdCut& cut, unsigned block) {
+    first = block * cut.each;
+    x0 = cut.begin(first);
+    n = cut.begin(first + cut.each) - x0;
+    equal = cut.each < kQdWarps || cut.base < 8;
+  }
+  __device__ __forceinline__ unsigned begin(const QdCut& cut, unsigned w) const {
+    static_assert(kQdWarps == 11, "warps 3 and 7");
+    return equal ? cut.begin(first + w) : x0 + n * (7 * w + (w > 3 ? 1 : 0) + (w > 7 ? 1 : 0)) / 79;
+  }
 };
 // A walk over the pieces of a range of chunks.
 struct QdWalk {
@@ -314,7 +331,7 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
 
   T* const out = reinterpret_cast<T*>(p.out);
   const QdCut cut(static_cast<unsigned>(tab.before[p.batch]) * p.heads, gridDim.x);
-  const unsigned first_warp = blockIdx.x * cut.each;
+  const QdRanges mine(cut, blockIdx.x);
   const int warps = cut.each;
   // (sequences without a visible key are in nobody's range: their output is zero)
   for (int b = blockIdx.x; b < p.batch; b += gridDim.x)
@@ -323,8 +340,8 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
 
   if (warp == kQdWarps) {
     // ---------------------------------------------------------------- copies: a lane for each warp
-    const unsigned v = first_warp + min(lane, warps - 1);
-    QdWalk walk = qd_walk(tab, p.batch, cut.begin(v), lane < warps ? cut.begin(v + 1) : 0u);
+    const unsigned v = min(lane, warps - 1);
+    QdWalk walk = qd_walk(tab, p.batch, mine.begin(cut, v), lane < warps ? mine.begin(cut, v + 1) : 0u);
     QdPiece it{};
     QdSeen see{};
     bool more = qd_next(tab, p.batch, walk, it);
@@ -419,7 +436,7 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
     bool ok = true;
     volatile int* const rec = records + warp * 16;
     {
-      const QdWalk walk = qd_walk(tab, p.batch, cut.begin(first_warp + warp), cut.begin(first_warp + warp + 1));
+      const QdWalk walk = qd_walk(tab, p.batch, mine.begin(cut, warp), mine.begin(cut, warp + 1));
       rec[0] = walk.x; rec[1] = walk.end; rec[2] = walk.head; rec[3] = walk.b;
     }
     for (;;) {
@@ -691,7 +708,7 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
         o[i][0] = fmaf((o[i][0] + eight[j][0]) * 0x1p24f, up, zs[j][0]); o[i][1] = fmaf((o[i][1] + eight[j][1]) * 0x1p24f, up, zs[j][1]);
         o[i][2] = fmaf((o[i][2] + eight[j][2]) * 0x1p20f, up, zs[j][0]); o[i][3] = fmaf((o[i][3] + eight[j][3]) * 0x1p20f, up, zs[j][1]);
       }
-      const unsigned X0 = cut.begin(first_warp), X1 = cut.begin(first_warp + warps), x0 = cut.begin(first_warp + warp), x1 = cut.begin(first_warp + warp + 1);
+      const unsigned X0 = mine.x0, X1 = mine.x0 + mine.n, x0 = mine.begin(cut, warp), x1 = mine.begin(cut, warp + 1);
       if (it.start >= x0 && it.stop <= x1) {
         float r[2];
 #pragma unroll
@@ -750,12 +767,12 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
       }
       // The warps of this block that end with the sequence share its heads (one that goes on with the next sequence has them to itself, where
       // nobody else has a piece); the i-th lane looks after the i-th of all warps that have one.
-      const unsigned at = cut.begin(first_warp + min(lane, warps)), behind = cut.begin(first_warp + min(lane + 1, warps));
+      const unsigned at = mine.begin(cut, min(lane, warps)), behind = mine.begin(cut, min(lane + 1, warps));
       const bool has = lane < warps && at < it.stop && behind > it.start;
       const uint32_t having = __ballot_sync(0xffffffffu, has), ending = __ballot_sync(0xffffffffu, has && behind <= it.stop);
       const int w0 = __ffs(having) - 1, n = __popc(having), each = max(1, __popc(ending)), h0 = warp - w0;
       if (h0 >= p.rep || (n > 1 && x1 > it.stop)) continue;
-      const unsigned begin = cut.begin(first_warp + min(w0 + lane, warps));
+      const unsigned begin = mine.begin(cut, min(w0 + lane, warps));
       const int from = (lane < n && begin < it.start ? (w0 + lane) * (ring_bytes / 4) : kQdWarps * ring_bytes / 4 + min(w0 + lane, kQdWarps - 1) * slot);
       if (!qd_wait(records + min(w0 + lane, kQdWarps - 1) * 16 + (begin < it.start ? 9 : 8), lane < n, abort_flag)) {
         if (p.status && lane == 0) atomicCAS(p.status, 0, kStatusTimeoutEpilogue);
