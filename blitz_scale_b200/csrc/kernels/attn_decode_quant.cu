@@ -990,7 +990,7 @@ int blitz_attn_decode_quant(const void* q, int64_t q_stride, const void* pool, c
                             int q_heads, int kv_heads, int dim, int group, int page_size, int max_pages, float sm_scale, int window,
                             int keep_first, float softcap, const void* sink, int static_table, int* status, int dtype, cudaStream_t stream) {
   if (batch <= 0) return 0;
-  if (!quant_kv_supported(dim, group, page_size) || kv_heads < 1 || q_heads % kv_heads || window < 0 || keep_first < 0 || softcap < 0.f) return -1;
+  if (!quant_kv_supported(dim, group, page_size) || max_pages < 1 || kv_heads < 1 || q_heads % kv_heads || window < 0 || keep_first < 0 || softcap < 0.f) return -1;
   if (((q_stride | out_stride) & 7) || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(pool) | reinterpret_cast<uintptr_t>(workspace)) & 15)) return -1;
   if (workspace == nullptr || workspace_bytes < blitz_attn_decode_quant_workspace_bytes(batch, q_heads, dim)) return -1;
   DecodeQuantParams p;

@@ -746,7 +746,7 @@ using namespace blitz;
 int blitz_quant_kv_store(const void* k, int64_t k_row, const void* v, int64_t v_row, const int32_t* slot, void* pool, int num_tokens,
                          int kv_heads, int dim, int group, int page_size, int max_pages, int* status, int dtype, cudaStream_t stream) {
   if (num_tokens <= 0) return 0;
-  if (!quant_kv_supported(dim, group, page_size) || kv_heads < 1 || ((k_row | v_row) & 7)) return -1;
+  if (!quant_kv_supported(dim, group, page_size) || max_pages < 1 || kv_heads < 1 || ((k_row | v_row) & 7)) return -1;
   if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(pool)) & 15) return -1;
   QuantStoreParams p{k, v, k_row, v_row, slot, (uint8_t*)pool, 0, num_tokens, kv_heads, quant_kv_shift(page_size), max_pages, status};
   return quant_kv_dispatch(dtype, dim, group, StoreLaunch{p, stream});
@@ -758,7 +758,7 @@ int blitz_quant_kv_store(const void* k, int64_t k_row, const void* v, int64_t v_
 int blitz_quant_kv_rope(void* qkv, const int32_t* pos, const int32_t* slot, void* pool, int num_tokens, int q_heads, int kv_heads, int dim, int group,
                         int page_size, int max_pages, float rope_theta, int static_meta, int* status, int dtype, cudaStream_t stream) {
   if (num_tokens <= 0) return 0;
-  if (!quant_kv_supported(dim, group, page_size) || kv_heads < 1 || q_heads < 0) return -1;
+  if (!quant_kv_supported(dim, group, page_size) || max_pages < 1 || kv_heads < 1 || q_heads < 0) return -1;
   if ((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(pool)) & 15) return -1;
   QuantRopeParams p{qkv, pos, slot, (uint8_t*)pool, num_tokens, q_heads, kv_heads, quant_kv_shift(page_size), max_pages, log2f(rope_theta), status};
   return quant_kv_dispatch(dtype, dim, group, RopeLaunch{p, static_meta, stream});
@@ -768,7 +768,7 @@ int blitz_quant_kv_rope(void* qkv, const int32_t* pos, const int32_t* slot, void
 int blitz_quant_kv_load(const void* pool, const int32_t* slot, int64_t rows, void* k, void* v, int kv_heads, int dim, int group, int page_size,
                         int max_pages, int* status, int dtype, cudaStream_t stream) {
   if (rows <= 0) return 0;
-  if (!quant_kv_supported(dim, group, page_size) || kv_heads < 1) return -1;
+  if (!quant_kv_supported(dim, group, page_size) || max_pages < 1 || kv_heads < 1) return -1;
   if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(pool)) & 15) return -1;
   QuantLoadParams p{(const uint8_t*)pool, slot, k, v, rows, 0, kv_heads, quant_kv_shift(page_size), max_pages, status};
   return quant_kv_dispatch(dtype, dim, group, LoadLaunch{p, stream});
@@ -778,7 +778,7 @@ int blitz_quant_kv_load(const void* pool, const int32_t* slot, int64_t rows, voi
 int blitz_quant_kv_pages(const void* pool, const int32_t* pages, int64_t count, void* k, void* v, int kv_heads, int dim, int group, int page_size,
                          int page_rows, int max_pages, int* status, int dtype, cudaStream_t stream) {
   if (count <= 0) return 0;
-  if (!quant_kv_supported(dim, group, page_size) || kv_heads < 1 || page_rows < page_size) return -1;
+  if (!quant_kv_supported(dim, group, page_size) || max_pages < 1 || kv_heads < 1 || page_rows < page_size) return -1;
   if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(pool)) & 15) return -1;
   QuantPagesParams p{(const uint8_t*)pool, pages, k, v, count * kv_heads * (page_size / 16), kv_heads, page_size, page_rows, max_pages, status};
   return quant_kv_dispatch(dtype, dim, group, PagesLaunch{p, stream});
@@ -804,7 +804,7 @@ int64_t blitz_quant_kv_portion_bytes(int64_t pages, int64_t first, int kv_heads,
 int blitz_quant_kv_portion(const void* pool, const int32_t* pages, int64_t count, int64_t first, const int32_t* work, int entries, int kv_heads, int dim,
                            int group, int page_size, int max_pages, void* scratch, int* status, int dtype, cudaStream_t stream) {
   if (count <= 0 || entries <= 0) return 0;
-  if (!quant_kv_supported(dim, group, page_size) || kv_heads < 1 || kv_heads > 128 || first < 0 || count + first > 0x7fffffff) return -1;
+  if (!quant_kv_supported(dim, group, page_size) || max_pages < 1 || kv_heads < 1 || kv_heads > 128 || first < 0 || count + first > 0x7fffffff) return -1;
   if ((reinterpret_cast<uintptr_t>(work) | reinterpret_cast<uintptr_t>(pool) | reinterpret_cast<uintptr_t>(scratch)) & 15) return -1;
   int64_t at[5];
   blitz_quant_kv_portion_bytes(count, first, kv_heads, dim, page_size, dtype, at);

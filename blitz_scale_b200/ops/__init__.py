@@ -480,6 +480,8 @@ def _quant(cache: QuantKV, *others: Optional[torch.Tensor]) -> torch.Tensor:
     blocks = shape[2]
     if blocks < 1 or blocks & (blocks - 1):
         raise ValueError(f"pages of a 4-bit cache hold 16 tokens times a power of two, got {16 * blocks}")
+    if shape[0] < 1 or shape[1] < 1:        # (a kernel reads the first page where it is told one that there is not)
+        raise ValueError(f"a cache without pages or heads: {tuple(shape)}")
     if at < 0 or at != _raw_device():
         raise ValueError(f"a cache on {pool.device}: the kernels run on the current CUDA device")
     for t in others:

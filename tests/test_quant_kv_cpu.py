@@ -131,3 +131,14 @@ def test_engines_that_take_no_4_bit_cache():
     for model, more in (("fafudra_tiny", {}), ("tiny", dict(tp=2))):
         with pytest.raises(ValueError, match="uniform models on one GPU"):
             Engine(model, num_pages=4, device=cpu, kv_bits=4, **more)
+
+
+def test_caches_without_pages_refused():
+    t, k = torch.zeros(3, dtype=torch.int32), torch.zeros(3, 128, dtype=torch.bfloat16)
+    empty = ops.quant_kv_pool(0, 16, 2, 64, 32, device="cpu")
+    q, base = torch.zeros(2, 256, dtype=torch.bfloat16), dict(q_heads=4, kv_heads=2, head_dim=64, page_size=16)
+    for call in (lambda: ops.quant_kv_store(k, k, t, empty), lambda: ops.quant_kv_load(empty, t), lambda: ops.quant_kv_pages(empty, t),
+                 lambda: ops.attn_decode(q, empty, t, t, t[:2], **base), lambda: ops.attn_prefill_paged(q, empty, t, torch.zeros(1, 8, dtype=torch.int32), **base),
+                 lambda: ops.rope_kv_store(torch.zeros(3, 8 * 64, dtype=torch.bfloat16), t, t, empty, rope_theta=1e4, **base)):
+        with pytest.raises(ValueError, match="without pages"):
+            call()

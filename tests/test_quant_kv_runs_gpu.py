@@ -111,3 +111,31 @@ def test_chunks_that_do_not_fit_are_refused(ops):
     table = torch.zeros(1 << 20, dtype=torch.int32, device=DEV)
     with pytest.raises(ValueError, match="chunks"):
         ops.attn_decode(q, cache, table, t([0, 1]), t([1]), q_heads=8, kv_heads=1, head_dim=64, page_size=1 << 16)
+
+
+def test_pages_that_there_are_not(ops):
+    """A page or slot behind the cache is an error that the host reads; nothing is written for it, and rows beside it are what they were."""
+    H, D, group, page, n = 2, 64, 32, 16, 40
+    cache, table, indptr, last, _ = filled(ops, [n], H, D, group, page, torch.bfloat16, 9)
+    pages, t = cache.pool.shape[0], lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    k, before = rows(3, H, D, torch.bfloat16, 10).to(DEV), cache.pool.clone()
+    qkv = torch.zeros(2, 4 * H * D, dtype=torch.bfloat16, device=DEV)
+    more = dict(q_heads=2 * H, kv_heads=H, head_dim=D, page_size=page)
+    q = torch.ones(n, 2 * H * D, dtype=torch.bfloat16, device=DEV)
+    out = torch.full((3, 2, page, H, D), 5.0, dtype=torch.bfloat16, device=DEV)
+    load = torch.full((3, H, D), 5.0, dtype=torch.bfloat16, device=DEV)
+    far = [pages * page, (1 << 31) - 1]
+    calls = [lambda: ops.quant_kv_store(k[:2], k[:2], t(far), cache), lambda: ops.quant_kv_load(cache, t([far[0], 1, far[1]]), k=load, v=load.clone()),
+             lambda: ops.quant_kv_pages(cache, t([pages, 0, -1]), out=out), lambda: ops.rope_kv_store(qkv, t([0, 1]), t(far), cache, rope_theta=1e4, **more)]
+    for bad in (pages, -1, 1 << 30):
+        wrong = table.clone()
+        wrong[1] = bad
+        calls += [lambda w=wrong: ops.attn_decode(q[:1], cache, w, indptr, last, **more),
+                  lambda w=wrong: ops.attn_prefill_paged(q, cache, w, ops.prefill_work_list([n], [n], page, DEV), **more)]
+    for i, call in enumerate(calls):
+        call()
+        with pytest.raises(RuntimeError):
+            ops.check_status()
+        assert torch.equal(cache.pool, before), i
+    assert (out[[0, 2]] == 5.0).all() and torch.equal(out[1, 0].flatten(0, 1), ops.quant_kv_load(cache, torch.arange(page, dtype=torch.int32, device=DEV))[0].flatten(0, 1))
+    assert (load[[0, 2]] == 5.0).all() and not (load[1] == 5.0).all()
