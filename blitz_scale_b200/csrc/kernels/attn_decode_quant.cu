@@ -31,12 +31,14 @@
 // number of sequences leave warps idle.  A sequence that is cut leaves its pieces' sums in shared memory, where the warps that end with it
 // wait for them and add them up, a head each (the warp it begins in comes to it last, the next one began with it: nobody waits long);
 // pieces in several blocks go through scratch and a ticket per head, and the last block adds up.  The order is that of the ranges,
-// whoever is last.
+// whoever is last.  Where whole sequences of a head make nearly equal work, that hand-over (2.5 us) is saved: a
+// block takes one of them (where there are no more of them than blocks and the longest costs less than that beside an equal share), or
+// the cuts between blocks move to the nearest beginning of one (where the longest alone costs less than that).
 //
 // Measured, bf16, 32 query heads over 8 of 128: 256 sequences of 512 tokens in groups of 32 39.7 us (172 MB, 4.3 TB/s; the 16-bit kernel
-// 98 us); one of 100003 in groups of 128 29.0 us (3.75 TB/s); 61 of 1100 on average in groups of 64 23.7 us (fp16); one of 977 10.3 us.  Bound by the stream where
-// it is long (5.7 TB/s beside the ends; the warps issue in half of the cycles); 10 us of every call are its ends: tables, first pages, and
-// pieces added up.
+// 98 us); one of 100003 in groups of 128 29.0 us (3.75 TB/s); 61 of 1100 on average in groups of 64 23.7 us (fp16); one of 977 9.5 us.  Bound by the stream where
+// it is long (5.7 TB/s beside the ends; the warps issue in half of the cycles); 9 to 10 us of every call are its ends: tables, first
+// pages, and pieces added up.
 #include "launch.cuh"
 #include "ptx.cuh"
 #include "mma.cuh"
@@ -63,6 +65,7 @@ struct DecodeQuantParams {
   float* part;         // [2 blocks][rep][D] sums, then [2 blocks][rep] of (maximum, sum of weights)
   int batch, kv_heads, heads, div, rep;  // heads: groups of at most 8 query heads, div of which share a KV head; rep: query heads of one
   int page_size, page_shift, max_pages, stages, static_table;
+  unsigned slack;  // chunks, of all blocks together, in the time that adding up pieces of several blocks takes
   float sign, scale_log2, cap_scale, cap_log2;  // the scale's sign (0, NaN: itself) goes into the queries, its magnitude into the factors
   int window, keep_first;
   const void* sink;
@@ -92,7 +95,7 @@ __device__ __forceinline__ QdSeen qd_seen(const DecodeQuantParams& p, int len) {
   v.c_window = max(v.lo / kQdChunk, v.n_first);
   return v;
 }
-// How `all` chunks are cut into ranges: `each` warps of a block take one (all of them where there are chunks enough; few chunks go to
+// How `all` chunks are cut into equal ranges: `each` warps of a block take one (all of them where there are chunks enough; few chunks go to
 // more blocks, whose warps then have an SM's pipes to themselves).
 struct QdCut {
   unsigned each, base, rem;
@@ -108,17 +111,20 @@ struct QdCut {
 // not with two others, get 8 chunks where the others get 7: with equal ranges they were done 14 % earlier (one sequence of 100003 tokens
 // 30.0 -> 29.0 us, 256 of 512 40.1 -> 39.7).
 struct QdRanges {
-  unsigned first, x0, n;
-  bool equal;
+  unsigned x0, n, base, rem;
+  bool weighted;
   __device__ __forceinline__ QdRanges(const QdCut& cut, unsigned block) {
-    first = block * cut.each;
+    const unsigned first = block * cut.each;
     x0 = cut.begin(first);
     n = cut.begin(first + cut.each) - x0;
-    equal = cut.each < kQdWarps || cut.base < 8;
+    base = cut.base;
+    rem = cut.rem > first ? min(cut.rem - first, cut.each) : 0u;
+    weighted = cut.each == kQdWarps && base >= 8;
   }
-  __device__ __forceinline__ unsigned begin(const QdCut& cut, unsigned w) const {
+  __device__ __forceinline__ QdRanges(unsigned begin, unsigned end) : x0(begin), n(end - begin), base(n / kQdWarps), rem(n % kQdWarps), weighted(base >= 8) {}
+  __device__ __forceinline__ unsigned begin(unsigned w) const {
     static_assert(kQdWarps == 11, "warps 3 and 7");
-    return equal ? cut.begin(first + w) : x0 + n * (7 * w + (w > 3 ? 1 : 0) + (w > 7 ? 1 : 0)) / 79;
+    return x0 + (weighted ? n * (7 * w + (w > 3 ? 1 : 0) + (w > 7 ? 1 : 0)) / 79 : w * base + min(w, rem));
   }
 };
 // A walk over the pieces of a range of chunks.
@@ -145,6 +151,20 @@ __device__ __forceinline__ QdWalk qd_walk(const QdTables& t, int batch, unsigned
     w.b = lo;
   }
   return w;
+}
+// The beginning of a sequence of a head that is nearest to chunk x of all.
+__device__ __forceinline__ unsigned qd_nearest(const QdTables& t, int batch, unsigned x) {
+  const unsigned each = t.before[batch], base = x / each * each;
+  const int y = x - base;
+  int lo = 0, hi = batch;  // the last one at or before y
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (t.before[mid] <= y) lo = mid;
+    else hi = mid - 1;
+  }
+  if (lo == batch) return base + each;
+  const int below = t.before[lo], above = t.before[lo + 1];
+  return base + (y - below <= above - y ? below : above);
 }
 __device__ __forceinline__ bool qd_next(const QdTables& t, int batch, QdWalk& w, QdPiece& it) {
   if (w.x >= w.end) return false;
@@ -311,8 +331,13 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
   __syncthreads();
   if (warp == 0) {
     const int each = (p.batch + 31) / 32, b0 = min(p.batch, lane * each), b1 = min(p.batch, b0 + each);
-    int sum = 0;
-    for (int b = b0; b < b1; ++b) sum += tab.before[b + 1];
+    int sum = 0, most = 0;
+    for (int b = b0; b < b1; ++b) {
+      sum += tab.before[b + 1];
+      most = max(most, tab.before[b + 1]);
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0) abort_flag[1] = most;
     int total = sum;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -327,12 +352,22 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
     }
   }
   __syncthreads();
+  const unsigned all = static_cast<unsigned>(tab.before[p.batch]) * p.heads, share = all / gridDim.x, items = p.batch * p.heads;
+  const unsigned most = abort_flag[1], slack = min(64u, p.slack / min(gridDim.x, items));
+  // Measured, equal shares -> whole sequences, us: 1 of 977 tokens 10.4 -> 9.5, 8 of 1000 11.7 -> 10.1, 16 of 4096 23.5 -> 22.3; with moved cuts 256
+  // of 100 18.6 -> 16.9, but 256 of 512 39.7 -> 40.5 (blocks that have 224 chunks beside those that have 208), so not for shares above 128.
+  const bool own = items <= gridDim.x && most <= share + slack, whole = own || (most <= slack && share <= 128);
+  auto cut_at = [&](unsigned c) {  // between blocks c - 1 and c
+    if (own) return c >= items ? all : static_cast<unsigned>(tab.before[p.batch]) * (c / p.batch) + tab.before[c % p.batch];
+    const unsigned x = c * share + min(c, all % gridDim.x);
+    return x == all ? all : qd_nearest(tab, p.batch, x);
+  };
   ptx::griddep_wait();
 
   T* const out = reinterpret_cast<T*>(p.out);
-  const QdCut cut(static_cast<unsigned>(tab.before[p.batch]) * p.heads, gridDim.x);
-  const QdRanges mine(cut, blockIdx.x);
-  const int warps = cut.each;
+  const QdCut cut(all, gridDim.x);
+  const QdRanges mine = whole ? QdRanges(cut_at(blockIdx.x), cut_at(blockIdx.x + 1)) : QdRanges(cut, blockIdx.x);
+  const int warps = whole ? kQdWarps : cut.each;
   // (sequences without a visible key are in nobody's range: their output is zero)
   for (int b = blockIdx.x; b < p.batch; b += gridDim.x)
     if (tab.before[b] == tab.before[b + 1])
@@ -341,7 +376,7 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
   if (warp == kQdWarps) {
     // ---------------------------------------------------------------- copies: a lane for each warp
     const unsigned v = min(lane, warps - 1);
-    QdWalk walk = qd_walk(tab, p.batch, mine.begin(cut, v), lane < warps ? mine.begin(cut, v + 1) : 0u);
+    QdWalk walk = qd_walk(tab, p.batch, mine.begin(v), lane < warps ? mine.begin(v + 1) : 0u);
     QdPiece it{};
     QdSeen see{};
     bool more = qd_next(tab, p.batch, walk, it);
@@ -436,7 +471,7 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
     bool ok = true;
     volatile int* const rec = records + warp * 16;
     {
-      const QdWalk walk = qd_walk(tab, p.batch, mine.begin(cut, warp), mine.begin(cut, warp + 1));
+      const QdWalk walk = qd_walk(tab, p.batch, mine.begin(warp), mine.begin(warp + 1));
       rec[0] = walk.x; rec[1] = walk.end; rec[2] = walk.head; rec[3] = walk.b;
     }
     for (;;) {
@@ -708,7 +743,7 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
         o[i][0] = fmaf((o[i][0] + eight[j][0]) * 0x1p24f, up, zs[j][0]); o[i][1] = fmaf((o[i][1] + eight[j][1]) * 0x1p24f, up, zs[j][1]);
         o[i][2] = fmaf((o[i][2] + eight[j][2]) * 0x1p20f, up, zs[j][0]); o[i][3] = fmaf((o[i][3] + eight[j][3]) * 0x1p20f, up, zs[j][1]);
       }
-      const unsigned X0 = mine.x0, X1 = mine.x0 + mine.n, x0 = mine.begin(cut, warp), x1 = mine.begin(cut, warp + 1);
+      const unsigned X0 = mine.x0, X1 = mine.x0 + mine.n, x0 = mine.begin(warp), x1 = mine.begin(warp + 1);
       if (it.start >= x0 && it.stop <= x1) {
         float r[2];
 #pragma unroll
@@ -767,12 +802,12 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
       }
       // The warps of this block that end with the sequence share its heads (one that goes on with the next sequence has them to itself, where
       // nobody else has a piece); the i-th lane looks after the i-th of all warps that have one.
-      const unsigned at = mine.begin(cut, min(lane, warps)), behind = mine.begin(cut, min(lane + 1, warps));
+      const unsigned at = mine.begin(min(lane, warps)), behind = mine.begin(min(lane + 1, warps));
       const bool has = lane < warps && at < it.stop && behind > it.start;
       const uint32_t having = __ballot_sync(0xffffffffu, has), ending = __ballot_sync(0xffffffffu, has && behind <= it.stop);
       const int w0 = __ffs(having) - 1, n = __popc(having), each = max(1, __popc(ending)), h0 = warp - w0;
       if (h0 >= p.rep || (n > 1 && x1 > it.stop)) continue;
-      const unsigned begin = mine.begin(cut, min(w0 + lane, warps));
+      const unsigned begin = mine.begin(min(w0 + lane, warps));
       const int from = (lane < n && begin < it.start ? (w0 + lane) * (ring_bytes / 4) : kQdWarps * ring_bytes / 4 + min(w0 + lane, kQdWarps - 1) * slot);
       if (!qd_wait(records + min(w0 + lane, kQdWarps - 1) * 16 + (begin < it.start ? 9 : 8), lane < n, abort_flag)) {
         if (p.status && lane == 0) atomicCAS(p.status, 0, kStatusTimeoutEpilogue);
@@ -999,6 +1034,7 @@ int blitz_attn_decode_quant(const void* q, int64_t q_stride, const void* pool, c
   p.part = (float*)((char*)workspace + ((int64_t)batch * q_heads * 4 + 255) / 256 * 256);
   p.page_size = page_size; p.max_pages = max_pages; p.page_shift = 0; p.stages = 2;
   while ((1 << p.page_shift) < page_size) ++p.page_shift;
+  p.slack = 15000000u / (2 * quant_kv(dim, group).block);  // 2.5 us at 6 TB/s (and 64 chunks of a block at the most, whose warps take 0.4 us for one)
   const float size = sm_scale < 0.f ? -sm_scale : sm_scale > 0.f ? sm_scale : 1.f;
   p.sign = sm_scale < 0.f ? -1.f : sm_scale > 0.f ? 1.f : sm_scale;
   p.scale_log2 = size * 1.4426950408889634f; p.cap_scale = softcap > 0.f ? size / softcap : 0.f; p.cap_log2 = softcap * 1.4426950408889634f;

@@ -70,6 +70,32 @@ def test_rows_in_runs(ops, D, group, dt, longest):
     assert int((cache.pool != 0).any(-1).sum()) <= int(want.sum()) * H
 
 
+# sequences of a head that a block has to itself, several that share one, some that are cut; empty ones among them
+WHOLE = [([32 * 37] * 18, 8), ([900 + 31 * i for i in range(18)] + [0], 8), ([0, 0, 1], 1), ([1] * 37, 4), ([200 - 3 * i for i in range(61)], 8),
+         ([0, 33] * 130 + [1], 4), ([3 * i for i in range(200)], 2), ([700] * 20, 8), ([5000] + [20] * 40, 2)]
+
+
+@pytest.mark.parametrize("case", range(len(WHOLE)))
+@pytest.mark.parametrize("window", [0, 70])
+def test_blocks_of_whole_sequences(ops, case, window):
+    (lens, H), rep, D, group, page, dt = WHOLE[case], 4, 64, 32, 16, torch.float16
+    cache, table, indptr, last, kept = filled(ops, lens, H, D, group, page, dt, 10 * case)
+    q = torch.randn(len(lens), rep * H, D, generator=torch.Generator().manual_seed(case)).to(dt)
+    got = ops.attn_decode(q.flatten(1).to(DEV), cache, table, indptr, last, q_heads=rep * H, kv_heads=H, head_dim=D, page_size=page, window=window)
+    got = got.cpu().double().view(len(lens), rep * H, D)
+    for s, n in enumerate(lens):
+        if n == 0:
+            assert not got[s].any()
+            continue
+        k, v, ks, kz, vs = kept[s]
+        at = torch.tensor([n - 1])
+        want = attention(q[s:s + 1], k, v, at, scale=D ** -0.5, window=window)
+        spread = attention(q[s:s + 1], k, 8 * vs.repeat_interleave(group, -1), at, scale=D ** -0.5, window=window)[0]
+        step = 2.0 ** -11 + 2.0 ** -15 + n / 16 * 2.0 ** -22        # (as for single tokens in general)
+        tol = tolerance(q[s:s + 1], kept[s], D ** -0.5, want, spread, step, dt, group) + n * 2.0 ** -28 * vs.max()
+        assert ((got[s] - want[0][0]).abs() <= tol[0]).all(), (s, n)
+
+
 def test_portions_of_many_rounds(ops):
     """More work than blocks, tiles of one row, of all rows and of none, rows of queries 2^-40 to 2^2 as large as others."""
     n, Q, H, D, group, page, dt = [1, 128, 129, 256, 257, 400, 700, 511], 32, 8, 128, 64, 64, torch.bfloat16
