@@ -31,12 +31,11 @@
 // number of sequences leave warps idle.  A sequence that is cut leaves its pieces' sums in shared memory, where the warps that end with it
 // wait for them and add them up, a head each (the warp it begins in comes to it last, the next one began with it: nobody waits long);
 // pieces in several blocks go through scratch and a ticket per head, and the last block adds up.  The order is that of the ranges,
-// whoever is last.  Where whole sequences of a head make nearly equal work, that hand-over (2.5 us) is saved: a
-// block takes one of them (where there are no more of them than blocks and the longest costs less than that beside an equal share), or
-// the cuts between blocks move to the nearest beginning of one (where the longest alone costs less than that).
+// whoever is last.  Where there are no more sequences of heads than blocks, and the longest costs less beside an equal share than
+// that hand-over (2.5 us), a block takes one of them whole.
 //
 // Measured, bf16, 32 query heads over 8 of 128: 256 sequences of 512 tokens in groups of 32 39.7 us (172 MB, 4.3 TB/s; the 16-bit kernel
-// 98 us); one of 100003 in groups of 128 29.0 us (3.75 TB/s); 61 of 1100 on average in groups of 64 23.7 us (fp16); one of 977 9.5 us.  Bound by the stream where
+// 98 us); one of 100003 in groups of 128 29.0 us (3.75 TB/s); 61 of 1100 on average in groups of 64 23.7 us (fp16); one of 977 9.2 us.  Bound by the stream where
 // it is long (5.7 TB/s beside the ends; the warps issue in half of the cycles); 9 to 10 us of every call are its ends: tables, first
 // pages, and pieces added up.
 #include "launch.cuh"
@@ -65,7 +64,7 @@ struct DecodeQuantParams {
   float* part;         // [2 blocks][rep][D] sums, then [2 blocks][rep] of (maximum, sum of weights)
   int batch, kv_heads, heads, div, rep;  // heads: groups of at most 8 query heads, div of which share a KV head; rep: query heads of one
   int page_size, page_shift, max_pages, stages, static_table;
-  unsigned slack;  // chunks, of all blocks together, in the time that adding up pieces of several blocks takes
+  unsigned slack, alone;  // chunks in the time that adding up pieces of several blocks takes: of all blocks together, of a block by itself
   float sign, scale_log2, cap_scale, cap_log2;  // the scale's sign (0, NaN: itself) goes into the queries, its magnitude into the factors
   int window, keep_first;
   const void* sink;
@@ -113,20 +112,26 @@ struct QdCut {
 struct QdRanges {
   unsigned x0, n, base, rem;
   bool weighted;
-  __device__ __forceinline__ QdRanges(const QdCut& cut, unsigned block) {
-    const unsigned first = block * cut.each;
-    x0 = cut.begin(first);
-    n = cut.begin(first + cut.each) - x0;
-    base = cut.base;
-    rem = cut.rem > first ? min(cut.rem - first, cut.each) : 0u;
-    weighted = cut.each == kQdWarps && base >= 8;
-  }
-  __device__ __forceinline__ QdRanges(unsigned begin, unsigned end) : x0(begin), n(end - begin), base(n / kQdWarps), rem(n % kQdWarps), weighted(base >= 8) {}
   __device__ __forceinline__ unsigned begin(unsigned w) const {
     static_assert(kQdWarps == 11, "warps 3 and 7");
     return x0 + (weighted ? n * (7 * w + (w > 3 ? 1 : 0) + (w > 7 ? 1 : 0)) / 79 : w * base + min(w, rem));
   }
+  // (kept in shared memory: the products need the registers)
+  __device__ __forceinline__ void keep(volatile int* to) const {
+    to[0] = x0; to[1] = n; to[2] = base; to[3] = rem; to[4] = weighted;
+  }
 };
+__device__ __forceinline__ QdRanges qd_ranges(const volatile int* kept) {
+  return {static_cast<unsigned>(kept[0]), static_cast<unsigned>(kept[1]), static_cast<unsigned>(kept[2]), static_cast<unsigned>(kept[3]), kept[4] != 0};
+}
+__device__ __forceinline__ QdRanges qd_ranges(const QdCut& cut, unsigned block) {
+  const unsigned first = block * cut.each, x0 = cut.begin(first);
+  return {x0, cut.begin(first + cut.each) - x0, cut.base, cut.rem > first ? min(cut.rem - first, cut.each) : 0u, cut.each == kQdWarps && cut.base >= 8};
+}
+__device__ __forceinline__ QdRanges qd_ranges(unsigned begin, unsigned end) {
+  const unsigned n = end - begin;
+  return {begin, n, n / kQdWarps, n % kQdWarps, n >= 8 * kQdWarps};
+}
 // A walk over the pieces of a range of chunks.
 struct QdWalk {
   unsigned x, end;
@@ -151,20 +156,6 @@ __device__ __forceinline__ QdWalk qd_walk(const QdTables& t, int batch, unsigned
     w.b = lo;
   }
   return w;
-}
-// The beginning of a sequence of a head that is nearest to chunk x of all.
-__device__ __forceinline__ unsigned qd_nearest(const QdTables& t, int batch, unsigned x) {
-  const unsigned each = t.before[batch], base = x / each * each;
-  const int y = x - base;
-  int lo = 0, hi = batch;  // the last one at or before y
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (t.before[mid] <= y) lo = mid;
-    else hi = mid - 1;
-  }
-  if (lo == batch) return base + each;
-  const int below = t.before[lo], above = t.before[lo + 1];
-  return base + (y - below <= above - y ? below : above);
 }
 __device__ __forceinline__ bool qd_next(const QdTables& t, int batch, QdWalk& w, QdPiece& it) {
   if (w.x >= w.end) return false;
@@ -304,7 +295,8 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
   tab.len = tab.before + kQdMaxBatch + 4;
   tab.page = tab.len + kQdMaxBatch;
   volatile int* const abort_flag = tab.page + kQdMaxBatch;
-  // [warp][16]: where its walk is, the piece it is at (kept here: the products need the registers), whether its sums are in its slot, its ring
+  // [warp][16]: where its walk is, the piece it is at (kept here: the products need the registers), whether its sums are in its slot, its ring, the
+  // block's ranges
   volatile int* const records = abort_flag + 8;
   uint64_t* const full = reinterpret_cast<uint64_t*>(tab.page + kQdMaxBatch + 8 + kQdWarps * 16);  // [warp][stage]
   uint64_t* const empty = full + kQdWarps * kQdMaxStages;
@@ -352,22 +344,16 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
     }
   }
   __syncthreads();
-  const unsigned all = static_cast<unsigned>(tab.before[p.batch]) * p.heads, share = all / gridDim.x, items = p.batch * p.heads;
-  const unsigned most = abort_flag[1], slack = min(64u, p.slack / min(gridDim.x, items));
-  // Measured, equal shares -> whole sequences, us: 1 of 977 tokens 10.4 -> 9.5, 8 of 1000 11.7 -> 10.1, 16 of 4096 23.5 -> 22.3; with moved cuts 256
-  // of 100 18.6 -> 16.9, but 256 of 512 39.7 -> 40.5 (blocks that have 224 chunks beside those that have 208), so not for shares above 128.
-  const bool own = items <= gridDim.x && most <= share + slack, whole = own || (most <= slack && share <= 128);
-  auto cut_at = [&](unsigned c) {  // between blocks c - 1 and c
-    if (own) return c >= items ? all : static_cast<unsigned>(tab.before[p.batch]) * (c / p.batch) + tab.before[c % p.batch];
-    const unsigned x = c * share + min(c, all % gridDim.x);
-    return x == all ? all : qd_nearest(tab, p.batch, x);
-  };
+  const unsigned each = tab.before[p.batch], all = each * p.heads, items = p.batch * p.heads;
+  // Measured, equal shares -> whole sequences, us, 32 heads over 8 of 128: 1 of 977 tokens 10.3 -> 9.2, 8 of 1000 11.6 -> 9.8, 16 of 2000 17.7 -> 13.7, 18 of 3000
+  // 21.0 -> 17.4; but 1 of 1500 11.0 -> 11.4.
+  const bool whole = items <= gridDim.x && static_cast<unsigned>(abort_flag[1]) <= all / gridDim.x + min(p.alone, p.slack / items);
   ptx::griddep_wait();
 
   T* const out = reinterpret_cast<T*>(p.out);
-  const QdCut cut(all, gridDim.x);
-  const QdRanges mine = whole ? QdRanges(cut_at(blockIdx.x), cut_at(blockIdx.x + 1)) : QdRanges(cut, blockIdx.x);
-  const int warps = whole ? kQdWarps : cut.each;
+  const unsigned own_head = blockIdx.x / p.batch, own_b = blockIdx.x % p.batch;  // (blocks behind the last one: nothing)
+  const QdRanges mine = !whole ? qd_ranges(QdCut(all, gridDim.x), blockIdx.x) : blockIdx.x >= items ? qd_ranges(all, all) : qd_ranges(own_head * each + tab.before[own_b], own_head * each + tab.before[own_b + 1]);
+  const int warps = whole ? kQdWarps : QdCut(all, gridDim.x).each;
   // (sequences without a visible key are in nobody's range: their output is zero)
   for (int b = blockIdx.x; b < p.batch; b += gridDim.x)
     if (tab.before[b] == tab.before[b + 1])
@@ -473,6 +459,7 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
     {
       const QdWalk walk = qd_walk(tab, p.batch, mine.begin(warp), mine.begin(warp + 1));
       rec[0] = walk.x; rec[1] = walk.end; rec[2] = walk.head; rec[3] = walk.b;
+      mine.keep(rec + 10);
     }
     for (;;) {
       QdPiece it;
@@ -743,6 +730,7 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
         o[i][0] = fmaf((o[i][0] + eight[j][0]) * 0x1p24f, up, zs[j][0]); o[i][1] = fmaf((o[i][1] + eight[j][1]) * 0x1p24f, up, zs[j][1]);
         o[i][2] = fmaf((o[i][2] + eight[j][2]) * 0x1p20f, up, zs[j][0]); o[i][3] = fmaf((o[i][3] + eight[j][3]) * 0x1p20f, up, zs[j][1]);
       }
+      const QdRanges mine = qd_ranges(rec + 10);
       const unsigned X0 = mine.x0, X1 = mine.x0 + mine.n, x0 = mine.begin(warp), x1 = mine.begin(warp + 1);
       if (it.start >= x0 && it.stop <= x1) {
         float r[2];
@@ -892,6 +880,7 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
         __threadfence();
         before = atomicAdd(ticket, have);
       }
+      const QdCut cut(static_cast<unsigned>(tab.before[p.batch]) * p.heads, gridDim.x);
       const int c0 = cut.range(it.start) / warps, blocks = static_cast<int>(cut.range(it.stop - 1) / warps) - c0 + 1;
       const bool is_last = asks && before + have == it.stop - it.start;
       if (is_last) {
@@ -1034,7 +1023,8 @@ int blitz_attn_decode_quant(const void* q, int64_t q_stride, const void* pool, c
   p.part = (float*)((char*)workspace + ((int64_t)batch * q_heads * 4 + 255) / 256 * 256);
   p.page_size = page_size; p.max_pages = max_pages; p.page_shift = 0; p.stages = 2;
   while ((1 << p.page_shift) < page_size) ++p.page_shift;
-  p.slack = 15000000u / (2 * quant_kv(dim, group).block);  // 2.5 us at 6 TB/s (and 64 chunks of a block at the most, whose warps take 0.4 us for one)
+  p.slack = 15000000u / (2 * quant_kv(dim, group).block);  // 2.5 us at 6 TB/s
+  p.alone = 184320u / (2 * quant_kv(dim, group).block);    // (what eleven warps compute in that time)
   const float size = sm_scale < 0.f ? -sm_scale : sm_scale > 0.f ? sm_scale : 1.f;
   p.sign = sm_scale < 0.f ? -1.f : sm_scale > 0.f ? 1.f : sm_scale;
   p.scale_log2 = size * 1.4426950408889634f; p.cap_scale = softcap > 0.f ? size / softcap : 0.f; p.cap_log2 = softcap * 1.4426950408889634f;

@@ -70,7 +70,7 @@ def test_rows_in_runs(ops, D, group, dt, longest):
     assert int((cache.pool != 0).any(-1).sum()) <= int(want.sum()) * H
 
 
-# sequences of a head that a block has to itself, several that share one, some that are cut; empty ones among them
+# sequences of a head that a block has to itself, more of them than blocks, some that are cut; empty ones among them
 WHOLE = [([32 * 37] * 18, 8), ([900 + 31 * i for i in range(18)] + [0], 8), ([0, 0, 1], 1), ([1] * 37, 4), ([200 - 3 * i for i in range(61)], 8),
          ([0, 33] * 130 + [1], 4), ([3 * i for i in range(200)], 2), ([700] * 20, 8), ([5000] + [20] * 40, 2)]
 
