@@ -167,7 +167,7 @@ template <typename T, int D, int GROUP>
 __global__ void __launch_bounds__(128) quant_kv_store_kernel(const QuantStoreParams p) {
   constexpr QuantKv F = quant_kv(D, GROUP);
   constexpr int LANES = D / 32, ROWS = 32 / LANES, PITCH = D / 8 + 4;  // (rows in different banks)
-  __shared__ __align__(16) uint32_t s_codes[4][ROWS * PITCH + 0];
+  __shared__ __align__(16) uint32_t s_codes[4][ROWS * PITCH];
   ptx::griddep_launch_dependents();
   ptx::griddep_wait();
   const int lane = threadIdx.x & 31, l = lane % LANES, row = lane / LANES;
@@ -253,9 +253,10 @@ struct QuantRopeParams {
 // there is what the 16-bit rows hold.  A block takes R tokens, whose angles it computes once; a warp four (row, head) pairs at a time:
 // four rows of a head (R = 4: values go out by words), or four heads of a row (R = 1: more blocks where there are few tokens).
 // STATIC: positions and slots that no kernel in flight writes: angles are ready when the projection is.
-// Measured, 32 query heads and 8 KV heads of 128: 8192 rows 51 us (195 MB, 3.8 TB/s; into a 16-bit cache 43 us), 256 rows 4.8 us, one row 3.0 us.
+// Measured, 32 query heads and 8 KV heads of 128: 8192 rows 46 us (195 MB, 4.2 TB/s; into a 16-bit cache 43 us), 256 rows 4.7 us, one row 2.9 us.  With
+// 74 registers a thread, three blocks on an SM, 8192 rows took 51 us.
 template <typename T, int D, int GROUP, int R, bool STATIC>
-__global__ void __launch_bounds__(256) quant_kv_rope_kernel(const QuantRopeParams p) {
+__global__ void __launch_bounds__(256, 4) quant_kv_rope_kernel(const QuantRopeParams p) {
   constexpr QuantKv F = quant_kv(D, GROUP);
   constexpr int LANES = D / 8, ROWS = 32 / LANES, HALF = D / 2;
   __shared__ float s_cos[R][HALF], s_sin[R][HALF];
@@ -282,16 +283,26 @@ __global__ void __launch_bounds__(256) quant_kv_rope_kernel(const QuantRopeParam
     const int page = s >> p.page_shift;
     return p.pool + (((static_cast<int64_t>(page) * p.kv_heads + kv) << (p.page_shift - 4)) + ((s - (page << p.page_shift)) >> 4)) * F.block;
   };
-  for (int unit = warp; unit < (R == 4 ? heads : (heads + 3) / 4); unit += 8) {
-    uint4 raw[4 / ROWS];
-    T* at[4 / ROWS];
+  const int units = R == 4 ? heads : (heads + 3) / 4;
+  uint4 raw[4 / ROWS], next[4 / ROWS];
+  T *at[4 / ROWS], *next_at[4 / ROWS];
+  auto fetch = [&](int unit) {
 #pragma unroll
     for (int k = 0; k < 4 / ROWS; ++k) {
       const int i = k * ROWS + lane / LANES, row = R == 4 ? i : 0, h = R == 4 ? unit : unit * 4 + i;
       const bool real = t0 + row < p.tokens && h < heads;
-      at[k] = real ? reinterpret_cast<T*>(p.qkv) + static_cast<int64_t>(t0 + row) * pitch + static_cast<int64_t>(h) * D + l * 8 : nullptr;
-      raw[k] = real ? *reinterpret_cast<const uint4*>(at[k]) : make_uint4(0, 0, 0, 0);
+      next_at[k] = real ? reinterpret_cast<T*>(p.qkv) + static_cast<int64_t>(t0 + row) * pitch + static_cast<int64_t>(h) * D + l * 8 : nullptr;
+      next[k] = real ? *reinterpret_cast<const uint4*>(next_at[k]) : make_uint4(0, 0, 0, 0);
     }
+  };
+  if (warp < units) fetch(warp);
+  for (int unit = warp; unit < units; unit += 8) {
+#pragma unroll
+    for (int k = 0; k < 4 / ROWS; ++k) {
+      raw[k] = next[k];
+      at[k] = next_at[k];
+    }
+    if (unit + 8 < units) fetch(unit + 8);  // (asked for a turn ahead)
 #pragma unroll
     for (int k = 0; k < 4 / ROWS; ++k) {
       const int i = k * ROWS + lane / LANES, row = R == 4 ? i : 0, h = R == 4 ? unit : unit * 4 + i;
