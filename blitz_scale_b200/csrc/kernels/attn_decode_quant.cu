@@ -60,7 +60,7 @@ struct DecodeQuantParams {
   const int32_t *indices, *indptr, *last_page_len;
   void* out;
   int64_t out_stride;
-  unsigned* tickets;   // [batch][query heads] pieces finished, zero between launches
+  unsigned* tickets;   // [batch][query heads] chunks finished, zero between launches
   float* part;         // [2 blocks][rep][D] sums, then [2 blocks][rep] of (maximum, sum of weights)
   int batch, kv_heads, heads, div, rep;  // heads: groups of at most 8 query heads, div of which share a KV head; rep: query heads of one
   int page_size, page_shift, max_pages, stages, static_table;
@@ -996,14 +996,18 @@ static inline int qd_groups(int rep) {
   return div;
 }
 
+// Bytes of the partial sums in a workspace, whatever a call's batch and heads: calls of any size share one, and nobody's sums may be where
+// another has its tickets.
+static inline int64_t qd_part_bytes() { return ((int64_t)2 * device_sm_count() * 8 * (128 + 2) * 4 + 255) / 256 * 256; }
+
 }  // namespace blitz
 
 extern "C" {
 using namespace blitz;
 
-// Scratch of a call: tickets, which have to be zero before the first call and are again after each, then partial sums.
+// Scratch of a call: partial sums, then tickets, which have to be zero before the first call and are again after each.
 int64_t blitz_attn_decode_quant_workspace_bytes(int batch, int q_heads, int dim) {
-  return ((int64_t)batch * q_heads * 4 + 255) / 256 * 256 + (int64_t)2 * device_sm_count() * 8 * (dim + 2) * 4;
+  return qd_part_bytes() + (int64_t)batch * q_heads * 4;
 }
 
 // q: [batch] rows with the query heads in their first q_heads * dim columns (pitch a multiple of 8, 16-byte aligned; so out).  A sequence
@@ -1020,7 +1024,7 @@ int blitz_attn_decode_quant(const void* q, int64_t q_stride, const void* pool, c
   DecodeQuantParams p;
   p.div = qd_groups(q_heads / kv_heads); p.rep = q_heads / kv_heads / p.div; p.heads = kv_heads * p.div; p.kv_heads = kv_heads;
   p.q_stride = q_stride; p.pool = (const uint8_t*)pool; p.indices = indices; p.out_stride = out_stride;
-  p.part = (float*)((char*)workspace + ((int64_t)batch * q_heads * 4 + 255) / 256 * 256);
+  p.part = (float*)workspace;
   p.page_size = page_size; p.max_pages = max_pages; p.page_shift = 0; p.stages = 2;
   while ((1 << p.page_shift) < page_size) ++p.page_shift;
   p.slack = 15000000u / (2 * quant_kv(dim, group).block);  // 2.5 us at 6 TB/s
@@ -1034,7 +1038,7 @@ int blitz_attn_decode_quant(const void* q, int64_t q_stride, const void* pool, c
     p.q = (const char*)q + (int64_t)b * q_stride * 2;
     p.out = (char*)out + (int64_t)b * out_stride * 2;
     p.indptr = indptr + b; p.last_page_len = last_page_len + b;
-    p.tickets = (unsigned*)workspace + (int64_t)b * q_heads;
+    p.tickets = (unsigned*)((char*)workspace + qd_part_bytes()) + (int64_t)b * q_heads;
     const int rc = quant_kv_dispatch(dtype, dim, group, DecodeQuantLaunch{p, device_sm_count(), stream});
     if (rc) return rc;
   }

@@ -594,7 +594,8 @@ def quant_kv_pages(cache: QuantKV, pages: torch.Tensor, *, dtype: torch.dtype = 
 
 
 def quant_attn_workspace_bytes(batch: int, q_heads: int, head_dim: int, device=None) -> int:
-    """Scratch of `attn_decode` over a 4-bit cache, for up to `batch` sequences: zero-filled before its first use, for one call at a time."""
+    """Scratch of `attn_decode` over a 4-bit cache, for calls of up to `batch` sequences, of as many query heads or fewer, in any order:
+    zero-filled before its first use, for one call at a time."""
     with torch.cuda.device(device):         # (None: the current one)
         return int(lib().blitz_attn_decode_quant_workspace_bytes(batch, q_heads, head_dim))
 
