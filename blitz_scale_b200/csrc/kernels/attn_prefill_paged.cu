@@ -50,11 +50,13 @@
 // neighbours share a reciprocal, 1 / a = b (c d) / (a b c d), unless a product of some four leaves the range of fp32 (one vote per
 // half a block).
 //
-// Operands in fp16 for a bf16 model (IO: the type of queries, sink and output): keys and values were divided by powers of two (a KV head's) so
-// that fp16 holds them, and each thread turns its row of queries into fp16 in shared memory, divided by a power of two near the row's
+// Operands in fp16 for a bf16 model (IO: the type of queries, sink and output): keys and values were divided by powers of two (of a sequence and KV
+// head) so that fp16 holds them, and each thread turns its row of queries into fp16 in shared memory, divided by a power of two near the row's
 // largest entry, as an item begins.  The row's scale and the output's factor make up for both.  A 4-bit cache read back for a pass
 // comes so (quant_kv.cu).  8192 rows of nine prompts, 32 heads of 128: 187 us where a bf16 cache takes 174 (what an item waits for at its start, and
 // registers); with queries converted by a pass before it 184 us behind 20 us of that.
+// PART: such a cache is in fp16 for most sequences and heads and in bf16 for those that fp16 does not hold; a launch with operands of either type takes
+// the items whose keys and values are of that type.
 //
 // Replaces FlashInfer's BatchPrefillWithRaggedKVCacheWrapper / paged wrapper calls and their host Plan()
 // (src/kernel/attention_prefill.cu:11-45, src/kernel/flashinfer_types.cu:24-49).
@@ -88,7 +90,8 @@ struct PagedPrefillParams {
   const void* sink;           // EXT: [q_heads] in the activation type, or null
   const void* bias;           // BIAS: [q_heads][bias_len] in the activation type (SIG: [q_heads], or null)
   int bias_len;
-  const float* kv_up;         // IO: powers of two taken out of keys and values [2][kv_heads]
+  const float2* forms;        // PART: [entries][kv_heads] powers of two taken out of keys and values, zeros where those are in bf16
+  const int* some_bf16;       // PART: whether any are
   int* status;
   long long* trace;  // profiling aid (null in production): clock stamps of CTA 0's first item, see the set_trace call
 };
@@ -112,12 +115,14 @@ struct PpCfg {
 struct PpItem {
   int seq_start, q_len, pg0, npages, kv_len, prefix, q0, nt, nblk, head, kv_head;
   int nblk_t[2];
+  float k_up;             // PART: the power of two taken out of the keys
   int n_first, b_window;  // key blocks walked: [0, n_first), then from b_window on
   __device__ __forceinline__ int block(int j) const { return j < n_first ? j : b_window + j - n_first; }
 };
 // Work item `idx` of the flattened list (entry x q head; the heads of one entry are neighbours, so CTAs that run
 // at the same time share its K and V in L2).
-template <bool EXT>
+// PART: an item of the other type has no blocks.
+template <bool EXT, bool PART, bool SCALED>
 __device__ __forceinline__ PpItem pp_item(const PagedPrefillParams& p, int idx) {
   PpItem it;
   const int entry = idx / p.q_heads;
@@ -143,6 +148,10 @@ __device__ __forceinline__ PpItem pp_item(const PagedPrefillParams& p, int idx) 
     for (int t = 0; t < 2; ++t)
       if (it.nblk_t[t] > 0) it.nblk_t[t] = it.n_first + max(0, it.nblk_t[t] - it.b_window);
   }
+  if (PART) {
+    it.k_up = __ldg(&p.forms[static_cast<int64_t>(entry) * p.kv_heads + it.kv_head].x);
+    if ((it.k_up != 0.f) != SCALED) it.nblk_t[0] = it.nblk_t[1] = 0;
+  }
   it.nblk = max(it.nblk_t[0], it.nblk_t[1]);
   return it;
 }
@@ -153,7 +162,7 @@ __device__ __forceinline__ int pp_index(int r, int total) {
   return idx < total ? idx : -1;
 }
 
-template <typename T, int HD, int VD, bool POLY, bool EXT, bool BIAS, bool SIG, typename IO = T>
+template <typename T, int HD, int VD, bool POLY, bool EXT, bool BIAS, bool SIG, typename IO = T, bool PART = false>
 __global__ void __launch_bounds__(kPpThreads, 1)
 attn_prefill_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                           const __grid_constant__ CUtensorMap tmap_v, const PagedPrefillParams p) {
@@ -187,7 +196,7 @@ attn_prefill_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
   float* s_bias = reinterpret_cast<float*>(sV + 2 * VB + C::kBarBytes);  // BIAS only
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int total = p.entries * p.q_heads;
+  int total = p.entries * p.q_heads;
 
   if (threadIdx.x == 0) {
     ptx::mbar_init(q_empty, 1);
@@ -219,6 +228,7 @@ attn_prefill_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
   const uint32_t tmem_base = *tmem_slot;
   ptx::griddep_launch_dependents();
   ptx::griddep_wait();  // queries, keys, values and the work list come from earlier kernels
+  if (PART && !SCALED && *p.some_bf16 == 0) total = 0;
   const uint32_t tmem_S = tmem_base;        // S_t (and P_t over its first 64 columns) at + 128 t
   const uint32_t tmem_O = tmem_base + 256;  // O_t at + VD t
 
@@ -251,7 +261,8 @@ attn_prefill_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
     for (int r = 0; r * static_cast<int>(gridDim.x) < total && ok; ++r) {
       const int idx = pp_index(r, total);
       if (idx < 0) continue;
-      const PpItem it = pp_item<EXT>(p, idx);
+      const PpItem it = pp_item<EXT, PART, SCALED>(p, idx);
+      if (PART && it.nblk == 0) continue;
       if (n_items > 0) ok = wait(q_empty, (n_items - 1) & 1);  // the previous item's S products have read Q
       if (!ok) break;
       if (lane == 0) {
@@ -266,7 +277,7 @@ attn_prefill_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
       if constexpr (SCALED) {  // the next item's queries into L2: what brings them to fp16 waits for them
         const int next = (r + 1) * static_cast<int>(gridDim.x) < total ? pp_index(r + 1, total) : -1;
         if (next >= 0 && lane < 2 * C::kSlabs) {
-          const PpItem n = pp_item<EXT>(p, next);
+          const PpItem n = pp_item<EXT, PART, SCALED>(p, next);
           const int t = lane / C::kSlabs;
           if (n.nblk_t[t] > 0) ptx::tma_prefetch_3d(&tmap_q, lane % C::kSlabs * 64, n.head, n.seq_start + n.q0 + t * kPpTile);
         }
@@ -321,7 +332,8 @@ attn_prefill_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
       for (int r = 0; r * static_cast<int>(gridDim.x) < total && ok; ++r) {
         const int idx = pp_index(r, total);
         if (idx < 0) continue;
-        const PpItem it = pp_item<EXT>(p, idx);
+        const PpItem it = pp_item<EXT, PART, SCALED>(p, idx);
+        if (PART && it.nblk == 0) continue;
         const int nb0 = it.nblk_t[0], nb1 = it.nblk_t[1], nblk = it.nblk;
         const bool tr = n_items == 0 && blockIdx.x == 0;
         uint64_t* const q_there = SCALED ? q_fp16 : q_full;
@@ -393,7 +405,7 @@ attn_prefill_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
     for (int r = 0; r * static_cast<int>(gridDim.x) < total && ok; ++r) {
       const int idx = pp_index(r, total);
       if (idx < 0) continue;
-      const PpItem it = pp_item<EXT>(p, idx);
+      const PpItem it = pp_item<EXT, PART, SCALED>(p, idx);
       const int my_blocks = it.nblk_t[t];
       if (my_blocks == 0) continue;  // a short last pair has no second tile
       const bool tracer = first && blockIdx.x == 0 && (warp & 3) == 0 && lane == 0;
@@ -408,7 +420,7 @@ attn_prefill_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
           ok = false;
           break;
         }
-        row_up = quant_kv_row_fp16<C::kSlabs>(sQ + t * TB + r_ * 128, SB, r_ & 7) * p.kv_up[it.kv_head];
+        row_up = quant_kv_row_fp16<C::kSlabs>(sQ + t * TB + r_ * 128, SB, r_ & 7) * it.k_up;
         ptx::fence_proxy_async_smem();
         ptx::mbar_arrive(&q_fp16[t]);
       }
@@ -645,7 +657,7 @@ attn_prefill_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
       if (EXT && p.sink != nullptr && l > 0.f)
         l += ptx::ex2_approx(to_f<IO>(reinterpret_cast<const IO*>(p.sink)[it.head]) * 1.4426950408889634f - m_ref);
       float inv = l > 0.f ? 1.f / l : 0.f;
-      if constexpr (SCALED) inv *= p.kv_up[p.kv_heads + it.kv_head];
+      if constexpr (SCALED) inv *= __ldg(&p.forms[static_cast<int64_t>(idx / p.q_heads) * p.kv_heads + it.kv_head].y);
       if (p.gate != nullptr && q_idx < it.q_len) {
         const T z = reinterpret_cast<const T*>(p.gate)[static_cast<int64_t>(it.seq_start + q_idx) * p.gate_stride + it.head];
         inv /= 1.f + expf(-to_f<T>(z));
@@ -683,15 +695,15 @@ attn_prefill_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
   }
 }
 
-template <typename T, int HD, int VD, bool POLY, bool EXT, bool BIAS, bool SIG, typename IO = T>
+template <typename T, int HD, int VD, bool POLY, bool EXT, bool BIAS, bool SIG, typename IO = T, bool PART = false>
 static int launch_paged_prefill(const CUtensorMap (&tm)[3], const PagedPrefillParams& p, int grid, cudaStream_t stream) {
   constexpr int kSmem = PpCfg<HD, VD>::kSmemBytes + (BIAS ? PpCfg<HD, VD>::kBiasFloats * 4 : 0);
   static PerDeviceOnce once;
   cudaError_t e = once.run([] {
-    return cudaFuncSetAttribute(attn_prefill_paged_kernel<T, HD, VD, POLY, EXT, BIAS, SIG, IO>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    return cudaFuncSetAttribute(attn_prefill_paged_kernel<T, HD, VD, POLY, EXT, BIAS, SIG, IO, PART>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   });
   if (e != cudaSuccess) return (int)e;
-  return (int)launch_pdl(attn_prefill_paged_kernel<T, HD, VD, POLY, EXT, BIAS, SIG, IO>, dim3(grid), dim3(kPpThreads), (size_t)kSmem, stream, tm[0], tm[1], tm[2], p);
+  return (int)launch_pdl(attn_prefill_paged_kernel<T, HD, VD, POLY, EXT, BIAS, SIG, IO, PART>, dim3(grid), dim3(kPpThreads), (size_t)kSmem, stream, tm[0], tm[1], tm[2], p);
 }
 
 static long long* g_pp_trace = nullptr;
@@ -720,7 +732,7 @@ static int prefill_paged(const void* q, int64_t q_stride, const void* k_pool, co
                              const int32_t* page_indices, const int32_t* work, int entries, int num_tokens,
                              int q_heads, int kv_heads, int dim, int vdim, int page_size, int page_rows, int max_pages,
                              float sm_scale, int flags, int window, int keep_first, int chunked, int sigmoid, float softcap, const void* sink,
-                             const void* bias, int bias_len, const void* gate, int64_t gate_stride, const float* kv_up, int* status,
+                             const void* bias, int bias_len, const void* gate, int64_t gate_stride, const float2* forms, const int* some_bf16, int* status,
                              int dtype, cudaStream_t stream) {
   if (num_tokens <= 0 || entries <= 0) return 0;
   if (dim < 8 || dim > 128 || (dim & 7) || vdim < 8 || vdim > 128 || (vdim & 7)) return -1;
@@ -745,7 +757,7 @@ static int prefill_paged(const void* q, int64_t q_stride, const void* k_pool, co
   p.q_heads = q_heads; p.kv_heads = kv_heads; p.page_size = page_size; p.box_tokens = bt;
   p.oob_row = (int)rows;
   p.scale_log2 = sm_scale * 1.4426950408889634f; p.status = status; p.trace = g_pp_trace;
-  p.chunked = chunked; p.kv_up = kv_up;
+  p.chunked = chunked; p.forms = forms; p.some_bf16 = some_bf16;
   p.window = window; p.keep_first = keep_first; p.sink = sink; p.bias = bias; p.bias_len = bias_len;
   p.cap_scale = softcap > 0.f ? sm_scale / softcap : 0.f; p.cap_log2 = softcap * 1.4426950408889634f;
   // tanh(z) = z (k0 + k1 z^2 + k2 z^4 + k3 z^6) for |z| <= 0.5 (Chebyshev interpolation of tanh(z) / z in z^2, absolute
@@ -778,14 +790,17 @@ static int prefill_paged(const void* q, int64_t q_stride, const void* k_pool, co
     if (poly) return sized(type, yes, no, no, no);
     return sized(type, no, no, no, no);
   };
-  if (kv_up != nullptr) {
+  if (forms != nullptr) {
     if (dim != vdim || (dim != 64 && dim != 128)) return -1;
-    auto scaled = [&](auto ext_) {
+    using B = __nv_bfloat16;
+    auto both = [&](auto size, auto ext_) {
+      constexpr int D = decltype(size)::value;
       constexpr bool X = decltype(ext_)::value;
-      return dim > 64 ? launch_paged_prefill<__half, 128, 128, false, X, false, false, __nv_bfloat16>(tm, p, grid, stream)
-                      : launch_paged_prefill<__half, 64, 64, false, X, false, false, __nv_bfloat16>(tm, p, grid, stream);
+      const int rc = launch_paged_prefill<__half, D, D, false, X, false, false, B, true>(tm, p, grid, stream);
+      return rc ? rc : launch_paged_prefill<B, D, D, false, X, false, false, B, true>(tm, p, grid, stream);
     };
-    return ext ? scaled(std::true_type{}) : scaled(std::false_type{});
+    auto sized_both = [&](auto ext_) { return dim > 64 ? both(std::integral_constant<int, 128>{}, ext_) : both(std::integral_constant<int, 64>{}, ext_); };
+    return ext ? sized_both(std::true_type{}) : sized_both(std::false_type{});
   }
   return dtype == 1 ? launch(__nv_bfloat16{}) : launch(__half{});
 }
@@ -797,18 +812,19 @@ int blitz_attn_prefill_paged(const void* q, int64_t q_stride, const void* k_pool
                              const void* bias, int bias_len, const void* gate, int64_t gate_stride, int* status, int dtype, cudaStream_t stream) {
   return prefill_paged(q, q_stride, k_pool, v_pool, out, out_stride, page_indices, work, entries, num_tokens, q_heads, kv_heads, dim, vdim, page_size,
                        page_rows, max_pages, sm_scale, flags, window, keep_first, chunked, sigmoid, softcap, sink, bias, bias_len, gate, gate_stride,
-                       nullptr, status, dtype, stream);
+                       nullptr, nullptr, status, dtype, stream);
 }
 
-// The same for a bf16 model (q, sink and out) with keys and values in fp16, which were multiplied by 1 / kv_up [2][kv_heads], powers of two.
-// dim 64 or 128.
+// The same for a bf16 model (q, sink and out) whose keys and values blitz_quant_kv_portion has read back: forms is the fourth part of its scratch,
+// some_bf16 what is behind the spans.  dim 64 or 128.
 int blitz_attn_prefill_scaled(const void* q, int64_t q_stride, const void* k_pool, const void* v_pool, void* out, int64_t out_stride,
                               const int32_t* page_indices, const int32_t* work, int entries, int num_tokens, int q_heads, int kv_heads, int dim,
                               int page_size, int page_rows, int max_pages, float sm_scale, int window, int keep_first, float softcap, const void* sink,
-                              const float* kv_up, int* status, cudaStream_t stream) {
-  if (kv_up == nullptr) return -1;
+                              const void* forms, const int* some_bf16, int* status, cudaStream_t stream) {
+  if (forms == nullptr || some_bf16 == nullptr) return -1;
   return prefill_paged(q, q_stride, k_pool, v_pool, out, out_stride, page_indices, work, entries, num_tokens, q_heads, kv_heads, dim, dim, page_size,
-                       page_rows, max_pages, sm_scale, 0, window, keep_first, 0, 0, softcap, sink, nullptr, 0, nullptr, 0, kv_up, status, 0, stream);
+                       page_rows, max_pages, sm_scale, 0, window, keep_first, 0, 0, softcap, sink, nullptr, 0, nullptr, 0, (const float2*)forms, some_bf16,
+                       status, 0, stream);
 }
 
 }  // extern "C"

@@ -464,7 +464,6 @@ __global__ void __launch_bounds__(128) quant_kv_load_kernel(const QuantLoadParam
 }
 
 // ------------------------------------------------------------------ pages back
-constexpr int kQuantSpanBlocks = 256;
 struct QuantPagesParams {
   const uint8_t* pool;
   const int32_t* pages;
@@ -474,55 +473,73 @@ struct QuantPagesParams {
   int* status;
   // for attention of portions: records of the pass (see attn_prefill_paged.cu), whose page numbers count from `first` pages before the first one
   const int32_t* work;
-  int entries, first;
+  int entries, first, pages_read;
   int32_t* table;     // numbers of the pages read back, for all of those that the records count
-  const float* spans; // SCALED: [2][kv_heads][kQuantSpanBlocks] largest magnitudes, by block
-  int span_blocks;
-  float* up;          // SCALED: [2][kv_heads] powers of two that were taken out of keys and values
+  uint4* spans;       // SCALED: [pages][kv_heads] what quant_kv_form takes, where a sequence's first page is; behind them whether some are held in bf16
+  float2* forms;      // SCALED: [entries][kv_heads] powers of two taken out of keys and values (zeros: held in bf16)
 };
 
-// Tokens of page `n` (counted as the records do) that its sequence has, -1: no record has it.  The whole warp asks.
-__device__ __forceinline__ int quant_kv_held(const QuantPagesParams& p, int n) {
-  int held = -1;
+// Tokens of page `n` (counted as the records do) that its sequence has, -1: no record has it; and the sequence's first page.  The whole warp asks.
+struct QuantHeld {
+  int tokens, start;
+};
+__device__ __forceinline__ QuantHeld quant_kv_held(const QuantPagesParams& p, int n) {
+  QuantHeld held{-1, -1};
   for (int e = threadIdx.x & 31; e < p.entries; e += 32) {
     const int4 r = __ldg(reinterpret_cast<const int4*>(p.work + e * 8));
-    if (n >= r.z && n < r.z + r.w) held = min(p.page_size, max(0, __ldg(p.work + e * 8 + 4) - (n - r.z) * p.page_size));
+    if (r.z >= p.first && n >= r.z && n < r.z + r.w) {
+      held.tokens = min(p.page_size, max(0, __ldg(p.work + e * 8 + 4) - (n - r.z) * p.page_size));
+      held.start = r.z - p.first;
+    }
   }
-  return __reduce_max_sync(0xffffffffu, held);
+  return {__reduce_max_sync(0xffffffffu, held.tokens), __reduce_max_sync(0xffffffffu, held.start)};
 }
-// The largest magnitudes of a pass's keys and values, by head: of every block, a part of them.  Half a warp looks at the scales of the
-// keys of 16 tokens, the other half at those of the values.
-// Measured: 8200 tokens of 8 heads of 128 7.6 us, 3900 4.6 us (latency: record, page, scales).
-template <int D, int GROUP>
-__global__ void __launch_bounds__(256) quant_kv_span_kernel(const QuantPagesParams p, float* __restrict__ spans) {
-  constexpr QuantKv F = quant_kv(D, GROUP);
-  constexpr int G = F.groups;
-  extern __shared__ int s_most[];  // [2][kv_heads] bits of numbers that are not negative
-  for (int i = threadIdx.x; i < 2 * p.kv_heads; i += blockDim.x) s_most[i] = 0;
+// No magnitudes yet.
+__global__ void __launch_bounds__(256) quant_kv_no_span_kernel(uint4* __restrict__ spans, int64_t n) {
   ptx::griddep_launch_dependents();
   ptx::griddep_wait();
-  __syncthreads();
-  const int lane = threadIdx.x & 31, blocks = p.page_size >> 4;
-  for (int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); unit < p.units; unit += static_cast<int64_t>(p.span_blocks) * 8) {
-    const int head = static_cast<int>(unit % p.kv_heads), b = static_cast<int>(unit / p.kv_heads % blocks);
-    const int n = static_cast<int>(unit / p.kv_heads / blocks), held = quant_kv_held(p, n + p.first), page = p.pages[n];
-    if (held <= b * 16 || page < 0 || page >= p.max_pages) continue;
-    const uint8_t* block = p.pool + ((static_cast<int64_t>(page) * p.kv_heads + head) * blocks + b) * F.block;
-    const __nv_bfloat16* w = reinterpret_cast<const __nv_bfloat16*>(block + (lane < 16 ? 0 : F.part) + F.codes) + (lane & 15) * 2 * G;
-    float most = 0.f;
-    if (b * 16 + (lane & 15) < held) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i < n) spans[i] = make_uint4(0, 0, 0, 0);
+}
+// The largest and smallest magnitudes of the groups of a sequence's keys and values, by head (maxima: in whatever order).  A warp takes up to 64 tokens of
+// a page and head, half of it looks at the scales of the keys of 16 tokens at a time, the other half at those of the values.
+template <int D, int GROUP>
+__global__ void __launch_bounds__(256) quant_kv_span_kernel(const QuantPagesParams p) {
+  constexpr QuantKv F = quant_kv(D, GROUP);
+  constexpr int G = F.groups, EACH = 4;
+  ptx::griddep_launch_dependents();
+  ptx::griddep_wait();
+  const int lane = threadIdx.x & 31, blocks = p.page_size >> 4, parts = (blocks + EACH - 1) / EACH;
+  const int64_t units = p.units / blocks * parts;
+  for (int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); unit < units; unit += static_cast<int64_t>(gridDim.x) * 8) {
+    const int head = static_cast<int>(unit % p.kv_heads), b0 = static_cast<int>(unit / p.kv_heads % parts) * EACH;
+    const int n = static_cast<int>(unit / p.kv_heads / parts), page = p.pages[n];
+    const QuantHeld held = quant_kv_held(p, n + p.first);
+    if (held.tokens <= b0 * 16 || page < 0 || page >= p.max_pages) continue;
+    const uint8_t* block = p.pool + ((static_cast<int64_t>(page) * p.kv_heads + head) * blocks + b0) * F.block + (lane < 16 ? 0 : F.part) + F.codes + (lane & 15) * 4 * G;
+    uint32_t w[EACH][G];
+#pragma unroll
+    for (int b = 0; b < EACH; ++b)
+#pragma unroll
+      for (int i = 0; i < G; ++i)  // (zeros: a group that does not count)
+        w[b][i] = (b0 + b) * 16 + (lane & 15) < held.tokens ? reinterpret_cast<const uint32_t*>(block + b * F.block)[i] : 0u;
+    auto number = [&](int b, int i) { return __uint_as_float(i & 1 ? w[b][i >> 1] & 0xffff0000u : w[b][i >> 1] << 16); };
+    uint32_t most = 0, least = 0;
+#pragma unroll
+    for (int b = 0; b < EACH; ++b)
 #pragma unroll
       for (int i = 0; i < G; ++i) {
-        const float s = __bfloat162float(w[i]), z = __bfloat162float(w[G + i]);
-        most = fmaxf(most, fmaxf(fabsf(z), fabsf(fmaf(15.f, s, z))));  // (NaN: not counted)
+        const float s = number(b, i), z = number(b, G + i), m = fmaxf(fabsf(z), fabsf(fmaf(15.f, s, z)));
+        if (m > 0.f) {  // (NaN: not counted)
+          most = max(most, __float_as_uint(m));
+          least = max(least, 0x7f800000u - __float_as_uint(m));
+        }
       }
-    }
-#pragma unroll
-    for (int d = 1; d < 16; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-    if ((lane & 15) == 0) atomicMax(&s_most[(lane >> 4) * p.kv_heads + head], __float_as_int(most));
+    const uint32_t both[4] = {__reduce_max_sync(0xffffffffu, lane < 16 ? most : 0u), __reduce_max_sync(0xffffffffu, lane < 16 ? least : 0u),
+                              __reduce_max_sync(0xffffffffu, lane < 16 ? 0u : most), __reduce_max_sync(0xffffffffu, lane < 16 ? 0u : least)};
+    const uint32_t mine = lane == 0 ? both[0] : lane == 1 ? both[1] : lane == 2 ? both[2] : both[3];
+    if (lane < 4 && mine != 0) atomicMax(reinterpret_cast<uint32_t*>(p.spans + static_cast<int64_t>(held.start) * p.kv_heads + head) + lane, mine);
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i < 2 * p.kv_heads; i += blockDim.x) spans[i * kQuantSpanBlocks + blockIdx.x] = __int_as_float(s_most[i]);
 }
 
 // The codes of a warp's 16 tokens of a head, 8 x 8 blocks of (token, dimension) at a time as tensor-core fragments have them.
@@ -534,9 +551,8 @@ __device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t a, uin
 // Bound by the 16-bit rows that it writes (four times the codes): 1024 pages of 64 tokens of 8 heads of 128 63 us (352 MB, 5.6 TB/s), 37 pages of 4 heads
 // of 64 3.4 us; for attention of portions 8200 tokens 15 us after their largest magnitudes are known.
 //
-// For attention of portions (WORK) the tokens behind a sequence's end are zeros, whatever the cache has there.  SCALED: keys and
-// values of a bf16 model go to fp16, which keeps three bits more of what z + s c is, divided by a power of two near the largest of their head, so that
-// the type's range does not matter.
+// For attention of portions (WORK) the tokens behind a sequence's end are zeros, whatever the cache has there.  SCALED: keys and values of a bf16
+// model go to fp16, divided by powers of two, or stay in bf16, as quant_kv_form says for their sequence and head.
 template <typename T, int D, int GROUP, bool WORK, bool SCALED>
 __global__ void __launch_bounds__(256, 3) quant_kv_pages_kernel(const QuantPagesParams p) {
   constexpr QuantKv F = quant_kv(D, GROUP);
@@ -551,28 +567,19 @@ __global__ void __launch_bounds__(256, 3) quant_kv_pages_kernel(const QuantPages
   uint8_t* const rows = s_rows[warp];
   const int blocks = p.page_size >> 4;
   if (WORK && blockIdx.x == 0)
-    for (int64_t i = threadIdx.x; i < p.units / p.kv_heads / blocks + p.first; i += 256) p.table[i] = max(0, static_cast<int>(i) - p.first);
-  __shared__ float s_down[SCALED ? 256 : 1];  // of keys, then of values, by head
-  if (SCALED) {
-    for (int i = warp; i < 2 * p.kv_heads; i += 8) {
-      float most = 0.f;
-#pragma unroll
-      for (int c = 0; c < kQuantSpanBlocks; c += 32)
-        if (c + lane < p.span_blocks) most = fmaxf(most, p.spans[i * kQuantSpanBlocks + c + lane]);
-      const float down = quant_kv_down(warp_max(most));
-      if (lane == 0) {
-        s_down[i] = down;
-        if (blockIdx.x == 0) p.up[i] = 1.f / down;
-      }
+    for (int64_t i = threadIdx.x; i < static_cast<int64_t>(p.pages_read) + p.first; i += 256) p.table[i] = max(0, static_cast<int>(i) - p.first);
+  if (SCALED)
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < static_cast<int64_t>(p.entries) * p.kv_heads; i += static_cast<int64_t>(gridDim.x) * 256) {
+      const int e = static_cast<int>(i / p.kv_heads), start = min(max(__ldg(p.work + e * 8 + 2) - p.first, 0), p.pages_read - 1);
+      const QuantForm form = quant_kv_form(__ldcg(p.spans + static_cast<int64_t>(start) * p.kv_heads + i % p.kv_heads));
+      p.forms[i] = form.fp16 ? make_float2(1.f / form.k_down, 1.f / form.v_down) : make_float2(0.f, 0.f);
+      if (!form.fp16) p.spans[static_cast<int64_t>(p.pages_read) * p.kv_heads].x = 1;
     }
-    __syncthreads();
-  }
   for (int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + warp; unit < p.units; unit += static_cast<int64_t>(gridDim.x) * 8) {
     const int head = static_cast<int>(unit % p.kv_heads), b = static_cast<int>(unit / p.kv_heads % blocks);
     const int64_t n = unit / p.kv_heads / blocks;
     const int page = p.pages[n];
     const bool bad = page < 0 || page >= p.max_pages;  // (the first page is read instead, and nothing written)
-    const float k_down = SCALED ? s_down[head] : 1.f, v_down = SCALED ? s_down[p.kv_heads + head] : 1.f;
     const uint8_t* block = p.pool + ((static_cast<int64_t>(bad ? 0 : page) * p.kv_heads + head) * blocks + b) * F.block;
     const int64_t row0 = n * p.page_rows + b * 16, pitch = static_cast<int64_t>(p.kv_heads) * D;
     // everything is asked for before anything is used
@@ -612,18 +619,21 @@ __global__ void __launch_bounds__(256, 3) quant_kv_pages_kernel(const QuantPages
 #pragma unroll
     for (int j = 0; j < 4; ++j) numbers(block + F.part + F.codes + (4 * t4 + j) * 4 * G, vs[j]);
     int held = p.page_size;
+    QuantForm form{true, 1.f, 1.f};
     if (WORK) {
-      held = quant_kv_held(p, static_cast<int>(n) + p.first);
-      if (held < 0) continue;  // (no record has the page)
+      const QuantHeld h = quant_kv_held(p, static_cast<int>(n) + p.first);
+      if (h.tokens < 0) continue;  // (no record has the page)
+      held = h.tokens;
+      if (SCALED) form = quant_kv_form(__ldcg(p.spans + static_cast<int64_t>(h.start) * p.kv_heads + head));
     }
     held -= b * 16;            // of these 16 tokens
     if (bad) {
       if (p.status && lane == 0) atomicCAS(p.status, 0, kStatusBadIndex);
       continue;
     }
-    constexpr float most = quant_kv_most<T>();
+    constexpr float most = SCALED ? quant_kv_most<__nv_bfloat16>() : quant_kv_most<T>();
     bool past = false;
-    if (!SCALED)
+    if (!SCALED || !form.fp16)
 #pragma unroll
     for (int i = 0; i < G; ++i) {
 #pragma unroll
@@ -631,6 +641,7 @@ __global__ void __launch_bounds__(256, 3) quant_kv_pages_kernel(const QuantPages
 #pragma unroll
       for (int j = 0; j < 4; ++j) past |= quant_kv_past(number(vs[j], i), number(vs[j], G + i), most);
     }
+    auto two = [&](float a, float b) { return !SCALED || form.fp16 ? pk2<T>(a, b) : pk2<__nv_bfloat16>(a, b); };
     auto out = [&](void* to, int row_bytes) {
       T* const d = reinterpret_cast<T*>(to) + row0 * pitch + static_cast<int64_t>(head) * D;
       __syncwarp();
@@ -646,7 +657,7 @@ __global__ void __launch_bounds__(256, 3) quant_kv_pages_kernel(const QuantPages
         float x[8];
         quant_kv_codes(kw[r][w], x);
         float sc = number(ks[r], w * 32 / GROUP), z = number(ks[r], G + w * 32 / GROUP);
-        if (SCALED) sc *= k_down, z *= k_down;
+        if (SCALED) sc *= form.k_down, z *= form.k_down;
         if (WORK && g + 8 * r >= held) sc = z = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = fmaf(sc, x[i], z);
@@ -654,7 +665,7 @@ __global__ void __launch_bounds__(256, 3) quant_kv_pages_kernel(const QuantPages
 #pragma unroll
           for (int i = 0; i < 8; ++i) x[i] = quant_kv_cut(x[i], most);
         }
-        stf8<T>(reinterpret_cast<T*>(rows + (g + 8 * r) * KROW) + 32 * w + 8 * t4, x);
+        *reinterpret_cast<uint4*>(rows + (g + 8 * r) * KROW + (32 * w + 8 * t4) * 2) = make_uint4(two(x[0], x[1]), two(x[2], x[3]), two(x[4], x[5]), two(x[6], x[7]));
       }
     out(p.k, KROW);
 #pragma unroll
@@ -667,7 +678,7 @@ __global__ void __launch_bounds__(256, 3) quant_kv_pages_kernel(const QuantPages
       for (int j = 0; j < 8; ++j) {
         const int tok = (j & 2) + (j >> 2);
         float sc = number(vs[tok], i), z = number(vs[tok], G + i);
-        if (SCALED) sc *= v_down, z *= v_down;
+        if (SCALED) sc *= form.v_down, z *= form.v_down;
         if (WORK && 4 * t4 + tok >= held) sc = z = 0.f;
         x[j] = fmaf(sc, x[j], z);
       }
@@ -678,7 +689,7 @@ __global__ void __launch_bounds__(256, 3) quant_kv_pages_kernel(const QuantPages
       // 8 x 8 blocks: dimensions 16 m + g by (tokens 4 t4, + 1), 16 m + 8 + g by the same, and both by (4 t4 + 2, + 3).  Lane i gives the address of
       // row i % 8 of block i / 8: its token (columns 2 t4, 2 t4 + 1 of a block are tokens 4 t4 (+ 2), + 1), eight dimensions.
       const int mat = lane >> 3, c = lane & 7, token = 4 * (c >> 1) + (c & 1) + (mat >> 1) * 2;
-      stmatrix_x4_trans(ptx::smem_u32(rows + token * ROW + m * 32 + (mat & 1) * 16), pk2<T>(x[0], x[4]), pk2<T>(x[1], x[5]), pk2<T>(x[2], x[6]), pk2<T>(x[3], x[7]));
+      stmatrix_x4_trans(ptx::smem_u32(rows + token * ROW + m * 32 + (mat & 1) * 16), two(x[0], x[4]), two(x[1], x[5]), two(x[2], x[6]), two(x[3], x[7]));
     }
     out(p.v, ROW);
   }
@@ -730,8 +741,7 @@ struct PagesLaunch {
   }
 };
 struct PortionLaunch {
-  QuantPagesParams& p;
-  float* spans;
+  const QuantPagesParams& p;
   cudaStream_t stream;
   template <typename T, int D, int GROUP>
   int operator()() const {
@@ -739,9 +749,11 @@ struct PortionLaunch {
     const unsigned page_blocks = (unsigned)(blocks < most ? blocks : most);
     if (std::is_same<T, __half>::value)
       return (int)launch_pdl(quant_kv_pages_kernel<__half, D, GROUP, true, false>, dim3(page_blocks), dim3(256), 0, stream, p);
-    p.spans = spans;
-    p.span_blocks = (int)(blocks < kQuantSpanBlocks ? blocks : kQuantSpanBlocks);
-    const int rc = (int)launch_pdl(quant_kv_span_kernel<D, GROUP>, dim3((unsigned)p.span_blocks), dim3(256), (size_t)2 * p.kv_heads * 4, stream, p, spans);
+    const int64_t spans = p.units / (p.page_size >> 4);  // (page, head) each
+    int rc = (int)launch_pdl(quant_kv_no_span_kernel, dim3((unsigned)(spans / 256 + 1)), dim3(256), 0, stream, p.spans, spans + 1);
+    if (rc) return rc;
+    const int64_t span_blocks = (spans * ((p.page_size + 63) / 64) + 7) / 8;
+    rc = (int)launch_pdl(quant_kv_span_kernel<D, GROUP>, dim3((unsigned)(span_blocks < most ? span_blocks : most)), dim3(256), 0, stream, p);
     if (rc) return rc;
     return (int)launch_pdl(quant_kv_pages_kernel<__half, D, GROUP, true, true>, dim3(page_blocks), dim3(256), 0, stream, p);
   }
@@ -796,11 +808,11 @@ int blitz_quant_kv_pages(const void* pool, const int32_t* pages, int64_t count, 
 }
 
 // Scratch of blitz_quant_kv_portion for `pages` pages and `first` more that the records count, in the order of its layout: keys and values read
-// back [pages][2][page_size][kv_heads][dim] in 16 bits, page numbers; of a bf16 model also the powers of two of keys and values, and the parts of
-// their largest magnitudes.  offsets (may be null): where the 4 parts begin, and the end.
-int64_t blitz_quant_kv_portion_bytes(int64_t pages, int64_t first, int kv_heads, int dim, int page_size, int dtype, int64_t* offsets) {
-  const int64_t h = dtype == 1 ? 2 * (int64_t)kv_heads : 0;
-  const int64_t sizes[4] = {pages * 4 * page_size * kv_heads * dim, (pages + first) * 4, h * 4, h * 4 * kQuantSpanBlocks};
+// back [pages][2][page_size][kv_heads][dim] in 16 bits, page numbers; of a bf16 model also the spans of keys and values, and what the `entries` records
+// find of them.  offsets (may be null): where the 4 parts begin, and the end.
+int64_t blitz_quant_kv_portion_bytes(int64_t pages, int64_t first, int entries, int kv_heads, int dim, int page_size, int dtype, int64_t* offsets) {
+  const int64_t sizes[4] = {pages * 4 * page_size * kv_heads * dim, (pages + first) * 4, dtype == 1 ? (pages * kv_heads + 1) * 16 : 0,
+                            dtype == 1 ? (int64_t)entries * kv_heads * 8 : 0};
   int64_t at = 0;
   for (int i = 0; i < 4; ++i) {
     if (offsets) offsets[i] = at;
@@ -811,18 +823,19 @@ int64_t blitz_quant_kv_portion_bytes(int64_t pages, int64_t first, int kv_heads,
 }
 
 // What attention of portions (blitz_attn_prefill_paged, or blitz_attn_prefill_scaled for a bf16 model) reads instead of a 4-bit cache: pages[n], the
-// (first + n)-th page that the records of `work` count, in 16 bits (of a bf16 model: fp16), zeros behind the end of its sequence.
+// (first + n)-th page that the records of `work` count, in 16 bits (of a bf16 model: as quant_kv_form says), zeros behind the end of its sequence.
 int blitz_quant_kv_portion(const void* pool, const int32_t* pages, int64_t count, int64_t first, const int32_t* work, int entries, int kv_heads, int dim,
                            int group, int page_size, int max_pages, void* scratch, int* status, int dtype, cudaStream_t stream) {
   if (count <= 0 || entries <= 0) return 0;
-  if (!quant_kv_supported(dim, group, page_size) || max_pages < 1 || kv_heads < 1 || kv_heads > 128 || first < 0 || count + first > 0x7fffffff) return -1;
+  if (!quant_kv_supported(dim, group, page_size) || max_pages < 1 || kv_heads < 1 || first < 0 || count + first > 0x7fffffff) return -1;
   if ((reinterpret_cast<uintptr_t>(work) | reinterpret_cast<uintptr_t>(pool) | reinterpret_cast<uintptr_t>(scratch)) & 15) return -1;
   int64_t at[5];
-  blitz_quant_kv_portion_bytes(count, first, kv_heads, dim, page_size, dtype, at);
+  blitz_quant_kv_portion_bytes(count, first, entries, kv_heads, dim, page_size, dtype, at);
   char* s = (char*)scratch;
   QuantPagesParams p{(const uint8_t*)pool, pages, s, s + (int64_t)page_size * kv_heads * dim * 2, count * kv_heads * (page_size / 16), kv_heads, page_size, 2 * page_size, max_pages, status};
-  p.work = work; p.entries = entries; p.first = (int)first; p.table = (int32_t*)(s + at[1]); p.up = (float*)(s + at[2]);
-  return quant_kv_dispatch(dtype, dim, group, PortionLaunch{p, (float*)(s + at[3]), stream});
+  p.work = work; p.entries = entries; p.first = (int)first; p.table = (int32_t*)(s + at[1]); p.spans = (uint4*)(s + at[2]);
+  p.pages_read = (int)count; p.forms = (float2*)(s + at[3]);
+  return quant_kv_dispatch(dtype, dim, group, PortionLaunch{p, stream});
 }
 
 }  // extern "C"

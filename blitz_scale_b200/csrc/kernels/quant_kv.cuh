@@ -102,6 +102,25 @@ __device__ __forceinline__ float quant_kv_down(float x) {
   return __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
 }
 
+// How a pass reads back the keys and values of a sequence and KV head of a bf16 model: in fp16, which keeps three bits more of what z + s c is,
+// divided by powers of two near the largest; or in bf16, as a 16-bit cache has them, where fp16 would not hold eleven bits of every group's
+// largest number (one is below 2^-14 of the largest of all), or the powers leave 2^-100 .. 2^100.  So neither another sequence nor a token that a row
+// does not see, or gives no weight, costs it more than those three bits.
+struct QuantForm {
+  bool fp16;
+  float k_down, v_down;
+};
+// span: bits of the largest magnitude of the keys' groups, bits of infinity less those of the smallest one that is not zero, the same of the
+// values' (zeros: there is nothing but zeros and what is no number).
+__device__ __forceinline__ QuantForm quant_kv_form(uint4 span) {
+  auto held = [](uint32_t most, uint32_t least) {
+    const float m = __uint_as_float(most);
+    return most == 0 || (m <= 0x1p100f && m >= 0x1p-100f && __uint_as_float(0x7f800000u - least) >= m * 0x1p-14f);
+  };
+  if (!held(span.x, span.y) || !held(span.z, span.w)) return {false, 1.f, 1.f};
+  return {true, quant_kv_down(__uint_as_float(span.x)), quant_kv_down(__uint_as_float(span.z))};
+}
+
 // A row of bf16 numbers in a tile that TMA wrote with a 128-byte swizzle, to fp16 where it stands, divided by a power of two near the largest,
 // which it returns.  row: of the first slab of 64 columns, `slab` bytes from one to the next; x: which exclusive-or its 16-byte pieces are at (lanes
 // that have rows next to each other then read different banks).

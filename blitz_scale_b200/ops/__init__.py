@@ -673,7 +673,7 @@ def _attn_portion_quant(q, cache, page_indices, work, q_heads, kv_heads, head_di
         return out
     L, pool, dt, status, stream = lib(), cache.pool, _DT[q.dtype], _status_ptr(q), _stream()
     at = (ctypes.c_int64 * 5)()
-    scratch = torch.empty(L.blitz_quant_kv_portion_bytes(n, skip_pages, kv_heads, head_dim, page_size, dt, at), dtype=torch.uint8, device=q.device)
+    scratch = torch.empty(L.blitz_quant_kv_portion_bytes(n, skip_pages, entries, kv_heads, head_dim, page_size, dt, at), dtype=torch.uint8, device=q.device)
     base = scratch.data_ptr()
     _check(L.blitz_quant_kv_portion(pool.data_ptr(), page_indices.data_ptr() + 4 * skip_pages, n, skip_pages, work.data_ptr(), entries, kv_heads,
                                     head_dim, cache.group, page_size, pool.shape[0], base, status, dt, stream), "blitz_quant_kv_portion")
@@ -681,7 +681,7 @@ def _attn_portion_quant(q, cache, page_indices, work, q_heads, kv_heads, head_di
     if dt == 1:
         _check(L.blitz_attn_prefill_scaled(q.data_ptr(), q.stride(0), base, values, out.data_ptr(), out.stride(0), base + at[1], work.data_ptr(), entries,
                                            T, q_heads, kv_heads, head_dim, page_size, 2 * page_size, n, scale, window, keep_first, softcap, snk,
-                                           base + at[2], status, stream), "blitz_attn_prefill_scaled")
+                                           base + at[3], base + at[2] + 16 * n * kv_heads, status, stream), "blitz_attn_prefill_scaled")
     else:
         _check(L.blitz_attn_prefill_paged(q.data_ptr(), q.stride(0), base, values, out.data_ptr(), out.stride(0), base + at[1], work.data_ptr(), entries, T,
                                           q_heads, kv_heads, head_dim, head_dim, page_size, 2 * page_size, n, scale, 0, window, keep_first, 0, 0, softcap,
@@ -774,8 +774,8 @@ def attn_prefill_paged(q: torch.Tensor, kv_layer: KVLayer, page_indices: torch.T
     as for `attn_decode` (no bias beside a window, cap or sink; with sigmoid weights a bias of one column).
 
     Over a 4-bit cache (QuantKV): the pages that ``work`` refers to are read back first, into scratch of this call (of a bf16 model in
-    fp16, as its queries enter, scaled so that the type's range does not matter); tokens behind a sequence's end may hold anything; no gate,
-    bias, ``chunked`` or ``sigmoid``; no record of ``work`` refers to the first ``skip_pages`` entries of ``page_indices``."""
+    fp16, as its queries enter, divided by powers of two of the sequence and head, or in bf16 where a sequence's keys or values of a head span
+    more than fp16 holds); tokens behind a sequence's end may hold anything; no gate, bias, ``chunked`` or ``sigmoid``; no record of ``work`` refers to the first ``skip_pages`` entries of ``page_indices``."""
     if isinstance(kv_layer, QuantKV):
         _quant_refuses(gate, bias, chunked, sigmoid)
         return _attn_portion_quant(q, kv_layer, page_indices, work, q_heads, kv_heads, head_dim, page_size, out, sm_scale, window, keep_first, softcap, sink,

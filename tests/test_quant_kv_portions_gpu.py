@@ -1,0 +1,145 @@
+"""Attention of portions over a 4-bit cache: keys and values of very different sizes, in one pass, one sequence, one head."""
+import pytest
+import torch
+
+from quant_kv_plain import attention, quantised, values
+from test_quant_kv_gpu import DEV, rows, tolerance
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from blitz_scale_b200 import ops as o
+    o.lib()
+    return o
+
+
+@pytest.fixture(autouse=True)
+def _status(ops):
+    yield
+    ops.check_status()
+
+
+class Pass:
+    """Rows of sequences [(tokens before, rows)], whose keys and values [tokens, heads, dim] are given; `lead` pages of nobody in front."""
+
+    def __init__(self, ops, seqs, kv, q, group, page, lead=0, **opts):
+        self.ops, self.group, self.page, self.lead, self.q = ops, group, page, lead, q
+        self.H, self.D = kv[0][0].shape[1:]
+        self.opts = {n: x.to(DEV) if isinstance(x, torch.Tensor) else x for n, x in opts.items()}
+        self.lens, self.rows = [a + b for a, b in seqs], [b for _, b in seqs]
+        used = [-(-n // page) for n in self.lens]
+        g = torch.Generator().manual_seed(len(seqs))
+        self.table = torch.randperm(sum(used) + 3, generator=g)[:sum(used)]
+        self.cache = ops.quant_kv_pool(sum(used) + 3, page, self.H, self.D, group)
+        self.cache.pool.fill_(255)
+        at = 0
+        for n, u, (k, v) in zip(self.lens, used, kv):
+            j = torch.arange(n)
+            slot = (self.table[at + j // page] * page + j % page).to(torch.int32).to(DEV)
+            ops.quant_kv_store(k.flatten(1).to(DEV), v.flatten(1).to(DEV), slot, self.cache)
+            at += u
+
+    def run(self, cache=None):
+        Q = self.q.shape[1]
+        pages = torch.cat([torch.zeros(self.lead, dtype=torch.long), self.table]).to(torch.int32).to(DEV)
+        work = self.ops.prefill_work_list([1] * bool(self.lead) + self.rows, [self.lead * self.page] * bool(self.lead) + self.lens, self.page, DEV,
+                                          skip=int(self.lead > 0))
+        x = torch.cat([torch.zeros(int(self.lead > 0), Q, self.D, dtype=self.q.dtype), self.q]).flatten(1).to(DEV)
+        more = dict(skip_pages=self.lead) if cache is None else {}
+        out = self.ops.attn_prefill_paged(x, self.cache if cache is None else cache, pages, work, q_heads=Q, kv_heads=self.H, head_dim=self.D,
+                                          page_size=self.page, **more, **self.opts)
+        return out[int(self.lead > 0):].cpu().view(-1, Q, self.D)
+
+    def run_16_bit(self):
+        """The same over a cache in bf16."""
+        cache = self.ops.quant_kv_pages(self.cache, torch.arange(self.cache.pool.shape[0], dtype=torch.int32, device=DEV))
+        # (what no sequence holds is no number, and the kernel of a 16-bit cache wants numbers)
+        return self.run(torch.nan_to_num(cache, nan=0.0))
+
+    def of(self, s):
+        first = sum(self.rows[:s])
+        return slice(first, first + self.rows[s])
+
+
+def _kv(lens, H, D, seed):
+    return [(rows(n, H, D, torch.bfloat16, seed + 2 * s), rows(n, H, D, torch.bfloat16, seed + 2 * s + 1)) for s, n in enumerate(lens)]
+
+
+SHAPES = [([(0, 300), (170, 90), (65, 400)], 8, 2, 128, 32, 64, 0, {}),
+          ([(0, 70), (3, 500), (0, 1)], 4, 4, 64, 64, 16, 5, {"window": 150, "keep_first": 2}),
+          ([(20, 20), (0, 410), (128, 128)], 6, 2, 128, 128, 128, 1, {"softcap": 30.0})]
+
+
+@pytest.mark.parametrize("shape", range(len(SHAPES)))
+@pytest.mark.parametrize("huge", [1e30, 3e5, -1e20])
+def test_large_numbers_of_a_sequence_leave_others_and_earlier_rows_alone(ops, shape, huge):
+    seqs, Q, H, D, group, page, lead, opts = SHAPES[shape]
+    kv = _kv([a + b for a, b in seqs], H, D, 50 * shape)
+    g = torch.Generator().manual_seed(shape)
+    q = torch.randn(sum(b for _, b in seqs), Q, D, generator=g).to(torch.bfloat16)
+    plain = Pass(ops, seqs, kv, q, group, page, lead, **opts).run()
+    at = seqs[1][0] + seqs[1][1] // 2          # a token that half of the rows see
+    k, v = (x.clone() for x in kv[1])
+    k[at, 0, D // 2], v[at, 0, 5] = huge, -huge
+    p = Pass(ops, seqs, [kv[0], (k, v), kv[2]], q, group, page, lead, **opts)
+    got = p.run()
+    for s in (0, 2):
+        assert torch.equal(got[p.of(s)], plain[p.of(s)])
+    mine, rep = got[p.of(1)], Q // H
+    assert torch.equal(mine[:, rep:], plain[p.of(1)][:, rep:])         # its other heads
+    # the head's rows: as over a cache in bf16 (no numbers where a score passes 2^31, here and there), and those before the token as right as there
+    assert torch.allclose(mine[:, :rep], p.run_16_bit()[p.of(1)][:, :rep], rtol=0, atol=0, equal_nan=True)
+    first, n = seqs[1][0], at - seqs[1][0]
+    (kc, ks, kz), (vc, vs, vz) = quantised(k[:at], group), quantised(v[:at], group)
+    kept = (values(kc, ks, kz, group), values(vc, vs, vz, group), ks, kz, vs)
+    x, half = q[p.of(1)][:n], 2.0 ** -8
+    want = attention(x, kept[0], kept[1], torch.arange(first, at), scale=D ** -0.5, **opts)
+    tol = tolerance(x, kept, D ** -0.5, want, want[1], half, torch.bfloat16, group, value_step=half)
+    assert ((mine[:n].double() - want[0]).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("shape", range(len(SHAPES)))
+def test_sequences_of_any_size_in_one_pass(ops, shape):
+    """Keys times powers of two that the sequence's queries take back, and values times powers of two: outputs times those, bit for bit."""
+    seqs, Q, H, D, group, page, lead, opts = SHAPES[shape]
+    kv = _kv([a + b for a, b in seqs], H, D, 50 * shape + 9)
+    q = torch.randn(sum(b for _, b in seqs), Q, D, generator=torch.Generator().manual_seed(shape)).to(torch.bfloat16)
+    plain = Pass(ops, seqs, kv, q, group, page, lead, **opts)
+    base = plain.run()
+    for turn in range(3):
+        e, f = ([(-60, 0, 45)[(s + turn) % 3] for s in range(3)], [(70, -50, 0)[(s + turn) % 3] for s in range(3)])
+        times = lambda x, n: (x.double() * 2.0 ** n).to(torch.bfloat16)  # noqa: E731
+        q2 = torch.cat([times(q[plain.of(s)], -e[s]) for s in range(3)])
+        p = Pass(ops, seqs, [(times(k, e[s]), times(v, f[s])) for s, (k, v) in enumerate(kv)], q2, group, page, lead, **opts)
+        got = p.run()
+        for s in range(3):
+            assert torch.equal(got[p.of(s)], times(base[p.of(s)], f[s])), (turn, s)
+
+
+@pytest.mark.parametrize("by", [-11, -20, -40])
+@pytest.mark.parametrize("what", ["k", "v", "group of v"])
+@pytest.mark.parametrize("D,group,page", [(128, 32, 64), (64, 32, 16)])
+def test_small_numbers_behind_a_window_keep_their_bits(ops, by, what, D, group, page):
+    """Rows that see nothing but tokens far smaller than earlier ones of their sequence (or a group of them that is): as right as over a cache in bf16."""
+    n, turn, window, Q, H = 700, 300, 130, 4, 2
+    k, v = _kv([n], H, D, 3)[0]
+    small = slice(turn, None), slice(None), slice(group if what == "group of v" else 0, None)
+    x = k if what == "k" else v
+    x[small] = (x[small].double() * 2.0 ** by).to(x.dtype)
+    q = torch.randn(n, Q, D, generator=torch.Generator().manual_seed(4)).to(torch.bfloat16)
+    if what == "k":
+        q[turn + window:] = (q[turn + window:].double() * 2.0 ** -by).to(q.dtype)
+    got = Pass(ops, [(0, n)], [(k, v)], q, group, page, window=window).run()[turn + window:]
+    (kc, ks, kz), (vc, vs, vz) = quantised(k[turn:], group), quantised(v[turn:], group)
+    kept = (values(kc, ks, kz, group), values(vc, vs, vz, group), ks, kz, vs)
+    x, half = q[turn + window:], 2.0 ** -8
+    want = attention(x, kept[0], kept[1], torch.arange(window, n - turn), scale=D ** -0.5, window=window)
+    # (the floor for values of order one)
+    tol = tolerance(x, kept, D ** -0.5, want, want[1], half, torch.bfloat16, group, value_step=half) - 1e-7
+    assert ((got.double() - want[0]).abs() <= tol).all()
+    # (sums that cancel take most of that: the outputs together are far closer)
+    assert (got.double() - want[0]).norm() <= 2.0 ** -7 * want[0].norm()
+    if what == "group of v":
+        assert (got.double() - want[0])[..., group:].norm() <= 2.0 ** -7 * want[0][..., group:].norm()
