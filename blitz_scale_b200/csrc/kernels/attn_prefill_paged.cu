@@ -421,6 +421,7 @@ attn_prefill_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
           break;
         }
         row_up = quant_kv_row_fp16<C::kSlabs>(sQ + t * TB + r_ * 128, SB, r_ & 7) * it.k_up;
+        row_up = fmaxf(row_up, 0x1p-126f / p.scale_log2);  // (a factor of zero would make numbers that are none of what is hidden)
         ptx::fence_proxy_async_smem();
         ptx::mbar_arrive(&q_fp16[t]);
       }

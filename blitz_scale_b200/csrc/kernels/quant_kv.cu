@@ -474,6 +474,7 @@ struct QuantPagesParams {
   // for attention of portions: records of the pass (see attn_prefill_paged.cu), whose page numbers count from `first` pages before the first one
   const int32_t* work;
   int entries, first, pages_read;
+  float k_sign;       // what keys are multiplied by (a scale's sign, or zero)
   int32_t* table;     // numbers of the pages read back, for all of those that the records count
   uint4* spans;       // SCALED: [pages][kv_heads] what quant_kv_form takes, where a sequence's first page is; behind them whether some are held in bf16
   float2* forms;      // SCALED: [entries][kv_heads] powers of two taken out of keys and values (zeros: held in bf16)
@@ -658,6 +659,7 @@ __global__ void __launch_bounds__(256, 3) quant_kv_pages_kernel(const QuantPages
         quant_kv_codes(kw[r][w], x);
         float sc = number(ks[r], w * 32 / GROUP), z = number(ks[r], G + w * 32 / GROUP);
         if (SCALED) sc *= form.k_down, z *= form.k_down;
+        if (WORK) sc *= p.k_sign, z *= p.k_sign;
         if (WORK && g + 8 * r >= held) sc = z = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = fmaf(sc, x[i], z);
@@ -824,8 +826,10 @@ int64_t blitz_quant_kv_portion_bytes(int64_t pages, int64_t first, int entries, 
 
 // What attention of portions (blitz_attn_prefill_paged, or blitz_attn_prefill_scaled for a bf16 model) reads instead of a 4-bit cache: pages[n], the
 // (first + n)-th page that the records of `work` count, in 16 bits (of a bf16 model: as quant_kv_form says), zeros behind the end of its sequence.
+// Keys are multiplied by k_sign: hidden scores are infinities that the attention kernel multiplies by its scale, which has to be positive, so the sign
+// of one that is not, or zero, goes into the keys.
 int blitz_quant_kv_portion(const void* pool, const int32_t* pages, int64_t count, int64_t first, const int32_t* work, int entries, int kv_heads, int dim,
-                           int group, int page_size, int max_pages, void* scratch, int* status, int dtype, cudaStream_t stream) {
+                           int group, int page_size, int max_pages, float k_sign, void* scratch, int* status, int dtype, cudaStream_t stream) {
   if (count <= 0 || entries <= 0) return 0;
   if (!quant_kv_supported(dim, group, page_size) || max_pages < 1 || kv_heads < 1 || first < 0 || count + first > 0x7fffffff) return -1;
   if ((reinterpret_cast<uintptr_t>(work) | reinterpret_cast<uintptr_t>(pool) | reinterpret_cast<uintptr_t>(scratch)) & 15) return -1;
@@ -834,7 +838,7 @@ int blitz_quant_kv_portion(const void* pool, const int32_t* pages, int64_t count
   char* s = (char*)scratch;
   QuantPagesParams p{(const uint8_t*)pool, pages, s, s + (int64_t)page_size * kv_heads * dim * 2, count * kv_heads * (page_size / 16), kv_heads, page_size, 2 * page_size, max_pages, status};
   p.work = work; p.entries = entries; p.first = (int)first; p.table = (int32_t*)(s + at[1]); p.spans = (uint4*)(s + at[2]);
-  p.pages_read = (int)count; p.forms = (float2*)(s + at[3]);
+  p.pages_read = (int)count; p.k_sign = k_sign; p.forms = (float2*)(s + at[3]);
   return quant_kv_dispatch(dtype, dim, group, PortionLaunch{p, stream});
 }
 

@@ -9,6 +9,7 @@ cache ``[page][K|V][token][kv_head][head_dim]`` per layer.
 from __future__ import annotations
 
 import ctypes
+import math
 import threading
 from typing import NamedTuple, Optional, Sequence, Union
 
@@ -675,9 +676,11 @@ def _attn_portion_quant(q, cache, page_indices, work, q_heads, kv_heads, head_di
     at = (ctypes.c_int64 * 5)()
     scratch = torch.empty(L.blitz_quant_kv_portion_bytes(n, skip_pages, entries, kv_heads, head_dim, page_size, dt, at), dtype=torch.uint8, device=q.device)
     base = scratch.data_ptr()
+    scale = head_dim ** -0.5 if sm_scale is None else sm_scale
+    sign, scale = (math.copysign(1.0, scale), abs(scale)) if abs(scale) > 0.0 else (scale, 1.0)        # (zero, NaN: itself)
     _check(L.blitz_quant_kv_portion(pool.data_ptr(), page_indices.data_ptr() + 4 * skip_pages, n, skip_pages, work.data_ptr(), entries, kv_heads,
-                                    head_dim, cache.group, page_size, pool.shape[0], base, status, dt, stream), "blitz_quant_kv_portion")
-    scale, values, snk = head_dim ** -0.5 if sm_scale is None else sm_scale, base + 2 * page_size * kv_heads * head_dim, None if sink is None else sink.data_ptr()
+                                    head_dim, cache.group, page_size, pool.shape[0], sign, base, status, dt, stream), "blitz_quant_kv_portion")
+    values, snk = base + 2 * page_size * kv_heads * head_dim, None if sink is None else sink.data_ptr()
     if dt == 1:
         _check(L.blitz_attn_prefill_scaled(q.data_ptr(), q.stride(0), base, values, out.data_ptr(), out.stride(0), base + at[1], work.data_ptr(), entries,
                                            T, q_heads, kv_heads, head_dim, page_size, 2 * page_size, n, scale, window, keep_first, softcap, snk,

@@ -143,3 +143,49 @@ def test_small_numbers_behind_a_window_keep_their_bits(ops, by, what, D, group, 
     assert (got.double() - want[0]).norm() <= 2.0 ** -7 * want[0].norm()
     if what == "group of v":
         assert (got.double() - want[0])[..., group:].norm() <= 2.0 ** -7 * want[0][..., group:].norm()
+
+
+@pytest.mark.parametrize("scale", [-0.11, 0.0, 0.07])
+@pytest.mark.parametrize("opts", [{}, {"softcap": 3.0}, {"window": 50, "keep_first": 1}])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_portion_scales(ops, scale, opts, dt):
+    """A factor of either sign, or zero, as for single tokens; queries and factor times powers of two that cancel change no bit."""
+    seqs, Q, H, D, group = [(0, 300), (70, 3), (200, 129)], 4, 2, 128, 32
+    kv = [(k.to(dt), v.to(dt)) for k, v in _kv([a + b for a, b in seqs], H, D, 7)]
+    q = torch.randn(sum(b for _, b in seqs), Q, D, generator=torch.Generator().manual_seed(3)).to(dt)
+    p = Pass(ops, seqs, kv, q, group, 64, sm_scale=scale, **opts)
+    got = p.run()
+    for s, (a, b) in enumerate(seqs):
+        (kc, ks, kz), (vc, vs, vz) = (quantised(x, group) for x in kv[s])
+        kept = (values(kc, ks, kz, group), values(vc, vs, vz, group), ks, kz, vs)
+        x, half = q[p.of(s)], 2.0 ** -11
+        want = attention(x, kept[0], kept[1], torch.arange(a, a + b), scale=scale, **opts)
+        tol = tolerance(x, kept, abs(scale), want, want[1], half, dt, group, value_step=half)
+        # (as in test_portions: below 2^-14 of the largest of the head, in steps of 2^-24)
+        floor = 2.0 ** -24 * kept[0].abs().amax() * x.double().abs().sum(-1) * abs(scale)
+        tol = tol + torch.expm1(2 * floor)[..., None] * want[1] + 2.0 ** -24 * kept[1].abs().amax()
+        assert ((got[p.of(s)].double() - want[0]).abs() <= tol).all(), s
+    # (fp16 has no more room for queries of order one)
+    for e in (-100, -30, 30, 100) if dt is torch.bfloat16 else (-3, 5):
+        q2 = (q.double() * 2.0 ** e).to(dt)
+        keep = (q2.double() * 2.0 ** -e == q.double()).all(-1)
+        again = Pass(ops, seqs, kv, q2, group, 64, sm_scale=scale * 2.0 ** -e, **opts).run()
+        assert torch.equal(again[keep], got[keep]) and keep.float().mean() > 0.9, e
+
+
+@pytest.mark.parametrize("opts", [{}, {"softcap": 3.0}, {"window": 50, "keep_first": 1}])
+@pytest.mark.parametrize("e,f", [(-90, -90), (-60, -99), (-110, -110), (-95, 0)])
+def test_scores_of_nothing(ops, opts, e, f):
+    """Keys times 2^e and queries times 2^f: scores far below what fp32 tells from zero weigh all visible keys alike."""
+    seqs, Q, H, D, group = [(0, 300), (70, 3), (200, 129)], 4, 2, 64, 32
+    times = lambda x, n: (x.double() * 2.0 ** n).to(torch.bfloat16)  # noqa: E731
+    kv = [(times(k, e), v) for k, v in _kv([a + b for a, b in seqs], H, D, 17)]
+    q = times(torch.randn(sum(b for _, b in seqs), Q, D, generator=torch.Generator().manual_seed(3)), f)
+    p = Pass(ops, seqs, kv, q, group, 64, **opts)
+    got = p.run()
+    for s, (a, b) in enumerate(seqs):
+        vc, vs, vz = quantised(kv[s][1], group)
+        v = values(vc, vs, vz, group)
+        want = attention(q[p.of(s)], torch.zeros_like(v), v, torch.arange(a, a + b), scale=0.0, **opts)
+        # values and weights in bf16 at the worst, and the output
+        assert ((got[p.of(s)].double() - want[0]).abs() <= (2.0 ** -7 + 2.0 ** -15) * want[1] + 2.0 ** -8 * want[0].abs() + 2.0 ** -24 * v.abs().amax()).all(), s
