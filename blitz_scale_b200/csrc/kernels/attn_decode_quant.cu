@@ -69,6 +69,7 @@ struct DecodeQuantParams {
   int window, keep_first;
   const void* sink;
   int* status;
+  int give_up;  // test aid: every other block begins as if a wait had run out
 };
 
 // Shared memory: rings, a slot per warp for the sums of its first piece (the last one's go into the ring), tables of the sequences, barriers.
@@ -183,15 +184,16 @@ __device__ __forceinline__ QdPiece qd_kept(const volatile int* from) {
 }
 
 // Waits (in a converged warp) until words of shared memory that other warps of the block write are not zero: a lane for each that counts.
+// Once a wait of the block has run out, none is waited for.
 __device__ __forceinline__ bool qd_wait(const volatile int* word, bool counts, volatile int* abort_flag) {
-  bool on = !counts || *word != 0;
   const uint64_t since = ptx::globaltimer_ns();
-  for (uint32_t it = 1; !__all_sync(0xffffffffu, on); on = !counts || *word != 0, ++it) {
-    __nanosleep(32);
-    if ((it & 63u) == 0 && __any_sync(0xffffffffu, *abort_flag != 0 || ptx::globaltimer_ns() - since > ptx::kDefaultWaitNs)) {
+  for (uint32_t it = 1;; ++it) {
+    if (__any_sync(0xffffffffu, *abort_flag != 0 || ((it & 63u) == 0 && ptx::globaltimer_ns() - since > ptx::kDefaultWaitNs))) {
       *abort_flag = 1;
       return false;
     }
+    if (__all_sync(0xffffffffu, !counts || *word != 0)) break;
+    __nanosleep(32);
   }
   __threadfence_block();
   return true;
@@ -306,7 +308,7 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
     ptx::mbar_init(&empty[threadIdx.x], 1);
   }
   if (threadIdx.x == 0) {
-    *abort_flag = 0;
+    *abort_flag = p.give_up && (blockIdx.x & 1);
   }
   if (threadIdx.x < kQdWarps) records[threadIdx.x * 16 + 8] = records[threadIdx.x * 16 + 9] = 0;
   ptx::fence_mbar_init();
@@ -433,8 +435,8 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
         }
       }
     }
-    // (after a time-out: no copy may land in shared memory that another block has by then)
-    if (lane < warps && *abort_flag) {
+    // (no copy may land in shared memory that another block has by then: a warp that gave up has not waited for its own)
+    if (lane < warps) {
       since = ptx::globaltimer_ns();
       for (int s = 0; s < p.stages; ++s) {
         if (stage == 0) phase ^= 1u;
@@ -797,10 +799,9 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
       if (h0 >= p.rep || (n > 1 && x1 > it.stop)) continue;
       const unsigned begin = mine.begin(min(w0 + lane, warps));
       const int from = (lane < n && begin < it.start ? (w0 + lane) * (ring_bytes / 4) : kQdWarps * ring_bytes / 4 + min(w0 + lane, kQdWarps - 1) * slot);
-      if (!qd_wait(records + min(w0 + lane, kQdWarps - 1) * 16 + (begin < it.start ? 9 : 8), lane < n, abort_flag)) {
-        if (p.status && lane == 0) atomicCAS(p.status, 0, kStatusTimeoutEpilogue);
-        continue;
-      }
+      // (a wait that ran out is an error that the host reads; the chunks are counted all the same, so that the tickets are zero after this call too)
+      const bool there = qd_wait(records + min(w0 + lane, kQdWarps - 1) * 16 + (begin < it.start ? 9 : 8), lane < n, abort_flag);
+      if (!there && p.status && lane == 0) atomicCAS(p.status, 0, kStatusTimeoutEpilogue);
       constexpr int C = D / 32;  // dimensions of a lane
       const bool inside = it.start >= X0 && it.stop <= X1;
       float* const part_ml = p.part + static_cast<int64_t>(2) * gridDim.x * p.rep * D;
@@ -865,8 +866,12 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
           }
         }
       };
-      if (h0 + each < p.rep) add_up(std::integral_constant<int, 4>{});
-      else add_up(std::integral_constant<int, 1>{});
+      if (!there) {
+      } else if (h0 + each < p.rep) {
+        add_up(std::integral_constant<int, 4>{});
+      } else {
+        add_up(std::integral_constant<int, 1>{});
+      }
       if (inside) continue;
 
       // ------------------------------------------------------------ pieces of several blocks: for each head, whoever is last adds them up
@@ -888,7 +893,7 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
         __threadfence();
       }
       __syncwarp();
-      uint32_t todo = __ballot_sync(0xffffffffu, is_last);
+      uint32_t todo = __ballot_sync(0xffffffffu, is_last && there);
       // H heads at a time, UNROLL of their pieces: eight loads are on their way
       auto merge = [&](auto heads, auto unroll) {
         constexpr int H = decltype(heads)::value, UNROLL = decltype(unroll)::value;
@@ -995,6 +1000,7 @@ static inline int qd_groups(int rep) {
   while (rep % div) ++div;
   return div;
 }
+static std::atomic<int> g_qd_give_up{0};
 
 // Bytes of the partial sums in a workspace, whatever a call's batch and heads: calls of any size share one, and nobody's sums may be where
 // another has its tickets.
@@ -1009,6 +1015,9 @@ using namespace blitz;
 int64_t blitz_attn_decode_quant_workspace_bytes(int batch, int q_heads, int dim) {
   return qd_part_bytes() + (int64_t)batch * q_heads * 4;
 }
+
+// Test aid: while `on` is not zero, every other block of the following launches begins as if a wait had run out.
+void blitz_attn_decode_quant_give_up(int on) { blitz::g_qd_give_up = on != 0; }
 
 // q: [batch] rows with the query heads in their first q_heads * dim columns (pitch a multiple of 8, 16-byte aligned; so out).  A sequence
 // without keys has an output of zeros.  static_table != 0 promises that the tables are not written by kernels still running in this
@@ -1032,7 +1041,7 @@ int blitz_attn_decode_quant(const void* q, int64_t q_stride, const void* pool, c
   const float size = sm_scale < 0.f ? -sm_scale : sm_scale > 0.f ? sm_scale : 1.f;
   p.sign = sm_scale < 0.f ? -1.f : sm_scale > 0.f ? 1.f : sm_scale;
   p.scale_log2 = size * 1.4426950408889634f; p.cap_scale = softcap > 0.f ? size / softcap : 0.f; p.cap_log2 = softcap * 1.4426950408889634f;
-  p.window = window; p.keep_first = keep_first; p.sink = sink; p.static_table = static_table; p.status = status;
+  p.window = window; p.keep_first = keep_first; p.sink = sink; p.static_table = static_table; p.status = status; p.give_up = g_qd_give_up;
   for (int b = 0; b < batch; b += kQdMaxBatch) {
     p.batch = batch - b < kQdMaxBatch ? batch - b : kQdMaxBatch;
     p.q = (const char*)q + (int64_t)b * q_stride * 2;

@@ -156,6 +156,7 @@ def _declare(L: ctypes.CDLL) -> None:
     sig("blitz_attn_prefill_scaled", [c_p, c_i64, c_p, c_p, c_p, c_i64, c_p, c_p, c_i, c_i, c_i, c_i, c_i, c_i, c_i, c_i, c_f, c_i, c_i, c_f, c_p, c_p,
                                       c_p, c_p, c_p])
     sig("blitz_attn_decode_quant_workspace_bytes", [c_i, c_i, c_i], c_i64)
+    sig("blitz_attn_decode_quant_give_up", [c_i], None)
     sig("blitz_attn_decode_quant", [c_p, c_i64, c_p, c_p, c_p, c_p, c_p, c_i64, c_p, c_i64, c_i, c_i, c_i, c_i, c_i, c_i, c_i, c_f, c_i, c_i, c_f,
                                     c_p, c_i, c_p, c_i, c_p])
     # comm kernels

@@ -83,6 +83,29 @@ def test_heads_of_both_sizes_share_a_workspace(ops):
             assert torch.equal(want, got) and want.isfinite().all()
 
 
+@pytest.mark.parametrize("Q,H,D,group", [(32, 8, 128, 32), (8, 1, 64, 64)])
+def test_a_call_that_gave_up_leaves_the_tickets_zero(ops, Q, H, D, group):
+    """A wait that ran out is an error that the host reads, and the next call with this workspace is right."""
+    sizes = [(2, 4000), (70, 900)]
+    calls = _calls(ops, sizes, Q, H, D, group, 64)
+    ws, tickets = torch.zeros(ops.quant_attn_workspace_bytes(70, Q, D), dtype=torch.uint8, device=DEV), ops.quant_attn_workspace_bytes(0, Q, D)
+    want = [torch.empty(n, Q * D, dtype=torch.bfloat16, device=DEV) for n, _ in sizes]
+    for (call, _), out in zip(calls, want):
+        call(out, ws)
+    for (call, _), out in zip(calls, want):
+        got = torch.empty_like(out)
+        ops.lib().blitz_attn_decode_quant_give_up(1)
+        try:
+            call(got, ws)
+        finally:
+            ops.lib().blitz_attn_decode_quant_give_up(0)
+        with pytest.raises(RuntimeError, match="timed out"):
+            ops.check_status()
+        assert not ws[tickets:].any()
+        call(got, ws)
+        assert torch.equal(got, out)
+
+
 @pytest.mark.parametrize("graphs", [False, True])
 def test_an_engine_whose_batch_changes(ops, graphs):
     """Requests of a thousand tokens and more, batches of one to sixty of them in turn: the tokens of every step are those of a runner whose
