@@ -470,6 +470,7 @@ struct QuantPagesParams {
   void *k, *v;       // page n's token `off` at row n * page_rows + off
   int64_t units;     // (page, 16 tokens of it, head) each
   int kv_heads, page_size, page_rows, max_pages;
+  int pool_heads, head0;  // heads of the pool, and the first of the kv_heads that are read
   int* status;
   // for attention of portions: records of the pass (see attn_prefill_paged.cu), whose page numbers count from `first` pages before the first one
   const int32_t* work;
@@ -517,7 +518,7 @@ __global__ void __launch_bounds__(256) quant_kv_span_kernel(const QuantPagesPara
     const int n = static_cast<int>(unit / p.kv_heads / parts), page = p.pages[n];
     const QuantHeld held = quant_kv_held(p, n + p.first);
     if (held.tokens <= b0 * 16 || page < 0 || page >= p.max_pages) continue;
-    const uint8_t* block = p.pool + ((static_cast<int64_t>(page) * p.kv_heads + head) * blocks + b0) * F.block + (lane < 16 ? 0 : F.part) + F.codes + (lane & 15) * 4 * G;
+    const uint8_t* block = p.pool + ((static_cast<int64_t>(page) * p.pool_heads + p.head0 + head) * blocks + b0) * F.block + (lane < 16 ? 0 : F.part) + F.codes + (lane & 15) * 4 * G;
     uint32_t w[EACH][G];
 #pragma unroll
     for (int b = 0; b < EACH; ++b)
@@ -581,7 +582,7 @@ __global__ void __launch_bounds__(256, 3) quant_kv_pages_kernel(const QuantPages
     const int64_t n = unit / p.kv_heads / blocks;
     const int page = p.pages[n];
     const bool bad = page < 0 || page >= p.max_pages;  // (the first page is read instead, and nothing written)
-    const uint8_t* block = p.pool + ((static_cast<int64_t>(bad ? 0 : page) * p.kv_heads + head) * blocks + b) * F.block;
+    const uint8_t* block = p.pool + ((static_cast<int64_t>(bad ? 0 : page) * p.pool_heads + p.head0 + head) * blocks + b) * F.block;
     const int64_t row0 = n * p.page_rows + b * 16, pitch = static_cast<int64_t>(p.kv_heads) * D;
     // everything is asked for before anything is used
     uint32_t kw[2][W], vw[D / 16];
@@ -805,7 +806,7 @@ int blitz_quant_kv_pages(const void* pool, const int32_t* pages, int64_t count, 
   if (count <= 0) return 0;
   if (!quant_kv_supported(dim, group, page_size) || max_pages < 1 || kv_heads < 1 || page_rows < page_size) return -1;
   if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(pool)) & 15) return -1;
-  QuantPagesParams p{(const uint8_t*)pool, pages, k, v, count * kv_heads * (page_size / 16), kv_heads, page_size, page_rows, max_pages, status};
+  QuantPagesParams p{(const uint8_t*)pool, pages, k, v, count * kv_heads * (page_size / 16), kv_heads, page_size, page_rows, max_pages, kv_heads, 0, status};
   return quant_kv_dispatch(dtype, dim, group, PagesLaunch{p, stream});
 }
 
@@ -825,18 +826,20 @@ int64_t blitz_quant_kv_portion_bytes(int64_t pages, int64_t first, int entries, 
 }
 
 // What attention of portions (blitz_attn_prefill_paged, or blitz_attn_prefill_scaled for a bf16 model) reads instead of a 4-bit cache: pages[n], the
-// (first + n)-th page that the records of `work` count, in 16 bits (of a bf16 model: as quant_kv_form says), zeros behind the end of its sequence.
+// (first + n)-th page that the records of `work` count, of its pool_heads heads those from head0 on, in 16 bits (of a bf16 model: as quant_kv_form says), zeros behind the end of its sequence.
 // Keys are multiplied by k_sign: hidden scores are infinities that the attention kernel multiplies by its scale, which has to be positive, so the sign
 // of one that is not, or zero, goes into the keys.
-int blitz_quant_kv_portion(const void* pool, const int32_t* pages, int64_t count, int64_t first, const int32_t* work, int entries, int kv_heads, int dim,
-                           int group, int page_size, int max_pages, float k_sign, void* scratch, int* status, int dtype, cudaStream_t stream) {
+int blitz_quant_kv_portion(const void* pool, const int32_t* pages, int64_t count, int64_t first, const int32_t* work, int entries, int pool_heads,
+                           int head0, int kv_heads, int dim, int group, int page_size, int max_pages, float k_sign, void* scratch, int* status, int dtype, cudaStream_t stream) {
   if (count <= 0 || entries <= 0) return 0;
-  if (!quant_kv_supported(dim, group, page_size) || max_pages < 1 || kv_heads < 1 || first < 0 || count + first > 0x7fffffff) return -1;
+  if (!quant_kv_supported(dim, group, page_size) || max_pages < 1 || kv_heads < 1 || head0 < 0 || head0 + kv_heads > pool_heads || first < 0 ||
+      count + first > 0x7fffffff)
+    return -1;
   if ((reinterpret_cast<uintptr_t>(work) | reinterpret_cast<uintptr_t>(pool) | reinterpret_cast<uintptr_t>(scratch)) & 15) return -1;
   int64_t at[5];
   blitz_quant_kv_portion_bytes(count, first, entries, kv_heads, dim, page_size, dtype, at);
   char* s = (char*)scratch;
-  QuantPagesParams p{(const uint8_t*)pool, pages, s, s + (int64_t)page_size * kv_heads * dim * 2, count * kv_heads * (page_size / 16), kv_heads, page_size, 2 * page_size, max_pages, status};
+  QuantPagesParams p{(const uint8_t*)pool, pages, s, s + (int64_t)page_size * kv_heads * dim * 2, count * kv_heads * (page_size / 16), kv_heads, page_size, 2 * page_size, max_pages, pool_heads, head0, status};
   p.work = work; p.entries = entries; p.first = (int)first; p.table = (int32_t*)(s + at[1]); p.spans = (uint4*)(s + at[2]);
   p.pages_read = (int)count; p.k_sign = k_sign; p.forms = (float2*)(s + at[3]);
   return quant_kv_dispatch(dtype, dim, group, PortionLaunch{p, stream});

@@ -123,6 +123,8 @@ class LlamaRunner:
         self.maxval = torch.empty(max_batch, dtype=torch.float32, device=dev)
         self._ws = {}
         self._ws_old: List[Optional[torch.Tensor]] = []
+        if self.quant:      # (what portions are read back into: a pass finds room for the whole cache, or for the heads that a part of it holds)
+            self._portion_room(kv_cache[0].pool.shape[0])
 
     # ------------------------------------------------------------------ pieces
     def _w(self, l: int, name: str) -> torch.Tensor:
@@ -152,6 +154,15 @@ class LlamaRunner:
             # heads of 128)
             self._ws_old.append(ws)
             ws = self._ws[key] = torch.zeros(n, dtype=torch.uint8, device=self.res.device)
+        return ws
+
+    def _portion_room(self, pages: int) -> torch.Tensor:
+        """Scratch of prefill attention over a 4-bit cache, for passes of up to `pages` pages."""
+        entries = self.max_tokens // ops.PREFILL_ROWS + self.max_batch
+        n = ops.quant_portion_workspace_bytes(pages, entries, self.kvh, self.hd, self.page_size, self.res.dtype)
+        ws = self._ws.get("portion")
+        if ws is None or ws.numel() < n:
+            ws = self._ws["portion"] = torch.empty(n, dtype=torch.uint8, device=self.res.device)
         return ws
 
     def _layer_cache(self, l: int, m: StepMeta) -> Union[torch.Tensor, ops.QuantKV]:
@@ -195,10 +206,12 @@ class LlamaRunner:
         if m.prefill_work is None:      # a caller that built the step by hand
             m.prefill_work = ops.prefill_work_list(m.seq_lens_host, m.kv_lens_host or m.seq_lens_host, self.page_size,
                                                    self.qkv.device, skip=ns)
-        # (a 4-bit cache: the pages of the single tokens' sequences, which come first, are not read back)
-        skip = sum(-(-n // self.page_size) for n in m.kv_lens_host[:ns]) if self.quant else 0
+        more = {}
+        if self.quant:      # (the pages of the single tokens' sequences, which come first, are not read back)
+            skip = m.view(("skip", ns), m.prefill_work, lambda _: sum(-(-n // self.page_size) for n in m.kv_lens_host[:ns]))
+            more = dict(skip_pages=skip, workspace=m.view("portion room", m.page_indices, lambda t: self._portion_room(t.shape[0])))
         ops.attn_prefill_paged(m.rows("qkv", self.qkv, T), kv, m.page_indices, m.prefill_work, q_heads=self.qh,
-                               kv_heads=self.kvh, head_dim=self.hd, page_size=self.page_size, out=m.rows("attn", self.attn, T), skip_pages=skip)
+                               kv_heads=self.kvh, head_dim=self.hd, page_size=self.page_size, out=m.rows("attn", self.attn, T), **more)
 
     def last_rows(self, m: StepMeta) -> torch.Tensor:
         """[batch, hidden]: the state `head` starts from, for the last row of every sequence of a prefill pass."""

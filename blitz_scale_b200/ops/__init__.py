@@ -661,34 +661,61 @@ def _attn_decode_quant(q, cache, indices, indptr, last_page_len, q_heads, kv_hea
     return out
 
 
-def _attn_portion_quant(q, cache, page_indices, work, q_heads, kv_heads, head_dim, page_size, out, sm_scale, window, keep_first, softcap, sink, skip_pages):
+QUANT_PORTION_BYTES = 1 << 28       # of keys and values that attention of portions reads back at a time (or those of one KV head, where that is more)
+
+
+def _quant_portion(pages: int, skip: int, entries: int, kv_heads: int, head_dim: int, page_size: int, dt: int, room: int) -> tuple:
+    """(KV heads whose pages fit into `room` bytes of scratch, one at least; bytes for so many)"""
+    need = lambda h: lib().blitz_quant_kv_portion_bytes(pages, skip, entries, h, head_dim, page_size, dt, None)  # noqa: E731
+    heads, size = kv_heads, need(kv_heads)
+    while size > room and heads > 1:
+        heads = max(1, min(heads - 1, room * heads // size))
+        size = need(heads)
+    return heads, size
+
+
+def quant_portion_workspace_bytes(pages: int, entries: int, kv_heads: int, head_dim: int, page_size: int, dtype: torch.dtype) -> int:
+    """Scratch of `attn_prefill_paged` over a 4-bit cache: for calls of up to ``pages`` pages (skipped ones and others) and ``entries`` records."""
+    return _quant_portion(pages, pages, entries, kv_heads, head_dim, page_size, _DT[dtype], QUANT_PORTION_BYTES)[1]
+
+
+def _attn_portion_quant(q, cache, page_indices, work, q_heads, kv_heads, head_dim, page_size, out, sm_scale, window, keep_first, softcap, sink, skip_pages,
+                        workspace):
     _int32(page_indices, None, "page_indices")
     P = page_indices.shape[0]
     if not 0 <= skip_pages <= P:
         raise ValueError(f"skip_pages {skip_pages} of {P} pages")
     if work.dtype != torch.int32 or work.dim() != 2 or work.shape[1] != 8 or not work.is_contiguous() or work.data_ptr() & 15:
         raise ValueError(f"work: records of prefill_work_list, got {tuple(work.shape)} {work.dtype}")
+    if workspace is not None and (workspace.dtype is not torch.uint8 or not workspace.is_contiguous() or workspace.data_ptr() & 255):
+        raise ValueError(f"workspace: bytes that start on a 256-byte boundary, got {workspace.dtype}")
     T, entries, n = q.shape[0], work.shape[0], P - skip_pages
-    out = _quant_attn(q, T, cache, q_heads, kv_heads, head_dim, page_size, window, keep_first, softcap, sink, out, page_indices, work)
+    out = _quant_attn(q, T, cache, q_heads, kv_heads, head_dim, page_size, window, keep_first, softcap, sink, out, page_indices, work, workspace)
     if entries == 0 or T == 0 or n == 0:
         return out
-    L, pool, dt, status, stream = lib(), cache.pool, _DT[q.dtype], _status_ptr(q), _stream()
-    at = (ctypes.c_int64 * 5)()
-    scratch = torch.empty(L.blitz_quant_kv_portion_bytes(n, skip_pages, entries, kv_heads, head_dim, page_size, dt, at), dtype=torch.uint8, device=q.device)
-    base = scratch.data_ptr()
+    L, pool, dt, status, stream, rep = lib(), cache.pool, _DT[q.dtype], _status_ptr(q), _stream(), q_heads // kv_heads
+    heads, size = _quant_portion(n, skip_pages, entries, kv_heads, head_dim, page_size, dt, QUANT_PORTION_BYTES if workspace is None else workspace.numel())
+    if workspace is None:
+        workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
+    elif workspace.numel() < size:
+        raise ValueError(f"workspace of {workspace.numel()} bytes, {size} are needed")
+    base, at = workspace.data_ptr(), (ctypes.c_int64 * 5)()
     scale = head_dim ** -0.5 if sm_scale is None else sm_scale
     sign, scale = (math.copysign(1.0, scale), abs(scale)) if abs(scale) > 0.0 else (scale, 1.0)        # (zero, NaN: itself)
-    _check(L.blitz_quant_kv_portion(pool.data_ptr(), page_indices.data_ptr() + 4 * skip_pages, n, skip_pages, work.data_ptr(), entries, kv_heads,
-                                    head_dim, cache.group, page_size, pool.shape[0], sign, base, status, dt, stream), "blitz_quant_kv_portion")
-    values, snk = base + 2 * page_size * kv_heads * head_dim, None if sink is None else sink.data_ptr()
-    if dt == 1:
-        _check(L.blitz_attn_prefill_scaled(q.data_ptr(), q.stride(0), base, values, out.data_ptr(), out.stride(0), base + at[1], work.data_ptr(), entries,
-                                           T, q_heads, kv_heads, head_dim, page_size, 2 * page_size, n, scale, window, keep_first, softcap, snk,
-                                           base + at[3], base + at[2] + 16 * n * kv_heads, status, stream), "blitz_attn_prefill_scaled")
-    else:
-        _check(L.blitz_attn_prefill_paged(q.data_ptr(), q.stride(0), base, values, out.data_ptr(), out.stride(0), base + at[1], work.data_ptr(), entries, T,
-                                          q_heads, kv_heads, head_dim, head_dim, page_size, 2 * page_size, n, scale, 0, window, keep_first, 0, 0, softcap,
-                                          snk, None, 0, None, 0, status, dt, stream), "blitz_attn_prefill_paged")
+    for h0 in range(0, kv_heads, heads):
+        hn = min(heads, kv_heads - h0)
+        L.blitz_quant_kv_portion_bytes(n, skip_pages, entries, hn, head_dim, page_size, dt, at)
+        _check(L.blitz_quant_kv_portion(pool.data_ptr(), page_indices.data_ptr() + 4 * skip_pages, n, skip_pages, work.data_ptr(), entries, kv_heads, h0, hn,
+                                        head_dim, cache.group, page_size, pool.shape[0], sign, base, status, dt, stream), "blitz_quant_kv_portion")
+        first, values, snk = 2 * h0 * rep * head_dim, base + 2 * page_size * hn * head_dim, None if sink is None else sink.data_ptr() + 2 * h0 * rep
+        if dt == 1:
+            _check(L.blitz_attn_prefill_scaled(q.data_ptr() + first, q.stride(0), base, values, out.data_ptr() + first, out.stride(0), base + at[1],
+                                               work.data_ptr(), entries, T, hn * rep, hn, head_dim, page_size, 2 * page_size, n, scale, window, keep_first,
+                                               softcap, snk, base + at[3], base + at[2] + 16 * n * hn, status, stream), "blitz_attn_prefill_scaled")
+        else:
+            _check(L.blitz_attn_prefill_paged(q.data_ptr() + first, q.stride(0), base, values, out.data_ptr() + first, out.stride(0), base + at[1],
+                                              work.data_ptr(), entries, T, hn * rep, hn, head_dim, head_dim, page_size, 2 * page_size, n, scale, 0, window,
+                                              keep_first, 0, 0, softcap, snk, None, 0, None, 0, status, dt, stream), "blitz_attn_prefill_paged")
     return out
 
 
@@ -761,6 +788,7 @@ def prefill_work_list(q_lens, kv_lens, page_size: int, device, skip: int = 0) ->
     return torch.tensor(rec, dtype=torch.int32).reshape(-1, 8).to(device, non_blocking=True)
 
 
+PREFILL_ROWS = 256          # rows of a record of prefill_work_list
 PREFILL_KEY_BLOCK = 128     # keys that attn_prefill_paged walks at a time
 
 
@@ -769,20 +797,22 @@ def attn_prefill_paged(q: torch.Tensor, kv_layer: KVLayer, page_indices: torch.T
                        sm_scale: Optional[float] = None, poly_exp: bool = False, window: int = 0, keep_first: int = 0,
                        softcap: float = 0.0, sink: Optional[torch.Tensor] = None,
                        gate: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, chunked: bool = False,
-                       sigmoid: bool = False, skip_pages: int = 0) -> torch.Tensor:
+                       sigmoid: bool = False, skip_pages: int = 0, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Causal attention of the pass's rows over the paged cache (which already holds the rows' own keys and values,
     after whatever earlier passes stored).  ``q``: rotated query columns, e.g. the fused qkv buffer (rope_kv_store);
     ``page_indices``: the sequences' page ids back to back, covering prefix + rows; ``work`` from `prefill_work_list`
     for the same sequences.  ``window`` / ``keep_first`` / ``softcap`` / ``sink`` / ``gate`` / ``bias`` / ``chunked`` / ``sigmoid``
     as for `attn_decode` (no bias beside a window, cap or sink; with sigmoid weights a bias of one column).
 
-    Over a 4-bit cache (QuantKV): the pages that ``work`` refers to are read back first, into scratch of this call (of a bf16 model in
-    fp16, as its queries enter, divided by powers of two of the sequence and head, or in bf16 where a sequence's keys or values of a head span
-    more than fp16 holds); tokens behind a sequence's end may hold anything; no gate, bias, ``chunked`` or ``sigmoid``; no record of ``work`` refers to the first ``skip_pages`` entries of ``page_indices``."""
+    Over a 4-bit cache (QuantKV): the pages that ``work`` refers to are read back first (of a bf16 model in fp16, as its queries enter, divided by
+    powers of two of the sequence and head, or in bf16 where a sequence's keys or values of a head span more than fp16 holds), as many KV heads at a time as
+    ``workspace`` has room for (`quant_portion_workspace_bytes`; for one call at a time; None: scratch of this call, of QUANT_PORTION_BYTES or
+    one head's pages at most).  Tokens behind a sequence's end may hold anything; no gate, bias, ``chunked`` or ``sigmoid``; no record of
+    ``work`` refers to the first ``skip_pages`` entries of ``page_indices``."""
     if isinstance(kv_layer, QuantKV):
         _quant_refuses(gate, bias, chunked, sigmoid)
         return _attn_portion_quant(q, kv_layer, page_indices, work, q_heads, kv_heads, head_dim, page_size, out, sm_scale, window, keep_first, softcap, sink,
-                                   skip_pages)
+                                   skip_pages, workspace)
     T = q.shape[0]
     kp, vp, page_rows, pages, vdim = _kv(kv_layer)
     if out is None:

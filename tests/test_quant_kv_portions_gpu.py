@@ -189,3 +189,67 @@ def test_scores_of_nothing(ops, opts, e, f):
         want = attention(q[p.of(s)], torch.zeros_like(v), v, torch.arange(a, a + b), scale=0.0, **opts)
         # values and weights in bf16 at the worst, and the output
         assert ((got[p.of(s)].double() - want[0]).abs() <= (2.0 ** -7 + 2.0 ** -15) * want[1] + 2.0 ** -8 * want[0].abs() + 2.0 ** -24 * v.abs().amax()).all(), s
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("opts", [{}, {"window": 100, "keep_first": 3, "sink": True}])
+@pytest.mark.parametrize("lead", [0, 3])
+def test_some_heads_at_a_time(ops, monkeypatch, dt, opts, lead):
+    """Scratch of a fixed size, whatever the pages of a pass: outputs bit for bit those of one round, large numbers in some heads or not."""
+    seqs, Q, H, D, group, page = [(900, 300), (0, 129), (77, 1)], 10, 5, 64, 32, 16
+    kv = [(k.to(dt), v.to(dt)) for k, v in _kv([a + b for a, b in seqs], H, D, 21)]
+    if dt is torch.bfloat16:
+        kv[0][0][5, 3, 1] = 2.0 ** 40
+    q = torch.randn(sum(b for _, b in seqs), Q, D, generator=torch.Generator().manual_seed(2)).to(dt)
+    opts = dict(opts)
+    if opts.pop("sink", False):
+        opts["sink"] = torch.randn(Q, generator=torch.Generator().manual_seed(1)).to(dt)
+    p = Pass(ops, seqs, kv, q, group, page, lead, **opts)
+    want, same = p.run(), lambda a, b: torch.allclose(a, b, rtol=0, atol=0, equal_nan=True)  # (a score past 2^31 is no number)
+    assert want.isfinite().float().mean() > 0.8
+    pages, entries = p.table.numel(), 4
+    whole, one = (ops._quant_portion(pages, lead, entries, h, D, page, ops._DT[dt], 1 << 40)[1] for h in (H, 1))
+    for room in (whole - 1, whole // 2, 2 * one + 1, one, 1):
+        monkeypatch.setattr(ops, "QUANT_PORTION_BYTES", room)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        got = p.run()
+        # (beside the scratch: tables, queries and output, and the allocator's 512 bytes of each)
+        assert torch.cuda.max_memory_allocated() - before <= max(room, one) + 3 * q.numel() * 2 + 65536
+        assert same(got, want), room
+        ws = torch.empty(max(room, one) // 256 * 256 + 256, dtype=torch.uint8, device=DEV)
+        p.opts["workspace"] = ws
+        assert same(p.run(), want), room
+        del p.opts["workspace"]
+    for bad in (torch.empty(one - 1, dtype=torch.uint8, device=DEV), torch.empty(whole, dtype=torch.int8, device=DEV), torch.empty(whole + 8, dtype=torch.uint8, device=DEV)[8:],
+                torch.empty(2 * whole, dtype=torch.uint8, device=DEV)[::2]):
+        p.opts["workspace"] = bad
+        with pytest.raises(ValueError, match="workspace"):
+            p.run()
+
+
+def test_an_engine_reserves_what_portions_take(ops, monkeypatch):
+    """Long prompts, and portions beside them, take no memory that the engine has not had since it was made."""
+    from blitz_scale_b200.runtime import core
+    from blitz_scale_b200.runtime.engine import Engine
+    g = torch.Generator().manual_seed(3)
+    prompts = [torch.randint(0, 4096, (n,), generator=g).tolist() for n in (3000, 17, 900)]
+    steps = [[2000, 0, 500], [500, 16, 399], [500, 1, 1]]
+    outs = []
+    for room in (1 << 28, 1 << 20):
+        monkeypatch.setattr(ops, "QUANT_PORTION_BYTES", room)
+        eng = Engine("tiny_gpu_wide", num_pages=256, page_size=16, max_batch=8, max_batch_tokens=4096, seed=0, kv_bits=4)
+        reserved = eng.runner._ws["portion"]
+        assert reserved.numel() <= max(room, 256 * 16 * 4 * 128 + 65536)
+        b = eng.new_batch(1, [core.SeqSpec(i, p, 6) for i, p in enumerate(prompts)])
+        got = []
+        for counts in steps:
+            torch.cuda.synchronize()
+            torch.cuda.reset_peak_memory_stats()
+            before = torch.cuda.memory_allocated()
+            got.append(eng.step(b, counts, [[c - 1] if c else [] for c in counts]))
+            assert torch.cuda.max_memory_allocated() - before <= 1 << 20        # (logits, tables)
+        assert eng.runner._ws["portion"] is reserved
+        outs.append(torch.cat(got))
+    assert torch.equal(*outs)
