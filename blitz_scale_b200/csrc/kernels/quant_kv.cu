@@ -347,7 +347,7 @@ struct QuantLoadParams {
   const int32_t* slot;
   void *k, *v;    // row r of both
   int64_t rows, units;  // (rows of a warp, head, keys or values) each
-  int kv_heads, page_shift, max_pages;
+  int kv_heads, page_shift, max_pages, zeros;  // zeros: of rows without a slot, bit 0: in k, bit 1: in v (else they are left as they are)
   int* status;
 };
 
@@ -443,8 +443,14 @@ __global__ void __launch_bounds__(128) quant_kv_load_kernel(const QuantLoadParam
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = codes[row * PITCH + dim(i) / 8];
   }
-  if (s < 0) return;
   T* const to = reinterpret_cast<T*>(value ? p.v : p.k) + ((t0 + row) * p.kv_heads + head) * D;
+  if (s < 0) {
+    if (((p.zeros >> static_cast<int>(value)) & 1) && t0 + row < p.rows) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(to + dim(i)) = make_uint4(0, 0, 0, 0);
+    }
+    return;
+  }
   auto number = [&](int i) { return __uint_as_float(i & 1 ? numbers[i >> 1] & 0xffff0000u : numbers[i >> 1] << 16); };
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -790,13 +796,14 @@ int blitz_quant_kv_rope(void* qkv, const int32_t* pos, const int32_t* slot, void
   return quant_kv_dispatch(dtype, dim, group, RopeLaunch{p, static_meta, stream});
 }
 
-// Row slot[r] to row r of k and v, in 16 bits (a negative slot: row r is left as it is).
+// Row slot[r] to row r of k and v, in 16 bits (a negative slot, or one that there is not: row r is left as it is, or zeros, in k where bit 0 of `zeros` is
+// set, in v bit 1).
 int blitz_quant_kv_load(const void* pool, const int32_t* slot, int64_t rows, void* k, void* v, int kv_heads, int dim, int group, int page_size,
-                        int max_pages, int* status, int dtype, cudaStream_t stream) {
+                        int max_pages, int zeros, int* status, int dtype, cudaStream_t stream) {
   if (rows <= 0) return 0;
   if (!quant_kv_supported(dim, group, page_size) || max_pages < 1 || kv_heads < 1) return -1;
   if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(pool)) & 15) return -1;
-  QuantLoadParams p{(const uint8_t*)pool, slot, k, v, rows, 0, kv_heads, quant_kv_shift(page_size), max_pages, status};
+  QuantLoadParams p{(const uint8_t*)pool, slot, k, v, rows, 0, kv_heads, quant_kv_shift(page_size), max_pages, zeros, status};
   return quant_kv_dispatch(dtype, dim, group, LoadLaunch{p, stream});
 }
 

@@ -550,9 +550,11 @@ def _rope_quant(qkv, pos, slot, cache, q_heads, kv_heads, head_dim, page_size, r
 
 def quant_kv_load(cache: QuantKV, slot: torch.Tensor, *, dtype: torch.dtype = torch.bfloat16, k: Optional[torch.Tensor] = None,
                   v: Optional[torch.Tensor] = None):
-    """Keys and values [T, kv_heads, dim] of slots of a 4-bit cache, rounded to 16 bits (rows with a negative slot are left as they are)."""
+    """Keys and values [T, kv_heads, dim] of slots of a 4-bit cache, rounded to 16 bits.  Rows with a negative slot are left as they are in a
+    ``k`` or ``v`` that is given, and zeros in one that is not."""
     pool, D, group = cache
     _int32(slot, None, "slot")
+    zeros = int(k is None) | 2 * int(v is None)
     n, (pages, H, blocks, _) = slot.shape[0], pool.shape
     if k is None and v is None:
         if dtype not in _DT:
@@ -568,7 +570,7 @@ def quant_kv_load(cache: QuantKV, slot: torch.Tensor, *, dtype: torch.dtype = to
             if t.shape != (n, H, D) or not t.is_contiguous() or t.dtype != k.dtype or t.data_ptr() & 15:
                 raise ValueError(f"k and v: contiguous {(n, H, D)} of one type, got {tuple(t.shape)} {t.dtype}")
         _quant(cache, slot, k, v)
-    rc = lib().blitz_quant_kv_load(pool.data_ptr(), slot.data_ptr(), n, k.data_ptr(), v.data_ptr(), H, D, group, 16 * blocks, pages, _status_ptr(pool), _dt(k),
+    rc = lib().blitz_quant_kv_load(pool.data_ptr(), slot.data_ptr(), n, k.data_ptr(), v.data_ptr(), H, D, group, 16 * blocks, pages, zeros, _status_ptr(pool), _dt(k),
                                    _stream())
     if rc:
         _check(rc, "blitz_quant_kv_load")

@@ -149,7 +149,7 @@ def _declare(L: ctypes.CDLL) -> None:
     # a cache held in 4 bits
     sig("blitz_quant_kv_store", [c_p, c_i64, c_p, c_i64, c_p, c_p, c_i, c_i, c_i, c_i, c_i, c_i, c_p, c_i, c_p])
     sig("blitz_quant_kv_rope", [c_p, c_p, c_p, c_p, c_i, c_i, c_i, c_i, c_i, c_i, c_i, c_f, c_i, c_p, c_i, c_p])
-    sig("blitz_quant_kv_load", [c_p, c_p, c_i64, c_p, c_p, c_i, c_i, c_i, c_i, c_i, c_p, c_i, c_p])
+    sig("blitz_quant_kv_load", [c_p, c_p, c_i64, c_p, c_p, c_i, c_i, c_i, c_i, c_i, c_i, c_p, c_i, c_p])
     sig("blitz_quant_kv_pages", [c_p, c_p, c_i64, c_p, c_p, c_i, c_i, c_i, c_i, c_i, c_i, c_p, c_i, c_p])
     sig("blitz_quant_kv_portion_bytes", [c_i64, c_i64, c_i, c_i, c_i, c_i, c_i, c_p], c_i64)
     sig("blitz_quant_kv_portion", [c_p, c_p, c_i64, c_i64, c_p, c_i, c_i, c_i, c_i, c_i, c_i, c_i, c_i, c_f, c_p, c_p, c_i, c_p])
