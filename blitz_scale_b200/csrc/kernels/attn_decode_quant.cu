@@ -751,7 +751,7 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
         T* to = out + it.b * p.out_stride + static_cast<int64_t>(it.head * p.rep + hq) * D + 2 * t4;
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-          const uint32_t a = qd_transposed(pk2<T>(o[i][0] * r[0], o[i][1] * r[1])), b = qd_transposed(pk2<T>(o[i][2] * r[0], o[i][3] * r[1]));
+          const uint32_t a = qd_transposed(quant_kv_means<T>(o[i][0] * r[0], o[i][1] * r[1])), b = qd_transposed(quant_kv_means<T>(o[i][2] * r[0], o[i][3] * r[1]));
           if (hq < p.rep && (!HALVES || (i * 16 / GROUP) / N == xq)) {
             *reinterpret_cast<uint32_t*>(to + 16 * i) = a;
             *reinterpret_cast<uint32_t*>(to + 16 * i + 8) = b;
@@ -816,7 +816,7 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
         const float r = sum != 0.f ? f * ptx::rcp_approx(sum) : 0.f;
         T* to = out + it.b * p.out_stride + static_cast<int64_t>(it.head * p.rep + hh) * D + lane * C;
 #pragma unroll
-        for (int i = 0; i < C; i += 2) stf2<T>(to + i, acc[i] * r, acc[i + 1] * r);
+        for (int i = 0; i < C; i += 2) *reinterpret_cast<uint32_t*>(to + i) = quant_kv_means<T>(acc[i] * r, acc[i + 1] * r);
       };
       auto four = [&](const float* v, float f, float (&acc)[C], bool global) {
         if (C == 4) {

@@ -84,6 +84,14 @@ template <typename T>
 __device__ __forceinline__ constexpr float quant_kv_most() { return std::is_same<T, __half>::value ? 65504.f : 3.3895313892515355e38f; }
 __device__ __forceinline__ bool quant_kv_past(float s, float z, float most) { return fmaxf(fabsf(z), fabsf(fmaf(15.f, s, z))) > most; }
 __device__ __forceinline__ float quant_kv_cut(float x, float most) { return fabsf(x) > most ? copysignf(most, x) : x; }
+// Two weighted means of such numbers, rounded to T (a in the lower half): no number that was quantised is past the type's largest finite one, so no mean is.
+template <typename T>
+__device__ __forceinline__ uint32_t quant_kv_means(float a, float b) {
+  uint32_t d;
+  if (std::is_same<T, __half>::value) asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(b), "f"(a));
+  else asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(b), "f"(a));
+  return d;
+}
 
 // Calls f with the element type and the sizes as types and constants.
 template <typename F>
