@@ -15,6 +15,16 @@ from __future__ import annotations
 from typing import Optional, Sequence, Tuple
 
 
+def same_on_all_ranks(what: str, value, group=None):
+    """`value`, if every rank of the group has the same; else an error on every rank that says who has what.  All ranks call."""
+    import torch.distributed as dist
+    all_ = [None] * dist.get_world_size(group)
+    dist.all_gather_object(all_, value, group=group)
+    if any(v != all_[0] for v in all_):
+        raise ValueError(f"{what} differs between ranks: " + ", ".join(f"{r}: {v}" for r, v in enumerate(all_)))
+    return value
+
+
 class LoadAgreement:
     def __init__(self, fabric, tp_ranks: Sequence[int], my_rank: int, flag0: int, layers: int):
         self.fabric, self.ranks, self.flag0, self.layers = fabric, list(tp_ranks), flag0, layers

@@ -31,7 +31,7 @@ from ..models.config import get_config
 from ..models.llama import TPComm
 from ..models.weights import WeightSegment
 from ..parallel import symm
-from ..parallel.agreement import LoadAgreement, StepLog
+from ..parallel.agreement import LoadAgreement, StepLog, same_on_all_ranks
 from ..pb.schema import pb
 from ..runtime import core
 from ..runtime.engine import Engine, kv_page_bytes
@@ -69,6 +69,10 @@ class GpuBackend(Backend):
             self.page_bytes = kv_page_bytes(self.cfg, page_size, tp, kv_bits, kv_group)
             self.kv_layer_stride = num_pages * self.page_bytes
             kv_bytes = self.cfg.layers * self.kv_layer_stride
+            if use_fabric and world > 1:
+                # (a push writes pages where the sender's sizes say they are in the receiver's pool)
+                same_on_all_ranks("the cache's form", {"kv_bits": kv_bits, "kv_group": kv_group if kv_bits == 4 else None,
+                                                       "page_size": page_size, "num_pages": num_pages})
         self.slot_bytes = max_batch_tokens * self.cfg.hidden * 2
         self.fabric: Optional[symm.PeerFabric] = None
         seg_buf = kv_buf = None
