@@ -50,6 +50,10 @@ class ModelConfig:
     def kv_bytes_per_token(self, tp: int = 1, elem: int = 2) -> int:
         return 2 * (self.kv_heads // tp) * self.head_dim * elem * self.layers
 
+    def kv_bytes_per_token_in_4_bits(self, tp: int = 1, group: int = 32) -> int:
+        """Codes, and a scale and an offset of 16 bits for every `group` dimensions of a head."""
+        return 2 * (self.kv_heads // tp) * (self.head_dim // 2 + 4 * (self.head_dim // group)) * self.layers
+
 
 # end-of-sequence ids of the published tokenizers: </s> = 2 (Llama-2, Mistral, OPT), <|end_of_text|> = 128001 (Llama-3),
 # <|endoftext|> = 151643 (Qwen-2.5); a chat-tuned checkpoint that ends turns with another id sets --eos-token-id

@@ -596,6 +596,9 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--block-size", type=int, default=64, help="tokens per KV page; must equal the workers' --page-size")
     ap.add_argument("--tokens-prefilled-per-sec", type=int, default=15000)
     ap.add_argument("--tokens-transferred-per-sec", type=int, default=96000)
+    ap.add_argument("--kv-bits", type=int, default=16, choices=[16, 4], help="bits of the workers' cached keys and values, as they were started "
+                    "with (for the flow report)")
+    ap.add_argument("--kv-group", type=int, default=32, choices=[32, 64, 128], help="the workers' --kv-group")
     for n, d in (("prefill-lower-bound", .5), ("prefill-upper-bound", .7), ("decode-lower-bound", .75),
                  ("decode-upper-bound", .95), ("migration-lower-bound", .4), ("migration-upper-bound", .8)):
         ap.add_argument("--" + n, type=float, default=d)
@@ -663,6 +666,11 @@ def build_parser() -> argparse.ArgumentParser:
     return ap
 
 
+def kv_mb_per_token(cfg, kv_bits: int = 16, kv_group: int = 32) -> float:
+    """What a migrated token adds to the flow report."""
+    return (cfg.kv_bytes_per_token(1, 2) if kv_bits == 16 else cfg.kv_bytes_per_token_in_4_bits(1, kv_group)) / 1e6
+
+
 def main(argv=None) -> None:
     a = build_parser().parse_args(argv)
     if a.ngrok or a.ngrok_authtoken or a.ngrok_edge:
@@ -716,7 +724,7 @@ def main(argv=None) -> None:
     try:
         from ..runtime import core as _core
         cfg.param_gb = _core.build_segment_layout(a.model_name, a.tensor_parallel_size, 2).total_bytes * a.tensor_parallel_size / 1e9
-        cfg.kv_mb_per_token = get_config(a.model_name).kv_bytes_per_token(1, 2) / 1e6
+        cfg.kv_mb_per_token = kv_mb_per_token(get_config(a.model_name), a.kv_bits, a.kv_group)
     except Exception:  # noqa: BLE001 - only feeds a metric
         pass
     async def amain():

@@ -1,4 +1,4 @@
-"""Replicas of a cluster have caches of one form: those of others are refused when the workers start."""
+"""Replicas of a cluster have caches of one form: those of others are refused when the workers start, and the router counts its bytes."""
 import multiprocessing
 
 import pytest
@@ -72,3 +72,15 @@ def test_workers_of_one_form_start(tmp_path):
 
 def test_groups_do_not_matter_to_a_16_bit_cache(tmp_path):
     assert _run(_backend, [dict(kv_bits=16, kv_group=32), dict(kv_bits=16, kv_group=64)], tmp_path) == ["the same"] * 2
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_bytes_of_a_migrated_token(group):
+    from blitz_scale_b200.models.config import get_config
+    from blitz_scale_b200.router.server import build_parser, kv_mb_per_token
+    from blitz_scale_b200.runtime.engine import kv_page_bytes
+    c = get_config("llama3_8b")
+    a = build_parser().parse_args(["--kv-bits", "4", "--kv-group", str(group), "--client-config", "[]", "--deployment-config-path", "x"])
+    assert kv_mb_per_token(c, a.kv_bits, a.kv_group) * 1e6 == pytest.approx(c.layers * kv_page_bytes(c, 64, kv_bits=4, kv_group=group) / 64)
+    a = build_parser().parse_args(["--client-config", "[]", "--deployment-config-path", "x"])
+    assert kv_mb_per_token(c, a.kv_bits, a.kv_group) * 1e6 == pytest.approx(c.kv_bytes_per_token())
