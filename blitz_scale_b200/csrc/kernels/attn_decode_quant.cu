@@ -10,8 +10,9 @@
 // A code, or 16 times one, is an fp16 number as its bits stand in a half's low byte: a denormal, c 2^-24, which the tensor cores multiply like any
 // other.  A word of 8 codes takes five instructions and no constant has to come off again.  Queries enter in fp16, a head divided by a power of
 // two that brings its largest entry to 2^14 .. 2^15 (2^10 .. 2^11 for what meets 16 times a code): bf16 and fp16 numbers are exact there down to
-// 2^-24 of the largest, and so are their products with codes.  Weights times scales are rounded to fp16, times a power of two that brings the
-// largest scale so far to 2^6 .. 2^7: 2^-11 of each down to scales 2^-20 of the largest, less below.  Their product with -8, one more matrix
+// 2^-24 of the largest, and so are their products with codes.  Weights times scales are rounded to fp16, times a power of two of the
+// head's that brings the largest scale so far that has a weight to 2^6 .. 2^7 (less, where tokens without one have larger scales): 2^-11 of each down to scales 2^-20 of
+// the largest, less below.  Their product with -8, one more matrix
 // product a group, makes the codes lie around zero, so that this rounding is not amplified by what cancels.  The part of z_j + 8 s_j stays in 32
 // bits; the sums of q_d z_g in the scores are one more product, in bf16, of z as stored with sums of q in two numbers.
 //
@@ -221,6 +222,10 @@ __device__ __forceinline__ uint32_t qd_transposed(uint32_t x) {
 }
 __device__ __forceinline__ float qd_low(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float qd_high(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+
+// Exponent of a positive number; 2^e, -126 <= e <= 127.
+__device__ __forceinline__ int qd_exponent(float x) { return static_cast<int>(__float_as_uint(x) >> 23) - 127; }
+__device__ __forceinline__ float qd_power(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
 
 // Scales and offsets of a token, of the groups that a lane's columns stand for (all, or half x of them).
 template <int G, bool HALVES>
@@ -536,8 +541,10 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
         }
       }
 
-      // `down` takes scales to 16 bits, `most` is the largest one that it is good for
-      float o[MT][4], eight[N][4], zs[N][2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, down = 1.f, most = 0.f;
+      // `down` takes weights times scales to 16 bits, of a column each; scales up to `lim` are within it, weights up to 2^8 taken into account.  `weighed`:
+      // exponent of the largest scale with a weight to speak of
+      float o[MT][4], eight[N][4], zs[N][2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, down[2] = {0x1p100f, 0x1p100f}, lim = 0.f;
+      int weighed[2] = {-200, -200}, credit[2] = {0, 0};
 #pragma unroll
       for (int i = 0; i < MT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 #pragma unroll
@@ -616,34 +623,63 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
             }
           }
         }
-        float top[2] = {s[0][0], s[0][1]}, wide = fmaxf(fmaxf(f[0].largest(), f[1].largest()), fmaxf(f[2].largest(), f[3].largest()));
+        const float large[4] = {f[0].largest(), f[1].largest(), f[2].largest(), f[3].largest()};
+        float top[2] = {s[0][0], s[0][1]}, wide = fmaxf(fmaxf(large[0], large[1]), fmaxf(large[2], large[3]));
 #pragma unroll
         for (int i = 2; i < 8; ++i) top[i & 1] = fmaxf(top[i & 1], s[i >> 2][i & 3]);
-        if (__any_sync(0xffffffffu, top[0] * by[0] > m[0] + 8.f || top[1] * by[1] > m[1] + 8.f || wide > most)) {
+        if (__builtin_expect(__any_sync(0xffffffffu, top[0] * by[0] > m[0] + 8.f || top[1] * by[1] > m[1] + 8.f || wide > lim), 0)) {
+          float narrow = INFINITY;  // the smallest scale that is not zero
+#pragma unroll
+          for (int i = 0; i < 4; ++i) narrow = large[i] > 0.f ? fminf(narrow, large[i]) : narrow;
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) {
             top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], d));
             top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], d));
             wide = fmaxf(wide, __shfl_xor_sync(0xffffffffu, wide, d));
+            narrow = fminf(narrow, __shfl_xor_sync(0xffffffffu, narrow, d));
           }
-          float a[2], more = 1.f;
-          if (wide > most) {  // 2^k <= wide < 2^(k + 1): up to 2^(k + 1), at 2^7 then
-            const int k = max(-100, static_cast<int>(__float_as_uint(wide) >> 23) - 127);
-            const float to = __uint_as_float(static_cast<uint32_t>(127 + 6 - k) << 23);
-            more = most > 0.f ? to / down : 1.f;  // (nothing has been added up yet: zeros)
-            down = to;
-            most = __uint_as_float(static_cast<uint32_t>(128 + k) << 23);
-          }
+          float grown[2], a[2], mine[2] = {wide, wide};
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             top[k] *= by[k];
-            a[k] = top[k] > m[k] ? ptx::ex2_approx(m[k] - top[k]) : 1.f;
+            grown[k] = top[k] > m[k] ? top[k] - m[k] : 0.f;
             m[k] = fmaxf(m[k], top[k]);
+            a[k] = ptx::ex2_approx(-grown[k]);
             l[k] *= a[k];
 #pragma unroll
             for (int i = 0; i < N; ++i) zs[i][k] *= a[k];
-            a[k] *= more;
           }
+          // scales of very different sizes, or none with a weight to speak of: the largest one that has one (below 2^-16 counted as if with it)
+          if (__builtin_expect(__any_sync(0xffffffffu, wide > 16.f * narrow || top[0] < m[0] - 16.f || top[1] < m[1] - 16.f), 0)) {
+            mine[0] = mine[1] = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              mine[i & 1] = fmaxf(mine[i & 1], large[i >> 1] * fminf(1.f, 65536.f * ptx::ex2_approx(fmaf(s[i >> 2][i & 3], by[i & 1], -m[i & 1]))));
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) {
+              mine[0] = fmaxf(mine[0], __shfl_xor_sync(0xffffffffu, mine[0], d));
+              mine[1] = fmaxf(mine[1], __shfl_xor_sync(0xffffffffu, mine[1], d));
+            }
+          }
+          int low = 126;
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            // (what was counted before has 2^-grown of its weight now; the first 24 of that, from 2^8 to 2^-16, leave it one to speak of)
+            credit[k] -= static_cast<int>(ceilf(fminf(grown[k], 500.f)));
+            weighed[k] += min(0, credit[k]);
+            credit[k] = max(0, credit[k]);
+            if (qd_exponent(mine[k]) >= weighed[k]) {
+              weighed[k] = qd_exponent(mine[k]);
+              credit[k] = 24;
+            }
+            // scales below 2^e are at 2^7 then: all that count, and others up to 2^12 times as large (no other chunk comes here for those)
+            const int was = 7 - qd_exponent(down[k]);
+            const int e = min(126, max(-93, max(weighed[k] + 1, min(max(qd_exponent(wide) + 1, was), weighed[k] + 13))));
+            a[k] = ptx::ex2_approx(static_cast<float>(was - e) - grown[k]);
+            down[k] = qd_power(7 - e);
+            low = min(low, e);
+          }
+          lim = qd_power(low);
 #pragma unroll
           for (int i = 0; i < MT; ++i) {
             o[i][0] *= a[0]; o[i][1] *= a[1]; o[i][2] *= a[0]; o[i][3] *= a[1];
@@ -671,17 +707,16 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
           }
           uint32_t b0[N], b1[N];
           if constexpr (N == 1) {
-            const float sa = fa.s[0] * down, sb = fb.s[0] * down;
             zs[0][0] = fmaf(s[u][0], fa.mid[0], fmaf(s[u][2], fb.mid[0], zs[0][0]));
             zs[0][1] = fmaf(s[u][1], fa.mid[0], fmaf(s[u][3], fb.mid[0], zs[0][1]));
-            b0[0] = qd_transposed(pk2<__half>(s[u][0] * sa, s[u][1] * sa));
-            b1[0] = qd_transposed(pk2<__half>(s[u][2] * sb, s[u][3] * sb));
+            b0[0] = qd_transposed(pk2<__half>(s[u][0] * (fa.s[0] * down[0]), s[u][1] * (fa.s[0] * down[1])));
+            b1[0] = qd_transposed(pk2<__half>(s[u][2] * (fb.s[0] * down[0]), s[u][3] * (fb.s[0] * down[1])));
           } else {  // two groups an instruction
-            const uint64_t down2 = ptx::f32x2(down, down);
+            const uint64_t down0 = ptx::f32x2(down[0], down[0]), down1 = ptx::f32x2(down[1], down[1]);
             const uint64_t w0 = ptx::f32x2(s[u][0], s[u][0]), w1 = ptx::f32x2(s[u][1], s[u][1]), w2 = ptx::f32x2(s[u][2], s[u][2]), w3 = ptx::f32x2(s[u][3], s[u][3]);
 #pragma unroll
             for (int i = 0; i < N; i += 2) {
-              const uint64_t sa = ptx::mul_f32x2(ptx::f32x2(fa.s[i], fa.s[(i + 1) % N]), down2), sb = ptx::mul_f32x2(ptx::f32x2(fb.s[i], fb.s[(i + 1) % N]), down2);
+              const uint64_t sa = ptx::f32x2(fa.s[i], fa.s[(i + 1) % N]), sb = ptx::f32x2(fb.s[i], fb.s[(i + 1) % N]);
               const uint64_t ma = ptx::f32x2(fa.mid[i], fa.mid[(i + 1) % N]), mb = ptx::f32x2(fb.mid[i], fb.mid[(i + 1) % N]);
 #pragma unroll
               for (int k = 0; k < 2; ++k) {
@@ -689,8 +724,8 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
                 zs[i][k] = z.x;
                 zs[(i + 1) % N][k] = z.y;
               }
-              const float2 p0 = ptx::f32x2_get(ptx::mul_f32x2(w0, sa)), p1 = ptx::f32x2_get(ptx::mul_f32x2(w1, sa));
-              const float2 p2 = ptx::f32x2_get(ptx::mul_f32x2(w2, sb)), p3 = ptx::f32x2_get(ptx::mul_f32x2(w3, sb));
+              const float2 p0 = ptx::f32x2_get(ptx::mul_f32x2(w0, ptx::mul_f32x2(sa, down0))), p1 = ptx::f32x2_get(ptx::mul_f32x2(w1, ptx::mul_f32x2(sa, down1)));
+              const float2 p2 = ptx::f32x2_get(ptx::mul_f32x2(w2, ptx::mul_f32x2(sb, down0))), p3 = ptx::f32x2_get(ptx::mul_f32x2(w3, ptx::mul_f32x2(sb, down1)));
               b0[i] = qd_transposed(pk2<__half>(p0.x, p1.x));
               b1[i] = qd_transposed(pk2<__half>(p2.x, p3.x));
               b0[(i + 1) % N] = qd_transposed(pk2<__half>(p0.y, p1.y));
@@ -725,12 +760,12 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
           for (int i = 0; i < N; ++i) zs[i][k] += __shfl_xor_sync(0xffffffffu, zs[i][k], d);
         }
       }
-      const float up = 1.f / down;
+      const float up[2] = {1.f / down[0], 1.f / down[1]};
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         const int j = (i * 16 / GROUP) % N;
-        o[i][0] = fmaf((o[i][0] + eight[j][0]) * 0x1p24f, up, zs[j][0]); o[i][1] = fmaf((o[i][1] + eight[j][1]) * 0x1p24f, up, zs[j][1]);
-        o[i][2] = fmaf((o[i][2] + eight[j][2]) * 0x1p20f, up, zs[j][0]); o[i][3] = fmaf((o[i][3] + eight[j][3]) * 0x1p20f, up, zs[j][1]);
+        o[i][0] = fmaf((o[i][0] + eight[j][0]) * 0x1p24f, up[0], zs[j][0]); o[i][1] = fmaf((o[i][1] + eight[j][1]) * 0x1p24f, up[1], zs[j][1]);
+        o[i][2] = fmaf((o[i][2] + eight[j][2]) * 0x1p20f, up[0], zs[j][0]); o[i][3] = fmaf((o[i][3] + eight[j][3]) * 0x1p20f, up[1], zs[j][1]);
       }
       const QdRanges mine = qd_ranges(rec + 10);
       const unsigned X0 = mine.x0, X1 = mine.x0 + mine.n, x0 = mine.begin(warp), x1 = mine.begin(warp + 1);
