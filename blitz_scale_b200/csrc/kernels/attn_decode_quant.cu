@@ -542,9 +542,9 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
       }
 
       // `down` takes weights times scales to 16 bits, of a column each; scales up to `lim` are within it, weights up to 2^8 taken into account.  `weighed`:
-      // exponent of the largest scale with a weight to speak of
+      // exponent of the largest scale with a weight to speak of, and (times 32) how many times that weight may still be halved
       float o[MT][4], eight[N][4], zs[N][2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, down[2] = {0x1p100f, 0x1p100f}, lim = 0.f;
-      int weighed[2] = {-200, -200}, credit[2] = {0, 0};
+      int weighed[2] = {-200 * 32, -200 * 32};
 #pragma unroll
       for (int i = 0; i < MT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 #pragma unroll
@@ -665,16 +665,11 @@ __global__ void __launch_bounds__(kQdThreads, 1) attn_decode_quant_kernel(const 
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             // (what was counted before has 2^-grown of its weight now; the first 24 of that, from 2^8 to 2^-16, leave it one to speak of)
-            credit[k] -= static_cast<int>(ceilf(fminf(grown[k], 500.f)));
-            weighed[k] += min(0, credit[k]);
-            credit[k] = max(0, credit[k]);
-            if (qd_exponent(mine[k]) >= weighed[k]) {
-              weighed[k] = qd_exponent(mine[k]);
-              credit[k] = 24;
-            }
+            const int credit = (weighed[k] & 31) - static_cast<int>(ceilf(fminf(grown[k], 500.f))), old = (weighed[k] >> 5) + min(0, credit), now = max(old, qd_exponent(mine[k]));
+            weighed[k] = now * 32 + (qd_exponent(mine[k]) >= old ? 24 : max(0, credit));
             // scales below 2^e are at 2^7 then: all that count, and others up to 2^12 times as large (no other chunk comes here for those)
             const int was = 7 - qd_exponent(down[k]);
-            const int e = min(126, max(-93, max(weighed[k] + 1, min(max(qd_exponent(wide) + 1, was), weighed[k] + 13))));
+            const int e = min(126, max(-93, max(now + 1, min(max(qd_exponent(wide) + 1, was), now + 13))));
             a[k] = ptx::ex2_approx(static_cast<float>(was - e) - grown[k]);
             down[k] = qd_power(7 - e);
             low = min(low, e);
