@@ -559,7 +559,8 @@ __device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t a, uin
 // Bound by the 16-bit rows that it writes (four times the codes): 1024 pages of 64 tokens of 8 heads of 128 63 us (352 MB, 5.6 TB/s), 37 pages of 4 heads
 // of 64 3.4 us; for attention of portions 8200 tokens 15 us after their largest magnitudes are known.
 //
-// For attention of portions (WORK) the tokens behind a sequence's end are zeros, whatever the cache has there.  SCALED: keys and values of a bf16
+// For attention of portions (WORK) the tokens behind a sequence's end are zeros, whatever the cache has there, and a value that is no number is handed to
+// those who see it by its token's key (products with values have a weight of zero for those who do not, which would not make it a number).  SCALED: keys and values of a bf16
 // model go to fp16, divided by powers of two, or stay in bf16, as quant_kv_form says for their sequence and head.
 template <typename T, int D, int GROUP, bool WORK, bool SCALED>
 __global__ void __launch_bounds__(256, 3) quant_kv_pages_kernel(const QuantPagesParams p) {
@@ -649,6 +650,16 @@ __global__ void __launch_bounds__(256, 3) quant_kv_pages_kernel(const QuantPages
 #pragma unroll
       for (int j = 0; j < 4; ++j) past |= quant_kv_past(number(vs[j], i), number(vs[j], G + i), most);
     }
+    // (WORK: tokens with a value that is no number)
+    auto no_number = [&](const uint32_t (&w)[G], int i) { return !(fabsf(number(w, G + i)) < INFINITY); };
+    uint32_t none = 0;
+    if (WORK) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < G; ++i) none |= no_number(vs[j], i) ? 1u << (4 * t4 + j) : 0u;
+      none = __reduce_or_sync(0xffffffffu, none);
+    }
     auto two = [&](float a, float b) { return !SCALED || form.fp16 ? pk2<T>(a, b) : pk2<__nv_bfloat16>(a, b); };
     auto out = [&](void* to, int row_bytes) {
       T* const d = reinterpret_cast<T*>(to) + row0 * pitch + static_cast<int64_t>(head) * D;
@@ -667,6 +678,7 @@ __global__ void __launch_bounds__(256, 3) quant_kv_pages_kernel(const QuantPages
         float sc = number(ks[r], w * 32 / GROUP), z = number(ks[r], G + w * 32 / GROUP);
         if (SCALED) sc *= form.k_down, z *= form.k_down;
         if (WORK) sc *= p.k_sign, z *= p.k_sign;
+        if (WORK && ((none >> (g + 8 * r)) & 1u)) z = NAN;
         if (WORK && g + 8 * r >= held) sc = z = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = fmaf(sc, x[i], z);
@@ -688,7 +700,7 @@ __global__ void __launch_bounds__(256, 3) quant_kv_pages_kernel(const QuantPages
         const int tok = (j & 2) + (j >> 2);
         float sc = number(vs[tok], i), z = number(vs[tok], G + i);
         if (SCALED) sc *= form.v_down, z *= form.v_down;
-        if (WORK && 4 * t4 + tok >= held) sc = z = 0.f;
+        if (WORK && (4 * t4 + tok >= held || no_number(vs[tok], i))) sc = z = 0.f;
         x[j] = fmaf(sc, x[j], z);
       }
       if (past) {

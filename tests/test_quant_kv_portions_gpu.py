@@ -253,3 +253,31 @@ def test_an_engine_reserves_what_portions_take(ops, monkeypatch):
         assert eng.runner._ws["portion"] is reserved
         outs.append(torch.cat(got))
     assert torch.equal(*outs)
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", range(len(SHAPES)))
+@pytest.mark.parametrize("what", ["k", "v", "both"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_what_is_no_number_reaches_rows_that_see_it(ops, dt, shape, what, bad):
+    """Rows before a token with such a key or value, rows whose window leaves it out, other heads and other sequences are bit for bit what they are without it."""
+    seqs, Q, H, D, group, page, lead, opts = SHAPES[shape]
+    kv = [(k.to(dt), v.to(dt)) for k, v in _kv([a + b for a, b in seqs], H, D, 50 * shape + 3)]
+    q = torch.randn(sum(b for _, b in seqs), Q, D, generator=torch.Generator().manual_seed(shape)).to(dt)
+    want = Pass(ops, seqs, kv, q, group, page, lead, **opts).run()
+    first, n = seqs[1]
+    at, rep = first + n // 2, Q // H
+    k, v = (x.clone() for x in kv[1])
+    if what != "v":
+        k[at, 1, 3] = bad
+    if what != "k":
+        v[at, 1, D - 1] = bad
+    p = Pass(ops, seqs, [kv[0], (k, v), kv[2]], q, group, page, lead, **opts)
+    got = p.run()
+    window = opts.get("window") or 1 << 30
+    sees = torch.zeros(got.shape[:2], dtype=torch.bool)
+    rows_at = torch.arange(first, first + n)
+    sees[p.of(1), rep:2 * rep] = ((rows_at >= at) & (rows_at < at + window))[:, None]
+    assert torch.equal(got[~sees], want[~sees])
+    last = got[sees][:, D - group:]             # (the group that holds the value; a key reaches all)
+    assert last.isnan().all() and sees.any()
