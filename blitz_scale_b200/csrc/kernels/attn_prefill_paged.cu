@@ -92,6 +92,7 @@ struct PagedPrefillParams {
   int bias_len;
   const float2* forms;        // PART: [entries][kv_heads] powers of two taken out of keys and values, zeros where those are in bf16
   const int* some_bf16;       // PART: whether any are
+  float least_up;             // IO: what makes the factor of scores 2^-126
   int* status;
   long long* trace;  // profiling aid (null in production): clock stamps of CTA 0's first item, see the set_trace call
 };
@@ -421,7 +422,7 @@ attn_prefill_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
           break;
         }
         row_up = quant_kv_row_fp16<C::kSlabs>(sQ + t * TB + r_ * 128, SB, r_ & 7) * it.k_up;
-        row_up = fmaxf(row_up, 0x1p-126f / p.scale_log2);  // (a factor of zero would make numbers that are none of what is hidden)
+        row_up = fmaxf(row_up, p.least_up);  // (a factor of zero would make numbers that are none of what is hidden)
         ptx::fence_proxy_async_smem();
         ptx::mbar_arrive(&q_fp16[t]);
       }
@@ -758,7 +759,7 @@ static int prefill_paged(const void* q, int64_t q_stride, const void* k_pool, co
   p.q_heads = q_heads; p.kv_heads = kv_heads; p.page_size = page_size; p.box_tokens = bt;
   p.oob_row = (int)rows;
   p.scale_log2 = sm_scale * 1.4426950408889634f; p.status = status; p.trace = g_pp_trace;
-  p.chunked = chunked; p.forms = forms; p.some_bf16 = some_bf16;
+  p.chunked = chunked; p.forms = forms; p.some_bf16 = some_bf16; p.least_up = 0x1p-126f / p.scale_log2;
   p.window = window; p.keep_first = keep_first; p.sink = sink; p.bias = bias; p.bias_len = bias_len;
   p.cap_scale = softcap > 0.f ? sm_scale / softcap : 0.f; p.cap_log2 = softcap * 1.4426950408889634f;
   // tanh(z) = z (k0 + k1 z^2 + k2 z^4 + k3 z^6) for |z| <= 0.5 (Chebyshev interpolation of tanh(z) / z in z^2, absolute
