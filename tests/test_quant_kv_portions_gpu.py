@@ -281,3 +281,39 @@ def test_what_is_no_number_reaches_rows_that_see_it(ops, dt, shape, what, bad):
     assert torch.equal(got[~sees], want[~sees])
     last = got[sees][:, D - group:]             # (the group that holds the value; a key reaches all)
     assert last.isnan().all() and sees.any()
+
+
+@pytest.mark.parametrize("own_room", [False, True])
+def test_captured_and_replayed(ops, own_room):
+    """Two passes in a graph, one after the other in the same scratch, with other numbers at each replay: some held in fp16, some in bf16."""
+    shapes, passes = [SHAPES[0], SHAPES[1]], []
+    for i, (seqs, Q, H, D, group, page, lead, opts) in enumerate(shapes):
+        kv = _kv([a + b for a, b in seqs], H, D, 90 + i)
+        q = torch.randn(sum(b for _, b in seqs), Q, D, generator=torch.Generator().manual_seed(i)).to(torch.bfloat16)
+        passes.append((Pass(ops, seqs, kv, q, group, page, 0, **opts), kv))
+    room = torch.empty(1 << 24, dtype=torch.uint8, device=DEV) if own_room else None
+    calls = []
+    for p, _ in passes:
+        args = (p.q.flatten(1).to(DEV), p.cache, p.table.to(torch.int32).to(DEV), ops.prefill_work_list(p.rows, p.lens, p.page, DEV))
+        more = dict(q_heads=p.q.shape[1], kv_heads=p.H, head_dim=p.D, page_size=p.page, workspace=room, **p.opts)
+        calls.append(lambda out, args=args, more=more: ops.attn_prefill_paged(*args, out=out, **more))
+    outs = [torch.zeros(p.q.shape[0], p.q.shape[1] * p.D, dtype=torch.bfloat16, device=DEV) for p, _ in passes]
+    for call, out in zip(calls, outs):
+        call(out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for call, out in zip(calls, outs):
+            call(out)
+    for by in (0, 25, 3, 40):
+        for p, kv in passes:            # a key and a value of the first sequence grow
+            k, v = (x[:1].clone() for x in kv[0])
+            k[0, 0, 1], v[0, 0, 2] = 2.0 ** min(by, 20), -(2.0 ** by)
+            slot = (p.table[:1] * p.page).to(torch.int32).to(DEV)
+            ops.quant_kv_store(k.flatten(1).to(DEV), v.flatten(1).to(DEV), slot, p.cache)
+        graph.replay()
+        got = [o.clone() for o in outs]
+        for call, out, g in zip(calls, outs, got):
+            out.fill_(7.0)
+            call(out)
+            assert torch.equal(out, g) and g.isfinite().all(), by
