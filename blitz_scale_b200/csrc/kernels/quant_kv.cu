@@ -476,8 +476,8 @@ struct QuantPagesParams {
   void *k, *v;       // page n's token `off` at row n * page_rows + off
   int64_t units;     // (page, 16 tokens of it, head) each
   int kv_heads, page_size, page_rows, max_pages;
-  int pool_heads, head0;  // heads of the pool, and the first of the kv_heads that are read
   int* status;
+  int pool_heads, head0;  // for attention of portions: heads of the pool, and the first of the kv_heads that are read
   // for attention of portions: records of the pass (see attn_prefill_paged.cu), whose page numbers count from `first` pages before the first one
   const int32_t* work;
   int entries, first, pages_read;
@@ -589,7 +589,7 @@ __global__ void __launch_bounds__(256, 3) quant_kv_pages_kernel(const QuantPages
     const int64_t n = unit / p.kv_heads / blocks;
     const int page = p.pages[n];
     const bool bad = page < 0 || page >= p.max_pages;  // (the first page is read instead, and nothing written)
-    const uint8_t* block = p.pool + ((static_cast<int64_t>(bad ? 0 : page) * p.pool_heads + p.head0 + head) * blocks + b) * F.block;
+    const uint8_t* block = p.pool + ((static_cast<int64_t>(bad ? 0 : page) * (WORK ? p.pool_heads : p.kv_heads) + (WORK ? p.head0 : 0) + head) * blocks + b) * F.block;
     const int64_t row0 = n * p.page_rows + b * 16, pitch = static_cast<int64_t>(p.kv_heads) * D;
     // everything is asked for before anything is used
     uint32_t kw[2][W], vw[D / 16];
@@ -825,7 +825,7 @@ int blitz_quant_kv_pages(const void* pool, const int32_t* pages, int64_t count, 
   if (count <= 0) return 0;
   if (!quant_kv_supported(dim, group, page_size) || max_pages < 1 || kv_heads < 1 || page_rows < page_size) return -1;
   if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(pool)) & 15) return -1;
-  QuantPagesParams p{(const uint8_t*)pool, pages, k, v, count * kv_heads * (page_size / 16), kv_heads, page_size, page_rows, max_pages, kv_heads, 0, status};
+  QuantPagesParams p{(const uint8_t*)pool, pages, k, v, count * kv_heads * (page_size / 16), kv_heads, page_size, page_rows, max_pages, status};
   return quant_kv_dispatch(dtype, dim, group, PagesLaunch{p, stream});
 }
 
@@ -858,7 +858,7 @@ int blitz_quant_kv_portion(const void* pool, const int32_t* pages, int64_t count
   int64_t at[5];
   blitz_quant_kv_portion_bytes(count, first, entries, kv_heads, dim, page_size, dtype, at);
   char* s = (char*)scratch;
-  QuantPagesParams p{(const uint8_t*)pool, pages, s, s + (int64_t)page_size * kv_heads * dim * 2, count * kv_heads * (page_size / 16), kv_heads, page_size, 2 * page_size, max_pages, pool_heads, head0, status};
+  QuantPagesParams p{(const uint8_t*)pool, pages, s, s + (int64_t)page_size * kv_heads * dim * 2, count * kv_heads * (page_size / 16), kv_heads, page_size, 2 * page_size, max_pages, status, pool_heads, head0};
   p.work = work; p.entries = entries; p.first = (int)first; p.table = (int32_t*)(s + at[1]); p.spans = (uint4*)(s + at[2]);
   p.pages_read = (int)count; p.k_sign = k_sign; p.forms = (float2*)(s + at[3]);
   return quant_kv_dispatch(dtype, dim, group, PortionLaunch{p, stream});
