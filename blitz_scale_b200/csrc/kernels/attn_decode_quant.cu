@@ -25,8 +25,9 @@
 // halves of the groups (HALVES): lanes of columns 0..3 handle the scales of the first half of the groups, the others those of the second.
 //
 // A warp takes chunks of 32 tokens by itself, through a ring of stages of its own; one more warp issues the copies (bulk copies: a
-// head's tokens in a page are one contiguous piece), a lane for each of the others.  Eleven warps have 168 registers each and none
-// spills; fifteen with 128 took 43.4 us where these took 40.3 (256 sequences of 512 tokens, 32 query heads over 8 of 128, groups of 32).
+// head's tokens in a page are one contiguous piece), a lane for each of the others.  Eleven warps have 168 registers each, which is enough but for
+// five to eight query heads over a KV head of 128 in groups of 32 (12 bytes spilled); fifteen with 128 took 43.4 us where these took 40.3 (256 sequences of 512
+// tokens, 32 query heads over 8 of 128, groups of 32).
 //
 // The chunks of all sequences of all heads, end to end, are cut into equal ranges, one per warp of the GPU, so that neither lengths nor the
 // number of sequences leave warps idle.  A sequence that is cut leaves its pieces' sums in shared memory, where the warps that end with it
@@ -35,9 +36,9 @@
 // whoever is last.  Where there are no more sequences of heads than blocks, and the longest costs less beside an equal share than
 // that hand-over (2.5 us), a block takes one of them whole.
 //
-// Measured, bf16, 32 query heads over 8 of 128: 256 sequences of 512 tokens in groups of 32 39.7 us (172 MB, 4.3 TB/s; the 16-bit kernel
-// 98 us); one of 100003 in groups of 128 29.0 us (3.75 TB/s); 61 of 1100 on average in groups of 64 23.7 us (fp16); one of 977 9.2 us.  Bound by the stream where
-// it is long (5.7 TB/s beside the ends; the warps issue in half of the cycles); 9 to 10 us of every call are its ends: tables, first
+// Measured, bf16, 32 query heads over 8 of 128: 256 sequences of 512 tokens in groups of 32 41.3 us (172 MB, 4.2 TB/s; the 16-bit kernel
+// 98 us); one of 100003 in groups of 128 29.8 us (3.65 TB/s); 61 of 1100 on average in groups of 64 24.7 us (fp16); one of 977 9.7 us.  Bound by the stream where
+// it is long (5.6 TB/s beside the ends; the warps issue in half of the cycles); 9 to 11 us of every call are its ends: tables, first
 // pages, and pieces added up.
 #include "launch.cuh"
 #include "ptx.cuh"

@@ -53,10 +53,10 @@
 // Operands in fp16 for a bf16 model (IO: the type of queries, sink and output): keys and values were divided by powers of two (of a sequence and KV
 // head) so that fp16 holds them, and each thread turns its row of queries into fp16 in shared memory, divided by a power of two near the row's
 // largest entry, as an item begins.  The row's scale and the output's factor make up for both.  A 4-bit cache read back for a pass
-// comes so (quant_kv.cu).  8192 rows of nine prompts, 32 heads of 128: 187 us where a bf16 cache takes 174 (what an item waits for at its start, and
+// comes so (quant_kv.cu).  8192 rows of nine prompts, 32 heads of 128: 190 us where a bf16 cache takes 174 (what an item waits for at its start, and
 // registers); with queries converted by a pass before it 184 us behind 20 us of that.
 // PART: such a cache is in fp16 for most sequences and heads and in bf16 for those that fp16 does not hold; a launch with operands of either type takes
-// the items whose keys and values are of that type.
+// the items whose keys and values are of that type (4 us where there are none in bf16).
 //
 // Replaces FlashInfer's BatchPrefillWithRaggedKVCacheWrapper / paged wrapper calls and their host Plan()
 // (src/kernel/attention_prefill.cu:11-45, src/kernel/flashinfer_types.cu:24-49).
