@@ -77,3 +77,20 @@ def test_single_tokens_over_the_largest_number_of_bf16(ops, sign):
     assert held.isfinite().all() and got.isfinite().all()
     # (a row of one token is that token: rounded once, by weights of one)
     assert ((got.double() - held.double()).abs() <= 2.0 ** -7 * most).all()
+
+
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("n", [1, 50])
+def test_portions_over_the_largest_number_of_bf16(ops, sign, n):
+    """Rows whose own value has all of the weight: the largest number stays one."""
+    H, D, group, page, most = 2, 64, 32, 64, torch.finfo(torch.bfloat16).max
+    v = torch.full((n, H * D), most * sign, dtype=torch.bfloat16)
+    v[:, ::group] = 0.0
+    k = torch.zeros(n, H, D, dtype=torch.bfloat16)
+    k[torch.arange(n), :, torch.arange(n)] = 64.0          # (keys at right angles, queries 64 times their own: every other weight is zero in fp32)
+    cache, t = ops.quant_kv_pool(1, page, H, D, group), lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    ops.quant_kv_store(k.flatten(1).to(DEV), v.to(DEV), t(list(range(n))), cache)
+    got = ops.attn_prefill_paged((64 * k).flatten(1).to(DEV), cache, t([0]), ops.prefill_work_list([n], [n], page, DEV), q_heads=H, kv_heads=H, head_dim=D,
+                                 page_size=page).cpu()
+    held = ops.quant_kv_load(cache, t(list(range(n))))[1].cpu().flatten(1)
+    assert held.isfinite().all() and torch.equal(got, held)
