@@ -317,3 +317,23 @@ def test_captured_and_replayed(ops, own_room):
             out.fill_(7.0)
             call(out)
             assert torch.equal(out, g) and g.isfinite().all(), by
+
+
+@pytest.mark.parametrize("H,rep,D,group,page", [(130, 1, 64, 64, 16), (1, 40, 128, 128, 1024)])
+def test_many_heads_and_large_pages(ops, H, rep, D, group, page):
+    seqs = [(0, 37), (700, 5)]
+    kv = _kv([a + b for a, b in seqs], H, D, 60)
+    q = torch.randn(42, H * rep, D, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    p = Pass(ops, seqs, kv, q, group, page)
+    got = p.run()
+    for s, (a, b) in enumerate(seqs):
+        kept = [quantised(x, group) for x in kv[s]]
+        (kc, ks, kz), (vc, vs, vz) = kept
+        kept = (values(kc, ks, kz, group), values(vc, vs, vz, group), ks, kz, vs)
+        x, half = q[p.of(s)], 2.0 ** -11
+        want = attention(x, kept[0], kept[1], torch.arange(a, a + b), scale=D ** -0.5)
+        tol = tolerance(x, kept, D ** -0.5, want, want[1], half, torch.bfloat16, group, value_step=half)
+        # (as in test_portions: below 2^-14 of the largest of the head, in steps of 2^-24)
+        floor = 2.0 ** -24 * kept[0].abs().amax() * x.double().abs().sum(-1) * D ** -0.5
+        tol = tol + torch.expm1(2 * floor)[..., None] * want[1] + 2.0 ** -24 * kept[1].abs().amax()
+        assert ((got[p.of(s)].double() - want[0]).abs() <= tol).all(), s
