@@ -422,7 +422,7 @@ def _exact_select(case, seed):
     for q in range(Q):
         z = state["logits"][q * k:q * k + k].double()
         v = (torch.log_softmax(z, 1) + state["scores"][q * k:q * k + k].double()[:, None]).flatten()
-        v = v.nan_to_num(nan=-math.inf)
+        v = v.nan_to_num(nan=-math.inf, neginf=-math.inf)
         least = torch.topk(v, min(n, v.numel())).values[-1]
         at = torch.nonzero(v >= least if least > -math.inf else v > -math.inf).flatten()
         got = sorted(zip((-v[at]).tolist(), at.tolist()))[:n]
