@@ -10,5 +10,6 @@ enum StatusCode : int {
   kStatusTimeoutFlag = 4,
   kStatusBadIndex = 5,
   kStatusTooLarge = 6,
+  kStatusNoPage = 7,
 };
 }  // namespace blitz

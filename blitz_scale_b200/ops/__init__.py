@@ -150,7 +150,7 @@ def check_status(device=None, reset: bool = True) -> int:
             for _, flags in _pair_ws.values():
                 flags.zero_()
         names = {1: "TMA producer wait timed out", 2: "MMA wait timed out", 3: "epilogue wait timed out",
-                 4: "flag wait timed out", 5: "index out of range", 6: "size beyond the supported maximum"}
+                 4: "flag wait timed out", 5: "index out of range", 6: "size beyond the supported maximum", 7: "no page left"}
         raise RuntimeError(f"kernel status {code}: {names.get(code, 'unknown')}")
     return code
 
@@ -1323,3 +1323,7 @@ def part_norm(x: torch.Tensor, w: torch.Tensor, parts: int, eps: float) -> torch
         rows = x[t:t + 65535]
         _check(lib().blitz_part_norm(_p(rows), x.stride(0), _p(w), eps, rows.shape[0], parts, width // parts, _dt3(x), _stream()), "blitz_part_norm")
     return x
+
+
+from .beams import (BeamFork, BeamStep, StepTables, attn_beams_workspace_bytes, attn_decode_beams, beam_fork, beam_select, copy_pages,  # noqa: E402,F401
+                    step_tables)
