@@ -1,6 +1,17 @@
 // Decode attention of beams: one query token per row, rows in groups (the beams of a request) whose first pages are the same.
 //
-// out = softmax(q K^T scale) V per head over the row's pages [page][K|V][token][kv_head][dim].
+// out = softmax(q K^T scale) V per head over the row's pages [page][K|V][token][kv_head][dim].  It is a stream over keys and values, so what counts is
+// that those of the common pages come from HBM once: their query rows (beams times the query heads of a KV head, up to 32) are two tiles of
+// 16 rows of one matrix product, mma.sync m16n8k16.  tcgen05 is not used on purpose: one SM streams 16 tokens of a head in the time of a thousand
+// such instructions, and rows are few.
+//
+// Work.  A segment is the common part of a group, or what a row has behind it.  Per KV head (and block of beams, where they are more than 32 rows) the
+// segments' steps of 16 tokens laid end to end are cut into equal ranges, and a warp takes one range of one head: neither long rows nor few of them leave
+// warps idle.  Neighbouring warps have the heads of the same tokens, which are neighbours in memory.  A range is as many pieces as it meets segments; a piece leaves its
+// sums in scratch (fp32), and a second kernel adds up a row's pieces, always in the same order.  Every block works out the ranges from the tables, so a
+// captured launch follows them.
+//
+// A warp is by itself: it copies its steps (cp.async, three ahead), and nothing in the loop waits for another warp.
 #include "launch.cuh"
 #include "ptx.cuh"
 #include "tmap.cuh"
@@ -10,6 +21,11 @@
 
 namespace blitz {
 
+constexpr int kBaWarps = 8, kBaThreads = 32 * kBaWarps;
+constexpr int kBaStep = 16;            // tokens
+constexpr int kBaRowsMost = 1024;      // rows of a launch
+constexpr int kBaTile = 32;            // query rows of a segment
+
 struct BeamAttnParams {
   const void* q;
   int64_t q_stride;
@@ -17,54 +33,452 @@ struct BeamAttnParams {
   const int32_t *indices, *indptr, *last_page_len, *shared;
   void* out;
   int64_t out_stride;
-  int rows, beams, q_heads, kv_heads, page, max_pages;
-  float scale, cap;
+  int rows, beams, groups;      // groups of beams
+  int q_heads, rep;             // query heads of a virtual head
+  int kv_div, kv_heads;         // virtual heads of a KV head
+  int per_block, blocks;        // beams of a block, blocks of a group
+  int heads;                    // virtual heads x blocks
+  int ranges_most;
+  int page_shift, max_pages;
+  float scale_log2, cap_scale, cap_log2;
   const void* sink;
+  int* line;                    // [blocks][groups + groups per_block] steps before a segment, [+ 1] all; [rows] lengths; [blocks groups] common pages
+  float *o_common, *o_own;      // partial sums
+  float2 *ml_common, *ml_own;   // maximum (log2 units) and sum of each
+  int static_table;
   int* status;
 };
 
-// A warp per row and query head.
+// Equal ranges of n steps.
+struct BaRanges {
+  int count, q, rem;
+  __device__ __forceinline__ BaRanges(int n, int most) {
+    count = max(1, min(most, n / 4));    // (64 tokens at least: a piece costs as much as one or two steps)
+    q = n / count;
+    rem = n - q * count;
+  }
+  __device__ __forceinline__ int begin(int r) const { return r * q + min(r, rem); }
+  __device__ __forceinline__ int of(int x) const { return x < rem * (q + 1) ? x / (q + 1) : rem + (x - rem * (q + 1)) / q; }
+};
+
+// Lengths, common pages and the line of segments, by all threads of a block; arrays in shared memory, or (write) in scratch too.
+__device__ __forceinline__ void ba_line(const BeamAttnParams& p, int* line, int* len, int* common, int* sums) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  for (int r = tid; r < p.rows; r += kBaThreads) {
+    const int pages = p.indptr[r + 1] - p.indptr[r];
+    len[r] = pages > 0 ? ((pages - 1) << p.page_shift) + p.last_page_len[r] : 0;
+  }
+  __syncthreads();
+  for (int i = tid; i < p.blocks * p.groups; i += kBaThreads) {
+    const int b = i / p.groups, g = i % p.groups;
+    int most = max(p.shared[g], 0);
+    bool any = false;
+    for (int j = b * p.per_block; j < min((b + 1) * p.per_block, p.beams); ++j) {
+      const int n = len[g * p.beams + j];
+      if (n > 0) {
+        any = true;
+        most = min(most, n >> p.page_shift);
+      }
+    }
+    common[i] = any ? most : 0;
+  }
+  __syncthreads();
+  const int per = p.groups * (1 + p.per_block), total = p.blocks * per;
+  const int each = (total + kBaThreads - 1) / kBaThreads, e0 = min(total, tid * each), e1 = min(total, e0 + each);
+  auto steps = [&](int e) {
+    const int b = e / per, i = e % per;
+    if (i < p.groups) return common[b * p.groups + i] << (p.page_shift - 4);
+    const int g = (i - p.groups) / p.per_block, j = b * p.per_block + (i - p.groups) % p.per_block;
+    const int n = j < p.beams ? len[g * p.beams + j] : 0;
+    return n > 0 ? (n - (common[b * p.groups + g] << p.page_shift) + kBaStep - 1) / kBaStep : 0;
+  };
+  int mine = 0;
+  for (int e = e0; e < e1; ++e) mine += steps(e);
+  int sum = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, sum, d);
+    if (lane >= d) sum += up;
+  }
+  if (lane == 31) sums[warp] = sum;
+  __syncthreads();
+  sum -= mine;
+  for (int w = 0; w < warp; ++w) sum += sums[w];
+  for (int e = e0; e < e1; ++e) {
+    line[e] = sum;
+    sum += steps(e);
+  }
+  if (e1 == total && e0 < total) line[total] = sum;
+  __syncthreads();
+}
+
+// A place on a warp's range: segment, and what of its row the steps are.
+struct BaPlace {
+  int seg, x;              // segment (of the block of beams), step on the line
+  int seg_beg, seg_end;    // its steps
+  int pages, tok0, len;    // first page in `indices`; token that its first step is; tokens of the row
+};
+
 template <typename T, int HD>
-__global__ void __launch_bounds__(128) attn_beams_kernel(const BeamAttnParams p) {
+__global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const BeamAttnParams p) {
+  constexpr int kRowBytes = HD * 2, kPieces = HD / 8;         // a token's key: 16-byte pieces
+  constexpr int kStage = 2 * kBaStep * kRowBytes;             // keys, then values
+  constexpr int kStages = HD == 128 ? 3 : 6;
+  extern __shared__ __align__(128) uint8_t ba_smem[];
+  __shared__ int sums[kBaWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per = p.groups * (1 + p.per_block);
+  int* line = reinterpret_cast<int*>(ba_smem + kBaWarps * kStages * kStage);
+  int* len = line + p.blocks * per + 1;
+  int* common = len + p.rows;
+  ptx::griddep_launch_dependents();
+  if (!p.static_table) ptx::griddep_wait();
+  ba_line(p, line, len, common, sums);
+  ptx::griddep_wait();
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i < p.blocks * per + 1 + p.rows + p.blocks * p.groups; i += kBaThreads) p.line[i] = line[i];
+
+  const int self = warp * gridDim.x + blockIdx.x;
+  const int hv = self % p.heads, range = self / p.heads;
+  const int block = hv % p.blocks, head = hv / p.blocks;       // head: virtual, of `rep` query heads
+  line += block * per;
+  common += block * p.groups;
+  const int base = line[0];
+  const BaRanges ranges(line[per] - base, p.ranges_most);
+  if (range >= ranges.count) return;
+  const int x_end = ranges.begin(range + 1);
+  const int64_t token_pitch = static_cast<int64_t>(p.kv_heads) * HD;
+  const T* kv = reinterpret_cast<const T*>(p.kv) + (head / p.kv_div) * HD;
+  const int page = 1 << p.page_shift;
+
+  auto enter = [&](BaPlace& a) {     // the segment that step a.x is in (a.seg: one at or before it)
+    while (line[a.seg + 1] - base <= a.x) ++a.seg;
+    a.seg_beg = line[a.seg] - base;
+    a.seg_end = min(line[a.seg + 1] - base, x_end);
+    int row, g;
+    if (a.seg < p.groups) {
+      g = a.seg;
+      row = g * p.beams + block * p.per_block;
+      while (len[row] == 0) ++row;                             // (a common part has a row with pages)
+      a.tok0 = 0;
+      a.len = common[g] << p.page_shift;
+    } else {
+      const int i = a.seg - p.groups;
+      g = i / p.per_block;
+      row = g * p.beams + block * p.per_block + i % p.per_block;
+      a.tok0 = common[g] << p.page_shift;
+      a.len = len[row];
+    }
+    a.pages = p.indptr[row];
+  };
+  BaPlace ld{}, at{};
+  ld.x = at.x = ranges.begin(range);
+  if (ld.x >= x_end) return;
+  {
+    int lo = 0, hi = per;      // line[lo] <= x < line[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (line[mid] - base <= ld.x) lo = mid;
+      else hi = mid;
+    }
+    ld.seg = at.seg = lo;
+  }
+  enter(ld);
+  enter(at);
+  const uint32_t ring = ptx::smem_u32(ba_smem) + warp * kStages * kStage;
+  int win = 0, win_base = -64;       // page ids: lane l holds entry win_base + l of the row's list
+  int ld_stage = 0;
+  auto load = [&]() {                // requests the next step
+    if (ld.x >= x_end) return;
+    if (ld.x >= ld.seg_end) {
+      enter(ld);
+      win_base = -64;
+    }
+    const int t0 = ld.tok0 + (ld.x - ld.seg_beg) * kBaStep, pg = t0 >> p.page_shift;
+    if (pg >= win_base + 32 || pg < win_base) {
+      win_base = pg;
+      const int last = (ld.len - 1) >> p.page_shift;
+      win = pg + lane <= last ? p.indices[ld.pages + pg + lane] : 0;
+      if (win < 0 || win >= p.max_pages) {
+        if (p.status) atomicCAS(p.status, 0, kStatusBadIndex);
+        win = 0;
+      }
+    }
+    const int id = __shfl_sync(0xffffffffu, win, pg - win_base);
+    const T* k = kv + ((static_cast<int64_t>(id) << (p.page_shift + 1)) + (t0 & (page - 1))) * token_pitch;
+    const T* v = k + page * token_pitch;
+    const uint32_t to = ring + ld_stage * kStage;
+    const int valid = ld.len - t0;
+#pragma unroll
+    for (int i = 0; i < kBaStep * kPieces / 32; ++i) {
+      const int n = i * 32 + lane, tok = n / kPieces, c = n % kPieces;
+      const uint32_t dst = to + tok * kRowBytes + (((c ^ tok) & 7) | (c & 8)) * 16, bytes = tok < valid ? 16u : 0u;
+      ptx::cp_async_16(dst, k + (tok < valid ? tok : 0) * token_pitch + c * 8, bytes);
+      ptx::cp_async_16(dst + kBaStep * kRowBytes, v + (tok < valid ? tok : 0) * token_pitch + c * 8, bytes);
+    }
+    ++ld.x;
+    if (++ld_stage == kStages) ld_stage = 0;
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) {
+    load();
+    ptx::cp_async_commit();
+  }
+  const int g8 = lane >> 2, t4 = lane & 3, mi = lane >> 3, mr = lane & 7;
+  int stage = 0;
+  // A piece: TILES of 16 query rows.
+  auto piece = [&](auto tiles) {
+    constexpr int TILES = decltype(tiles)::value;
+    const bool shared_part = at.seg < p.groups;
+    const int i0 = at.seg - p.groups;
+    const int row0 = shared_part ? at.seg * p.beams + block * p.per_block : i0 / p.per_block * p.beams + block * p.per_block + i0 % p.per_block;
+    const int live = shared_part ? min(p.per_block, p.beams - block * p.per_block) * p.rep : p.rep;       // query rows
+    uint32_t qa[TILES][HD / 16][4];
+#pragma unroll
+    for (int t = 0; t < TILES; ++t)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int i = t * 16 + half * 8 + g8, r = i / p.rep;
+        const T* q = reinterpret_cast<const T*>(p.q) + (row0 + r) * p.q_stride + (head * p.rep + i - r * p.rep) * HD;
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ++ks)
+#pragma unroll
+          for (int hi = 0; hi < 2; ++hi)
+            qa[t][ks][half + 2 * hi] = i < live ? *reinterpret_cast<const uint32_t*>(q + ks * 16 + hi * 8 + 2 * t4) : 0u;
+      }
+    float o[TILES][HD / 8][4], m[TILES][2], l[TILES][2];
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+      m[t][0] = m[t][1] = -INFINITY;
+      l[t][0] = l[t][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < HD / 8; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.f;
+    }
+    for (; at.x < at.seg_end; ++at.x) {
+      load();
+      ptx::cp_async_commit();
+      ptx::cp_async_wait<kStages - 1>();
+      __syncwarp();
+      const uint32_t kbase = ring + stage * kStage, vbase = kbase + kBaStep * kRowBytes;
+      float s[TILES][2][4] = {};
+      {
+        const int tok = (mi >> 1) * 8 + mr;
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ++ks) {
+          const int c = ks * 2 + (mi & 1);
+          uint32_t b0, b1, b2, b3;
+          ldmatrix_x4(kbase + tok * kRowBytes + (((c ^ tok) & 7) | (c & 8)) * 16, b0, b1, b2, b3);
+#pragma unroll
+          for (int t = 0; t < TILES; ++t) {
+            mma16816<T>(s[t][0], qa[t][ks][0], qa[t][ks][1], qa[t][ks][2], qa[t][ks][3], b0, b1);
+            mma16816<T>(s[t][1], qa[t][ks][0], qa[t][ks][1], qa[t][ks][2], qa[t][ks][3], b2, b3);
+          }
+        }
+      }
+      const int valid = at.len - (at.tok0 + (at.x - at.seg_beg) * kBaStep);
+      uint32_t pa[TILES][4];
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) {
+        float top[2] = {m[t][0], m[t][1]};
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float& x = s[t][h][e];
+            x = p.cap_log2 > 0.f ? p.cap_log2 * ptx::tanh_ex2(x * p.cap_scale) : x * p.scale_log2;
+            if (h * 8 + 2 * t4 + (e & 1) >= valid) x = -INFINITY;
+            top[e >> 1] = fmaxf(top[e >> 1], x);
+          }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 1));
+          top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 2));
+        }
+        if (__any_sync(0xffffffffu, top[0] > m[t][0] || top[1] > m[t][1])) {
+          const float a0 = ptx::ex2_approx(m[t][0] - top[0]), a1 = ptx::ex2_approx(m[t][1] - top[1]);
+          l[t][0] *= a0;
+          l[t][1] *= a1;
+#pragma unroll
+          for (int i = 0; i < HD / 8; ++i) {
+            o[t][i][0] *= a0;
+            o[t][i][1] *= a0;
+            o[t][i][2] *= a1;
+            o[t][i][3] *= a1;
+          }
+          m[t][0] = top[0];
+          m[t][1] = top[1];
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s[t][h][e] = ptx::ex2_approx(s[t][h][e] - m[t][e >> 1]);
+            l[t][e >> 1] += s[t][h][e];
+          }
+        pa[t][0] = pk2<T>(s[t][0][0], s[t][0][1]);
+        pa[t][1] = pk2<T>(s[t][0][2], s[t][0][3]);
+        pa[t][2] = pk2<T>(s[t][1][0], s[t][1][1]);
+        pa[t][3] = pk2<T>(s[t][1][2], s[t][1][3]);
+      }
+      {
+        const int tok = (mi & 1) * 8 + mr;
+#pragma unroll
+        for (int np = 0; np < HD / 16; ++np) {
+          const int c = np * 2 + (mi >> 1);
+          uint32_t b0, b1, b2, b3;
+          ldmatrix_x4_trans(vbase + tok * kRowBytes + (((c ^ tok) & 7) | (c & 8)) * 16, b0, b1, b2, b3);
+#pragma unroll
+          for (int t = 0; t < TILES; ++t) {
+            mma16816<T>(o[t][2 * np], pa[t][0], pa[t][1], pa[t][2], pa[t][3], b0, b1);
+            mma16816<T>(o[t][2 * np + 1], pa[t][0], pa[t][1], pa[t][2], pa[t][3], b2, b3);
+          }
+        }
+      }
+      __syncwarp();       // the stage is free
+      if (++stage == kStages) stage = 0;
+    }
+    // the piece's sums: number `range` + segment of this head
+    const int64_t slot = shared_part ? (static_cast<int64_t>(hv) * (p.ranges_most + p.groups) + range + at.seg) * kBaTile
+                                     : (static_cast<int64_t>(hv) * (p.ranges_most + p.groups * p.per_block) + range + i0) * p.rep;
+    float* po = shared_part ? p.o_common : p.o_own;
+    float2* pml = shared_part ? p.ml_common : p.ml_own;
+#pragma unroll
+    for (int t = 0; t < TILES; ++t)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float& sum = l[t][half];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        const int i = t * 16 + half * 8 + g8;
+        if (i < live) {
+          if (t4 == 0) pml[slot + i] = make_float2(m[t][half], sum);
+          float* to = po + (slot + i) * HD + 2 * t4;
+#pragma unroll
+          for (int k = 0; k < HD / 8; ++k) *reinterpret_cast<float2*>(to + k * 8) = make_float2(o[t][k][2 * half], o[t][k][2 * half + 1]);
+        }
+      }
+  };
+  while (at.x < x_end) {
+    if (at.x >= at.seg_end) enter(at);
+    if (at.seg < p.groups && p.per_block * p.rep > 16) piece(std::integral_constant<int, 2>{});
+    else piece(std::integral_constant<int, 1>{});
+  }
+}
+
+// Adds up the pieces of a row and query head: those of its group's common part, then its own.  WARPS of them share one's pieces (few
+// rows), or each warp has its own.
+template <typename T, int HD, int WARPS>
+__global__ void __launch_bounds__(kBaThreads) attn_beams_merge_kernel(const BeamAttnParams p) {
+  constexpr int kLanes = HD / 4, kTeams = WARPS * 32 / kLanes;      // lanes that hold a row of sums; teams that take every n-th piece
   ptx::griddep_launch_dependents();
   ptx::griddep_wait();
-  constexpr int N = HD / 32;
-  const int lane = threadIdx.x & 31, item = blockIdx.x * 4 + (threadIdx.x >> 5);
+  __shared__ float4 part[WARPS > 1 ? kTeams : 1][kLanes];
+  __shared__ float2 part_ml[WARPS > 1 ? kTeams : 1];
+  const int item = WARPS > 1 ? blockIdx.x : blockIdx.x * kBaWarps + (threadIdx.x >> 5);
   if (item >= p.rows * p.q_heads) return;
-  const int row = item / p.q_heads, head = item % p.q_heads, h = head / (p.q_heads / p.kv_heads);
-  const T* q = reinterpret_cast<const T*>(p.q) + row * p.q_stride + head * HD + lane * N;
-  const int first = p.indptr[row], pages = p.indptr[row + 1] - first;
-  const int length = pages > 0 ? (pages - 1) * p.page + p.last_page_len[row] : 0;
-  float x[N], o[N] = {}, m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int i = 0; i < N; ++i) x[i] = ldf(q + i);
-  if (p.sink) {
-    m = ldf(reinterpret_cast<const T*>(p.sink) + head);
-    l = 1.f;
-  }
-  const int64_t pitch = static_cast<int64_t>(p.kv_heads) * HD;
-  for (int t = 0; t < length; ++t) {
-    int page = p.indices[first + t / p.page];
-    if (page < 0 || page >= p.max_pages) {
-      if (p.status && lane == 0) atomicCAS(p.status, 0, kStatusBadIndex);
-      page = 0;
+  const int tid = WARPS > 1 ? threadIdx.x : threadIdx.x & 31;
+  const int row = item / p.q_heads, qh = item % p.q_heads, head = qh / p.rep;
+  const int g = row / p.beams, j = row % p.beams, block = j / p.per_block, jb = j % p.per_block;
+  const int per = p.groups * (1 + p.per_block);
+  const int* line = p.line + block * per;
+  const int base = line[0];
+  const BaRanges ranges(line[per] - base, p.ranges_most);
+  const int hv = head * p.blocks + block, team = tid / kLanes, c = tid % kLanes;
+  const int c0 = line[g] - base, c1 = line[g + 1] - base, own = p.groups + g * p.per_block + jb;
+  const int o0 = line[own] - base, o1 = line[own + 1] - base;
+  const int r0 = c0 < c1 ? ranges.of(c0) : 0, n0 = c0 < c1 ? ranges.of(c1 - 1) - r0 + 1 : 0;
+  const int r1 = o0 < o1 ? ranges.of(o0) : 0, n1 = o0 < o1 ? ranges.of(o1 - 1) - r1 + 1 : 0;
+  const bool live = p.line[p.blocks * per + 1 + row] > 0;
+  const int64_t common = (static_cast<int64_t>(hv) * (p.ranges_most + p.groups) + r0 + g) * kBaTile + jb * p.rep + qh % p.rep;
+  const int64_t mine = (static_cast<int64_t>(hv) * (p.ranges_most + p.groups * p.per_block) + r1 + own - p.groups) * p.rep + qh % p.rep;
+  float M = -INFINITY, L = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](float m, float l, const float4& x) {
+    const float top = fmaxf(M, m), a = M > -INFINITY ? ptx::ex2_approx(M - top) : 0.f, b = m > -INFINITY ? ptx::ex2_approx(m - top) : 0.f;
+    acc.x = acc.x * a + x.x * b;
+    acc.y = acc.y * a + x.y * b;
+    acc.z = acc.z * a + x.z * b;
+    acc.w = acc.w * a + x.w * b;
+    L = L * a + l * b;
+    M = top;
+  };
+  if (live) {
+#pragma unroll 4
+    for (int i = team; i < n0 + n1; i += kTeams) {
+      const bool sh = i < n0;
+      const int64_t at = sh ? common + static_cast<int64_t>(i) * kBaTile : mine + static_cast<int64_t>(i - n0) * p.rep;
+      const float2 ml = (sh ? p.ml_common : p.ml_own)[at];
+      add(ml.x, ml.y, *reinterpret_cast<const float4*>((sh ? p.o_common : p.o_own) + at * HD + 4 * c));
     }
-    const T* k = reinterpret_cast<const T*>(p.kv) + (static_cast<int64_t>(page) * 2 * p.page + t % p.page) * pitch + h * HD + lane * N;
-    const T* v = k + p.page * pitch;
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) s += x[i] * ldf(k + i);
-    s = warp_sum(s) * p.scale;
-    if (p.cap > 0.f) s = p.cap * tanhf(s / p.cap);
-    const float top = fmaxf(m, s), keep = expf(m - top), w = expf(s - top);
-    l = l * keep + w;
-    m = top;
-#pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = o[i] * keep + w * ldf(v + i);
   }
-  T* out = reinterpret_cast<T*>(p.out) + row * p.out_stride + head * HD + lane * N;
-#pragma unroll
-  for (int i = 0; i < N; ++i) stf(out + i, l > 0.f ? o[i] / l : 0.f);
+  if constexpr (WARPS > 1) {
+    part[team][c] = acc;
+    if (c == 0) part_ml[team] = make_float2(M, L);
+    __syncthreads();
+    if (team > 0) return;
+    for (int i = 1; i < kTeams; ++i) add(part_ml[i].x, part_ml[i].y, part[i][c]);
+  } else if constexpr (kTeams > 1) {     // (two halves of a warp)
+    const float4 x = make_float4(__shfl_xor_sync(0xffffffffu, acc.x, 16), __shfl_xor_sync(0xffffffffu, acc.y, 16), __shfl_xor_sync(0xffffffffu, acc.z, 16),
+                                 __shfl_xor_sync(0xffffffffu, acc.w, 16));
+    const float m = __shfl_xor_sync(0xffffffffu, M, 16), l = __shfl_xor_sync(0xffffffffu, L, 16);
+    if (team > 0) return;
+    add(m, l, x);
+  }
+  if (p.sink && live) {
+    const float s = ldf(reinterpret_cast<const T*>(p.sink) + qh) * 1.4426950408889634f;
+    add(s, 1.f, make_float4(0.f, 0.f, 0.f, 0.f));
+  }
+  const float f = L > 0.f ? 1.f / L : 0.f;
+  stf4(reinterpret_cast<T*>(p.out) + row * p.out_stride + static_cast<int64_t>(qh) * HD + 4 * c, make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
+}
+
+// How a call is divided, and its scratch.
+struct BaPlan {
+  int rep, kv_div, per_block, blocks, heads, ranges, rows;       // rows: of a launch
+  int64_t line, ml_common, ml_own, o_common, o_own, bytes;       // offsets
+};
+static BaPlan ba_plan(int rows, int beams, int q_heads, int kv_heads, int hd) {
+  BaPlan b;
+  const int group = q_heads / kv_heads;
+  b.kv_div = (group + 15) / 16;
+  while (group % b.kv_div) ++b.kv_div;
+  b.rep = group / b.kv_div;
+  const int most = kBaTile / b.rep;
+  b.blocks = (beams + most - 1) / most;
+  b.per_block = (beams + b.blocks - 1) / b.blocks;
+  b.blocks = (beams + b.per_block - 1) / b.per_block;
+  b.heads = kv_heads * b.kv_div * b.blocks;
+  b.ranges = device_sm_count() * kBaWarps / b.heads;
+  if (b.ranges < 1) b.ranges = 1;
+  b.rows = kBaRowsMost / beams * beams;
+  if (b.rows > rows) b.rows = rows;
+  const int64_t groups = b.rows / beams, n_common = b.heads * (b.ranges + groups) * kBaTile, n_own = b.heads * (b.ranges + groups * b.per_block) * b.rep;
+  auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
+  b.line = 0;
+  b.ml_common = up(4 * (b.blocks * groups * (1 + b.per_block) + 1 + b.rows + b.blocks * groups));
+  b.ml_own = b.ml_common + up(8 * n_common);
+  b.o_common = b.ml_own + up(8 * n_own);
+  b.o_own = b.o_common + up(4 * n_common * hd);
+  b.bytes = b.o_own + up(4 * n_own * hd);
+  return b;
+}
+
+template <typename T, int HD>
+static int ba_launch(const BeamAttnParams& p, cudaStream_t stream) {
+  auto kern = attn_beams_kernel<T, HD>;
+  constexpr int kRing = kBaWarps * (HD == 128 ? 3 : 6) * 2 * kBaStep * HD * 2;
+  const int per = p.groups * (1 + p.per_block);
+  static PerDeviceOnce once;
+  cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 1024); });
+  if (e != cudaSuccess) return (int)e;
+  const int workers = p.heads * p.ranges_most;
+  const size_t smem = kRing + 4 * static_cast<size_t>(p.blocks * per + 1 + p.rows + p.blocks * p.groups);
+  e = launch_pdl(kern, dim3((workers + kBaWarps - 1) / kBaWarps), dim3(kBaThreads), smem, stream, p);
+  if (e != cudaSuccess) return (int)e;
+  const int items = p.rows * p.q_heads;
+  // few rows: a block for each, so that the many pieces of a long one are added up by eight warps
+  if (items <= 8 * device_sm_count()) return (int)launch_pdl(attn_beams_merge_kernel<T, HD, kBaWarps>, dim3(items), dim3(kBaThreads), 0, stream, p);
+  return (int)launch_pdl(attn_beams_merge_kernel<T, HD, 1>, dim3((items + kBaWarps - 1) / kBaWarps), dim3(kBaThreads), 0, stream, p);
 }
 
 }  // namespace blitz
@@ -72,21 +486,51 @@ __global__ void __launch_bounds__(128) attn_beams_kernel(const BeamAttnParams p)
 extern "C" {
 using namespace blitz;
 
-int64_t blitz_attn_beams_workspace_bytes(int rows, int beams, int q_heads, int kv_heads, int head_dim) { return 256; }
+int64_t blitz_attn_beams_workspace_bytes(int rows, int beams, int q_heads, int kv_heads, int head_dim) {
+  if (rows < 1 || beams < 1 || beams > 64 || kv_heads < 1 || q_heads < kv_heads) return 256;
+  return ba_plan((rows + beams - 1) / beams * beams, beams, q_heads, kv_heads, head_dim).bytes;
+}
 
+// kv [max_pages][2][page][kv_heads][head_dim]; rows in groups of `beams`; shared [rows / beams].  page: 16 tokens times a power of two.  cap 0 and sink null: none.
+// static_table != 0 promises that indices, indptr, last_page_len and shared are not written by kernels still running in this stream.
 int blitz_attn_beams(const void* q, int64_t q_stride, const void* kv, const int32_t* indices, const int32_t* indptr, const int32_t* last_page_len,
                      const int32_t* shared, void* out, int64_t out_stride, void* workspace, int64_t workspace_bytes, int rows, int beams, int q_heads,
                      int kv_heads, int head_dim, int page, int max_pages, float scale, float cap, const void* sink, int static_table, int* status, int dtype,
                      cudaStream_t stream) {
   if (rows <= 0) return 0;
-  if (beams < 1 || rows % beams || kv_heads < 1 || q_heads % kv_heads || (head_dim != 64 && head_dim != 128) || page < 1 || max_pages < 1 ||
-      workspace_bytes < blitz_attn_beams_workspace_bytes(rows, beams, q_heads, kv_heads, head_dim))
+  if (beams < 1 || beams > 64 || rows % beams || kv_heads < 1 || q_heads < 1 || q_heads % kv_heads || (head_dim != 64 && head_dim != 128) || page < 16 ||
+      (page & (page - 1)) || max_pages < 1 || (q_stride & 7) || (out_stride & 7))
     return -1;
-  BeamAttnParams p{q, q_stride, kv, indices, indptr, last_page_len, shared, out, out_stride, rows, beams, q_heads, kv_heads, page, max_pages, scale, cap, sink, status};
-  cudaError_t e = cudaSuccess;
-  const dim3 grid((rows * q_heads + 3) / 4);
-  BLITZ_DISPATCH_DTYPE(dtype, (e = launch_pdl(head_dim == 64 ? attn_beams_kernel<T, 64> : attn_beams_kernel<T, 128>, grid, dim3(128), 0, stream, p)));
-  return (int)e;
+  const BaPlan b = ba_plan(rows, beams, q_heads, kv_heads, head_dim);
+  if (workspace_bytes < b.bytes) return -1;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  BeamAttnParams p;
+  p.q_stride = q_stride; p.kv = kv; p.indices = indices; p.out_stride = out_stride;
+  p.beams = beams; p.q_heads = q_heads; p.rep = b.rep; p.kv_div = b.kv_div; p.kv_heads = kv_heads;
+  p.per_block = b.per_block; p.blocks = b.blocks; p.heads = b.heads; p.ranges_most = b.ranges;
+  p.page_shift = 31 - __builtin_clz(page); p.max_pages = max_pages;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.cap_scale = cap > 0.f ? scale / cap : 0.f;
+  p.cap_log2 = cap * 1.4426950408889634f;
+  p.sink = sink;
+  p.line = reinterpret_cast<int*>(ws + b.line);
+  p.ml_common = reinterpret_cast<float2*>(ws + b.ml_common);
+  p.ml_own = reinterpret_cast<float2*>(ws + b.ml_own);
+  p.o_common = reinterpret_cast<float*>(ws + b.o_common);
+  p.o_own = reinterpret_cast<float*>(ws + b.o_own);
+  p.static_table = static_table; p.status = status;
+  for (int r = 0; r < rows; r += b.rows) {
+    p.rows = rows - r < b.rows ? rows - r : b.rows;
+    p.groups = p.rows / beams;
+    p.q = static_cast<const uint8_t*>(q) + 2 * r * q_stride;
+    p.out = static_cast<uint8_t*>(out) + 2 * r * out_stride;
+    p.indptr = indptr + r; p.last_page_len = last_page_len + r; p.shared = shared + r / beams;
+    int rc;
+    if (dtype == 1) rc = head_dim == 128 ? ba_launch<__nv_bfloat16, 128>(p, stream) : ba_launch<__nv_bfloat16, 64>(p, stream);
+    else rc = head_dim == 128 ? ba_launch<__half, 128>(p, stream) : ba_launch<__half, 64>(p, stream);
+    if (rc) return rc;
+  }
+  return 0;
 }
 
 }  // extern "C"
