@@ -20,11 +20,12 @@ constexpr int kBeamMost = 64;  // beams of a request, and candidates of it
 // The second kernel, a block per request, adds up the sums, turns logits into values and orders them in 64 bits: candidates of
 // different beams may be nearer to one another than fp32 tells apart, and an exchange of two would be a wrong token.
 //
-// A chunk stays in registers between its two uses.  First the maxima of groups of threads: the n-th largest of them is a bound below the n-th
+// A chunk is looked at twice, so it waits in shared memory (cp.async; six blocks an SM, 192 KB under way; in registers it left room for one or two).
+// First the maxima of groups of threads: the n-th largest of them is a bound below the n-th
 // largest logit, which few others pass (64 groups, n = 32: 1.4 n are expected).  Then exponentials, and what passes the bound goes to
-// shared memory, where every candidate counts those above it.
-constexpr int kSelVectors = 8;    // 16-byte pieces a thread holds
-constexpr int kSelRoom = 1024;    // candidates of a chunk in shared memory
+// a list, where every candidate counts those above it.
+constexpr int kSelVectors = 8;    // 16-byte pieces a thread looks after
+constexpr int kSelRoom = 512;     // candidates of a chunk
 
 template <typename T>
 struct SelRow {
@@ -50,21 +51,39 @@ __device__ __forceinline__ void sel_unpack(const uint4& v, float (&f)[SelRow<T>:
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-struct SelPart {   // of a chunk: its largest logit m, the sum of exp(z - m)
-  float m, s;
+// The largest of a piece.  (16-bit types: two at a time.)
+template <typename T>
+__device__ __forceinline__ float sel_max(const uint4& v) {
+  if constexpr (sizeof(T) == 4) {
+    return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+  } else {
+    using T2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
+    auto two = [](uint32_t u) { return *reinterpret_cast<T2*>(&u); };
+    const T2 a = __hmax2(__hmax2(two(v.x), two(v.y)), __hmax2(two(v.z), two(v.w)));
+    const float2 f = cvt2<T>(*reinterpret_cast<const uint32_t*>(&a));
+    return fmaxf(f.x, f.y);
+  }
+}
+
+// Of a chunk: its largest logit m; c, and the sum of 2^(z L - c), L = log2 e in fp32 and c = m L rounded.  Off by the rounding of L for what lies
+// between z and m alone, once the merge has taken out m's own part.  Where m is so large that the rounding of c would be of a term's size: `far`, and s the
+// sum of exp(z - m).
+struct SelPart {
+  float m, c, s, far;
 };
+constexpr float kSelHuge = 65536.f;
 
 template <typename T>
-__global__ void __launch_bounds__(kBeamThreads)
+__global__ void __launch_bounds__(kBeamThreads, 6)
 beam_scan_kernel(const T* __restrict__ logits, int64_t stride, int vocab, int chunks, int n, SelPart* __restrict__ parts, uint64_t* __restrict__ keys) {
   constexpr int E = SelRow<T>::kElems;
-  ptx::griddep_launch_dependents();
-  ptx::griddep_wait();
-  __shared__ float top[128];
+  __shared__ uint4 data[kSelVectors * kBeamThreads];
+  __shared__ __align__(16) float top[128];
   __shared__ float warp_top[kBeamThreads / 32], warp_sum_[kBeamThreads / 32];
   __shared__ float bound;
-  __shared__ int found;
+  __shared__ int found, passed;
   __shared__ uint64_t cand[kSelRoom];
+  __shared__ uint16_t pieces[kSelVectors * kBeamThreads];     // that have a number which passes the bound
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t row = blockIdx.x / chunks;
   const int chunk = blockIdx.x % chunks;
@@ -72,33 +91,29 @@ beam_scan_kernel(const T* __restrict__ logits, int64_t stride, int vocab, int ch
   // pieces start on 16-byte boundaries, wherever the row does: the first one has `lead` elements before the row
   const int lead = static_cast<int>((reinterpret_cast<uintptr_t>(z) & 15) / sizeof(T));
   const int first = chunk * SelRow<T>::kChunk + tid * E - lead;   // element of the thread's first piece
-  uint4 data[kSelVectors];
-  auto again = [&] {       // (keeps the compiler from holding on to the unpacked numbers, twice as many registers)
-#pragma unroll
-    for (int j = 0; j < kSelVectors; ++j) asm volatile("" : "+r"(data[j].x), "+r"(data[j].y), "+r"(data[j].z), "+r"(data[j].w));
-  };
+  if (tid == 0) found = passed = 0;
+  ptx::griddep_launch_dependents();
+  ptx::griddep_wait();
 #pragma unroll
   for (int j = 0; j < kSelVectors; ++j) {
     const int at = first + j * kBeamThreads * E;
     if (at >= 0 && at + E <= vocab) {
-      data[j] = ld_nc16(z + at);
+      ptx::cp_async_16(ptx::smem_u32(&data[j * kBeamThreads + tid]), z + at, 16);
     } else {
-      T piece[E];
-#pragma unroll
+      T* piece = reinterpret_cast<T*>(&data[j * kBeamThreads + tid]);
       for (int e = 0; e < E; ++e) {
         if (at + e >= 0 && at + e < vocab) piece[e] = z[at + e];
         else stf(&piece[e], -INFINITY);
       }
-      memcpy(&data[j], piece, 16);
     }
   }
-  float mine = -INFINITY;
+  ptx::cp_async_commit();
+  ptx::cp_async_wait<0>();        // (a thread reads what it has copied itself)
+  float largest[kSelVectors], mine = -INFINITY;      // of each piece
 #pragma unroll
   for (int j = 0; j < kSelVectors; ++j) {
-    float f[E];
-    sel_unpack<T>(data[j], f);
-#pragma unroll
-    for (int e = 0; e < E; ++e) mine = fmaxf(mine, f[e]);
+    largest[j] = sel_max<T>(data[j * kBeamThreads + tid]);
+    mine = fmaxf(mine, largest[j]);
   }
   // groups: 32, 64 or 128 of them, at least twice n
   const int groups = n <= 16 ? 32 : n <= 32 ? 64 : 128, width = kBeamThreads / groups;
@@ -107,7 +122,6 @@ beam_scan_kernel(const T* __restrict__ logits, int64_t stride, int vocab, int ch
   if ((tid & (width - 1)) == 0) top[tid / width] = g;
   const float w = warp_max(mine);
   if (lane == 0) warp_top[warp] = w;
-  if (tid == 0) found = 0;
   __syncthreads();
   float m = warp_top[0];
 #pragma unroll
@@ -115,78 +129,65 @@ beam_scan_kernel(const T* __restrict__ logits, int64_t stride, int vocab, int ch
   if (tid < groups) {
     const float v = top[tid];
     int above = 0;
-    for (int i = 0; i < groups; ++i) above += top[i] > v || (top[i] == v && i < tid);
+    for (int i = 0; i < groups; i += 4) {
+      const float4 o = *reinterpret_cast<const float4*>(&top[i]);
+      above += (o.x > v || (o.x == v && i < tid)) + (o.y > v || (o.y == v && i + 1 < tid)) + (o.z > v || (o.z == v && i + 2 < tid)) +
+               (o.w > v || (o.w == v && i + 3 < tid));
+    }
     if (above == n - 1) bound = v;
   }
   __syncthreads();
   const float least = bound;
-  const float ref = m > -INFINITY ? m : 0.f;    // (a chunk of minus infinities: its sum is 0)
-  auto each = [&](auto&& take) {       // take(element, number) for all that pass the bound
-#pragma unroll
-    for (int j = 0; j < kSelVectors; ++j) {
-      float f[E];
-      sel_unpack<T>(data[j], f);
-      bool any = false;
-#pragma unroll
-      for (int e = 0; e < E; ++e) any |= f[e] >= least;
-      if (any) {
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (f[e] >= least && f[e] > -INFINITY) take(first + j * kBeamThreads * E + e, f[e]);
-      }
-    }
-  };
+  const bool huge = fabsf(m) > kSelHuge && m > -INFINITY;
+  const float c = m > -INFINITY ? m * kLog2e : 0.f;    // (a chunk of minus infinities: its sum is 0)
   auto key = [](int at, float x) { return static_cast<uint64_t>(sel_ordered(x)) << 32 | (0xffffffffu - static_cast<uint32_t>(at)); };
+#pragma unroll
+  for (int j = 0; j < kSelVectors; ++j)
+    if (largest[j] >= least && largest[j] > -INFINITY) pieces[atomicAdd(&passed, 1)] = static_cast<uint16_t>(j * kBeamThreads + tid);
   float sum = 0.f;
-  again();
 #pragma unroll
   for (int j = 0; j < kSelVectors; ++j) {
     float f[E];
-    sel_unpack<T>(data[j], f);
+    sel_unpack<T>(data[j * kBeamThreads + tid], f);
     float part = 0.f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) part += ptx::ex2_approx((f[e] - ref) * kLog2e);
+    for (int e = 0; e < E; ++e) part += ptx::ex2_approx(fmaf(f[e], kLog2e, -c));
     sum += part;
   }
-  again();
-  each([&](int at, float x) {
-    const int i = atomicAdd(&found, 1);
-    if (i < kSelRoom) cand[i] = key(at, x);
-  });
+  if (huge) {
+    sum = 0.f;
+#pragma unroll 1
+    for (int i = 0; i < kSelVectors * E; ++i)
+      sum += ptx::ex2_approx((ldf(reinterpret_cast<const T*>(&data[i / E * kBeamThreads + tid]) + i % E) - m) * kLog2e);
+  }
   sum = warp_sum(sum);
   if (lane == 0) warp_sum_[warp] = sum;
   __syncthreads();
-  int count = found;
-  if (count > kSelRoom) {
-    // Many equal numbers, or large ones of few groups: the bound is moved up by halves until no more pass it than there is room for.  (Keys
-    // differ from one another, so some bound lets n to kSelRoom through.)
-    uint64_t lo = key(0x7fffffff, least), hi = ~0ull;
-    for (int i = 0; i < 64; ++i) {
-      const uint64_t mid = lo + (hi - lo) / 2;
-      __syncthreads();
-      if (tid == 0) found = 0;
-      __syncthreads();
-      int here = 0;
-      each([&](int at, float x) { here += key(at, x) >= mid; });
-      here = __reduce_add_sync(0xffffffffu, here);
-      if (lane == 0 && here) atomicAdd(&found, here);
-      __syncthreads();
-      count = found;
-      if (count > kSelRoom) lo = mid;
-      else if (count < n) hi = mid;
-      else {
-        __syncthreads();
-        if (tid == 0) found = 0;
-        __syncthreads();
-        each([&](int at, float x) {
-          const uint64_t k = key(at, x);
-          if (k >= mid) cand[atomicAdd(&found, 1)] = k;
-        });
-        __syncthreads();
-        break;
+  // candidates: numbers of those pieces from the bound on.  Where there are too many (equal numbers, or large ones of few groups) the bound is
+  // moved up by halves until there is room for them.  (Keys differ from one another, so some bound lets n to kSelRoom through.)
+  uint64_t lo = 0, hi = ~0ull, mid = key(0x7fffffff, least);
+  int count;
+  for (int turn = 0;; ++turn) {
+#pragma unroll 1
+    for (int i = tid; i < passed * E; i += kBeamThreads) {
+      const int piece = pieces[i / E], e = i % E;
+      const uint64_t k = key(chunk * SelRow<T>::kChunk + piece * E - lead + e, ldf(reinterpret_cast<const T*>(&data[piece]) + e));
+      if (k >= mid && k >> 32) {
+        const int at = atomicAdd(&found, 1);
+        if (at < kSelRoom) cand[at] = k;
       }
     }
+    __syncthreads();
+    count = found;
+    if (count <= kSelRoom && (count >= n || turn == 0)) break;
+    if (turn > 64) break;      // (not reached)
+    (count > kSelRoom ? lo : hi) = mid;
+    mid = lo + (hi - lo) / 2;
+    __syncthreads();
+    if (tid == 0) found = 0;
+    __syncthreads();
   }
+  count = min(count, kSelRoom);
   uint64_t* out = keys + static_cast<int64_t>(blockIdx.x) * n;
   for (int i = tid; i < count; i += kBeamThreads) {
     const uint64_t mykey = cand[i];
@@ -199,7 +200,7 @@ beam_scan_kernel(const T* __restrict__ logits, int64_t stride, int vocab, int ch
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < kBeamThreads / 32; ++i) s += warp_sum_[i];
-    parts[blockIdx.x] = SelPart{m, s};
+    parts[blockIdx.x] = SelPart{m, c, s, huge ? 1.f : 0.f};
   }
 }
 
@@ -207,109 +208,152 @@ struct SelOut {
   float* score;
   int32_t *parent, *token;
 };
+// A candidate: its value as 64 bits in the order of the numbers (0: none), its beam and token.  (Comparisons of doubles took half the kernel's time.)
 struct SelCand {
-  double v;
-  int32_t row, token;
+  uint64_t v, place;
 };
-__device__ __forceinline__ bool sel_before(const SelCand& a, const SelCand& b) {
-  return a.v > b.v || (a.v == b.v && (a.row < b.row || (a.row == b.row && a.token < b.token)));
+__device__ __forceinline__ bool sel_before(const SelCand& a, const SelCand& b) { return a.v > b.v || (a.v == b.v && a.place < b.place); }
+__device__ __forceinline__ float sel_value(const SelCand& a) {
+  return static_cast<float>(__longlong_as_double(static_cast<long long>(a.v ^ (a.v >> 63 ? 1ull << 63 : ~0ull))));
 }
 
-// A block per request.  Of the chunks' lists those whose first entry is among the n best first entries are looked at: the n best are in them.
+// A block per request: of the chunks' candidates the n best, by a bound as in the scan.  Neighbouring candidates of a list are in different groups, so that lists
+// that have most of the best ones do not let more through.  (An earlier form took heads of the lists one after the other: 20 us for n = 24.)
+constexpr int kSelListRoom = 8192;      // keys that wait in shared memory, where they are no more
+constexpr int kSelBestRoom = 1024;
 __global__ void __launch_bounds__(kBeamThreads)
 beam_merge_kernel(const SelPart* __restrict__ parts, const uint64_t* __restrict__ keys, const float* __restrict__ scores, int beams, int chunks, int n,
                   int keep, const int32_t* __restrict__ ended, int num_ended, SelOut all, SelOut next) {
+  constexpr int kWarps = kBeamThreads / 32;
+  extern __shared__ __align__(16) uint64_t held[];
+  __shared__ __align__(16) uint64_t top[kBeamThreads];
+  __shared__ SelCand cand[kSelBestRoom], best[kBeamMost];
+  __shared__ double norm[kBeamMost], base[kBeamMost];
+  __shared__ uint64_t bound;
+  __shared__ int found;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, num = beams * chunks * n;
+  const int64_t q = blockIdx.x;
+  parts += q * beams * chunks;
+  keys += q * num;
+  const bool in_shared = num <= kSelListRoom;
+  if (tid == 0) found = 0;
+  if (tid < n) best[tid] = SelCand{0, ~0ull};
   ptx::griddep_launch_dependents();
   ptx::griddep_wait();
-  extern __shared__ __align__(16) uint8_t sel_smem[];
-  SelCand* cand = reinterpret_cast<SelCand*>(sel_smem);               // [n n]
-  SelCand* heads = cand + n * n;                                      // [beams chunks]
-  SelCand* best = heads + beams * chunks;                             // [n]
-  __shared__ double norm[kBeamMost], base[kBeamMost];
-  __shared__ int lists[kBeamMost], found;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, num = beams * chunks;
-  const int64_t q = blockIdx.x;
-  parts += q * num;
-  keys += q * num * n;
-  if (tid == 0) found = 0;
-  for (int b = warp; b < beams; b += kBeamThreads / 32) {
+  if (in_shared) {
+#pragma unroll 8
+    for (int i = tid; i < num; i += kBeamThreads) held[i] = keys[i];
+  }
+  for (int b = warp; b < beams; b += kWarps) {
     const SelPart* row = parts + b * chunks;
-    float m = -INFINITY;
-    for (int i = lane; i < chunks; i += 32) m = fmaxf(m, row[i].m);
+    const float score = scores[q * beams + b];
+    const SelPart one = lane < chunks ? row[lane] : SelPart{-INFINITY, 0.f, 0.f, 0.f};
+    float m = one.m;
+    for (int i = lane + 32; i < chunks; i += 32) m = fmaxf(m, row[i].m);
     m = warp_max(m);
-    double s = 0.0;
-    for (int i = lane; i < chunks; i += 32)
-      s += static_cast<double>(row[i].s) * (row[i].m > -INFINITY ? exp(static_cast<double>(row[i].m) - m) : 1.0);   // (1: NaN stays, 0 does)
-#pragma unroll
-    for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+    // sum of exp(z - m): of a chunk, s exp(c ln 2 - m) exp(-d m'), L ln 2 = 1 + d, m' its largest
+    constexpr double kLn2 = 0.69314718055994531, kD = static_cast<double>(kLog2e) * kLn2 - 1.0;
+    auto share = [&](const SelPart& x) {
+      if (!(x.m > -INFINITY)) return x.s;      // (0, or NaN)
+      return x.s * (x.far != 0.f ? expf(x.m - m) : expf(static_cast<float>(x.c * kLn2 - m - kD * x.m)));
+    };
+    float s = share(one);
+    for (int i = lane + 32; i < chunks; i += 32) s += share(row[i]);
+    s = warp_sum(s);
     if (lane == 0) {
-      norm[b] = m + log(s);
-      base[b] = scores[q * beams + b];
+      // log s = log f + e log 2 with f from 1 to 2: in fp32 off by 2^-24, where log s would be by 2^-21
+      int e = 1;
+      const bool number = s > 0.f && s < INFINITY;
+      const float f = number ? 2.f * frexpf(s, &e) : s;
+      norm[b] = static_cast<double>(m) + (static_cast<double>(logf(f)) + (e - 1) * kLn2);
+      base[b] = score;
     }
   }
   __syncthreads();
-  auto entry = [&](int list, int i) {
-    const uint64_t k = keys[static_cast<int64_t>(list) * n + i];
-    const int b = list / chunks;
-    const double x = k ? base[b] + (static_cast<double>(sel_number(static_cast<uint32_t>(k >> 32))) - norm[b]) : -INFINITY;
-    const double v = x > -INFINITY ? x : -INFINITY;      // (what is no number is no candidate)
-    return SelCand{v, b, static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(k))};
+  auto made = [&](int i) {
+    const uint64_t k = in_shared ? held[i] : keys[i];
+    if (k == 0) return SelCand{0, ~0ull};
+    const int b = i / (chunks * n);
+    const double v = base[b] + (static_cast<double>(sel_number(static_cast<uint32_t>(k >> 32))) - norm[b]) + 0.0;      // (-0 as 0)
+    const uint64_t u = static_cast<uint64_t>(__double_as_longlong(v));
+    // (what is no number is no candidate)
+    return v > -INFINITY ? SelCand{u ^ (u >> 63 ? ~0ull : 1ull << 63), static_cast<uint64_t>(b) << 32 | (0xffffffffu - static_cast<uint32_t>(k))} : SelCand{0, ~0ull};
   };
-  for (int i = tid; i < num; i += kBeamThreads) heads[i] = entry(i, 0);
-  if (tid < n) {
-    lists[tid] = -1;
-    best[tid] = SelCand{-INFINITY, -1, -1};
+  uint64_t mine = 0;
+#pragma unroll 4
+  for (int i = tid; i < num; i += kBeamThreads) mine = max(mine, made(i).v);
+  top[tid] = mine;
+  __syncthreads();
+  const int groups = n <= 32 ? 64 : 128;
+  if (tid < groups) {
+    for (int i = tid + groups; i < kBeamThreads; i += groups) mine = max(mine, top[i]);
+    top[tid] = mine;
   }
   __syncthreads();
+  if (tid < groups) {
+    int above = 0;
+#pragma unroll 8
+    for (int i = 0; i < groups; ++i) above += top[i] > mine || (top[i] == mine && i < tid);
+    if (above == n - 1) bound = mine;
+  }
+  __syncthreads();
+  const uint64_t least = bound > 0 ? bound : 1;
+#pragma unroll 4
   for (int i = tid; i < num; i += kBeamThreads) {
-    const SelCand h = heads[i];
-    if (!(h.v > -INFINITY)) continue;
-    int above = 0;
-    for (int k = 0; k < num; ++k) above += sel_before(heads[k], h);
-    if (above < n) lists[above] = i;
+    const SelCand e = made(i);
+    if (e.v >= least) {
+      const int at = atomicAdd(&found, 1);
+      if (at < kSelBestRoom) cand[at] = e;
+    }
   }
   __syncthreads();
-  const bool cut = num >= n && lists[n - 1] >= 0;
-  const SelCand least = cut ? heads[lists[n - 1]] : SelCand{-INFINITY, 0, 0};
-  for (int i = tid; i < n * n; i += kBeamThreads) {
-    const int list = lists[i / n];
-    if (list < 0) continue;
-    const SelCand e = entry(list, i % n);
-    if (e.v > -INFINITY && !(cut && sel_before(least, e))) cand[atomicAdd(&found, 1)] = e;
-  }
-  __syncthreads();
-  for (int i = tid; i < found; i += kBeamThreads) {
-    const SelCand e = cand[i];
-    int above = 0;
-    for (int k = 0; k < found; ++k) above += sel_before(cand[k], e);
-    if (above < n) best[above] = e;
-  }
-  __syncthreads();
-  for (int i = tid; i < n; i += kBeamThreads) {
-    all.score[q * n + i] = static_cast<float>(best[i].v);
-    all.parent[q * n + i] = best[i].row;
-    all.token[q * n + i] = best[i].token;
-  }
-  if (warp == 0) {
-    int before = 0;
-    for (int i0 = 0; i0 < n; i0 += 32) {
-      const int i = i0 + lane;
-      bool on = i < n && best[i].row >= 0;
-      for (int e = 0; on && e < num_ended; ++e) on = ended[e] != best[i].token;
-      const unsigned who = __ballot_sync(0xffffffffu, on);
-      const int at = before + __popc(who & ((1u << lane) - 1));
-      if (on && at < keep) {
-        next.score[q * keep + at] = static_cast<float>(best[i].v);
-        next.parent[q * keep + at] = best[i].row;
-        next.token[q * keep + at] = best[i].token;
+  const int count = found;
+  if (count <= kSelBestRoom) {
+    for (int i = tid; i < count; i += kBeamThreads) {
+      const SelCand e = cand[i];
+      int above = 0;
+#pragma unroll 4
+      for (int k = 0; k < count; ++k) above += sel_before(cand[k], e);
+      if (above < n) best[above] = e;
+    }
+  } else {
+    // many equal values: one after the other, the best of those behind the last one
+    SelCand last{~0ull, 0};
+    for (int j = 0; j < n; ++j) {
+      SelCand first{0, ~0ull};
+      for (int i = tid; i < num; i += kBeamThreads) {
+        const SelCand e = made(i);
+        if (e.v && sel_before(last, e) && sel_before(e, first)) first = e;
       }
-      before += __popc(who);
-    }
-    for (int i = before + lane; i < keep; i += 32) {
-      next.score[q * keep + i] = -INFINITY;
-      next.parent[q * keep + i] = next.token[q * keep + i] = -1;
+      __syncthreads();
+      cand[tid] = first;
+      __syncthreads();
+      for (int i = 0; i < kBeamThreads; ++i)
+        if (sel_before(cand[i], first)) first = cand[i];
+      if (tid == 0) best[j] = first;
+      last = first;
+      if (first.v == 0) break;
     }
   }
+  __syncthreads();
+  if (warp > 0) return;
+  auto give = [](const SelOut& to, int64_t at, const SelCand& e) {
+    to.score[at] = e.v ? sel_value(e) : -INFINITY;
+    to.parent[at] = e.v ? static_cast<int32_t>(e.place >> 32) : -1;
+    to.token[at] = e.v ? static_cast<int32_t>(e.place) : -1;
+  };
+  int before = 0;
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    const int i = i0 + lane;
+    if (i < n) give(all, q * n + i, best[i]);
+    bool on = i < n && best[i].v != 0;
+    for (int e = 0; on && e < num_ended; ++e) on = ended[e] != static_cast<int32_t>(best[i].place);
+    const unsigned who = __ballot_sync(0xffffffffu, on);
+    const int at = before + __popc(who & ((1u << lane) - 1));
+    if (on && at < keep) give(next, q * keep + at, best[i]);
+    before += __popc(who);
+  }
+  for (int i = before + lane; i < keep; i += 32) give(next, q * keep + i, SelCand{0, ~0ull});
 }
 
 // ------------------------------------------------------------------ tables of the beams that go on
@@ -322,50 +366,58 @@ struct ForkParams {
 };
 
 // A block per request.  A bit per page says which ones the children keep; the fresh ones are the first of the request's own without it.
+// Latency bounds it: lengths, then tables, are two rounds of loads, all of a round at once.
 __global__ void __launch_bounds__(kBeamThreads) beam_fork_kernel(const ForkParams p) {
-  ptx::griddep_launch_dependents();
-  ptx::griddep_wait();
   extern __shared__ uint32_t used[];
-  __shared__ int par[kBeamMost], len[kBeamMost], again[kBeamMost], want[kBeamMost], fresh[kBeamMost], sums[kBeamThreads / 32];
+  __shared__ int par[kBeamMost], len[kBeamMost], again[kBeamMost], want[kBeamMost], fresh[kBeamMost], held[kBeamMost], sums[kBeamThreads / 32];
   __shared__ int wanted;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t q = blockIdx.x;
   const int words = (p.num_pages + 31) / 32;
   for (int i = tid; i < words; i += kBeamThreads) used[i] = 0;
   auto report = [&](int code) { if (p.status) atomicCAS(p.status, 0, code); };
+  ptx::griddep_launch_dependents();
+  ptx::griddep_wait();
+  const int first_pool = tid < p.pool_size ? p.pool[q * p.pool_stride + tid] : -1;
   if (tid < p.to) {
-    const int b = p.parents[q * p.to + tid];
+    par[tid] = p.parents[q * p.to + tid];
+    fresh[tid] = -1;
+  } else if (tid >= kBeamMost && tid < kBeamMost + p.from) {
+    held[tid - kBeamMost] = p.cached[q * p.from + tid - kBeamMost];
+  }
+  __syncthreads();
+  if (tid < p.to) {
+    const int b = par[tid];
     int n = -1;
     if (b >= 0 && b < p.from) {
-      n = p.cached[q * p.from + b];
-      if (n >= 0 && n / p.page >= p.width) {
+      n = max(held[b], -1);
+      if (n / p.page >= p.width) {
         report(kStatusTooLarge);
         n = -1;
       }
     } else if (b >= p.from) {
       report(kStatusBadIndex);
     }
-    par[tid] = b;
-    len[tid] = n < 0 ? -1 : n;
-    fresh[tid] = -1;
-  }
-  __syncthreads();
-  if (tid < p.to) {
-    int seen = 0;
-    for (int i = 0; i < tid; ++i) seen |= len[i] >= 0 && par[i] == par[tid];
+    int seen = 0;         // (children of one parent are all alive or all dead)
+    for (int i = 0; i < tid; ++i) seen |= par[i] == b;
+    len[tid] = n;
     again[tid] = seen;
   }
   __syncthreads();
-  // pages that children keep (a parent's once)
-  for (int j = 0; j < p.to; ++j) {
-    if (len[j] < 0 || again[j]) continue;
-    const int32_t* row = p.table + (q * p.from + par[j]) * p.table_stride;
-    const int keeps = (len[j] + p.page - 1) / p.page;
-    for (int i = tid; i < keeps; i += kBeamThreads) {
-      const int pg = row[i];
-      if (pg >= 0 && pg < p.num_pages) atomicOr(&used[pg >> 5], 1u << (pg & 31));
-      else report(kStatusBadIndex);
+  // children's tables without their fresh pages, and the pages that they keep (a parent's once)
+#pragma unroll 4
+  for (int it = tid; it < p.to * p.width; it += kBeamThreads) {
+    const int j = it / p.width, i = it - j * p.width, n = len[j];
+    const int keeps = n < 0 ? 0 : again[j] ? n / p.page : (n + p.page - 1) / p.page;
+    int pg = -1;
+    if (i < keeps) {
+      pg = p.table[(q * p.from + par[j]) * p.table_stride + i];
+      if (!again[j]) {
+        if (pg >= 0 && pg < p.num_pages) atomicOr(&used[pg >> 5], 1u << (pg & 31));
+        else report(kStatusBadIndex);
+      }
     }
+    p.out_table[q * p.to * p.width + it] = pg;
   }
   if (warp == 0) {       // which children want a fresh page: theirs is the one of their number among them
     int before = 0;
@@ -381,7 +433,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_fork_kernel(const ForkParam
   __syncthreads();
   int got = 0;
   for (int i0 = 0; i0 < p.pool_size && got < wanted; i0 += kBeamThreads) {
-    const int i = i0 + tid, pg = i < p.pool_size ? p.pool[q * p.pool_stride + i] : -1;
+    const int i = i0 + tid, pg = i0 == 0 ? first_pool : i < p.pool_size ? p.pool[q * p.pool_stride + i] : -1;
     const bool free = pg >= 0 && pg < p.num_pages && !(used[pg >> 5] >> (pg & 31) & 1);
     const unsigned who = __ballot_sync(0xffffffffu, free);
     if (lane == 0) sums[warp] = __popc(who);
@@ -395,23 +447,19 @@ __global__ void __launch_bounds__(kBeamThreads) beam_fork_kernel(const ForkParam
     got += total;
     __syncthreads();
   }
-  for (int j = 0; j < p.to; ++j) {
-    const int n = len[j], full = n / p.page, part = n % p.page;
-    const bool wants = want[j] >= 0;
-    const int page = wants ? fresh[want[j]] : -1;
-    const bool live = n >= 0 && (!wants || page >= 0);
-    const int keeps = !live ? 0 : wants ? full : (n + p.page - 1) / p.page;
-    const int32_t* row = p.table + (q * p.from + par[j]) * p.table_stride;
-    int32_t* to = p.out_table + (q * p.to + j) * p.width;
-    for (int i = tid; i < p.width; i += kBeamThreads) to[i] = i < keeps ? row[i] : live && wants && i == full ? page : -1;
-    if (tid == 0) {
-      const bool copies = live && wants && part > 0;
-      if (n >= 0 && !live) report(kStatusNoPage);
-      p.out_cached[q * p.to + j] = live ? n : -1;
-      p.src[q * p.to + j] = copies ? row[full] : -1;
-      p.dst[q * p.to + j] = copies ? page : -1;
-      p.tokens[q * p.to + j] = copies ? part : 0;
+  if (tid < p.to) {
+    const int n = len[tid], page = want[tid] >= 0 ? fresh[want[tid]] : -1, full = n / p.page;
+    const bool live = n >= 0 && (want[tid] < 0 || page >= 0), copies = live && want[tid] >= 0 && n % p.page > 0;
+    const int64_t j = q * p.to + tid;
+    if (live && want[tid] >= 0) p.out_table[j * p.width + full] = page;
+    if (n >= 0 && !live) {
+      report(kStatusNoPage);
+      for (int i = 0; i < p.width; ++i) p.out_table[j * p.width + i] = -1;
     }
+    p.out_cached[j] = live ? n : -1;
+    p.src[j] = copies ? p.table[(q * p.from + par[tid]) * p.table_stride + full] : -1;
+    p.dst[j] = copies ? page : -1;
+    p.tokens[j] = copies ? n % p.page : 0;
   }
 }
 
@@ -636,12 +684,12 @@ int blitz_beam_select(const void* logits, int64_t stride, const float* scores, i
   BLITZ_DISPATCH_DTYPE3(dtype, (e = launch_pdl(beam_scan_kernel<T>, dim3(rows * chunks), dim3(kBeamThreads), 0, stream, (const T*)logits, stride, vocab, chunks, n,
                                                parts, keys)));
   if (e != cudaSuccess) return (int)e;
-  const size_t smem = sizeof(SelCand) * (static_cast<size_t>(n) * n + static_cast<size_t>(beams) * chunks + n);
-  if (smem > 200 * 1024) return -1;
+  const int64_t num = static_cast<int64_t>(beams) * chunks * n;
+  if (num > 0x7fffffff) return -1;
   static PerDeviceOnce once;
-  e = once.run([] { return cudaFuncSetAttribute(beam_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024); });
+  e = once.run([] { return cudaFuncSetAttribute(beam_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 8 * kSelListRoom); });
   if (e != cudaSuccess) return (int)e;
-  return (int)launch_pdl(beam_merge_kernel, dim3(rows / beams), dim3(kBeamThreads), smem, stream, parts, keys, scores, beams, chunks, n, keep, ended, num_ended,
+  return (int)launch_pdl(beam_merge_kernel, dim3(rows / beams), dim3(kBeamThreads), num <= kSelListRoom ? 8 * (size_t)num : 0, stream, parts, keys, scores, beams, chunks, n, keep, ended, num_ended,
                          SelOut{score, parent, token}, SelOut{next_score, next_parent, next_token});
 }
 
