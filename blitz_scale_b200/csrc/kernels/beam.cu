@@ -16,40 +16,30 @@ constexpr int kBeamMost = 64;  // beams of a request, and candidates of it
 // ------------------------------------------------------------------ selection
 // value(b, v) = score[b] + z[v] - log sum_u exp z[u], the n largest of a request's beams, ties to the lowest (b, v).
 //
-// A block takes a chunk of a row of logits: the sum of exponentials, and the chunk's n largest logits (those of a row order its values).
-// The second kernel, a block per request, adds up the sums, turns logits into values and orders them in 64 bits: candidates of
+// The scan streams the logits once: a warp takes a stretch of a row, and leaves the sum of exponentials beside its largest logit, and the largest
+// logit of every group of 512.  Nothing else is done beside the stream: a selection in it (bounds, lists and barriers for every 32 KB) took two to
+// three times the stream's time.  The second kernel, a block per request, knows the sums, hence the values of the groups' largest; the n best elements are in
+// the n best groups, which it reads again (1 KB each, out of L2 as a rule).  Values are pairs of fp32, 48 bits: candidates of
 // different beams may be nearer to one another than fp32 tells apart, and an exchange of two would be a wrong token.
-//
-// A chunk is looked at twice, so it waits in shared memory (cp.async; six blocks an SM, 192 KB under way; in registers it left room for one or two).
-// First the maxima of groups of threads: the n-th largest of them is a bound below the n-th
-// largest logit, which few others pass (64 groups, n = 32: 1.4 n are expected).  Then exponentials, and what passes the bound goes to
-// a list, where every candidate counts those above it.
-constexpr int kSelVectors = 8;    // 16-byte pieces a thread looks after
-constexpr int kSelRoom = 512;     // candidates of a chunk
+constexpr int kSelGroup = 512;
+constexpr int kSelWarps = 48;       // warps of an SM that the scan counts on
+constexpr int kSelStretch = 32;     // groups of a stretch at most (sums of more lose digits)
 
-template <typename T>
-struct SelRow {
-  static constexpr int kElems = 16 / sizeof(T);
-  static constexpr int kChunk = kBeamThreads * kSelVectors * kElems;
-};
-
-// Numbers in the order of their bits (-0 as 0); what has no number, or minus infinity, is no candidate: 0.
+// Numbers in the order of their bits (-0 as 0); minus infinity: 0.
 __device__ __forceinline__ uint32_t sel_ordered(float x) {
   const uint32_t u = __float_as_uint(x + 0.f);
   return x > -INFINITY ? (u ^ (u >> 31 ? 0xffffffffu : 0x80000000u)) : 0u;
 }
-__device__ __forceinline__ float sel_number(uint32_t o) { return __uint_as_float(o ^ (o >> 31 ? 0x80000000u : 0xffffffffu)); }
+__device__ __forceinline__ float sel_number(uint32_t o) { return o ? __uint_as_float(o ^ (o >> 31 ? 0x80000000u : 0xffffffffu)) : -INFINITY; }
 
 template <typename T>
-__device__ __forceinline__ void sel_unpack(const uint4& v, float (&f)[SelRow<T>::kElems]) {
+__device__ __forceinline__ void sel_unpack(const uint4& v, float (&f)[16 / sizeof(T)]) {
   if constexpr (sizeof(T) == 4) {
     f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
   } else {
     unpack8<T>(v, f);
   }
 }
-
-constexpr float kLog2e = 1.4426950408889634f;
 
 // The largest of a piece.  (16-bit types: two at a time.)
 template <typename T>
@@ -65,295 +55,321 @@ __device__ __forceinline__ float sel_max(const uint4& v) {
   }
 }
 
-// Of a chunk: its largest logit m; c, and the sum of 2^(z L - c), L = log2 e in fp32 and c = m L rounded.  Off by the rounding of L for what lies
-// between z and m alone, once the merge has taken out m's own part.  Where m is so large that the rounding of c would be of a term's size: `far`, and s the
-// sum of exp(z - m).
-struct SelPart {
-  float m, c, s, far;
-};
-constexpr float kSelHuge = 65536.f;
-
+// A row in groups: those begin on 16-byte boundaries, wherever the row does, so its first one may have some elements before the row.
 template <typename T>
-__global__ void __launch_bounds__(kBeamThreads, 6)
-beam_scan_kernel(const T* __restrict__ logits, int64_t stride, int vocab, int chunks, int n, SelPart* __restrict__ parts, uint64_t* __restrict__ keys) {
-  constexpr int E = SelRow<T>::kElems;
-  __shared__ uint4 data[kSelVectors * kBeamThreads];
-  __shared__ __align__(16) float top[128];
-  __shared__ float warp_top[kBeamThreads / 32], warp_sum_[kBeamThreads / 32];
-  __shared__ float bound;
-  __shared__ int found, passed;
-  __shared__ uint64_t cand[kSelRoom];
-  __shared__ uint16_t pieces[kSelVectors * kBeamThreads];     // that have a number which passes the bound
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int64_t row = blockIdx.x / chunks;
-  const int chunk = blockIdx.x % chunks;
-  const T* z = logits + row * stride;
-  // pieces start on 16-byte boundaries, wherever the row does: the first one has `lead` elements before the row
-  const int lead = static_cast<int>((reinterpret_cast<uintptr_t>(z) & 15) / sizeof(T));
-  const int first = chunk * SelRow<T>::kChunk + tid * E - lead;   // element of the thread's first piece
-  if (tid == 0) found = passed = 0;
-  ptx::griddep_launch_dependents();
+struct SelRow {
+  static constexpr int E = 16 / sizeof(T), NV = kSelGroup / (32 * E);      // elements of a piece, pieces of a group that a lane has
+  static constexpr int kRing = sizeof(T) == 2 ? 4 : 3;                      // groups of a warp that wait in shared memory or are on their way
+};
+// Element `at` of a row and those behind it, a piece, into shared memory; outside the row: -inf.
+template <typename T>
+__device__ __forceinline__ void sel_piece(uint4* to, const T* z, int at, int vocab) {
+  constexpr int E = 16 / sizeof(T);
+  if (at >= 0 && at + E <= vocab) {
+    ptx::cp_async_16(ptx::smem_u32(to), z + at, 16);
+  } else {
+#pragma unroll 1
+    for (int e = 0; e < E; ++e) {
+      if (at + e >= 0 && at + e < vocab) reinterpret_cast<T*>(to)[e] = z[at + e];
+      else stf(reinterpret_cast<T*>(to) + e, -INFINITY);
+    }
+  }
+}
+
+struct SelPart {   // of a stretch: its largest logit m, the sum of exp(z - m)
+  float m, s;
+};
+
+// A stretch is `length` groups of a row, `per_row` stretches and `groups` groups a row.
+template <typename T>
+__global__ void __launch_bounds__(kBeamThreads, sizeof(T) == 4 ? 4 : 6)
+beam_scan_kernel(const T* __restrict__ logits, int64_t stride, int rows, int vocab, int groups, int per_row, int length, SelPart* __restrict__ parts,
+                 float* __restrict__ largest) {
+  constexpr int E = SelRow<T>::E, NV = SelRow<T>::NV, kRing = SelRow<T>::kRing;
+  __shared__ uint4 ring[kBeamThreads / 32][kRing][NV * 32];
   ptx::griddep_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t self = static_cast<int64_t>(blockIdx.x) * (kBeamThreads / 32) + warp;
+  if (self >= static_cast<int64_t>(rows) * per_row) return;
+  const int row = static_cast<int>(self / per_row), g0 = static_cast<int>(self % per_row) * length, g1 = min(groups, g0 + length);
+  const T* z = logits + row * stride;
+  const int lead = static_cast<int>((reinterpret_cast<uintptr_t>(z) & 15) / sizeof(T));
+  int ahead = g0, put = 0;
+  auto load = [&]() {
+    if (ahead < g1) {
+      const int first = ahead * kSelGroup - lead, at = first + lane * E;
+      uint4* to = &ring[warp][put][lane];
+      if (first >= 0 && first + kSelGroup <= vocab) {
 #pragma unroll
-  for (int j = 0; j < kSelVectors; ++j) {
-    const int at = first + j * kBeamThreads * E;
-    if (at >= 0 && at + E <= vocab) {
-      ptx::cp_async_16(ptx::smem_u32(&data[j * kBeamThreads + tid]), z + at, 16);
-    } else {
-      T* piece = reinterpret_cast<T*>(&data[j * kBeamThreads + tid]);
-      for (int e = 0; e < E; ++e) {
-        if (at + e >= 0 && at + e < vocab) piece[e] = z[at + e];
-        else stf(&piece[e], -INFINITY);
+        for (int j = 0; j < NV; ++j) ptx::cp_async_16(ptx::smem_u32(to + j * 32), z + at + j * 32 * E, 16);
+      } else {
+#pragma unroll 1
+        for (int j = 0; j < NV; ++j) sel_piece(to + j * 32, z, at + j * 32 * E, vocab);
       }
     }
-  }
-  ptx::cp_async_commit();
-  ptx::cp_async_wait<0>();        // (a thread reads what it has copied itself)
-  float largest[kSelVectors], mine = -INFINITY;      // of each piece
-#pragma unroll
-  for (int j = 0; j < kSelVectors; ++j) {
-    largest[j] = sel_max<T>(data[j * kBeamThreads + tid]);
-    mine = fmaxf(mine, largest[j]);
-  }
-  // groups: 32, 64 or 128 of them, at least twice n
-  const int groups = n <= 16 ? 32 : n <= 32 ? 64 : 128, width = kBeamThreads / groups;
-  float g = mine;
-  for (int d = 1; d < width; d <<= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, d));
-  if ((tid & (width - 1)) == 0) top[tid / width] = g;
-  const float w = warp_max(mine);
-  if (lane == 0) warp_top[warp] = w;
-  __syncthreads();
-  float m = warp_top[0];
-#pragma unroll
-  for (int i = 1; i < kBeamThreads / 32; ++i) m = fmaxf(m, warp_top[i]);
-  if (tid < groups) {
-    const float v = top[tid];
-    int above = 0;
-    for (int i = 0; i < groups; i += 4) {
-      const float4 o = *reinterpret_cast<const float4*>(&top[i]);
-      above += (o.x > v || (o.x == v && i < tid)) + (o.y > v || (o.y == v && i + 1 < tid)) + (o.z > v || (o.z == v && i + 2 < tid)) +
-               (o.w > v || (o.w == v && i + 3 < tid));
-    }
-    if (above == n - 1) bound = v;
-  }
-  __syncthreads();
-  const float least = bound;
-  const bool huge = fabsf(m) > kSelHuge && m > -INFINITY;
-  const float c = m > -INFINITY ? m * kLog2e : 0.f;    // (a chunk of minus infinities: its sum is 0)
-  auto key = [](int at, float x) { return static_cast<uint64_t>(sel_ordered(x)) << 32 | (0xffffffffu - static_cast<uint32_t>(at)); };
-#pragma unroll
-  for (int j = 0; j < kSelVectors; ++j)
-    if (largest[j] >= least && largest[j] > -INFINITY) pieces[atomicAdd(&passed, 1)] = static_cast<uint16_t>(j * kBeamThreads + tid);
-  float sum = 0.f;
-#pragma unroll
-  for (int j = 0; j < kSelVectors; ++j) {
-    float f[E];
-    sel_unpack<T>(data[j * kBeamThreads + tid], f);
-    float part = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) part += ptx::ex2_approx(fmaf(f[e], kLog2e, -c));
-    sum += part;
-  }
-  if (huge) {
-    sum = 0.f;
+    ptx::cp_async_commit();
+    ++ahead;
+    if (++put == kRing) put = 0;
+  };
 #pragma unroll 1
-    for (int i = 0; i < kSelVectors * E; ++i)
-      sum += ptx::ex2_approx((ldf(reinterpret_cast<const T*>(&data[i / E * kBeamThreads + tid]) + i % E) - m) * kLog2e);
+  for (int i = 0; i < kRing - 1; ++i) load();
+  constexpr float kLog2e = 1.4426950408889634f;
+  const uint64_t log2e = ptx::f32x2(kLog2e, kLog2e);
+  float m = -INFINITY, sum = 0.f;       // (of the warp; of the lane)
+  int get = 0;
+#pragma unroll 1
+  for (int g = g0; g < g1; ++g) {
+    load();
+    ptx::cp_async_wait<kRing - 1>();      // (a lane reads what it has copied itself)
+    uint4 cur[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) cur[j] = ring[warp][get][j * 32 + lane];
+    if (++get == kRing) get = 0;
+    float top = sel_max<T>(cur[0]);
+#pragma unroll
+    for (int j = 1; j < NV; ++j) top = fmaxf(top, sel_max<T>(cur[j]));
+    top = sel_number(__reduce_max_sync(0xffffffffu, sel_ordered(top)));
+    if (lane == 0) largest[static_cast<int64_t>(row) * groups + g] = top;
+    if (top > m) {
+      sum *= ptx::ex2_approx((m - top) * kLog2e);
+      m = top;
+    }
+    const float ref = m > -INFINITY ? -m : 0.f;      // (nothing but minus infinities: they add nothing, and a NaN stays one)
+    const uint64_t back = ptx::f32x2(ref, ref);
+    uint64_t part = 0;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      float f[E];
+      sel_unpack<T>(cur[j], f);
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {
+        const float2 x = ptx::f32x2_get(ptx::mul_f32x2(ptx::add_f32x2(ptx::f32x2(f[e], f[e + 1]), back), log2e));
+        part = ptx::add_f32x2(part, ptx::f32x2(ptx::ex2_approx(x.x), ptx::ex2_approx(x.y)));
+      }
+    }
+    const float2 two = ptx::f32x2_get(part);
+    sum += two.x + two.y;
   }
+  // (not before: blocks of the next kernel that wait beside those of a scan took a quarter of its rate)
+  ptx::griddep_launch_dependents();
   sum = warp_sum(sum);
-  if (lane == 0) warp_sum_[warp] = sum;
-  __syncthreads();
-  // candidates: numbers of those pieces from the bound on.  Where there are too many (equal numbers, or large ones of few groups) the bound is
-  // moved up by halves until there is room for them.  (Keys differ from one another, so some bound lets n to kSelRoom through.)
-  uint64_t lo = 0, hi = ~0ull, mid = key(0x7fffffff, least);
-  int count;
-  for (int turn = 0;; ++turn) {
-#pragma unroll 1
-    for (int i = tid; i < passed * E; i += kBeamThreads) {
-      const int piece = pieces[i / E], e = i % E;
-      const uint64_t k = key(chunk * SelRow<T>::kChunk + piece * E - lead + e, ldf(reinterpret_cast<const T*>(&data[piece]) + e));
-      if (k >= mid && k >> 32) {
-        const int at = atomicAdd(&found, 1);
-        if (at < kSelRoom) cand[at] = k;
-      }
-    }
-    __syncthreads();
-    count = found;
-    if (count <= kSelRoom && (count >= n || turn == 0)) break;
-    if (turn > 64) break;      // (not reached)
-    (count > kSelRoom ? lo : hi) = mid;
-    mid = lo + (hi - lo) / 2;
-    __syncthreads();
-    if (tid == 0) found = 0;
-    __syncthreads();
-  }
-  count = min(count, kSelRoom);
-  uint64_t* out = keys + static_cast<int64_t>(blockIdx.x) * n;
-  for (int i = tid; i < count; i += kBeamThreads) {
-    const uint64_t mykey = cand[i];
-    int above = 0;
-    for (int k = 0; k < count; ++k) above += cand[k] > mykey;
-    if (above < n) out[above] = mykey;
-  }
-  if (tid >= count && tid < n) out[tid] = 0;
-  if (tid == 0) {
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < kBeamThreads / 32; ++i) s += warp_sum_[i];
-    parts[blockIdx.x] = SelPart{m, c, s, huge ? 1.f : 0.f};
-  }
+  if (lane == 0) parts[self] = SelPart{m, sum};
 }
 
 struct SelOut {
   float* score;
   int32_t *parent, *token;
 };
-// A candidate: its value as 64 bits in the order of the numbers (0: none), its beam and token.  (Comparisons of doubles took half the kernel's time.)
+// A value (two fp32 in the order of their bits, the larger first; 0: none), and behind it its place, the bits turned: of equal values the lowest place comes
+// first.  Together one number of 128 bits, the larger the better.
 struct SelCand {
-  uint64_t v, place;
+  uint64_t v, early;
 };
-__device__ __forceinline__ bool sel_before(const SelCand& a, const SelCand& b) { return a.v > b.v || (a.v == b.v && a.place < b.place); }
-__device__ __forceinline__ float sel_value(const SelCand& a) {
-  return static_cast<float>(__longlong_as_double(static_cast<long long>(a.v ^ (a.v >> 63 ? 1ull << 63 : ~0ull))));
+__device__ __forceinline__ SelCand sel_cand(uint64_t v, uint64_t place) { return SelCand{v, ~place}; }
+// 1 if a comes before b.  (The borrow of b - a: a comparison with branches takes each lane by itself where values are equal, 250 cycles instead of 10.)
+__device__ __forceinline__ uint32_t sel_before(const SelCand& a, const SelCand& b) {
+  uint32_t less;
+  asm("{\n\t.reg .u32 t;\n\t"
+      "sub.cc.u32 t, %1, %5;\n\tsubc.cc.u32 t, %2, %6;\n\tsubc.cc.u32 t, %3, %7;\n\tsubc.cc.u32 t, %4, %8;\n\tsubc.u32 %0, 0, 0;\n\t}"
+      : "=r"(less)
+      : "r"(static_cast<uint32_t>(b.early)), "r"(static_cast<uint32_t>(b.early >> 32)), "r"(static_cast<uint32_t>(b.v)), "r"(static_cast<uint32_t>(b.v >> 32)),
+        "r"(static_cast<uint32_t>(a.early)), "r"(static_cast<uint32_t>(a.early >> 32)), "r"(static_cast<uint32_t>(a.v)), "r"(static_cast<uint32_t>(a.v >> 32)));
+  return -less;
+}
+__device__ __forceinline__ float sel_value(const SelCand& a) { return sel_number(static_cast<uint32_t>(a.v >> 32)); }
+// a + b as the rounded sum and what the rounding left out
+__device__ __forceinline__ float2 two_sum(float a, float b) {
+  const float s = __fadd_rn(a, b), t = __fadd_rn(s, -a);
+  return make_float2(s, __fadd_rn(__fadd_rn(a, -__fadd_rn(s, -t)), __fadd_rn(b, -t)));
+}
+// base + (z - norm), norm = hi + lo.  What is no number, or minus infinity, is no candidate.
+__device__ __forceinline__ uint64_t sel_make(float z, float base, float2 norm) {
+  const float2 d = two_sum(z, -norm.x), v = two_sum(d.x, base);
+  const float rest = __fadd_rn(__fadd_rn(d.y, -norm.y), v.y), hi = __fadd_rn(v.x, rest), lo = __fadd_rn(rest, -__fadd_rn(hi, -v.x));
+  const uint32_t o = sel_ordered(hi);
+  return o ? static_cast<uint64_t>(o) << 32 | sel_ordered(lo) : 0ull;
 }
 
-// A block per request: of the chunks' candidates the n best, by a bound as in the scan.  Neighbouring candidates of a list are in different groups, so that lists
-// that have most of the best ones do not let more through.  (An earlier form took heads of the lists one after the other: 20 us for n = 24.)
-constexpr int kSelListRoom = 8192;      // keys that wait in shared memory, where they are no more
-constexpr int kSelBestRoom = 1024;
+constexpr int kSelRoom = 1024;       // candidates in shared memory
+constexpr int kSelBounds = 128;      // numbers of which the n-th largest is the first bound
+
+// The n best of what `each` goes through, in order, into best[n]; `bound`: a candidate that at least n are not behind ({0, 0}: none known).  each(take) calls take(c) for
+// all that may count, by all threads of the block.  Where there is no room for those that pass the bound, the n-th best of those that found room is the next bound.
+template <typename Each>
+__device__ __forceinline__ void sel_best(int n, SelCand bound, SelCand* cand, SelCand* best, int* found, const Each& each) {
+  const int tid = threadIdx.x;
+  while (true) {
+    if (tid == 0) *found = 0;
+    if (tid < n) best[tid] = SelCand{0, 0};
+    __syncthreads();
+    each([&](const SelCand& c) {
+      if (c.v && !sel_before(bound, c)) {
+        const int at = atomicAdd(found, 1);
+        if (at < kSelRoom) cand[at] = c;
+      }
+    });
+    __syncthreads();
+    const int total = *found, count = min(total, kSelRoom);
+    for (int i = tid; i < count; i += kBeamThreads) {
+      const SelCand c = cand[i];
+      int above = 0;
+#pragma unroll 4
+      for (int k = 0; k < count; ++k) above += sel_before(cand[k], c);
+      if (above < n) best[above] = c;
+    }
+    __syncthreads();
+    if (total <= kSelRoom) return;
+    bound = best[n - 1];
+    __syncthreads();
+  }
+}
+
+template <typename T>
 __global__ void __launch_bounds__(kBeamThreads)
-beam_merge_kernel(const SelPart* __restrict__ parts, const uint64_t* __restrict__ keys, const float* __restrict__ scores, int beams, int chunks, int n,
-                  int keep, const int32_t* __restrict__ ended, int num_ended, SelOut all, SelOut next) {
-  constexpr int kWarps = kBeamThreads / 32;
-  extern __shared__ __align__(16) uint64_t held[];
-  __shared__ __align__(16) uint64_t top[kBeamThreads];
-  __shared__ SelCand cand[kSelBestRoom], best[kBeamMost];
-  __shared__ double norm[kBeamMost], base[kBeamMost];
-  __shared__ uint64_t bound;
-  __shared__ int found;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, num = beams * chunks * n;
+beam_pick_kernel(const T* __restrict__ logits, int64_t stride, int vocab, int groups, int per_row, const SelPart* __restrict__ parts,
+                 const float* __restrict__ largest, const float* __restrict__ scores, int beams, int n, int keep, const int32_t* __restrict__ ended,
+                 int num_ended, SelOut all, SelOut next) {
+  constexpr int kWarps = kBeamThreads / 32, kAhead = 8;
+  extern __shared__ __align__(16) uint4 held[];      // elements of the n best groups
+  __shared__ SelCand cand[kSelRoom], best[kBeamMost], tops[kSelBounds];
+  __shared__ float2 norm[kBeamMost];
+  __shared__ float base[kBeamMost], low[kBeamMost];
+  __shared__ int from[kBeamMost], first[kBeamMost], found, hits;
+  __shared__ uint16_t hit[kSelRoom];
+  __shared__ SelCand bound;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, num = beams * groups;
   const int64_t q = blockIdx.x;
-  parts += q * beams * chunks;
-  keys += q * num;
-  const bool in_shared = num <= kSelListRoom;
-  if (tid == 0) found = 0;
-  if (tid < n) best[tid] = SelCand{0, ~0ull};
+  if (tid == 0) hits = 0;
+  parts += q * beams * per_row;
+  largest += q * num;
   ptx::griddep_launch_dependents();
   ptx::griddep_wait();
-  if (in_shared) {
-#pragma unroll 8
-    for (int i = tid; i < num; i += kBeamThreads) held[i] = keys[i];
-  }
+  float ahead[kAhead];       // (on their way while the sums are added up)
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k) ahead[k] = tid + k * kBeamThreads < num ? largest[tid + k * kBeamThreads] : -INFINITY;
   for (int b = warp; b < beams; b += kWarps) {
-    const SelPart* row = parts + b * chunks;
+    const SelPart* row = parts + b * per_row;
     const float score = scores[q * beams + b];
-    const SelPart one = lane < chunks ? row[lane] : SelPart{-INFINITY, 0.f, 0.f, 0.f};
-    float m = one.m;
-    for (int i = lane + 32; i < chunks; i += 32) m = fmaxf(m, row[i].m);
+    SelPart some[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) some[k] = lane + 32 * k < per_row ? row[lane + 32 * k] : SelPart{-INFINITY, 0.f};
+    float m = some[0].m, s = 0.f;
+#pragma unroll
+    for (int k = 1; k < kAhead; ++k) m = fmaxf(m, some[k].m);
+    for (int i = lane + 32 * kAhead; i < per_row; i += 32) m = fmaxf(m, row[i].m);
     m = warp_max(m);
-    // sum of exp(z - m): of a chunk, s exp(c ln 2 - m) exp(-d m'), L ln 2 = 1 + d, m' its largest
-    constexpr double kLn2 = 0.69314718055994531, kD = static_cast<double>(kLog2e) * kLn2 - 1.0;
-    auto share = [&](const SelPart& x) {
-      if (!(x.m > -INFINITY)) return x.s;      // (0, or NaN)
-      return x.s * (x.far != 0.f ? expf(x.m - m) : expf(static_cast<float>(x.c * kLn2 - m - kD * x.m)));
-    };
-    float s = share(one);
-    for (int i = lane + 32; i < chunks; i += 32) s += share(row[i]);
+    auto share = [&](const SelPart& x) { return x.s * (x.m > -INFINITY ? ptx::ex2_approx((x.m - m) * 1.4426950408889634f) : 1.f); };      // (1: 0 and NaN stay)
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) s += share(some[k]);
+    for (int i = lane + 32 * kAhead; i < per_row; i += 32) s += share(row[i]);
     s = warp_sum(s);
     if (lane == 0) {
       // log s = log f + e log 2 with f from 1 to 2: in fp32 off by 2^-24, where log s would be by 2^-21
       int e = 1;
       const bool number = s > 0.f && s < INFINITY;
       const float f = number ? 2.f * frexpf(s, &e) : s;
-      norm[b] = static_cast<double>(m) + (static_cast<double>(logf(f)) + (e - 1) * kLn2);
+      const double x = static_cast<double>(m) + (static_cast<double>(logf(f)) + (e - 1) * 0.69314718055994531);
+      const float hi = static_cast<float>(x);
+      norm[b] = make_float2(hi, static_cast<float>(x - hi));      // (an infinity: NaN)
       base[b] = score;
     }
   }
   __syncthreads();
-  auto made = [&](int i) {
-    const uint64_t k = in_shared ? held[i] : keys[i];
-    if (k == 0) return SelCand{0, ~0ull};
-    const int b = i / (chunks * n);
-    const double v = base[b] + (static_cast<double>(sel_number(static_cast<uint32_t>(k >> 32))) - norm[b]) + 0.0;      // (-0 as 0)
-    const uint64_t u = static_cast<uint64_t>(__double_as_longlong(v));
-    // (what is no number is no candidate)
-    return v > -INFINITY ? SelCand{u ^ (u >> 63 ? ~0ull : 1ull << 63), static_cast<uint64_t>(b) << 32 | (0xffffffffu - static_cast<uint32_t>(k))} : SelCand{0, ~0ull};
+  auto group = [&](int i, float z) {
+    const int b = min(i / groups, beams - 1);
+    return sel_cand(sel_make(z, base[b], norm[b]), i);
   };
-  uint64_t mine = 0;
-#pragma unroll 4
-  for (int i = tid; i < num; i += kBeamThreads) mine = max(mine, made(i).v);
-  top[tid] = mine;
-  __syncthreads();
-  const int groups = n <= 32 ? 64 : 128;
-  if (tid < groups) {
-    for (int i = tid + groups; i < kBeamThreads; i += groups) mine = max(mine, top[i]);
-    top[tid] = mine;
+  // A first bound: of the largest of pairs of threads the n-th.
+  SelCand mine{0, static_cast<uint64_t>(tid)};       // (each none another one)
+  uint64_t mine_v[kAhead];
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k) {
+    const SelCand c = group(tid + k * kBeamThreads, ahead[k]);
+    mine_v[k] = c.v;
+    if (c.v > mine.v) mine = c;       // (places rise)
   }
-  __syncthreads();
-  if (tid < groups) {
+  for (int i = tid + kAhead * kBeamThreads; i < num; i += kBeamThreads) {
+    const SelCand c = group(i, largest[i]);
+    if (c.v > mine.v) mine = c;
+  }
+  {
+    const SelCand other{__shfl_xor_sync(0xffffffffu, mine.v, 1), __shfl_xor_sync(0xffffffffu, mine.early, 1)};
+    if (sel_before(other, mine)) mine = other;
+    if ((tid & 1) == 0) tops[tid >> 1] = mine;
+    __syncthreads();
     int above = 0;
 #pragma unroll 8
-    for (int i = 0; i < groups; ++i) above += top[i] > mine || (top[i] == mine && i < tid);
+    for (int i = 0; i < kSelBounds / 2; ++i) above += sel_before(tops[2 * i + (tid & 1)], mine);
+    above += __shfl_xor_sync(0xffffffffu, above, 1);
     if (above == n - 1) bound = mine;
+    __syncthreads();
+  }
+  sel_best(n, bound, cand, best, &found, [&](auto&& take) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) take(sel_cand(mine_v[k], tid + k * kBeamThreads));
+    for (int i = tid + kAhead * kBeamThreads; i < num; i += kBeamThreads) take(group(i, largest[i]));
+  });
+  // The n best elements are in these groups: one in any other group has their largest elements before it.  Those that reach the bound are in few pieces, which are
+  // shared out by elements.
+  constexpr int E = SelRow<T>::E, kPieces = 32 * SelRow<T>::NV;
+  if (tid < n) {
+    const int f = best[tid].v ? static_cast<int>(~best[tid].early) : -1, b = f < 0 ? -1 : f / groups;
+    from[tid] = b;
+    if (f >= 0) first[tid] = (f - b * groups) * kSelGroup - static_cast<int>((reinterpret_cast<uintptr_t>(logits + (q * beams + b) * stride) & 15) / sizeof(T));
+  }
+  const SelCand least = best[n - 1].v ? SelCand{best[n - 1].v, 0} : SelCand{0, 0};
+  if (tid < beams) {       // a row's logits below this one are worth less than the bound
+    const float v = sel_value(least), x = v - base[tid] + norm[tid].x, y = x - 1e-6f * (fabsf(v) + fabsf(base[tid]) + fabsf(norm[tid].x));
+    low[tid] = least.v && y > -INFINITY ? y : -INFINITY;
   }
   __syncthreads();
-  const uint64_t least = bound > 0 ? bound : 1;
-#pragma unroll 4
-  for (int i = tid; i < num; i += kBeamThreads) {
-    const SelCand e = made(i);
-    if (e.v >= least) {
-      const int at = atomicAdd(&found, 1);
-      if (at < kSelBestRoom) cand[at] = e;
+#pragma unroll 2
+  for (int i = tid; i < n * kPieces; i += kBeamThreads) {
+    const int b = from[i / kPieces], at = first[i / kPieces] + i % kPieces * E;
+    if (b < 0) break;
+    const T* z = logits + (q * beams + b) * stride;
+    sel_piece(&held[i], z, at, vocab);
+  }
+  ptx::cp_async_commit();
+  ptx::cp_async_wait<0>();      // (a thread looks at what it has copied itself, until the next barrier)
+#pragma unroll 2
+  for (int i = tid; i < n * kPieces; i += kBeamThreads) {
+    const int b = from[i / kPieces];
+    if (b < 0) break;
+    if (sel_max<T>(held[i]) >= low[b]) {
+      const int at = atomicAdd(&hits, 1);
+      if (at < kSelRoom) hit[at] = static_cast<uint16_t>(i);
     }
   }
   __syncthreads();
-  const int count = found;
-  if (count <= kSelBestRoom) {
-    for (int i = tid; i < count; i += kBeamThreads) {
-      const SelCand e = cand[i];
-      int above = 0;
-#pragma unroll 4
-      for (int k = 0; k < count; ++k) above += sel_before(cand[k], e);
-      if (above < n) best[above] = e;
+  sel_best(n, least, cand, best, &found, [&](auto&& take) {
+    const bool few = hits <= kSelRoom;
+#pragma unroll 1
+    for (int t = tid; t < (few ? hits : n * kPieces) * E; t += kBeamThreads) {
+      const int i = few ? hit[t / E] : t / E, b = from[i / kPieces];
+      if (b < 0) break;
+      const float y = ldf(reinterpret_cast<const T*>(&held[i]) + t % E);
+      if (y >= low[b]) take(sel_cand(sel_make(y, base[b], norm[b]), static_cast<uint64_t>(b) << 32 | static_cast<uint32_t>(first[i / kPieces] + i % kPieces * E + t % E)));
     }
-  } else {
-    // many equal values: one after the other, the best of those behind the last one
-    SelCand last{~0ull, 0};
-    for (int j = 0; j < n; ++j) {
-      SelCand first{0, ~0ull};
-      for (int i = tid; i < num; i += kBeamThreads) {
-        const SelCand e = made(i);
-        if (e.v && sel_before(last, e) && sel_before(e, first)) first = e;
-      }
-      __syncthreads();
-      cand[tid] = first;
-      __syncthreads();
-      for (int i = 0; i < kBeamThreads; ++i)
-        if (sel_before(cand[i], first)) first = cand[i];
-      if (tid == 0) best[j] = first;
-      last = first;
-      if (first.v == 0) break;
-    }
-  }
-  __syncthreads();
+  });
   if (warp > 0) return;
   auto give = [](const SelOut& to, int64_t at, const SelCand& e) {
     to.score[at] = e.v ? sel_value(e) : -INFINITY;
-    to.parent[at] = e.v ? static_cast<int32_t>(e.place >> 32) : -1;
-    to.token[at] = e.v ? static_cast<int32_t>(e.place) : -1;
+    to.parent[at] = e.v ? static_cast<int32_t>(~e.early >> 32) : -1;
+    to.token[at] = e.v ? static_cast<int32_t>(~e.early) : -1;
   };
   int before = 0;
   for (int i0 = 0; i0 < n; i0 += 32) {
     const int i = i0 + lane;
     if (i < n) give(all, q * n + i, best[i]);
     bool on = i < n && best[i].v != 0;
-    for (int e = 0; on && e < num_ended; ++e) on = ended[e] != static_cast<int32_t>(best[i].place);
+    for (int e = 0; on && e < num_ended; ++e) on = ended[e] != static_cast<int32_t>(~best[i].early);
     const unsigned who = __ballot_sync(0xffffffffu, on);
     const int at = before + __popc(who & ((1u << lane) - 1));
     if (on && at < keep) give(next, q * keep + at, best[i]);
     before += __popc(who);
   }
-  for (int i = before + lane; i < keep; i += 32) give(next, q * keep + i, SelCand{0, ~0ull});
+  for (int i = before + lane; i < keep; i += 32) give(next, q * keep + i, SelCand{0, 0});
 }
 
 // ------------------------------------------------------------------ tables of the beams that go on
@@ -654,20 +670,28 @@ __global__ void __launch_bounds__(kBeamThreads) step_tables_kernel(const TablePa
   }
 }
 
+// How a selection's rows are cut: groups and stretches of a row, groups of a stretch.
+struct SelPlan {
+  int groups, per_row, length;
+  int64_t largest, bytes;       // where the groups' largest are in the scratch, its size
+  SelPlan(int64_t rows, int vocab, int dtype) {
+    // (a row may begin behind a 16-byte boundary: up to 7 elements more)
+    groups = static_cast<int>((static_cast<int64_t>(vocab) + (dtype == 2 ? 3 : 7) + kSelGroup - 1) / kSelGroup);
+    const int64_t warps = static_cast<int64_t>(kSelWarps) * device_sm_count() / (rows < 1 ? 1 : rows);
+    length = warps < 1 ? kSelStretch : static_cast<int>((groups + warps - 1) / warps);
+    if (length > kSelStretch) length = kSelStretch;
+    per_row = (groups + length - 1) / length;
+    largest = (8 * rows * per_row + 255) / 256 * 256;
+    bytes = largest + 4 * rows * groups;
+  }
+};
+
 }  // namespace blitz
 
 extern "C" {
 using namespace blitz;
 
-static int beam_chunks(int vocab, int dtype) {
-  // (a row may begin behind a 16-byte boundary: up to 7 elements more)
-  const int chunk = dtype == 2 ? SelRow<float>::kChunk : SelRow<__half>::kChunk, lead = dtype == 2 ? 3 : 7;
-  return (vocab + lead + chunk - 1) / chunk;
-}
-
-int64_t blitz_beam_select_workspace_bytes(int rows, int vocab, int n, int dtype) {
-  return static_cast<int64_t>(rows) * beam_chunks(vocab, dtype) * (static_cast<int64_t>(sizeof(SelPart)) + 8 * n);
-}
+int64_t blitz_beam_select_workspace_bytes(int rows, int vocab, int n, int dtype) { return SelPlan(rows, vocab, dtype).bytes; }
 
 // logits [rows][stride] in fp16 (0), bf16 (1) or fp32 (2); scores [rows]; a request's beams are consecutive rows.  score, parent and token:
 // [rows / beams][n], next_*: [rows / beams][keep].  ended: tokens that end a sequence (num_ended of them).
@@ -676,21 +700,24 @@ int blitz_beam_select(const void* logits, int64_t stride, const float* scores, i
                       int32_t* next_token, int dtype, cudaStream_t stream) {
   if (rows <= 0) return 0;
   if (vocab < 1 || beams < 1 || beams > kBeamMost || rows % beams || n < 1 || n > kBeamMost || keep < 1 || keep > n || num_ended < 0) return -1;
-  const int chunks = beam_chunks(vocab, dtype);
-  if (static_cast<int64_t>(rows) * chunks > 0x7fffffff) return -1;
+  const SelPlan plan(rows, vocab, dtype);
+  const int64_t blocks = (static_cast<int64_t>(rows) * plan.per_row + kBeamThreads / 32 - 1) / (kBeamThreads / 32);
+  if (blocks > 0x7fffffff || static_cast<int64_t>(beams) * plan.groups > 0x7fffffff || vocab > 0x7fffffff - 2 * kSelGroup) return -1;
   SelPart* parts = reinterpret_cast<SelPart*>(workspace);
-  uint64_t* keys = reinterpret_cast<uint64_t*>(parts + static_cast<int64_t>(rows) * chunks);
+  float* largest = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + plan.largest);
   cudaError_t e = cudaSuccess;
-  BLITZ_DISPATCH_DTYPE3(dtype, (e = launch_pdl(beam_scan_kernel<T>, dim3(rows * chunks), dim3(kBeamThreads), 0, stream, (const T*)logits, stride, vocab, chunks, n,
-                                               parts, keys)));
-  if (e != cudaSuccess) return (int)e;
-  const int64_t num = static_cast<int64_t>(beams) * chunks * n;
-  if (num > 0x7fffffff) return -1;
-  static PerDeviceOnce once;
-  e = once.run([] { return cudaFuncSetAttribute(beam_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 8 * kSelListRoom); });
-  if (e != cudaSuccess) return (int)e;
-  return (int)launch_pdl(beam_merge_kernel, dim3(rows / beams), dim3(kBeamThreads), num <= kSelListRoom ? 8 * (size_t)num : 0, stream, parts, keys, scores, beams, chunks, n, keep, ended, num_ended,
-                         SelOut{score, parent, token}, SelOut{next_score, next_parent, next_token});
+  BLITZ_DISPATCH_DTYPE3(dtype, {
+    e = launch_pdl(beam_scan_kernel<T>, dim3((unsigned)blocks), dim3(kBeamThreads), 0, stream, (const T*)logits, stride, rows, vocab, plan.groups, plan.per_row,
+                   plan.length, parts, largest);
+    static PerDeviceOnce once;
+    if (e == cudaSuccess)
+      e = once.run([] { return cudaFuncSetAttribute(beam_pick_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBeamMost * kSelGroup * (int)sizeof(T)); });
+    if (e == cudaSuccess)
+      e = launch_pdl(beam_pick_kernel<T>, dim3(rows / beams), dim3(kBeamThreads), n * kSelGroup * sizeof(T), stream, (const T*)logits, stride, vocab, plan.groups, plan.per_row,
+                     (const SelPart*)parts, (const float*)largest, scores, beams, n, keep, ended, num_ended, SelOut{score, parent, token},
+                     SelOut{next_score, next_parent, next_token});
+  });
+  return (int)e;
 }
 
 // table [requests from][width], cached [requests from], parents [requests][to], pool [requests][pool_size]; the children's table
