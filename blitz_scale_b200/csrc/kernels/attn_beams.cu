@@ -40,9 +40,10 @@ struct BeamAttnParams {
   int heads;                    // virtual heads x blocks
   int ranges_most;
   int page_shift, max_pages;
-  float scale_log2, cap_scale, cap_log2;
+  float scale_log2, cap_scale, cap_log2;      // the scale's size (1 under a cap, or where it is zero); keep and flip: zero or its sign, for the queries
+  uint32_t keep, flip;
   const void* sink;
-  int* line;                    // [blocks][groups + groups per_block] steps before a segment, [+ 1] all; [rows] lengths; [blocks groups] common pages
+  int2* runs;                   // [blocks][groups + groups per_block] of each segment: its first piece's range, pieces
   float *o_common, *o_own;      // partial sums
   float2 *ml_common, *ml_own;   // maximum (log2 units) and sum of each
   int static_table;
@@ -135,8 +136,13 @@ __global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const BeamAtt
   if (!p.static_table) ptx::griddep_wait();
   ba_line(p, line, len, common, sums);
   ptx::griddep_wait();
-  if (blockIdx.x == 0)
-    for (int i = threadIdx.x; i < p.blocks * per + 1 + p.rows + p.blocks * p.groups; i += kBaThreads) p.line[i] = line[i];
+  // where each segment's pieces are, for the merge
+  for (int e = blockIdx.x + threadIdx.x * gridDim.x; e < p.blocks * per; e += gridDim.x * kBaThreads) {
+    const int* of = line + e / per * per;
+    const BaRanges ranges(of[per] - of[0], p.ranges_most);
+    const int x0 = line[e] - of[0], x1 = line[e + 1] - of[0], r = x0 < x1 ? ranges.of(x0) : 0;
+    p.runs[e] = make_int2(r, x0 < x1 ? ranges.of(x1 - 1) - r + 1 : 0);
+  }
 
   const int self = warp * gridDim.x + blockIdx.x;
   const int hv = self % p.heads, range = self / p.heads;
@@ -186,6 +192,9 @@ __global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const BeamAtt
   enter(ld);
   enter(at);
   const uint32_t ring = ptx::smem_u32(ba_smem) + warp * kStages * kStage;
+  // a lane copies 16 bytes at column lane % kPieces of every (32 / kPieces)-th token; 16-byte columns are turned by the token's number, so that ldmatrix meets no bank twice
+  const int64_t lane_at = lane / kPieces * token_pitch + lane % kPieces * 8;
+  const uint32_t ring_dst = ring + lane / kPieces * kRowBytes + (((lane % kPieces ^ lane / kPieces) & 7 | lane % kPieces & 8) << 4);
   int win = 0, win_base = -64;       // page ids: lane l holds entry win_base + l of the row's list
   int ld_stage = 0;
   auto load = [&]() {                // requests the next step
@@ -205,16 +214,26 @@ __global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const BeamAtt
       }
     }
     const int id = __shfl_sync(0xffffffffu, win, pg - win_base);
-    const T* k = kv + ((static_cast<int64_t>(id) << (p.page_shift + 1)) + (t0 & (page - 1))) * token_pitch;
+    const T* k = kv + ((static_cast<int64_t>(id) << (p.page_shift + 1)) + (t0 & (page - 1))) * token_pitch + lane_at;
     const T* v = k + page * token_pitch;
-    const uint32_t to = ring + ld_stage * kStage;
-    const int valid = ld.len - t0;
+    const uint32_t to = ring_dst + ld_stage * kStage;
+    constexpr int kTokens = 32 / kPieces, kTurns = kBaStep / kTokens;      // of an instruction; instructions
+    const int64_t step = kTokens * token_pitch;
+    if (ld.len - t0 >= kBaStep) {
 #pragma unroll
-    for (int i = 0; i < kBaStep * kPieces / 32; ++i) {
-      const int n = i * 32 + lane, tok = n / kPieces, c = n % kPieces;
-      const uint32_t dst = to + tok * kRowBytes + (((c ^ tok) & 7) | (c & 8)) * 16, bytes = tok < valid ? 16u : 0u;
-      ptx::cp_async_16(dst, k + (tok < valid ? tok : 0) * token_pitch + c * 8, bytes);
-      ptx::cp_async_16(dst + kBaStep * kRowBytes, v + (tok < valid ? tok : 0) * token_pitch + c * 8, bytes);
+      for (int i = 0; i < kTurns; ++i) {
+        const uint32_t dst = (to ^ (i * kTokens & 7) << 4) + i * kTokens * kRowBytes;
+        ptx::cp_async_16(dst, k + i * step, 16);
+        ptx::cp_async_16(dst + kBaStep * kRowBytes, v + i * step, 16);
+      }
+    } else {      // the row's last step: zeros behind its end, whatever the page holds there
+      const int valid = ld.len - t0 - lane / kPieces;
+#pragma unroll 1
+      for (int i = 0; i < kTurns; ++i) {
+        const uint32_t dst = (to ^ (i * kTokens & 7) << 4) + i * kTokens * kRowBytes, bytes = i * kTokens < valid ? 16u : 0u;
+        ptx::cp_async_16(dst, bytes ? k + i * step : kv, bytes);
+        ptx::cp_async_16(dst + kBaStep * kRowBytes, bytes ? v + i * step : kv, bytes);
+      }
     }
     ++ld.x;
     if (++ld_stage == kStages) ld_stage = 0;
@@ -225,6 +244,10 @@ __global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const BeamAtt
     ptx::cp_async_commit();
   }
   const int g8 = lane >> 2, t4 = lane & 3, mi = lane >> 3, mr = lane & 7;
+  // what the lane reads of a stage with ldmatrix: keys of its token from 16-byte column mi & 1 on, values of its token from column mi >> 1 on
+  const int k_tok = (mi >> 1) * 8 + mr, v_tok = (mi & 1) * 8 + mr;
+  const uint32_t k_at = ring + k_tok * kRowBytes + (((mi & 1) ^ k_tok & 7) << 4);
+  const uint32_t v_at = ring + (kBaStep + v_tok) * kRowBytes + (((mi >> 1) ^ v_tok & 7) << 4);
   int stage = 0;
   // A piece: TILES of 16 query rows.
   auto piece = [&](auto tiles) {
@@ -244,7 +267,7 @@ __global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const BeamAtt
         for (int ks = 0; ks < HD / 16; ++ks)
 #pragma unroll
           for (int hi = 0; hi < 2; ++hi)
-            qa[t][ks][half + 2 * hi] = i < live ? *reinterpret_cast<const uint32_t*>(q + ks * 16 + hi * 8 + 2 * t4) : 0u;
+            qa[t][ks][half + 2 * hi] = i < live ? *reinterpret_cast<const uint32_t*>(q + ks * 16 + hi * 8 + 2 * t4) & p.keep ^ p.flip : 0u;
       }
     float o[TILES][HD / 8][4], m[TILES][2], l[TILES][2];
 #pragma unroll
@@ -259,15 +282,13 @@ __global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const BeamAtt
       ptx::cp_async_commit();
       ptx::cp_async_wait<kStages - 1>();
       __syncwarp();
-      const uint32_t kbase = ring + stage * kStage, vbase = kbase + kBaStep * kRowBytes;
+      const uint32_t kbase = k_at + stage * kStage, vbase = v_at + stage * kStage;
       float s[TILES][2][4] = {};
       {
-        const int tok = (mi >> 1) * 8 + mr;
 #pragma unroll
         for (int ks = 0; ks < HD / 16; ++ks) {
-          const int c = ks * 2 + (mi & 1);
           uint32_t b0, b1, b2, b3;
-          ldmatrix_x4(kbase + tok * kRowBytes + (((c ^ tok) & 7) | (c & 8)) * 16, b0, b1, b2, b3);
+          ldmatrix_x4((kbase ^ (ks * 2 & 7) << 4) + (ks * 2 & 8) * 16, b0, b1, b2, b3);
 #pragma unroll
           for (int t = 0; t < TILES; ++t) {
             mma16816<T>(s[t][0], qa[t][ks][0], qa[t][ks][1], qa[t][ks][2], qa[t][ks][3], b0, b1);
@@ -276,26 +297,31 @@ __global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const BeamAtt
         }
       }
       const int valid = at.len - (at.tok0 + (at.x - at.seg_beg) * kBaStep);
+      if (p.cap_log2 > 0.f) {
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) s[t][e >> 2][e & 3] = p.cap_log2 * ptx::tanh_ex2(s[t][e >> 2][e & 3] * p.cap_scale);
+      }
+      if (valid < kBaStep) {
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if ((e >> 2) * 8 + 2 * t4 + (e & 1) >= valid) s[t][e >> 2][e & 3] = -INFINITY;
+      }
       uint32_t pa[TILES][4];
 #pragma unroll
       for (int t = 0; t < TILES; ++t) {
         float top[2] = {m[t][0], m[t][1]};
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float& x = s[t][h][e];
-            x = p.cap_log2 > 0.f ? p.cap_log2 * ptx::tanh_ex2(x * p.cap_scale) : x * p.scale_log2;
-            if (h * 8 + 2 * t4 + (e & 1) >= valid) x = -INFINITY;
-            top[e >> 1] = fmaxf(top[e >> 1], x);
-          }
-#pragma unroll
         for (int k = 0; k < 2; ++k) {
+          top[k] = ptx::fmax3(top[k], fmaxf(s[t][0][2 * k], s[t][0][2 * k + 1]), fmaxf(s[t][1][2 * k], s[t][1][2 * k + 1]));
           top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 1));
           top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 2));
         }
         if (__any_sync(0xffffffffu, top[0] > m[t][0] || top[1] > m[t][1])) {
-          const float a0 = ptx::ex2_approx(m[t][0] - top[0]), a1 = ptx::ex2_approx(m[t][1] - top[1]);
+          const float a0 = ptx::ex2_approx(m[t][0] * p.scale_log2 - top[0] * p.scale_log2), a1 = ptx::ex2_approx(m[t][1] * p.scale_log2 - top[1] * p.scale_log2);
           l[t][0] *= a0;
           l[t][1] *= a1;
 #pragma unroll
@@ -308,25 +334,24 @@ __global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const BeamAtt
           m[t][0] = top[0];
           m[t][1] = top[1];
         }
+        const float ref[2] = {-m[t][0] * p.scale_log2, -m[t][1] * p.scale_log2};
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int e = 0; e < 8; ++e) {
+          float& x = s[t][e >> 2][e & 3];
+          x = ptx::ex2_approx(fmaf(x, p.scale_log2, ref[(e >> 1) & 1]));
+        }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            s[t][h][e] = ptx::ex2_approx(s[t][h][e] - m[t][e >> 1]);
-            l[t][e >> 1] += s[t][h][e];
-          }
+        for (int k = 0; k < 2; ++k) l[t][k] += (s[t][0][2 * k] + s[t][0][2 * k + 1]) + (s[t][1][2 * k] + s[t][1][2 * k + 1]);
         pa[t][0] = pk2<T>(s[t][0][0], s[t][0][1]);
         pa[t][1] = pk2<T>(s[t][0][2], s[t][0][3]);
         pa[t][2] = pk2<T>(s[t][1][0], s[t][1][1]);
         pa[t][3] = pk2<T>(s[t][1][2], s[t][1][3]);
       }
       {
-        const int tok = (mi & 1) * 8 + mr;
 #pragma unroll
         for (int np = 0; np < HD / 16; ++np) {
-          const int c = np * 2 + (mi >> 1);
           uint32_t b0, b1, b2, b3;
-          ldmatrix_x4_trans(vbase + tok * kRowBytes + (((c ^ tok) & 7) | (c & 8)) * 16, b0, b1, b2, b3);
+          ldmatrix_x4_trans((vbase ^ (np * 2 & 7) << 4) + (np * 2 & 8) * 16, b0, b1, b2, b3);
 #pragma unroll
           for (int t = 0; t < TILES; ++t) {
             mma16816<T>(o[t][2 * np], pa[t][0], pa[t][1], pa[t][2], pa[t][3], b0, b1);
@@ -351,7 +376,7 @@ __global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const BeamAtt
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
         const int i = t * 16 + half * 8 + g8;
         if (i < live) {
-          if (t4 == 0) pml[slot + i] = make_float2(m[t][half], sum);
+          if (t4 == 0) pml[slot + i] = make_float2(m[t][half] * p.scale_log2, sum);
           float* to = po + (slot + i) * HD + 2 * t4;
 #pragma unroll
           for (int k = 0; k < HD / 8; ++k) *reinterpret_cast<float2*>(to + k * 8) = make_float2(o[t][k][2 * half], o[t][k][2 * half + 1]);
@@ -371,62 +396,91 @@ template <typename T, int HD, int WARPS>
 __global__ void __launch_bounds__(kBaThreads) attn_beams_merge_kernel(const BeamAttnParams p) {
   constexpr int kLanes = HD / 4, kTeams = WARPS * 32 / kLanes;      // lanes that hold a row of sums; teams that take every n-th piece
   ptx::griddep_launch_dependents();
-  ptx::griddep_wait();
   __shared__ float4 part[WARPS > 1 ? kTeams : 1][kLanes];
-  __shared__ float2 part_ml[WARPS > 1 ? kTeams : 1];
   const int item = WARPS > 1 ? blockIdx.x : blockIdx.x * kBaWarps + (threadIdx.x >> 5);
+  const int tid = WARPS > 1 ? threadIdx.x : threadIdx.x & 31, lane = tid & 31, team = tid / kLanes, c = tid % kLanes;
+  const int row = item / p.q_heads, qh = item - row * p.q_heads, head = qh / p.rep;
+  const int g = row / p.beams, j = row - g * p.beams, block = j / p.per_block, jb = j - block * p.per_block;
+  const int hv = head * p.blocks + block, own = g * p.per_block + jb;
+  const int2* runs = p.runs + block * p.groups * (1 + p.per_block);
+  ptx::griddep_wait();
   if (item >= p.rows * p.q_heads) return;
-  const int tid = WARPS > 1 ? threadIdx.x : threadIdx.x & 31;
-  const int row = item / p.q_heads, qh = item % p.q_heads, head = qh / p.rep;
-  const int g = row / p.beams, j = row % p.beams, block = j / p.per_block, jb = j % p.per_block;
-  const int per = p.groups * (1 + p.per_block);
-  const int* line = p.line + block * per;
-  const int base = line[0];
-  const BaRanges ranges(line[per] - base, p.ranges_most);
-  const int hv = head * p.blocks + block, team = tid / kLanes, c = tid % kLanes;
-  const int c0 = line[g] - base, c1 = line[g + 1] - base, own = p.groups + g * p.per_block + jb;
-  const int o0 = line[own] - base, o1 = line[own + 1] - base;
-  const int r0 = c0 < c1 ? ranges.of(c0) : 0, n0 = c0 < c1 ? ranges.of(c1 - 1) - r0 + 1 : 0;
-  const int r1 = o0 < o1 ? ranges.of(o0) : 0, n1 = o0 < o1 ? ranges.of(o1 - 1) - r1 + 1 : 0;
-  const bool live = p.line[p.blocks * per + 1 + row] > 0;
-  const int64_t common = (static_cast<int64_t>(hv) * (p.ranges_most + p.groups) + r0 + g) * kBaTile + jb * p.rep + qh % p.rep;
-  const int64_t mine = (static_cast<int64_t>(hv) * (p.ranges_most + p.groups * p.per_block) + r1 + own - p.groups) * p.rep + qh % p.rep;
-  float M = -INFINITY, L = 0.f;
+  const int2 c_run = runs[g], o_run = runs[p.groups + own];
+  const float snk = p.sink ? ldf(reinterpret_cast<const T*>(p.sink) + qh) * 1.4426950408889634f : -INFINITY;
+  // (a row without tokens has no own pieces and, where others of its group have tokens, must not have theirs)
+  const int pages = p.indptr[row + 1] - p.indptr[row];
+  const bool live = pages > 0 && ((pages - 1) << p.page_shift) + p.last_page_len[row] > 0;
+  const int n0 = live ? c_run.y : 0, n = live ? n0 + o_run.y : 0;
+  const int64_t common = (static_cast<int64_t>(hv) * (p.ranges_most + p.groups) + c_run.x + g) * kBaTile + jb * p.rep + qh - head * p.rep;
+  const int64_t mine = (static_cast<int64_t>(hv) * (p.ranges_most + p.groups * p.per_block) + o_run.x + own - n0) * p.rep + qh - head * p.rep;
+  auto at = [&](int i) { return i < n0 ? common + i * kBaTile : mine + static_cast<int64_t>(i) * p.rep; };
+  auto ml = [&](int i) { return (i < n0 ? p.ml_common : p.ml_own)[at(i)]; };
+  auto sums = [&](int i) { return *reinterpret_cast<const float4*>((i < n0 ? p.o_common : p.o_own) + at(i) * HD + 4 * c); };
+  // Latency bounds this kernel: as many loads as registers hold are on their way at once, sums before their weights are known.  A lane holds the
+  // maxima of every 32nd piece.
+  constexpr int kHeld = WARPS > 1 ? 5 : 1, kEarly = 8;
+  float2 held[kHeld];
+  float4 early[kEarly];
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k) held[k] = lane + 32 * k < n ? ml(lane + 32 * k) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+  for (int k = 0; k < kEarly; ++k) early[k] = team + kTeams * k < n ? sums(team + kTeams * k) : make_float4(0.f, 0.f, 0.f, 0.f);
+  float M = live ? snk : -INFINITY, L = 0.f;
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k) M = fmaxf(M, held[k].x);
+  for (int i = lane + 32 * kHeld; i < n; i += 32) M = fmaxf(M, ml(i).x);
+  M = warp_max(M);
+  const float ref = M > -INFINITY ? M : 0.f;
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k) {
+    held[k].x = ptx::ex2_approx(held[k].x - ref);
+    L += held[k].y * held[k].x;
+  }
+  for (int i = lane + 32 * kHeld; i < n; i += 32) {
+    const float2 x = ml(i);
+    L += x.y * ptx::ex2_approx(x.x - ref);
+  }
+  L = warp_sum(L) + (p.sink && live ? ptx::ex2_approx(snk - ref) : 0.f);
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto add = [&](float m, float l, const float4& x) {
-    const float top = fmaxf(M, m), a = M > -INFINITY ? ptx::ex2_approx(M - top) : 0.f, b = m > -INFINITY ? ptx::ex2_approx(m - top) : 0.f;
-    acc.x = acc.x * a + x.x * b;
-    acc.y = acc.y * a + x.y * b;
-    acc.z = acc.z * a + x.z * b;
-    acc.w = acc.w * a + x.w * b;
-    L = L * a + l * b;
-    M = top;
+  auto add = [&](const float4& x, float w) {
+    acc.x += x.x * w;
+    acc.y += x.y * w;
+    acc.z += x.z * w;
+    acc.w += x.w * w;
   };
-  if (live) {
-#pragma unroll 4
-    for (int i = team; i < n0 + n1; i += kTeams) {
-      const bool sh = i < n0;
-      const int64_t at = sh ? common + static_cast<int64_t>(i) * kBaTile : mine + static_cast<int64_t>(i - n0) * p.rep;
-      const float2 ml = (sh ? p.ml_common : p.ml_own)[at];
-      add(ml.x, ml.y, *reinterpret_cast<const float4*>((sh ? p.o_common : p.o_own) + at * HD + 4 * c));
+#pragma unroll
+  for (int k = 0; k < kEarly; ++k) {
+    static_assert(kEarly * kTeams <= 32 * kHeld, "the early pieces' maxima are held");
+    add(early[k], __shfl_sync(0xffffffffu, held[kTeams * k / 32].x, (team + kTeams * k) & 31));
+  }
+  for (int i0 = team + kTeams * kEarly; i0 < n; i0 += kTeams * kEarly) {
+    float top[kEarly];
+#pragma unroll
+    for (int k = 0; k < kEarly; ++k) {
+      const bool in = i0 + kTeams * k < n;
+      top[k] = in ? ml(i0 + kTeams * k).x : -INFINITY;
+      early[k] = in ? sums(i0 + kTeams * k) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
+#pragma unroll
+    for (int k = 0; k < kEarly; ++k) add(early[k], ptx::ex2_approx(top[k] - ref));
   }
   if constexpr (WARPS > 1) {
     part[team][c] = acc;
-    if (c == 0) part_ml[team] = make_float2(M, L);
     __syncthreads();
     if (team > 0) return;
-    for (int i = 1; i < kTeams; ++i) add(part_ml[i].x, part_ml[i].y, part[i][c]);
+    for (int i = 1; i < kTeams; ++i) {
+      const float4 x = part[i][c];
+      acc.x += x.x;
+      acc.y += x.y;
+      acc.z += x.z;
+      acc.w += x.w;
+    }
   } else if constexpr (kTeams > 1) {     // (two halves of a warp)
-    const float4 x = make_float4(__shfl_xor_sync(0xffffffffu, acc.x, 16), __shfl_xor_sync(0xffffffffu, acc.y, 16), __shfl_xor_sync(0xffffffffu, acc.z, 16),
-                                 __shfl_xor_sync(0xffffffffu, acc.w, 16));
-    const float m = __shfl_xor_sync(0xffffffffu, M, 16), l = __shfl_xor_sync(0xffffffffu, L, 16);
+    acc.x += __shfl_xor_sync(0xffffffffu, acc.x, 16);
+    acc.y += __shfl_xor_sync(0xffffffffu, acc.y, 16);
+    acc.z += __shfl_xor_sync(0xffffffffu, acc.z, 16);
+    acc.w += __shfl_xor_sync(0xffffffffu, acc.w, 16);
     if (team > 0) return;
-    add(m, l, x);
-  }
-  if (p.sink && live) {
-    const float s = ldf(reinterpret_cast<const T*>(p.sink) + qh) * 1.4426950408889634f;
-    add(s, 1.f, make_float4(0.f, 0.f, 0.f, 0.f));
   }
   const float f = L > 0.f ? 1.f / L : 0.f;
   stf4(reinterpret_cast<T*>(p.out) + row * p.out_stride + static_cast<int64_t>(qh) * HD + 4 * c, make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
@@ -435,7 +489,7 @@ __global__ void __launch_bounds__(kBaThreads) attn_beams_merge_kernel(const Beam
 // How a call is divided, and its scratch.
 struct BaPlan {
   int rep, kv_div, per_block, blocks, heads, ranges, rows;       // rows: of a launch
-  int64_t line, ml_common, ml_own, o_common, o_own, bytes;       // offsets
+  int64_t runs, ml_common, ml_own, o_common, o_own, bytes;       // offsets
 };
 static BaPlan ba_plan(int rows, int beams, int q_heads, int kv_heads, int hd) {
   BaPlan b;
@@ -454,8 +508,8 @@ static BaPlan ba_plan(int rows, int beams, int q_heads, int kv_heads, int hd) {
   if (b.rows > rows) b.rows = rows;
   const int64_t groups = b.rows / beams, n_common = b.heads * (b.ranges + groups) * kBaTile, n_own = b.heads * (b.ranges + groups * b.per_block) * b.rep;
   auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
-  b.line = 0;
-  b.ml_common = up(4 * (b.blocks * groups * (1 + b.per_block) + 1 + b.rows + b.blocks * groups));
+  b.runs = 0;
+  b.ml_common = up(8 * b.blocks * groups * (1 + b.per_block));
   b.ml_own = b.ml_common + up(8 * n_common);
   b.o_common = b.ml_own + up(8 * n_own);
   b.o_own = b.o_common + up(4 * n_common * hd);
@@ -509,11 +563,15 @@ int blitz_attn_beams(const void* q, int64_t q_stride, const void* kv, const int3
   p.beams = beams; p.q_heads = q_heads; p.rep = b.rep; p.kv_div = b.kv_div; p.kv_heads = kv_heads;
   p.per_block = b.per_block; p.blocks = b.blocks; p.heads = b.heads; p.ranges_most = b.ranges;
   p.page_shift = 31 - __builtin_clz(page); p.max_pages = max_pages;
-  p.scale_log2 = scale * 1.4426950408889634f;
+  // scores enter the exponent with the scale's size (largest scores are looked for before it), its sign goes into the queries; under a cap they are log2 already
+  const bool plain = !(cap > 0.f);
+  p.keep = plain && scale == 0.f ? 0u : ~0u;
+  p.flip = plain && scale < 0.f ? 0x80008000u : 0u;
+  p.scale_log2 = plain && scale != 0.f ? fabsf(scale) * 1.4426950408889634f : 1.f;
   p.cap_scale = cap > 0.f ? scale / cap : 0.f;
   p.cap_log2 = cap * 1.4426950408889634f;
   p.sink = sink;
-  p.line = reinterpret_cast<int*>(ws + b.line);
+  p.runs = reinterpret_cast<int2*>(ws + b.runs);
   p.ml_common = reinterpret_cast<float2*>(ws + b.ml_common);
   p.ml_own = reinterpret_cast<float2*>(ws + b.ml_own);
   p.o_common = reinterpret_cast<float*>(ws + b.o_common);
