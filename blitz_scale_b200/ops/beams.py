@@ -7,6 +7,7 @@ and can be captured into a graph.
 """
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import NamedTuple, Optional, Union
 
 import torch
@@ -56,7 +57,7 @@ def _here(t: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
     if at < 0 or at != _raw_device():
         raise ValueError(f"a tensor on {t.device}: the kernels run on the current CUDA device")
     for o in others:
-        if o is not None and o.get_device() != at:
+        if not (o is None or o.get_device() == at):
             raise ValueError(f"a tensor on {o.device}, another on {t.device}: the kernels run on the current CUDA device")
 
 
@@ -68,9 +69,21 @@ def _ints(t: torch.Tensor, shape: tuple, what: str) -> torch.Tensor:
 
 def _rows_of(t: torch.Tensor, what: str) -> tuple:
     """(rows, columns, pitch) of a table of int32"""
-    if t.dtype is not torch.int32 or t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise ValueError(f"{what}: rows of int32, got {tuple(t.shape)} {t.dtype}")
-    return t.shape[0], t.shape[1], t.stride(0)
+    shape, step = t.shape, t.stride()
+    if t.dtype is not torch.int32 or len(shape) != 2 or (shape[1] > 1 and step[1] != 1):
+        raise ValueError(f"{what}: rows of int32, got {tuple(shape)} {t.dtype}")
+    return shape[0], shape[1], step[0]
+
+
+@lru_cache(256)
+def _select_scratch(rows: int, vocab: int, n: int, dt: int, device: int) -> int:
+    """Scratch of a selection on the current device, in 32-bit words."""
+    return (lib().blitz_beam_select_workspace_bytes(rows, vocab, n, dt) + 3) // 4
+
+
+@lru_cache(256)
+def _attn_scratch(rows: int, beams: int, q_heads: int, kv_heads: int, head_dim: int, device: int) -> int:
+    return int(lib().blitz_attn_beams_workspace_bytes(rows, beams, q_heads, kv_heads, head_dim))
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int = 1, *, n: int = 0, keep: int = 0, ended: Optional[torch.Tensor] = None,
@@ -79,11 +92,13 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int = 1, *, n
     ``scores`` [requests * beams] in fp32, -inf for a row that has ended.  A continuation's value is the row's score plus the token's log
     probability, a softmax over the whole row; one that is no number (rows with a NaN or +inf) counts as -inf.  Ties go to the lowest beam, then the
     lowest token.  ``ended``: int32 tokens that end a sequence; ``keep`` (beams): how many continuations go on.  At most 64 beams and candidates."""
-    if logits.dtype not in _DT3:
+    dt = _DT3.get(logits.dtype)
+    if dt is None:
         raise TypeError(f"kernel takes fp16/bf16/fp32 tensors, got {logits.dtype}")
-    if logits.dim() != 2 or logits.shape[1] < 1 or (logits.shape[1] > 1 and logits.stride(1) != 1):
-        raise ValueError(f"logits: rows of numbers, got {tuple(logits.shape)}, strides {logits.stride()}")
-    rows, V = logits.shape
+    shape, step = logits.shape, logits.stride()
+    if len(shape) != 2 or shape[1] < 1 or (step[1] != 1 and shape[1] > 1):
+        raise ValueError(f"logits: rows of numbers, got {tuple(shape)}, strides {step}")
+    rows, V = shape
     n = n or 2 * beams
     keep = keep or min(beams, n)
     if not 1 <= beams <= BEAMS_MAX or rows % beams or not 1 <= n <= BEAMS_MAX or not 1 <= keep <= n:
@@ -95,8 +110,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int = 1, *, n
     Q = rows // beams
     if out is None:
         _here(logits, scores, ended)
-        out = BeamStep(scores.new_empty((Q, n)), *scores.new_empty((2, Q, n), dtype=torch.int32).unbind(), scores.new_empty((Q, keep)),
-                       *scores.new_empty((2, Q, keep), dtype=torch.int32).unbind())
+        a, b, c = scores.new_empty((3, Q, n)).unbind()
+        d, e, f = scores.new_empty((3, Q, keep)).unbind()
+        out = BeamStep(a, b.view(torch.int32), c.view(torch.int32), d, e.view(torch.int32), f.view(torch.int32))
     else:
         _here(logits, scores, ended, *out)
         for t, m, what in zip(out, (n, n, n, keep, keep, keep), BeamStep._fields):
@@ -104,10 +120,14 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int = 1, *, n
                 raise ValueError(f"{what}: {Q} x {m} contiguous numbers, got {tuple(t.shape)} {t.dtype}")
     if rows == 0:
         return out
-    L, dt = lib(), _DT3[logits.dtype]
-    work = torch.empty(L.blitz_beam_select_workspace_bytes(rows, V, n, dt), dtype=torch.uint8, device=logits.device)
-    _check(L.blitz_beam_select(logits.data_ptr(), logits.stride(0), scores.data_ptr(), rows, V, beams, n, keep, None if ended is None else ended.data_ptr(),
-                               0 if ended is None else ended.shape[0], work.data_ptr(), *[t.data_ptr() for t in out], dt, _stream()), "blitz_beam_select")
+    L = lib()
+    work = scores.new_empty(_select_scratch(rows, V, n, dt, _raw_device()))
+    a, b, c, d, e, f = out
+    rc = L.blitz_beam_select(logits.data_ptr(), step[0], scores.data_ptr(), rows, V, beams, n, keep, None if ended is None else ended.data_ptr(),
+                             0 if ended is None else ended.shape[0], work.data_ptr(), a.data_ptr(), b.data_ptr(), c.data_ptr(), d.data_ptr(), e.data_ptr(),
+                             f.data_ptr(), dt, _stream())
+    if rc:
+        _check(rc, "blitz_beam_select")
     return out
 
 
@@ -137,7 +157,9 @@ def beam_fork(table: torch.Tensor, cached: torch.Tensor, parents: torch.Tensor, 
         raise ValueError(f"cached: {rows} numbers, got {cached.shape[0]}")
     if out is None:
         _here(table, cached, parents, pool)
-        out = BeamFork(table.new_empty((Q * to, W)), *table.new_empty((4, Q * to)).unbind())
+        R = Q * to
+        new, a, b, c, d = table.new_empty(R * (W + 4)).split_with_sizes((R * W, R, R, R, R))
+        out = BeamFork(new.view(R, W), a, b, c, d)
     else:
         _here(table, cached, parents, pool, *out)
         _ints(out.table, (Q * to, W), "out.table")
@@ -146,24 +168,27 @@ def beam_fork(table: torch.Tensor, cached: torch.Tensor, parents: torch.Tensor, 
         if out.table.untyped_storage().data_ptr() == table.untyped_storage().data_ptr() and \
                 out.table.data_ptr() < table.data_ptr() + 4 * ((rows - 1) * pitch + W) and table.data_ptr() < out.table.data_ptr() + 4 * Q * to * W:
             raise ValueError("out.table shares memory with the table")
-    _check(lib().blitz_beam_fork(table.data_ptr(), pitch, cached.data_ptr(), parents.data_ptr(), pool.data_ptr(), pool_pitch, Q, k, to, W, P, page_size,
-                                 num_pages, *[t.data_ptr() for t in out], _status_ptr(table), _stream()), "blitz_beam_fork")
+    a, b, c, d, e = out
+    rc = lib().blitz_beam_fork(table.data_ptr(), pitch, cached.data_ptr(), parents.data_ptr(), pool.data_ptr(), pool_pitch, Q, k, to, W, P, page_size, num_pages,
+                               a.data_ptr(), b.data_ptr(), c.data_ptr(), d.data_ptr(), e.data_ptr(), _status_ptr(table), _stream())
+    if rc:
+        _check(rc, "blitz_beam_fork")
     return out
 
 
 def _copy(t: torch.Tensor, layers: bool, parts: int, page: int, src, dst, tokens) -> None:
     """Copies in one tensor [layers?, pages, ...]; parts > 0: pages are that many runs of `page` tokens."""
-    if not t.is_contiguous() or t.dim() < 1 + layers:
-        raise ValueError(f"a cache is one contiguous tensor, got {tuple(t.shape)}, strides {t.stride()}")
-    size = t.element_size()
-    L, pages = (t.shape[0] if layers else 1), t.shape[int(layers)]
-    whole = t.stride(int(layers)) * size if t.numel() else 0
-    n = src.shape[0]
-    if n == 0 or whole == 0:
+    shape, i = t.shape, 1 if layers else 0
+    if not t.is_contiguous() or len(shape) < 1 + i:
+        raise ValueError(f"a cache is one contiguous tensor, got {tuple(shape)}, strides {t.stride()}")
+    whole, n, pages = t.stride(i) * t.element_size(), src.shape[0], shape[i]
+    if n == 0 or t.numel() == 0:
         return
     run = whole // parts
-    _check(lib().blitz_copy_pages(t.data_ptr(), L, pages * whole, pages, whole, parts, run, run, run // page, src.data_ptr(), dst.data_ptr(),
-                                  None if tokens is None else tokens.data_ptr(), n, _status_ptr(t), _stream()), "blitz_copy_pages")
+    rc = lib().blitz_copy_pages(t.data_ptr(), shape[0] if layers else 1, pages * whole, pages, whole, parts, run, run, run // page, src.data_ptr(), dst.data_ptr(),
+                                None if tokens is None else tokens.data_ptr(), n, _status_ptr(t), _stream())
+    if rc:
+        _check(rc, "blitz_copy_pages")
 
 
 def copy_pages(cache: Union[torch.Tensor, KVPair, LatentKV, QuantKV], src: torch.Tensor, dst: torch.Tensor, tokens: Optional[torch.Tensor] = None, *,
@@ -218,8 +243,9 @@ def step_tables(table: torch.Tensor, cached: torch.Tensor, counts: Optional[torc
     T = tokens if ragged else R
     if out is None:
         _here(table, cached, counts)
-        new = table.new_empty
-        out = StepTables(new(entries), new(R + 1), new(R), *new((2, T)).unbind(), new(R + 1) if ragged else None, new(R // beams) if beams else None)
+        extra = R + 1 if ragged else 0, R // beams if beams else 0
+        parts = table.new_empty(entries + 2 * (R + T) + 1 + sum(extra)).split_with_sizes((entries, R + 1, R, T, T, *extra))
+        out = StepTables(*parts[:5], parts[5] if ragged else None, parts[6] if beams else None)
     else:
         sizes = (entries, R + 1, R, T, T, R + 1 if ragged else None, R // beams if beams else None)
         for t, n, what in zip(out, sizes, StepTables._fields):
@@ -234,9 +260,12 @@ def step_tables(table: torch.Tensor, cached: torch.Tensor, counts: Optional[torc
                 t.zero_()
         out.slot.fill_(-1)
         return out
-    ptr = [None if t is None else t.data_ptr() for t in out]
-    _check(lib().blitz_step_tables(table.data_ptr(), pitch, cached.data_ptr(), counts.data_ptr() if ragged else None, R, W, page_size, beams, entries, tokens, *ptr,
-                                   _status_ptr(table), _stream()), "blitz_step_tables")
+    a, b, c, d, e, f, g = out
+    rc = lib().blitz_step_tables(table.data_ptr(), pitch, cached.data_ptr(), counts.data_ptr() if ragged else None, R, W, page_size, beams, entries, tokens, a.data_ptr(),
+                                 b.data_ptr(), c.data_ptr(), d.data_ptr(), e.data_ptr(), None if f is None else f.data_ptr(), None if g is None else g.data_ptr(),
+                                 _status_ptr(table), _stream())
+    if rc:
+        _check(rc, "blitz_step_tables")
     return out
 
 
@@ -286,7 +315,7 @@ def attn_decode_beams(q: torch.Tensor, kv_layer: torch.Tensor, indices: torch.Te
         return out
     L = lib()
     if workspace is None:
-        workspace = torch.empty(L.blitz_attn_beams_workspace_bytes(R, beams, q_heads, kv_heads, head_dim), dtype=torch.uint8, device=q.device)
+        workspace = q.new_empty(_attn_scratch(R, beams, q_heads, kv_heads, head_dim, _raw_device()), dtype=torch.uint8)
     elif workspace.dtype is not torch.uint8 or not workspace.is_contiguous() or workspace.data_ptr() & 255:
         raise ValueError(f"workspace: bytes that start on a 256-byte boundary, got {workspace.dtype}")
     rc = L.blitz_attn_beams(q.data_ptr(), q.stride(0), kv_layer.data_ptr(), indices.data_ptr(), indptr.data_ptr(), last_page_len.data_ptr(), shared.data_ptr(),
