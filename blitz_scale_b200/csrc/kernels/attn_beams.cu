@@ -11,7 +11,8 @@
 // sums in scratch (fp32), and a second kernel adds up a row's pieces, always in the same order.  Every block works out the ranges from the tables, so a
 // captured launch follows them.
 //
-// A warp is by itself: it copies its steps (cp.async, three ahead), and nothing in the loop waits for another warp.
+// A warp is by itself: it has a ring of three steps (192 KB an SM), asks for the next one (TMA, boxes of 16 tokens x 64 columns) and computes, and nothing in the
+// loop waits for another warp.  (With cp.async instead a warp stood for 2000 to 4000 cycles of a step in its own requests, and computed, 750 to 1500, only then.)
 #include "launch.cuh"
 #include "ptx.cuh"
 #include "tmap.cuh"
@@ -40,7 +41,7 @@ struct BeamAttnParams {
   int heads;                    // virtual heads x blocks
   int ranges_most;
   int page_shift, max_pages;
-  float scale_log2, cap_scale, cap_log2;      // the scale's size (1 under a cap, or where it is zero); keep and flip: zero or its sign, for the queries
+  float scale_log2, slack, cap_scale, cap_log2;      // the scale's size (1 under a cap, or where it is zero); keep and flip: zero or its sign, for the queries
   uint32_t keep, flip;
   const void* sink;
   int2* runs;                   // [blocks][groups + groups per_block] of each segment: its first piece's range, pieces
@@ -121,17 +122,24 @@ struct BaPlace {
 };
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const BeamAttnParams p) {
-  constexpr int kRowBytes = HD * 2, kPieces = HD / 8;         // a token's key: 16-byte pieces
-  constexpr int kStage = 2 * kBaStep * kRowBytes;             // keys, then values
+__global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const __grid_constant__ CUtensorMap tmap, const BeamAttnParams p) {
+  constexpr int kSlab = kBaStep * 128, kSlabs = HD / 64;       // 64 columns of a step's keys, 128 bytes a token, 16-byte columns turned by the token's number
+  constexpr int kStage = 2 * kSlabs * kSlab;                  // keys, then values
   constexpr int kStages = HD == 128 ? 3 : 6;
-  extern __shared__ __align__(128) uint8_t ba_smem[];
+  extern __shared__ uint8_t ba_raw[];
+  uint8_t* ba_smem = ba_raw + (1024 - (ptx::smem_u32(ba_raw) & 1023)) % 1024;
   __shared__ int sums[kBaWarps];
+  __shared__ uint64_t arrived[kBaWarps][kStages];
+  __shared__ int abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int per = p.groups * (1 + p.per_block);
   int* line = reinterpret_cast<int*>(ba_smem + kBaWarps * kStages * kStage);
   int* len = line + p.blocks * per + 1;
   int* common = len + p.rows;
+  if (threadIdx.x == 0) abort_flag = 0;
+  if (lane < kStages) ptx::mbar_init(&arrived[warp][lane], 1);
+  ptx::fence_mbar_init();
+  if (threadIdx.x == 0) ptx::tma_prefetch_desc(&tmap);
   ptx::griddep_launch_dependents();
   if (!p.static_table) ptx::griddep_wait();
   ba_line(p, line, len, common, sums);
@@ -153,9 +161,7 @@ __global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const BeamAtt
   const BaRanges ranges(line[per] - base, p.ranges_most);
   if (range >= ranges.count) return;
   const int x_end = ranges.begin(range + 1);
-  const int64_t token_pitch = static_cast<int64_t>(p.kv_heads) * HD;
-  const T* kv = reinterpret_cast<const T*>(p.kv) + (head / p.kv_div) * HD;
-  const int page = 1 << p.page_shift;
+  const int page = 1 << p.page_shift, kv_head = head / p.kv_div;
 
   auto enter = [&](BaPlace& a) {     // the segment that step a.x is in (a.seg: one at or before it)
     while (line[a.seg + 1] - base <= a.x) ++a.seg;
@@ -191,10 +197,8 @@ __global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const BeamAtt
   }
   enter(ld);
   enter(at);
-  const uint32_t ring = ptx::smem_u32(ba_smem) + warp * kStages * kStage;
-  // a lane copies 16 bytes at column lane % kPieces of every (32 / kPieces)-th token; 16-byte columns are turned by the token's number, so that ldmatrix meets no bank twice
-  const int64_t lane_at = lane / kPieces * token_pitch + lane % kPieces * 8;
-  const uint32_t ring_dst = ring + lane / kPieces * kRowBytes + (((lane % kPieces ^ lane / kPieces) & 7 | lane % kPieces & 8) << 4);
+  uint8_t* ring_at = ba_smem + warp * kStages * kStage;
+  const uint32_t ring = ptx::smem_u32(ring_at);
   int win = 0, win_base = -64;       // page ids: lane l holds entry win_base + l of the row's list
   int ld_stage = 0;
   auto load = [&]() {                // requests the next step
@@ -214,41 +218,30 @@ __global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const BeamAtt
       }
     }
     const int id = __shfl_sync(0xffffffffu, win, pg - win_base);
-    const T* k = kv + ((static_cast<int64_t>(id) << (p.page_shift + 1)) + (t0 & (page - 1))) * token_pitch + lane_at;
-    const T* v = k + page * token_pitch;
-    const uint32_t to = ring_dst + ld_stage * kStage;
-    constexpr int kTokens = 32 / kPieces, kTurns = kBaStep / kTokens;      // of an instruction; instructions
-    const int64_t step = kTokens * token_pitch;
-    if (ld.len - t0 >= kBaStep) {
+    if (ptx::elect_one()) {
+      // (whole steps: pages are multiples of them)
+      const int z = (id << (p.page_shift + 1)) + (t0 & (page - 1));
+      uint8_t* to = ring_at + ld_stage * kStage;
+      ptx::mbar_expect_tx(&arrived[warp][ld_stage], kStage);
 #pragma unroll
-      for (int i = 0; i < kTurns; ++i) {
-        const uint32_t dst = (to ^ (i * kTokens & 7) << 4) + i * kTokens * kRowBytes;
-        ptx::cp_async_16(dst, k + i * step, 16);
-        ptx::cp_async_16(dst + kBaStep * kRowBytes, v + i * step, 16);
-      }
-    } else {      // the row's last step: zeros behind its end, whatever the page holds there
-      const int valid = ld.len - t0 - lane / kPieces;
-#pragma unroll 1
-      for (int i = 0; i < kTurns; ++i) {
-        const uint32_t dst = (to ^ (i * kTokens & 7) << 4) + i * kTokens * kRowBytes, bytes = i * kTokens < valid ? 16u : 0u;
-        ptx::cp_async_16(dst, bytes ? k + i * step : kv, bytes);
-        ptx::cp_async_16(dst + kBaStep * kRowBytes, bytes ? v + i * step : kv, bytes);
+      for (int i = 0; i < kSlabs; ++i) {
+        ptx::tma_load_3d(to + i * kSlab, &tmap, &arrived[warp][ld_stage], i * 64, kv_head, z);
+        ptx::tma_load_3d(to + (kSlabs + i) * kSlab, &tmap, &arrived[warp][ld_stage], i * 64, kv_head, z + page);
       }
     }
     ++ld.x;
     if (++ld_stage == kStages) ld_stage = 0;
   };
 #pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) {
-    load();
-    ptx::cp_async_commit();
-  }
+  for (int i = 0; i < kStages - 1; ++i) load();
   const int g8 = lane >> 2, t4 = lane & 3, mi = lane >> 3, mr = lane & 7;
   // what the lane reads of a stage with ldmatrix: keys of its token from 16-byte column mi & 1 on, values of its token from column mi >> 1 on
   const int k_tok = (mi >> 1) * 8 + mr, v_tok = (mi & 1) * 8 + mr;
-  const uint32_t k_at = ring + k_tok * kRowBytes + (((mi & 1) ^ k_tok & 7) << 4);
-  const uint32_t v_at = ring + (kBaStep + v_tok) * kRowBytes + (((mi >> 1) ^ v_tok & 7) << 4);
+  const uint32_t k_at = ring + k_tok * 128 + (((mi & 1) ^ k_tok & 7) << 4);
+  const uint32_t v_at = ring + kSlabs * kSlab + v_tok * 128 + (((mi >> 1) ^ v_tok & 7) << 4);
   int stage = 0;
+  uint32_t phase = 0;
+  bool ok = true;       // (after a wait that ran out the warp waits no more: the status word says so)
   // A piece: TILES of 16 query rows.
   auto piece = [&](auto tiles) {
     constexpr int TILES = decltype(tiles)::value;
@@ -269,18 +262,27 @@ __global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const BeamAtt
           for (int hi = 0; hi < 2; ++hi)
             qa[t][ks][half + 2 * hi] = i < live ? *reinterpret_cast<const uint32_t*>(q + ks * 16 + hi * 8 + 2 * t4) & p.keep ^ p.flip : 0u;
       }
-    float o[TILES][HD / 8][4], m[TILES][2], l[TILES][2];
+    float o[TILES][HD / 8][4], m[TILES][2], l[TILES][2], limit[TILES][2];
 #pragma unroll
     for (int t = 0; t < TILES; ++t) {
-      m[t][0] = m[t][1] = -INFINITY;
+      m[t][0] = m[t][1] = limit[t][0] = limit[t][1] = -INFINITY;
       l[t][0] = l[t][1] = 0.f;
 #pragma unroll
       for (int i = 0; i < HD / 8; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.f;
     }
     for (; at.x < at.seg_end; ++at.x) {
       load();
-      ptx::cp_async_commit();
-      ptx::cp_async_wait<kStages - 1>();
+      if (ok && !ptx::bounded_mbar_wait(&arrived[warp][stage], phase, &abort_flag)) {
+        if (p.status && lane == 0) atomicCAS(p.status, 0, kStatusTimeoutProducer);
+        ok = false;
+      }
+      const int valid = at.len - (at.tok0 + (at.x - at.seg_beg) * kBaStep);
+      if (valid < kBaStep) {      // the row's last step: zeros for values behind its end, whatever the page holds there
+        for (int i = lane; i < kBaStep * kSlabs * 8; i += 32)
+          if (i / (kSlabs * 8) >= valid)
+            *reinterpret_cast<uint4*>(ring_at + stage * kStage + (kSlabs + i / 8 % kSlabs) * kSlab + i / (kSlabs * 8) * 128 + i % 8 * 16) = make_uint4(0, 0, 0, 0);
+        ptx::fence_proxy_async_smem();
+      }
       __syncwarp();
       const uint32_t kbase = k_at + stage * kStage, vbase = v_at + stage * kStage;
       float s[TILES][2][4] = {};
@@ -288,7 +290,7 @@ __global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const BeamAtt
 #pragma unroll
         for (int ks = 0; ks < HD / 16; ++ks) {
           uint32_t b0, b1, b2, b3;
-          ldmatrix_x4((kbase ^ (ks * 2 & 7) << 4) + (ks * 2 & 8) * 16, b0, b1, b2, b3);
+          ldmatrix_x4((kbase ^ (ks * 2 & 7) << 4) + ks / 4 * kSlab, b0, b1, b2, b3);
 #pragma unroll
           for (int t = 0; t < TILES; ++t) {
             mma16816<T>(s[t][0], qa[t][ks][0], qa[t][ks][1], qa[t][ks][2], qa[t][ks][3], b0, b1);
@@ -296,7 +298,6 @@ __global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const BeamAtt
           }
         }
       }
-      const int valid = at.len - (at.tok0 + (at.x - at.seg_beg) * kBaStep);
       if (p.cap_log2 > 0.f) {
 #pragma unroll
         for (int t = 0; t < TILES; ++t)
@@ -310,31 +311,44 @@ __global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const BeamAtt
           for (int e = 0; e < 8; ++e)
             if ((e >> 2) * 8 + 2 * t4 + (e & 1) >= valid) s[t][e >> 2][e & 3] = -INFINITY;
       }
+      // The weights' reference: the largest score at first, a later one only where a score is 2^8 above it (weights up to 256 cost no precision; a maximum that is
+      // followed costs four shuffles, and a vote, in every step).
       uint32_t pa[TILES][4];
+      float top[TILES][2];
+      bool over = false;
 #pragma unroll
-      for (int t = 0; t < TILES; ++t) {
-        float top[2] = {m[t][0], m[t][1]};
+      for (int t = 0; t < TILES; ++t)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          top[k] = ptx::fmax3(top[k], fmaxf(s[t][0][2 * k], s[t][0][2 * k + 1]), fmaxf(s[t][1][2 * k], s[t][1][2 * k + 1]));
-          top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 1));
-          top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 2));
+          top[t][k] = fmaxf(fmaxf(s[t][0][2 * k], s[t][0][2 * k + 1]), fmaxf(s[t][1][2 * k], s[t][1][2 * k + 1]));
+          over |= top[t][k] > limit[t][k];
         }
-        if (__any_sync(0xffffffffu, top[0] > m[t][0] || top[1] > m[t][1])) {
-          const float a0 = ptx::ex2_approx(m[t][0] * p.scale_log2 - top[0] * p.scale_log2), a1 = ptx::ex2_approx(m[t][1] * p.scale_log2 - top[1] * p.scale_log2);
-          l[t][0] *= a0;
-          l[t][1] *= a1;
+      if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+          float a[2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            float x = fmaxf(top[t][k], __shfl_xor_sync(0xffffffffu, top[t][k], 1));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+            x = fmaxf(x, m[t][k]);
+            a[k] = ptx::ex2_approx(__fmul_rn(m[t][k], p.scale_log2) - __fmul_rn(x, p.scale_log2));
+            m[t][k] = x;
+            limit[t][k] = x + p.slack;
+            l[t][k] *= a[k];
+          }
 #pragma unroll
           for (int i = 0; i < HD / 8; ++i) {
-            o[t][i][0] *= a0;
-            o[t][i][1] *= a0;
-            o[t][i][2] *= a1;
-            o[t][i][3] *= a1;
+            o[t][i][0] *= a[0];
+            o[t][i][1] *= a[0];
+            o[t][i][2] *= a[1];
+            o[t][i][3] *= a[1];
           }
-          m[t][0] = top[0];
-          m[t][1] = top[1];
         }
-        const float ref[2] = {-m[t][0] * p.scale_log2, -m[t][1] * p.scale_log2};
+      }
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) {
+        const float ref[2] = {-__fmul_rn(m[t][0], p.scale_log2), -__fmul_rn(m[t][1], p.scale_log2)};
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           float& x = s[t][e >> 2][e & 3];
@@ -351,7 +365,7 @@ __global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const BeamAtt
 #pragma unroll
         for (int np = 0; np < HD / 16; ++np) {
           uint32_t b0, b1, b2, b3;
-          ldmatrix_x4_trans((vbase ^ (np * 2 & 7) << 4) + (np * 2 & 8) * 16, b0, b1, b2, b3);
+          ldmatrix_x4_trans((vbase ^ (np * 2 & 7) << 4) + np / 4 * kSlab, b0, b1, b2, b3);
 #pragma unroll
           for (int t = 0; t < TILES; ++t) {
             mma16816<T>(o[t][2 * np], pa[t][0], pa[t][1], pa[t][2], pa[t][3], b0, b1);
@@ -360,7 +374,10 @@ __global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const BeamAtt
         }
       }
       __syncwarp();       // the stage is free
-      if (++stage == kStages) stage = 0;
+      if (++stage == kStages) {
+        stage = 0;
+        phase ^= 1;
+      }
     }
     // the piece's sums: number `range` + segment of this head
     const int64_t slot = shared_part ? (static_cast<int64_t>(hv) * (p.ranges_most + p.groups) + range + at.seg) * kBaTile
@@ -518,7 +535,7 @@ static BaPlan ba_plan(int rows, int beams, int q_heads, int kv_heads, int hd) {
 }
 
 template <typename T, int HD>
-static int ba_launch(const BeamAttnParams& p, cudaStream_t stream) {
+static int ba_launch(const CUtensorMap& tmap, const BeamAttnParams& p, cudaStream_t stream) {
   auto kern = attn_beams_kernel<T, HD>;
   constexpr int kRing = kBaWarps * (HD == 128 ? 3 : 6) * 2 * kBaStep * HD * 2;
   const int per = p.groups * (1 + p.per_block);
@@ -526,8 +543,8 @@ static int ba_launch(const BeamAttnParams& p, cudaStream_t stream) {
   cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 1024); });
   if (e != cudaSuccess) return (int)e;
   const int workers = p.heads * p.ranges_most;
-  const size_t smem = kRing + 4 * static_cast<size_t>(p.blocks * per + 1 + p.rows + p.blocks * p.groups);
-  e = launch_pdl(kern, dim3((workers + kBaWarps - 1) / kBaWarps), dim3(kBaThreads), smem, stream, p);
+  const size_t smem = 1024 + kRing + 4 * static_cast<size_t>(p.blocks * per + 1 + p.rows + p.blocks * p.groups);
+  e = launch_pdl(kern, dim3((workers + kBaWarps - 1) / kBaWarps), dim3(kBaThreads), smem, stream, tmap, p);
   if (e != cudaSuccess) return (int)e;
   const int items = p.rows * p.q_heads;
   // few rows: a block for each, so that the many pieces of a long one are added up by eight warps
@@ -557,6 +574,9 @@ int blitz_attn_beams(const void* q, int64_t q_stride, const void* kv, const int3
     return -1;
   const BaPlan b = ba_plan(rows, beams, q_heads, kv_heads, head_dim);
   if (workspace_bytes < b.bytes) return -1;
+  // a pool as [token of a plane][head][64 columns]; a box is a step's
+  CUtensorMap tmap;
+  if (!get_tmap_3d(&tmap, kv, head_dim, kv_heads, (uint64_t)max_pages * 2 * page, (uint64_t)head_dim * 2, (uint64_t)head_dim * 2 * kv_heads, 64, 1, kBaStep)) return -2;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   BeamAttnParams p;
   p.q_stride = q_stride; p.kv = kv; p.indices = indices; p.out_stride = out_stride;
@@ -568,6 +588,7 @@ int blitz_attn_beams(const void* q, int64_t q_stride, const void* kv, const int3
   p.keep = plain && scale == 0.f ? 0u : ~0u;
   p.flip = plain && scale < 0.f ? 0x80008000u : 0u;
   p.scale_log2 = plain && scale != 0.f ? fabsf(scale) * 1.4426950408889634f : 1.f;
+  p.slack = 8.f / p.scale_log2;
   p.cap_scale = cap > 0.f ? scale / cap : 0.f;
   p.cap_log2 = cap * 1.4426950408889634f;
   p.sink = sink;
@@ -584,8 +605,8 @@ int blitz_attn_beams(const void* q, int64_t q_stride, const void* kv, const int3
     p.out = static_cast<uint8_t*>(out) + 2 * r * out_stride;
     p.indptr = indptr + r; p.last_page_len = last_page_len + r; p.shared = shared + r / beams;
     int rc;
-    if (dtype == 1) rc = head_dim == 128 ? ba_launch<__nv_bfloat16, 128>(p, stream) : ba_launch<__nv_bfloat16, 64>(p, stream);
-    else rc = head_dim == 128 ? ba_launch<__half, 128>(p, stream) : ba_launch<__half, 64>(p, stream);
+    if (dtype == 1) rc = head_dim == 128 ? ba_launch<__nv_bfloat16, 128>(tmap, p, stream) : ba_launch<__nv_bfloat16, 64>(tmap, p, stream);
+    else rc = head_dim == 128 ? ba_launch<__half, 128>(tmap, p, stream) : ba_launch<__half, 64>(tmap, p, stream);
     if (rc) return rc;
   }
   return 0;

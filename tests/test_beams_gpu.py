@@ -358,7 +358,7 @@ def _close(out, want, dtype, kv):
     """Weights (of sum one) enter the second product with half a step of the type, the output is rounded once: half a step each of the largest value's size.
     Scores of size s are off by s 2^-22 or so: within the slack."""
     half = torch.finfo(dtype).eps / 2
-    top = kv[:, 1].abs().max().double().item()
+    top = kv[:, 1].double().nan_to_num(nan=0.0, posinf=0.0, neginf=0.0).clamp(-1e6, 1e6).abs().max().item()
     off = (out.double().cpu() - want).abs()
     assert (off <= half * (want.abs() + top * 1.25) + 1e-30).all(), (off.max().item(), half * top)
 
@@ -459,6 +459,17 @@ def test_attention_pages_that_there_are_not():
     ops.attn_decode_beams(q, kv, indices, indptr, last, shared, beams=2, q_heads=8, kv_heads=2, head_dim=64, page_size=16)
     with pytest.raises(RuntimeError, match="index"):
         ops.check_status()
+
+
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 64)])
+def test_attention_behind_a_row_s_end(dim, page):
+    """Whatever a page holds behind its row's last token does not matter: numbers, infinities, NaN."""
+    case = _attend_case(6, [(3, [1, 15, 17]), (0, [40, -1, 9])], 3, page, 2, 4, dim, BF)
+    want = _attend(case, 3, page, 2, 4, dim, BF)
+    for pages, n in zip(case[6], case[7]):
+        if n % page:
+            case[1][pages[-1], :, n % page:] = torch.tensor([math.nan, math.inf, -math.inf, 3e38], device="cuda").to(BF).repeat(dim // 4)
+    assert torch.equal(_attend(case, 3, page, 2, 4, dim, BF), want)
 
 
 def test_attention_captured():
