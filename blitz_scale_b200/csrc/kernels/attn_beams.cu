@@ -68,7 +68,7 @@ __device__ __forceinline__ void ba_line(const BeamAttnParams& p, int* line, int*
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   for (int r = tid; r < p.rows; r += kBaThreads) {
     const int pages = p.indptr[r + 1] - p.indptr[r];
-    len[r] = pages > 0 ? ((pages - 1) << p.page_shift) + p.last_page_len[r] : 0;
+    len[r] = pages > 0 ? ((pages - 1) << p.page_shift) + min(max(p.last_page_len[r], 0), 1 << p.page_shift) : 0;
   }
   __syncthreads();
   for (int i = tid; i < p.blocks * p.groups; i += kBaThreads) {

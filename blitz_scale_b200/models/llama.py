@@ -51,6 +51,8 @@ class StepMeta:
     # `pos` and `slot` are read ahead of the pass's own order: no kernel that may still run when the pass starts writes them.  Whoever
     # makes a step whose positions come by a copy may say so; a step whose positions a kernel writes leaves it.
     static_positions: bool = False
+    beams: int = 0                                          # of a decode step: rows come in groups of so many beams of a request (runtime/beams.py),
+    shared: Optional[torch.Tensor] = None                   # whose first pages are the same, [batch / beams] of them
     _views: Dict = field(default_factory=dict, init=False, repr=False, compare=False)   # see `view`; a copy with other sizes has its own
 
     def view(self, key, base: torch.Tensor, make: Callable):
@@ -156,6 +158,14 @@ class LlamaRunner:
             ws = self._ws[key] = torch.zeros(n, dtype=torch.uint8, device=self.res.device)
         return ws
 
+    def _beam_workspace(self, m: StepMeta) -> torch.Tensor:
+        n = ops.attn_beams_workspace_bytes(m.batch, m.beams, q_heads=self.qh, kv_heads=self.kvh, head_dim=self.hd, device=self.res.device)
+        ws = self._ws.get("beams")
+        if ws is None or ws.numel() < n:
+            self._ws_old.append(ws)         # (captured graphs may name an earlier one)
+            ws = self._ws["beams"] = torch.empty(n, dtype=torch.uint8, device=self.res.device)
+        return ws
+
     def _portion_room(self, pages: int) -> torch.Tensor:
         """Scratch of prefill attention over a 4-bit cache, for passes of up to `pages` pages."""
         entries = self.max_tokens // ops.PREFILL_ROWS + self.max_batch
@@ -179,6 +189,9 @@ class LlamaRunner:
                           head_dim=self.hd, page_size=self.page_size, rope_theta=c.rope_theta, static_meta=m.static_positions)
         if m.is_prefill:
             self._prefill_attention(l, m)
+        elif m.shared is not None:
+            ops.attn_decode_beams(qkv, kv, m.page_indices, m.page_indptr, m.last_page_len, m.shared, beams=m.beams, q_heads=self.qh, kv_heads=self.kvh,
+                                  head_dim=self.hd, page_size=self.page_size, workspace=self._beam_workspace(m), static_table=m.static_positions, out=attn)
         else:
             ops.attn_decode(qkv, kv, m.page_indices, m.page_indptr, m.last_page_len,
                             q_heads=self.qh, kv_heads=self.kvh, head_dim=self.hd, page_size=self.page_size,

@@ -1325,5 +1325,5 @@ def part_norm(x: torch.Tensor, w: torch.Tensor, parts: int, eps: float) -> torch
     return x
 
 
-from .beams import (BeamFork, BeamStep, StepTables, attn_beams_workspace_bytes, attn_decode_beams, beam_fork, beam_select, copy_pages,  # noqa: E402,F401
-                    step_tables)
+from .beams import (BEAMS_MAX, BeamFork, BeamStep, StepTables, attn_beams_workspace_bytes, attn_decode_beams, beam_fork, beam_select,  # noqa: E402,F401
+                    copy_pages, step_tables)

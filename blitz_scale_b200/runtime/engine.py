@@ -167,6 +167,7 @@ class Engine:
         self.batches: Dict[int, "core.Batch"] = {}
         self.use_graphs = use_graphs
         self._graphs: Dict[tuple, torch.cuda.CUDAGraph] = {}
+        self._beam_buffers: Dict[tuple, object] = {}        # what the graphs of beam search read (runtime/beams.py)
         self.stream = torch.cuda.Stream(device=self.device)
         self.h2d_bytes = 0
         self.d2h_bytes = 0
@@ -316,6 +317,15 @@ class Engine:
         out = self._tokens_to_host(toks, B)
         batch.append_tokens(out, True)
         return out
+
+    def beam_search(self, prompts: Sequence[Sequence[int]], beams: int, max_new_tokens: int, *, eos: Sequence[int] = (), length_penalty: float = 1.0,
+                    best: Optional[int] = None) -> list:
+        """The most probable continuations of every prompt that `beams` beams find: for each a list of runtime.beams.Hypothesis, best first, `best` (beams) of
+        them, ranked by log probability / length ^ `length_penalty`.  A continuation ends with one of the tokens `eos` or after `max_new_tokens`.  Pages (and
+        state slots) for beams x requests are reserved for the time of the call; requests beyond max_batch / beams run one group after the other.
+        RuntimeError, with nothing kept, where the cache has too few pages."""
+        from .beams import beam_search
+        return beam_search(self, prompts, beams, max_new_tokens, eos=eos, length_penalty=length_penalty, best=best)
 
     @torch.no_grad()
     def step(self, batch: "core.Batch", counts: Sequence[int], want: Sequence[Sequence[int]] = ()) -> Optional[torch.Tensor]:
@@ -479,6 +489,7 @@ class Engine:
         """Drop every captured decode graph (first step of an orderly exit: the graphs hold kernel arguments that
         name peer memory and, with the NCCL runner, collectives of its communicator)."""
         self._graphs.clear()
+        self._beam_buffers.clear()
 
     def close_regions(self) -> None:
         """Drop the symmetric regions this engine owns (the fused tensor-parallel state); see parallel/teardown.py."""
