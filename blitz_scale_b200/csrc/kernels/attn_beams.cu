@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const __grid_
 // Adds up the pieces of a row and query head: those of its group's common part, then its own.  WARPS of them share one's pieces (few
 // rows), or each warp has its own.
 template <typename T, int HD, int WARPS>
-__global__ void __launch_bounds__(kBaThreads) attn_beams_merge_kernel(const BeamAttnParams p) {
+__global__ void __launch_bounds__(kBaThreads, WARPS > 1 ? 2 : 4) attn_beams_merge_kernel(const BeamAttnParams p) {
   constexpr int kLanes = HD / 4, kTeams = WARPS * 32 / kLanes;      // lanes that hold a row of sums; teams that take every n-th piece
   ptx::griddep_launch_dependents();
   __shared__ float4 part[WARPS > 1 ? kTeams : 1][kLanes];
