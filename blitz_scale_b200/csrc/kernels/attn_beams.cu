@@ -13,6 +13,13 @@
 //
 // A warp is by itself: it has a ring of three steps (192 KB an SM), asks for the next one (TMA, boxes of 16 tokens x 64 columns) and computes, and nothing in the
 // loop waits for another warp.  (With cp.async instead a warp stood for 2000 to 4000 cycles of a step in its own requests, and computed, 750 to 1500, only then.)
+//
+// Rounded to 16 bits: the weights, as operands of the second product, and the output.  Scores, maxima, sums and pieces are fp32.
+//
+// Measured, 32 query over 8 KV heads of 128, bf16, us in a graph (bytes of each token once, at the copy rate): 4 beams of 100144 tokens 78.6 (63.1), of 1014 tokens 11.0 (0.75);
+// 32 x 8 beams of 1301 on average, 101 of them their own, 73.0 (44.5).  What bounds it: memory at 5.8 TB/s while all warps run, but
+// equal ranges end between 42 and 61 us (32 x 8) or 52 and 68 (the long one), SMs and warps are not served evenly; then 3 us for tables and first loads, 6.6 to 7.7 for the merge.
+// Tried: queries and page ids of the next piece asked for a piece ahead 77.8 (32 x 8), the heads of a range on one SM 76.4 (79.9 the long one).
 #include "launch.cuh"
 #include "ptx.cuh"
 #include "tmap.cuh"
@@ -570,7 +577,7 @@ int blitz_attn_beams(const void* q, int64_t q_stride, const void* kv, const int3
                      cudaStream_t stream) {
   if (rows <= 0) return 0;
   if (beams < 1 || beams > 64 || rows % beams || kv_heads < 1 || q_heads < 1 || q_heads % kv_heads || (head_dim != 64 && head_dim != 128) || page < 16 ||
-      (page & (page - 1)) || max_pages < 1 || (q_stride & 7) || (out_stride & 7))
+      (page & (page - 1)) || max_pages < 1 || static_cast<int64_t>(max_pages) * 2 * page > 0x7fffffff || (q_stride & 7) || (out_stride & 7))
     return -1;
   const BaPlan b = ba_plan(rows, beams, q_heads, kv_heads, head_dim);
   if (workspace_bytes < b.bytes) return -1;

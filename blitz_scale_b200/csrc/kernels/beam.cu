@@ -21,6 +21,10 @@ constexpr int kBeamMost = 64;  // beams of a request, and candidates of it
 // three times the stream's time.  The second kernel, a block per request, knows the sums, hence the values of the groups' largest; the n best elements are in
 // the n best groups, which it reads again (1 KB each, out of L2 as a rule).  Values are pairs of fp32, 48 bits: candidates of
 // different beams may be nearer to one another than fp32 tells apart, and an exchange of two would be a wrong token.
+//
+// Measured, us in a graph (bytes once at the copy rate): 256 rows of 128256 logits in bf16, 8 beams, n = 24, 23.2 (10.0), of which the scan 15.8; 65 rows of 50257 in fp32
+// 11.2 (2.0); one request of four beams 8.2 (0.2).  The scan is bound by its instructions, a fifth of them the exponentials, and the time until all warps have
+// their first groups; the second kernel by a chain of some ten short rounds through shared memory.
 constexpr int kSelGroup = 512;
 constexpr int kSelWarps = 48;       // warps of an SM that the scan counts on
 constexpr int kSelStretch = 32;     // groups of a stretch at most (sums of more lose digits)
@@ -382,7 +386,7 @@ struct ForkParams {
 };
 
 // A block per request.  A bit per page says which ones the children keep; the fresh ones are the first of the request's own without it.
-// Latency bounds it: lengths, then tables, are two rounds of loads, all of a round at once.
+// Latency bounds it: lengths, then tables, are two rounds of loads, all of a round at once (3.4 us for one request of 4 beams, 4.4 for 32 of 8; child after child 5.8 and 10.0).
 __global__ void __launch_bounds__(kBeamThreads) beam_fork_kernel(const ForkParams p) {
   extern __shared__ uint32_t used[];
   __shared__ int par[kBeamMost], len[kBeamMost], again[kBeamMost], want[kBeamMost], fresh[kBeamMost], held[kBeamMost], sums[kBeamThreads / 32];
@@ -490,7 +494,8 @@ struct CopyParams {
 };
 constexpr int kCopyPiece = 32768;
 
-// A block per piece of 32 KB.  U: what all addresses are multiples of.
+// A block per piece of 32 KB, each thread with eight 16-byte loads under way; HBM bounds it (99 MB, 256 rows of 8 layers, 28.5 us, 6.9 TB/s read and written).  U: what all
+// addresses are multiples of.
 template <typename U>
 __global__ void __launch_bounds__(kBeamThreads) copy_pages_kernel(const CopyParams p) {
   ptx::griddep_launch_dependents();
@@ -534,7 +539,7 @@ struct TableParams {
 constexpr int kTableMostRows = 8192;
 
 // Every block adds up the rows' pages and tokens by itself (a few thousand numbers at most) and looks after its share of the entries: which row
-// an entry belongs to is found by halves.
+// an entry belongs to is found by halves.  One launch and three rounds of loads: 3.5 us for 4 rows, 3.9 for 61 rows of 8192 new tokens.
 __global__ void __launch_bounds__(kBeamThreads) step_tables_kernel(const TableParams p) {
   ptx::griddep_launch_dependents();
   ptx::griddep_wait();

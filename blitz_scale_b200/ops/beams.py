@@ -89,8 +89,8 @@ def _attn_scratch(rows: int, beams: int, q_heads: int, kv_heads: int, head_dim: 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int = 1, *, n: int = 0, keep: int = 0, ended: Optional[torch.Tensor] = None,
                 out: Optional[BeamStep] = None) -> BeamStep:
     """The ``n`` (2 beams) best continuations of every request.  ``logits`` [requests * beams, vocab] in fp16, bf16 or fp32, rows of any pitch;
-    ``scores`` [requests * beams] in fp32, -inf for a row that has ended.  A continuation's value is the row's score plus the token's log
-    probability, a softmax over the whole row; one that is no number (rows with a NaN or +inf) counts as -inf.  Ties go to the lowest beam, then the
+    ``scores`` [requests * beams] in fp32, finite, or -inf for a row that has ended.  A continuation's value is the row's score plus the token's log
+    probability, a softmax over the whole row; one that is no number (rows with a NaN or +inf), or below what fp32 holds, counts as -inf.  Ties go to the lowest beam, then the
     lowest token.  ``ended``: int32 tokens that end a sequence; ``keep`` (beams): how many continuations go on.  At most 64 beams and candidates."""
     dt = _DT3.get(logits.dtype)
     if dt is None:

@@ -166,10 +166,14 @@ class _Search:
         self.batch, self.pages, self.slots = None, [], []
 
     # ------------------------------------------------------------------ one step
+    def _at_once(self) -> bool:
+        """Whether the cache is one that attention reads once for a request's beams; others go through attn_decode, row by row."""
+        e = self.e
+        return e.cfg.family != "hybrid" and e.kv_bits == 16 and e.cfg.head_dim in (64, 128) and e.page_size >= 16
+
     def _step_meta(self, rows: int, buf: _Buffers, splits: int) -> StepMeta:
-        e, t = self.e, buf.tables
-        # (other caches go through attn_decode, row by row)
-        shared = t.shared if e.cfg.family != "hybrid" and e.kv_bits == 16 and e.cfg.head_dim in (64, 128) and e.page_size >= 16 else None
+        t = buf.tables
+        shared = t.shared if self._at_once() else None
         return StepMeta(ids=buf.ids, pos=t.pos, slot=t.slot, page_indices=t.indices, page_indptr=t.indptr, last_page_len=t.last_page_len, seq_slot=buf.seq_slot,
                         batch=rows, num_tokens=rows, num_splits=splits, static_positions=True, beams=self.beams, shared=shared)
 
@@ -206,7 +210,7 @@ class _Search:
         groups = _graph_rows(Q, k, e.max_batch)
         rows, width = groups * k, 1 << (self.width - 1).bit_length()
         longest = max(self.lens) + self.budget
-        splits = e.choose_splits(Q * k, longest, sum(self.lens) * k + Q * k * self.budget)
+        splits = 1 if self._at_once() else e.choose_splits(Q * k, longest, sum(self.lens) * k + Q * k * self.budget)
         key = ("beams", rows, k, width, splits)
         if key not in e._beam_buffers:
             e._beam_buffers[key] = _Buffers(rows, k, width, dev)

@@ -104,6 +104,14 @@ def test_select_no_numbers():
         _select(z.to(dtype), torch.zeros(8, device="cuda"), 4, 8)
 
 
+def test_select_rows_of_one_memory():
+    """Rows that are one row, as at the beginning of a search, and rows of a narrower view."""
+    z = torch.randn(1, 3001, generator=torch.Generator("cuda").manual_seed(2), device="cuda").to(BF)
+    got = _select(z.expand(4, -1), torch.tensor([0.0, -1.0, -math.inf, -0.5], device="cuda"), 4)
+    assert got.token[0, 0] == z[0].argmax() and got.parent[0, 0] == 0
+    _select(z.view(3001)[:3000].view(4, 750)[:, 3:], torch.zeros(4, device="cuda"), 2, 9, 4)
+
+
 def test_select_ended_tokens():
     z = torch.full((4, 300), -5.0, device="cuda")
     z[:, 7], z[:, 9], z[:, 11] = 5.0, 4.0, 3.0
@@ -399,6 +407,13 @@ def test_attention_heads(rep, beams):
     groups[1] = (0, [max(1, t) for t in groups[1][1]])
     for dim in (64, 128):
         _attend(_attend_case(rep, groups, beams, 16, 2, rep, dim, BF), beams, 16, 2, rep, dim, BF)
+
+
+@pytest.mark.parametrize("rows,beams", [(1100, 5), (1030, 1), (2048, 64)])
+def test_attention_of_many_rows(rows, beams):
+    """More rows than one launch takes."""
+    groups = [(i % 3, [1 + (i + j) % 20 if (i + j) % 7 else -1 for j in range(beams)]) for i in range(rows // beams)]
+    _attend(_attend_case(rows, groups, beams, 16, 1, 2, 64, BF), beams, 16, 1, 2, 64, BF)
 
 
 @pytest.mark.parametrize("dim", [64, 128])
