@@ -163,6 +163,7 @@ beam_scan_kernel(const T* __restrict__ logits, int64_t stride, int rows, int voc
 struct SelOut {
   float* score;
   int32_t *parent, *token;
+  int64_t pitch;      // from a request's to the next one's
 };
 // A value (two fp32 in the order of their bits, the larger first; 0: none), and behind it its place, the bits turned: of equal values the lowest place comes
 // first.  Together one number of 128 bits, the larger the better.
@@ -365,21 +366,21 @@ beam_pick_kernel(const T* __restrict__ logits, int64_t stride, int vocab, int gr
   int before = 0;
   for (int i0 = 0; i0 < n; i0 += 32) {
     const int i = i0 + lane;
-    if (i < n) give(all, q * n + i, best[i]);
+    if (i < n) give(all, q * all.pitch + i, best[i]);
     bool on = i < n && best[i].v != 0;
     for (int e = 0; on && e < num_ended; ++e) on = ended[e] != static_cast<int32_t>(~best[i].early);
     const unsigned who = __ballot_sync(0xffffffffu, on);
     const int at = before + __popc(who & ((1u << lane) - 1));
-    if (on && at < keep) give(next, q * keep + at, best[i]);
+    if (on && at < keep) give(next, q * next.pitch + at, best[i]);
     before += __popc(who);
   }
-  for (int i = before + lane; i < keep; i += 32) give(next, q * keep + i, SelCand{0, 0});
+  for (int i = before + lane; i < keep; i += 32) give(next, q * next.pitch + i, SelCand{0, 0});
 }
 
 // ------------------------------------------------------------------ tables of the beams that go on
 struct ForkParams {
   const int32_t *table, *cached, *parents, *pool;
-  int64_t table_stride, pool_stride;
+  int64_t table_stride, pool_stride, parents_stride;
   int width, from, to, pool_size, page, num_pages;   // from: beams of a request in `table`; to: children
   int32_t *out_table, *out_cached, *src, *dst, *tokens;
   int* status;
@@ -400,7 +401,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_fork_kernel(const ForkParam
   ptx::griddep_wait();
   const int first_pool = tid < p.pool_size ? p.pool[q * p.pool_stride + tid] : -1;
   if (tid < p.to) {
-    par[tid] = p.parents[q * p.to + tid];
+    par[tid] = p.parents[q * p.parents_stride + tid];
     fresh[tid] = -1;
   } else if (tid >= kBeamMost && tid < kBeamMost + p.from) {
     held[tid - kBeamMost] = p.cached[q * p.from + tid - kBeamMost];
@@ -699,10 +700,10 @@ using namespace blitz;
 int64_t blitz_beam_select_workspace_bytes(int rows, int vocab, int n, int dtype) { return SelPlan(rows, vocab, dtype).bytes; }
 
 // logits [rows][stride] in fp16 (0), bf16 (1) or fp32 (2); scores [rows]; a request's beams are consecutive rows.  score, parent and token:
-// [rows / beams][n], next_*: [rows / beams][keep].  ended: tokens that end a sequence (num_ended of them).
+// [rows / beams][n], pitch apart, next_*: [rows / beams][keep], next_pitch.  ended: tokens that end a sequence (num_ended of them).
 int blitz_beam_select(const void* logits, int64_t stride, const float* scores, int rows, int vocab, int beams, int n, int keep, const int32_t* ended,
                       int num_ended, void* workspace, float* score, int32_t* parent, int32_t* token, float* next_score, int32_t* next_parent,
-                      int32_t* next_token, int dtype, cudaStream_t stream) {
+                      int32_t* next_token, int64_t pitch, int64_t next_pitch, int dtype, cudaStream_t stream) {
   if (rows <= 0) return 0;
   if (vocab < 1 || beams < 1 || beams > kBeamMost || rows % beams || n < 1 || n > kBeamMost || keep < 1 || keep > n || num_ended < 0) return -1;
   const SelPlan plan(rows, vocab, dtype);
@@ -719,15 +720,15 @@ int blitz_beam_select(const void* logits, int64_t stride, const float* scores, i
       e = once.run([] { return cudaFuncSetAttribute(beam_pick_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBeamMost * kSelGroup * (int)sizeof(T)); });
     if (e == cudaSuccess)
       e = launch_pdl(beam_pick_kernel<T>, dim3(rows / beams), dim3(kBeamThreads), n * kSelGroup * sizeof(T), stream, (const T*)logits, stride, vocab, plan.groups, plan.per_row,
-                     (const SelPart*)parts, (const float*)largest, scores, beams, n, keep, ended, num_ended, SelOut{score, parent, token},
-                     SelOut{next_score, next_parent, next_token});
+                     (const SelPart*)parts, (const float*)largest, scores, beams, n, keep, ended, num_ended, SelOut{score, parent, token, pitch},
+                     SelOut{next_score, next_parent, next_token, next_pitch});
   });
   return (int)e;
 }
 
 // table [requests from][width], cached [requests from], parents [requests][to], pool [requests][pool_size]; the children's table
 // [requests to][width], cached, and the copies to make (src, dst, tokens; -1: none).
-int blitz_beam_fork(const int32_t* table, int64_t table_stride, const int32_t* cached, const int32_t* parents, const int32_t* pool, int64_t pool_stride,
+int blitz_beam_fork(const int32_t* table, int64_t table_stride, const int32_t* cached, const int32_t* parents, int64_t parents_stride, const int32_t* pool, int64_t pool_stride,
                     int requests, int from, int to, int width, int pool_size, int page, int num_pages, int32_t* out_table, int32_t* out_cached, int32_t* src,
                     int32_t* dst, int32_t* tokens, int* status, cudaStream_t stream) {
   if (requests <= 0) return 0;
@@ -737,7 +738,7 @@ int blitz_beam_fork(const int32_t* table, int64_t table_stride, const int32_t* c
   static PerDeviceOnce once;
   cudaError_t e = once.run([] { return cudaFuncSetAttribute(beam_fork_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024); });
   if (e != cudaSuccess) return (int)e;
-  ForkParams p{table, cached, parents, pool, table_stride, pool_stride, width, from, to, pool_size, page, num_pages, out_table, out_cached, src, dst, tokens, status};
+  ForkParams p{table, cached, parents, pool, table_stride, pool_stride, parents_stride, width, from, to, pool_size, page, num_pages, out_table, out_cached, src, dst, tokens, status};
   return (int)launch_pdl(beam_fork_kernel, dim3(requests), dim3(kBeamThreads), smem, stream, p);
 }
 

@@ -161,8 +161,8 @@ def _declare(L: ctypes.CDLL) -> None:
                                     c_p, c_i, c_p, c_i, c_p])
     # beam search
     sig("blitz_beam_select_workspace_bytes", [c_i, c_i, c_i, c_i], c_i64)
-    sig("blitz_beam_select", [c_p, c_i64, c_p, c_i, c_i, c_i, c_i, c_i, c_p, c_i, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_i, c_p])
-    sig("blitz_beam_fork", [c_p, c_i64, c_p, c_p, c_p, c_i64, c_i, c_i, c_i, c_i, c_i, c_i, c_i, c_p, c_p, c_p, c_p, c_p, c_p, c_p])
+    sig("blitz_beam_select", [c_p, c_i64, c_p, c_i, c_i, c_i, c_i, c_i, c_p, c_i, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_i64, c_i64, c_i, c_p])
+    sig("blitz_beam_fork", [c_p, c_i64, c_p, c_p, c_i64, c_p, c_i64, c_i, c_i, c_i, c_i, c_i, c_i, c_i, c_p, c_p, c_p, c_p, c_p, c_p, c_p])
     sig("blitz_copy_pages", [c_p, c_i, c_i64, c_i, c_i64, c_i, c_i64, c_i64, c_i64, c_p, c_p, c_p, c_i, c_p, c_p])
     sig("blitz_step_tables", [c_p, c_i64, c_p, c_p, c_i, c_i, c_i, c_i, c_i, c_i, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_p])
     sig("blitz_attn_beams_workspace_bytes", [c_i, c_i, c_i, c_i, c_i], c_i64)

@@ -20,7 +20,8 @@ BEAMS_MAX = 64      # beams of a request, and candidates of it
 
 class BeamStep(NamedTuple):
     """The best continuations of every request, [requests, n], best first: score, the beam it comes from and its token (-inf, -1 and -1 where there
-    is none); and those that go on, [requests, keep]: the first ones whose token does not end a sequence."""
+    is none); and those that go on, [requests, keep]: the first ones whose token does not end a sequence.  (Where `beam_select` makes them, the first three
+    are columns of one tensor.)"""
     score: torch.Tensor
     parent: torch.Tensor
     token: torch.Tensor
@@ -67,6 +68,11 @@ def _ints(t: torch.Tensor, shape: tuple, what: str) -> torch.Tensor:
     return t
 
 
+def _numbers(t: torch.Tensor, n: int, what: str) -> None:
+    if t.dtype is not torch.int32 or t.shape != (n,) or not t.is_contiguous():
+        raise ValueError(f"{what}: {n} int32 numbers, got {tuple(t.shape)} {t.dtype}")
+
+
 def _rows_of(t: torch.Tensor, what: str) -> tuple:
     """(rows, columns, pitch) of a table of int32"""
     shape, step = t.shape, t.stride()
@@ -110,22 +116,25 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int = 1, *, n
     Q = rows // beams
     if out is None:
         _here(logits, scores, ended)
-        a, b, c = scores.new_empty((3, Q, n)).unbind()
-        d, e, f = scores.new_empty((3, Q, keep)).unbind()
-        out = BeamStep(a, b.view(torch.int32), c.view(torch.int32), d, e.view(torch.int32), f.view(torch.int32))
+        pitch, next_pitch = 3 * n, keep
+        a, b, c = scores.new_empty((Q, pitch), dtype=torch.int32).split_with_sizes((n, n, n), 1)
+        d, e, f = scores.new_empty((3, Q, keep), dtype=torch.int32).unbind()
+        a, d = a.view(torch.float32), d.view(torch.float32)
+        out = BeamStep(a, b, c, d, e, f)
     else:
         _here(logits, scores, ended, *out)
         for t, m, what in zip(out, (n, n, n, keep, keep, keep), BeamStep._fields):
             if t.dtype is not (torch.float32 if what.endswith("score") else torch.int32) or t.numel() != Q * m or not t.is_contiguous():
                 raise ValueError(f"{what}: {Q} x {m} contiguous numbers, got {tuple(t.shape)} {t.dtype}")
+        pitch, next_pitch = n, keep
+        a, b, c, d, e, f = out
     if rows == 0:
         return out
     L = lib()
     work = scores.new_empty(_select_scratch(rows, V, n, dt, _raw_device()))
-    a, b, c, d, e, f = out
     rc = L.blitz_beam_select(logits.data_ptr(), step[0], scores.data_ptr(), rows, V, beams, n, keep, None if ended is None else ended.data_ptr(),
                              0 if ended is None else ended.shape[0], work.data_ptr(), a.data_ptr(), b.data_ptr(), c.data_ptr(), d.data_ptr(), e.data_ptr(),
-                             f.data_ptr(), dt, _stream())
+                             f.data_ptr(), pitch, next_pitch, dt, _stream())
     if rc:
         _check(rc, "blitz_beam_select")
     return out
@@ -141,20 +150,16 @@ def beam_fork(table: torch.Tensor, cached: torch.Tensor, parents: torch.Tensor, 
     child keeps.  A child that there is no page for is a dead row, and the status word says so.  State slots of recurrent layers move alike: a
     table of one column with pages of two tokens, of which one is there.  ``out`` shares no memory with the inputs."""
     rows, W, pitch = _rows_of(table, "table")
-    if parents.dim() != 2 or pool.dim() != 2 or parents.shape[0] < 1:
-        raise ValueError(f"parents and pool: a row per request, got {tuple(parents.shape)} and {tuple(pool.shape)}")
-    Q, to = parents.shape
-    k = rows // Q
-    if rows != Q * k or not 1 <= k <= BEAMS_MAX or not 1 <= to <= BEAMS_MAX or W < 1:
+    Q, to, parents_pitch = _rows_of(parents, "parents")
+    pool_rows, P, pool_pitch = _rows_of(pool, "pool")
+    k = rows // Q if Q else 0
+    if Q < 1 or rows != Q * k or not 1 <= k <= BEAMS_MAX or not 1 <= to <= BEAMS_MAX or W < 1:
         raise ValueError(f"a table of {rows} rows of {W} pages for {Q} requests with {to} children each (at most {BEAMS_MAX} beams)")
     if page_size < 1 or not 1 <= num_pages <= 1600000:
         raise ValueError(f"{num_pages} pages of {page_size} tokens")
-    P, pool_pitch = _rows_of(pool, "pool")[1:]
-    if pool.shape[0] != Q:
+    if pool_rows != Q:
         raise ValueError(f"pool: a row for each of {Q} requests, got {tuple(pool.shape)}")
-    _ints(parents, (Q, to), "parents")
-    if _int32(cached, rows, "cached").shape[0] != rows:
-        raise ValueError(f"cached: {rows} numbers, got {cached.shape[0]}")
+    _numbers(cached, rows, "cached")
     if out is None:
         _here(table, cached, parents, pool)
         R = Q * to
@@ -169,7 +174,7 @@ def beam_fork(table: torch.Tensor, cached: torch.Tensor, parents: torch.Tensor, 
                 out.table.data_ptr() < table.data_ptr() + 4 * ((rows - 1) * pitch + W) and table.data_ptr() < out.table.data_ptr() + 4 * Q * to * W:
             raise ValueError("out.table shares memory with the table")
     a, b, c, d, e = out
-    rc = lib().blitz_beam_fork(table.data_ptr(), pitch, cached.data_ptr(), parents.data_ptr(), pool.data_ptr(), pool_pitch, Q, k, to, W, P, page_size, num_pages,
+    rc = lib().blitz_beam_fork(table.data_ptr(), pitch, cached.data_ptr(), parents.data_ptr(), parents_pitch, pool.data_ptr(), pool_pitch, Q, k, to, W, P, page_size, num_pages,
                                a.data_ptr(), b.data_ptr(), c.data_ptr(), d.data_ptr(), e.data_ptr(), _status_ptr(table), _stream())
     if rc:
         _check(rc, "blitz_beam_fork")
@@ -229,23 +234,21 @@ def step_tables(table: torch.Tensor, cached: torch.Tensor, counts: Optional[torc
     pages, new tokens counted, that the rows of each group of so many have in common.  Rows that do not fit into ``entries`` or ``tokens``, and all
     behind them, sit the step out, as does one whose tokens its table has no place for; the status word says so."""
     R, W, pitch = _rows_of(table, "table")
-    if _int32(cached, R, "cached").shape[0] != R:
-        raise ValueError(f"cached: {R} numbers, got {cached.shape[0]}")
+    _numbers(cached, R, "cached")
     entries = entries or R * W
     ragged = counts is not None
     if page_size < 1 or W < 1 or R * W * page_size >= 1 << 31 or not 0 <= R <= 8192 or entries < 0 or tokens < 0 or beams < 0 or (beams and R % beams):
         raise ValueError(f"{R} rows of {W} pages of {page_size} tokens, {beams} beams, {entries} entries, {tokens} tokens")
     if ragged:
-        if _int32(counts, R, "counts").shape[0] != R:
-            raise ValueError(f"counts: {R} numbers, got {counts.shape[0]}")
+        _numbers(counts, R, "counts")
     elif tokens:
         raise ValueError("tokens: with counts")
     T = tokens if ragged else R
     if out is None:
         _here(table, cached, counts)
-        extra = R + 1 if ragged else 0, R // beams if beams else 0
-        parts = table.new_empty(entries + 2 * (R + T) + 1 + sum(extra)).split_with_sizes((entries, R + 1, R, T, T, *extra))
-        out = StepTables(*parts[:5], parts[5] if ragged else None, parts[6] if beams else None)
+        x, y = R + 1 if ragged else 0, R // beams if beams else 0
+        a, b, c, d, e, f, g = table.new_empty(entries + 2 * (R + T) + 1 + x + y).split_with_sizes((entries, R + 1, R, T, T, x, y))
+        out = StepTables(a, b, c, d, e, f if ragged else None, g if beams else None)
     else:
         sizes = (entries, R + 1, R, T, T, R + 1 if ragged else None, R // beams if beams else None)
         for t, n, what in zip(out, sizes, StepTables._fields):
