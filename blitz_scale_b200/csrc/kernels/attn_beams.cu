@@ -11,15 +11,16 @@
 // sums in scratch (fp32), and a second kernel adds up a row's pieces, always in the same order.  Every block works out the ranges from the tables, so a
 // captured launch follows them.
 //
-// A warp is by itself: it has a ring of three steps (192 KB an SM), asks for the next one (TMA, boxes of 16 tokens x 64 columns) and computes, and nothing in the
-// loop waits for another warp.  (With cp.async instead a warp stood for 2000 to 4000 cycles of a step in its own requests, and computed, 750 to 1500, only then.)
+// A warp is by itself: it asks for its next step (TMA, boxes of 16 tokens x 64 columns) and computes the one that is there, and nothing in the
+// loop waits for another warp.  (With cp.async instead a warp stood for 2000 to 4000 cycles of a step in its own requests, and computed, 750 to 1500, only then.)  Two
+// steps of a warp, 128 KB an SM, are enough to keep memory busy; with three more requests wait in its queues, and SMs are served less evenly.
 //
 // Rounded to 16 bits: the weights, as operands of the second product, and the output.  Scores, maxima, sums and pieces are fp32.
 //
-// Measured, 32 query over 8 KV heads of 128, bf16, us in a graph (bytes of each token once, at the copy rate): 4 beams of 100144 tokens 78.6 (63.1), of 1014 tokens 11.0 (0.75);
-// 32 x 8 beams of 1301 on average, 101 of them their own, 73.0 (44.5).  What bounds it: memory at 5.8 TB/s while all warps run, but
-// equal ranges end between 42 and 61 us (32 x 8) or 52 and 68 (the long one), SMs and warps are not served evenly; then 3 us for tables and first loads, 6.6 to 7.7 for the merge.
-// Tried: queries and page ids of the next piece asked for a piece ahead 77.8 (32 x 8), the heads of a range on one SM 76.4 (79.9 the long one).
+// Measured, 32 query over 8 KV heads of 128, bf16, us in a graph (bytes of each token once, at the copy rate): 4 beams of 100144 tokens 76.2 (63.1), of 1014 tokens 11.0 (0.75);
+// 32 x 8 beams of 1301 on average, 101 of them their own, 67.9 (44.5).  What bounds it: memory at 6.0 to 6.7 TB/s while all warps run, but
+// equal ranges end between 41 and 57 us (32 x 8) or 57 and 66 (the long one); then 3 us for tables and first loads, 6.6 to 7.7 for the merge.
+// Tried: three steps under way 72.9 (78.8 the long one), one 79.6 (84.3); queries and page ids of the next piece asked for a piece ahead 70.4; the heads of a range on one SM 72.8.
 #include "launch.cuh"
 #include "ptx.cuh"
 #include "tmap.cuh"
@@ -132,7 +133,7 @@ template <typename T, int HD>
 __global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const __grid_constant__ CUtensorMap tmap, const BeamAttnParams p) {
   constexpr int kSlab = kBaStep * 128, kSlabs = HD / 64;       // 64 columns of a step's keys, 128 bytes a token, 16-byte columns turned by the token's number
   constexpr int kStage = 2 * kSlabs * kSlab;                  // keys, then values
-  constexpr int kStages = HD == 128 ? 3 : 6;
+  constexpr int kStages = HD == 128 ? 2 : 4;
   extern __shared__ uint8_t ba_raw[];
   uint8_t* ba_smem = ba_raw + (1024 - (ptx::smem_u32(ba_raw) & 1023)) % 1024;
   __shared__ int sums[kBaWarps];
@@ -544,7 +545,7 @@ static BaPlan ba_plan(int rows, int beams, int q_heads, int kv_heads, int hd) {
 template <typename T, int HD>
 static int ba_launch(const CUtensorMap& tmap, const BeamAttnParams& p, cudaStream_t stream) {
   auto kern = attn_beams_kernel<T, HD>;
-  constexpr int kRing = kBaWarps * (HD == 128 ? 3 : 6) * 2 * kBaStep * HD * 2;
+  constexpr int kRing = kBaWarps * (HD == 128 ? 2 : 4) * 2 * kBaStep * HD * 2;
   const int per = p.groups * (1 + p.per_block);
   static PerDeviceOnce once;
   cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 1024); });
