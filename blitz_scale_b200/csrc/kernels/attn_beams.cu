@@ -74,6 +74,7 @@ struct BaRanges {
 // Lengths, common pages and the line of segments, by all threads of a block; arrays in shared memory, or (write) in scratch too.
 __device__ __forceinline__ void ba_line(const BeamAttnParams& p, int* line, int* len, int* common, int* sums) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int shared0 = tid < p.blocks * p.groups ? p.shared[tid % p.groups] : 0;      // (asked for together with the lengths)
   for (int r = tid; r < p.rows; r += kBaThreads) {
     const int pages = p.indptr[r + 1] - p.indptr[r];
     len[r] = pages > 0 ? ((pages - 1) << p.page_shift) + min(max(p.last_page_len[r], 0), 1 << p.page_shift) : 0;
@@ -81,7 +82,7 @@ __device__ __forceinline__ void ba_line(const BeamAttnParams& p, int* line, int*
   __syncthreads();
   for (int i = tid; i < p.blocks * p.groups; i += kBaThreads) {
     const int b = i / p.groups, g = i % p.groups;
-    int most = max(p.shared[g], 0);
+    int most = max(i == tid ? shared0 : p.shared[g], 0);
     bool any = false;
     for (int j = b * p.per_block; j < min((b + 1) * p.per_block, p.beams); ++j) {
       const int n = len[g * p.beams + j];
@@ -144,6 +145,9 @@ __global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const __grid_
   int* line = reinterpret_cast<int*>(ba_smem + kBaWarps * kStages * kStage);
   int* len = line + p.blocks * per + 1;
   int* common = len + p.rows;
+  const int self = warp * gridDim.x + blockIdx.x;
+  const int hv = self % p.heads, range = self / p.heads;
+  const int block = hv % p.blocks, head = hv / p.blocks;       // head: virtual, of `rep` query heads
   if (threadIdx.x == 0) abort_flag = 0;
   if (lane < kStages) ptx::mbar_init(&arrived[warp][lane], 1);
   ptx::fence_mbar_init();
@@ -160,9 +164,6 @@ __global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const __grid_
     p.runs[e] = make_int2(r, x0 < x1 ? ranges.of(x1 - 1) - r + 1 : 0);
   }
 
-  const int self = warp * gridDim.x + blockIdx.x;
-  const int hv = self % p.heads, range = self / p.heads;
-  const int block = hv % p.blocks, head = hv / p.blocks;       // head: virtual, of `rep` query heads
   line += block * per;
   common += block * p.groups;
   const int base = line[0];
