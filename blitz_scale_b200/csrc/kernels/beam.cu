@@ -80,6 +80,13 @@ __device__ __forceinline__ void sel_piece(uint4* to, const T* z, int at, int voc
   }
 }
 
+// The largest of a warp's numbers (those that are none apart).
+__device__ __forceinline__ float sel_redux(float x) {
+  float y;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 struct SelPart {   // of a stretch: its largest logit m, the sum of exp(z - m)
   float m, s;
 };
@@ -132,7 +139,7 @@ beam_scan_kernel(const T* __restrict__ logits, int64_t stride, int rows, int voc
     float top = sel_max<T>(cur[0]);
 #pragma unroll
     for (int j = 1; j < NV; ++j) top = fmaxf(top, sel_max<T>(cur[j]));
-    top = sel_number(__reduce_max_sync(0xffffffffu, sel_ordered(top)));
+    top = sel_redux(top);
     if (lane == 0) largest[static_cast<int64_t>(row) * groups + g] = top;
     if (top > m) {
       sum *= ptx::ex2_approx((m - top) * kLog2e);
