@@ -203,35 +203,78 @@ __device__ __forceinline__ uint64_t sel_make(float z, float base, float2 norm) {
 }
 
 constexpr int kSelRoom = 1024;       // candidates in shared memory
-constexpr int kSelBounds = 128;      // numbers of which the n-th largest is the first bound
+constexpr int kSelNear = 256;        // of them, those that are compared with one another
+constexpr int kSelBounds = 128;      // numbers of which the n-th largest is a bound
 
-// The n best of what `each` goes through, in order, into best[n]; `bound`: a candidate that at least n are not behind ({0, 0}: none known).  each(take) calls take(c) for
+struct SelShared {
+  SelCand cand[kSelRoom], near[kSelNear], tops[kSelBounds], best[kBeamMost], bound;
+  int found, close;
+};
+
+// A candidate that at least n are not behind: every thread has the best one of its own in `mine`, and of the best of pairs of threads it is the n-th.  (Threads
+// without one have {0, thread}: each another one.)
+__device__ __forceinline__ SelCand sel_bound(int n, SelCand mine, SelShared& sh) {
+  const int tid = threadIdx.x;
+  const SelCand other{__shfl_xor_sync(0xffffffffu, mine.v, 1), __shfl_xor_sync(0xffffffffu, mine.early, 1)};
+  if (sel_before(other, mine)) mine = other;
+  if ((tid & 1) == 0) sh.tops[tid >> 1] = mine;
+  __syncthreads();
+  int above = 0;
+#pragma unroll 8
+  for (int i = 0; i < kSelBounds / 2; ++i) above += sel_before(sh.tops[2 * i + (tid & 1)], mine);
+  above += __shfl_xor_sync(0xffffffffu, above, 1);
+  if (above == n - 1) sh.bound = mine;
+  __syncthreads();
+  return sh.bound;
+}
+
+// The n best of what `each` goes through, in order, into sh.best; `bound`: a candidate that at least n are not behind ({0, 0}: none known).  each(take) calls take(c) for
 // all that may count, by all threads of the block.  Where there is no room for those that pass the bound, the n-th best of those that found room is the next bound.
 template <typename Each>
-__device__ __forceinline__ void sel_best(int n, SelCand bound, SelCand* cand, SelCand* best, int* found, const Each& each) {
+__device__ __forceinline__ void sel_best(int n, SelCand bound, SelShared& sh, const Each& each) {
   const int tid = threadIdx.x;
   while (true) {
-    if (tid == 0) *found = 0;
-    if (tid < n) best[tid] = SelCand{0, 0};
+    if (tid == 0) sh.found = sh.close = 0;
+    if (tid < n) sh.best[tid] = SelCand{0, 0};
     __syncthreads();
     each([&](const SelCand& c) {
       if (c.v && !sel_before(bound, c)) {
-        const int at = atomicAdd(found, 1);
-        if (at < kSelRoom) cand[at] = c;
+        const int at = atomicAdd(&sh.found, 1);
+        if (at < kSelRoom) sh.cand[at] = c;
       }
     });
     __syncthreads();
-    const int total = *found, count = min(total, kSelRoom);
+    const int total = sh.found;
+    const SelCand* list = sh.cand;
+    int count = min(total, kSelRoom);
+    if (count > kSelNear) {      // (few rows, small vocabularies: comparing a thousand with one another takes 20 us)
+      SelCand mine{0, static_cast<uint64_t>(tid)};
+      for (int i = tid; i < count; i += kBeamThreads)
+        if (sel_before(sh.cand[i], mine)) mine = sh.cand[i];
+      const SelCand least = sel_bound(n, mine, sh);
+      for (int i = tid; i < count; i += kBeamThreads) {
+        const SelCand c = sh.cand[i];
+        if (!sel_before(least, c)) {
+          const int at = atomicAdd(&sh.close, 1);
+          if (at < kSelNear) sh.near[at] = c;
+        }
+      }
+      __syncthreads();
+      if (sh.close <= kSelNear) {
+        list = sh.near;
+        count = sh.close;
+      }
+    }
     for (int i = tid; i < count; i += kBeamThreads) {
-      const SelCand c = cand[i];
+      const SelCand c = list[i];
       int above = 0;
 #pragma unroll 4
-      for (int k = 0; k < count; ++k) above += sel_before(cand[k], c);
-      if (above < n) best[above] = c;
+      for (int k = 0; k < count; ++k) above += sel_before(list[k], c);
+      if (above < n) sh.best[above] = c;
     }
     __syncthreads();
     if (total <= kSelRoom) return;
-    bound = best[n - 1];
+    bound = sh.best[n - 1];
     __syncthreads();
   }
 }
@@ -243,12 +286,12 @@ beam_pick_kernel(const T* __restrict__ logits, int64_t stride, int vocab, int gr
                  int num_ended, SelOut all, SelOut next) {
   constexpr int kWarps = kBeamThreads / 32, kAhead = 8;
   extern __shared__ __align__(16) uint4 held[];      // elements of the n best groups
-  __shared__ SelCand cand[kSelRoom], best[kBeamMost], tops[kSelBounds];
+  __shared__ SelShared sh;
+  SelCand* best = sh.best;
   __shared__ float2 norm[kBeamMost];
   __shared__ float base[kBeamMost], low[kBeamMost];
-  __shared__ int from[kBeamMost], first[kBeamMost], found, hits;
+  __shared__ int from[kBeamMost], first[kBeamMost], hits;
   __shared__ uint16_t hit[kSelRoom];
-  __shared__ SelCand bound;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, num = beams * groups;
   const int64_t q = blockIdx.x;
   if (tid == 0) hits = 0;
@@ -291,7 +334,6 @@ beam_pick_kernel(const T* __restrict__ logits, int64_t stride, int vocab, int gr
     const int b = min(i / groups, beams - 1);
     return sel_cand(sel_make(z, base[b], norm[b]), i);
   };
-  // A first bound: of the largest of pairs of threads the n-th.
   SelCand mine{0, static_cast<uint64_t>(tid)};       // (each none another one)
   uint64_t mine_v[kAhead];
 #pragma unroll
@@ -304,19 +346,8 @@ beam_pick_kernel(const T* __restrict__ logits, int64_t stride, int vocab, int gr
     const SelCand c = group(i, largest[i]);
     if (c.v > mine.v) mine = c;
   }
-  {
-    const SelCand other{__shfl_xor_sync(0xffffffffu, mine.v, 1), __shfl_xor_sync(0xffffffffu, mine.early, 1)};
-    if (sel_before(other, mine)) mine = other;
-    if ((tid & 1) == 0) tops[tid >> 1] = mine;
-    __syncthreads();
-    int above = 0;
-#pragma unroll 8
-    for (int i = 0; i < kSelBounds / 2; ++i) above += sel_before(tops[2 * i + (tid & 1)], mine);
-    above += __shfl_xor_sync(0xffffffffu, above, 1);
-    if (above == n - 1) bound = mine;
-    __syncthreads();
-  }
-  sel_best(n, bound, cand, best, &found, [&](auto&& take) {
+  const SelCand bound = sel_bound(n, mine, sh);
+  sel_best(n, bound, sh, [&](auto&& take) {
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) take(sel_cand(mine_v[k], tid + k * kBeamThreads));
     for (int i = tid + kAhead * kBeamThreads; i < num; i += kBeamThreads) take(group(i, largest[i]));
@@ -329,11 +360,14 @@ beam_pick_kernel(const T* __restrict__ logits, int64_t stride, int vocab, int gr
     from[tid] = b;
     if (f >= 0) first[tid] = (f - b * groups) * kSelGroup - static_cast<int>((reinterpret_cast<uintptr_t>(logits + (q * beams + b) * stride) & 15) / sizeof(T));
   }
-  const SelCand least = best[n - 1].v ? SelCand{best[n - 1].v, 0} : SelCand{0, 0};
-  if (tid < beams) {       // a row's logits below this one are worth less than the bound
-    const float v = sel_value(least), x = v - base[tid] + norm[tid].x, y = x - 1e-6f * (fabsf(v) + fabsf(base[tid]) + fabsf(norm[tid].x));
-    low[tid] = least.v && y > -INFINITY ? y : -INFINITY;
-  }
+  SelCand least = best[n - 1].v ? SelCand{best[n - 1].v, 0} : SelCand{0, 0};
+  auto lowest = [&] {      // a row's logits below this one are worth less than the bound
+    if (tid < beams) {
+      const float v = sel_value(least), x = v - base[tid] + norm[tid].x, y = x - 1e-6f * (fabsf(v) + fabsf(base[tid]) + fabsf(norm[tid].x));
+      low[tid] = least.v && y > -INFINITY ? y : -INFINITY;
+    }
+  };
+  lowest();
   __syncthreads();
 #pragma unroll 2
   for (int i = tid; i < n * kPieces; i += kBeamThreads) {
@@ -344,17 +378,34 @@ beam_pick_kernel(const T* __restrict__ logits, int64_t stride, int vocab, int gr
   }
   ptx::cp_async_commit();
   ptx::cp_async_wait<0>();      // (a thread looks at what it has copied itself, until the next barrier)
+  for (int turn = 0;; ++turn) {
 #pragma unroll 2
-  for (int i = tid; i < n * kPieces; i += kBeamThreads) {
-    const int b = from[i / kPieces];
-    if (b < 0) break;
-    if (sel_max<T>(held[i]) >= low[b]) {
-      const int at = atomicAdd(&hits, 1);
-      if (at < kSelRoom) hit[at] = static_cast<uint16_t>(i);
+    for (int i = tid; i < n * kPieces; i += kBeamThreads) {
+      const int b = from[i / kPieces];
+      if (b < 0) break;
+      if (sel_max<T>(held[i]) >= low[b]) {
+        const int at = atomicAdd(&hits, 1);
+        if (at < kSelRoom) hit[at] = static_cast<uint16_t>(i);
+      }
     }
+    __syncthreads();
+    if (turn > 0 || hits <= kSelNear) break;
+    // many pieces (small vocabularies, where few groups are not among the best): the n-th of their largest is a higher bound
+    SelCand top{0, static_cast<uint64_t>(tid)};
+#pragma unroll 1
+    for (int t = tid; t < (hits <= kSelRoom ? hits : n * kPieces); t += kBeamThreads) {
+      const int i = hits <= kSelRoom ? hit[t] : t, b = from[i / kPieces];
+      if (b < 0) break;
+      const SelCand c = sel_cand(sel_make(sel_max<T>(held[i]), base[b], norm[b]), i);
+      if (c.v && sel_before(c, top)) top = c;
+    }
+    const SelCand higher = sel_bound(n, top, sh);
+    if (higher.v > least.v) least = SelCand{higher.v, 0};
+    lowest();
+    if (tid == 0) hits = 0;
+    __syncthreads();
   }
-  __syncthreads();
-  sel_best(n, least, cand, best, &found, [&](auto&& take) {
+  sel_best(n, least, sh, [&](auto&& take) {
     const bool few = hits <= kSelRoom;
 #pragma unroll 1
     for (int t = tid; t < (few ? hits : n * kPieces) * E; t += kBeamThreads) {
