@@ -15,10 +15,12 @@
 // loop waits for another warp.  (With cp.async instead a warp stood for 2000 to 4000 cycles of a step in its own requests, and computed, 750 to 1500, only then.)  Two
 // steps of a warp, 128 KB an SM, are enough to keep memory busy; with three more requests wait in its queues, and SMs are served less evenly.
 //
-// Rounded to 16 bits: the weights, as operands of the second product, and the output.  Scores, maxima, sums and pieces are fp32.
+// Rounded to 16 bits: the weights, as operands of the second product, and the output.  Scores, maxima, sums and pieces are fp32.  Errors against 64 bits: bf16 0.0023 where the output's
+// rounding alone is 0.0017, fp16 0.00028 (0.00021), as decode attention has them.  Weights as two 16-bit numbers take that away and cost 8 us of 67 (32 x 8 beams; 5 where only tiles
+// of up to 16 rows have them).
 //
-// Measured, 32 query over 8 KV heads of 128, bf16, us in a graph (bytes of each token once, at the copy rate): 4 beams of 100144 tokens 76.2 (63.1), of 1014 tokens 11.0 (0.75);
-// 32 x 8 beams of 1301 on average, 101 of them their own, 67.9 (44.5).  What bounds it: memory at 6.0 to 6.7 TB/s while all warps run, but
+// Measured, 32 query over 8 KV heads of 128, bf16, us in a graph (bytes of each token once, at the copy rate): 4 beams of 100144 tokens 76.0 (63.1), of 1014 tokens 9.9 (0.75);
+// 32 x 8 beams of 1301 on average, 101 of them their own, 67.2 (44.5).  What bounds it: memory at 6.0 to 6.7 TB/s while all warps run, but
 // equal ranges end between 41 and 57 us (32 x 8) or 57 and 66 (the long one); then 3 us for tables and first loads, 6.6 to 7.7 for the merge.
 // Tried: three steps under way 72.9 (78.8 the long one), one 79.6 (84.3); queries and page ids of the next piece asked for a piece ahead 70.4; the heads of a range on one SM 72.8.
 #include "launch.cuh"
