@@ -22,8 +22,8 @@ constexpr int kBeamMost = 64;  // beams of a request, and candidates of it
 // the n best groups, which it reads again (1 KB each, out of L2 as a rule).  Values are pairs of fp32, 48 bits: candidates of
 // different beams may be nearer to one another than fp32 tells apart, and an exchange of two would be a wrong token.
 //
-// Measured, us in a graph (bytes once at the copy rate): 256 rows of 128256 logits in bf16, 8 beams, n = 24, 23.2 (10.0), of which the scan 15.8; 65 rows of 50257 in fp32
-// 11.2 (2.0); one request of four beams 8.2 (0.2).  The scan is bound by its instructions, a fifth of them the exponentials, and the time until all warps have
+// Measured, us in a graph (bytes once at the copy rate): 256 rows of 128256 logits in bf16, 8 beams, n = 24, 23.0 (10.0), of which the scan 15.4; 65 rows of 50257 in fp32
+// 11.2 (2.0); one request of four beams 8.4 (0.2).  The scan is bound by its instructions, a fifth of them the exponentials, and the time until all warps have
 // their first groups; the second kernel by a chain of some ten short rounds through shared memory.
 constexpr int kSelGroup = 512;
 constexpr int kSelWarps = 48;       // warps of an SM that the scan counts on
