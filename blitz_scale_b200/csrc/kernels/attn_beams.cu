@@ -134,6 +134,19 @@ struct BaPlace {
   int pages, tok0, len;    // first page in `indices`; token that its first step is; tokens of the row
 };
 
+// A wait that ran out: the status word, and as long again for each of the `count` copies that are under way from this stage on.
+__device__ __noinline__ void ba_give_up(int* status, uint64_t* arrived, int stages, int stage, uint32_t phase, int count) {
+  if (status) atomicCAS(status, 0, kStatusTimeoutProducer);
+  for (; count > 0; --count) {
+    int none = 0;
+    ptx::bounded_mbar_wait(&arrived[stage], phase, &none);
+    if (++stage == stages) {
+      stage = 0;
+      phase ^= 1;
+    }
+  }
+}
+
 template <typename T, int HD>
 __global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const __grid_constant__ CUtensorMap tmap, const BeamAttnParams p) {
   constexpr int kSlab = kBaStep * 128, kSlabs = HD / 64;       // 64 columns of a step's keys, 128 bytes a token, 16-byte columns turned by the token's number
@@ -254,7 +267,7 @@ __global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const __grid_
   const uint32_t v_at = ring + kSlabs * kSlab + v_tok * 128 + (((mi >> 1) ^ v_tok & 7) << 4);
   int stage = 0;
   uint32_t phase = 0;
-  bool ok = true;       // (after a wait that ran out the warp waits no more: the status word says so)
+  bool ok = true;       // (a wait that ran out: the status word says so, and the warp ends when its copies have arrived)
   // A piece: TILES of 16 query rows.
   auto piece = [&](auto tiles) {
     constexpr int TILES = decltype(tiles)::value;
@@ -285,9 +298,11 @@ __global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const __grid_
     }
     for (; at.x < at.seg_end; ++at.x) {
       load();
-      if (ok && !ptx::bounded_mbar_wait(&arrived[warp][stage], phase, &abort_flag)) {
-        if (p.status && lane == 0) atomicCAS(p.status, 0, kStatusTimeoutProducer);
+      if (!__all_sync(0xffffffffu, ptx::bounded_mbar_wait(&arrived[warp][stage], phase, &abort_flag))) {
+        if (lane == 0) ba_give_up(p.status, arrived[warp], kStages, stage, phase, ld.x - at.x);
+        __syncwarp();
         ok = false;
+        return;
       }
       const int valid = at.len - (at.tok0 + (at.x - at.seg_beg) * kBaStep);
       if (valid < kBaStep) {      // the row's last step: zeros for values behind its end, whatever the page holds there
@@ -413,7 +428,7 @@ __global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const __grid_
         }
       }
   };
-  while (at.x < x_end) {
+  while (ok && at.x < x_end) {
     if (at.x >= at.seg_end) enter(at);
     if (at.seg < p.groups && p.per_block * p.rep > 16) piece(std::integral_constant<int, 2>{});
     else piece(std::integral_constant<int, 1>{});
