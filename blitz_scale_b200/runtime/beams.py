@@ -120,7 +120,7 @@ class _Search:
         self.e, self.beams, self.budget, self.Q = engine, beams, budget, len(prompts)
         self.lens = [len(p) for p in prompts]
         self.history = [BeamHistory(beams, ended, length_penalty, budget) for _ in prompts]
-        self.n = min(ops.BEAMS_MAX, beams * (1 + max(1, len(ended))))
+        self.n = beams * (1 + max(1, len(ended)))        # (so many of them may end that this is what leaves `beams`)
         dev = engine.device
         self.ended = torch.tensor(list(ended), dtype=torch.int32, device=dev) if len(ended) else None
         specs = [core.SeqSpec(i, list(map(int, p)), 1) for i, p in enumerate(prompts)]
@@ -289,11 +289,12 @@ def beam_search(engine, prompts: Sequence[Sequence[int]], beams: int, max_new_to
         raise RuntimeError("beam search runs on one GPU")
     if not engine.status.fully_loaded():
         raise RuntimeError("model parameters are not loaded")
-    if not 1 <= beams <= ops.BEAMS_MAX // 2 or beams > engine.max_batch:
-        raise ValueError(f"{beams} beams (at most {ops.BEAMS_MAX // 2}, and max_batch={engine.max_batch})")
+    eos = sorted({int(t) for t in eos})
+    most = min(ops.BEAMS_MAX // (1 + max(1, len(eos))), engine.max_batch)
+    if not 1 <= beams <= most:
+        raise ValueError(f"{beams} beams: at most {most} with {len(eos)} tokens that end a continuation, {ops.BEAMS_MAX} candidates and max_batch={engine.max_batch}")
     if max_new_tokens < 1 or any(len(p) < 1 for p in prompts):
         raise ValueError("a prompt of one token and a budget of one at least")
-    eos = [int(t) for t in eos]
     if not all(0 <= t < engine.cfg.vocab for p in (eos, *prompts) for t in p):
         raise ValueError(f"tokens of a vocabulary of {engine.cfg.vocab}")
     per, out = max(1, engine.max_batch // beams), []

@@ -124,6 +124,9 @@ def test_refusals():
             e.beam_search(*args)
     with pytest.raises(ValueError):
         e.beam_search([[1]], 2, 4, eos=[5000])
+    with pytest.raises(ValueError, match="at most 6 with 9"):
+        e.beam_search([[1]], 7, 4, eos=range(9))
+    assert len(e.beam_search([[1]], 6, 2, eos=[*range(9), *range(9)])[0]) == 6
     with pytest.raises(RuntimeError, match="too few free pages"):
         e.beam_search([[1] * 100], 8, 100)
     with pytest.raises(RuntimeError, match="too few free pages"):
