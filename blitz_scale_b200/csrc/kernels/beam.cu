@@ -623,7 +623,7 @@ __global__ void __launch_bounds__(kBeamThreads) step_tables_kernel(const TablePa
   for (int r = r0; r < r1; ++r) {
     const int n = new_tokens(r);
     toks[r + 1] = n;
-    pages[r + 1] = n ? (p.cached[r] + n + p.page - 1) / p.page : 0;
+    pages[r + 1] = n ? (p.cached[r] + n - 1) / p.page + 1 : 0;
     np += pages[r + 1];
     nt += n;
   }
@@ -662,6 +662,11 @@ __global__ void __launch_bounds__(kBeamThreads) step_tables_kernel(const TablePa
   if (rows < p.rows && tid == 0 && blockIdx.x == 0) report(kStatusTooLarge);
   const int total = pages[rows], total_t = toks[rows];
   const int self = blockIdx.x * kBeamThreads + tid, all = gridDim.x * kBeamThreads;
+  auto slot_of = [&](int pg, int at) {       // (-1 where there is no page, or a number that can be none)
+    const int64_t slot = static_cast<int64_t>(pg) * p.page + at % p.page;
+    if (slot > 0x7fffffff) report(kStatusBadIndex);
+    return pg >= 0 && slot <= 0x7fffffff ? static_cast<int>(slot) : -1;
+  };
   auto row_of = [&](const int* begin, int x) {       // the last row that begins at or before x and is not empty
     int lo = 0, hi = rows;                           // begin[lo] <= x < begin[hi]
     while (hi - lo > 1) {
@@ -686,9 +691,8 @@ __global__ void __launch_bounds__(kBeamThreads) step_tables_kernel(const TablePa
     const int n = r < rows ? toks[r + 1] - toks[r] : 0, c = p.cached[r];
     p.last[r] = n ? (c + n - 1) % p.page + 1 : 0;
     if (p.counts == nullptr) {
-      const int pg = n ? p.table[r * p.table_stride + c / p.page] : -1;
       p.pos[r] = n ? c : 0;
-      p.slot[r] = pg >= 0 ? pg * p.page + c % p.page : -1;
+      p.slot[r] = n ? slot_of(p.table[r * p.table_stride + c / p.page], c) : -1;
     }
   }
   if (p.counts) {
@@ -697,8 +701,7 @@ __global__ void __launch_bounds__(kBeamThreads) step_tables_kernel(const TablePa
       if (t < total_t) {
         const int r = row_of(toks, t);
         at = p.cached[r] + t - toks[r];
-        const int pg = p.table[r * p.table_stride + at / p.page];
-        if (pg >= 0) slot = pg * p.page + at % p.page;
+        slot = slot_of(p.table[r * p.table_stride + at / p.page], at);
       }
       p.pos[t] = at;
       p.slot[t] = slot;

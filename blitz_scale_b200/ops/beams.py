@@ -3,7 +3,7 @@
 A request's beams are `beams` consecutive rows.  A row's table names its pages; rows of a request share pages that are full, and of a partly
 filled page each has its own.  A step: `attn_decode_beams` in every layer, `beam_select` on the logits, `beam_fork` for the tables of
 the beams that go on, `copy_pages` for what two of them cannot share, `step_tables` for the next step's inputs.  Everything stays on the GPU
-and can be captured into a graph.
+and can be captured into a graph.  Outputs that a caller gives (`out`) share no memory with the inputs.
 """
 from __future__ import annotations
 
@@ -148,12 +148,12 @@ def beam_fork(table: torch.Tensor, cached: torch.Tensor, parents: torch.Tensor, 
     parent's full pages; a partly filled one goes to the parent's first child, and the others get a fresh page and a copy (`copy_pages`);
     where all pages are full the child gets a fresh one, so that every child has room for a token.  Fresh pages are the first ones of the pool that no
     child keeps.  A child that there is no page for is a dead row, and the status word says so.  State slots of recurrent layers move alike: a
-    table of one column with pages of two tokens, of which one is there.  ``out`` shares no memory with the inputs."""
+    table of one column with pages of two tokens, of which one is there."""
     rows, W, pitch = _rows_of(table, "table")
     Q, to, parents_pitch = _rows_of(parents, "parents")
     pool_rows, P, pool_pitch = _rows_of(pool, "pool")
-    k = rows // Q if Q else 0
-    if Q < 1 or rows != Q * k or not 1 <= k <= BEAMS_MAX or not 1 <= to <= BEAMS_MAX or W < 1:
+    k = rows // Q if Q else 1
+    if rows != Q * k or not 1 <= k <= BEAMS_MAX or not 1 <= to <= BEAMS_MAX or W < 1 or to * W >= 1 << 31:
         raise ValueError(f"a table of {rows} rows of {W} pages for {Q} requests with {to} children each (at most {BEAMS_MAX} beams)")
     if page_size < 1 or not 1 <= num_pages <= 1600000:
         raise ValueError(f"{num_pages} pages of {page_size} tokens")

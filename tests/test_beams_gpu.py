@@ -572,3 +572,53 @@ def test_a_step_captured():
         _close(out, plain.attend(q, cache[1], [t[:-(-m // page)] for t, m in zip(table, lengths)], lengths, kvh * rep, kvh, dim), BF, cache)
         cached = [c + 1 if c >= 0 else c for c in cached]
         sc = scores.tolist()
+
+
+def test_tables_of_pages_that_there_are_not():
+    """A number whose slots do not fit into 32 bits gives none, and the status word says so; one without a page gives none."""
+    table, cached = i32([[1 << 25, 5], [3, 1 << 30], [-1, -1], [7, 9]]), i32([7, 64, 3, 70])
+    for counts, want in ((None, [-1, -1, -1, 9 * 64 + 6]), (i32([1, 0, 2, 3]), [-1, -1, -1, 9 * 64 + 6, 9 * 64 + 7, 9 * 64 + 8])):
+        got = ops.step_tables(table, cached, counts, page_size=64, tokens=0 if counts is None else 6)
+        with pytest.raises(RuntimeError, match="index out of range"):
+            ops.check_status()
+        assert got.slot.tolist() == want
+    got = ops.step_tables(i32([[0]]), i32([(1 << 31) - 3]), page_size=(1 << 31) - 1)
+    ops.check_status()
+    assert got.indptr.tolist() == [0, 1] and got.last_page_len.tolist() == [(1 << 31) - 2] and got.slot.tolist() == [(1 << 31) - 3]
+
+
+def test_no_requests():
+    none = torch.empty(0, 3, dtype=torch.int32, device="cuda")
+    got = ops.beam_fork(none, none[:, 0].contiguous(), torch.empty(0, 4, dtype=torch.int32, device="cuda"), none, page_size=16, num_pages=9)
+    assert [tuple(t.shape) for t in got] == [(0, 3), (0,), (0,), (0,), (0,)]
+    ops.check_status()
+
+
+def test_select_rows_far_apart():
+    """Rows whose elements are more than 2^32 behind the first one's."""
+    pitch = (1 << 31) - 11
+    room = torch.empty(2 * pitch + pitch // 2, dtype=BF, device="cuda")
+    z = torch.as_strided(room, (3, 1003), (pitch, 1), 5)
+    z.copy_(torch.randn(3, 1003, generator=torch.Generator("cuda").manual_seed(2), device="cuda"))
+    _select(z, torch.zeros(3, device="cuda"), 3)
+
+
+def test_pages_far_behind():
+    """Attention over, and copies of, pages more than 2^32 elements into a cache."""
+    page, kvh, rep, dim, beams = 64, 8, 2, 128, 3
+    last = (1 << 32) // (2 * page * kvh * dim) + 40
+    cache = torch.empty(last + 1, 2, page, kvh, dim, dtype=BF, device="cuda")
+    g = torch.Generator("cuda").manual_seed(8)
+    near = torch.randn(8, 2, page, kvh, dim, generator=g, device="cuda").to(BF)
+    cache[:8] = near
+    to = i32(list(range(last - 7, last + 1)))
+    ops.copy_pages(cache, i32(list(range(8))), to)
+    assert torch.equal(cache[-8:], near)
+    q = torch.randn(beams, kvh * rep * dim, generator=g, device="cuda").to(BF)
+    tables = [[0, 1, 2 + b] for b in range(beams)]
+    indptr, tail, shared = i32([0, 3, 6, 9]), i32([5, 64, 17]), i32([2])
+    more = dict(beams=beams, q_heads=kvh * rep, kv_heads=kvh, head_dim=dim, page_size=page)
+    want = ops.attn_decode_beams(q, near, i32(sum(tables, [])), indptr, tail, shared, **more)
+    got = ops.attn_decode_beams(q, cache, i32([last - 7 + p for t in tables for p in t]), indptr, tail, shared, **more)
+    ops.check_status()
+    assert torch.equal(got, want)
