@@ -20,7 +20,7 @@
 // of up to 16 rows have them).
 //
 // Measured, 32 query over 8 KV heads of 128, bf16, us in a graph (bytes of each token once, at the copy rate): 4 beams of 100144 tokens 76.0 (63.1), of 1014 tokens 9.9 (0.75);
-// 32 x 8 beams of 1301 on average, 101 of them their own, 67.2 (44.5).  What bounds it: memory at 6.0 to 6.7 TB/s while all warps run, but
+// 32 x 8 beams of 1301 on average, 101 of them their own, 67.6 (44.5).  What bounds it: memory at 6.0 to 6.7 TB/s while all warps run, but
 // equal ranges end between 41 and 57 us (32 x 8) or 57 and 66 (the long one); then 3 us for tables and first loads, 6.6 to 7.7 for the merge.
 // Tried: three steps under way 72.9 (78.8 the long one), one 79.6 (84.3); queries and page ids of the next piece asked for a piece ahead 70.4; the heads of a range on one SM 72.8.
 #include "launch.cuh"
