@@ -168,8 +168,8 @@ class _Search:
     # ------------------------------------------------------------------ one step
     def _at_once(self) -> bool:
         """Whether the cache is one that attention reads once for a request's beams; others go through attn_decode, row by row."""
-        e = self.e
-        return e.cfg.family != "hybrid" and e.kv_bits == 16 and e.cfg.head_dim in (64, 128) and e.page_size >= 16
+        e, ps = self.e, self.e.page_size
+        return e.cfg.family != "hybrid" and e.kv_bits == 16 and e.cfg.head_dim in (64, 128) and ps >= 16 and ps & (ps - 1) == 0
 
     def _step_meta(self, rows: int, buf: _Buffers, splits: int) -> StepMeta:
         t = buf.tables

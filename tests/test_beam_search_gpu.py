@@ -79,6 +79,18 @@ def test_uniform_model(monkeypatch, use_graphs, page, lens, beams):
     _checked(e, _prompts(lens, 4096), beams, 20, SLACK, monkeypatch=monkeypatch)
 
 
+@pytest.mark.parametrize("page", [8, 48])
+def test_pages_that_attention_of_beams_does_not_take(monkeypatch, page):
+    e = Engine("tiny_gpu", num_pages=200, page_size=page, max_batch=16, max_batch_tokens=512)
+    prompts, free = _prompts([1, 47, 100], 4096, seed=7), e.pool.free_pages
+    if page == 48:        # (nor does the engine's prefill)
+        with pytest.raises(RuntimeError, match="not supported"):
+            e.beam_search(prompts, 3, 12)
+        assert e.pool.free_pages == free
+    else:
+        _checked(e, prompts, 3, 12, SLACK, monkeypatch=monkeypatch)
+
+
 def test_searches_that_end(monkeypatch):
     e = Engine("tiny_gpu", num_pages=200, page_size=16, max_batch=16, max_batch_tokens=512)
     prompts = _prompts([20, 7], 4096, seed=1)
