@@ -194,10 +194,15 @@ __device__ __forceinline__ float2 two_sum(float a, float b) {
   const float s = __fadd_rn(a, b), t = __fadd_rn(s, -a);
   return make_float2(s, __fadd_rn(__fadd_rn(a, -__fadd_rn(s, -t)), __fadd_rn(b, -t)));
 }
-// base + (z - norm), norm = hi + lo.  What is no number, or minus infinity, is no candidate.
-__device__ __forceinline__ uint64_t sel_make(float z, float base, float2 norm) {
-  const float2 d = two_sum(z, -norm.x), v = two_sum(d.x, base);
-  const float rest = __fadd_rn(__fadd_rn(d.y, -norm.y), v.y), hi = __fadd_rn(v.x, rest), lo = __fadd_rn(rest, -__fadd_rn(hi, -v.x));
+// Of a row: its score, its largest logit, and the log of the sum of exp(z - largest) as hi + lo.  (Apart: a row that is masked by the type's lowest number everywhere
+// has a largest logit in which the log of its sum disappears, in 64 bits too.)
+struct SelNorm {
+  float base, top, hi, lo;
+};
+// base + ((z - top) - log of the sum).  What is no number, or minus infinity, is no candidate.
+__device__ __forceinline__ uint64_t sel_make(float z, const SelNorm& r) {
+  const float2 d = two_sum(z, -r.top), e = two_sum(d.x, -r.hi), v = two_sum(e.x, r.base);
+  const float rest = __fadd_rn(__fadd_rn(__fadd_rn(d.y, -r.lo), e.y), v.y), hi = __fadd_rn(v.x, rest), lo = __fadd_rn(rest, -__fadd_rn(hi, -v.x));
   const uint32_t o = sel_ordered(hi);
   return o ? static_cast<uint64_t>(o) << 32 | sel_ordered(lo) : 0ull;
 }
@@ -288,8 +293,8 @@ beam_pick_kernel(const T* __restrict__ logits, int64_t stride, int vocab, int gr
   extern __shared__ __align__(16) uint4 held[];      // elements of the n best groups
   __shared__ SelShared sh;
   SelCand* best = sh.best;
-  __shared__ float2 norm[kBeamMost];
-  __shared__ float base[kBeamMost], low[kBeamMost];
+  __shared__ __align__(16) SelNorm norm[kBeamMost];
+  __shared__ float low[kBeamMost];
   __shared__ int from[kBeamMost], first[kBeamMost], hits;
   __shared__ uint16_t hit[kSelRoom];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, num = beams * groups;
@@ -323,16 +328,15 @@ beam_pick_kernel(const T* __restrict__ logits, int64_t stride, int vocab, int gr
       int e = 1;
       const bool number = s > 0.f && s < INFINITY;
       const float f = number ? 2.f * frexpf(s, &e) : s;
-      const double x = static_cast<double>(m) + (static_cast<double>(logf(f)) + (e - 1) * 0.69314718055994531);
+      const double x = static_cast<double>(logf(f)) + (e - 1) * 0.69314718055994531;
       const float hi = static_cast<float>(x);
-      norm[b] = make_float2(hi, static_cast<float>(x - hi));      // (an infinity: NaN)
-      base[b] = score;
+      norm[b] = SelNorm{score, m, hi, static_cast<float>(x - hi)};      // (an infinity: NaN)
     }
   }
   __syncthreads();
   auto group = [&](int i, float z) {
     const int b = min(i / groups, beams - 1);
-    return sel_cand(sel_make(z, base[b], norm[b]), i);
+    return sel_cand(sel_make(z, norm[b]), i);
   };
   SelCand mine{0, static_cast<uint64_t>(tid)};       // (each none another one)
   uint64_t mine_v[kAhead];
@@ -363,7 +367,8 @@ beam_pick_kernel(const T* __restrict__ logits, int64_t stride, int vocab, int gr
   SelCand least = best[n - 1].v ? SelCand{best[n - 1].v, 0} : SelCand{0, 0};
   auto lowest = [&] {      // a row's logits below this one are worth less than the bound
     if (tid < beams) {
-      const float v = sel_value(least), x = v - base[tid] + norm[tid].x, y = x - 1e-6f * (fabsf(v) + fabsf(base[tid]) + fabsf(norm[tid].x));
+      const SelNorm r = norm[tid];
+      const float v = sel_value(least), x = v - r.base + r.hi + r.top, y = x - 1e-6f * (fabsf(v) + fabsf(r.base) + fabsf(r.hi) + fabsf(r.top));
       low[tid] = least.v && y > -INFINITY ? y : -INFINITY;
     }
   };
@@ -396,7 +401,7 @@ beam_pick_kernel(const T* __restrict__ logits, int64_t stride, int vocab, int gr
     for (int t = tid; t < (hits <= kSelRoom ? hits : n * kPieces); t += kBeamThreads) {
       const int i = hits <= kSelRoom ? hit[t] : t, b = from[i / kPieces];
       if (b < 0) break;
-      const SelCand c = sel_cand(sel_make(sel_max<T>(held[i]), base[b], norm[b]), i);
+      const SelCand c = sel_cand(sel_make(sel_max<T>(held[i]), norm[b]), i);
       if (c.v && sel_before(c, top)) top = c;
     }
     const SelCand higher = sel_bound(n, top, sh);
@@ -412,7 +417,7 @@ beam_pick_kernel(const T* __restrict__ logits, int64_t stride, int vocab, int gr
       const int i = few ? hit[t / E] : t / E, b = from[i / kPieces];
       if (b < 0) break;
       const float y = ldf(reinterpret_cast<const T*>(&held[i]) + t % E);
-      if (y >= low[b]) take(sel_cand(sel_make(y, base[b], norm[b]), static_cast<uint64_t>(b) << 32 | static_cast<uint32_t>(first[i / kPieces] + i % kPieces * E + t % E)));
+      if (y >= low[b]) take(sel_cand(sel_make(y, norm[b]), static_cast<uint64_t>(b) << 32 | static_cast<uint32_t>(first[i / kPieces] + i % kPieces * E + t % E)));
     }
   });
   if (warp > 0) return;
