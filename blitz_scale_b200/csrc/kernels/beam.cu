@@ -59,12 +59,17 @@ __device__ __forceinline__ float sel_max(const uint4& v) {
   }
 }
 
-// A row in groups: those begin on 16-byte boundaries, wherever the row does, so its first one may have some elements before the row.
+// A row in groups, which begin with its first element, wherever in memory that is: a row's sum does not depend on where it begins, so beams of equal logits and scores have equal
+// values.  Copies go by pieces of 16 bytes on their boundaries; where the row begins behind one (by `lead` elements), a group has a piece more, and numbers are shifted as
+// they are read (256 rows of 128257 logits in bf16 24.1 us where 128256 take 21.6; 65 rows of 50257 in fp32 12.3).
 template <typename T>
 struct SelRow {
   static constexpr int E = 16 / sizeof(T), NV = kSelGroup / (32 * E);      // elements of a piece, pieces of a group that a lane has
   static constexpr int kRing = sizeof(T) == 2 ? 4 : 3;                      // groups of a warp that wait in shared memory or are on their way
+  static constexpr int kPieces = 32 * NV;                                   // pieces of a group, but for shifted ones' last
 };
+template <typename T>
+__device__ __forceinline__ int sel_lead(const T* z) { return static_cast<int>((reinterpret_cast<uintptr_t>(z) & 15) / sizeof(T)); }
 // Element `at` of a row and those behind it, a piece, into shared memory; outside the row: -inf.
 template <typename T>
 __device__ __forceinline__ void sel_piece(uint4* to, const T* z, int at, int vocab) {
@@ -80,6 +85,14 @@ __device__ __forceinline__ void sel_piece(uint4* to, const T* z, int at, int voc
   }
 }
 
+// A piece's worth of numbers, from 32-bit word WORDS of piece a on (`half`: 16 bits behind it), the rest from b.
+template <int WORDS>
+__device__ __forceinline__ uint4 sel_shifted(const uint4& a, const uint4& b, int half) {
+  const uint32_t w[9] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, 0u};
+  return make_uint4(__funnelshift_r(w[WORDS], w[WORDS + 1], half), __funnelshift_r(w[WORDS + 1], w[WORDS + 2], half), __funnelshift_r(w[WORDS + 2], w[WORDS + 3], half),
+                    __funnelshift_r(w[WORDS + 3], w[WORDS + 4], half));
+}
+
 // The largest of a warp's numbers (those that are none apart).
 __device__ __forceinline__ float sel_redux(float x) {
   float y;
@@ -91,31 +104,35 @@ struct SelPart {   // of a stretch: its largest logit m, the sum of exp(z - m)
   float m, s;
 };
 
-// A stretch is `length` groups of a row, `per_row` stretches and `groups` groups a row.
-template <typename T>
+// A stretch is `length` groups of a row, `per_row` stretches and `groups` groups a row.  SHIFTED: some rows begin off the boundaries (a kernel apart, since
+// the other one is 2 us of 23 faster without what these need).
+template <typename T, bool SHIFTED>
 __global__ void __launch_bounds__(kBeamThreads, sizeof(T) == 4 ? 4 : 6)
 beam_scan_kernel(const T* __restrict__ logits, int64_t stride, int rows, int vocab, int groups, int per_row, int length, SelPart* __restrict__ parts,
                  float* __restrict__ largest) {
   constexpr int E = SelRow<T>::E, NV = SelRow<T>::NV, kRing = SelRow<T>::kRing;
-  __shared__ uint4 ring[kBeamThreads / 32][kRing][NV * 32];
+  extern __shared__ __align__(16) uint4 sel_ring[];
+  auto ring = reinterpret_cast<uint4 (*)[kRing][SelRow<T>::kPieces + SHIFTED]>(sel_ring);
   ptx::griddep_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t self = static_cast<int64_t>(blockIdx.x) * (kBeamThreads / 32) + warp;
   if (self >= static_cast<int64_t>(rows) * per_row) return;
   const int row = static_cast<int>(self / per_row), g0 = static_cast<int>(self % per_row) * length, g1 = min(groups, g0 + length);
   const T* z = logits + row * stride;
-  const int lead = static_cast<int>((reinterpret_cast<uintptr_t>(z) & 15) / sizeof(T));
+  const int lead = SHIFTED ? sel_lead(z) : 0;
   int ahead = g0, put = 0;
   auto load = [&]() {
     if (ahead < g1) {
       const int first = ahead * kSelGroup - lead, at = first + lane * E;
       uint4* to = &ring[warp][put][lane];
-      if (first >= 0 && first + kSelGroup <= vocab) {
+      if (first >= 0 && first + kSelGroup + (SHIFTED ? E : 0) <= vocab) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) ptx::cp_async_16(ptx::smem_u32(to + j * 32), z + at + j * 32 * E, 16);
+        if (SHIFTED && lane == 0) ptx::cp_async_16(ptx::smem_u32(to + NV * 32), z + at + kSelGroup, 16);
       } else {
 #pragma unroll 1
-        for (int j = 0; j < NV; ++j) sel_piece(to + j * 32, z, at + j * 32 * E, vocab);
+        for (int j = 0; j < NV + SHIFTED; ++j)
+          if (j < NV || lane == 0) sel_piece(to + j * 32, z, at + j * 32 * E, vocab);
       }
     }
     ptx::cp_async_commit();
@@ -131,10 +148,24 @@ beam_scan_kernel(const T* __restrict__ logits, int64_t stride, int rows, int voc
 #pragma unroll 1
   for (int g = g0; g < g1; ++g) {
     load();
-    ptx::cp_async_wait<kRing - 1>();      // (a lane reads what it has copied itself)
+    ptx::cp_async_wait<kRing - 1>();      // (a lane reads what it has copied itself, and where numbers are shifted what its neighbour has)
     uint4 cur[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) cur[j] = ring[warp][get][j * 32 + lane];
+    if (SHIFTED && lead > 0) {
+      __syncwarp();
+      auto shift = [&](auto words) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+          cur[j] = sel_shifted<decltype(words)::value>(cur[j], ring[warp][get][j * 32 + lane + 1], sizeof(T) == 2 ? (lead & 1) * 16 : 0);
+      };
+      const int words = lead * static_cast<int>(sizeof(T)) / 4;
+      if (words == 0) shift(std::integral_constant<int, 0>{});
+      else if (words == 1) shift(std::integral_constant<int, 1>{});
+      else if (words == 2) shift(std::integral_constant<int, 2>{});
+      else shift(std::integral_constant<int, 3>{});
+      __syncwarp();
+    }
     if (++get == kRing) get = 0;
     float top = sel_max<T>(cur[0]);
 #pragma unroll
@@ -284,18 +315,19 @@ __device__ __forceinline__ void sel_best(int n, SelCand bound, SelShared& sh, co
   }
 }
 
+// (two blocks of an SM: left to itself the compiler takes 64 registers, and spills)
 template <typename T>
-__global__ void __launch_bounds__(kBeamThreads)
+__global__ void __launch_bounds__(kBeamThreads, 2)
 beam_pick_kernel(const T* __restrict__ logits, int64_t stride, int vocab, int groups, int per_row, const SelPart* __restrict__ parts,
                  const float* __restrict__ largest, const float* __restrict__ scores, int beams, int n, int keep, const int32_t* __restrict__ ended,
-                 int num_ended, SelOut all, SelOut next) {
+                 int num_ended, bool aligned, SelOut all, SelOut next) {
   constexpr int kWarps = kBeamThreads / 32, kAhead = 8;
   extern __shared__ __align__(16) uint4 held[];      // elements of the n best groups
   __shared__ SelShared sh;
   SelCand* best = sh.best;
   __shared__ __align__(16) SelNorm norm[kBeamMost];
   __shared__ float low[kBeamMost];
-  __shared__ int from[kBeamMost], first[kBeamMost], hits;
+  __shared__ int from[kBeamMost], first[kBeamMost], start[kBeamMost], hits;
   __shared__ uint16_t hit[kSelRoom];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, num = beams * groups;
   const int64_t q = blockIdx.x;
@@ -358,11 +390,16 @@ beam_pick_kernel(const T* __restrict__ logits, int64_t stride, int vocab, int gr
   });
   // The n best elements are in these groups: one in any other group has their largest elements before it.  Those that reach the bound are in few pieces, which are
   // shared out by elements.
-  constexpr int E = SelRow<T>::E, kPieces = 32 * SelRow<T>::NV;
+  constexpr int E = SelRow<T>::E, kPieces = SelRow<T>::kPieces;
+  const int pieces = aligned ? kPieces : kPieces + 1;      // (of a group: the first and the last one may have elements of its neighbours, which do not count)
+  auto group_of = [&](int i) { return aligned ? i / kPieces : i / (kPieces + 1); };
   if (tid < n) {
     const int f = best[tid].v ? static_cast<int>(~best[tid].early) : -1, b = f < 0 ? -1 : f / groups;
     from[tid] = b;
-    if (f >= 0) first[tid] = (f - b * groups) * kSelGroup - static_cast<int>((reinterpret_cast<uintptr_t>(logits + (q * beams + b) * stride) & 15) / sizeof(T));
+    if (f >= 0) {
+      start[tid] = (f - b * groups) * kSelGroup;
+      first[tid] = start[tid] - sel_lead(logits + (q * beams + b) * stride);
+    }
   }
   SelCand least = best[n - 1].v ? SelCand{best[n - 1].v, 0} : SelCand{0, 0};
   auto lowest = [&] {      // a row's logits below this one are worth less than the bound
@@ -375,18 +412,18 @@ beam_pick_kernel(const T* __restrict__ logits, int64_t stride, int vocab, int gr
   lowest();
   __syncthreads();
 #pragma unroll 2
-  for (int i = tid; i < n * kPieces; i += kBeamThreads) {
-    const int b = from[i / kPieces], at = first[i / kPieces] + i % kPieces * E;
+  for (int i = tid; i < n * pieces; i += kBeamThreads) {
+    const int at = group_of(i), b = from[at];
     if (b < 0) break;
     const T* z = logits + (q * beams + b) * stride;
-    sel_piece(&held[i], z, at, vocab);
+    sel_piece(&held[i], z, first[at] + (i - at * pieces) * E, vocab);
   }
   ptx::cp_async_commit();
   ptx::cp_async_wait<0>();      // (a thread looks at what it has copied itself, until the next barrier)
   for (int turn = 0;; ++turn) {
 #pragma unroll 2
-    for (int i = tid; i < n * kPieces; i += kBeamThreads) {
-      const int b = from[i / kPieces];
+    for (int i = tid; i < n * pieces; i += kBeamThreads) {
+      const int b = from[group_of(i)];
       if (b < 0) break;
       if (sel_max<T>(held[i]) >= low[b]) {
         const int at = atomicAdd(&hits, 1);
@@ -398,9 +435,10 @@ beam_pick_kernel(const T* __restrict__ logits, int64_t stride, int vocab, int gr
     // many pieces (small vocabularies, where few groups are not among the best): the n-th of their largest is a higher bound
     SelCand top{0, static_cast<uint64_t>(tid)};
 #pragma unroll 1
-    for (int t = tid; t < (hits <= kSelRoom ? hits : n * kPieces); t += kBeamThreads) {
-      const int i = hits <= kSelRoom ? hit[t] : t, b = from[i / kPieces];
+    for (int t = tid; t < (hits <= kSelRoom ? hits : n * pieces); t += kBeamThreads) {
+      const int i = hits <= kSelRoom ? hit[t] : t, at = group_of(i), b = from[at];
       if (b < 0) break;
+      if (!aligned && (i == at * pieces || i == at * pieces + kPieces)) continue;
       const SelCand c = sel_cand(sel_make(sel_max<T>(held[i]), norm[b]), i);
       if (c.v && sel_before(c, top)) top = c;
     }
@@ -413,11 +451,13 @@ beam_pick_kernel(const T* __restrict__ logits, int64_t stride, int vocab, int gr
   sel_best(n, least, sh, [&](auto&& take) {
     const bool few = hits <= kSelRoom;
 #pragma unroll 1
-    for (int t = tid; t < (few ? hits : n * kPieces) * E; t += kBeamThreads) {
-      const int i = few ? hit[t / E] : t / E, b = from[i / kPieces];
+    for (int t = tid; t < (few ? hits : n * pieces) * E; t += kBeamThreads) {
+      const int i = few ? hit[t / E] : t / E, at = group_of(i), b = from[at];
       if (b < 0) break;
+      const int token = first[at] + (i - at * pieces) * E + t % E;
       const float y = ldf(reinterpret_cast<const T*>(&held[i]) + t % E);
-      if (y >= low[b]) take(sel_cand(sel_make(y, norm[b]), static_cast<uint64_t>(b) << 32 | static_cast<uint32_t>(first[i / kPieces] + i % kPieces * E + t % E)));
+      if (y >= low[b] && static_cast<unsigned>(token - start[at]) < kSelGroup)
+        take(sel_cand(sel_make(y, norm[b]), static_cast<uint64_t>(b) << 32 | static_cast<uint32_t>(token)));
     }
   });
   if (warp > 0) return;
@@ -746,9 +786,8 @@ __global__ void __launch_bounds__(kBeamThreads) step_tables_kernel(const TablePa
 struct SelPlan {
   int groups, per_row, length;
   int64_t largest, bytes;       // where the groups' largest are in the scratch, its size
-  SelPlan(int64_t rows, int vocab, int dtype) {
-    // (a row may begin behind a 16-byte boundary: up to 7 elements more)
-    groups = static_cast<int>((static_cast<int64_t>(vocab) + (dtype == 2 ? 3 : 7) + kSelGroup - 1) / kSelGroup);
+  SelPlan(int64_t rows, int vocab) {
+    groups = static_cast<int>((static_cast<int64_t>(vocab) + kSelGroup - 1) / kSelGroup);
     const int64_t warps = static_cast<int64_t>(kSelWarps) * device_sm_count() / (rows < 1 ? 1 : rows);
     length = warps < 1 ? kSelStretch : static_cast<int>((groups + warps - 1) / warps);
     if (length > kSelStretch) length = kSelStretch;
@@ -763,7 +802,7 @@ struct SelPlan {
 extern "C" {
 using namespace blitz;
 
-int64_t blitz_beam_select_workspace_bytes(int rows, int vocab, int n, int dtype) { return SelPlan(rows, vocab, dtype).bytes; }
+int64_t blitz_beam_select_workspace_bytes(int rows, int vocab, int n, int dtype) { return SelPlan(rows, vocab).bytes; }
 
 // logits [rows][stride] in fp16 (0), bf16 (1) or fp32 (2); scores [rows]; a request's beams are consecutive rows.  score, parent and token:
 // [rows / beams][n], pitch apart, next_*: [rows / beams][keep], next_pitch.  ended: tokens that end a sequence (num_ended of them).
@@ -772,22 +811,29 @@ int blitz_beam_select(const void* logits, int64_t stride, const float* scores, i
                       int32_t* next_token, int64_t pitch, int64_t next_pitch, int dtype, cudaStream_t stream) {
   if (rows <= 0) return 0;
   if (vocab < 1 || beams < 1 || beams > kBeamMost || rows % beams || n < 1 || n > kBeamMost || keep < 1 || keep > n || num_ended < 0) return -1;
-  const SelPlan plan(rows, vocab, dtype);
+  const SelPlan plan(rows, vocab);
   const int64_t blocks = (static_cast<int64_t>(rows) * plan.per_row + kBeamThreads / 32 - 1) / (kBeamThreads / 32);
   if (blocks > 0x7fffffff || static_cast<int64_t>(beams) * plan.groups > 0x7fffffff || vocab > 0x7fffffff - 2 * kSelGroup) return -1;
   SelPart* parts = reinterpret_cast<SelPart*>(workspace);
   float* largest = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + plan.largest);
   cudaError_t e = cudaSuccess;
   BLITZ_DISPATCH_DTYPE3(dtype, {
-    e = launch_pdl(beam_scan_kernel<T>, dim3((unsigned)blocks), dim3(kBeamThreads), 0, stream, (const T*)logits, stride, rows, vocab, plan.groups, plan.per_row,
-                   plan.length, parts, largest);
+    constexpr int kRing = kBeamThreads / 32 * SelRow<T>::kRing * 16;       // bytes of the scan's rings for each piece of a group
+    const bool aligned = ((reinterpret_cast<uintptr_t>(logits) | static_cast<uint64_t>(stride) * sizeof(T)) & 15) == 0;
+    const int pieces = aligned ? SelRow<T>::kPieces : SelRow<T>::kPieces + 1;
+    auto scan = aligned ? beam_scan_kernel<T, false> : beam_scan_kernel<T, true>;
     static PerDeviceOnce once;
+    e = once.run([] {
+      const cudaError_t first = cudaFuncSetAttribute(beam_scan_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing * (SelRow<T>::kPieces + 1));
+      return first != cudaSuccess ? first
+                                  : cudaFuncSetAttribute(beam_pick_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBeamMost * (SelRow<T>::kPieces + 1) * 16);
+    });
     if (e == cudaSuccess)
-      e = once.run([] { return cudaFuncSetAttribute(beam_pick_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBeamMost * kSelGroup * (int)sizeof(T)); });
+      e = launch_pdl(scan, dim3((unsigned)blocks), dim3(kBeamThreads), kRing * pieces, stream, (const T*)logits, stride, rows, vocab, plan.groups, plan.per_row,
+                     plan.length, parts, largest);
     if (e == cudaSuccess)
-      e = launch_pdl(beam_pick_kernel<T>, dim3(rows / beams), dim3(kBeamThreads), n * kSelGroup * sizeof(T), stream, (const T*)logits, stride, vocab, plan.groups, plan.per_row,
-                     (const SelPart*)parts, (const float*)largest, scores, beams, n, keep, ended, num_ended, SelOut{score, parent, token, pitch},
-                     SelOut{next_score, next_parent, next_token, next_pitch});
+      e = launch_pdl(beam_pick_kernel<T>, dim3(rows / beams), dim3(kBeamThreads), n * pieces * 16, stream, (const T*)logits, stride, vocab, plan.groups, plan.per_row, (const SelPart*)parts, (const float*)largest, scores, beams, n, keep, ended, num_ended, aligned,
+                     SelOut{score, parent, token, pitch}, SelOut{next_score, next_parent, next_token, next_pitch});
   });
   return (int)e;
 }
