@@ -51,6 +51,7 @@ struct BeamAttnParams {
   int heads;                    // virtual heads x blocks
   int ranges_most;
   int page_shift, max_pages;
+  float least;                  // the lowest reference: finite, times the scale too
   float scale_log2, slack, cap_scale, cap_log2;      // the scale's size (1 under a cap, or where it is zero); keep and flip: zero or its sign, for the queries
   uint32_t keep, flip;
   const void* sink;
@@ -291,7 +292,8 @@ __global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const __grid_
     float o[TILES][HD / 8][4], m[TILES][2], l[TILES][2], limit[TILES][2];
 #pragma unroll
     for (int t = 0; t < TILES; ++t) {
-      m[t][0] = m[t][1] = limit[t][0] = limit[t][1] = -INFINITY;
+      m[t][0] = m[t][1] = p.least;        // (finite: scores of minus infinity alone leave a piece of no weight)
+      limit[t][0] = limit[t][1] = -INFINITY;
       l[t][0] = l[t][1] = 0.f;
 #pragma unroll
       for (int i = 0; i < HD / 8; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.f;
@@ -527,7 +529,7 @@ __global__ void __launch_bounds__(kBaThreads, WARPS > 1 ? 2 : 4) attn_beams_merg
     acc.w += __shfl_xor_sync(0xffffffffu, acc.w, 16);
     if (team > 0) return;
   }
-  const float f = L > 0.f ? 1.f / L : 0.f;
+  const float f = live ? 1.f / L : 0.f;      // (live rows without weight: no number)
   stf4(reinterpret_cast<T*>(p.out) + row * p.out_stride + static_cast<int64_t>(qh) * HD + 4 * c, make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
 }
 
@@ -617,6 +619,7 @@ int blitz_attn_beams(const void* q, int64_t q_stride, const void* kv, const int3
   p.flip = plain && scale < 0.f ? 0x80008000u : 0u;
   p.scale_log2 = plain && scale != 0.f ? fabsf(scale) * 1.4426950408889634f : 1.f;
   p.slack = 8.f / p.scale_log2;
+  p.least = -3.4e38f / fmaxf(p.scale_log2, 1.f);
   p.cap_scale = cap > 0.f ? scale / cap : 0.f;
   p.cap_log2 = cap * 1.4426950408889634f;
   p.sink = sink;
