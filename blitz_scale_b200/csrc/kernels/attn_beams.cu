@@ -23,6 +23,8 @@
 // 32 x 8 beams of 1301 on average, 101 of them their own, 67.6 (44.5).  What bounds it: memory at 6.0 to 6.7 TB/s while all warps run, but
 // equal ranges end between 41 and 57 us (32 x 8) or 57 and 66 (the long one); then 3 us for tables and first loads, 6.6 to 7.7 for the merge.
 // Tried: three steps under way 72.9 (78.8 the long one), one 79.6 (84.3); queries and page ids of the next piece asked for a piece ahead 70.4; the heads of a range on one SM 72.8.
+#include <cfloat>
+
 #include "launch.cuh"
 #include "ptx.cuh"
 #include "tmap.cuh"
@@ -51,13 +53,12 @@ struct BeamAttnParams {
   int heads;                    // virtual heads x blocks
   int ranges_most;
   int page_shift, max_pages;
-  float least;                  // the lowest reference: finite, times the scale too
   float scale_log2, slack, cap_scale, cap_log2;      // the scale's size (1 under a cap, or where it is zero); keep and flip: zero or its sign, for the queries
   uint32_t keep, flip;
   const void* sink;
   int2* runs;                   // [blocks][groups + groups per_block] of each segment: its first piece's range, pieces
   float *o_common, *o_own;      // partial sums
-  float2 *ml_common, *ml_own;   // maximum (log2 units) and sum of each
+  float2 *ml_common, *ml_own;   // reference (before the scale) and sum of each
   int static_table;
   int* status;
 };
@@ -261,6 +262,7 @@ __global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const __grid_
   };
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) load();
+  const uint64_t scale2 = ptx::f32x2(p.scale_log2, p.scale_log2);
   const int g8 = lane >> 2, t4 = lane & 3, mi = lane >> 3, mr = lane & 7;
   // what the lane reads of a stage with ldmatrix: keys of its token from 16-byte column mi & 1 on, values of its token from column mi >> 1 on
   const int k_tok = (mi >> 1) * 8 + mr, v_tok = (mi & 1) * 8 + mr;
@@ -292,7 +294,7 @@ __global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const __grid_
     float o[TILES][HD / 8][4], m[TILES][2], l[TILES][2], limit[TILES][2];
 #pragma unroll
     for (int t = 0; t < TILES; ++t) {
-      m[t][0] = m[t][1] = p.least;        // (finite: scores of minus infinity alone leave a piece of no weight)
+      m[t][0] = m[t][1] = -FLT_MAX;        // (finite: scores of minus infinity alone leave a piece of no weight)
       limit[t][0] = limit[t][1] = -INFINITY;
       l[t][0] = l[t][1] = 0.f;
 #pragma unroll
@@ -362,7 +364,7 @@ __global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const __grid_
             float x = fmaxf(top[t][k], __shfl_xor_sync(0xffffffffu, top[t][k], 1));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
             x = fmaxf(x, m[t][k]);
-            a[k] = ptx::ex2_approx(__fmul_rn(m[t][k], p.scale_log2) - __fmul_rn(x, p.scale_log2));
+            a[k] = ptx::ex2_approx((m[t][k] - x) * p.scale_log2);
             m[t][k] = x;
             limit[t][k] = x + p.slack;
             l[t][k] *= a[k];
@@ -378,11 +380,14 @@ __global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const __grid_
       }
 #pragma unroll
       for (int t = 0; t < TILES; ++t) {
-        const float ref[2] = {-__fmul_rn(m[t][0], p.scale_log2), -__fmul_rn(m[t][1], p.scale_log2)};
+        // (the reference is taken off before the scale: times it a large one is rounded by more than an exponential bears)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float& x = s[t][e >> 2][e & 3];
-          x = ptx::ex2_approx(fmaf(x, p.scale_log2, ref[(e >> 1) & 1]));
+        for (int e = 0; e < 8; e += 2) {
+          const float ref = -m[t][(e >> 1) & 1];
+          float* x = &s[t][e >> 2][e & 3];
+          const float2 y = ptx::f32x2_get(ptx::mul_f32x2(ptx::add_f32x2(ptx::f32x2(x[0], x[1]), ptx::f32x2(ref, ref)), scale2));
+          x[0] = ptx::ex2_approx(y.x);
+          x[1] = ptx::ex2_approx(y.y);
         }
 #pragma unroll
         for (int k = 0; k < 2; ++k) l[t][k] += (s[t][0][2 * k] + s[t][0][2 * k + 1]) + (s[t][1][2 * k] + s[t][1][2 * k + 1]);
@@ -423,7 +428,7 @@ __global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const __grid_
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
         const int i = t * 16 + half * 8 + g8;
         if (i < live) {
-          if (t4 == 0) pml[slot + i] = make_float2(m[t][half] * p.scale_log2, sum);
+          if (t4 == 0) pml[slot + i] = make_float2(m[t][half], sum);
           float* to = po + (slot + i) * HD + 2 * t4;
 #pragma unroll
           for (int k = 0; k < HD / 8; ++k) *reinterpret_cast<float2*>(to + k * 8) = make_float2(o[t][k][2 * half], o[t][k][2 * half + 1]);
@@ -472,22 +477,25 @@ __global__ void __launch_bounds__(kBaThreads, WARPS > 1 ? 2 : 4) attn_beams_merg
   for (int k = 0; k < kHeld; ++k) held[k] = lane + 32 * k < n ? ml(lane + 32 * k) : make_float2(-INFINITY, 0.f);
 #pragma unroll
   for (int k = 0; k < kEarly; ++k) early[k] = team + kTeams * k < n ? sums(team + kTeams * k) : make_float4(0.f, 0.f, 0.f, 0.f);
-  float M = live ? snk : -INFINITY, L = 0.f;
+  float M = -INFINITY, L = 0.f;
 #pragma unroll
   for (int k = 0; k < kHeld; ++k) M = fmaxf(M, held[k].x);
   for (int i = lane + 32 * kHeld; i < n; i += 32) M = fmaxf(M, ml(i).x);
   M = warp_max(M);
   const float ref = M > -INFINITY ? M : 0.f;
+  // weights beside the largest reference, or beside the sink where that is larger
+  const float sink_above = snk > -INFINITY ? snk - ref * p.scale_log2 : -INFINITY, less = fmaxf(sink_above, 0.f);
+  auto weight = [&](float x) { return ptx::ex2_approx(fmaf(x - ref, p.scale_log2, -less)); };
 #pragma unroll
   for (int k = 0; k < kHeld; ++k) {
-    held[k].x = ptx::ex2_approx(held[k].x - ref);
+    held[k].x = weight(held[k].x);
     L += held[k].y * held[k].x;
   }
   for (int i = lane + 32 * kHeld; i < n; i += 32) {
     const float2 x = ml(i);
-    L += x.y * ptx::ex2_approx(x.x - ref);
+    L += x.y * weight(x.x);
   }
-  L = warp_sum(L) + (p.sink && live ? ptx::ex2_approx(snk - ref) : 0.f);
+  L = warp_sum(L) + (p.sink && live ? ptx::ex2_approx(fminf(sink_above, 0.f)) : 0.f);
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   auto add = [&](const float4& x, float w) {
     acc.x += x.x * w;
@@ -509,7 +517,7 @@ __global__ void __launch_bounds__(kBaThreads, WARPS > 1 ? 2 : 4) attn_beams_merg
       early[k] = in ? sums(i0 + kTeams * k) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
 #pragma unroll
-    for (int k = 0; k < kEarly; ++k) add(early[k], ptx::ex2_approx(top[k] - ref));
+    for (int k = 0; k < kEarly; ++k) add(early[k], weight(top[k]));
   }
   if constexpr (WARPS > 1) {
     part[team][c] = acc;
@@ -619,7 +627,6 @@ int blitz_attn_beams(const void* q, int64_t q_stride, const void* kv, const int3
   p.flip = plain && scale < 0.f ? 0x80008000u : 0u;
   p.scale_log2 = plain && scale != 0.f ? fabsf(scale) * 1.4426950408889634f : 1.f;
   p.slack = 8.f / p.scale_log2;
-  p.least = -3.4e38f / fmaxf(p.scale_log2, 1.f);
   p.cap_scale = cap > 0.f ? scale / cap : 0.f;
   p.cap_log2 = cap * 1.4426950408889634f;
   p.sink = sink;

@@ -88,6 +88,19 @@ def test_rows_of_minus_infinity_alone():
     assert (out == 0).all()
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_scores_of_the_largest_numbers(dtype):
+    """Scores up to what fp32 holds: below the largest ones nothing has weight."""
+    q, kv, lists, lengths = _case(3, [30, 5], 16, 1, 2, 64, dtype)
+    q.fill_(1.0)
+    big = torch.finfo(dtype).max / 128
+    for p in range(kv.shape[0]):
+        kv[p, 0] = -big
+    kv[1, 0, 3], kv[1, 0, 9] = -big / 2, -big / 2
+    for scale in (None, 1.0, 1.5):
+        _checked(q, kv, lists, lengths, 3, 1, 2, **({} if scale is None else dict(sm_scale=scale)))
+
+
 def test_calls_repeat_themselves():
     """The same call gives the same bits, whatever the warps' order was."""
     q, kv, lists, lengths = _case(70, [100, 37, 200, 1, 64, 9, 18, 77], 64, 8, 4, 128, BF)
