@@ -149,6 +149,11 @@ __device__ __noinline__ void ba_give_up(int* status, uint64_t* arrived, int stag
   }
 }
 
+// All weights are 2^-8 of what they are beside their reference, so that they are one at most and sums of bf16 values stay below tokens x values.  (fp16: its values are far
+// from what fp32 holds, and small weights would lose digits.)
+template <typename T>
+__host__ __device__ constexpr float ba_small() { return std::is_same<T, __nv_bfloat16>::value ? 8.f : 0.f; }
+
 template <typename T, int HD>
 __global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const __grid_constant__ CUtensorMap tmap, const BeamAttnParams p) {
   constexpr int kSlab = kBaStep * 128, kSlabs = HD / 64;       // 64 columns of a step's keys, 128 bytes a token, 16-byte columns turned by the token's number
@@ -262,7 +267,7 @@ __global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const __grid_
   };
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) load();
-  const uint64_t scale2 = ptx::f32x2(p.scale_log2, p.scale_log2);
+  const uint64_t scale2 = ptx::f32x2(p.scale_log2, p.scale_log2), small2 = ptx::f32x2(-ba_small<T>(), -ba_small<T>());
   const int g8 = lane >> 2, t4 = lane & 3, mi = lane >> 3, mr = lane & 7;
   // what the lane reads of a stage with ldmatrix: keys of its token from 16-byte column mi & 1 on, values of its token from column mi >> 1 on
   const int k_tok = (mi >> 1) * 8 + mr, v_tok = (mi & 1) * 8 + mr;
@@ -343,7 +348,7 @@ __global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const __grid_
           for (int e = 0; e < 8; ++e)
             if ((e >> 2) * 8 + 2 * t4 + (e & 1) >= valid) s[t][e >> 2][e & 3] = -INFINITY;
       }
-      // The weights' reference: the largest score at first, a later one only where a score is 2^8 above it (weights up to 256 cost no precision; a maximum that is
+      // The weights' reference: the largest score at first, a later one only where a score is 2^8 above it (weights 256 times as large cost no precision; a maximum that is
       // followed costs four shuffles, and a vote, in every step).
       uint32_t pa[TILES][4];
       float top[TILES][2];
@@ -385,7 +390,7 @@ __global__ void __launch_bounds__(kBaThreads, 1) attn_beams_kernel(const __grid_
         for (int e = 0; e < 8; e += 2) {
           const float ref = -m[t][(e >> 1) & 1];
           float* x = &s[t][e >> 2][e & 3];
-          const float2 y = ptx::f32x2_get(ptx::mul_f32x2(ptx::add_f32x2(ptx::f32x2(x[0], x[1]), ptx::f32x2(ref, ref)), scale2));
+          const float2 y = ptx::f32x2_get(ptx::fma_f32x2(ptx::add_f32x2(ptx::f32x2(x[0], x[1]), ptx::f32x2(ref, ref)), scale2, small2));
           x[0] = ptx::ex2_approx(y.x);
           x[1] = ptx::ex2_approx(y.y);
         }
@@ -495,7 +500,7 @@ __global__ void __launch_bounds__(kBaThreads, WARPS > 1 ? 2 : 4) attn_beams_merg
     const float2 x = ml(i);
     L += x.y * weight(x.x);
   }
-  L = warp_sum(L) + (p.sink && live ? ptx::ex2_approx(fminf(sink_above, 0.f)) : 0.f);
+  L = warp_sum(L) + (p.sink && live ? ptx::ex2_approx(fminf(sink_above, 0.f) - ba_small<T>()) : 0.f);
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   auto add = [&](const float4& x, float w) {
     acc.x += x.x * w;

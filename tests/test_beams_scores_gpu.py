@@ -101,6 +101,19 @@ def test_scores_of_the_largest_numbers(dtype):
         _checked(q, kv, lists, lengths, 3, 1, 2, **({} if scale is None else dict(sm_scale=scale)))
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("common", [0, 8])
+def test_values_near_the_largest_number(dim, common):
+    """Values whose mean fp32 holds, behind scores that rise by 2^7.9 from step to step of a piece: weights are one at most, so that sums stay below tokens x values."""
+    page, kvh, rep = 16, 1, 4
+    q, kv, lists, lengths = _case(common, [64, 33], page, kvh, rep, dim, BF)
+    q.fill_(1.0)
+    kv[:, 0] = 0.0
+    kv[1::2, 0, :, :, 0] = 7.875
+    kv[:, 1] = kv[:, 1].abs().clamp(0.5, 1.0) * 1.5e36
+    _checked(q, kv, lists, lengths, common, kvh, rep, sm_scale=math.log(2.0))
+
+
 def test_calls_repeat_themselves():
     """The same call gives the same bits, whatever the warps' order was."""
     q, kv, lists, lengths = _case(70, [100, 37, 200, 1, 64, 9, 18, 77], 64, 8, 4, 128, BF)
