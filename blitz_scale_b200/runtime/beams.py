@@ -120,7 +120,7 @@ class _Search:
         self.e, self.beams, self.budget, self.Q = engine, beams, budget, len(prompts)
         self.lens = [len(p) for p in prompts]
         self.history = [BeamHistory(beams, ended, length_penalty, budget) for _ in prompts]
-        self.n = beams * (1 + max(1, len(ended)))        # (so many of them may end that this is what leaves `beams`)
+        self.n = min(ops.BEAMS_MAX, beams * (1 + max(1, len(ended))))        # (so many of them may end that this is what leaves `beams`)
         dev = engine.device
         self.ended = torch.tensor(list(ended), dtype=torch.int32, device=dev) if len(ended) else None
         specs = [core.SeqSpec(i, list(map(int, p)), 1) for i, p in enumerate(prompts)]
@@ -290,7 +290,7 @@ def beam_search(engine, prompts: Sequence[Sequence[int]], beams: int, max_new_to
     if not engine.status.fully_loaded():
         raise RuntimeError("model parameters are not loaded")
     eos = sorted({int(t) for t in eos})
-    most = min(ops.BEAMS_MAX // (1 + max(1, len(eos))), engine.max_batch)
+    most = min(ops.BEAMS_MAX // (1 + len(eos)), engine.max_batch)
     if not 1 <= beams <= most:
         raise ValueError(f"{beams} beams: at most {most} with {len(eos)} tokens that end a continuation, {ops.BEAMS_MAX} candidates and max_batch={engine.max_batch}")
     if max_new_tokens < 1 or any(len(p) < 1 for p in prompts):

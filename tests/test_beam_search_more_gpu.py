@@ -1,0 +1,40 @@
+"""Engine.beam_search: as many beams as selection takes, logits that are no numbers, many shapes, greedy decoding beside one beam, caches full of what others left."""
+import pytest
+import torch
+
+from blitz_scale_b200.runtime import core
+from blitz_scale_b200.runtime.engine import Engine
+
+pytestmark = pytest.mark.gpu
+
+
+def _prompts(lens, vocab, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randint(0, vocab, (n,), generator=g).tolist() for n in lens]
+
+
+def _fed(engine, tokens, last):
+    """Log probabilities [last, vocab] behind the last `last` prefixes of `tokens`, in one pass over a request of their own."""
+    b = engine.new_batch(77, [core.SeqSpec(0, tokens, 1)])
+    try:
+        return torch.log_softmax(engine.step(b, [len(tokens)], [list(range(len(tokens) - last, len(tokens)))]).double(), 1).cpu()
+    finally:
+        b.clear()
+
+
+# Logits of this model are of order one, in bf16: off by 2^-8 each way, and the hidden states behind them by as much again per layer's worth of roundings.
+SLACK = 0.06
+
+
+@pytest.mark.parametrize("beams,eos", [(33, []), (64, []), (32, [5]), (21, [5, 9])])
+def test_as_many_beams_as_there_are(beams, eos):
+    """beams x (1 + tokens that end a continuation) up to 64."""
+    e = Engine("tiny_gpu", num_pages=400, page_size=16, max_batch=64, max_batch_tokens=512)
+    prompt = _prompts([20], 4096, seed=8)[0]
+    found = e.beam_search([prompt], beams, 5, eos=eos)[0]
+    assert len(found) == beams and len({tuple(h.tokens) for h in found}) == beams
+    for h in found[:3] + found[-3:]:
+        p = _fed(e, prompt + h.tokens[:-1], len(h.tokens))
+        assert abs(sum(p[i, t].item() for i, t in enumerate(h.tokens)) - h.log_prob) <= SLACK * len(h.tokens)
+    with pytest.raises(ValueError, match=f"at most {64 // (1 + len(eos))} "):
+        e.beam_search([prompt], 64 // (1 + len(eos)) + 1, 5, eos=eos)
