@@ -279,6 +279,8 @@ class _Search:
         p = [x.tolist() for x in p]
         for q, h in enumerate(self.history):
             lists = [[(p[i][j], p[i + 1][j], p[i + 2][j]) for j in range(q * m, q * m + m) if p[i + 1][j] >= 0] for i, m in ((0, self.n), (3, self.beams))]
+            if not h.done and not lists[0]:
+                raise RuntimeError("beam search: the logits of a request are no numbers (NaN or infinity)")
             h.take(Candidates(*lists))
 
 

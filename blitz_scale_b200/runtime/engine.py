@@ -324,7 +324,7 @@ class Engine:
         them, ranked by log probability / length ^ `length_penalty`.  A continuation ends with one of the tokens `eos` or after `max_new_tokens`; beams x (1 + tokens
         that end one) are 64 at most, and beams max_batch.  Pages (and
         state slots) for beams x requests are reserved for the time of the call; requests beyond max_batch / beams run one group after the other.
-        RuntimeError, with nothing kept, where the cache has too few pages."""
+        RuntimeError, with nothing kept, where the cache has too few pages, or all rows of a running request have logits that are no numbers."""
         from .beams import beam_search
         return beam_search(self, prompts, beams, max_new_tokens, eos=eos, length_penalty=length_penalty, best=best)
 

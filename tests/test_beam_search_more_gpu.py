@@ -38,3 +38,22 @@ def test_as_many_beams_as_there_are(beams, eos):
         assert abs(sum(p[i, t].item() for i, t in enumerate(h.tokens)) - h.log_prob) <= SLACK * len(h.tokens)
     with pytest.raises(ValueError, match=f"at most {64 // (1 + len(eos))} "):
         e.beam_search([prompt], 64 // (1 + len(eos)) + 1, 5, eos=eos)
+
+
+@pytest.mark.parametrize("after", [0, 3])
+def test_logits_that_are_no_numbers(monkeypatch, after):
+    e = Engine("tiny_gpu", num_pages=200, page_size=16, max_batch=8, max_batch_tokens=512, use_graphs=False)
+    free, forward, calls = e.pool.free_pages, e.runner.forward, []
+
+    def spoilt(meta, **more):
+        out = forward(meta, **more)
+        if len(calls) == after:
+            e.runner.logits[4 if after else 1:].fill_(float("nan"))
+        calls.append(meta)
+        return out
+    monkeypatch.setattr(e.runner, "forward", spoilt)
+    with pytest.raises(RuntimeError, match="no numbers"):
+        e.beam_search(_prompts([20, 7], 4096, seed=1), 4, 6)
+    assert len(calls) == after + 1 and e.pool.free_pages == free
+    monkeypatch.undo()
+    assert [len(x) for x in e.beam_search(_prompts([20, 7], 4096, seed=1), 4, 6)] == [4, 4]
