@@ -92,6 +92,23 @@ class _Buffers:
         self.tables = ops.StepTables(new(rows * width), new(rows + 1), new(rows), new(rows), new(rows), None, new(rows // beams))
 
 
+GRAPHS_MOST = 16      # shapes of steps that an engine keeps a graph and buffers for
+
+
+def _buffers(engine, key: tuple, rows: int, beams: int, width: int) -> _Buffers:
+    """The buffers of steps of one shape.  Those that were not used for the longest time make room for a new one, their graph with them.  (No step is under way.)"""
+    kept = engine._beam_buffers        # (the last used one is the last)
+    buf = kept.pop(key, None)
+    if buf is None:
+        while len(kept) >= GRAPHS_MOST:
+            old = next(iter(kept))
+            engine._graphs.pop(old, None)
+            del kept[old]
+        buf = _Buffers(rows, beams, width, engine.device)
+    kept[key] = buf
+    return buf
+
+
 def _graph_rows(groups: int, beams: int, most: int) -> int:
     """Groups of a step: the next power of two, where the engine's batch has room for it (steps of similar batches share a graph)."""
     n = 1
@@ -212,9 +229,7 @@ class _Search:
         longest = max(self.lens) + self.budget
         splits = 1 if self._at_once() else e.choose_splits(Q * k, longest, sum(self.lens) * k + Q * k * self.budget)
         key = ("beams", rows, k, width, splits)
-        if key not in e._beam_buffers:
-            e._beam_buffers[key] = _Buffers(rows, k, width, dev)
-        buf = e._beam_buffers[key]
+        buf = _buffers(e, key, rows, k, width)
         pools, states = _tensors(e)
         # the request's rows before its first step: one, with the prompt
         pad = lambda x, m: x + [-1] * (m - len(x))  # noqa: E731

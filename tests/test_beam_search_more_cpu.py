@@ -31,3 +31,18 @@ def test_requests_without_candidates():
     assert s.history[0].tokens(0) == [4, 3]
     with pytest.raises(RuntimeError, match="no numbers"):
         s._note(_step(([NONE] * 4, [NONE] * 2), ([NONE] * 4, [NONE] * 2)))
+
+
+def test_shapes_that_are_kept(monkeypatch):
+    """Graphs and buffers of the last used shapes of steps, dropped together; other graphs of the engine stay."""
+    monkeypatch.setattr(rb, "_Buffers", lambda *shape: shape)
+    monkeypatch.setattr(rb, "GRAPHS_MOST", 3)
+
+    class engine:
+        device, _beam_buffers, _graphs = "cpu", {}, {(8, 1): "decode"}
+    for i in (1, 2, 3, 1, 4, 1, 5, 5, 2):
+        assert rb._buffers(engine, ("beams", i), i, 1, 2) == (i, 1, 2, "cpu")
+        engine._graphs[("beams", i)] = i
+        assert len(engine._beam_buffers) <= 3
+    assert list(engine._beam_buffers) == [("beams", i) for i in (1, 5, 2)]
+    assert engine._graphs == {(8, 1): "decode", ("beams", 1): 1, ("beams", 5): 5, ("beams", 2): 2}

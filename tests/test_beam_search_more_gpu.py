@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from blitz_scale_b200.runtime import beams as rb
 from blitz_scale_b200.runtime import core
 from blitz_scale_b200.runtime.engine import Engine
 
@@ -57,3 +58,15 @@ def test_logits_that_are_no_numbers(monkeypatch, after):
     assert len(calls) == after + 1 and e.pool.free_pages == free
     monkeypatch.undo()
     assert [len(x) for x in e.beam_search(_prompts([20, 7], 4096, seed=1), 4, 6)] == [4, 4]
+
+
+def test_searches_of_many_shapes(monkeypatch):
+    """What is found does not depend on the graphs that came and went before."""
+    monkeypatch.setattr(rb, "GRAPHS_MOST", 2)
+    e = Engine("tiny_gpu", num_pages=300, page_size=16, max_batch=16, max_batch_tokens=512)
+    shapes = [(1, 4, 20), (2, 3, 20), (3, 5, 20), (1, 4, 200), (1, 4, 20), (2, 3, 20), (1, 16, 30)]
+    found = []
+    for n, beams, length in shapes:
+        found.append(e.beam_search(_prompts([length] * n, 4096, seed=length), beams, 8))
+        assert len(e._beam_buffers) <= 2 and sum(key[0] == "beams" for key in e._graphs) <= 2
+    assert found[0] == found[4] and found[1] == found[5]
