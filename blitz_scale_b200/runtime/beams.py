@@ -9,6 +9,7 @@ The reference serves greedily only (src/kernel/sampler.cu:7-141); this is an add
 """
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 from typing import Dict, List, NamedTuple, Optional, Sequence, Tuple
 
@@ -310,6 +311,12 @@ def beam_search(engine, prompts: Sequence[Sequence[int]], beams: int, max_new_to
     most = min(ops.BEAMS_MAX // (1 + len(eos)), engine.max_batch)
     if not 1 <= beams <= most:
         raise ValueError(f"{beams} beams: at most {most} with {len(eos)} tokens that end a continuation, {ops.BEAMS_MAX} candidates and max_batch={engine.max_batch}")
+    try:
+        longest = float(max_new_tokens) ** length_penalty if max_new_tokens > 0 else 1.0
+    except OverflowError:
+        longest = math.inf
+    if not 0.0 < longest < math.inf or (best is not None and best < 1):
+        raise ValueError(f"a length penalty of {length_penalty} over {max_new_tokens} tokens, the best {best}")
     if max_new_tokens < 1 or any(len(p) < 1 for p in prompts):
         raise ValueError("a prompt of one token and a budget of one at least")
     if not all(0 <= t < engine.cfg.vocab for p in (eos, *prompts) for t in p):

@@ -320,7 +320,7 @@ class Engine:
 
     def beam_search(self, prompts: Sequence[Sequence[int]], beams: int, max_new_tokens: int, *, eos: Sequence[int] = (), length_penalty: float = 1.0,
                     best: Optional[int] = None) -> list:
-        """The most probable continuations of every prompt that `beams` beams find: for each a list of runtime.beams.Hypothesis, best first, `best` (beams) of
+        """The most probable continuations of every prompt that `beams` beams find: for each a list of runtime.beams.Hypothesis, best first, `best` (beams; one at least) of
         them, ranked by log probability / length ^ `length_penalty`.  A continuation ends with one of the tokens `eos` or after `max_new_tokens`; beams x (1 + tokens
         that end one) are 64 at most, and beams max_batch.  Pages (and
         state slots) for beams x requests are reserved for the time of the call; requests beyond max_batch / beams run one group after the other.

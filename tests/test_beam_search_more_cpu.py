@@ -46,3 +46,22 @@ def test_shapes_that_are_kept(monkeypatch):
         assert len(engine._beam_buffers) <= 3
     assert list(engine._beam_buffers) == [("beams", i) for i in (1, 5, 2)]
     assert engine._graphs == {(8, 1): "decode", ("beams", 1): 1, ("beams", 5): 5, ("beams", 2): 2}
+
+
+class _Engine:
+    """As much of an engine as the checks of arguments look at."""
+    tp, max_batch = 1, 8
+
+    class status:
+        fully_loaded = staticmethod(lambda: True)
+
+    class cfg:
+        vocab = 100
+
+
+@pytest.mark.parametrize("more", [dict(best=0), dict(best=-1), dict(length_penalty=math.nan), dict(length_penalty=math.inf), dict(length_penalty=-math.inf), dict(length_penalty=1e4),
+                                  dict(length_penalty=-1e4)])
+def test_refusals(more):
+    with pytest.raises(ValueError, match="length penalty"):
+        rb.beam_search(_Engine(), [[1, 2]], 4, 20, **more)
+    assert rb.beam_search(_Engine(), [], 4, 20, length_penalty=-2.0, best=1) == []
