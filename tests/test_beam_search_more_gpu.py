@@ -70,3 +70,31 @@ def test_searches_of_many_shapes(monkeypatch):
         found.append(e.beam_search(_prompts([length] * n, 4096, seed=length), beams, 8))
         assert len(e._beam_buffers) <= 2 and sum(key[0] == "beams" for key in e._graphs) <= 2
     assert found[0] == found[4] and found[1] == found[5]
+
+
+def test_one_beam_takes_what_greedy_decoding_takes():
+    """Token by token, up to one where the two largest logits are nearer than what two ways of computing them differ by."""
+    e = Engine("tiny_gpu", num_pages=200, page_size=16, max_batch=8, max_batch_tokens=512)
+    for prompt in _prompts([30, 1, 64, 15, 100], 4096, seed=2):
+        batch = e.new_batch(1, [core.SeqSpec(0, prompt, 12)])
+        greedy = [t for step in [e.prefill(batch)] + [e.decode(batch) for _ in range(11)] for t in step]
+        batch.clear()
+        found = e.beam_search([prompt], 1, 12)[0]
+        assert len(found) == 1 and len(found[0].tokens) == 12
+        same = next((i for i, (a, b) in enumerate(zip(greedy, found[0].tokens)) if a != b), 12)
+        if same < 12:
+            p = _fed(e, prompt + greedy[:same], 1)[0]
+            assert abs(p[greedy[same]] - p[found[0].tokens[same]]) <= 2 * SLACK
+
+
+@pytest.mark.parametrize("page,lens,beams", [(16, [1, 16, 33, 47], 4), (64, [5, 64, 130], 5)])
+def test_caches_full_of_what_others_left(page, lens, beams):
+    """Pages that no request has written hold large numbers: a token that a copy leaves out, or a page taken for another, would take all the weight.  What is
+    found is what an empty cache gives, to the last bit."""
+    e = Engine("tiny_gpu", num_pages=200, page_size=page, max_batch=32, max_batch_tokens=512)
+    prompts = _prompts(lens, 4096, seed=9)
+    found = []
+    for left in (0.0, 100.0, -3.0):
+        e.kv.fill_(left)
+        found.append(e.beam_search(prompts, beams, 2 * page + 3 if page == 16 else 70))
+    assert found[0] == found[1] == found[2]
