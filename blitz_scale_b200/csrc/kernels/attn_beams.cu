@@ -16,11 +16,11 @@
 // steps of a warp, 128 KB an SM, are enough to keep memory busy; with three more requests wait in its queues, and SMs are served less evenly.
 //
 // Rounded to 16 bits: the weights, as operands of the second product, and the output.  Scores, maxima, sums and pieces are fp32.  Errors against 64 bits: bf16 0.0023 where the output's
-// rounding alone is 0.0017, fp16 0.00028 (0.00021), as decode attention has them.  Weights as two 16-bit numbers take that away and cost 8 us of 67 (32 x 8 beams; 5 where only tiles
+// rounding alone is 0.0017, fp16 0.00027 (0.00021), as decode attention has them.  Weights as two 16-bit numbers take that away and cost 8 us of 67 (32 x 8 beams; 5 where only tiles
 // of up to 16 rows have them).
 //
-// Measured, 32 query over 8 KV heads of 128, bf16, us in a graph (bytes of each token once, at the copy rate): 4 beams of 100144 tokens 76.0 (63.1), of 1014 tokens 9.9 (0.75);
-// 32 x 8 beams of 1301 on average, 101 of them their own, 67.6 (44.5).  What bounds it: memory at 6.0 to 6.7 TB/s while all warps run, but
+// Measured, 32 query over 8 KV heads of 128, bf16, us in a graph (bytes of each token once, at the copy rate): 4 beams of 100144 tokens 74.5 to 75.5 (63.1), of 1014 tokens 9.7 (0.75);
+// 32 x 8 beams of 1301 on average, 101 of them their own, 65.7 to 67.2 (44.5).  What bounds it: memory at 6.0 to 6.7 TB/s while all warps run, but
 // equal ranges end between 41 and 57 us (32 x 8) or 57 and 66 (the long one); then 3 us for tables and first loads, 6.6 to 7.7 for the merge.
 // Tried: three steps under way 72.9 (78.8 the long one), one 79.6 (84.3); queries and page ids of the next piece asked for a piece ahead 70.4; the heads of a range on one SM 72.8.
 #include <cfloat>
@@ -77,7 +77,7 @@ struct BaRanges {
   __device__ __forceinline__ int of(int x) const { return x < rem * (q + 1) ? x / (q + 1) : rem + (x - rem * (q + 1)) / q; }
 };
 
-// Lengths, common pages and the line of segments, by all threads of a block; arrays in shared memory, or (write) in scratch too.
+// Lengths, common pages and the line of segments, by all threads of a block; arrays in shared memory.
 __device__ __forceinline__ void ba_line(const BeamAttnParams& p, int* line, int* len, int* common, int* sums) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int shared0 = tid < p.blocks * p.groups ? p.shared[tid % p.groups] : 0;      // (asked for together with the lengths)

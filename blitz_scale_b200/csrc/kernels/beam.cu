@@ -19,11 +19,12 @@ constexpr int kBeamMost = 64;  // beams of a request, and candidates of it
 // The scan streams the logits once: a warp takes a stretch of a row, and leaves the sum of exponentials beside its largest logit, and the largest
 // logit of every group of 512.  Nothing else is done beside the stream: a selection in it (bounds, lists and barriers for every 32 KB) took two to
 // three times the stream's time.  The second kernel, a block per request, knows the sums, hence the values of the groups' largest; the n best elements are in
-// the n best groups, which it reads again (1 KB each, out of L2 as a rule).  Values are pairs of fp32, 48 bits: candidates of
-// different beams may be nearer to one another than fp32 tells apart, and an exchange of two would be a wrong token.
+// the n best groups, which it reads again (1 KB each, out of L2 as a rule).  Values are pairs of fp32, 48 bits, so that a beam's candidates, and those of beams with equal
+// logits, keep the order of their logits, which fp32 values would not tell apart.  The sums behind them are fp32: a score is off by 3e-8 as a rule and 5e-6 at
+// most, and candidates of different rows that are nearer than that may come in either order.
 //
-// Measured, us in a graph (bytes once at the copy rate): 256 rows of 128256 logits in bf16, 8 beams, n = 24, 23.0 (10.0), of which the scan 15.4; 65 rows of 50257 in fp32
-// 11.2 (2.0); one request of four beams 8.4 (0.2).  The scan is bound by its instructions, a fifth of them the exponentials, and the time until all warps have
+// Measured, us in a graph (bytes once at the copy rate): 256 rows of 128256 logits in bf16, 8 beams, n = 24, 22.2 (10.0), of which the scan 15; 65 rows of 50257 in fp32
+// 12.3 (2.0); one request of four beams 8.6 (0.2).  The scan is bound by its instructions, a fifth of them the exponentials, and the time until all warps have
 // their first groups; the second kernel by a chain of some ten short rounds through shared memory.
 constexpr int kSelGroup = 512;
 constexpr int kSelWarps = 48;       // warps of an SM that the scan counts on

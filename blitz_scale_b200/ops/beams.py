@@ -97,7 +97,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int = 1, *, n
     """The ``n`` (2 beams) best continuations of every request.  ``logits`` [requests * beams, vocab] in fp16, bf16 or fp32, rows of any pitch;
     ``scores`` [requests * beams] in fp32, finite, or -inf for a row that has ended.  A continuation's value is the row's score plus the token's log
     probability, a softmax over the whole row; one that is no number (rows with a NaN or +inf), or below what fp32 holds, counts as -inf.  Ties go to the lowest beam, then the
-    lowest token.  ``ended``: int32 tokens that end a sequence; ``keep`` (beams): how many continuations go on.  At most 64 beams and candidates."""
+    lowest token: tokens of equal logits in a row, and beams of equal logits and scores, wherever in memory their rows begin.  (A row's log probabilities are off by 5e-6
+    at most, all alike: candidates of rows with other logits that are nearer than that may come in either order.)  ``ended``: int32 tokens that end a sequence; ``keep`` (beams): how many continuations go on.  At most 64 beams and candidates."""
     dt = _DT3.get(logits.dtype)
     if dt is None:
         raise TypeError(f"kernel takes fp16/bf16/fp32 tensors, got {logits.dtype}")
@@ -283,7 +284,8 @@ def attn_decode_beams(q: torch.Tensor, kv_layer: torch.Tensor, indices: torch.Te
                       out: Optional[torch.Tensor] = None, sm_scale: Optional[float] = None, softcap: float = 0.0, sink: Optional[torch.Tensor] = None,
                       static_table: bool = False) -> torch.Tensor:
     """Decode attention (see `attn_decode`) of rows in groups of ``beams`` whose first pages are the same: the first ``shared`` [rows / beams] pages
-    of a group, full in every row of it that has pages, are read once for all its rows.  q [rows, >= q_heads * head_dim]; a 16-bit cache of heads of 64 or 128
+    of a group, full in every row of it that has pages, are read once for all its rows.  Scores of -inf have no weight; a row of nothing else is NaN, as its softmax (zeros with a ``sink``).  Sums are fp32: finite as long as tokens
+    times the largest value is.  q [rows, >= q_heads * head_dim]; a 16-bit cache of heads of 64 or 128
     [pages, 2, page, kv_heads, dim], pages of 16 tokens times a power of two; rows without pages are zeros."""
     dt = q.dtype
     if dt not in _DT:
