@@ -10,7 +10,14 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA device (run on the B200 box)")
 
 
+# These expect -1.0 for each of 40001 equal tokens behind a score of -1, where their softmax is -1 - log 40001: the plain form they compare with takes the log of a row's sum off
+# together with its largest number, 3.4e38, in which it disappears (tests/test_beams_values_gpu.py has the value).  They fail, and come last, so that a run that stops at the first
+# failure has run all others.
+WRONG_VALUE = ("test_select_values[dtype0-one row lowest]", "test_select_values[dtype1-one row lowest]")
+
+
 def pytest_collection_modifyitems(config, items):
+    items.sort(key=lambda it: it.name in WRONG_VALUE)
     try:
         import torch
         has = torch.cuda.is_available()
